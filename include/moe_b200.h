@@ -40,7 +40,8 @@ typedef enum moe_status {
   MOE_ERR_WORKSPACE = 4,
   MOE_ERR_ALIGNMENT = 5,
   MOE_ERR_TIMEOUT = 6,
-  MOE_ERR_CODEBOOK = 7
+  MOE_ERR_CODEBOOK = 7,
+  MOE_ERR_PAGE = 8
 } moe_status_t;
 
 #define MOE_MAX_EXPERTS 16
@@ -63,6 +64,11 @@ typedef struct moe_nf4_expert {
   moe_nf4_matrix_t w2;
 } moe_nf4_expert_t;
 
+/* Element types of the paged-serving operators. */
+#define MOE_DTYPE_F16 0
+#define MOE_DTYPE_BF16 1
+#define MOE_DTYPE_F32 2
+
 /* Text for a status code (static storage). */
 const char* moe_status_string(int status);
 
@@ -82,13 +88,16 @@ uint64_t moe_launch_count(void);
  *   2  the experts of one launch carry different NF4 codebooks (the kernels
  *      decode every expert with expert 0's w1 codebook for gate/up and its
  *      w2 codebook for down); the outputs are invalid;
- *   4  a kernel found its shared-memory layout not as planned and skipped.
+ *   4  a kernel found its shared-memory layout not as planned and skipped;
+ *   8  a position, sequence id, page, length or offset read from device memory
+ *      was out of range: nothing outside the buffers was touched, the rows
+ *      concerned are not valid.
  * Synchronous (device-to-host copies).  *value is 0 when nothing was set. */
 int moe_take_device_error(int* value);
 
 /* Synchronises `stream`, then turns the device error words into a status:
- * MOE_ERR_TIMEOUT (bit 1), MOE_ERR_CODEBOOK (bit 2), MOE_ERR_CUDA (bit 4 or a
- * CUDA error), else MOE_OK.  The words are cleared.  Call it at the points
+ * MOE_ERR_TIMEOUT (bit 1), MOE_ERR_CODEBOOK (bit 2), MOE_ERR_PAGE (bit 8),
+ * MOE_ERR_CUDA (bit 4 or a CUDA error), else MOE_OK.  The words are cleared.  Call it at the points
  * where the caller synchronises anyway (end of a step, before reading
  * results back) to learn whether the launches since the last check were valid.
  * No counterpart in the reference (its library calls raise synchronously). */
@@ -414,6 +423,60 @@ int moe_ep_return_partials_p2p(const float* y_part, int S, const int32_t* recv_c
                                int G, int rank, int cap, int hidden,
                                const uint64_t* peer_back, const uint64_t* peer_flags,
                                int32_t* seq, int32_t* done, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Ragged, paged serving: one decode engine's chain of operators.  No
+ * counterpart in the reference, whose cache is a growing DynamicCache of one
+ * sequence (engine/engine.py:326-378) and whose only decoding is greedy.
+ *
+ * A paged cache is two arrays [num_pages, kv_heads, page_size, head_dim]
+ * (keys, values), 16-byte aligned; *_page_stride is the number of elements
+ * from one page to the next (at least a page, a multiple of 8), a page itself
+ * is contiguous.  block_table int32 [seqs, max_pages] (rows table_stride
+ * elements apart) lists each sequence's pages: its position p is row
+ * p % page_size of page table[b][p / page_size].  Entries past a sequence's
+ * last page are never read.  Two sequences may list the same page.
+ *
+ * dtype: MOE_DTYPE_F16 or MOE_DTYPE_BF16; head_dim: 64 or 128; heads a
+ * multiple of kv_heads (query head h reads KV head h / (heads / kv_heads)).
+ * What is read from device memory (positions, sequence ids, pages, lengths,
+ * offsets) is checked there; a value out of range touches nothing outside the
+ * buffers and sets the device error word (MOE_ERR_PAGE from
+ * moe_stream_check).
+ *
+ * moe_rope_append: rows of a fused q/k/v projection, [tokens, (heads + 2
+ *   kv_heads) * head_dim], qkv_stride elements apart (a multiple of 8).
+ *   Rotates q and k by the token's position p in fp32 (the two halves of a
+ *   head are a pair: y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin; cos / sin
+ *   fp32 [max_pos, head_dim / 2]), rounds once, writes k and v to the token's
+ *   slot and q to q_out [tokens, heads, head_dim].  seq_ids int32 [tokens], or
+ *   NULL: token t belongs to sequence t.  A token with a negative position is
+ *   padding: a zero q row, nothing appended.
+ */
+int moe_rope_append(const uint16_t* qkv, int64_t qkv_stride, const float* cos, const float* sin,
+                    int64_t max_pos, const int32_t* positions, const int32_t* seq_ids,
+                    int64_t tokens, uint16_t* k_pages, uint16_t* v_pages, int64_t k_page_stride,
+                    int64_t v_page_stride, int64_t num_pages, int page_size,
+                    const int32_t* block_table, int64_t table_stride, int seqs, int max_pages,
+                    int heads, int kv_heads, int head_dim, int dtype, uint16_t* q_out,
+                    void* stream);
+
+/* moe_paged_attention: o[b,h] = softmax(scale q[b,h] . K_b^T) V_b over the
+ *   first lengths[b] positions of sequence b (0: a row of zeros; the token
+ *   appended last counts).  q [seqs, heads, head_dim], rows q_stride elements
+ *   apart; out [seqs, heads, head_dim] packed.  fp32 scores, softmax and sums;
+ *   the probabilities are rounded to the element type for the product with V.
+ *   What lies in a page past a sequence's end (infinities, NaN) has no effect.
+ *   page_size % 16 == 0, seqs <= 8191, scale > 0.  The workspace needs no
+ *   initialisation.  Results do not vary from call to call. */
+size_t moe_paged_attention_workspace_size(int seqs, int max_pages, int page_size, int heads,
+                                          int kv_heads, int head_dim);
+int moe_paged_attention(const uint16_t* q, int64_t q_stride, uint16_t* k_pages,
+                        uint16_t* v_pages, int64_t k_page_stride, int64_t v_page_stride,
+                        int64_t num_pages, int page_size, const int32_t* block_table,
+                        int64_t table_stride, int seqs, int max_pages, const int32_t* lengths,
+                        int heads, int kv_heads, int head_dim, int dtype, float scale,
+                        uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -16,6 +16,7 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmoe_b200.so"
 MOE_MAX_EXPERTS = 16
 MOE_ERR_TIMEOUT = 6
 MOE_ERR_CODEBOOK = 7
+MOE_ERR_PAGE = 8
 MOE_NOALLOC_SCRATCH_BYTES = 4 << 20
 
 
@@ -91,6 +92,15 @@ SIGNATURES: dict[str, tuple] = {
     "moe_experts_forward_partials": (c_int, [ctypes.POINTER(NF4Expert), c_int, c_void_p, c_void_p,
                                              c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                              c_size_t, c_void_p]),
+    "moe_rope_append": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                                c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int,
+                                c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,
+                                c_void_p, c_void_p]),
+    "moe_paged_attention_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "moe_paged_attention": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                                    c_int64, c_int, c_void_p, c_int64, c_int, c_int, c_void_p,
+                                    c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p,
+                                    c_size_t, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

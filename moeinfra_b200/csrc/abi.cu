@@ -102,6 +102,7 @@ extern "C" const char* moe_status_string(int status) {
     case MOE_ERR_ALIGNMENT: return "pointer not 16-byte aligned";
     case MOE_ERR_TIMEOUT: return "device wait timed out";
     case MOE_ERR_CODEBOOK: return "experts of one launch carry different NF4 codebooks";
+    case MOE_ERR_PAGE: return "position, sequence, page or offset out of range on the device";
     default: return "unknown status";
   }
 }
@@ -140,6 +141,7 @@ extern "C" int moe_stream_check(void* stream) {
   if (st != MOE_OK) return st;
   if (v & moe::kErrWaitTimeout) return MOE_ERR_TIMEOUT;
   if (v & moe::kErrCodebook) return MOE_ERR_CODEBOOK;
+  if (v & moe::kErrPage) return MOE_ERR_PAGE;
   if (v & moe::kErrSmemLayout) return MOE_ERR_CUDA;
   return MOE_OK;
 }

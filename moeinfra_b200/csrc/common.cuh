@@ -101,6 +101,7 @@ __device__ __forceinline__ bool wait_peer_flag(const int32_t* flags, int s, cons
 constexpr int kErrWaitTimeout = 1;    // a bounded wait ran out
 constexpr int kErrCodebook = 2;       // experts of one launch carry different codebooks
 constexpr int kErrSmemLayout = 4;     // shared-memory layout not as planned (launch skipped)
+constexpr int kErrPage = 8;           // a position, sequence, page or offset out of range (skipped)
 
 // Each translation unit whose kernels report errors owns one device word
 // (device code is compiled per file, without relocatable linking, so a word

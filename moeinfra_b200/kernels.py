@@ -583,3 +583,167 @@ def ep_return_partials_p2p(y_part: torch.Tensor, recv_counts: torch.Tensor, num_
         _p(y_part), y_part.shape[1], _p(recv_counts), num_experts, world, rank, cap,
         y_part.shape[2], ctypes.c_void_p(peer_back), ctypes.c_void_p(peer_flags),
         ctypes.c_void_p(seq), ctypes.c_void_p(done), _stream(dev)), "moe_ep_return_partials_p2p")
+
+
+# ---------------------------------------------------------------------------
+# Ragged, paged serving: rotation + cache append, attention, sampling
+# ---------------------------------------------------------------------------
+
+_DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_serve_ws: dict = {}
+
+
+def _serve_scratch(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    """Scratch of the serving operators: one buffer per (device, stream, power of two), kept.
+
+    Calls on one stream are ordered and every kernel waits for its predecessor before it
+    touches scratch.  A call under stream capture gets scratch of its own from the graph's
+    pool: graphs captured on one stream may be replayed side by side.
+    """
+    if torch.cuda.is_current_stream_capturing():
+        return _workspace(nbytes, dev)
+    key = (dev.index, stream, max(nbytes - 1, 0).bit_length())
+    ws = _serve_ws.get(key)
+    if ws is None:
+        ws = _serve_ws[key] = _workspace(1 << key[2], dev)
+    return ws
+
+
+def _serve_check(what: str, dev: torch.device, *named) -> None:
+    """Each of ``named`` = (name, tensor, dtype, shape, contiguous dims): the last so many
+    dimensions packed; None in a shape is any size."""
+    for name, t, dtype, shape, packed in named:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: {name} must be a torch.Tensor")
+        if not t.is_cuda:
+            raise RuntimeError(
+                f"{what}: {name} is on {t.device}; the B200 kernels run on CUDA tensors only "
+                "(there is no CPU path)")
+        if t.device != dev:
+            raise ValueError(f"{what}: {name} is on {t.device}, expected {dev}")
+        if t.dtype is not dtype:
+            raise ValueError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+        size = t.shape
+        if len(size) != len(shape) or any(w is not None and w != n for w, n in zip(shape, size)):
+            want = ", ".join("*" if w is None else str(w) for w in shape)
+            raise ValueError(f"{what}: {name} must be [{want}], got {tuple(size)}")
+        if t.is_contiguous():
+            continue
+        run = 1
+        stride = t.stride()
+        for i in range(len(size) - 1, len(size) - 1 - packed, -1):
+            if size[i] != 1 and stride[i] != run:
+                raise ValueError(f"{what}: {name} must be contiguous in its last {packed} "
+                                 "dimension(s)")
+            run *= size[i]
+
+
+def _page_geometry(what: str, k_pages, v_pages, block_table):
+    """(dtype, num_pages, kv_heads, page_size, head_dim) of a paged cache."""
+    if not isinstance(k_pages, torch.Tensor) or k_pages.ndim != 4:
+        raise ValueError(f"{what}: k_pages must be [pages, kv_heads, page_size, head_dim]")
+    if k_pages.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{what}: k_pages must be float16 or bfloat16, got {k_pages.dtype}")
+    n, kv, page, hd = shape = k_pages.shape
+    dev, dt = k_pages.device, k_pages.dtype
+    _serve_check(what, dev, ("k_pages", k_pages, dt, shape, 3), ("v_pages", v_pages, dt, shape, 3),
+                 ("block_table", block_table, torch.int32, (None, None), 1))
+    if hd not in (64, 128):
+        raise ValueError(f"{what}: head_dim must be 64 or 128, got {hd}")
+    return dt, n, kv, page, hd
+
+
+def _outer_stride(t: torch.Tensor) -> int:
+    """Elements from one index of the first dimension to the next (packed when there is one)."""
+    return t.stride(0) if t.shape[0] > 1 else t.numel()
+
+
+@_on_device
+def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                block_table: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                num_heads: int, seq_ids: torch.Tensor | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotate q and k of fused projection rows and append k and v to the paged cache.
+
+    ``qkv`` [tokens, (num_heads + 2 * kv_heads) * head_dim] (rows may be strided), fp16 or bf16;
+    ``cos`` / ``sin`` fp32 [max_positions, head_dim / 2]; ``positions`` int32 [tokens] in the
+    token's own sequence (negative: padding, a zero q row and nothing appended); ``block_table``
+    int32 [sequences, max_pages]; ``k_pages`` / ``v_pages`` [pages, kv_heads, page_size, head_dim],
+    written in place; ``seq_ids`` int32 [tokens] (None: token t is sequence t, the decode step).
+    Returns q [tokens, num_heads, head_dim].  A position, sequence or page out of range appends
+    nothing and shows in :func:`check_device`.
+    """
+    what = "rope_append"
+    dt, n_pages, kv, page, hd = _page_geometry(what, k_pages, v_pages, block_table)
+    dev = k_pages.device
+    _serve_check(what, dev, ("qkv", qkv, dt, (None, (num_heads + 2 * kv) * hd), 1),
+                 ("positions", positions, torch.int32, (None,), 1),
+                 ("cos", cos, torch.float32, (None, hd // 2), 2),
+                 ("sin", sin, torch.float32, tuple(cos.shape), 2))
+    T = qkv.shape[0]
+    if positions.shape[0] != T:
+        raise ValueError(f"{what}: positions must be [{T}], got {tuple(positions.shape)}")
+    seqs, max_pages = block_table.shape
+    if seq_ids is not None:
+        _serve_check(what, dev, ("seq_ids", seq_ids, torch.int32, (T,), 1))
+    elif seqs < T:
+        raise ValueError(f"{what}: block_table has {seqs} sequences for {T} tokens")
+    if out is None:
+        out = torch.empty((T, num_heads, hd), dtype=dt, device=dev)
+    else:
+        _serve_check(what, dev, ("out", out, dt, (T, num_heads, hd), 3))
+    check(_native.lib().moe_rope_append(
+        qkv.data_ptr(), _outer_stride(qkv) if T else qkv.shape[1], cos.data_ptr(), sin.data_ptr(),
+        cos.shape[0], positions.data_ptr(), None if seq_ids is None else seq_ids.data_ptr(), T,
+        k_pages.data_ptr(), v_pages.data_ptr(), _outer_stride(k_pages), _outer_stride(v_pages), n_pages,
+        page, block_table.data_ptr(), _outer_stride(block_table) if seqs else max_pages, seqs,
+        max_pages, num_heads, kv, hd, _DTYPE_CODES[dt], out.data_ptr(),
+        torch.cuda.current_stream(dev).cuda_stream), "moe_rope_append")
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_ws_bytes(device: int, seqs: int, max_pages: int, page: int, heads: int, kv: int,
+                    hd: int) -> int:
+    return _native.lib().moe_paged_attention_workspace_size(seqs, max_pages, page, heads, kv, hd)
+
+
+@_on_device
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    block_table: torch.Tensor, lengths: torch.Tensor,
+                    scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence over its cached keys and values.
+
+    ``q`` [sequences, heads, head_dim] (rows may be strided), ``lengths`` int32 [sequences]: the
+    positions each sequence sees, the token just appended included (0: a row of zeros); the rest
+    as in :func:`rope_append`; ``page_size`` a multiple of 16.  ``scale`` defaults to
+    ``head_dim ** -0.5``.  Returns [sequences, heads, head_dim].
+    """
+    what = "paged_attention"
+    dt, n_pages, kv, page, hd = _page_geometry(what, k_pages, v_pages, block_table)
+    dev = k_pages.device
+    seqs, max_pages = block_table.shape
+    _serve_check(what, dev, ("q", q, dt, (seqs, None, hd), 2),
+                 ("lengths", lengths, torch.int32, (seqs,), 1))
+    heads = q.shape[1]
+    if page % 16:
+        raise ValueError(f"{what}: page_size must be a multiple of 16, got {page}")
+    if heads == 0 or heads % kv:
+        raise ValueError(f"{what}: {heads} query heads do not divide over {kv} KV heads")
+    if out is None:
+        out = torch.empty((seqs, heads, hd), dtype=dt, device=dev)
+    else:
+        _serve_check(what, dev, ("out", out, dt, (seqs, heads, hd), 3))
+    if seqs == 0:
+        return out
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    nbytes = _paged_ws_bytes(dev.index, seqs, max_pages, page, heads, kv, hd)
+    ws = _serve_scratch(dev, stream, nbytes)
+    check(_native.lib().moe_paged_attention(
+        q.data_ptr(), _outer_stride(q), k_pages.data_ptr(),
+        v_pages.data_ptr(), _outer_stride(k_pages), _outer_stride(v_pages), n_pages, page,
+        block_table.data_ptr(), _outer_stride(block_table), seqs, max_pages,
+        lengths.data_ptr(), heads, kv, hd, _DTYPE_CODES[dt],
+        hd ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(), nbytes, stream),
+        "moe_paged_attention")
+    return out
