@@ -377,51 +377,76 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_attention(const PagedArgs
   __syncthreads();
 
   // ---- join the warps' pieces, unit by unit, in the order of the keys ----
+  // Lane k holds the k-th piece of the CTA; every warp sees the same list and
+  // takes its share of the (unit, head) sums, one row of HD values each.
+  const int held = lane < 2 * kWarps ? s_unit[lane] : -1;
+  const uint32_t used = __ballot_sync(0xffffffffu, held >= 0);
+  const int pieces = __popc(used);
+  int slot = 0;
+  for (uint32_t rest = used, k = 0; rest; rest &= rest - 1, ++k)
+    if (lane == (int)k) slot = __ffs(rest) - 1;
+  const int unit_k = __shfl_sync(0xffffffffu, held, slot);
+  const int ends_k = lane < pieces ? s_ends[slot] : 0;
+  const int unit_before = __shfl_up_sync(0xffffffffu, unit_k, 1);
+  uint32_t starts = __ballot_sync(0xffffffffu, lane < pieces && (lane == 0 || unit_k != unit_before));
+  const uint32_t firsts = __ballot_sync(0xffffffffu, ends_k & 1);
+  const uint32_t lasts = __ballot_sync(0xffffffffu, ends_k & 2);
+  const float* src = (slot & 1) ? reinterpret_cast<const float*>(smem + (slot >> 1) * S * stage_bytes<HD>())
+                                : a.warp_part + ((int64_t)blockIdx.x * kWarps + (slot >> 1)) * piece_floats<HD, NT>();
   int2 start = make_int2(-1, 0);
-  for (int i = 0; i < 2 * kWarps;) {
-    const int unit = s_unit[i];
-    if (unit < 0) {
-      ++i;
-      continue;
-    }
-    int j = i, ends = 0;
-    for (; j < 2 * kWarps && (s_unit[j] == unit || s_unit[j] < 0); ++j)
-      if (s_unit[j] == unit) ends |= s_ends[j];
-    float* dst = a.part + ((int64_t)blockIdx.x * 2 + (ends & 1)) * piece_floats<HD, NT>();
-    for (int e = tid; e < kHeads * HD; e += kThreads) {
-      const int col = e / HD, d = e % HD;
-      float mm = -INFINITY;
-      for (int s = i; s < j; ++s)
-        if (s_unit[s] == unit) mm = fmaxf(mm, s_ml[s][0][col]);
-      float ll = 0.f, oo = 0.f;
-      for (int s = i; s < j; ++s) {
-        if (s_unit[s] != unit) continue;
-        const float ms = s_ml[s][0][col];
-        const float f = ms == mm ? 1.f : exp2_approx(ms - mm);
-        const float* src = (s & 1)
-                               ? reinterpret_cast<const float*>(smem + (s >> 1) * S * stage_bytes<HD>())
-                               : a.warp_part + ((int64_t)blockIdx.x * kWarps + (s >> 1)) * piece_floats<HD, NT>();
-        ll += f * s_ml[s][1][col];
-        oo += f * src[col * kPitch + d];
+  int turn = 0;
+  while (starts) {
+    const int i = __ffs(starts) - 1;
+    starts &= starts - 1;
+    const int j = starts ? __ffs(starts) - 1 : pieces;
+    const uint32_t range = ((1u << j) - 1) & ~((1u << i) - 1);
+    const int unit = __shfl_sync(0xffffffffu, unit_k, i);
+    const bool first = firsts & range, last = lasts & range;
+    const int cols = min(kHeads, a.group - unit % a.parts * kHeads);
+    float* dst = a.part + ((int64_t)blockIdx.x * 2 + (first ? 1 : 0)) * piece_floats<HD, NT>();
+    for (int col = 0; col < cols; ++col, turn = turn + 1 == kWarps ? 0 : turn + 1) {
+      if (turn != warp) continue;
+      const bool mine = lane >= i && lane < j;
+      const float ms = mine ? s_ml[slot][0][col] : -INFINITY;
+      float mm = ms;
+#pragma unroll
+      for (int off = 16; off; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
+      const float f = ms == mm ? 1.f : exp2_approx(ms - mm);
+      float ll = mine ? f * s_ml[slot][1][col] : 0.f;
+#pragma unroll
+      for (int off = 16; off; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
+      constexpr int kVec = HD / 32;
+      float acc[kVec] = {};
+#pragma unroll 4
+      for (int k = i; k < j; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        const float* p = reinterpret_cast<const float*>(
+                             __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), k)) +
+                         col * kPitch + lane * kVec;
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) acc[v] += fk * p[v];
       }
-      if (ends == 3) {
+      if (first && last) {
+        const float inv = 1.f / ll;
         const int h = head_of(unit, col >> 3, col & 7);
-        if (h >= 0)
-          a.out[((int64_t)(unit / per_seq) * kv.kv_heads * a.group + h) * HD + d] = T::one(oo / ll);
+        uint32_t* o32 = reinterpret_cast<uint32_t*>(
+            a.out + ((int64_t)(unit / per_seq) * kv.kv_heads * a.group + h) * HD + lane * kVec);
+#pragma unroll
+        for (int v = 0; v < kVec; v += 2) o32[v / 2] = T::pack(acc[v] * inv, acc[v + 1] * inv);
       } else {
-        dst[col * kPitch + d] = oo;
-        if (d == 0) {
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) dst[col * kPitch + lane * kVec + v] = acc[v];
+        if (lane == 0) {
           dst[kHeads * kPitch + col] = mm;
           dst[kHeads * kPitch + kHeads + col] = ll;
         }
       }
     }
-    if (ends == 1) {  // further pieces lie in the CTAs after this one
+    if (first && !last) {  // further pieces lie in the CTAs after this one
       const int b = unit / per_seq, n = (prefix[b + 1] - prefix[b]) / per_seq;
       const int end = prefix[b] + (unit - b * per_seq + 1) * n;
       start = make_int2(unit, (end - 1) / share - (int)blockIdx.x + 1);
     }
-    i = j;
   }
   if (!a.whole && tid == 0) a.meta[blockIdx.x] = start;
 }
