@@ -467,8 +467,10 @@ int moe_rope_append(const uint16_t* qkv, int64_t qkv_stride, const float* cos, c
  *   apart; out [seqs, heads, head_dim] packed.  fp32 scores, softmax and sums;
  *   the probabilities are rounded to the element type for the product with V.
  *   What lies in a page past a sequence's end (infinities, NaN) has no effect.
- *   page_size % 16 == 0, seqs <= 8191, scale > 0.  The workspace needs no
- *   initialisation.  Results do not vary from call to call. */
+ *   page_size % 16 == 0, seqs <= 4095, scale > 0.  The first 4096
+ *   bytes of the workspace (counters) must be zero before its first call; every
+ *   call leaves them zero, so a workspace serves calls of any shape it is large
+ *   enough for, one after another.  Results do not vary from call to call. */
 size_t moe_paged_attention_workspace_size(int seqs, int max_pages, int page_size, int heads,
                                           int kv_heads, int head_dim);
 int moe_paged_attention(const uint16_t* q, int64_t q_stride, uint16_t* k_pages,

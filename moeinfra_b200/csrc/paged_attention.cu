@@ -23,8 +23,8 @@
 //     (tcgen05 wants 128 rows; with at most 16 heads to a key they would be
 //     empty, and the memory bound is already reached.)
 //   * Pieces of a (sequence, KV head) are joined in the order of their keys:
-//     within a CTA through shared memory, between CTAs by a second small
-//     launch.  The sums' order depends on the lengths and the GPU only.
+//     within a CTA through shared memory, between CTAs by the last of them to
+//     finish.  The sums' order depends on the lengths and the GPU only.
 #include "paged.cuh"
 
 namespace moe {
@@ -35,7 +35,7 @@ MOE_DEFINE_ERROR_WORD()
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kChunk = 16;          // keys per chunk (a page holds whole chunks)
-constexpr int kMaxSeqs = 8191;      // their chunk counts' prefix sums sit in shared memory
+constexpr int kMaxSeqs = 4095;      // their lengths and chunk counts sit in shared memory
 // Smallest share of a CTA in chunks when the line is cut: below it a CTA's
 // pieces cost more to join than they save.
 constexpr int kMinShare = 16;
@@ -47,12 +47,14 @@ struct PagedArgs {
   const int32_t* lengths;
   KvPages kv;
   float scale_log2;       // scale * log2(e)
-  int group;              // query heads per KV head
-  int parts;              // head tiles of a group (more than one above 16 heads)
-  bool whole;             // one CTA per unit: no cut, no second launch
+  int heads, per_seq;     // query heads; units (head tiles) of a sequence
+  int tile;               // query heads of a unit, at most 8 * NT
+  int parts;              // units of a KV head (more than one above 16 heads)
+  int page_chunks;        // chunks of a page
+  int page_shift;         // log2 of that, or -1
+  int* counts;            // [CTAs]: pieces written of the unit that starts in a CTA; zero between calls
   float* part;            // [CTAs][2] pieces
   float* warp_part;       // [CTAs][kWarps] pieces
-  int2* meta;             // [CTAs]: the unit whose pieces start in the CTA, their count
 };
 
 // A piece in memory: O [heads of a tile][HD + 4] fp32 (the pad keeps the 4
@@ -67,22 +69,24 @@ constexpr int stage_bytes() { return 2 * kChunk * HD * 2; }
 template <int HD>
 constexpr int ring_bytes() { return kWarps * stages<HD>() * stage_bytes<HD>(); }
 template <int HD>
-int smem_bytes(int seqs) { return ring_bytes<HD>() + (seqs + 1) * 4; }
+int smem_bytes(int seqs) { return ring_bytes<HD>() + (2 * seqs + 1) * 4; }
 
-// Chunk x of the line: its sequence, unit (head tile of a sequence), and place.
+// Chunk x of the line: its sequence b, unit u (head tile) in it, the unit's
+// number of chunks n and the chunk's place kc in it.  prefix counts the chunks
+// of one unit per sequence.
 struct Where {
-  int b, unit, n, kc;
+  int b, u, n, kc;
 };
 __device__ __forceinline__ Where where(int x, const int* prefix, int seqs, int per_seq) {
-  int lo = 0, hi = seqs;  // last b with prefix[b] <= x
+  int lo = 0, hi = seqs;  // last b with prefix[b] * per_seq <= x
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (prefix[mid] <= x) lo = mid;
+    if (prefix[mid] * per_seq <= x) lo = mid;
     else hi = mid;
   }
-  const int n = (prefix[lo + 1] - prefix[lo]) / per_seq;
-  const int r = x - prefix[lo], u = r / n;
-  return Where{lo, lo * per_seq + u, n, r - u * n};
+  const int n = prefix[lo + 1] - prefix[lo];
+  const uint32_t r = x - prefix[lo] * per_seq, u = r / (uint32_t)n;
+  return Where{lo, (int)u, n, (int)(r - u * n)};
 }
 
 __device__ __forceinline__ int clamp_len(int len, const KvPages& kv) {
@@ -90,24 +94,86 @@ __device__ __forceinline__ int clamp_len(int len, const KvPages& kv) {
   return len < 0 ? 0 : (len > most ? static_cast<int>(most) : len);
 }
 
-template <typename T, int HD, int NT>
+// One lane's HD / 32 values of output row (b, h), divided by the softmax's sum.
+template <typename T, int HD>
+__device__ __forceinline__ void write_row(const PagedArgs& a, int b, int h, int lane,
+                                          const float (&acc)[HD / 32], float sum) {
+  constexpr int kVec = HD / 32;
+  const float inv = __fdividef(1.f, sum);
+  uint32_t* o = reinterpret_cast<uint32_t*>(a.out + ((int64_t)b * a.heads + h) * HD + lane * kVec);
+#pragma unroll
+  for (int v = 0; v < kVec; v += 2) o[v / 2] = T::pack(acc[v] * inv, acc[v + 1] * inv);
+}
+
+// WHOLE: CTA x has unit x to itself (see whole_units).  Then nothing depends on
+// the other sequences' lengths, and the unit's pages, its queries and its
+// length are read at once instead of one after the other.
+template <typename T, int HD, int NT, bool WHOLE>
 __global__ void __launch_bounds__(kThreads, 1) k_paged_attention(const PagedArgs a) {
   constexpr int S = stages<HD>(), kHeads = NT * 8, kPitch = HD + 4;
   constexpr int kRow = HD * 2;                  // bytes of a row
   constexpr int kTile = kChunk * kRow;          // bytes of a chunk's keys (or values)
   extern __shared__ __align__(128) unsigned char smem[];
   int* prefix = reinterpret_cast<int*>(smem + ring_bytes<HD>());
+  int* s_len = prefix + a.kv.seqs + 1;
   __shared__ int s_scan[kWarps];
-  __shared__ int4 s_info[kWarps][S];            // unit, b, rows that count, bit 0 first / bit 1 last
-  __shared__ int s_unit[2 * kWarps], s_ends[2 * kWarps];
+  __shared__ int4 s_info[kWarps][S];            // b, u, rows that count, bit 0 first / bit 1 last
+  __shared__ int4 s_piece[2 * kWarps];           // b (or -1), u, bit 0 first / bit 1 last
   __shared__ float s_ml[2 * kWarps][2][kHeads];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const KvPages& kv = a.kv;
-  const int per_seq = kv.kv_heads * a.parts;
+  const int per_seq = a.per_seq;
+  // Rows sit at their own pitch, 16-byte pieces exchanged by the low bits of
+  // the row: the 8 rows of an ldmatrix tile touch all banks.
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) +
+                        warp * S * stage_bytes<HD>();
+  constexpr int kPieces = HD / 8, kRows = 32 / kPieces, kSame = 8 / kRows;
+  const int cp_row = lane / kPieces, cp_piece = lane % kPieces;
+  uint32_t cp_at[kSame];  // the pattern repeats after 8 rows
+#pragma unroll
+  for (int i = 0; i < kSame; ++i) {
+    const int r = i * kRows + cp_row;
+    cp_at[i] = ring + r * kRow + ((cp_piece ^ r) << 4);
+  }
+  const int cp_el = cp_row * HD + cp_piece * 8;
+  uint32_t qf[NT][HD / 16][2];
+  auto load_q = [&](uint32_t (&dst)[NT][HD / 16][2], int b, int u) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const bool real = nt * 8 + g < a.tile;
+      const uint16_t* src =
+          a.q + b * a.q_stride + (int64_t)(u * a.tile + (real ? nt * 8 + g : 0)) * HD + 2 * t4;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        dst[nt][kk][0] = !real ? 0u : *reinterpret_cast<const uint32_t*>(src + kk * 16);
+        dst[nt][kk][1] = !real ? 0u : *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8);
+      }
+    }
+  };
+  if (tid < 2 * kWarps) s_piece[tid] = make_int4(-1, 0, 0, 0);
   pdl_trigger();
   pdl_wait();
 
-  // Prefix sums of the sequences' chunk counts (all units of a sequence).
+  int lo, hi, share = 0;  // this CTA's chunks (WHOLE: counted in the unit)
+  int own_b = 0, own_u = 0, own_len = 0;
+  int64_t own_page[2] = {};  // WHOLE: pages of the chunks lane and lane + 32
+  if constexpr (WHOLE) {
+    own_b = blockIdx.x / (uint32_t)per_seq;
+    own_u = blockIdx.x - own_b * per_seq;
+    const int len = a.lengths[own_b];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int kc = lane + 32 * i, entry = a.page_shift >= 0 ? kc >> a.page_shift : kc / a.page_chunks;
+      own_page[i] = entry < kv.max_pages ? kv.table[own_b * kv.table_stride + entry] : -1;
+    }
+    load_q(qf, own_b, own_u);
+    own_len = clamp_len(len, kv);
+    if (own_len != len && tid == 0) set_device_error(kErrPage);
+    lo = 0;
+    hi = (own_len + kChunk - 1) / kChunk;
+  }
+  // Prefix sums of the sequences' chunk counts.
+  if constexpr (!WHOLE) {
   int run = 0;
   for (int b0 = 0; b0 < kv.seqs; b0 += kThreads) {
     const int b = b0 + tid;
@@ -115,7 +181,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_attention(const PagedArgs
     if (b < kv.seqs) {
       const int len = a.lengths[b], c = clamp_len(len, kv);
       if (c != len && blockIdx.x == 0) set_device_error(kErrPage);
-      n = (c + kChunk - 1) / kChunk * per_seq;
+      s_len[b] = c;
+      n = (c + kChunk - 1) / kChunk;
     }
     int inc = n;
 #pragma unroll
@@ -136,94 +203,90 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_attention(const PagedArgs
     __syncthreads();
   }
   if (tid == 0) prefix[kv.seqs] = run;
-  if (tid < 2 * kWarps) s_unit[tid] = -1;
   __syncthreads();
-  const int total = run;
-
-  // Sequences without keys: zeros.
-  for (int b = blockIdx.x; b < kv.seqs; b += gridDim.x) {
-    if (prefix[b + 1] != prefix[b]) continue;
-    uint32_t* o = reinterpret_cast<uint32_t*>(a.out + (int64_t)b * kv.kv_heads * a.group * HD);
-    for (int i = tid; i < kv.kv_heads * a.group * HD / 2; i += kThreads) o[i] = 0;
-  }
-
-  int lo, hi, share = 0;  // this CTA's chunks
-  if (a.whole) {
-    const int b = blockIdx.x / per_seq, u = blockIdx.x % per_seq;
-    const int n = (prefix[b + 1] - prefix[b]) / per_seq;
-    lo = prefix[b] + u * n;
-    hi = lo + n;
-  } else {
-    share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, kMinShare);
-    lo = (int)min((int64_t)blockIdx.x * share, (int64_t)total);
-    hi = min(lo + share, total);
+  const int total = run * per_seq;
+  share = max((int)(((uint32_t)total + gridDim.x - 1) / gridDim.x), kMinShare);
+  lo = (int)min((int64_t)blockIdx.x * share, (int64_t)total);
+  hi = min(lo + share, total);
   }
   const int each = (hi - lo + kWarps - 1) / kWarps;
   const int ws = min(lo + warp * each, hi), we = min(ws + each, hi);
 
   // ---- this warp's chunks [ws, we) ----
-  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) +
-                        warp * S * stage_bytes<HD>();
-  // Rows sit at their own pitch, 16-byte pieces exchanged by the low bits of
-  // the row: the 8 rows of an ldmatrix tile touch all banks.
-  constexpr int kPieces = HD / 8, kRows = 32 / kPieces;
-  const int cp_row = lane / kPieces, cp_piece = lane % kPieces;
   // Places of the next 32 chunks, one per lane (computed once per 32).
   int d_base = ws;
   int64_t d_k = 0, d_v = 0;
-  int d_unit = 0, d_b = 0, d_rows = 0, d_ends = 0;
+  int d_u = 0, d_b = 0, d_rows = 0, d_ends = 0;
   auto look_up = [&](int base) {
     d_base = base;
     const int x = base + lane;
+    Where w{own_b, own_u, hi, x};
+    int64_t page = 0;
+    int entry = 0;
+    if constexpr (WHOLE) {
+      const int64_t p0 = __shfl_sync(0xffffffffu, own_page[0], x & 31);
+      const int64_t p1 = __shfl_sync(0xffffffffu, own_page[1], x & 31);
+      page = x < 32 ? p0 : p1;
+    }
     if (x >= we) return;
-    const Where w = where(x, prefix, kv.seqs, per_seq);
-    const int p0 = w.kc * kChunk;
-    int64_t page = kv.table[w.b * kv.table_stride + p0 / kv.page_size];
+    if constexpr (!WHOLE) w = where(x, prefix, kv.seqs, per_seq);
+    entry = a.page_shift >= 0 ? w.kc >> a.page_shift : w.kc / a.page_chunks;
+    if constexpr (!WHOLE) page = kv.table[w.b * kv.table_stride + entry];
     if (page < 0 || page >= kv.num_pages) {
       set_device_error(kErrPage);
       page = 0;
     }
-    const int head = (w.unit - w.b * per_seq) / a.parts;
-    const int64_t in_page = ((int64_t)head * kv.page_size + p0 % kv.page_size) * HD;
+    const int head = a.parts == 1 ? w.u : w.u / a.parts;
+    const int64_t in_page =
+        ((int64_t)head * kv.page_size + (w.kc - entry * a.page_chunks) * kChunk) * HD;
     d_k = page * kv.k_stride + in_page;
     d_v = page * kv.v_stride + in_page;
-    d_unit = w.unit;
+    d_u = w.u;
     d_b = w.b;
-    d_rows = min(kChunk, clamp_len(a.lengths[w.b], kv) - p0);
+    d_rows = min(kChunk, (WHOLE ? own_len : s_len[w.b]) - w.kc * kChunk);
     d_ends = (w.kc == 0 ? 1 : 0) | (w.kc == w.n - 1 ? 2 : 0);
   };
+
+  // A unit's queries are loaded when its first chunk is issued, ahead of their
+  // use, where the registers allow it (not for 16 heads of 128).
+  constexpr bool kAhead = !WHOLE && NT * HD <= 128;
+  uint32_t qn[NT][HD / 16][2];
+  int ahead_b = -1, ahead_u = 0;  // whose queries qn holds
+
   auto issue = [&](int x, int stage) {
     if (x < we) {
       if (x - d_base == 32) look_up(x);
       const int from = x - d_base;
       const int64_t ok = __shfl_sync(0xffffffffu, d_k, from), ov = __shfl_sync(0xffffffffu, d_v, from);
       const int rows = __shfl_sync(0xffffffffu, d_rows, from);
-      if (lane == from) s_info[warp][stage] = make_int4(d_unit, d_b, d_rows, d_ends);
-      const uint32_t dst = ring + stage * stage_bytes<HD>();
+      if (lane == from) s_info[warp][stage] = make_int4(d_b, d_u, d_rows, d_ends);
+      const uint32_t off = stage * stage_bytes<HD>();
+      const uint16_t *pk = kv.k + ok + cp_el, *pv = kv.v + ov + cp_el;
 #pragma unroll
       for (int i = 0; i < kChunk / kRows; ++i) {
-        const int r = i * kRows + cp_row;
-        const uint32_t at = dst + r * kRow + ((cp_piece ^ (r & 7)) << 4);
-        const int64_t el = (int64_t)r * HD + cp_piece * 8;
-        cp_async16(at, kv.k + ok + el, r < rows);
-        cp_async16(at + kTile, kv.v + ov + el, r < rows);
+        const uint32_t at = cp_at[i % kSame] + off + i / kSame * 8 * kRow;
+        const bool take = i * kRows + cp_row < rows;
+        cp_async16(at, pk + i * kRows * HD, take);
+        cp_async16(at + kTile, pv + i * kRows * HD, take);
+      }
+      if constexpr (kAhead) {
+        const int ends = __shfl_sync(0xffffffffu, d_ends, from);
+        if (ahead_b < 0 && ((ends & 1) || x == ws)) {
+          ahead_b = __shfl_sync(0xffffffffu, d_b, from);
+          ahead_u = __shfl_sync(0xffffffffu, d_u, from);
+          load_q(qn, ahead_b, ahead_u);
+        }
       }
     }
     cp_async_commit();
   };
 
-  uint32_t qf[NT][HD / 16][2];
   float o[NT][HD / 16][4];
   float m[NT][2], l[NT][2];
-  int cur = -1, cur_b = 0;
+  int cur_b = -1, cur_u = 0;  // the unit at hand
   bool cur_first = false;
-
-  auto head_of = [&](int unit, int nt, int col) {  // query head of a column, or -1
-    const int u = unit % per_seq, h = (u % a.parts) * kHeads + nt * 8 + col;
-    return h < a.group ? u / a.parts * a.group + h : -1;
-  };
   if (ws < we) look_up(ws);
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < S - 1; ++s) issue(ws + s, s);
   int stage = 0;
   for (int x = ws; x < we; ++x) {
@@ -233,21 +296,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_attention(const PagedArgs
     cp_async_wait<S - 1>();
     __syncwarp();
     const int4 info = s_info[warp][stage];
-    if (info.x != cur) {  // a new unit: its queries, an empty softmax
-      cur = info.x;
-      cur_b = info.y;
+    if (cur_b < 0) {  // a new unit: its queries, an empty softmax
+      cur_b = info.x;
+      cur_u = info.y;
       cur_first = info.w & 1;
+      if (kAhead && ahead_b == cur_b && ahead_u == cur_u) {
+        ahead_b = -1;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            qf[nt][kk][0] = qn[nt][kk][0];
+            qf[nt][kk][1] = qn[nt][kk][1];
+          }
+      } else if (!WHOLE) {
+        load_q(qf, cur_b, cur_u);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int h = head_of(cur, nt, g);
-        const uint16_t* src = a.q + cur_b * a.q_stride + (int64_t)(h < 0 ? 0 : h) * HD + 2 * t4;
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          qf[nt][kk][0] = h < 0 ? 0u : *reinterpret_cast<const uint32_t*>(src + kk * 16);
-          qf[nt][kk][1] = h < 0 ? 0u : *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[nt][kk][i] = 0.f;
-        }
+        for (int i = 0; i < HD / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
         m[nt][0] = m[nt][1] = -INFINITY;
         l[nt][0] = l[nt][1] = 0.f;
       }
@@ -332,10 +400,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_attention(const PagedArgs
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int h = head_of(cur, nt, 2 * t4 + c);
-          if (h < 0) continue;
-          const float inv = 1.f / l[nt][c];
-          uint16_t* dst = a.out + ((int64_t)cur_b * kv.kv_heads * a.group + h) * HD;
+          const int col = nt * 8 + 2 * t4 + c;
+          if (col >= a.tile) continue;
+          const float inv = __fdividef(1.f, l[nt][c]);
+          uint16_t* dst = a.out + ((int64_t)cur_b * a.heads + cur_u * a.tile + col) * HD;
 #pragma unroll
           for (int i = 0; i < HD / 16; ++i) {
             dst[i * 16 + g] = T::one(o[nt][i][c] * inv);
@@ -366,73 +434,69 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_attention(const PagedArgs
             s_ml[slot][1][col] = l[nt][c];
           }
         }
-      if (lane == 0) {
-        s_unit[slot] = cur;
-        s_ends[slot] = (cur_first ? 1 : 0) | (unit_ends ? 2 : 0);
-      }
+      if (lane == 0)
+        s_piece[slot] = make_int4(cur_b, cur_u, (cur_first ? 1 : 0) | (unit_ends ? 2 : 0), 0);
     }
-    cur = -1;
+    cur_b = -1;
   }
   cp_async_wait<0>();
   __syncthreads();
 
   // ---- join the warps' pieces, unit by unit, in the order of the keys ----
-  // Lane k holds the k-th piece of the CTA; every warp sees the same list and
-  // takes its share of the (unit, head) sums, one row of HD values each.
-  const int held = lane < 2 * kWarps ? s_unit[lane] : -1;
-  const uint32_t used = __ballot_sync(0xffffffffu, held >= 0);
-  const int pieces = __popc(used);
-  int slot = 0;
-  for (uint32_t rest = used, k = 0; rest; rest &= rest - 1, ++k)
-    if (lane == (int)k) slot = __ffs(rest) - 1;
-  const int unit_k = __shfl_sync(0xffffffffu, held, slot);
-  const int ends_k = lane < pieces ? s_ends[slot] : 0;
-  const int unit_before = __shfl_up_sync(0xffffffffu, unit_k, 1);
-  uint32_t starts = __ballot_sync(0xffffffffu, lane < pieces && (lane == 0 || unit_k != unit_before));
-  const uint32_t firsts = __ballot_sync(0xffffffffu, ends_k & 1);
-  const uint32_t lasts = __ballot_sync(0xffffffffu, ends_k & 2);
-  const float* src = (slot & 1) ? reinterpret_cast<const float*>(smem + (slot >> 1) * S * stage_bytes<HD>())
-                                : a.warp_part + ((int64_t)blockIdx.x * kWarps + (slot >> 1)) * piece_floats<HD, NT>();
-  int2 start = make_int2(-1, 0);
+  // Lane i holds slot i; every warp sees the same slots and takes its share of
+  // the (unit, head) sums, one row of HD values each.  A warp holds at most one
+  // piece of a unit, so a sum has at most kWarps terms: all are read at once.
+  constexpr int kVec = HD / 32;
+  const int4 held = s_piece[lane & (2 * kWarps - 1)];
+  const bool full = lane < 2 * kWarps && held.x >= 0;
+  const uint32_t used = __ballot_sync(0xffffffffu, full);
+  const uint32_t firsts = __ballot_sync(0xffffffffu, full && (held.z & 1));
+  const uint32_t lasts = __ballot_sync(0xffffffffu, full && (held.z & 2));
+  // A sum begins at the first piece and after each last one.
+  const uint32_t below = used & ((1u << lane) - 1);
+  uint32_t starts = __ballot_sync(
+      0xffffffffu, full && (below == 0 || (lasts >> (31 - __clz(below)) & 1)));
+  int open = 0;              // pieces of units that other CTAs share: bit 0 and 1 as the slot
   int turn = 0;
   while (starts) {
     const int i = __ffs(starts) - 1;
     starts &= starts - 1;
-    const int j = starts ? __ffs(starts) - 1 : pieces;
-    const uint32_t range = ((1u << j) - 1) & ~((1u << i) - 1);
-    const int unit = __shfl_sync(0xffffffffu, unit_k, i);
-    const bool first = firsts & range, last = lasts & range;
-    const int cols = min(kHeads, a.group - unit % a.parts * kHeads);
+    const uint32_t range = used & ~((1u << i) - 1) & (starts ? (starts & -starts) - 1 : ~0u);
+    const int b = WHOLE ? own_b : __shfl_sync(0xffffffffu, held.x, i);
+    const int u = WHOLE ? own_u : __shfl_sync(0xffffffffu, held.y, i);
+    const bool first = firsts & range, last = lasts & range, all = WHOLE || (first && last);
     float* dst = a.part + ((int64_t)blockIdx.x * 2 + (first ? 1 : 0)) * piece_floats<HD, NT>();
-    for (int col = 0; col < cols; ++col, turn = turn + 1 == kWarps ? 0 : turn + 1) {
-      if (turn != warp) continue;
-      const bool mine = lane >= i && lane < j;
-      const float ms = mine ? s_ml[slot][0][col] : -INFINITY;
-      float mm = ms;
+    if (!all) open |= first ? 2 : 1;
+    for (int col = (warp - turn) & (kWarps - 1); col < a.tile; col += kWarps) {
+      float ms[kWarps], val[kWarps][kVec], mm = -INFINITY, ll = 0.f, acc[kVec] = {};
+      uint32_t rest = range;
 #pragma unroll
-      for (int off = 16; off; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
-      const float f = ms == mm ? 1.f : exp2_approx(ms - mm);
-      float ll = mine ? f * s_ml[slot][1][col] : 0.f;
+      for (int k = 0; k < kWarps; ++k) {
+        const int sk = rest ? __ffs(rest) - 1 : -1;
+        rest &= rest - 1;
+        ms[k] = -INFINITY;
+        if (sk < 0) continue;
+        const float* p =
+            ((sk & 1) ? reinterpret_cast<const float*>(smem + (sk >> 1) * S * stage_bytes<HD>())
+                      : a.warp_part + ((int64_t)blockIdx.x * kWarps + (sk >> 1)) * piece_floats<HD, NT>()) +
+            col * kPitch + lane * kVec;
 #pragma unroll
-      for (int off = 16; off; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
-      constexpr int kVec = HD / 32;
-      float acc[kVec] = {};
-#pragma unroll 4
-      for (int k = i; k < j; ++k) {
-        const float fk = __shfl_sync(0xffffffffu, f, k);
-        const float* p = reinterpret_cast<const float*>(
-                             __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(src), k)) +
-                         col * kPitch + lane * kVec;
-#pragma unroll
-        for (int v = 0; v < kVec; ++v) acc[v] += fk * p[v];
+        for (int v = 0; v < kVec; ++v) val[k][v] = p[v];
+        ms[k] = s_ml[sk][0][col];
+        mm = fmaxf(mm, ms[k]);
       }
-      if (first && last) {
-        const float inv = 1.f / ll;
-        const int h = head_of(unit, col >> 3, col & 7);
-        uint32_t* o32 = reinterpret_cast<uint32_t*>(
-            a.out + ((int64_t)(unit / per_seq) * kv.kv_heads * a.group + h) * HD + lane * kVec);
+      rest = range;
 #pragma unroll
-        for (int v = 0; v < kVec; v += 2) o32[v / 2] = T::pack(acc[v] * inv, acc[v + 1] * inv);
+      for (int k = 0; k < kWarps; ++k) {
+        if (!rest) continue;
+        const float f = ms[k] == mm ? 1.f : exp2_approx(ms[k] - mm);
+        ll += f * s_ml[__ffs(rest) - 1][1][col];
+        rest &= rest - 1;
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) acc[v] += f * val[k][v];
+      }
+      if (all) {
+        write_row<T, HD>(a, b, u * a.tile + col, lane, acc, ll);
       } else {
 #pragma unroll
         for (int v = 0; v < kVec; ++v) dst[col * kPitch + lane * kVec + v] = acc[v];
@@ -442,69 +506,99 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_attention(const PagedArgs
         }
       }
     }
-    if (first && !last) {  // further pieces lie in the CTAs after this one
-      const int b = unit / per_seq, n = (prefix[b + 1] - prefix[b]) / per_seq;
-      const int end = prefix[b] + (unit - b * per_seq + 1) * n;
-      start = make_int2(unit, (end - 1) / share - (int)blockIdx.x + 1);
+    turn += a.tile;
+  }
+
+  // Sequences without keys: zeros.
+  if constexpr (WHOLE) {
+    if (hi == 0)
+      for (int col = warp; col < a.tile; col += kWarps) {
+        const float none[kVec] = {};
+        write_row<T, HD>(a, own_b, own_u * a.tile + col, lane, none, 1.f);
+      }
+  } else {
+  for (int b = blockIdx.x; b < kv.seqs; b += gridDim.x) {
+    if (prefix[b + 1] != prefix[b]) continue;
+    uint32_t* o = reinterpret_cast<uint32_t*>(a.out + (int64_t)b * a.heads * HD);
+    for (int i = tid; i < a.heads * HD / 2; i += kThreads) o[i] = 0;
+  }
+  if (!open) return;
+
+  // ---- join the CTAs' pieces: the last CTA of a unit to get here does it ----
+  // A unit is counted at the CTA that holds its start.  Whoever finds the count
+  // full sees every piece (each CTA's are fenced before its count) and sets the
+  // counter back to zero for the next launch.
+  // Bit 0: the piece of the unit that the CTA's first chunk belongs to; bit 1:
+  // that of its last chunk.
+  __shared__ int4 s_join[2];  // b, u, first CTA, pieces (0: not the last)
+  __threadfence();
+  __syncthreads();
+  if (tid < 2) {
+    s_join[tid].w = 0;
+    if (open >> tid & 1) {
+      const Where w = where(tid ? hi - 1 : lo, prefix, kv.seqs, per_seq);
+      const int from = prefix[w.b] * per_seq + w.u * w.n;
+      const int c0 = from / share, np = (from + w.n - 1) / share - c0 + 1;
+      if (atomicAdd(a.counts + c0, 1) == np - 1) {
+        a.counts[c0] = 0;
+        s_join[tid] = make_int4(w.b, w.u, c0, np);
+      }
     }
   }
-  if (!a.whole && tid == 0) a.meta[blockIdx.x] = start;
-}
-
-// Joins the pieces of the unit that starts in CTA x of the first launch and
-// ends in another; one block per head of the tile, one thread per dimension.
-template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(HD) k_paged_join(const PagedArgs a) {
-  constexpr int kHeads = NT * 8, kPitch = HD + 4, kPiece = piece_floats<HD, NT>();
-  pdl_trigger();
-  pdl_wait();
-  const int2 meta = a.meta[blockIdx.x];
-  if (meta.x < 0) return;
-  const int col = blockIdx.y, d = threadIdx.x;
-  const int per_seq = a.kv.kv_heads * a.parts, u = meta.x % per_seq;
-  const int h = u % a.parts * kHeads + col;
-  if (h >= a.group) return;
-  // Piece 0 is the CTA's second, the others the first of the CTAs after it.
-  const float* base = a.part + (int64_t)blockIdx.x * 2 * kPiece;
-  float mm = -INFINITY, ll = 0.f, oo = 0.f;
+  __syncthreads();
+  for (int w = 0; w < 2; ++w) {
+    const int4 job = s_join[w];
+    const int np = job.w;
+    if (np == 0) continue;
+    __threadfence();
+    // Piece 0 is CTA c0's second, the others the first of the CTAs after it.
+    const float* base = a.part + (int64_t)job.z * 2 * piece_floats<HD, NT>();
+    for (int col = warp; col < a.tile; col += kWarps) {
+      float mm = -INFINITY, ll = 0.f, acc[kVec] = {};
 #pragma unroll 4
-  for (int i = 0; i < meta.y; ++i) {
-    const float* p = base + (int64_t)(i == 0 ? 1 : 2 * i) * kPiece;
-    const float ms = p[kHeads * kPitch + col], ls = p[kHeads * kPitch + kHeads + col];
-    const float os = p[col * kPitch + d];
-    const float nm = fmaxf(mm, ms);
-    const float f0 = mm == nm ? 1.f : exp2_approx(mm - nm), f1 = ms == nm ? 1.f : exp2_approx(ms - nm);
-    ll = ll * f0 + ls * f1;
-    oo = oo * f0 + os * f1;
-    mm = nm;
+      for (int k = 0; k < np; ++k) {
+        const float* p = base + (int64_t)(k == 0 ? 1 : 2 * k) * piece_floats<HD, NT>();
+        const float ms = __ldcg(p + kHeads * kPitch + col), ls = __ldcg(p + kHeads * kPitch + kHeads + col);
+        float val[kVec];
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) val[v] = __ldcg(p + col * kPitch + lane * kVec + v);
+        const float nm = fmaxf(mm, ms);
+        const float f0 = mm == nm ? 1.f : exp2_approx(mm - nm), f1 = ms == nm ? 1.f : exp2_approx(ms - nm);
+        ll = ll * f0 + ls * f1;
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) acc[v] = acc[v] * f0 + val[v] * f1;
+        mm = nm;
+      }
+      write_row<T, HD>(a, job.x, job.y * a.tile + col, lane, acc, ll);
+    }
   }
-  a.out[((int64_t)(meta.x / per_seq) * a.kv.kv_heads * a.group + u / a.parts * a.group + h) * HD + d] =
-      T::one(oo / ll);
+  }
 }
 
-template <typename T, int HD, int NT>
+template <typename T, int HD, int NT, bool WHOLE>
 bool paged_attr() {
-  return cudaFuncSetAttribute(k_paged_attention<T, HD, NT>,
+  return cudaFuncSetAttribute(k_paged_attention<T, HD, NT, WHOLE>,
                               cudaFuncAttributeMaxDynamicSharedMemorySize,
                               smem_bytes<HD>(kMaxSeqs)) == cudaSuccess;
 }
 
 // Whether a call gives each unit (sequence, KV head, head tile) a CTA of its
 // own: few units and a table that holds at most 64 chunks (1024 tokens) each.
-// Its 8 warps then read up to 8 chunks one after the other, which takes no
-// longer than the second launch that joins a cut would.
 bool whole_units(int64_t units, int64_t chunks) { return units <= sm_count() && chunks <= 64; }
 
 struct Shape {
-  int parts, nt;
+  int parts, tile, nt;
   int64_t units, chunks;
   int ctas;
   bool whole;
 };
 Shape shape_of(int64_t seqs, int kv_heads, int group, int64_t max_tokens) {
   Shape s;
-  s.nt = group <= 8 ? 1 : 2;
+  // Groups above 16 heads are read by several units, of equal numbers of heads.
   s.parts = static_cast<int>(ceil_div(group, 16));
+  while (group % s.parts) ++s.parts;
+  s.tile = group / s.parts;
+  s.nt = s.tile <= 8 ? 1 : 2;
   s.units = seqs * kv_heads * s.parts;
   s.chunks = ceil_div(max_tokens, kChunk);
   s.whole = whole_units(s.units, s.chunks);
@@ -512,35 +606,32 @@ Shape shape_of(int64_t seqs, int kv_heads, int group, int64_t max_tokens) {
   return s;
 }
 
-size_t workspace_floats(const Shape& s, int hd) {
-  if (s.whole) return (size_t)s.ctas * kWarps * (s.nt * 8 * (hd + 4) + 2 * s.nt * 8);
-  return (size_t)s.ctas * (2 + kWarps) * (s.nt * 8 * (hd + 4) + 2 * s.nt * 8) + (size_t)s.ctas * 2;
+// The counters lead, so that calls of any shape keep them at the same place.
+constexpr size_t kCountBytes = 4096;
+size_t workspace_size(const Shape& s, int hd) {
+  if (s.whole) return kCountBytes;
+  return kCountBytes +
+         sizeof(float) * s.ctas * (2 + kWarps) * (s.nt * 8 * (hd + 4) + 2 * s.nt * 8);
 }
 
-template <typename T, int HD, int NT>
-int launch_paged(PagedArgs& a, const Shape& sh, float* ws, cudaStream_t s) {
-  if (!once_per_device(reinterpret_cast<const void*>(&paged_attr<T, HD, NT>), &paged_attr<T, HD, NT>))
+template <typename T, int HD, int NT, bool WHOLE>
+int launch_paged(PagedArgs& a, const Shape& sh, cudaStream_t s) {
+  if (!once_per_device(reinterpret_cast<const void*>(&paged_attr<T, HD, NT, WHOLE>),
+                       &paged_attr<T, HD, NT, WHOLE>))
     return MOE_ERR_CUDA;
-  a.warp_part = ws;
-  a.part = ws + (size_t)sh.ctas * kWarps * piece_floats<HD, NT>();
-  a.meta = reinterpret_cast<int2*>(a.part + (size_t)sh.ctas * 2 * piece_floats<HD, NT>());
-  if (launch_pdl(k_paged_attention<T, HD, NT>, dim3(sh.ctas), dim3(kThreads),
-                 smem_bytes<HD>(a.kv.seqs), s, a) != cudaSuccess)
-    return MOE_ERR_CUDA;
-  MOE_CHECK_LAUNCH();
-  if (sh.whole) return MOE_OK;
-  const int cols = a.group < NT * 8 ? a.group : NT * 8;
-  if (launch_pdl(k_paged_join<T, HD, NT>, dim3(sh.ctas, cols), dim3(HD), 0, s, a) != cudaSuccess)
+  a.part = a.warp_part + (size_t)sh.ctas * kWarps * piece_floats<HD, NT>();
+  if (launch_pdl(k_paged_attention<T, HD, NT, WHOLE>, dim3(sh.ctas), dim3(kThreads),
+                 WHOLE ? ring_bytes<HD>() : smem_bytes<HD>(a.kv.seqs), s, a) != cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
   return MOE_OK;
 }
 
-template <typename T>
-int launch_typed(PagedArgs& a, const Shape& sh, int hd, float* ws, cudaStream_t s) {
-  if (hd == 64)
-    return sh.nt == 1 ? launch_paged<T, 64, 1>(a, sh, ws, s) : launch_paged<T, 64, 2>(a, sh, ws, s);
-  return sh.nt == 1 ? launch_paged<T, 128, 1>(a, sh, ws, s) : launch_paged<T, 128, 2>(a, sh, ws, s);
+template <typename T, int HD>
+int launch_wide(PagedArgs& a, const Shape& sh, cudaStream_t s) {
+  if (sh.whole)
+    return sh.nt == 1 ? launch_paged<T, HD, 1, true>(a, sh, s) : launch_paged<T, HD, 2, true>(a, sh, s);
+  return sh.nt == 1 ? launch_paged<T, HD, 1, false>(a, sh, s) : launch_paged<T, HD, 2, false>(a, sh, s);
 }
 
 }  // namespace
@@ -553,7 +644,7 @@ extern "C" size_t moe_paged_attention_workspace_size(int seqs, int max_pages, in
       (head_dim != 64 && head_dim != 128))
     return 0;
   const Shape sh = shape_of(seqs, kv_heads, heads / kv_heads, (int64_t)max_pages * page_size);
-  return workspace_floats(sh, head_dim) * sizeof(float);
+  return workspace_size(sh, head_dim);
 }
 
 extern "C" int moe_paged_attention(const uint16_t* q, int64_t q_stride, uint16_t* k_pages,
@@ -584,7 +675,7 @@ extern "C" int moe_paged_attention(const uint16_t* q, int64_t q_stride, uint16_t
   // Chunk numbers are 32-bit on the device.
   if ((int64_t)max_pages * page_size > INT32_MAX || sh.units * sh.chunks > INT32_MAX)
     return MOE_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < workspace_floats(sh, head_dim) * sizeof(float))
+  if (!workspace || workspace_bytes < workspace_size(sh, head_dim))
     return MOE_ERR_WORKSPACE;
   if (!aligned16(workspace)) return MOE_ERR_ALIGNMENT;
   PagedArgs a{};
@@ -595,11 +686,18 @@ extern "C" int moe_paged_attention(const uint16_t* q, int64_t q_stride, uint16_t
   a.kv = KvPages{k_pages, v_pages, k_page_stride, v_page_stride, num_pages, block_table,
                  table_stride, seqs, max_pages, page_size, kv_heads};
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.group = heads / kv_heads;
+  a.heads = heads;
+  a.per_seq = kv_heads * sh.parts;
+  a.tile = sh.tile;
   a.parts = sh.parts;
-  a.whole = sh.whole;
+  a.page_chunks = page_size / kChunk;
+  a.page_shift = -1;
+  for (int i = 0; i < 27; ++i)
+    if (a.page_chunks == 1 << i) a.page_shift = i;
+  a.counts = static_cast<int*>(workspace);
+  a.warp_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCountBytes);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  float* ws = static_cast<float*>(workspace);
-  return dtype == MOE_DTYPE_F16 ? launch_typed<F16>(a, sh, head_dim, ws, s)
-                                : launch_typed<BF16>(a, sh, head_dim, ws, s);
+  if (dtype == MOE_DTYPE_F16)
+    return head_dim == 64 ? launch_wide<F16, 64>(a, sh, s) : launch_wide<F16, 128>(a, sh, s);
+  return head_dim == 64 ? launch_wide<BF16, 64>(a, sh, s) : launch_wide<BF16, 128>(a, sh, s);
 }

@@ -590,22 +590,26 @@ def ep_return_partials_p2p(y_part: torch.Tensor, recv_counts: torch.Tensor, num_
 # ---------------------------------------------------------------------------
 
 _DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_COUNTER_BYTES = 4096  # the part of a workspace that has to be zero before its first call
 _serve_ws: dict = {}
 
 
 def _serve_scratch(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    """Scratch of the serving operators: one buffer per (device, stream, power of two), kept.
+    """Scratch of the serving operators, its leading counters zeroed (every call leaves them so).
 
-    Calls on one stream are ordered and every kernel waits for its predecessor before it
-    touches scratch.  A call under stream capture gets scratch of its own from the graph's
-    pool: graphs captured on one stream may be replayed side by side.
+    One buffer per (device, stream, power of two), kept: calls on one stream are ordered and
+    every kernel waits for its predecessor before it touches scratch.  A call under stream
+    capture gets scratch of its own, zeroed by the graph: graphs captured on one stream may be
+    replayed side by side.
     """
     if torch.cuda.is_current_stream_capturing():
-        return _workspace(nbytes, dev)
+        ws = _workspace(nbytes, dev)
+        ws[:_COUNTER_BYTES].zero_()
+        return ws
     key = (dev.index, stream, max(nbytes - 1, 0).bit_length())
     ws = _serve_ws.get(key)
     if ws is None:
-        ws = _serve_ws[key] = _workspace(1 << key[2], dev)
+        ws = _serve_ws[key] = torch.zeros(1 << key[2], dtype=torch.uint8, device=dev)
     return ws
 
 
@@ -708,16 +712,29 @@ def _paged_ws_bytes(device: int, seqs: int, max_pages: int, page: int, heads: in
     return _native.lib().moe_paged_attention_workspace_size(seqs, max_pages, page, heads, kv, hd)
 
 
+def paged_attention_workspace(block_table: torch.Tensor, page_size: int, num_heads: int,
+                              kv_heads: int, head_dim: int) -> torch.Tensor:
+    """A workspace for :func:`paged_attention` calls with tables of this size."""
+    nbytes = _paged_ws_bytes(block_table.device.index, *block_table.shape, page_size, num_heads,
+                             kv_heads, head_dim)
+    return torch.zeros(nbytes, dtype=torch.uint8, device=block_table.device)
+
+
 @_on_device
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                     block_table: torch.Tensor, lengths: torch.Tensor,
-                    scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                    scale: float | None = None, out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one new token per sequence over its cached keys and values.
 
     ``q`` [sequences, heads, head_dim] (rows may be strided), ``lengths`` int32 [sequences]: the
     positions each sequence sees, the token just appended included (0: a row of zeros); the rest
     as in :func:`rope_append`; ``page_size`` a multiple of 16.  ``scale`` defaults to
     ``head_dim ** -0.5``.  Returns [sequences, heads, head_dim].
+
+    ``workspace``: a buffer from :func:`paged_attention_workspace` that no call on another
+    stream uses at the same time; by default the module keeps one per stream (and a captured
+    call zeroes one of its own at every replay, which a given workspace spares).
     """
     what = "paged_attention"
     dt, n_pages, kv, page, hd = _page_geometry(what, k_pages, v_pages, block_table)
@@ -738,12 +755,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         return out
     stream = torch.cuda.current_stream(dev).cuda_stream
     nbytes = _paged_ws_bytes(dev.index, seqs, max_pages, page, heads, kv, hd)
-    ws = _serve_scratch(dev, stream, nbytes)
+    if workspace is None:
+        workspace = _serve_scratch(dev, stream, nbytes)
+    elif workspace.numel() < nbytes:
+        raise ValueError(f"{what}: workspace has {workspace.numel()} bytes, needs {nbytes}")
     check(_native.lib().moe_paged_attention(
         q.data_ptr(), _outer_stride(q), k_pages.data_ptr(),
         v_pages.data_ptr(), _outer_stride(k_pages), _outer_stride(v_pages), n_pages, page,
         block_table.data_ptr(), _outer_stride(block_table), seqs, max_pages,
         lengths.data_ptr(), heads, kv, hd, _DTYPE_CODES[dt],
-        hd ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(), nbytes, stream),
+        hd ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(), nbytes, stream),
         "moe_paged_attention")
     return out

@@ -341,7 +341,7 @@ def test_host_checks_precede_every_launch():
     assert attend(H=7) == 1 and attend(scale=0.0) == 1 and attend(scale=float("nan")) == 1
     assert attend(q=None) == 1 and attend(qs=64) == 1
     assert attend(hd=256) == 2 and attend(page=24) == 2 and attend(dtype=2) == 2
-    assert attend(seqs=8192) == 2
+    assert attend(seqs=4096) == 2
     assert attend(bytes_=need - 1) == 4 and attend(ws=None) == 4
     assert attend(q=odd) == 5 and attend(ws=odd) == 5
     assert _native.status_string(8) != "unknown status"
