@@ -480,6 +480,27 @@ int moe_paged_attention(const uint16_t* q, int64_t q_stride, uint16_t* k_pages,
                         int heads, int kv_heads, int head_dim, int dtype, float scale,
                         uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* moe_prompt_attention: o[t,h] = softmax(scale q[t,h] . K^T) V over t's own
+ *   sequence, for packed sequences: sequence b's queries are rows
+ *   cu_q[b] .. cu_q[b+1] of q [q_rows, heads, head_dim], its keys and values
+ *   rows cu_k[b] .. cu_k[b+1] of k and v [k_rows, kv_heads, head_dim] (int32
+ *   offsets, seqs + 1 each; any lengths, zero included).  Row and head strides
+ *   in elements, multiples of 8.  causal != 0: the queries are the last of the
+ *   sequence's positions, query i sees keys j <= i + len_k - len_q; a query
+ *   without keys gives zeros.  max_q / max_k: no sequence is longer (one that
+ *   is counts as out of range, and so do offsets outside the rows; rows of such
+ *   a sequence are not written).  out [q_rows, heads, head_dim] packed.  fp32
+ *   scores, softmax and sums; the probabilities are rounded to the element type
+ *   for the product with V.  Values of other sequences have no effect.
+ *   scale > 0. */
+int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t q_head_stride,
+                         int64_t q_rows, const uint16_t* k, int64_t k_stride,
+                         int64_t k_head_stride, const uint16_t* v, int64_t v_stride,
+                         int64_t v_head_stride, int64_t k_rows, const int32_t* cu_q,
+                         const int32_t* cu_k, int seqs, int max_q, int max_k, int heads,
+                         int kv_heads, int head_dim, int causal, int dtype, float scale,
+                         uint16_t* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

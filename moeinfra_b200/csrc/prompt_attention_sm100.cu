@@ -1,0 +1,520 @@
+// Causal (or full) attention over packed prompts of different lengths, with
+// grouped heads, on the 5th-generation tensor cores.
+//
+//   o[t, h] = sum_j softmax_j(scale q[t,h] . k_j) v_j
+//
+// over the keys j of t's sequence, j <= t + (len_k - len_q) if causal: the
+// queries are the last len_q of len_k positions (len_k < len_q leaves the
+// first rows without keys: zeros).
+//
+// One pass over the keys with the softmax's running maximum m and sum l.  A
+// persistent CTA per SM walks items of (256 query rows of one sequence, head),
+// the longest first.  An item is two tiles of 128 rows that take turns, so one
+// tile's softmax overlaps the other's products:
+//   warps 0-3, 4-7  softmax of tile 0 and 1, one thread per row:
+//                   S (tensor memory) -> registers, maximum, p = 2^(c s - c m),
+//                   P (16 bits) -> tensor memory over S; at the end O / l
+//   warp 8          lane 0 loads Q, K and V tiles with TMA (no multicast)
+//   warp 9          lane 0 issues tcgen05.mma: S = Q K^T (both from shared
+//                   memory), O += P V (P from tensor memory, V as stored)
+// Tensor memory: S of both tiles (2 x 128 columns), O of both (2 x HD).
+// MMAs of one thread execute in order, which orders everything but the
+// softmax: S(j) complete implies O(j-1) complete, so the softmax warps may
+// rescale O between S(j) and their P(j) without a further barrier.
+//
+// O is rescaled only when a row's maximum grew by more than 2^8 since the
+// reference in use (m is then that reference): probabilities stay below 2^8,
+// O and l are sums of the same factor, and the quotient is exact either way.
+//
+// Barriers: q_full / q_empty, full / empty of the K and V ring, s_full (S of a
+// tile), p_ready (P stored, O rescaled), o_full (last product of a tile).
+// Every wait is bounded, as in the grouped GEMM: on a timeout the error word
+// is set, the roles stop, and the CTA waits (bounded) for what it issued
+// before it frees its tensor memory.
+#include "paged.cuh"
+#include "sm100_ptx.cuh"
+
+namespace moe {
+namespace {
+
+MOE_DEFINE_ERROR_WORD()
+
+constexpr int kM = 128;         // rows of a tile
+constexpr int kN = 128;         // keys of a step
+constexpr int kSoftWarps = 8, kTmaWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 10 * 32;
+constexpr float kLazy = 8.f;    // log2 of what a row's maximum may grow before O is rescaled
+// P is rounded to 16 bits with m's reference up to 2^kLazy low: fp16 takes 2^7
+// on top (2^15 fits, normal down to 2^-21 of the reference); bf16 needs none.
+template <typename T>
+constexpr float prob_shift() { return T::kBf16 ? 0.f : 7.f; }
+
+template <int HD>
+struct Cfg {
+  static constexpr uint32_t kHalf = kM * 128;                  // 64 dims of a tile: 16 KB
+  static constexpr uint32_t kTile = kHalf * (HD / 64);         // a Q, K or V tile
+  static constexpr int kStages = HD == 128 ? 5 : 10;           // K and V tiles in flight
+  static constexpr uint32_t kSmem = (2 + kStages) * kTile + 1024;
+  static constexpr uint32_t kS = 0, kO = 2 * kN;               // TMEM columns
+};
+
+struct PromptArgs {
+  const int32_t *cu_q, *cu_k;
+  int64_t rows_q, rows_k;       // rows of q, and of k and v
+  int seqs, heads, group;       // group: query heads per KV head
+  int max_q, max_k;
+  int blocks;                   // ceil(max_q / 256)
+  bool causal;
+  float scale_log2;
+  uint16_t* out;                // [rows_q, heads, HD]
+  uint64_t wait_ns;
+};
+
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
+  return mbar_wait_or(bar, parity, limit_ns, [] { set_device_error(kErrWaitTimeout); });
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
+  int ok = 0;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, limit_ns) ? 1 : 0;
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  __syncwarp();
+  return ok != 0;
+}
+
+// fp32 accumulate, M = 128; b_rows: B is stored along N (V) instead of K.
+template <typename T>
+__device__ __forceinline__ uint32_t instr_desc(int n, bool b_rows) {
+  const uint32_t ab = T::kBf16 ? ((1u << 7) | (1u << 10)) : 0u;
+  return (1u << 4) | ab | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kM >> 4) << 24);
+}
+
+struct Item {
+  int h, q0;             // head, first query row in the sequence
+  int len_q, len_k;
+  int64_t row_q, row_k;  // the sequence's first rows
+  int steps[2];          // key steps of tile 0 and 1
+  bool live[2];          // whether the tile has rows
+};
+
+// Item x of the launch; false where the sequence has no such block.  A
+// sequence whose offsets do not describe rows of q and k, or that is longer
+// than the call said, counts as empty (error bit set).
+__device__ __forceinline__ bool get_item(const PromptArgs& a, int64_t x, Item& it) {
+  const int per = a.seqs * a.heads;
+  const int blk = static_cast<int>(x / per), r = static_cast<int>(x - (int64_t)blk * per);
+  const int b = r / a.heads;
+  it.h = r - b * a.heads;
+  it.q0 = (a.blocks - 1 - blk) * 2 * kM;
+  const int q_lo = a.cu_q[b], q_hi = a.cu_q[b + 1], k_lo = a.cu_k[b], k_hi = a.cu_k[b + 1];
+  it.len_q = q_hi - q_lo;
+  it.len_k = k_hi - k_lo;
+  it.row_q = q_lo;
+  it.row_k = k_lo;
+  if (q_lo < 0 || q_hi < q_lo || q_hi > a.rows_q || k_lo < 0 || k_hi < k_lo || k_hi > a.rows_k ||
+      it.len_q > a.max_q || it.len_k > a.max_k) {
+    if (threadIdx.x == 0) set_device_error(kErrPage);
+    return false;
+  }
+  if (it.q0 >= it.len_q) return false;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int first = it.q0 + t * kM;
+    it.live[t] = first < it.len_q;
+    int keys = it.len_k;
+    if (a.causal) keys = min(keys, min(first + kM, it.len_q) + it.len_k - it.len_q);
+    it.steps[t] = it.live[t] && keys > 0 ? (keys + kN - 1) / kN : 0;
+  }
+  return true;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_prompt_attention(const PromptArgs a, const __grid_constant__ CUtensorMap map_q,
+                       const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v) {
+  using C = Cfg<HD>;
+  constexpr int NS = C::kStages;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t s_qfull, s_qempty, s_full[NS], s_empty[NS], s_sfull[2],
+      s_pready[2], s_ofull[2], s_tail, s_drain;
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (saddr(smem_raw) + 1023u) & ~1023u;
+  const uint32_t q_at = base, ring = base + 2 * C::kTile;
+
+  if (threadIdx.x == 0) {
+    mbar_init(saddr(&s_qfull), 1);
+    mbar_init(saddr(&s_qempty), 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(saddr(&s_full[i]), 1);
+      mbar_init(saddr(&s_empty[i]), 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(saddr(&s_sfull[t]), 1);
+      mbar_init(saddr(&s_pready[t]), 4);
+      mbar_init(saddr(&s_ofull[t]), 1);
+    }
+    mbar_init(saddr(&s_tail), 1);
+    mbar_init(saddr(&s_drain), 1);
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     saddr(&s_tmem)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_trigger();
+  pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const int64_t items = (int64_t)a.blocks * a.seqs * a.heads;
+  Item it;
+
+  if (warp < kSoftWarps) {
+    // ---------------- softmax: one thread per row of tile t ----------------
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + C::kS + t * kN + lane_base;
+    const uint32_t o_at = tmem + C::kO + t * HD + lane_base;
+    uint32_t n_s = 0, n_o = 0;  // phases of s_full and o_full
+    for (int64_t x = blockIdx.x; x < items; x += gridDim.x) {
+      if (__any_sync(0xffffffffu, s_abort)) break;  // the same decision in every lane
+      if (!get_item(a, x, it) || !it.live[t]) continue;
+      const int q = it.q0 + t * kM + row;
+      const int steps = it.steps[t];
+      // Keys this row sees.
+      const int seen = a.causal ? min(it.len_k, q + 1 + it.len_k - it.len_q) : it.len_k;
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < steps; ++j) {
+        if (!warp_wait(saddr(&s_sfull[t]), n_s++ & 1, a.wait_ns)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[kN];
+#pragma unroll
+        for (int c = 0; c < kN; c += 32) tmem_ld32(s_at + c, s + c);
+        tmem_wait_ld();
+        const int vis = seen - j * kN;
+        if (__any_sync(0xffffffffu, vis < kN)) {
+#pragma unroll
+          for (int c = 0; c < kN; ++c)
+            if (c >= vis) s[c] = 0xff800000u;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < kN; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+        if (__any_sync(0xffffffffu, top > m + (m == -INFINITY ? 0.f : kLazy))) {
+          const float nm = fmaxf(m, top);
+          const float f = m == nm ? 1.f : exp2_approx(m - nm);
+          m = nm;
+          l *= f;
+          if (j > 0) {
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_at + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st32(o_at + c, o);
+            }
+          }
+        }
+        const float ref = (m == -INFINITY ? 0.f : m) - prob_shift<T>();
+        float sum[4] = {};
+        uint32_t p[kN / 2];
+#pragma unroll
+        for (int c = 0; c < kN; c += 2) {
+          const float p0 = exp2_approx(fmaf(__uint_as_float(s[c]), a.scale_log2, -ref));
+          const float p1 = exp2_approx(fmaf(__uint_as_float(s[c + 1]), a.scale_log2, -ref));
+          sum[c & 2] += p0;
+          sum[(c & 2) + 1] += p1;
+          p[c / 2] = T::pack(p0, p1);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st32(s_at, p);
+        tmem_st32(s_at + 32, p + 32);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(saddr(&s_pready[t]));
+      }
+      if (ok && steps > 0) ok = warp_wait(saddr(&s_ofull[t]), n_o++ & 1, a.wait_ns);
+      if (!ok) {
+        s_abort = 1;
+        break;
+      }
+      tc_fence_after();
+      const float inv = l > 0.f || l != l ? __fdividef(1.f, l) : 0.f;
+      uint4* dst = reinterpret_cast<uint4*>(a.out + ((it.row_q + q) * a.heads + it.h) * HD);
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        if (steps > 0) {
+          tmem_ld32(o_at + c, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0;
+        }
+        if (q < it.len_q) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              w[k] = inv == 0.f ? 0u
+                                : T::pack(__uint_as_float(o[i + 2 * k]) * inv,
+                                          __uint_as_float(o[i + 2 * k + 1]) * inv);
+            dst[(c + i) / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  } else if (warp == kTmaWarp) {
+    // ---------------- TMA producer ----------------
+    uint32_t g = 0, n_q = 0, n_tail = 0;
+    bool ok = true;
+    for (int64_t x = blockIdx.x; x < items && ok; x += gridDim.x) {
+      if (__any_sync(0xffffffffu, s_abort)) break;
+      if (!get_item(a, x, it)) continue;
+      const int steps = max(it.steps[0], it.steps[1]);
+      if (steps == 0) continue;
+      if (!warp_wait(saddr(&s_qempty), (n_q++ & 1) ^ 1, a.wait_ns)) {
+        s_abort = 1;
+        break;
+      }
+      if (lane == 0) {
+        const uint32_t bar = saddr(&s_qfull);
+        mbar_expect_tx(bar, ((it.steps[0] > 0) + (it.steps[1] > 0)) * C::kTile);
+        for (int t = 0; t < 2; ++t)
+          if (it.steps[t] > 0)
+            for (int hf = 0; hf < HD / 64; ++hf)
+              tma_load_3d(q_at + t * C::kTile + hf * C::kHalf, &map_q, bar, hf * 64, it.h,
+                          static_cast<int>(it.row_q) + it.q0 + t * kM);
+      }
+      const int kvh = it.h / a.group;
+      for (int i = 0; i < 2 * steps; ++i, ++g) {  // K(0), V(0), K(1), ...
+        const int s = g % NS, j = i >> 1;
+        ok = warp_wait(saddr(&s_empty[s]), ((g / NS) & 1) ^ 1, a.wait_ns);
+        if (!ok) break;
+        const uint32_t dst = ring + s * C::kTile, full = saddr(&s_full[s]);
+        // Rows past the sequence's last key belong to the next one: scores of
+        // such keys are dropped, but a probability of 0 does not silence an
+        // infinity or NaN among their values.  Those rows become zeros before
+        // the tile is handed on.
+        const int rows = it.len_k - j * kN;
+        const bool tail = (i & 1) && rows < kN;
+        if (lane == 0) {
+          const uint32_t bar = tail ? saddr(&s_tail) : full;
+          mbar_expect_tx(bar, C::kTile);
+          for (int hf = 0; hf < HD / 64; ++hf)
+            tma_load_3d(dst + hf * C::kHalf, (i & 1) ? &map_v : &map_k, bar, hf * 64, kvh,
+                        static_cast<int>(it.row_k) + j * kN);
+        }
+        if (tail) {
+          ok = warp_wait(saddr(&s_tail), n_tail++ & 1, a.wait_ns);
+          if (!ok) break;
+          for (int hf = 0; hf < HD / 64; ++hf)
+            for (uint32_t at = rows * 128 + lane * 16; at < C::kHalf; at += 512)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + hf * C::kHalf + at),
+                           "r"(0)
+                           : "memory");
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full);
+        }
+      }
+    }
+    if (!ok) s_abort = 1;
+    // Copies issued into stages never consumed (timeout): let them land.
+    if (s_abort && lane == 0) {
+      for (uint32_t j = g > (uint32_t)NS ? g - NS : 0; j < g; ++j)
+        mbar_wait(saddr(&s_full[j % NS]), (j / NS) & 1, a.wait_ns);
+      if (n_q > 0) mbar_wait(saddr(&s_qfull), (n_q - 1) & 1, a.wait_ns);
+    }
+  } else if (lane == 0) {
+    // ---------------- MMA issuer ----------------
+    const uint32_t d_qk = instr_desc<T>(kN, false), d_pv = instr_desc<T>(HD, true);
+    uint32_t g = 0, n_q = 0, n_p[2] = {0, 0};
+    bool issued = false, ok = true;
+    auto full = [&](uint32_t slot) {
+      ok = ok && mbar_wait(saddr(&s_full[slot % NS]), (slot / NS) & 1, a.wait_ns);
+      return ok;
+    };
+    auto product_qk = [&](int t, uint32_t slot) {
+      const uint32_t qa = q_at + t * C::kTile, ka = ring + (slot % NS) * C::kTile;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        const uint32_t off = kk / 4 * C::kHalf + kk % 4 * 32;
+        tc_mma(tmem + C::kS + t * kN, smem_desc(qa + off), smem_desc(ka + off), d_qk, kk != 0);
+      }
+      tc_commit(saddr(&s_sfull[t]));
+      issued = true;
+    };
+    for (int64_t x = blockIdx.x; x < items && !s_abort && ok; x += gridDim.x) {
+      if (!get_item(a, x, it)) continue;
+      const int steps = max(it.steps[0], it.steps[1]);
+      if (steps == 0) continue;
+      ok = mbar_wait(saddr(&s_qfull), n_q++ & 1, a.wait_ns);
+      if (!ok || !full(g)) break;
+      tc_fence_after();
+      for (int t = 0; t < 2; ++t)
+        if (it.steps[t] > 0) product_qk(t, g);
+      tc_commit(saddr(&s_empty[g % NS]));
+      if (steps == 1) tc_commit(saddr(&s_qempty));
+      for (int j = 0; j < steps && ok; ++j) {
+        const uint32_t v = g + 2 * j + 1, k = g + 2 * j + 2;
+        bool have_k = false;
+        if (!full(v)) break;
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (j >= it.steps[t]) continue;
+          ok = mbar_wait(saddr(&s_pready[t]), n_p[t]++ & 1, a.wait_ns);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t va = ring + (v % NS) * C::kTile;
+#pragma unroll
+          for (int kk = 0; kk < kN / 16; ++kk)
+            tc_mma_ta(tmem + C::kO + t * HD, tmem + C::kS + t * kN + kk * 8,
+                      smem_desc_mn(va + kk * 2048, C::kHalf), d_pv, j != 0 || kk != 0);
+          if (j + 1 == it.steps[t]) {
+            tc_commit(saddr(&s_ofull[t]));
+          } else {
+            if (!have_k && !full(k)) break;
+            have_k = true;
+            tc_fence_after();
+            product_qk(t, k);
+          }
+        }
+        if (!ok) break;
+        tc_commit(saddr(&s_empty[v % NS]));
+        if (j + 1 < steps) tc_commit(saddr(&s_empty[k % NS]));
+        if (j + 2 == steps) tc_commit(saddr(&s_qempty));
+      }
+      g += 2 * steps;
+    }
+    if (!ok) s_abort = 1;
+    // After a timeout, wait (bounded) for the MMAs already issued.
+    if (s_abort && issued) {
+      tc_commit(saddr(&s_drain));
+      mbar_wait(saddr(&s_drain), 0, a.wait_ns);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u)
+                 : "memory");
+  }
+}
+
+// [rows, heads, HD] with any row and head strides (multiples of 16 bytes):
+// boxes of 128 rows x 64 dims of one head, 128-byte swizzle.
+bool make_map(CUtensorMap* map, const uint16_t* x, int64_t rows, int heads, int hd, int64_t row_stride,
+              int64_t head_stride, bool bf16) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
+  const cuuint32_t box[3] = {64, 1, kM};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<uint16_t*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int HD>
+bool prompt_attr() {
+  return cudaFuncSetAttribute(k_prompt_attention<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              Cfg<HD>::kSmem) == cudaSuccess;
+}
+
+template <typename T, int HD>
+int launch_prompt(const PromptArgs& a, const CUtensorMap& q, const CUtensorMap& k,
+                  const CUtensorMap& v, cudaStream_t s) {
+  if (!once_per_device(reinterpret_cast<const void*>(&prompt_attr<T, HD>), &prompt_attr<T, HD>))
+    return MOE_ERR_CUDA;
+  const int64_t items = (int64_t)a.blocks * a.seqs * a.heads;
+  const int grid = static_cast<int>(items < sm_count() ? items : sm_count());
+  if (launch_pdl(k_prompt_attention<T, HD>, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, s, a, q, k,
+                 v) != cudaSuccess)
+    return MOE_ERR_CUDA;
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+
+bool bad_strides(int64_t row, int64_t head, int64_t heads, int64_t hd) {
+  return row < hd || (heads > 1 && head < hd);
+}
+
+}  // namespace
+}  // namespace moe
+
+extern "C" int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t q_head_stride,
+                                    int64_t q_rows, const uint16_t* k, int64_t k_stride,
+                                    int64_t k_head_stride, const uint16_t* v, int64_t v_stride,
+                                    int64_t v_head_stride, int64_t k_rows, const int32_t* cu_q,
+                                    const int32_t* cu_k, int seqs, int max_q, int max_k, int heads,
+                                    int kv_heads, int head_dim, int causal, int dtype, float scale,
+                                    uint16_t* out, void* stream) {
+  using namespace moe;
+  if (q_rows < 0 || k_rows < 0 || q_rows > INT32_MAX - 256 || k_rows > INT32_MAX - 256 || seqs < 0 ||
+      max_q < 0 || max_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || !(scale > 0.f))
+    return MOE_ERR_INVALID_ARG;
+  if (dtype != MOE_DTYPE_F16 && dtype != MOE_DTYPE_BF16) return MOE_ERR_UNSUPPORTED;
+  if (head_dim != 64 && head_dim != 128) return MOE_ERR_UNSUPPORTED;
+  if (bad_strides(q_stride, q_head_stride, heads, head_dim) ||
+      bad_strides(k_stride, k_head_stride, kv_heads, head_dim) ||
+      bad_strides(v_stride, v_head_stride, kv_heads, head_dim))
+    return MOE_ERR_INVALID_ARG;
+  if (q_rows == 0 || seqs == 0 || max_q == 0) return MOE_OK;
+  if ((int64_t)seqs * heads > INT32_MAX) return MOE_ERR_UNSUPPORTED;
+  if (!q || !cu_q || !cu_k || !out || (k_rows > 0 && (!k || !v))) return MOE_ERR_INVALID_ARG;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) ||
+      ((q_stride | q_head_stride | k_stride | k_head_stride | v_stride | v_head_stride) & 7))
+    return MOE_ERR_ALIGNMENT;
+  const bool bf16 = dtype == MOE_DTYPE_BF16;
+  CUtensorMap mq, mk, mv;
+  // Without any key no K or V tile is loaded: the maps then describe q.
+  const bool none = k_rows == 0;
+  if (!make_map(&mq, q, q_rows, heads, head_dim, q_stride, q_head_stride, bf16) ||
+      !make_map(&mk, none ? q : k, none ? q_rows : k_rows, none ? heads : kv_heads, head_dim,
+                none ? q_stride : k_stride, none ? q_head_stride : k_head_stride, bf16) ||
+      !make_map(&mv, none ? q : v, none ? q_rows : k_rows, none ? heads : kv_heads, head_dim,
+                none ? q_stride : v_stride, none ? q_head_stride : v_head_stride, bf16))
+    return MOE_ERR_CUDA;
+  PromptArgs a{};
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.rows_q = q_rows;
+  a.rows_k = k_rows;
+  a.seqs = seqs;
+  a.heads = heads;
+  a.group = heads / kv_heads;
+  a.max_q = max_q;
+  a.max_k = max_k;
+  a.blocks = static_cast<int>(ceil_div(max_q, 2 * kM));
+  a.causal = causal != 0;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = out;
+  a.wait_ns = wait_limit_ns();
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (bf16)
+    return head_dim == 64 ? launch_prompt<BF16, 64>(a, mq, mk, mv, s)
+                          : launch_prompt<BF16, 128>(a, mq, mk, mv, s);
+  return head_dim == 64 ? launch_prompt<F16, 64>(a, mq, mk, mv, s)
+                        : launch_prompt<F16, 128>(a, mq, mk, mv, s);
+}

@@ -767,3 +767,64 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         hd ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(), nbytes, stream),
         "moe_paged_attention")
     return out
+
+
+@_on_device
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     max_seqlen: int, cu_seqlens_k: torch.Tensor | None = None,
+                     max_seqlen_k: int | None = None, causal: bool = True,
+                     scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention over packed prompts of different lengths.
+
+    ``q`` [rows, heads, head_dim], ``k`` / ``v`` [rows_k, kv_heads, head_dim] (rows and heads may
+    be strided), fp16 or bf16, head_dim 64 or 128; sequence b's queries are rows
+    ``cu_seqlens[b] .. cu_seqlens[b+1]`` (int32, on the device), none longer than ``max_seqlen``;
+    its keys likewise by ``cu_seqlens_k`` / ``max_seqlen_k`` (default: the queries').  Causal: the
+    queries are the last of their sequence's positions; one that sees no key gives zeros.  Returns
+    [rows, heads, head_dim].
+    """
+    what = "prompt_attention"
+    if not isinstance(q, torch.Tensor) or q.ndim != 3:
+        raise ValueError(f"{what}: q must be [rows, heads, head_dim]")
+    dt, dev = q.dtype, q.device
+    if dt not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{what}: q must be float16 or bfloat16, got {dt}")
+    T, heads, hd = q.shape
+    if hd not in (64, 128):
+        raise ValueError(f"{what}: head_dim must be 64 or 128, got {hd}")
+    _serve_check(what, dev, ("q", q, dt, q.shape, 1), ("k", k, dt, (None, None, hd), 1))
+    _serve_check(what, dev, ("v", v, dt, k.shape, 1),
+                 ("cu_seqlens", cu_seqlens, torch.int32, (None,), 1))
+    kv, seqs = k.shape[1], cu_seqlens.shape[0] - 1
+    if seqs < 0 or kv == 0 or heads == 0 or heads % kv:
+        raise ValueError(f"{what}: {heads} query heads do not divide over {kv} KV heads, or "
+                         "cu_seqlens is empty")
+    if cu_seqlens_k is None:
+        cu_seqlens_k = cu_seqlens
+        if max_seqlen_k is None:
+            max_seqlen_k = max_seqlen
+    elif max_seqlen_k is None:
+        raise ValueError(f"{what}: cu_seqlens_k needs max_seqlen_k")
+    else:
+        _serve_check(what, dev, ("cu_seqlens_k", cu_seqlens_k, torch.int32, (seqs + 1,), 1))
+    if out is None:
+        out = torch.empty((T, heads, hd), dtype=dt, device=dev)
+    else:
+        _serve_check(what, dev, ("out", out, dt, (T, heads, hd), 3))
+    check(_native.lib().moe_prompt_attention(
+        q.data_ptr(), *_row_strides(q), T, k.data_ptr(), *_row_strides(k), v.data_ptr(),
+        *_row_strides(v), k.shape[0], cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), seqs,
+        max_seqlen, max_seqlen_k, heads, kv, hd, causal, _DTYPE_CODES[dt],
+        hd ** -0.5 if scale is None else scale, out.data_ptr(),
+        torch.cuda.current_stream(dev).cuda_stream), "moe_prompt_attention")
+    return out
+
+
+def _row_strides(t: torch.Tensor) -> tuple[int, int]:
+    """Strides of [rows, heads, hd] in elements (packed where a dimension has one entry)."""
+    row, head, _ = t.stride()
+    if t.shape[1] <= 1:
+        head = t.shape[2]
+    if t.shape[0] <= 1:
+        row = max(t.shape[1], 1) * head
+    return row, head

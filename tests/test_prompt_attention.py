@@ -1,0 +1,231 @@
+"""Attention over packed prompts against its formula in 64 bits.
+
+Tolerance: ``oracle.serving.attention_bound`` (derived from the formats' roundings).
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import serving as ref
+
+gpu = pytest.mark.gpu
+
+
+def _offsets(lens):
+    return torch.tensor([0] + lens).cumsum(0).int()
+
+
+def _inputs(lens, lens_k, H, KV, hd, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(sum(lens), H, hd, generator=g).to(dtype)
+    k, v = (torch.randn(sum(lens_k), KV, hd, generator=g).to(dtype) for _ in range(2))
+    return q, k, v
+
+
+def _run(q, k, v, lens, lens_k, causal=True, scale=None, **kw):
+    from moeinfra_b200 import kernels
+
+    same = lens is lens_k
+    return kernels.prompt_attention(
+        q.cuda(), k.cuda(), v.cuda(), _offsets(lens).cuda(), max(lens),
+        cu_seqlens_k=None if same else _offsets(lens_k).cuda(),
+        max_seqlen_k=None if same else max(lens_k), causal=causal, scale=scale, **kw)
+
+
+def _check(q, k, v, lens, lens_k=None, causal=True, scale=None):
+    from moeinfra_b200 import kernels
+
+    lens_k = lens if lens_k is None else lens_k
+    got = _run(q, k, v, lens, lens_k, causal, scale)
+    kernels.check_device()
+    a = c = 0
+    for n, m in zip(lens, lens_k):
+        want, weight, off = ref.attention(q[a:a + n], k[c:c + m], v[c:c + m],
+                                          q.shape[2] ** -0.5 if scale is None else scale, causal)
+        bound = ref.attention_bound(q.dtype, want, weight, off)
+        err = (got[a:a + n].double().cpu() - want).abs()
+        assert (err <= bound).all(), (n, m, float((err / bound).max()))
+        a, c = a + n, c + m
+    return got
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H,KV", [(4, 1), (2, 2), (6, 2), (7, 1)])
+def test_heads_and_types(dtype, hd, H, KV):
+    lens = [40, 1, 200, 129]
+    _check(*_inputs(lens, lens, H, KV, hd, dtype, seed=H), lens)
+
+
+@gpu
+@pytest.mark.parametrize("lens", [[1], [2], [127], [128], [129], [255], [256], [257], [385],
+                                  [1000], [0, 5, 0], [0], [300, 0, 0, 17, 256, 1, 128],
+                                  list(range(1, 60)), [513] * 9, [1700, 3]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_lengths(lens, causal):
+    """Tiles of 128 rows and keys, blocks of 256 rows: their edges, one and zero tokens."""
+    _check(*_inputs(lens, lens, 2, 1, 64, torch.float16, seed=len(lens)), lens, causal=causal)
+
+
+@gpu
+@pytest.mark.parametrize("lens,lens_k", [
+    ([1, 1, 1], [300, 1, 128]), ([40, 7], [296, 7]), ([256, 130], [700, 131]),
+    ([100, 20], [30, 0]), ([300], [1]), ([5, 400, 5], [0, 300, 260]), ([3], [0])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_keys_of_other_lengths(lens, lens_k, causal):
+    """Prompts that continue earlier keys, single tokens, and more queries than keys: rows that
+    see nothing are zeros."""
+    q, k, v = _inputs(lens, lens_k, 4, 2, 128, torch.bfloat16, seed=5)
+    got = _check(q, k, v, lens, lens_k, causal)
+    a = 0
+    for n, m in zip(lens, lens_k):
+        blind = n if m == 0 else max(0, n - m) if causal else 0
+        assert not got[a:a + blind].any()
+        a += n
+
+
+@gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_other_sequences_have_no_effect(bad):
+    """Infinities and NaN in the rows of the neighbours, which share tiles with a sequence's end."""
+    lens = [100, 40, 200, 130]
+    q, k, v = _inputs(lens, lens, 2, 1, 128, torch.float16, seed=1)
+    clean = _run(q, k, v, lens, lens)
+    for t in (q, k, v):
+        t[100:140] = bad
+    got = _run(q, k, v, lens, lens)
+    for lo, hi in ((0, 100), (140, 470)):
+        assert torch.equal(got[lo:hi], clean[lo:hi])
+
+
+@gpu
+def test_strides_and_streams():
+    """q, k and v as views of one projection; a call on another stream."""
+    from moeinfra_b200 import kernels
+
+    lens, H, KV, hd = [150, 33], 4, 2, 64
+    g = torch.Generator().manual_seed(3)
+    qkv = torch.randn(sum(lens), H + 2 * KV, hd, generator=g).half()
+    parts = [t.contiguous() for t in (qkv[:, :H], qkv[:, H:H + KV], qkv[:, H + KV:])]
+    want = _check(*parts, lens)
+    d, cu = qkv.cuda(), _offsets(lens).cuda()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = kernels.prompt_attention(d[:, :H], d[:, H:H + KV], d[:, H + KV:], cu, max(lens))
+    s.synchronize()
+    assert torch.equal(got, want)
+    # Every second head of a wider tensor.
+    wide = torch.randn(sum(lens), 2 * H, hd, generator=g).half()
+    want = _check(wide[:, ::2].contiguous(), *parts[1:], lens)
+    got = kernels.prompt_attention(wide.cuda()[:, ::2], d[:, H:H + KV], d[:, H + KV:], cu, max(lens))
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_growing_and_peaked_scores():
+    """Scores that rise along the keys (each step raises the maximum, by less and by more than
+    what is left standing), one key far above the rest, and all scores far below zero."""
+    n, hd = 700, 64
+    g = torch.Generator().manual_seed(0)
+    v = torch.randn(n, 1, hd, generator=g).half()
+    q = torch.zeros(n, 1, hd)
+    q[..., 0] = 1.0
+    ramps = [torch.linspace(0, 60, n), torch.linspace(0, 3, n), torch.linspace(60, 0, n),
+             torch.full((n,), -500.0), torch.where(torch.arange(n) == 300, 12.0, 0.0),
+             torch.where(torch.arange(n) % 128 == 0, 20.0, -3.0)]
+    for ramp in ramps:
+        k = torch.zeros(n, 1, hd)
+        k[:, 0, 0] = ramp
+        for causal in (True, False):
+            _check(q.half(), k.half(), v, [n], causal=causal, scale=1.0)
+            _check(q.bfloat16(), k.bfloat16(), v.bfloat16(), [n], causal=causal, scale=1.0)
+
+
+@gpu
+def test_a_captured_call_follows_its_offsets():
+    from moeinfra_b200 import kernels
+
+    q, k, v = (t.cuda() for t in _inputs([300], [300], 2, 1, 64, torch.float16))
+    cu = _offsets([300, 0, 0]).cuda()
+    kernels.prompt_attention(q, k, v, cu, 300)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = kernels.prompt_attention(q, k, v, cu, 300)
+    for lens in ([300, 0, 0], [1, 259, 40], [100, 100, 100]):
+        cu.copy_(_offsets(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, kernels.prompt_attention(q, k, v, cu, 300))
+
+
+@gpu
+def test_bad_offsets_are_reported():
+    """Offsets that fall, leave the rows or exceed the stated length: that sequence's rows are not
+    written, the others are right."""
+    from moeinfra_b200 import kernels
+
+    q, k, v = _inputs([200], [200], 2, 1, 64, torch.float16)
+    want = _run(q[:60], k[:60], v[:60], [60], [60])
+    for cu in ([0, 60, 20], [0, 60, 201], [0, 60, 1 << 30], [0, 60, 171], [0, 60, -4]):
+        out = torch.full((200, 2, 64), 7.0, dtype=torch.float16, device="cuda")
+        kernels.prompt_attention(q.cuda(), k.cuda(), v.cuda(), torch.tensor(cu).int().cuda(), 110,
+                                 out=out)
+        with pytest.raises(RuntimeError, match="out of range"):
+            kernels.check_device()
+        assert torch.equal(out[:60], want) and (out[60:] == 7).all()
+    kernels.check_device()
+
+
+def test_host_checks_precede_every_launch():
+    import ctypes
+
+    from moeinfra_b200 import _native
+
+    lib, f, odd = _native.lib(), ctypes.c_void_p(0x100000), ctypes.c_void_p(0x100008)
+
+    def attend(q=f, rows=10, seqs=2, H=4, KV=2, hd=128, dtype=0, scale=1.0, stride=None, out=f,
+               max_q=8, k=f, head=None):
+        return lib.moe_prompt_attention(q, H * hd if stride is None else stride,
+                                        hd if head is None else head, rows, k, KV * hd, hd, f,
+                                        KV * hd, hd, rows, f, f, seqs, max_q, 8, H, KV, hd, 1, dtype,
+                                        scale, out, None)
+
+    assert attend(rows=0) == 0 and attend(seqs=0) == 0 and attend(max_q=0) == 0
+    assert attend(rows=-1) == 1 and attend(H=5) == 1 and attend(q=None) == 1 and attend(k=None) == 1
+    assert attend(scale=0.0) == 1 and attend(scale=float("nan")) == 1 and attend(stride=8) == 1
+    assert attend(head=64) == 1 and attend(seqs=-1) == 1
+    assert attend(hd=96) == 2 and attend(dtype=2) == 2
+    assert attend(q=odd) == 5 and attend(out=odd) == 5 and attend(stride=516) == 5
+
+
+def test_wrapper_refuses_cpu_tensors():
+    from moeinfra_b200 import kernels
+
+    q = torch.zeros(4, 2, 64, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        kernels.prompt_attention(q, q, q, torch.tensor([0, 4]).int(), 4)
+
+
+@gpu
+def test_wrapper_refuses_wrong_shapes_and_types():
+    from moeinfra_b200 import kernels
+
+    q = torch.zeros(4, 4, 64, dtype=torch.float16, device="cuda")
+    kv = torch.zeros(4, 2, 64, dtype=torch.float16, device="cuda")
+    cu = torch.tensor([0, 4]).int().cuda()
+
+    def attend(q=q, k=kv, v=kv, cu=cu, **kw):
+        return kernels.prompt_attention(q, k, v, cu, 4, **kw)
+
+    attend()
+    for bad in (dict(q=q.float()), dict(q=q[..., :48]), dict(k=kv.bfloat16()), dict(v=kv[:3]),
+                dict(q=q[:, :3]), dict(cu=cu.long()), dict(cu=cu[:0]), dict(q=q[0]),
+                dict(out=q.bfloat16()), dict(cu_seqlens_k=cu), dict(k=kv.transpose(1, 2)),
+                dict(cu_seqlens_k=cu[:1], max_seqlen_k=4)):
+        with pytest.raises(ValueError):
+            attend(**bad)
+    with pytest.raises(RuntimeError):
+        attend(scale=0.0)
