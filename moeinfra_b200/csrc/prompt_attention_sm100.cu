@@ -42,7 +42,11 @@ MOE_DEFINE_ERROR_WORD()
 constexpr int kM = 128;         // rows of a tile
 constexpr int kN = 128;         // keys of a step
 constexpr int kSoftWarps = 8, kTmaWarp = 8, kMmaWarp = 9;
-constexpr int kThreads = 10 * 32;
+constexpr int kThreads = 12 * 32;  // three warpgroups: registers are moved between them
+// Registers a thread: 12 warps x 168 at launch, of which the softmax warps
+// (a row of 128 scores each) take kSoftRegs and the others keep kOtherRegs.
+constexpr int kSoftRegs = 208, kOtherRegs = 72;
+constexpr int kRegs = 2 * 128 * kSoftRegs + 128 * kOtherRegs;
 constexpr float kLazy = 8.f;    // log2 of what a row's maximum may grow before O is rescaled
 // P is rounded to 16 bits with m's reference up to 2^kLazy low: fp16 takes 2^7
 // on top (2^15 fits, normal down to 2^-21 of the reference); bf16 needs none.
@@ -89,12 +93,79 @@ __device__ __forceinline__ uint32_t instr_desc(int n, bool b_rows) {
          ((uint32_t)(kM >> 4) << 24);
 }
 
+// Two fp32 values in one 64-bit register pair: Blackwell's packed arithmetic
+// takes one issue slot for both.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
+  return pair(exp2_approx(lo_of(x)), exp2_approx(hi_of(x)));
+}
+// 2^x of a pair in ordinary arithmetic: x = n + f with n = round(x) (adding
+// 1.5 * 2^23 leaves n in the low bits of the sum) and |f| <= 1/2, 2^f by its
+// minimax polynomial, n added to the exponent.  Coefficients: Remez exchange
+// on the relative error over [-1/2, 1/2]; degree 3 is off by at most 7.5e-5 (a
+// bf16 probability rounds by 2e-3), degree 4 by 2.6e-6 (fp16: 4.9e-4).
+// Arguments below -120 give 2^-120 (a masked score too: a row that sees nothing
+// is told by its maximum).  NaN gives an infinite or NaN product with V.
+template <typename T>
+__device__ __forceinline__ uint64_t exp2_fma(uint64_t x) {
+  constexpr float kBig = 12582912.f;
+  x = pair(max_nan(lo_of(x), -120.f), max_nan(hi_of(x), -120.f));
+  const uint64_t r = add2(x, pair(kBig, kBig));
+  const uint64_t n = add2(r, pair(-kBig, -kBig));
+  const uint64_t f = fma2(n, pair(-1.f, -1.f), x);
+  uint64_t p;
+  if constexpr (T::kBf16) {
+    p = fma2(pair(0.0551716691f, 0.0551716691f), f, pair(0.242611122f, 0.242611122f));
+    p = fma2(p, f, pair(0.693260985f, 0.693260985f));
+    p = fma2(p, f, pair(0.999928074f, 0.999928074f));
+  } else {
+    p = fma2(pair(0.00957010201f, 0.00957010201f), f, pair(0.0559178603f, 0.0559178603f));
+    p = fma2(p, f, pair(0.240247448f, 0.240247448f));
+    p = fma2(p, f, pair(0.693121815f, 0.693121815f));
+    p = fma2(p, f, pair(0.999999261f, 0.999999261f));
+  }
+  const uint32_t lo = (uint32_t)p + ((uint32_t)r << 23);
+  const uint32_t hi = (uint32_t)(p >> 32) + ((uint32_t)(r >> 32) << 23);
+  return pair(__uint_as_float(lo), __uint_as_float(hi));
+}
+// Of 8 pairs, those that go through exp2_fma: see the kernel's comment.
+#ifndef FMA_OF_8
+#define FMA_OF_8 2
+#endif
+constexpr int kFmaOf8 = FMA_OF_8;
+
 struct Item {
   int h, q0;             // head, first query row in the sequence
   int len_q, len_k;
   int64_t row_q, row_k;  // the sequence's first rows
-  int steps[2];          // key steps of tile 0 and 1
-  bool live[2];          // whether the tile has rows
+  int steps0, steps1;    // key steps of tile 0 and 1
+  bool live0, live1;     // whether the tile has rows
 };
 
 // Item x of the launch; false where the sequence has no such block.  A
@@ -117,14 +188,15 @@ __device__ __forceinline__ bool get_item(const PromptArgs& a, int64_t x, Item& i
     return false;
   }
   if (it.q0 >= it.len_q) return false;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int first = it.q0 + t * kM;
-    it.live[t] = first < it.len_q;
+  it.live0 = true;
+  it.live1 = it.q0 + kM < it.len_q;
+  auto steps = [&](int first) {
     int keys = it.len_k;
     if (a.causal) keys = min(keys, min(first + kM, it.len_q) + it.len_k - it.len_q);
-    it.steps[t] = it.live[t] && keys > 0 ? (keys + kN - 1) / kN : 0;
-  }
+    return keys > 0 ? (keys + kN - 1) / kN : 0;
+  };
+  it.steps0 = steps(it.q0);
+  it.steps1 = it.live1 ? steps(it.q0 + kM) : 0;
   return true;
 }
 
@@ -137,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int NS = C::kStages;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t s_qfull, s_qempty, s_full[NS], s_empty[NS], s_sfull[2],
-      s_pready[2], s_ofull[2], s_tail, s_drain;
+      s_pready[2][2], s_ofull[2], s_tail, s_drain;
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -153,7 +225,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(saddr(&s_sfull[t]), 1);
-      mbar_init(saddr(&s_pready[t]), 4);
+      mbar_init(saddr(&s_pready[t][0]), 4);
+      mbar_init(saddr(&s_pready[t][1]), 4);
       mbar_init(saddr(&s_ofull[t]), 1);
     }
     mbar_init(saddr(&s_tail), 1);
@@ -178,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Item it;
 
   if (warp < kSoftWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     // ---------------- softmax: one thread per row of tile t ----------------
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -186,9 +260,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t n_s = 0, n_o = 0;  // phases of s_full and o_full
     for (int64_t x = blockIdx.x; x < items; x += gridDim.x) {
       if (__any_sync(0xffffffffu, s_abort)) break;  // the same decision in every lane
-      if (!get_item(a, x, it) || !it.live[t]) continue;
+      if (!get_item(a, x, it) || !(t ? it.live1 : it.live0)) continue;
       const int q = it.q0 + t * kM + row;
-      const int steps = it.steps[t];
+      const int steps = t ? it.steps1 : it.steps0;
       // Keys this row sees.
       const int seen = a.causal ? min(it.len_k, q + 1 + it.len_k - it.len_q) : it.len_k;
       float m = -INFINITY, l = 0.f;
@@ -211,7 +285,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < kN; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
+        for (int c = 0; c < kN; c += 2)
+          mx[c / 2 & 3] = max3(mx[c / 2 & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
         if (__any_sync(0xffffffffu, top > m + (m == -INFINITY ? 0.f : kLazy))) {
           const float nm = fmaxf(m, top);
@@ -231,23 +306,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         const float ref = (m == -INFINITY ? 0.f : m) - prob_shift<T>();
-        float sum[4] = {};
-        uint32_t p[kN / 2];
+        const uint64_t c2 = pair(a.scale_log2, a.scale_log2), r2 = pair(-ref, -ref);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int c = 0; c < kN; c += 2) {
-          const float p0 = exp2_approx(fmaf(__uint_as_float(s[c]), a.scale_log2, -ref));
-          const float p1 = exp2_approx(fmaf(__uint_as_float(s[c + 1]), a.scale_log2, -ref));
-          sum[c & 2] += p0;
-          sum[(c & 2) + 1] += p1;
-          p[c / 2] = T::pack(p0, p1);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t p[kN / 4];
+#pragma unroll
+          for (int c = 0; c < kN / 2; c += 2) {
+            const int k = half * (kN / 2) + c;
+            const uint64_t x = fma2(pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c2, r2);
+            const uint64_t e = c / 2 % 8 < kFmaOf8 ? exp2_fma<T>(x) : exp2_mufu(x);
+            sum[c / 2 & 1] = add2(sum[c / 2 & 1], e);
+            p[c / 2] = T::pack(lo_of(e), hi_of(e));
+          }
+          tmem_st32(s_at + half * (kN / 4), p);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(saddr(&s_pready[t][half]));
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st32(s_at, p);
-        tmem_st32(s_at + 32, p + 32);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(saddr(&s_pready[t]));
+        sum[0] = add2(sum[0], sum[1]);
+        l += lo_of(sum[0]) + hi_of(sum[0]);
       }
       if (ok && steps > 0) ok = warp_wait(saddr(&s_ofull[t]), n_o++ & 1, a.wait_ns);
       if (!ok) {
@@ -255,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       tc_fence_after();
-      const float inv = l > 0.f || l != l ? __fdividef(1.f, l) : 0.f;
+      const float inv = m == -INFINITY ? 0.f : __fdividef(1.f, l);
       uint4* dst = reinterpret_cast<uint4*>(a.out + ((it.row_q + q) * a.heads + it.h) * HD);
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
@@ -282,14 +361,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
     }
-  } else if (warp == kTmaWarp) {
+  } else {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  if (warp == kTmaWarp) {
     // ---------------- TMA producer ----------------
     uint32_t g = 0, n_q = 0, n_tail = 0;
     bool ok = true;
     for (int64_t x = blockIdx.x; x < items && ok; x += gridDim.x) {
       if (__any_sync(0xffffffffu, s_abort)) break;
       if (!get_item(a, x, it)) continue;
-      const int steps = max(it.steps[0], it.steps[1]);
+      const int steps = max(it.steps0, it.steps1);
       if (steps == 0) continue;
       if (!warp_wait(saddr(&s_qempty), (n_q++ & 1) ^ 1, a.wait_ns)) {
         s_abort = 1;
@@ -297,9 +378,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (lane == 0) {
         const uint32_t bar = saddr(&s_qfull);
-        mbar_expect_tx(bar, ((it.steps[0] > 0) + (it.steps[1] > 0)) * C::kTile);
+        mbar_expect_tx(bar, ((it.steps0 > 0) + (it.steps1 > 0)) * C::kTile);
+#pragma unroll
         for (int t = 0; t < 2; ++t)
-          if (it.steps[t] > 0)
+          if ((t ? it.steps1 : it.steps0) > 0)
             for (int hf = 0; hf < HD / 64; ++hf)
               tma_load_3d(q_at + t * C::kTile + hf * C::kHalf, &map_q, bar, hf * 64, it.h,
                           static_cast<int>(it.row_q) + it.q0 + t * kM);
@@ -344,72 +426,98 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(saddr(&s_full[j % NS]), (j / NS) & 1, a.wait_ns);
       if (n_q > 0) mbar_wait(saddr(&s_qfull), (n_q - 1) & 1, a.wait_ns);
     }
-  } else if (lane == 0) {
+  } else if (warp == kMmaWarp) {
     // ---------------- MMA issuer ----------------
+    // The whole warp walks the loop and one elected lane issues: addresses and
+    // descriptors are then uniform over the warp and stay in uniform registers
+    // (with one lane in the branch each instruction took ~150 cycles to issue).
     const uint32_t d_qk = instr_desc<T>(kN, false), d_pv = instr_desc<T>(HD, true);
-    uint32_t g = 0, n_q = 0, n_p[2] = {0, 0};
+    const uint32_t leader = elect_one();
+    const uint64_t desc_q = smem_desc(q_at), desc_k = smem_desc(ring);
+    const uint64_t desc_v = smem_desc_mn(ring, C::kHalf);
+    uint32_t slot = 0, turn = 0;  // of the ring: the next tile, and the parity of its barrier
+    uint32_t n_q = 0, n_p0 = 0, n_p1 = 0;
     bool issued = false, ok = true;
-    auto full = [&](uint32_t slot) {
-      ok = ok && mbar_wait(saddr(&s_full[slot % NS]), (slot / NS) & 1, a.wait_ns);
+    auto next = [&](uint32_t& at) {  // waits for the ring's next tile
+      at = slot;
+      ok = ok && mbar_wait(saddr(&s_full[slot]), turn, a.wait_ns);
+      if (++slot == NS) {
+        slot = 0;
+        turn ^= 1;
+      }
       return ok;
     };
-    auto product_qk = [&](int t, uint32_t slot) {
-      const uint32_t qa = q_at + t * C::kTile, ka = ring + (slot % NS) * C::kTile;
+    auto product_qk = [&](int t, uint32_t k) {
+      const uint64_t qd = desc_q + t * (C::kTile >> 4), kd = desc_k + k * (C::kTile >> 4);
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
-        const uint32_t off = kk / 4 * C::kHalf + kk % 4 * 32;
-        tc_mma(tmem + C::kS + t * kN, smem_desc(qa + off), smem_desc(ka + off), d_qk, kk != 0);
+        const uint32_t off = (kk / 4 * C::kHalf + kk % 4 * 32) >> 4;
+        tc_mma_if(leader, tmem + C::kS + t * kN, qd + off, kd + off, d_qk, kk != 0);
       }
-      tc_commit(saddr(&s_sfull[t]));
+      tc_commit_if(leader, saddr(&s_sfull[t]));
       issued = true;
     };
-    for (int64_t x = blockIdx.x; x < items && !s_abort && ok; x += gridDim.x) {
+    for (int64_t x = blockIdx.x; x < items && ok; x += gridDim.x) {
+      if (__any_sync(0xffffffffu, s_abort)) break;
       if (!get_item(a, x, it)) continue;
-      const int steps = max(it.steps[0], it.steps[1]);
+      const int steps0 = __shfl_sync(0xffffffffu, it.steps0, 0);
+      const int steps1 = __shfl_sync(0xffffffffu, it.steps1, 0);
+      const int steps = max(steps0, steps1);
       if (steps == 0) continue;
       ok = mbar_wait(saddr(&s_qfull), n_q++ & 1, a.wait_ns);
-      if (!ok || !full(g)) break;
+      uint32_t k, v;
+      if (!next(k)) break;
       tc_fence_after();
-      for (int t = 0; t < 2; ++t)
-        if (it.steps[t] > 0) product_qk(t, g);
-      tc_commit(saddr(&s_empty[g % NS]));
-      if (steps == 1) tc_commit(saddr(&s_qempty));
-      for (int j = 0; j < steps && ok; ++j) {
-        const uint32_t v = g + 2 * j + 1, k = g + 2 * j + 2;
-        bool have_k = false;
-        if (!full(v)) break;
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (j >= it.steps[t]) continue;
-          ok = mbar_wait(saddr(&s_pready[t]), n_p[t]++ & 1, a.wait_ns);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t va = ring + (v % NS) * C::kTile;
 #pragma unroll
-          for (int kk = 0; kk < kN / 16; ++kk)
-            tc_mma_ta(tmem + C::kO + t * HD, tmem + C::kS + t * kN + kk * 8,
-                      smem_desc_mn(va + kk * 2048, C::kHalf), d_pv, j != 0 || kk != 0);
-          if (j + 1 == it.steps[t]) {
-            tc_commit(saddr(&s_ofull[t]));
+      for (int t = 0; t < 2; ++t)
+        if ((t ? steps1 : steps0) > 0) product_qk(t, k);
+      tc_commit_if(leader, saddr(&s_empty[k]));
+      if (steps == 1) tc_commit_if(leader, saddr(&s_qempty));
+      for (int j = 0; j < steps; ++j) {
+        if (!next(v)) break;
+        const bool more = j + 1 < steps;
+        bool have_k = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int steps_t = t ? steps1 : steps0;
+          if (j >= steps_t || !ok) continue;
+          const uint64_t vd = desc_v + v * (C::kTile >> 4);
+          uint32_t& n_p = t ? n_p1 : n_p0;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            ok = ok && mbar_wait(saddr(&s_pready[t][half]), n_p & 1, a.wait_ns);
+            tc_fence_after();
+            if (ok) {
+#pragma unroll
+              for (int kk = half * (kN / 32); kk < (half + 1) * (kN / 32); ++kk)
+                tc_mma_ta_if(leader, tmem + C::kO + t * HD, tmem + C::kS + t * kN + kk * 8,
+                             vd + (kk * 2048 >> 4), d_pv, j != 0 || kk != 0);
+            }
+          }
+          ++n_p;
+          if (!ok) continue;
+          if (j + 1 == steps_t) {
+            tc_commit_if(leader, saddr(&s_ofull[t]));
           } else {
-            if (!have_k && !full(k)) break;
+            if (!have_k && !next(k)) continue;
             have_k = true;
             tc_fence_after();
             product_qk(t, k);
           }
         }
         if (!ok) break;
-        tc_commit(saddr(&s_empty[v % NS]));
-        if (j + 1 < steps) tc_commit(saddr(&s_empty[k % NS]));
-        if (j + 2 == steps) tc_commit(saddr(&s_qempty));
+        tc_commit_if(leader, saddr(&s_empty[v]));
+        if (more) tc_commit_if(leader, saddr(&s_empty[k]));
+        if (j + 2 == steps) tc_commit_if(leader, saddr(&s_qempty));
       }
-      g += 2 * steps;
     }
     if (!ok) s_abort = 1;
     // After a timeout, wait (bounded) for the MMAs already issued.
     if (s_abort && issued) {
-      tc_commit(saddr(&s_drain));
+      tc_commit_if(leader, saddr(&s_drain));
       mbar_wait(saddr(&s_drain), 0, a.wait_ns);
     }
+  }
   }
   tc_fence_before();
   __syncthreads();
@@ -438,7 +546,12 @@ bool make_map(CUtensorMap* map, const uint16_t* x, int64_t rows, int heads, int 
 
 template <typename T, int HD>
 bool prompt_attr() {
-  return cudaFuncSetAttribute(k_prompt_attention<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  // The warps' register shares must not exceed what the block is launched
+  // with: the last to ask would wait for good.
+  cudaFuncAttributes at;
+  return cudaFuncGetAttributes(&at, k_prompt_attention<T, HD>) == cudaSuccess &&
+         at.numRegs * kThreads >= kRegs &&
+         cudaFuncSetAttribute(k_prompt_attention<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               Cfg<HD>::kSmem) == cudaSuccess;
 }
 
