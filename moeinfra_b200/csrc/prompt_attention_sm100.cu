@@ -9,25 +9,32 @@
 //
 // One pass over the keys with the softmax's running maximum m and sum l.  A
 // persistent CTA per SM walks items of (256 query rows of one sequence, head),
-// the longest first.  An item is two tiles of 128 rows that take turns, so one
-// tile's softmax overlaps the other's products:
+// the longest first.  An item is two tiles of 128 rows, so that one tile's
+// softmax overlaps the other's products:
 //   warps 0-3, 4-7  softmax of tile 0 and 1, one thread per row:
 //                   S (tensor memory) -> registers, maximum, p = 2^(c s - c m),
-//                   P (16 bits) -> tensor memory over S; at the end O / l
+//                   P (16 bits) -> tensor memory; at the end O / l
 //   warp 8          lane 0 loads Q, K and V tiles with TMA (no multicast)
-//   warp 9          lane 0 issues tcgen05.mma: S = Q K^T (both from shared
-//                   memory), O += P V (P from tensor memory, V as stored)
-// Tensor memory: S of both tiles (2 x 128 columns), O of both (2 x HD).
-// MMAs of one thread execute in order, which orders everything but the
-// softmax: S(j) complete implies O(j-1) complete, so the softmax warps may
-// rescale O between S(j) and their P(j) without a further barrier.
+//   warps 9, 10     tcgen05.mma of tile 0 and 1: S = Q K^T (both from shared memory),
+//                   O += P V (P from tensor memory, V as stored)
+//   warp 11         idle (registers are shared out by warpgroups)
+//
+// What bounds a step: 64 cycles of tensor core per 128 x 128 x 16 product
+// (measured, both kinds), 16 exponentials a cycle, and the latency of the
+// chain S -> softmax -> P -> products (about 400 cycles from issue to a
+// waiting warp).  The chain is cut by giving P columns of its own: S is in
+// registers after the first ~150 cycles of a softmax, and the next Q K^T is
+// issued then, not after P V.  Tensor memory has 512 columns for two tiles'
+// S, P and O: with head_dim 128 a step takes 80 keys (2 x (80 + 40 + 128)),
+// with head_dim 64 128 keys (2 x (128 + 64 + 64)).
 //
 // O is rescaled only when a row's maximum grew by more than 2^8 since the
 // reference in use (m is then that reference): probabilities stay below 2^8,
 // O and l are sums of the same factor, and the quotient is exact either way.
 //
-// Barriers: q_full / q_empty, full / empty of the K and V ring, s_full (S of a
-// tile), p_ready (P stored, O rescaled), o_full (last product of a tile).
+// Barriers: q_full / q_empty, full / empty of the K and V ring, and per tile
+// s_full (S computed), s_free (S read), p_ready (P stored, O rescaled), pv_done
+// (P read, O updated).
 // Every wait is bounded, as in the grouped GEMM: on a timeout the error word
 // is set, the roles stop, and the CTA waits (bounded) for what it issued
 // before it frees its tensor memory.
@@ -40,12 +47,11 @@ namespace {
 MOE_DEFINE_ERROR_WORD()
 
 constexpr int kM = 128;         // rows of a tile
-constexpr int kN = 128;         // keys of a step
 constexpr int kSoftWarps = 8, kTmaWarp = 8, kMmaWarp = 9;
 constexpr int kThreads = 12 * 32;  // three warpgroups: registers are moved between them
 // Registers a thread: 12 warps x 168 at launch, of which the softmax warps
 // (a row of 128 scores each) take kSoftRegs and the others keep kOtherRegs.
-constexpr int kSoftRegs = 208, kOtherRegs = 72;
+constexpr int kSoftRegs = 200, kOtherRegs = 104;
 constexpr int kRegs = 2 * 128 * kSoftRegs + 128 * kOtherRegs;
 constexpr float kLazy = 8.f;    // log2 of what a row's maximum may grow before O is rescaled
 // P is rounded to 16 bits with m's reference up to 2^kLazy low: fp16 takes 2^7
@@ -55,11 +61,17 @@ constexpr float prob_shift() { return T::kBf16 ? 0.f : 7.f; }
 
 template <int HD>
 struct Cfg {
-  static constexpr uint32_t kHalf = kM * 128;                  // 64 dims of a tile: 16 KB
-  static constexpr uint32_t kTile = kHalf * (HD / 64);         // a Q, K or V tile
-  static constexpr int kStages = HD == 128 ? 5 : 10;           // K and V tiles in flight
-  static constexpr uint32_t kSmem = (2 + kStages) * kTile + 1024;
-  static constexpr uint32_t kS = 0, kO = 2 * kN;               // TMEM columns
+  static constexpr int kN = HD == 128 ? 80 : 128;              // keys of a step
+  // A tile's 64 dims: rows of 128 bytes, in swizzled groups of 8 (1024 bytes).
+  static constexpr uint32_t kHalfQ = kM * 128, kHalfK = kN * 128;
+  static constexpr uint32_t kTileQ = kHalfQ * (HD / 64), kTileK = kHalfK * (HD / 64);
+  static constexpr int kStages = HD == 128 ? 8 : 10;           // K and V tiles in flight
+  static constexpr uint32_t kSmem = 2 * kTileQ + kStages * kTileK + 1024;
+  // TMEM columns of tile 0, and how much further tile 1's are.
+  static constexpr uint32_t kS = 0, kS1 = kN, kP = 2 * kN, kP1 = (kN / 2 + 15) / 16 * 16;
+  static constexpr uint32_t kO = 512 - 2 * HD, kO1 = HD;
+  static_assert(kP + 2 * kP1 <= kO, "TMEM columns");
+  static_assert(kSmem + 1024 <= 227 * 1024, "shared memory");
 };
 
 struct PromptArgs {
@@ -77,12 +89,9 @@ struct PromptArgs {
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
   return mbar_wait_or(bar, parity, limit_ns, [] { set_device_error(kErrWaitTimeout); });
 }
+// A whole warp's wait, with one result for all lanes.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
-  int ok = 0;
-  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, limit_ns) ? 1 : 0;
-  ok = __shfl_sync(0xffffffffu, ok, 0);
-  __syncwarp();
-  return ok != 0;
+  return mbar_poll_or(bar, parity, limit_ns, [] { set_device_error(kErrWaitTimeout); });
 }
 
 // fp32 accumulate, M = 128; b_rows: B is stored along N (V) instead of K.
@@ -160,6 +169,20 @@ __device__ __forceinline__ uint64_t exp2_fma(uint64_t x) {
 #endif
 constexpr int kFmaOf8 = FMA_OF_8;
 
+// kN consecutive columns of the thread's own lane.
+template <int N>
+__device__ __forceinline__ void load_cols(uint32_t at, uint32_t* v) {
+#pragma unroll
+  for (int c = 0; c < N / 32 * 32; c += 32) tmem_ld32(at + c, v + c);
+  if constexpr (N % 32 == 16) tmem_ld16(at + N / 32 * 32, v + N / 32 * 32);
+}
+template <int N>
+__device__ __forceinline__ void store_cols(uint32_t at, const uint32_t* v) {
+#pragma unroll
+  for (int c = 0; c < N / 32 * 32; c += 32) tmem_st32(at + c, v + c);
+  if constexpr (N % 32 == 8) tmem_st8(at + N / 32 * 32, v + N / 32 * 32);
+}
+
 struct Item {
   int h, q0;             // head, first query row in the sequence
   int len_q, len_k;
@@ -171,6 +194,7 @@ struct Item {
 // Item x of the launch; false where the sequence has no such block.  A
 // sequence whose offsets do not describe rows of q and k, or that is longer
 // than the call said, counts as empty (error bit set).
+template <int HD>
 __device__ __forceinline__ bool get_item(const PromptArgs& a, int64_t x, Item& it) {
   const int per = a.seqs * a.heads;
   const int blk = static_cast<int>(x / per), r = static_cast<int>(x - (int64_t)blk * per);
@@ -190,6 +214,7 @@ __device__ __forceinline__ bool get_item(const PromptArgs& a, int64_t x, Item& i
   if (it.q0 >= it.len_q) return false;
   it.live0 = true;
   it.live1 = it.q0 + kM < it.len_q;
+  constexpr int kN = Cfg<HD>::kN;
   auto steps = [&](int first) {
     int keys = it.len_k;
     if (a.causal) keys = min(keys, min(first + kM, it.len_q) + it.len_k - it.len_q);
@@ -206,31 +231,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                        const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v) {
   using C = Cfg<HD>;
-  constexpr int NS = C::kStages;
+  constexpr int NS = C::kStages, kN = C::kN;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t s_qfull, s_qempty, s_full[NS], s_empty[NS], s_sfull[2],
-      s_pready[2][2], s_ofull[2], s_tail, s_drain;
+      s_sfree[2], s_pready[2], s_pvdone[2], s_tail, s_drain[2];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (saddr(smem_raw) + 1023u) & ~1023u;
-  const uint32_t q_at = base, ring = base + 2 * C::kTile;
+  const uint32_t q_at = base, ring = base + 2 * C::kTileQ;
 
   if (threadIdx.x == 0) {
     mbar_init(saddr(&s_qfull), 1);
-    mbar_init(saddr(&s_qempty), 1);
+    mbar_init(saddr(&s_qempty), 2);
     for (int i = 0; i < NS; ++i) {
       mbar_init(saddr(&s_full[i]), 1);
-      mbar_init(saddr(&s_empty[i]), 1);
+      mbar_init(saddr(&s_empty[i]), 2);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(saddr(&s_sfull[t]), 1);
-      mbar_init(saddr(&s_pready[t][0]), 4);
-      mbar_init(saddr(&s_pready[t][1]), 4);
-      mbar_init(saddr(&s_ofull[t]), 1);
+      mbar_init(saddr(&s_sfree[t]), 4);
+      mbar_init(saddr(&s_pready[t]), 4);
+      mbar_init(saddr(&s_pvdone[t]), 1);
+      mbar_init(saddr(&s_drain[t]), 1);
     }
     mbar_init(saddr(&s_tail), 1);
-    mbar_init(saddr(&s_drain), 1);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -255,12 +280,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- softmax: one thread per row of tile t ----------------
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + C::kS + t * kN + lane_base;
-    const uint32_t o_at = tmem + C::kO + t * HD + lane_base;
-    uint32_t n_s = 0, n_o = 0;  // phases of s_full and o_full
+    const uint32_t s_at = tmem + C::kS + t * C::kS1 + lane_base;
+    const uint32_t p_at = tmem + C::kP + t * C::kP1 + lane_base;
+    const uint32_t o_at = tmem + C::kO + t * C::kO1 + lane_base;
+    uint32_t n_s = 0, n_pv = 0;  // phases of s_full and pv_done
     for (int64_t x = blockIdx.x; x < items; x += gridDim.x) {
       if (__any_sync(0xffffffffu, s_abort)) break;  // the same decision in every lane
-      if (!get_item(a, x, it) || !(t ? it.live1 : it.live0)) continue;
+      if (!get_item<HD>(a, x, it) || !(t ? it.live1 : it.live0)) continue;
       const int q = it.q0 + t * kM + row;
       const int steps = t ? it.steps1 : it.steps0;
       // Keys this row sees.
@@ -274,9 +300,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         uint32_t s[kN];
-#pragma unroll
-        for (int c = 0; c < kN; c += 32) tmem_ld32(s_at + c, s + c);
+        load_cols<kN>(s_at, s);
         tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(saddr(&s_sfree[t]));
         const int vis = seen - j * kN;
         if (__any_sync(0xffffffffu, vis < kN)) {
 #pragma unroll
@@ -288,6 +316,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < kN; c += 2)
           mx[c / 2 & 3] = max3(mx[c / 2 & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+        // P's columns and O are free once the previous product is done.
+        if (j > 0) {
+          if (!warp_wait(saddr(&s_pvdone[t]), n_pv++ & 1, a.wait_ns)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
         if (__any_sync(0xffffffffu, top > m + (m == -INFINITY ? 0.f : kLazy))) {
           const float nm = fmaxf(m, top);
           const float f = m == nm ? 1.f : exp2_approx(m - nm);
@@ -308,27 +344,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float ref = (m == -INFINITY ? 0.f : m) - prob_shift<T>();
         const uint64_t c2 = pair(a.scale_log2, a.scale_log2), r2 = pair(-ref, -ref);
         uint64_t sum[2] = {0, 0};
+        uint32_t p[kN / 2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t p[kN / 4];
-#pragma unroll
-          for (int c = 0; c < kN / 2; c += 2) {
-            const int k = half * (kN / 2) + c;
-            const uint64_t x = fma2(pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c2, r2);
-            const uint64_t e = c / 2 % 8 < kFmaOf8 ? exp2_fma<T>(x) : exp2_mufu(x);
-            sum[c / 2 & 1] = add2(sum[c / 2 & 1], e);
-            p[c / 2] = T::pack(lo_of(e), hi_of(e));
-          }
-          tmem_st32(s_at + half * (kN / 4), p);
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(saddr(&s_pready[t][half]));
+        for (int c = 0; c < kN; c += 2) {
+          const uint64_t x = fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2, r2);
+          const uint64_t e = c / 2 % 8 < kFmaOf8 ? exp2_fma<T>(x) : exp2_mufu(x);
+          sum[c / 2 & 1] = add2(sum[c / 2 & 1], e);
+          p[c / 2] = T::pack(lo_of(e), hi_of(e));
         }
+        store_cols<kN / 2>(p_at, p);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(saddr(&s_pready[t]));
         sum[0] = add2(sum[0], sum[1]);
         l += lo_of(sum[0]) + hi_of(sum[0]);
       }
-      if (ok && steps > 0) ok = warp_wait(saddr(&s_ofull[t]), n_o++ & 1, a.wait_ns);
+      if (ok && steps > 0) ok = warp_wait(saddr(&s_pvdone[t]), n_pv++ & 1, a.wait_ns);
       if (!ok) {
         s_abort = 1;
         break;
@@ -365,11 +397,45 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == kTmaWarp) {
     // ---------------- TMA producer ----------------
+    // K(j + 1) goes before V(j), over the items' borders too: the order of use.
     uint32_t g = 0, n_q = 0, n_tail = 0;
     bool ok = true;
+    Item last;
+    int held = -1;  // step of `last` whose V is still to be loaded
+    auto load = [&](bool is_v, const Item& at, int j) {
+      const int s = g % NS;
+      ok = ok && warp_wait(saddr(&s_empty[s]), ((g / NS) & 1) ^ 1, a.wait_ns);
+      if (!ok) return;
+      ++g;
+      const uint32_t dst = ring + s * C::kTileK, full = saddr(&s_full[s]);
+      // Rows past the sequence's last key belong to the next one: scores of
+      // such keys are dropped, but a probability of 0 does not silence an
+      // infinity or NaN among their values.  Those rows become zeros before
+      // the tile is handed on.
+      const int rows = at.len_k - j * kN;
+      const bool tail = is_v && rows < kN;
+      if (lane == 0) {
+        const uint32_t bar = tail ? saddr(&s_tail) : full;
+        mbar_expect_tx(bar, C::kTileK);
+        for (int hf = 0; hf < HD / 64; ++hf)
+          tma_load_3d(dst + hf * C::kHalfK, is_v ? &map_v : &map_k, bar, hf * 64, at.h / a.group,
+                      static_cast<int>(at.row_k) + j * kN);
+      }
+      if (!tail) return;
+      ok = warp_wait(saddr(&s_tail), n_tail++ & 1, a.wait_ns);
+      if (!ok) return;
+      for (int hf = 0; hf < HD / 64; ++hf)
+        for (uint32_t z = rows * 128 + lane * 16; z < C::kHalfK; z += 512)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + hf * C::kHalfK + z),
+                       "r"(0)
+                       : "memory");
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full);
+    };
     for (int64_t x = blockIdx.x; x < items && ok; x += gridDim.x) {
       if (__any_sync(0xffffffffu, s_abort)) break;
-      if (!get_item(a, x, it)) continue;
+      if (!get_item<HD>(a, x, it)) continue;
       const int steps = max(it.steps0, it.steps1);
       if (steps == 0) continue;
       if (!warp_wait(saddr(&s_qempty), (n_q++ & 1) ^ 1, a.wait_ns)) {
@@ -378,47 +444,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (lane == 0) {
         const uint32_t bar = saddr(&s_qfull);
-        mbar_expect_tx(bar, ((it.steps0 > 0) + (it.steps1 > 0)) * C::kTile);
+        mbar_expect_tx(bar, ((it.steps0 > 0) + (it.steps1 > 0)) * C::kTileQ);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
           if ((t ? it.steps1 : it.steps0) > 0)
             for (int hf = 0; hf < HD / 64; ++hf)
-              tma_load_3d(q_at + t * C::kTile + hf * C::kHalf, &map_q, bar, hf * 64, it.h,
+              tma_load_3d(q_at + t * C::kTileQ + hf * C::kHalfQ, &map_q, bar, hf * 64, it.h,
                           static_cast<int>(it.row_q) + it.q0 + t * kM);
       }
-      const int kvh = it.h / a.group;
-      for (int i = 0; i < 2 * steps; ++i, ++g) {  // K(0), V(0), K(1), ...
-        const int s = g % NS, j = i >> 1;
-        ok = warp_wait(saddr(&s_empty[s]), ((g / NS) & 1) ^ 1, a.wait_ns);
-        if (!ok) break;
-        const uint32_t dst = ring + s * C::kTile, full = saddr(&s_full[s]);
-        // Rows past the sequence's last key belong to the next one: scores of
-        // such keys are dropped, but a probability of 0 does not silence an
-        // infinity or NaN among their values.  Those rows become zeros before
-        // the tile is handed on.
-        const int rows = it.len_k - j * kN;
-        const bool tail = (i & 1) && rows < kN;
-        if (lane == 0) {
-          const uint32_t bar = tail ? saddr(&s_tail) : full;
-          mbar_expect_tx(bar, C::kTile);
-          for (int hf = 0; hf < HD / 64; ++hf)
-            tma_load_3d(dst + hf * C::kHalf, (i & 1) ? &map_v : &map_k, bar, hf * 64, kvh,
-                        static_cast<int>(it.row_k) + j * kN);
-        }
-        if (tail) {
-          ok = warp_wait(saddr(&s_tail), n_tail++ & 1, a.wait_ns);
-          if (!ok) break;
-          for (int hf = 0; hf < HD / 64; ++hf)
-            for (uint32_t at = rows * 128 + lane * 16; at < C::kHalf; at += 512)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + hf * C::kHalf + at),
-                           "r"(0)
-                           : "memory");
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full);
-        }
+      for (int j = 0; j < steps && ok; ++j) {
+        load(false, it, j);
+        if (held >= 0) load(true, last, held);
+        last = it;
+        held = j;
       }
     }
+    if (held >= 0) load(true, last, held);
     if (!ok) s_abort = 1;
     // Copies issued into stages never consumed (timeout): let them land.
     if (s_abort && lane == 0) {
@@ -426,96 +467,103 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(saddr(&s_full[j % NS]), (j / NS) & 1, a.wait_ns);
       if (n_q > 0) mbar_wait(saddr(&s_qfull), (n_q - 1) & 1, a.wait_ns);
     }
-  } else if (warp == kMmaWarp) {
-    // ---------------- MMA issuer ----------------
+  } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+    // ---------------- MMA issuers: one warp per tile ----------------
     // The whole warp walks the loop and one elected lane issues: addresses and
     // descriptors are then uniform over the warp and stay in uniform registers
     // (with one lane in the branch each instruction took ~150 cycles to issue).
+    // A warp of its own per tile: between two products there are ~100
+    // instructions of waits and bookkeeping, which share issue slots with the
+    // softmax warps, and one tile's waits do not hold up the other's products.
+    const int t = warp - kMmaWarp;
     const uint32_t d_qk = instr_desc<T>(kN, false), d_pv = instr_desc<T>(HD, true);
     const uint32_t leader = elect_one();
-    const uint64_t desc_q = smem_desc(q_at), desc_k = smem_desc(ring);
-    const uint64_t desc_v = smem_desc_mn(ring, C::kHalf);
+    const uint64_t desc_q = smem_desc(q_at + t * C::kTileQ), desc_k = smem_desc(ring);
+    const uint64_t desc_v = smem_desc_mn(ring, C::kHalfK);
+    const uint32_t s_col = tmem + C::kS + t * C::kS1, p_col = tmem + C::kP + t * C::kP1;
+    const uint32_t o_col = tmem + C::kO + t * C::kO1;
     uint32_t slot = 0, turn = 0;  // of the ring: the next tile, and the parity of its barrier
-    uint32_t n_q = 0, n_p0 = 0, n_p1 = 0;
-    bool issued = false, ok = true;
-    auto next = [&](uint32_t& at) {  // waits for the ring's next tile
-      at = slot;
-      ok = ok && mbar_wait(saddr(&s_full[slot]), turn, a.wait_ns);
+    uint32_t n_q = 0, n_qk = 0, n_pv = 0;
+    bool ok = true;
+    auto next = [&]() {  // waits for the ring's next tile and takes its slot
+      const uint32_t at = slot;
+      ok = ok && warp_wait(saddr(&s_full[slot]), turn, a.wait_ns);
       if (++slot == NS) {
         slot = 0;
         turn ^= 1;
       }
-      return ok;
+      return at;
     };
-    auto product_qk = [&](int t, uint32_t k) {
-      const uint64_t qd = desc_q + t * (C::kTile >> 4), kd = desc_k + k * (C::kTile >> 4);
-#pragma unroll
-      for (int kk = 0; kk < HD / 16; ++kk) {
-        const uint32_t off = (kk / 4 * C::kHalf + kk % 4 * 32) >> 4;
-        tc_mma_if(leader, tmem + C::kS + t * kN, qd + off, kd + off, d_qk, kk != 0);
-      }
-      tc_commit_if(leader, saddr(&s_sfull[t]));
-      issued = true;
-    };
-    for (int64_t x = blockIdx.x; x < items && ok; x += gridDim.x) {
-      if (__any_sync(0xffffffffu, s_abort)) break;
-      if (!get_item(a, x, it)) continue;
-      const int steps0 = __shfl_sync(0xffffffffu, it.steps0, 0);
-      const int steps1 = __shfl_sync(0xffffffffu, it.steps1, 0);
-      const int steps = max(steps0, steps1);
-      if (steps == 0) continue;
-      ok = mbar_wait(saddr(&s_qfull), n_q++ & 1, a.wait_ns);
-      uint32_t k, v;
-      if (!next(k)) break;
+    auto product_qk = [&](uint32_t k) {  // S, once the last one is read
+      if (n_qk > 0) ok = ok && warp_wait(saddr(&s_sfree[t]), (n_qk - 1) & 1, a.wait_ns);
+      if (!ok) return;
+      ++n_qk;
       tc_fence_after();
+      const uint64_t kd = desc_k + k * (C::kTileK >> 4);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if ((t ? steps1 : steps0) > 0) product_qk(t, k);
-      tc_commit_if(leader, saddr(&s_empty[k]));
-      if (steps == 1) tc_commit_if(leader, saddr(&s_qempty));
-      for (int j = 0; j < steps; ++j) {
-        if (!next(v)) break;
-        const bool more = j + 1 < steps;
-        bool have_k = false;
+      for (int kk = 0; kk < HD / 16; ++kk)
+        tc_mma_if(leader, s_col, desc_q + ((kk / 4 * C::kHalfQ + kk % 4 * 32) >> 4),
+                  kd + ((kk / 4 * C::kHalfK + kk % 4 * 32) >> 4), d_qk, kk != 0);
+      tc_commit_if(leader, saddr(&s_sfull[t]));
+    };
+    auto product_pv = [&](uint32_t v, bool first) {
+      ok = ok && warp_wait(saddr(&s_pready[t]), n_pv & 1, a.wait_ns);
+      if (!ok) return;
+      ++n_pv;
+      tc_fence_after();
+      const uint64_t vd = desc_v + v * (C::kTileK >> 4);
+      const uint32_t add = first ? 0 : 1;
+      tc_mma_ta_if(leader, o_col, p_col, vd, d_pv, add);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int steps_t = t ? steps1 : steps0;
-          if (j >= steps_t || !ok) continue;
-          const uint64_t vd = desc_v + v * (C::kTile >> 4);
-          uint32_t& n_p = t ? n_p1 : n_p0;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            ok = ok && mbar_wait(saddr(&s_pready[t][half]), n_p & 1, a.wait_ns);
-            tc_fence_after();
-            if (ok) {
-#pragma unroll
-              for (int kk = half * (kN / 32); kk < (half + 1) * (kN / 32); ++kk)
-                tc_mma_ta_if(leader, tmem + C::kO + t * HD, tmem + C::kS + t * kN + kk * 8,
-                             vd + (kk * 2048 >> 4), d_pv, j != 0 || kk != 0);
-            }
-          }
-          ++n_p;
-          if (!ok) continue;
-          if (j + 1 == steps_t) {
-            tc_commit_if(leader, saddr(&s_ofull[t]));
-          } else {
-            if (!have_k && !next(k)) continue;
-            have_k = true;
-            tc_fence_after();
-            product_qk(t, k);
-          }
-        }
-        if (!ok) break;
-        tc_commit_if(leader, saddr(&s_empty[v]));
-        if (more) tc_commit_if(leader, saddr(&s_empty[k]));
-        if (j + 2 == steps) tc_commit_if(leader, saddr(&s_qempty));
+      for (int kk = 1; kk < kN / 16; ++kk)
+        tc_mma_ta_if(leader, o_col, p_col + kk * 8, vd + (kk * 2048 >> 4), d_pv, 1);
+      tc_commit_if(leader, saddr(&s_pvdone[t]));
+    };
+    // Steps of all items as one sequence, Q K^T of the next step before P V of
+    // this one, over the items' borders too.  A slot is released by both warps,
+    // after the last product that reads it or at once.
+    struct Step {
+      int j, mine, both;  // step of the item; the tile's steps and the item's
+    };
+    int64_t x = (int64_t)blockIdx.x - gridDim.x;
+    auto advance = [&](Step& s) {  // the sequence's next step; false at its end
+      if (++s.j < s.both) return true;
+      for (;;) {
+        x += gridDim.x;
+        if (x >= items || __any_sync(0xffffffffu, s_abort)) return false;
+        if (!get_item<HD>(a, x, it)) continue;
+        s.mine = __shfl_sync(0xffffffffu, t ? it.steps1 : it.steps0, 0);
+        s.both = __shfl_sync(0xffffffffu, max(it.steps0, it.steps1), 0);
+        s.j = 0;
+        if (s.both > 0) return true;
       }
+    };
+    auto start = [&](const Step& s) {  // Q K^T of a step
+      if (s.j == 0) ok = ok && warp_wait(saddr(&s_qfull), n_q++ & 1, a.wait_ns);
+      const uint32_t k = next();
+      if (ok && s.j < s.mine) product_qk(k);
+      if (!ok) return;
+      tc_commit_if(leader, saddr(&s_empty[k]));
+      if (s.j + 1 == s.both) tc_commit_if(leader, saddr(&s_qempty));
+    };
+    Step now{0, 0, 0};
+    bool have = advance(now);
+    if (have) start(now);
+    while (have && ok) {
+      Step after = now;
+      have = advance(after);
+      if (have) start(after);
+      const uint32_t v = next();
+      if (ok && now.j < now.mine) product_pv(v, now.j == 0);
+      if (!ok) break;
+      tc_commit_if(leader, saddr(&s_empty[v]));
+      now = after;
     }
     if (!ok) s_abort = 1;
     // After a timeout, wait (bounded) for the MMAs already issued.
-    if (s_abort && issued) {
-      tc_commit_if(leader, saddr(&s_drain));
-      mbar_wait(saddr(&s_drain), 0, a.wait_ns);
+    if (__any_sync(0xffffffffu, s_abort)) {
+      tc_commit_if(leader, saddr(&s_drain[t]));
+      warp_wait(saddr(&s_drain[t]), 0, a.wait_ns);
     }
   }
   }
@@ -529,14 +577,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // [rows, heads, HD] with any row and head strides (multiples of 16 bytes):
-// boxes of 128 rows x 64 dims of one head, 128-byte swizzle.
+// boxes of box_rows rows x 64 dims of one head, 128-byte swizzle.
 bool make_map(CUtensorMap* map, const uint16_t* x, int64_t rows, int heads, int hd, int64_t row_stride,
-              int64_t head_stride, bool bf16) {
+              int64_t head_stride, bool bf16, int box_rows) {
   auto fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
   const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
-  const cuuint32_t box[3] = {64, 1, kM};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows};
   const cuuint32_t estr[3] = {1, 1, 1};
   return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
             const_cast<uint16_t*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -603,11 +651,12 @@ extern "C" int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t
   CUtensorMap mq, mk, mv;
   // Without any key no K or V tile is loaded: the maps then describe q.
   const bool none = k_rows == 0;
-  if (!make_map(&mq, q, q_rows, heads, head_dim, q_stride, q_head_stride, bf16) ||
+  const int keys = head_dim == 64 ? Cfg<64>::kN : Cfg<128>::kN;
+  if (!make_map(&mq, q, q_rows, heads, head_dim, q_stride, q_head_stride, bf16, kM) ||
       !make_map(&mk, none ? q : k, none ? q_rows : k_rows, none ? heads : kv_heads, head_dim,
-                none ? q_stride : k_stride, none ? q_head_stride : k_head_stride, bf16) ||
+                none ? q_stride : k_stride, none ? q_head_stride : k_head_stride, bf16, keys) ||
       !make_map(&mv, none ? q : v, none ? q_rows : k_rows, none ? heads : kv_heads, head_dim,
-                none ? q_stride : v_stride, none ? q_head_stride : v_head_stride, bf16))
+                none ? q_stride : v_stride, none ? q_head_stride : v_head_stride, bf16, keys))
     return MOE_ERR_CUDA;
   PromptArgs a{};
   a.cu_q = cu_q;

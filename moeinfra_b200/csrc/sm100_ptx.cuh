@@ -43,6 +43,35 @@ __device__ __forceinline__ bool mbar_wait_or(uint32_t bar, uint32_t parity, uint
   }
   return true;
 }
+// One try without a time hint: 14 cycles where the phase is complete (the hint
+// makes it 70); the thread may still be suspended for a short while.
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// mbar_wait_or on such polls, by all lanes of a warp, with one result for the
+// warp: for waits that are nearly always over already or about to be.
+template <typename F>
+__device__ __forceinline__ bool mbar_poll_or(uint32_t bar, uint32_t parity, uint64_t limit_ns,
+                                             F timed_out) {
+  bool ok = mbar_poll(bar, parity);
+  if (!ok) {
+    const uint64_t t0 = globaltimer_ns();
+    for (int n = 0; !ok; ++n) {
+      ok = mbar_poll(bar, parity);
+      if (!ok && (n & 63) == 63 && globaltimer_ns() - t0 > limit_ns) break;
+    }
+  }
+  ok = __all_sync(0xffffffffu, ok);
+  if (!ok) timed_out();
+  return ok;
+}
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
