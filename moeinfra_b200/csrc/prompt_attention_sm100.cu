@@ -8,9 +8,13 @@
 // first rows without keys: zeros).
 //
 // One pass over the keys with the softmax's running maximum m and sum l.  A
-// persistent CTA per SM walks items of (256 query rows of one sequence, head),
-// the longest first.  An item is two tiles of 128 rows, so that one tile's
-// softmax overlaps the other's products:
+// persistent CTA per SM walks items of 256 rows, the longest first.  The rows
+// are the queries of neighbouring tokens of one sequence for P heads of one KV
+// head (P the largest power of two that divides the group, up to 16): with 4
+// heads 64 tokens, so that a short prompt or a sequence's end leaves few rows
+// empty and the causal edge cuts closer to it than 256 tokens would.  An item
+// is two tiles of 128 rows, so that one tile's softmax overlaps the other's
+// products:
 //   warps 0-3, 4-7  softmax of tile 0 and 1, one thread per row:
 //                   S (tensor memory) -> registers, maximum, p = 2^(c s - c m),
 //                   P (16 bits) -> tensor memory; at the end O / l
@@ -26,7 +30,7 @@
 // registers after the first ~150 cycles of a softmax, and the next Q K^T is
 // issued then, not after P V.  Tensor memory has 512 columns for two tiles'
 // S, P and O: with head_dim 128 a step takes 80 keys (2 x (80 + 40 + 128)),
-// with head_dim 64 128 keys (2 x (128 + 64 + 64)).
+// with head_dim 64 96 keys (the softmax's registers hold no more).
 //
 // O is rescaled only when a row's maximum grew by more than 2^8 since the
 // reference in use (m is then that reference): probabilities stay below 2^8,
@@ -61,12 +65,14 @@ constexpr float prob_shift() { return T::kBf16 ? 0.f : 7.f; }
 
 template <int HD>
 struct Cfg {
-  static constexpr int kN = HD == 128 ? 80 : 128;              // keys of a step
+  static constexpr int kN = HD == 128 ? 80 : 96;              // keys of a step
   // A tile's 64 dims: rows of 128 bytes, in swizzled groups of 8 (1024 bytes).
   static constexpr uint32_t kHalfQ = kM * 128, kHalfK = kN * 128;
   static constexpr uint32_t kTileQ = kHalfQ * (HD / 64), kTileK = kHalfK * (HD / 64);
-  static constexpr int kStages = HD == 128 ? 8 : 10;           // K and V tiles in flight
-  static constexpr uint32_t kSmem = 2 * kTileQ + kStages * kTileK + 1024;
+  static constexpr int kStages = HD == 128 ? 6 : 11;           // K and V tiles in flight
+  // On its way out a softmax warp's O passes 32 rows x 64 dims of shared memory.
+  static constexpr uint32_t kOut = 32 * 128;
+  static constexpr uint32_t kSmem = 2 * kTileQ + kStages * kTileK + kSoftWarps * kOut + 1024;
   // TMEM columns of tile 0, and how much further tile 1's are.
   static constexpr uint32_t kS = 0, kS1 = kN, kP = 2 * kN, kP1 = (kN / 2 + 15) / 16 * 16;
   static constexpr uint32_t kO = 512 - 2 * HD, kO1 = HD;
@@ -78,8 +84,9 @@ struct PromptArgs {
   const int32_t *cu_q, *cu_k;
   int64_t rows_q, rows_k;       // rows of q, and of k and v
   int seqs, heads, group;       // group: query heads per KV head
+  int pack;                     // log2 of the heads that share a tile
   int max_q, max_k;
-  int blocks;                   // ceil(max_q / 256)
+  int blocks;                   // ceil(max_q / tokens of an item)
   bool causal;
   float scale_log2;
   uint16_t* out;                // [rows_q, heads, HD]
@@ -181,10 +188,11 @@ __device__ __forceinline__ void store_cols(uint32_t at, const uint32_t* v) {
 #pragma unroll
   for (int c = 0; c < N / 32 * 32; c += 32) tmem_st32(at + c, v + c);
   if constexpr (N % 32 == 8) tmem_st8(at + N / 32 * 32, v + N / 32 * 32);
+  if constexpr (N % 32 == 16) tmem_st16(at + N / 32 * 32, v + N / 32 * 32);
 }
 
 struct Item {
-  int h, q0;             // head, first query row in the sequence
+  int h, q0;             // first head, first token in the sequence
   int len_q, len_k;
   int64_t row_q, row_k;  // the sequence's first rows
   int steps0, steps1;    // key steps of tile 0 and 1
@@ -196,11 +204,11 @@ struct Item {
 // than the call said, counts as empty (error bit set).
 template <int HD>
 __device__ __forceinline__ bool get_item(const PromptArgs& a, int64_t x, Item& it) {
-  const int per = a.seqs * a.heads;
+  const int groups = a.heads >> a.pack, per = a.seqs * groups;
   const int blk = static_cast<int>(x / per), r = static_cast<int>(x - (int64_t)blk * per);
-  const int b = r / a.heads;
-  it.h = r - b * a.heads;
-  it.q0 = (a.blocks - 1 - blk) * 2 * kM;
+  const int b = r / groups, tokens = kM >> a.pack;
+  it.h = (r - b * groups) << a.pack;
+  it.q0 = (a.blocks - 1 - blk) * 2 * tokens;
   const int q_lo = a.cu_q[b], q_hi = a.cu_q[b + 1], k_lo = a.cu_k[b], k_hi = a.cu_k[b + 1];
   it.len_q = q_hi - q_lo;
   it.len_k = k_hi - k_lo;
@@ -213,15 +221,15 @@ __device__ __forceinline__ bool get_item(const PromptArgs& a, int64_t x, Item& i
   }
   if (it.q0 >= it.len_q) return false;
   it.live0 = true;
-  it.live1 = it.q0 + kM < it.len_q;
+  it.live1 = it.q0 + tokens < it.len_q;
   constexpr int kN = Cfg<HD>::kN;
   auto steps = [&](int first) {
     int keys = it.len_k;
-    if (a.causal) keys = min(keys, min(first + kM, it.len_q) + it.len_k - it.len_q);
+    if (a.causal) keys = min(keys, min(first + tokens, it.len_q) + it.len_k - it.len_q);
     return keys > 0 ? (keys + kN - 1) / kN : 0;
   };
   it.steps0 = steps(it.q0);
-  it.steps1 = it.live1 ? steps(it.q0 + kM) : 0;
+  it.steps1 = it.live1 ? steps(it.q0 + tokens) : 0;
   return true;
 }
 
@@ -272,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const int64_t items = (int64_t)a.blocks * a.seqs * a.heads;
+  const int64_t items = (int64_t)a.blocks * a.seqs * (a.heads >> a.pack);
   Item it;
 
   if (warp < kSoftWarps) {
@@ -287,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int64_t x = blockIdx.x; x < items; x += gridDim.x) {
       if (__any_sync(0xffffffffu, s_abort)) break;  // the same decision in every lane
       if (!get_item<HD>(a, x, it) || !(t ? it.live1 : it.live0)) continue;
-      const int q = it.q0 + t * kM + row;
+      const int first = it.q0 + t * (kM >> a.pack), q = first + (row >> a.pack);  // the row's token
       const int steps = t ? it.steps1 : it.steps0;
       // Keys this row sees.
       const int seen = a.causal ? min(it.len_k, q + 1 + it.len_k - it.len_q) : it.len_k;
@@ -367,29 +375,49 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       const float inv = m == -INFINITY ? 0.f : __fdividef(1.f, l);
-      uint4* dst = reinterpret_cast<uint4*>(a.out + ((it.row_q + q) * a.heads + it.h) * HD);
+      // A thread holds a row; written out that way every 16 bytes would touch a
+      // line of its own.  64 dims at a time the warp's rows cross shared memory
+      // and leave as whole 128-byte lines.
+      const uint32_t stage = base + 2 * C::kTileQ + NS * C::kTileK + warp * C::kOut;
+      const int col8 = lane & 7, heads_mask = (1 << a.pack) - 1;
 #pragma unroll 1
-      for (int c = 0; c < HD; c += 32) {
-        uint32_t o[32];
-        if (steps > 0) {
-          tmem_ld32(o_at + c, o);
-          tmem_wait_ld();
-        } else {
+      for (int c = 0; c < HD; c += 64) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0;
-        }
-        if (q < it.len_q) {
+        for (int hf = 0; hf < 64; hf += 32) {
+          uint32_t o[32];
+          if (steps > 0) {
+            tmem_ld32(o_at + c + hf, o);
+            tmem_wait_ld();
+          }
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
+          for (int i = 0; i < 4; ++i) {
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               w[k] = inv == 0.f ? 0u
-                                : T::pack(__uint_as_float(o[i + 2 * k]) * inv,
-                                          __uint_as_float(o[i + 2 * k + 1]) * inv);
-            dst[(c + i) / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+                                : T::pack(__uint_as_float(o[8 * i + 2 * k]) * inv,
+                                          __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             stage + lane * 128 + (((hf / 8 + i) ^ (lane & 7)) << 4)),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
           }
         }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + (lane >> 3), tile_row = (warp & 3) * 32 + r;
+          const int token = first + (tile_row >> a.pack), head = it.h + (tile_row & heads_mask);
+          uint4 w;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                       : "r"(stage + r * 128 + ((col8 ^ (r & 7)) << 4))
+                       : "memory");
+          if (token < it.len_q)
+            *reinterpret_cast<uint4*>(a.out + ((it.row_q + token) * a.heads + head) * HD + c +
+                                      col8 * 8) = w;
+        }
+        __syncwarp();
       }
       tc_fence_before();
     }
@@ -450,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if ((t ? it.steps1 : it.steps0) > 0)
             for (int hf = 0; hf < HD / 64; ++hf)
               tma_load_3d(q_at + t * C::kTileQ + hf * C::kHalfQ, &map_q, bar, hf * 64, it.h,
-                          static_cast<int>(it.row_q) + it.q0 + t * kM);
+                          static_cast<int>(it.row_q) + it.q0 + t * (kM >> a.pack));
       }
       for (int j = 0; j < steps && ok; ++j) {
         load(false, it, j);
@@ -577,14 +605,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // [rows, heads, HD] with any row and head strides (multiples of 16 bytes):
-// boxes of box_rows rows x 64 dims of one head, 128-byte swizzle.
+// boxes of box_rows rows x box_heads heads x 64 dims, 128-byte swizzle.
 bool make_map(CUtensorMap* map, const uint16_t* x, int64_t rows, int heads, int hd, int64_t row_stride,
-              int64_t head_stride, bool bf16, int box_rows) {
+              int64_t head_stride, bool bf16, int box_rows, int box_heads) {
   auto fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
   const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
-  const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
   const cuuint32_t estr[3] = {1, 1, 1};
   return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
             const_cast<uint16_t*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -608,7 +636,7 @@ int launch_prompt(const PromptArgs& a, const CUtensorMap& q, const CUtensorMap& 
                   const CUtensorMap& v, cudaStream_t s) {
   if (!once_per_device(reinterpret_cast<const void*>(&prompt_attr<T, HD>), &prompt_attr<T, HD>))
     return MOE_ERR_CUDA;
-  const int64_t items = (int64_t)a.blocks * a.seqs * a.heads;
+  const int64_t items = (int64_t)a.blocks * a.seqs * (a.heads >> a.pack);
   const int grid = static_cast<int>(items < sm_count() ? items : sm_count());
   if (launch_pdl(k_prompt_attention<T, HD>, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, s, a, q, k,
                  v) != cudaSuccess)
@@ -651,12 +679,15 @@ extern "C" int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t
   CUtensorMap mq, mk, mv;
   // Without any key no K or V tile is loaded: the maps then describe q.
   const bool none = k_rows == 0;
+  int pack = 0;
+  while (pack < 4 && heads / kv_heads % (2 << pack) == 0) ++pack;
   const int keys = head_dim == 64 ? Cfg<64>::kN : Cfg<128>::kN;
-  if (!make_map(&mq, q, q_rows, heads, head_dim, q_stride, q_head_stride, bf16, kM) ||
+  if (!make_map(&mq, q, q_rows, heads, head_dim, q_stride, q_head_stride, bf16, kM >> pack,
+                1 << pack) ||
       !make_map(&mk, none ? q : k, none ? q_rows : k_rows, none ? heads : kv_heads, head_dim,
-                none ? q_stride : k_stride, none ? q_head_stride : k_head_stride, bf16, keys) ||
+                none ? q_stride : k_stride, none ? q_head_stride : k_head_stride, bf16, keys, 1) ||
       !make_map(&mv, none ? q : v, none ? q_rows : k_rows, none ? heads : kv_heads, head_dim,
-                none ? q_stride : v_stride, none ? q_head_stride : v_head_stride, bf16, keys))
+                none ? q_stride : v_stride, none ? q_head_stride : v_head_stride, bf16, keys, 1))
     return MOE_ERR_CUDA;
   PromptArgs a{};
   a.cu_q = cu_q;
@@ -668,7 +699,8 @@ extern "C" int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t
   a.group = heads / kv_heads;
   a.max_q = max_q;
   a.max_k = max_k;
-  a.blocks = static_cast<int>(ceil_div(max_q, 2 * kM));
+  a.pack = pack;
+  a.blocks = static_cast<int>(ceil_div(max_q, 2 * kM >> pack));
   a.causal = causal != 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = out;

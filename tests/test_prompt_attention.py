@@ -53,7 +53,7 @@ def _check(q, k, v, lens, lens_k=None, causal=True, scale=None):
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("hd", [64, 128])
-@pytest.mark.parametrize("H,KV", [(4, 1), (2, 2), (6, 2), (7, 1)])
+@pytest.mark.parametrize("H,KV", [(4, 1), (2, 2), (6, 2), (7, 1), (8, 1), (32, 2), (32, 1)])
 def test_heads_and_types(dtype, hd, H, KV):
     lens = [40, 1, 200, 129]
     _check(*_inputs(lens, lens, H, KV, hd, dtype, seed=H), lens)
