@@ -21,7 +21,7 @@
 //   warp 8          lane 0 loads Q, K and V tiles with TMA (no multicast)
 //   warps 9, 10     tcgen05.mma of tile 0 and 1: S = Q K^T (both from shared memory),
 //                   O += P V (P from tensor memory, V as stored)
-//   warp 11         idle (registers are shared out by warpgroups)
+//   warp 11         looks the items up, some ahead of their use
 //
 // What bounds a step: 64 cycles of tensor core per 128 x 128 x 16 product
 // (measured, both kinds), 16 exponentials a cycle, and the latency of the
@@ -191,24 +191,25 @@ __device__ __forceinline__ void store_cols(uint32_t at, const uint32_t* v) {
   if constexpr (N % 32 == 16) tmem_st16(at + N / 32 * 32, v + N / 32 * 32);
 }
 
-struct Item {
-  int h, q0;             // first head, first token in the sequence
+struct __align__(16) Item {
+  int h, q0;            // first head (-1: no more items), first token in the sequence
   int len_q, len_k;
-  int64_t row_q, row_k;  // the sequence's first rows
-  int steps0, steps1;    // key steps of tile 0 and 1
-  bool live0, live1;     // whether the tile has rows
+  int row_q, row_k;     // the sequence's first rows
+  int steps0, steps1;   // key steps of tile 0 and 1
 };
+constexpr int kItems = 4;                   // items looked up ahead
+constexpr int kReaders = kSoftWarps + 3;    // warps that read each of them
 
 // Item x of the launch; false where the sequence has no such block.  A
 // sequence whose offsets do not describe rows of q and k, or that is longer
 // than the call said, counts as empty (error bit set).
 template <int HD>
-__device__ __forceinline__ bool get_item(const PromptArgs& a, int64_t x, Item& it) {
-  const int groups = a.heads >> a.pack, per = a.seqs * groups;
-  const int blk = static_cast<int>(x / per), r = static_cast<int>(x - (int64_t)blk * per);
-  const int b = r / groups, tokens = kM >> a.pack;
+__device__ __forceinline__ bool get_item(const PromptArgs& a, uint32_t x, Item& it) {
+  const uint32_t groups = a.heads >> a.pack, per = a.seqs * groups;
+  const uint32_t blk = x / per, r = x - blk * per, b = r / groups;
+  const int tokens = kM >> a.pack;
   it.h = (r - b * groups) << a.pack;
-  it.q0 = (a.blocks - 1 - blk) * 2 * tokens;
+  it.q0 = (a.blocks - 1 - (int)blk) * 2 * tokens;
   const int q_lo = a.cu_q[b], q_hi = a.cu_q[b + 1], k_lo = a.cu_k[b], k_hi = a.cu_k[b + 1];
   it.len_q = q_hi - q_lo;
   it.len_k = k_hi - k_lo;
@@ -216,20 +217,18 @@ __device__ __forceinline__ bool get_item(const PromptArgs& a, int64_t x, Item& i
   it.row_k = k_lo;
   if (q_lo < 0 || q_hi < q_lo || q_hi > a.rows_q || k_lo < 0 || k_hi < k_lo || k_hi > a.rows_k ||
       it.len_q > a.max_q || it.len_k > a.max_k) {
-    if (threadIdx.x == 0) set_device_error(kErrPage);
+    set_device_error(kErrPage);
     return false;
   }
   if (it.q0 >= it.len_q) return false;
-  it.live0 = true;
-  it.live1 = it.q0 + tokens < it.len_q;
   constexpr int kN = Cfg<HD>::kN;
   auto steps = [&](int first) {
     int keys = it.len_k;
     if (a.causal) keys = min(keys, min(first + tokens, it.len_q) + it.len_k - it.len_q);
-    return keys > 0 ? (keys + kN - 1) / kN : 0;
+    return first < it.len_q && keys > 0 ? (keys + kN - 1) / kN : 0;
   };
   it.steps0 = steps(it.q0);
-  it.steps1 = it.live1 ? steps(it.q0 + tokens) : 0;
+  it.steps1 = steps(it.q0 + tokens);
   return true;
 }
 
@@ -237,12 +236,15 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     k_prompt_attention(const PromptArgs a, const __grid_constant__ CUtensorMap map_q,
                        const __grid_constant__ CUtensorMap map_k,
-                       const __grid_constant__ CUtensorMap map_v) {
+                       const __grid_constant__ CUtensorMap map_v,
+                       const __grid_constant__ CUtensorMap map_o) {
   using C = Cfg<HD>;
   constexpr int NS = C::kStages, kN = C::kN;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t s_qfull, s_qempty, s_full[NS], s_empty[NS], s_sfull[2],
-      s_sfree[2], s_pready[2], s_pvdone[2], s_tail, s_drain[2];
+      s_sfree[2], s_pready[2], s_pvdone[2], s_tail, s_drain[2],
+      s_itfull[kItems], s_itempty[kItems];
+  __shared__ Item s_item[kItems];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -264,6 +266,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(saddr(&s_drain[t]), 1);
     }
     mbar_init(saddr(&s_tail), 1);
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(saddr(&s_itfull[i]), 1);
+      mbar_init(saddr(&s_itempty[i]), kReaders);
+    }
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -280,8 +286,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const int64_t items = (int64_t)a.blocks * a.seqs * (a.heads >> a.pack);
+  // The items of this CTA in order, from the look-up warp; the same for every
+  // reading warp.  False at the end or after a timeout.
   Item it;
+  uint32_t n_it = 0;
+  auto next_item = [&]() {
+    const uint32_t i = n_it % kItems;
+    if (!warp_wait(saddr(&s_itfull[i]), n_it / kItems & 1, a.wait_ns)) {
+      s_abort = 1;
+      return false;
+    }
+    it = s_item[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(saddr(&s_itempty[i]));
+    ++n_it;
+    return it.h >= 0 && !__any_sync(0xffffffffu, s_abort);
+  };
 
   if (warp < kSoftWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
@@ -291,11 +311,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_at = tmem + C::kS + t * C::kS1 + lane_base;
     const uint32_t p_at = tmem + C::kP + t * C::kP1 + lane_base;
     const uint32_t o_at = tmem + C::kO + t * C::kO1 + lane_base;
+    const uint32_t stage = base + 2 * C::kTileQ + NS * C::kTileK + warp * C::kOut;
     uint32_t n_s = 0, n_pv = 0;  // phases of s_full and pv_done
-    for (int64_t x = blockIdx.x; x < items; x += gridDim.x) {
-      if (__any_sync(0xffffffffu, s_abort)) break;  // the same decision in every lane
-      if (!get_item<HD>(a, x, it) || !(t ? it.live1 : it.live0)) continue;
+    while (next_item()) {
       const int first = it.q0 + t * (kM >> a.pack), q = first + (row >> a.pack);  // the row's token
+      if (first >= it.len_q) continue;
       const int steps = t ? it.steps1 : it.steps0;
       // Keys this row sees.
       const int seen = a.causal ? min(it.len_k, q + 1 + it.len_k - it.len_q) : it.len_k;
@@ -376,12 +396,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const float inv = m == -INFINITY ? 0.f : __fdividef(1.f, l);
       // A thread holds a row; written out that way every 16 bytes would touch a
-      // line of its own.  64 dims at a time the warp's rows cross shared memory
-      // and leave as whole 128-byte lines.
-      const uint32_t stage = base + 2 * C::kTileQ + NS * C::kTileK + warp * C::kOut;
-      const int col8 = lane & 7, heads_mask = (1 << a.pack) - 1;
+      // line of its own.  64 dims at a time the warp's 32 rows cross shared
+      // memory (in the swizzle that the TMA store undoes); where the sequence
+      // ends among them the lanes write whole 128-byte lines themselves.
+      const int lane_row = (warp & 3) * 32, heads_mask = (1 << a.pack) - 1;
+      const int warp_token = first + (lane_row >> a.pack);
+      const bool whole = warp_token + (32 >> a.pack) <= it.len_q;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 64) {
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store read it
+        __syncwarp();
 #pragma unroll
         for (int hf = 0; hf < 64; hf += 32) {
           uint32_t o[32];
@@ -403,34 +427,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                          : "memory");
           }
         }
+        if (whole) {
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&map_o, stage, c, it.h + (lane_row & heads_mask), it.row_q + warp_token);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          continue;
+        }
         __syncwarp();
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 8; ++i) {
-          const int r = i * 4 + (lane >> 3), tile_row = (warp & 3) * 32 + r;
-          const int token = first + (tile_row >> a.pack), head = it.h + (tile_row & heads_mask);
+          const int r = i * 4 + (lane >> 3), col8 = lane & 7;
+          const int token = first + ((lane_row + r) >> a.pack), head = it.h + (r & heads_mask);
           uint4 w;
           asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                        : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                        : "r"(stage + r * 128 + ((col8 ^ (r & 7)) << 4))
                        : "memory");
           if (token < it.len_q)
-            *reinterpret_cast<uint4*>(a.out + ((it.row_q + token) * a.heads + head) * HD + c +
-                                      col8 * 8) = w;
+            *reinterpret_cast<uint4*>(a.out + ((int64_t)(it.row_q + token) * a.heads + head) * HD +
+                                      c + col8 * 8) = w;
         }
-        __syncwarp();
       }
       tc_fence_before();
     }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == kTmaWarp) {
     // ---------------- TMA producer ----------------
-    // K(j + 1) goes before V(j), over the items' borders too: the order of use.
+    // Q, K(0), then K(j + 1), V(j): the order of use.
     uint32_t g = 0, n_q = 0, n_tail = 0;
     bool ok = true;
-    Item last;
-    int held = -1;  // step of `last` whose V is still to be loaded
-    auto load = [&](bool is_v, const Item& at, int j) {
+    int kv_head = 0;
+    auto load = [&](bool is_v, int j) {
       const int s = g % NS;
       ok = ok && warp_wait(saddr(&s_empty[s]), ((g / NS) & 1) ^ 1, a.wait_ns);
       if (!ok) return;
@@ -440,14 +472,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // such keys are dropped, but a probability of 0 does not silence an
       // infinity or NaN among their values.  Those rows become zeros before
       // the tile is handed on.
-      const int rows = at.len_k - j * kN;
+      const int rows = it.len_k - j * kN;
       const bool tail = is_v && rows < kN;
       if (lane == 0) {
         const uint32_t bar = tail ? saddr(&s_tail) : full;
         mbar_expect_tx(bar, C::kTileK);
         for (int hf = 0; hf < HD / 64; ++hf)
-          tma_load_3d(dst + hf * C::kHalfK, is_v ? &map_v : &map_k, bar, hf * 64, at.h / a.group,
-                      static_cast<int>(at.row_k) + j * kN);
+          tma_load_3d(dst + hf * C::kHalfK, is_v ? &map_v : &map_k, bar, hf * 64, kv_head,
+                      it.row_k + j * kN);
       }
       if (!tail) return;
       ok = warp_wait(saddr(&s_tail), n_tail++ & 1, a.wait_ns);
@@ -461,15 +493,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(full);
     };
-    for (int64_t x = blockIdx.x; x < items && ok; x += gridDim.x) {
-      if (__any_sync(0xffffffffu, s_abort)) break;
-      if (!get_item<HD>(a, x, it)) continue;
+    while (ok && next_item()) {
       const int steps = max(it.steps0, it.steps1);
       if (steps == 0) continue;
-      if (!warp_wait(saddr(&s_qempty), (n_q++ & 1) ^ 1, a.wait_ns)) {
-        s_abort = 1;
-        break;
-      }
+      kv_head = it.h / a.group;
+      ok = warp_wait(saddr(&s_qempty), (n_q++ & 1) ^ 1, a.wait_ns);
+      if (!ok) break;
       if (lane == 0) {
         const uint32_t bar = saddr(&s_qfull);
         mbar_expect_tx(bar, ((it.steps0 > 0) + (it.steps1 > 0)) * C::kTileQ);
@@ -478,16 +507,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if ((t ? it.steps1 : it.steps0) > 0)
             for (int hf = 0; hf < HD / 64; ++hf)
               tma_load_3d(q_at + t * C::kTileQ + hf * C::kHalfQ, &map_q, bar, hf * 64, it.h,
-                          static_cast<int>(it.row_q) + it.q0 + t * (kM >> a.pack));
+                          it.row_q + it.q0 + t * (kM >> a.pack));
       }
-      for (int j = 0; j < steps && ok; ++j) {
-        load(false, it, j);
-        if (held >= 0) load(true, last, held);
-        last = it;
-        held = j;
+      load(false, 0);
+      for (int j = 0; j < steps; ++j) {
+        if (j + 1 < steps) load(false, j + 1);
+        load(true, j);
       }
     }
-    if (held >= 0) load(true, last, held);
     if (!ok) s_abort = 1;
     // Copies issued into stages never consumed (timeout): let them land.
     if (s_abort && lane == 0) {
@@ -547,45 +574,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_mma_ta_if(leader, o_col, p_col + kk * 8, vd + (kk * 2048 >> 4), d_pv, 1);
       tc_commit_if(leader, saddr(&s_pvdone[t]));
     };
-    // Steps of all items as one sequence, Q K^T of the next step before P V of
-    // this one, over the items' borders too.  A slot is released by both warps,
-    // after the last product that reads it or at once.
-    struct Step {
-      int j, mine, both;  // step of the item; the tile's steps and the item's
-    };
-    int64_t x = (int64_t)blockIdx.x - gridDim.x;
-    auto advance = [&](Step& s) {  // the sequence's next step; false at its end
-      if (++s.j < s.both) return true;
-      for (;;) {
-        x += gridDim.x;
-        if (x >= items || __any_sync(0xffffffffu, s_abort)) return false;
-        if (!get_item<HD>(a, x, it)) continue;
-        s.mine = __shfl_sync(0xffffffffu, t ? it.steps1 : it.steps0, 0);
-        s.both = __shfl_sync(0xffffffffu, max(it.steps0, it.steps1), 0);
-        s.j = 0;
-        if (s.both > 0) return true;
+    // A slot is released by both warps, after the last product that reads it.
+    while (ok && next_item()) {
+      const int mine = __shfl_sync(0xffffffffu, t ? it.steps1 : it.steps0, 0);
+      const int both = __shfl_sync(0xffffffffu, max(it.steps0, it.steps1), 0);
+      if (both == 0) continue;
+      ok = warp_wait(saddr(&s_qfull), n_q++ & 1, a.wait_ns);
+      for (int j = -1; j < both; ++j) {  // Q K^T of step j + 1, P V of step j
+        if (j + 1 < both) {
+          const uint32_t k = next();
+          if (ok && j + 1 < mine) product_qk(k);
+          if (!ok) break;
+          tc_commit_if(leader, saddr(&s_empty[k]));
+          if (j + 2 == both) tc_commit_if(leader, saddr(&s_qempty));
+        }
+        if (j < 0) continue;
+        const uint32_t v = next();
+        if (ok && j < mine) product_pv(v, j == 0);
+        if (!ok) break;
+        tc_commit_if(leader, saddr(&s_empty[v]));
       }
-    };
-    auto start = [&](const Step& s) {  // Q K^T of a step
-      if (s.j == 0) ok = ok && warp_wait(saddr(&s_qfull), n_q++ & 1, a.wait_ns);
-      const uint32_t k = next();
-      if (ok && s.j < s.mine) product_qk(k);
-      if (!ok) return;
-      tc_commit_if(leader, saddr(&s_empty[k]));
-      if (s.j + 1 == s.both) tc_commit_if(leader, saddr(&s_qempty));
-    };
-    Step now{0, 0, 0};
-    bool have = advance(now);
-    if (have) start(now);
-    while (have && ok) {
-      Step after = now;
-      have = advance(after);
-      if (have) start(after);
-      const uint32_t v = next();
-      if (ok && now.j < now.mine) product_pv(v, now.j == 0);
-      if (!ok) break;
-      tc_commit_if(leader, saddr(&s_empty[v]));
-      now = after;
     }
     if (!ok) s_abort = 1;
     // After a timeout, wait (bounded) for the MMAs already issued.
@@ -593,6 +601,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_commit_if(leader, saddr(&s_drain[t]));
       warp_wait(saddr(&s_drain[t]), 0, a.wait_ns);
     }
+  } else {
+    // ---------------- look-up of the items, 32 at a time ----------------
+    const uint32_t items = (uint32_t)a.blocks * a.seqs * (a.heads >> a.pack);
+    uint32_t n = 0;
+    bool ok = true;
+    auto push = [&](uint32_t from) {  // lane `from` hands its item on
+      ok = ok && warp_wait(saddr(&s_itempty[n % kItems]), (n / kItems & 1) ^ 1, a.wait_ns);
+      if (!ok) return;
+      if (lane == (int)from) {
+        s_item[n % kItems] = it;
+        mbar_arrive(saddr(&s_itfull[n % kItems]));
+      }
+      ++n;
+    };
+    for (uint64_t x0 = blockIdx.x; x0 < items && ok; x0 += 32ull * gridDim.x) {
+      if (__any_sync(0xffffffffu, s_abort)) break;
+      const uint64_t x = x0 + (uint64_t)lane * gridDim.x;
+      const bool some = x < items && get_item<HD>(a, (uint32_t)x, it);
+      for (uint32_t rest = __ballot_sync(0xffffffffu, some); rest && ok; rest &= rest - 1)
+        push(__ffs(rest) - 1);
+    }
+    it.h = -1;
+    push(0);
+    if (!ok) s_abort = 1;
   }
   }
   tc_fence_before();
@@ -633,13 +665,13 @@ bool prompt_attr() {
 
 template <typename T, int HD>
 int launch_prompt(const PromptArgs& a, const CUtensorMap& q, const CUtensorMap& k,
-                  const CUtensorMap& v, cudaStream_t s) {
+                  const CUtensorMap& v, const CUtensorMap& o, cudaStream_t s) {
   if (!once_per_device(reinterpret_cast<const void*>(&prompt_attr<T, HD>), &prompt_attr<T, HD>))
     return MOE_ERR_CUDA;
   const int64_t items = (int64_t)a.blocks * a.seqs * (a.heads >> a.pack);
   const int grid = static_cast<int>(items < sm_count() ? items : sm_count());
   if (launch_pdl(k_prompt_attention<T, HD>, dim3(grid), dim3(kThreads), Cfg<HD>::kSmem, s, a, q, k,
-                 v) != cudaSuccess)
+                 v, o) != cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
   return MOE_OK;
@@ -670,7 +702,7 @@ extern "C" int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t
       bad_strides(v_stride, v_head_stride, kv_heads, head_dim))
     return MOE_ERR_INVALID_ARG;
   if (q_rows == 0 || seqs == 0 || max_q == 0) return MOE_OK;
-  if ((int64_t)seqs * heads > INT32_MAX) return MOE_ERR_UNSUPPORTED;
+  if (ceil_div(max_q, 16) * seqs * heads > INT32_MAX) return MOE_ERR_UNSUPPORTED;
   if (!q || !cu_q || !cu_k || !out || (k_rows > 0 && (!k || !v))) return MOE_ERR_INVALID_ARG;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) ||
       ((q_stride | q_head_stride | k_stride | k_head_stride | v_stride | v_head_stride) & 7))
@@ -682,6 +714,10 @@ extern "C" int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t
   int pack = 0;
   while (pack < 4 && heads / kv_heads % (2 << pack) == 0) ++pack;
   const int keys = head_dim == 64 ? Cfg<64>::kN : Cfg<128>::kN;
+  CUtensorMap mo;  // a warp's rows of the output: 32 / P tokens x P heads
+  if (!make_map(&mo, out, q_rows, heads, head_dim, (int64_t)heads * head_dim, head_dim, bf16,
+                32 >> pack, 1 << pack))
+    return MOE_ERR_CUDA;
   if (!make_map(&mq, q, q_rows, heads, head_dim, q_stride, q_head_stride, bf16, kM >> pack,
                 1 << pack) ||
       !make_map(&mk, none ? q : k, none ? q_rows : k_rows, none ? heads : kv_heads, head_dim,
@@ -707,8 +743,8 @@ extern "C" int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t
   a.wait_ns = wait_limit_ns();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (bf16)
-    return head_dim == 64 ? launch_prompt<BF16, 64>(a, mq, mk, mv, s)
-                          : launch_prompt<BF16, 128>(a, mq, mk, mv, s);
-  return head_dim == 64 ? launch_prompt<F16, 64>(a, mq, mk, mv, s)
-                        : launch_prompt<F16, 128>(a, mq, mk, mv, s);
+    return head_dim == 64 ? launch_prompt<BF16, 64>(a, mq, mk, mv, mo, s)
+                          : launch_prompt<BF16, 128>(a, mq, mk, mv, mo, s);
+  return head_dim == 64 ? launch_prompt<F16, 64>(a, mq, mk, mv, mo, s)
+                        : launch_prompt<F16, 128>(a, mq, mk, mv, mo, s);
 }
