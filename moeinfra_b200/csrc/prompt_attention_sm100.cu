@@ -404,8 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool whole = warp_token + (32 >> a.pack) <= it.len_q;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 64) {
-        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store read it
-        __syncwarp();
+        uint32_t w[32];
 #pragma unroll
         for (int hf = 0; hf < 64; hf += 32) {
           uint32_t o[32];
@@ -414,19 +413,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_wait_ld();
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              w[k] = inv == 0.f ? 0u
-                                : T::pack(__uint_as_float(o[8 * i + 2 * k]) * inv,
-                                          __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                             stage + lane * 128 + (((hf / 8 + i) ^ (lane & 7)) << 4)),
-                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                         : "memory");
-          }
+          for (int i = 0; i < 16; ++i)
+            w[hf / 2 + i] = inv == 0.f ? 0u
+                                       : T::pack(__uint_as_float(o[2 * i]) * inv,
+                                                 __uint_as_float(o[2 * i + 1]) * inv);
         }
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store read it
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 +
+                                                                        ((i ^ (lane & 7)) << 4)),
+                       "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3])
+                       : "memory");
         if (whole) {
           fence_proxy_async();
           __syncwarp();
