@@ -492,14 +492,16 @@ int moe_paged_attention(const uint16_t* q, int64_t q_stride, uint16_t* k_pages,
  *   a sequence are not written).  out [q_rows, heads, head_dim] packed.  fp32
  *   scores, softmax and sums; the probabilities are rounded to the element type
  *   for the product with V.  Values of other sequences have no effect.
- *   scale > 0. */
+ *   scale > 0.  The workspace (counters) must be zero before its first call and
+ *   is left zero, as moe_paged_attention's, which may be the same. */
+size_t moe_prompt_attention_workspace_size(void);
 int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t q_head_stride,
                          int64_t q_rows, const uint16_t* k, int64_t k_stride,
                          int64_t k_head_stride, const uint16_t* v, int64_t v_stride,
                          int64_t v_head_stride, int64_t k_rows, const int32_t* cu_q,
                          const int32_t* cu_k, int seqs, int max_q, int max_k, int heads,
                          int kv_heads, int head_dim, int causal, int dtype, float scale,
-                         uint16_t* out, void* stream);
+                         uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

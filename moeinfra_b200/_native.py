@@ -104,7 +104,8 @@ SIGNATURES: dict[str, tuple] = {
     "moe_prompt_attention": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64,
                                      c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
                                      c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                     c_int, c_float, c_void_p, c_void_p]),
+                                     c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "moe_prompt_attention_workspace_size": (c_size_t, []),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -90,6 +90,7 @@ struct PromptArgs {
   bool causal;
   float scale_log2;
   uint16_t* out;                // [rows_q, heads, HD]
+  uint32_t* counts;             // items claimed, CTAs done: zero between calls
   uint64_t wait_ns;
 };
 
@@ -197,7 +198,7 @@ struct __align__(16) Item {
   int row_q, row_k;     // the sequence's first rows
   int steps0, steps1;   // key steps of tile 0 and 1
 };
-constexpr int kItems = 4;                   // items looked up ahead
+constexpr int kItems = 2;                   // items looked up ahead
 constexpr int kReaders = kSoftWarps + 3;    // warps that read each of them
 
 // Item x of the launch; false where the sequence has no such block.  A
@@ -601,9 +602,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       warp_wait(saddr(&s_drain[t]), 0, a.wait_ns);
     }
   } else {
-    // ---------------- look-up of the items, 32 at a time ----------------
+    // ---------------- look-up of the items ----------------
+    // A CTA starts with the item of its own number and claims further ones from
+    // a counter as it goes: lengths, empty blocks and the clocks differ too much
+    // for a fixed share (64 prompts of 129 to 512 tokens: 138 us, 103 of them
+    // at the median CTA).  Claims are small while they hold work and grow over
+    // runs of blocks past their sequences' ends.
     const uint32_t items = (uint32_t)a.blocks * a.seqs * (a.heads >> a.pack);
-    uint32_t n = 0;
+    uint32_t n = 0, x0 = blockIdx.x, size = 1;
     bool ok = true;
     auto push = [&](uint32_t from) {  // lane `from` hands its item on
       ok = ok && warp_wait(saddr(&s_itempty[n % kItems]), (n / kItems & 1) ^ 1, a.wait_ns);
@@ -614,12 +620,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       ++n;
     };
-    for (uint64_t x0 = blockIdx.x; x0 < items && ok; x0 += 32ull * gridDim.x) {
+    while (x0 < items && ok) {
       if (__any_sync(0xffffffffu, s_abort)) break;
-      const uint64_t x = x0 + (uint64_t)lane * gridDim.x;
-      const bool some = x < items && get_item<HD>(a, (uint32_t)x, it);
-      for (uint32_t rest = __ballot_sync(0xffffffffu, some); rest && ok; rest &= rest - 1)
-        push(__ffs(rest) - 1);
+      const bool some = lane < (int)size && x0 + lane < items && get_item<HD>(a, x0 + lane, it);
+      const uint32_t live = __ballot_sync(0xffffffffu, some);
+      for (uint32_t rest = live; rest && ok; rest &= rest - 1) push(__ffs(rest) - 1);
+      size = live ? 1 : min(2 * size, 32u);
+      if (lane == 0) x0 = gridDim.x + atomicAdd(a.counts, size);
+      x0 = __shfl_sync(0xffffffffu, x0, 0);
+    }
+    // The last CTA to get here sets the counters back: nobody claims any more.
+    if (lane == 0) {
+      __threadfence();
+      if (atomicAdd(a.counts + 1, 1) == gridDim.x - 1) a.counts[0] = a.counts[1] = 0;
     }
     it.h = -1;
     push(0);
@@ -683,13 +696,16 @@ bool bad_strides(int64_t row, int64_t head, int64_t heads, int64_t hd) {
 }  // namespace
 }  // namespace moe
 
+extern "C" size_t moe_prompt_attention_workspace_size(void) { return 16; }
+
 extern "C" int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t q_head_stride,
                                     int64_t q_rows, const uint16_t* k, int64_t k_stride,
                                     int64_t k_head_stride, const uint16_t* v, int64_t v_stride,
                                     int64_t v_head_stride, int64_t k_rows, const int32_t* cu_q,
                                     const int32_t* cu_k, int seqs, int max_q, int max_k, int heads,
                                     int kv_heads, int head_dim, int causal, int dtype, float scale,
-                                    uint16_t* out, void* stream) {
+                                    uint16_t* out, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
   using namespace moe;
   if (q_rows < 0 || k_rows < 0 || q_rows > INT32_MAX - 256 || k_rows > INT32_MAX - 256 || seqs < 0 ||
       max_q < 0 || max_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || !(scale > 0.f))
@@ -706,6 +722,9 @@ extern "C" int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) ||
       ((q_stride | q_head_stride | k_stride | k_head_stride | v_stride | v_head_stride) & 7))
     return MOE_ERR_ALIGNMENT;
+  if (!workspace || workspace_bytes < moe_prompt_attention_workspace_size())
+    return MOE_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return MOE_ERR_ALIGNMENT;
   const bool bf16 = dtype == MOE_DTYPE_BF16;
   CUtensorMap mq, mk, mv;
   // Without any key no K or V tile is loaded: the maps then describe q.
@@ -739,6 +758,7 @@ extern "C" int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t
   a.causal = causal != 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = out;
+  a.counts = static_cast<uint32_t*>(workspace);
   a.wait_ns = wait_limit_ns();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (bf16)

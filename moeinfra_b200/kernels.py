@@ -590,6 +590,7 @@ def ep_return_partials_p2p(y_part: torch.Tensor, recv_counts: torch.Tensor, num_
 # ---------------------------------------------------------------------------
 
 _DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+PROMPT_WORKSPACE_BYTES = 16
 _COUNTER_BYTES = 4096  # the part of a workspace that has to be zero before its first call
 _serve_ws: dict = {}
 
@@ -757,8 +758,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     nbytes = _paged_ws_bytes(dev.index, seqs, max_pages, page, heads, kv, hd)
     if workspace is None:
         workspace = _serve_scratch(dev, stream, nbytes)
-    elif workspace.numel() < nbytes:
-        raise ValueError(f"{what}: workspace has {workspace.numel()} bytes, needs {nbytes}")
+    elif workspace.numel() * workspace.element_size() < nbytes:
+        raise ValueError(f"{what}: workspace needs {nbytes} bytes")
     check(_native.lib().moe_paged_attention(
         q.data_ptr(), _outer_stride(q), k_pages.data_ptr(),
         v_pages.data_ptr(), _outer_stride(k_pages), _outer_stride(v_pages), n_pages, page,
@@ -773,7 +774,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                      max_seqlen: int, cu_seqlens_k: torch.Tensor | None = None,
                      max_seqlen_k: int | None = None, causal: bool = True,
-                     scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                     scale: float | None = None, out: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Attention over packed prompts of different lengths.
 
     ``q`` [rows, heads, head_dim], ``k`` / ``v`` [rows_k, kv_heads, head_dim] (rows and heads may
@@ -781,7 +783,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ``cu_seqlens[b] .. cu_seqlens[b+1]`` (int32, on the device), none longer than ``max_seqlen``;
     its keys likewise by ``cu_seqlens_k`` / ``max_seqlen_k`` (default: the queries').  Causal: the
     queries are the last of their sequence's positions; one that sees no key gives zeros.  Returns
-    [rows, heads, head_dim].
+    [rows, heads, head_dim].  ``workspace``: as for :func:`paged_attention`, of at least
+    ``PROMPT_WORKSPACE_BYTES`` zeroed bytes (the same buffer may serve both).
     """
     what = "prompt_attention"
     if not isinstance(q, torch.Tensor) or q.ndim != 3:
@@ -811,12 +814,17 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         out = torch.empty((T, heads, hd), dtype=dt, device=dev)
     else:
         _serve_check(what, dev, ("out", out, dt, (T, heads, hd), 3))
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if workspace is None:
+        workspace = _serve_scratch(dev, stream, PROMPT_WORKSPACE_BYTES)
+    elif workspace.numel() * workspace.element_size() < PROMPT_WORKSPACE_BYTES:
+        raise ValueError(f"{what}: workspace needs {PROMPT_WORKSPACE_BYTES} bytes")
     check(_native.lib().moe_prompt_attention(
         q.data_ptr(), *_row_strides(q), T, k.data_ptr(), *_row_strides(k), v.data_ptr(),
         *_row_strides(v), k.shape[0], cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), seqs,
         max_seqlen, max_seqlen_k, heads, kv, hd, causal, _DTYPE_CODES[dt],
-        hd ** -0.5 if scale is None else scale, out.data_ptr(),
-        torch.cuda.current_stream(dev).cuda_stream), "moe_prompt_attention")
+        hd ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(),
+        PROMPT_WORKSPACE_BYTES, stream), "moe_prompt_attention")
     return out
 
 

@@ -187,17 +187,18 @@ def test_host_checks_precede_every_launch():
     lib, f, odd = _native.lib(), ctypes.c_void_p(0x100000), ctypes.c_void_p(0x100008)
 
     def attend(q=f, rows=10, seqs=2, H=4, KV=2, hd=128, dtype=0, scale=1.0, stride=None, out=f,
-               max_q=8, k=f, head=None):
+               max_q=8, k=f, head=None, ws=f, bytes_=16):
         return lib.moe_prompt_attention(q, H * hd if stride is None else stride,
                                         hd if head is None else head, rows, k, KV * hd, hd, f,
                                         KV * hd, hd, rows, f, f, seqs, max_q, 8, H, KV, hd, 1, dtype,
-                                        scale, out, None)
+                                        scale, out, ws, bytes_, None)
 
     assert attend(rows=0) == 0 and attend(seqs=0) == 0 and attend(max_q=0) == 0
     assert attend(rows=-1) == 1 and attend(H=5) == 1 and attend(q=None) == 1 and attend(k=None) == 1
     assert attend(scale=0.0) == 1 and attend(scale=float("nan")) == 1 and attend(stride=8) == 1
     assert attend(head=64) == 1 and attend(seqs=-1) == 1
     assert attend(hd=96) == 2 and attend(dtype=2) == 2
+    assert attend(ws=None) == 4 and attend(bytes_=15) == 4 and attend(ws=odd) == 5
     assert attend(q=odd) == 5 and attend(out=odd) == 5 and attend(stride=516) == 5
 
 
@@ -229,3 +230,5 @@ def test_wrapper_refuses_wrong_shapes_and_types():
             attend(**bad)
     with pytest.raises(RuntimeError):
         attend(scale=0.0)
+    with pytest.raises(ValueError, match="workspace"):
+        attend(workspace=torch.zeros(8, dtype=torch.uint8, device="cuda"))
