@@ -198,7 +198,7 @@ struct __align__(16) Item {
   int row_q, row_k;     // the sequence's first rows
   int steps0, steps1;   // key steps of tile 0 and 1
 };
-constexpr int kItems = 2;                   // items looked up ahead
+constexpr int kItems = 1;                   // items looked up ahead
 constexpr int kReaders = kSoftWarps + 3;    // warps that read each of them
 
 // Item x of the launch; false where the sequence has no such block.  A
@@ -609,7 +609,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // at the median CTA).  Claims are small while they hold work and grow over
     // runs of blocks past their sequences' ends.
     const uint32_t items = (uint32_t)a.blocks * a.seqs * (a.heads >> a.pack);
-    uint32_t n = 0, x0 = blockIdx.x, size = 1;
+    uint32_t n = 0, x0 = blockIdx.x, size = 1, n_q = 0;
+    int steps = 0;  // of the last item handed on
     bool ok = true;
     auto push = [&](uint32_t from) {  // lane `from` hands its item on
       ok = ok && warp_wait(saddr(&s_itempty[n % kItems]), (n / kItems & 1) ^ 1, a.wait_ns);
@@ -618,6 +619,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         s_item[n % kItems] = it;
         mbar_arrive(saddr(&s_itfull[n % kItems]));
       }
+      steps = __shfl_sync(0xffffffffu, max(it.steps0, it.steps1), from);
+      n_q += steps > 0;
       ++n;
     };
     while (x0 < items && ok) {
@@ -626,6 +629,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t live = __ballot_sync(0xffffffffu, some);
       for (uint32_t rest = live; rest && ok; rest &= rest - 1) push(__ffs(rest) - 1);
       size = live ? 1 : min(2 * size, 32u);
+      // In the last rounds an item is claimed late, once the one at hand has
+      // issued its last Q K^T: a claim made early binds it to a busy CTA (one
+      // prompt of 2048: 47 us early, 39 late).
+      if (steps > 0 && x0 + 2 * gridDim.x > items)
+        ok = ok && warp_wait(saddr(&s_qempty), (n_q - 1) & 1, a.wait_ns);
       if (lane == 0) x0 = gridDim.x + atomicAdd(a.counts, size);
       x0 = __shfl_sync(0xffffffffu, x0, 0);
     }
@@ -635,6 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (atomicAdd(a.counts + 1, 1) == gridDim.x - 1) a.counts[0] = a.counts[1] = 0;
     }
     it.h = -1;
+    it.steps0 = it.steps1 = 0;
     push(0);
     if (!ok) s_abort = 1;
   }
