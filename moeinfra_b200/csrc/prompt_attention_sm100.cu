@@ -201,15 +201,14 @@ struct __align__(16) Item {
 constexpr int kItems = 1;                   // items looked up ahead
 constexpr int kReaders = kSoftWarps + 3;    // warps that read each of them
 
-// Item x of the launch; false where the sequence has no such block.  A
-// sequence whose offsets do not describe rows of q and k, or that is longer
-// than the call said, counts as empty (error bit set).
+// Block x of the launch (all heads of 256 >> pack tokens of a sequence, the last
+// tokens first); false where the sequence has no such block.  A sequence whose
+// offsets do not describe rows of q and k, or that is longer than the call
+// said, counts as empty (error bit set).
 template <int HD>
-__device__ __forceinline__ bool get_item(const PromptArgs& a, uint32_t x, Item& it) {
-  const uint32_t groups = a.heads >> a.pack, per = a.seqs * groups;
-  const uint32_t blk = x / per, r = x - blk * per, b = r / groups;
+__device__ __forceinline__ bool get_block(const PromptArgs& a, uint32_t x, Item& it) {
+  const uint32_t blk = x / a.seqs, b = x - blk * a.seqs;
   const int tokens = kM >> a.pack;
-  it.h = (r - b * groups) << a.pack;
   it.q0 = (a.blocks - 1 - (int)blk) * 2 * tokens;
   const int q_lo = a.cu_q[b], q_hi = a.cu_q[b + 1], k_lo = a.cu_k[b], k_hi = a.cu_k[b + 1];
   it.len_q = q_hi - q_lo;
@@ -603,15 +602,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------- look-up of the items ----------------
-    // A CTA starts with the item of its own number and claims further ones from
-    // a counter as it goes: lengths, empty blocks and the clocks differ too much
-    // for a fixed share (64 prompts of 129 to 512 tokens: 138 us, 103 of them
-    // at the median CTA).  Claims are small while they hold work and grow over
-    // runs of blocks past their sequences' ends.
-    const uint32_t items = (uint32_t)a.blocks * a.seqs * (a.heads >> a.pack);
-    uint32_t n = 0, x0 = blockIdx.x, size = 1, n_q = 0;
-    int steps = 0;  // of the last item handed on
-    bool ok = true;
+    // Items are the head groups of each block that has rows, in order.  A CTA
+    // starts with the item of its own number and claims further ones from a
+    // counter as it goes: lengths and clocks differ too much for a fixed share
+    // (64 prompts of 129 to 512 tokens: 138 us, 103 of them at the median CTA).
+    // To find an item's block, every CTA walks the blocks, 32 at a time, and
+    // counts those with rows.
+    const uint32_t groups = a.heads >> a.pack, blocks = (uint32_t)a.blocks * a.seqs;
+    uint32_t n = 0, n_q = 0, at = 0, before = 0, live = 0;
+    bool ok = true, mine = false;
+    auto look = [&]() {  // the next 32 blocks
+      mine = at + lane < blocks && get_block<HD>(a, at + lane, it);
+      live = __ballot_sync(0xffffffffu, mine);
+      at += 32;
+    };
     auto push = [&](uint32_t from) {  // lane `from` hands its item on
       ok = ok && warp_wait(saddr(&s_itempty[n % kItems]), (n / kItems & 1) ^ 1, a.wait_ns);
       if (!ok) return;
@@ -619,23 +623,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         s_item[n % kItems] = it;
         mbar_arrive(saddr(&s_itfull[n % kItems]));
       }
-      steps = __shfl_sync(0xffffffffu, max(it.steps0, it.steps1), from);
-      n_q += steps > 0;
       ++n;
     };
-    while (x0 < items && ok) {
-      if (__any_sync(0xffffffffu, s_abort)) break;
-      const bool some = lane < (int)size && x0 + lane < items && get_item<HD>(a, x0 + lane, it);
-      const uint32_t live = __ballot_sync(0xffffffffu, some);
-      for (uint32_t rest = live; rest && ok; rest &= rest - 1) push(__ffs(rest) - 1);
-      size = live ? 1 : min(2 * size, 32u);
+    uint32_t y = blockIdx.x;
+    look();
+    while (ok && !__any_sync(0xffffffffu, s_abort)) {
+      const uint32_t block = y / groups;
+      while (block >= before + __popc(live) && at < blocks) {
+        before += __popc(live);
+        look();
+      }
+      if (block >= before + __popc(live)) break;
+      it.h = (y - block * groups) << a.pack;
+      const uint32_t from = __ffs(__ballot_sync(
+          0xffffffffu, mine && __popc(live & ((1u << lane) - 1)) == block - before)) - 1;
+      push(from);
+      const int steps = __shfl_sync(0xffffffffu, max(it.steps0, it.steps1), from);
       // In the last rounds an item is claimed late, once the one at hand has
       // issued its last Q K^T: a claim made early binds it to a busy CTA (one
       // prompt of 2048: 47 us early, 39 late).
-      if (steps > 0 && x0 + 2 * gridDim.x > items)
+      if (steps > 0) ++n_q;
+      if (steps > 0 && y + 2 * gridDim.x > blocks * groups)
         ok = ok && warp_wait(saddr(&s_qempty), (n_q - 1) & 1, a.wait_ns);
-      if (lane == 0) x0 = gridDim.x + atomicAdd(a.counts, size);
-      x0 = __shfl_sync(0xffffffffu, x0, 0);
+      if (lane == 0) y = gridDim.x + atomicAdd(a.counts, 1);
+      y = __shfl_sync(0xffffffffu, y, 0);
     }
     // The last CTA to get here sets the counters back: nobody claims any more.
     if (lane == 0) {
