@@ -503,6 +503,23 @@ int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t q_head_str
                          int kv_heads, int head_dim, int causal, int dtype, float scale,
                          uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* moe_sample_tokens: one token per row of logits [rows, vocab] (fp16, bf16 or
+ *   fp32, rows stride elements apart, vocab <= 262144).  With m a row's maximum,
+ *   e_i = exp((x_i - m) / temperature) in fp32 (1 where x_i == m; NaN logits
+ *   count as -inf) and the integer weights w_i = trunc(2^40 e_i), over the tokens
+ *   by falling logit, equal ones by rising index: top_k > 0 keeps the first
+ *   top_k; top_p < 1 keeps of those the shortest prefix that holds at least
+ *   ceil(top_p * their sum) (one token at least); min_p keeps of those
+ *   e_i >= min_p (above 1 as 1).  tokens[row] is the first index, in index order,
+ *   whose running sum of the kept weights exceeds floor(uniforms[row] * their
+ *   sum); probs[row] its share of that sum.  temperature <= 0 or top_k == 1: the
+ *   lowest index of the maximum, probability 1.  Integer sums: the token depends
+ *   on its row and numbers alone, not on the launch. */
+int moe_sample_tokens(const void* logits, int64_t stride, int64_t rows, int vocab, int dtype,
+                      const float* uniforms, const float* temperature, const int32_t* top_k,
+                      const float* top_p, const float* min_p, int64_t* tokens, float* probs,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -106,6 +106,8 @@ SIGNATURES: dict[str, tuple] = {
                                      c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                      c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "moe_prompt_attention_workspace_size": (c_size_t, []),
+    "moe_sample_tokens": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

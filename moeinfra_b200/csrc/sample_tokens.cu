@@ -1,0 +1,474 @@
+// Sampling one token per row of logits: temperature, top-k, top-p, min-p, from
+// random numbers the caller gives.  No counterpart in the reference (greedy
+// decoding only, engine/engine.py:579-663).
+//
+// For a row x of V logits (NaN counts as -inf), m its maximum:
+//   d_i = 0 where x_i == m, else (x_i - m) / temperature
+//   w_i = trunc(2^40 exp(d_i)), exp in fp32, w as a 64-bit integer
+// Tokens are ordered by falling x, equal ones by rising index.
+//   top-k keeps the first k; W = sum of their w
+//   top-p keeps of those the shortest prefix with sum >= ceil(p W)
+//   min-p keeps of those exp(d_i) >= min_p
+// W' = sum of the w kept, r = floor(u W'); the token is the first kept index,
+// in index order, whose inclusive sum of w exceeds r, its probability w / W'.
+// Temperature 0, or k = 1: the maximum of lowest index, probability 1.
+//
+// Sums of integers do not depend on their order, so the token does not either:
+// the same logits and numbers give the same token however a row is split.  40
+// bits below the maximum leave every weight that has a chance to be drawn
+// fp32's precision, and 2^18 of them fit 64 bits with room to spare.
+//
+// Bound by latency where rows are few (a row is 64 KB at 32000 fp16 logits; the
+// rest is a chain of reductions), by instruction issue where they are many.  A
+// row is spread over a cluster of CTAs whose threads hold it in registers, as
+// integers of the same order ("keys"):
+//   * no sort: the k-th token and the top-p boundary are found by search over
+//     the keys, 8 ways a pass.  A pass adds each weight to the sums of the
+//     thresholds below it (21 instructions a logit), over the logits that are
+//     still between the bounds; register slots that hold none of these for a
+//     whole warp are skipped.  The first thresholds sit where a language
+//     model's boundary usually lies, 0.5 to 16 below the maximum in units of
+//     the temperature; correctness does not depend on them.
+//   * 16-bit logits have 16-bit keys: half the passes.
+//   * Per pass one cluster barrier: warps reduce in two integer reductions of
+//     32 bits each, a CTA's sums go to every CTA of the cluster through
+//     distributed shared memory.
+#include <cooperative_groups.h>
+
+#include "paged.cuh"
+
+namespace moe {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMaxCluster = 16;            // 8 is the portable size; 16 only where a row needs it
+constexpr int kMaxPer = 32;                // logits a thread holds at most
+constexpr int kMaxVocab = kMaxCluster * kThreads * kMaxPer;
+constexpr float kScale = 1099511627776.f;  // 2^40
+constexpr uint32_t kAll = 0xffffffffu;
+
+struct SampleArgs {
+  const void* logits;
+  int64_t stride;
+  int vocab, cluster;
+  const float *uniforms, *temperature, *top_p, *min_p;
+  const int32_t* top_k;
+  int64_t* tokens;
+  float* probs;
+};
+
+// Logits as keys: unsigned integers of the same order, NaN as -inf, -0 as 0.
+// Every key is above 0, which stands for "no logit".
+template <typename T>
+struct Logit;
+struct Half16 {
+  using Raw = uint16_t;
+  static constexpr int kVec = 8;
+  // `inf`: the format's infinity, above which are NaNs.
+  static __device__ __forceinline__ uint32_t key(uint32_t b, uint32_t inf) {
+    if ((b & 0x7FFFu) > inf) b = 0x8000u | inf;
+    if (b == 0x8000u) b = 0;
+    return b & 0x8000u ? (~b & 0xFFFFu) : (b | 0x8000u);
+  }
+  static __device__ __forceinline__ uint32_t raw(uint32_t k) {
+    return k & 0x8000u ? (k & 0x7FFFu) : (~k & 0xFFFFu);
+  }
+};
+template <>
+struct Logit<F16> : Half16 {
+  static __device__ __forceinline__ uint32_t key(uint16_t b) { return Half16::key(b, 0x7C00u); }
+  static __device__ __forceinline__ float value(uint32_t k) { return h2f((uint16_t)raw(k)); }
+  static __device__ __forceinline__ uint32_t key_near(float x) { return key(f2h(x)); }
+};
+template <>
+struct Logit<BF16> : Half16 {
+  static __device__ __forceinline__ uint32_t key(uint16_t b) { return Half16::key(b, 0x7F80u); }
+  static __device__ __forceinline__ float value(uint32_t k) { return __uint_as_float(raw(k) << 16); }
+  static __device__ __forceinline__ uint32_t key_near(float x) { return key(BF16::one(x)); }
+};
+template <>
+struct Logit<float> {
+  using Raw = float;
+  static constexpr int kVec = 4;
+  static __device__ __forceinline__ uint32_t key(float x) {
+    if (x != x) x = -INFINITY;
+    const uint32_t b = __float_as_uint(x + 0.f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+  }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+  }
+  static __device__ __forceinline__ uint32_t key_near(float x) { return key(x); }
+};
+
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) { return __shfl_sync(kAll, v, lane); }
+__device__ __forceinline__ uint64_t weight(float e) { return __float2ull_rz(e * kScale); }
+
+// Sums over the cluster, 8 values at a time: lane j of every warp ends up with
+// the sum of value j % 8.  slot(r, j): what CTA r contributed to the last one;
+// warp_sum[w][j]: what warp w of this CTA did.
+struct Exchange {
+  cg::cluster_group cluster;
+  int rank, size, warp, lane, turn = 0;
+  uint64_t (*warp_sum)[8];
+  uint64_t (*slots)[kMaxCluster][8];  // two of these, used in turn
+
+  __device__ __forceinline__ uint64_t slot(int r, int j) const { return slots[turn ^ 1][r][j]; }
+  __device__ __forceinline__ void give(uint64_t mine) {  // lane j < 8: the CTA's value j
+    const uint32_t to = lane >> 3, j = lane & 7;
+    uint64_t* at = &slots[turn][rank][j];
+    for (int r = to; r < size; r += 4) *cluster.map_shared_rank(at, r) = mine;
+  }
+  template <int N>
+  __device__ __forceinline__ uint64_t sum(const uint64_t (&v)[N]) {
+    uint64_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {  // 27 bits and the rest: 32 of them fit 32 bits
+      const uint32_t lo = __reduce_add_sync(kAll, (uint32_t)v[j] & 0x7FFFFFFu);
+      const uint32_t hi = __reduce_add_sync(kAll, (uint32_t)(v[j] >> 27));
+      if ((lane & 7) == j) mine = lo + ((uint64_t)hi << 27);
+    }
+    if (lane < 8) warp_sum[warp][lane] = mine;
+    __syncthreads();
+    if (warp == 0) {
+      uint64_t s = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; w += 4) s += warp_sum[w + (lane >> 3)][lane & 7];
+      s += __shfl_xor_sync(kAll, s, 8);
+      s += __shfl_xor_sync(kAll, s, 16);
+      give(s);
+    }
+    cluster.sync();
+    uint64_t s = 0;
+    for (int r = lane >> 3; r < size; r += 4) s += slots[turn][r][lane & 7];
+    s += __shfl_xor_sync(kAll, s, 8);
+    s += __shfl_xor_sync(kAll, s, 16);
+    turn ^= 1;
+    return s;
+  }
+  __device__ __forceinline__ uint64_t max(uint64_t v) {  // of all threads, in every thread
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const uint64_t u = __shfl_xor_sync(kAll, v, o);
+      v = u > v ? u : v;
+    }
+    if (lane == 0) warp_sum[warp][0] = v;
+    __syncthreads();
+    if (warp == 0) {
+      v = warp_sum[lane & (kWarps - 1)][0];
+#pragma unroll
+      for (int o = kWarps / 2; o; o >>= 1) {
+        const uint64_t u = __shfl_xor_sync(kAll, v, o);
+        v = u > v ? u : v;
+      }
+      if ((lane & 7) == 0) give(v);
+    }
+    cluster.sync();
+    v = slots[turn][0][0];
+    for (int r = 1; r < size; ++r) {
+      const uint64_t u = slots[turn][r][0];
+      v = u > v ? u : v;
+    }
+    turn ^= 1;
+    return v;
+  }
+};
+
+template <typename T, int PER>
+__global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
+  using L = Logit<T>;
+  constexpr int kVec = L::kVec, kIters = PER / kVec;
+  __shared__ uint64_t s_warp[kWarps][8], s_slots[2][kMaxCluster][8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Exchange ex{cg::this_cluster(), 0, a.cluster, warp, lane, 0, s_warp, s_slots};
+  ex.rank = blockIdx.x % a.cluster;
+  const int64_t row = blockIdx.x / a.cluster;
+  ex.cluster.barrier_arrive();  // waited for before the first store to another CTA
+  pdl_trigger();
+  pdl_wait();
+
+  // ---- the row: element v of step i of a lane has index first + i * 32 * kVec + v ----
+  uint32_t key[PER];
+  const int first = ((ex.rank * kWarps + warp) * kIters * 32 + lane) * kVec;
+  const typename L::Raw* x = static_cast<const typename L::Raw*>(a.logits) + row * a.stride;
+  const bool wide = (reinterpret_cast<uintptr_t>(x) & 15u) == 0;
+#pragma unroll
+  for (int i = 0; i < kIters; ++i) {
+    const int at = first + i * 32 * kVec;
+    if (wide && at + kVec <= a.vocab) {
+      const uint4 v = *reinterpret_cast<const uint4*>(x + at);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        if constexpr (kVec == 8) key[i * kVec + j] = L::key((uint16_t)(w[j / 2] >> (16 * (j & 1))));
+        else key[i * kVec + j] = L::key(__uint_as_float(w[j]));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) key[i * kVec + j] = at + j < a.vocab ? L::key(x[at + j]) : 0u;
+    }
+  }
+  const float temperature = a.temperature[row], u = a.uniforms[row], p = a.top_p[row];
+  const float min_p = fminf(a.min_p[row], 1.f);  // above 1 the maxima stay
+  const int k = a.top_k[row];
+
+  // ---- the maximum and its lowest index ----
+  uint64_t best = 0;
+#pragma unroll
+  for (int c = 0; c < PER; ++c) {
+    const uint32_t index = first + c / kVec * 32 * kVec + c % kVec;
+    const uint64_t v = (uint64_t)key[c] << 32 | (0xFFFFFFFFu - index);
+    best = v > best ? v : best;
+  }
+  ex.cluster.barrier_wait();
+  best = ex.max(best);
+  const uint32_t top = (uint32_t)(best >> 32);
+  if (!(temperature > 0.f) || k == 1) {
+    if (ex.rank == 0 && threadIdx.x == 0) {
+      a.tokens[row] = 0xFFFFFFFFu - (uint32_t)best;
+      a.probs[row] = 1.f;
+    }
+    return;
+  }
+  const float m = L::value(top);
+  auto exp_of = [&](uint32_t key) {
+    return key == top ? 1.f : key == 0 ? 0.f : expf(__fdiv_rn(L::value(key) - m, temperature));
+  };
+  float e[PER];
+#pragma unroll
+  for (int c = 0; c < PER; ++c) e[c] = exp_of(key[c]);
+
+  // Sums of the weights (or counts) of the keys in [lo, hi) that are >= the
+  // threshold t of lane 1 .. 7 (lane 0: >= t too), as lane j's result.
+  auto pass = [&](bool count, uint32_t lo, uint32_t hi, uint32_t t) {
+    uint32_t th[8], slots = 0;
+    uint64_t sum[8] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) th[j] = __shfl_sync(kAll, t, j);
+#pragma unroll
+    for (int c = 0; c < PER; ++c) slots |= (key[c] - lo < hi - lo ? 1u : 0u) << c;
+    const uint32_t used = __reduce_or_sync(kAll, slots);
+#pragma unroll
+    for (int c = 0; c < PER; ++c) {
+      if (!(used >> c & 1)) continue;
+      const uint64_t w = !(slots >> c & 1) ? 0ull : count ? 1ull : weight(e[c]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[j] += key[c] >= th[j] ? w : 0ull;
+    }
+    return ex.sum(sum);
+  };
+  // The largest key whose sum over it and all above is >= need, and the sum
+  // above it.  t, s: thresholds of a first pass (rising with the lane, lane 0
+  // not among them) and their sums.  lo's sum is known to be enough, hi's not.
+  struct Bound {
+    uint32_t key;
+    uint64_t above;
+  };
+  auto search = [&](bool count, uint64_t need, uint32_t lo, uint32_t hi, uint32_t t, uint64_t s) {
+    uint64_t above = 0;
+    for (;;) {
+      const uint32_t enough = __ballot_sync(kAll, lane >= 1 && lane < 8 && s >= need) | 1u;
+      const int j = 31 - __clz(enough);  // sums fall as thresholds rise
+      const uint32_t t_lo = __shfl_sync(kAll, t, j), t_hi = __shfl_sync(kAll, t, (j + 1) & 7);
+      const uint64_t s_hi = shfl64(s, (j + 1) & 7);
+      if (j > 0 && t_lo > lo) lo = t_lo;
+      if (j < 7 && t_hi < hi) {
+        hi = t_hi;
+        above = s_hi;
+      }
+      if (hi - lo <= 1) return Bound{lo, above};
+      const uint32_t step = (hi - lo + 7) / 8;
+      const uint64_t next = (uint64_t)lo + (uint64_t)step * (lane & 7);
+      t = next < hi ? (uint32_t)next : hi;
+      s = above + pass(count, lo, hi, t);
+    }
+  };
+  // First thresholds: lane 7 the nearest to the maximum.
+  const float reach[8] = {0.f, 16.f, 11.f, 8.f, 5.5f, 3.5f, 1.75f, 0.5f};
+  float mine = 0.f;
+#pragma unroll
+  for (int j = 1; j < 8; ++j)
+    if ((lane & 7) == j) mine = reach[j];
+  uint32_t guess = L::key_near(m - mine * temperature);
+  if (guess > top) guess = top;
+
+  // ---- top-k: keys above k_key, and the first k_ties of those equal to it ----
+  uint32_t cut = 0;    // keys above it are kept
+  uint64_t ties = 0;   // and so many of those equal to it, by index
+  const bool by_k = k > 0 && k < a.vocab;
+  if (by_k) {
+    const uint64_t s = pass(true, 1, top + 1, guess);
+    const Bound b = search(true, k, 1, top + 1, guess, s);
+    cut = b.key;
+    ties = k - b.above;
+  }
+  // ---- top-p ----
+  if (p < 1.f) {
+    const uint64_t s = pass(false, 1, top + 1, (lane & 7) == 0 ? cut + 1 : guess);
+    const uint64_t total = shfl64(s, 0) + ties * (cut ? weight(exp_of(cut)) : 0ull);
+    const double want = ceil(__dmul_rn((double)p, __ull2double_rn(total)));
+    uint64_t need = want >= 1.0 ? __double2ull_rz(want) : 1ull;
+    if (need > total) need = total;
+    const uint32_t lo = cut ? cut : 1u;
+    const Bound b = search(false, need, lo, top + 1, guess, s);
+    const uint64_t w = weight(exp_of(b.key));
+    const uint64_t n = (need - b.above + w - 1) / w;
+    ties = b.key == cut && n > ties ? ties : n;
+    cut = b.key;
+  }
+  // ---- what is kept, per warp and CTA ----
+  uint64_t sums[2] = {0, 0};
+#pragma unroll
+  for (int c = 0; c < PER; ++c) {
+    if (key[c] > cut && e[c] >= min_p) sums[0] += weight(e[c]);
+    if (key[c] == cut) ++sums[1];
+  }
+  ex.sum(sums);
+  const float e_cut = cut ? exp_of(cut) : 0.f;
+  const uint64_t w_cut = cut && e_cut >= min_p ? weight(e_cut) : 0ull;
+  auto kept = [&](uint64_t equal, uint64_t before) {  // of `equal` ties after `before` others
+    return before >= ties ? 0ull : (ties - before < equal ? ties - before : equal);
+  };
+  uint64_t total = 0, mine_before = 0, ties_before = 0, seen = 0, mine_all = 0;
+  for (int r = 0; r < a.cluster; ++r) {
+    const uint64_t n = ex.slot(r, 1), w = ex.slot(r, 0) + kept(n, seen) * w_cut;
+    if (r == ex.rank) {
+      mine_before = total;
+      mine_all = w;
+      ties_before = seen;
+    }
+    total += w;
+    seen += n;
+  }
+  const double at = floor(__dmul_rn((double)u, __ull2double_rn(total)));
+  uint64_t r = at >= 1.0 ? __double2ull_rz(at) : 0ull;
+  if (r > total - 1) r = total - 1;
+  if (r < mine_before || r >= mine_before + mine_all) return;
+  // ---- the CTA that holds the token: its warp, step, lane, element ----
+  uint64_t run = mine_before, warp_all = 0;
+  for (int w = 0; w <= warp; ++w) {
+    if (w > 0) {
+      run += warp_all;
+      ties_before += s_warp[w - 1][1];
+    }
+    warp_all = s_warp[w][0] + kept(s_warp[w][1], ties_before) * w_cut;
+  }
+  if (r < run || r >= run + warp_all) return;
+#pragma unroll
+  for (int i = 0; i < kIters; ++i) {
+    uint64_t own = 0;
+    uint32_t equal = 0;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const int c = i * kVec + j;
+      if (key[c] > cut && e[c] >= min_p) own += weight(e[c]);
+      equal += key[c] == cut;
+    }
+    uint32_t equal_in = equal;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(kAll, equal_in, o);
+      if (lane >= o) equal_in += v;
+    }
+    uint64_t before = ties_before + equal_in - equal;
+    uint64_t in = own + kept(equal, before) * w_cut;
+    const uint64_t lane_all = in;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t v = __shfl_up_sync(kAll, in, o);
+      if (lane >= o) in += v;
+    }
+    uint64_t at_lane = run + in - lane_all;
+    if (r >= at_lane && r < at_lane + lane_all) {
+      bool found = false;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        const int c = i * kVec + j;
+        uint64_t w = key[c] > cut && e[c] >= min_p ? weight(e[c]) : 0ull;
+        if (key[c] == cut) {
+          w = before < ties ? w_cut : 0ull;
+          ++before;
+        }
+        if (!found && r < at_lane + w) {
+          found = true;
+          a.tokens[row] = first + i * 32 * kVec + j;
+          a.probs[row] = (float)(__ull2double_rn(w) / __ull2double_rn(total));
+        }
+        at_lane += w;
+      }
+    }
+    run += shfl64(in, 31);
+    ties_before += __shfl_sync(kAll, equal_in, 31);
+    if (r < run) return;
+  }
+}
+
+template <typename T, int PER>
+bool sample_attr() {
+  return cudaFuncSetAttribute(k_sample<T, PER>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) ==
+         cudaSuccess;
+}
+
+template <typename T, int PER>
+int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t s) {
+  if (!once_per_device(reinterpret_cast<const void*>(&sample_attr<T, PER>), &sample_attr<T, PER>))
+    return MOE_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * a.cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = a.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, k_sample<T, PER>, a) != cudaSuccess) return MOE_ERR_CUDA;
+  MOE_CHECK_LAUNCH();
+  return MOE_OK;
+}
+
+// CTAs of a row and logits of a thread: as many CTAs as give a thread 8 logits
+// while all rows' CTAs fit the GPU at once (two to an SM), else fewer and fuller
+// ones, whose passes have fewer barriers per logit.
+template <typename T>
+int launch_rows(SampleArgs& a, int64_t rows, cudaStream_t s) {
+  int per = 8;
+  auto ctas = [&](int n) {
+    int c = 1;
+    while ((int64_t)c * kThreads * n < a.vocab) c *= 2;
+    return c;
+  };
+  while (per < kMaxPer && (ctas(per) > 8 || rows * ctas(per) > 2 * sm_count())) per *= 2;
+  a.cluster = ctas(per);
+  if (rows * a.cluster > INT32_MAX) return MOE_ERR_UNSUPPORTED;
+  if (per == 8) return launch_sample<T, 8>(a, rows, s);
+  if (per == 16) return launch_sample<T, 16>(a, rows, s);
+  return launch_sample<T, 32>(a, rows, s);
+}
+
+}  // namespace
+}  // namespace moe
+
+extern "C" int moe_sample_tokens(const void* logits, int64_t stride, int64_t rows, int vocab,
+                                 int dtype, const float* uniforms, const float* temperature,
+                                 const int32_t* top_k, const float* top_p, const float* min_p,
+                                 int64_t* tokens, float* probs, void* stream) {
+  using namespace moe;
+  if (rows < 0 || vocab < 1 || (rows > 1 && stride < vocab)) return MOE_ERR_INVALID_ARG;
+  if (dtype != MOE_DTYPE_F16 && dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F32)
+    return MOE_ERR_UNSUPPORTED;
+  if (vocab > kMaxVocab) return MOE_ERR_UNSUPPORTED;
+  if (rows == 0) return MOE_OK;
+  if (!logits || !uniforms || !temperature || !top_k || !top_p || !min_p || !tokens || !probs)
+    return MOE_ERR_INVALID_ARG;
+  SampleArgs a{logits, stride, vocab, 1, uniforms, temperature, top_p, min_p, top_k, tokens, probs};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == MOE_DTYPE_F16) return launch_rows<F16>(a, rows, s);
+  if (dtype == MOE_DTYPE_BF16) return launch_rows<BF16>(a, rows, s);
+  return launch_rows<float>(a, rows, s);
+}

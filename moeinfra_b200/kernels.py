@@ -836,3 +836,37 @@ def _row_strides(t: torch.Tensor) -> tuple[int, int]:
     if t.shape[0] <= 1:
         row = max(t.shape[1], 1) * head
     return row, head
+
+
+@_on_device
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch.Tensor,
+                  top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor):
+    """``(tokens int64 [rows], probs fp32 [rows])``: one token per row of ``logits`` [rows, vocab].
+
+    ``logits`` fp16, bf16 or fp32 (rows may be strided, vocab <= 262144); ``uniforms`` fp32 [rows]
+    in [0, 1), the row's random number; ``temperature`` / ``top_p`` / ``min_p`` fp32 and ``top_k``
+    int32 [rows].  Temperature 0 takes the maximum (lowest index); top_k 0, top_p 1 and min_p 0 are
+    off; the filters apply in that order, top-p to what top-k leaves.  ``probs`` is the token's
+    share of what the filters leave.  The same row and numbers give the same token in any batch.
+    """
+    what = "sample_tokens"
+    if not isinstance(logits, torch.Tensor) or logits.ndim != 2:
+        raise ValueError(f"{what}: logits must be [rows, vocab]")
+    code = _DTYPE_CODES.get(logits.dtype)
+    if code is None:
+        raise ValueError(f"{what}: logits must be float16, bfloat16 or float32, got {logits.dtype}")
+    dev = logits.device
+    rows, vocab = logits.shape
+    f32 = torch.float32
+    _serve_check(what, dev, ("logits", logits, logits.dtype, logits.shape, 1),
+                 ("uniforms", uniforms, f32, (rows,), 1), ("temperature", temperature, f32, (rows,), 1),
+                 ("top_k", top_k, torch.int32, (rows,), 1), ("top_p", top_p, f32, (rows,), 1),
+                 ("min_p", min_p, f32, (rows,), 1))
+    tokens = torch.empty(rows, dtype=torch.int64, device=dev)
+    probs = torch.empty(rows, dtype=f32, device=dev)
+    check(_native.lib().moe_sample_tokens(
+        logits.data_ptr(), _outer_stride(logits), rows, vocab, code, uniforms.data_ptr(),
+        temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
+        tokens.data_ptr(), probs.data_ptr(), torch.cuda.current_stream(dev).cuda_stream),
+        "moe_sample_tokens")
+    return tokens, probs

@@ -66,3 +66,50 @@ def attention_bound(dtype: torch.dtype, out, weight, off):
     """
     u = ROUNDING[dtype]
     return u * out.abs() + (u + 2 * off + 2.0 ** -19) * weight + SMALLEST[dtype]
+
+
+def sample(x, u: float, temperature: float, top_k: int, top_p: float, min_p: float):
+    """One row of the sampler: (token, probability), in Python integers over float32 exponentials.
+
+    The definition's exponential is fp32's, which libraries round differently in the last place;
+    the third value says whether the token is sure all the same: every boundary it depends on is
+    further off than all weights moved by one part in 2^21 could carry it.
+    """
+    import math
+
+    import numpy as np
+
+    x = np.asarray(x, np.float32) + np.float32(0)
+    x = np.where(np.isnan(x), np.float32(-np.inf), x)
+    m = x.max()
+    order = sorted(range(len(x)), key=lambda i: (-x[i], i))
+    if not temperature > 0 or top_k == 1:
+        return order[0], 1.0, True
+    with np.errstate(invalid="ignore", over="ignore"):
+        d = np.where(x == m, np.float32(0), (x - m) / np.float32(temperature))
+    e = np.exp(d.astype(np.float64)).astype(np.float32)
+    w = [int(float(v) * 2.0 ** 40) for v in e]
+    kept = order[:top_k] if 0 < top_k < len(x) else order
+    sure = True
+    if np.float32(top_p) < 1:
+        total = sum(w[i] for i in kept)
+        need = max(1, min(total, math.ceil(float(np.float32(top_p)) * total)))
+        run, n = 0, 0
+        while run < need:
+            run += w[kept[n]]
+            n += 1
+        slack = total >> 21
+        sure &= run - need > slack and need - (run - w[kept[n - 1]]) > slack
+        kept = kept[:n]
+    lim = min(np.float32(min_p), np.float32(1))
+    sure &= all(abs(float(e[i]) - float(lim)) > 2e-6 * float(lim) for i in kept if e[i] != 1)
+    kept = sorted(i for i in kept if e[i] >= lim)
+    total = sum(w[i] for i in kept)
+    r = max(0, min(total - 1, math.floor(float(np.float32(u)) * total)))
+    run = 0
+    for i in kept:
+        if run + w[i] > r:
+            sure &= run + w[i] - r > (total >> 21) and (r - run > (total >> 21) or run == 0)
+            return i, w[i] / total, sure
+        run += w[i]
+    raise AssertionError("the sums cover every r")
