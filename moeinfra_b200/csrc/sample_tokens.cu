@@ -23,13 +23,17 @@
 // row is spread over a cluster of CTAs whose threads hold it in registers, as
 // integers of the same order ("keys"):
 //   * no sort: the k-th token and the top-p boundary are found by search over
-//     the keys, 8 ways a pass.  A pass adds each weight to the sums of the
-//     thresholds below it (21 instructions a logit), over the logits that are
-//     still between the bounds; register slots that hold none of these for a
-//     whole warp are skipped.  The first thresholds sit where a language
-//     model's boundary usually lies, 0.5 to 16 below the maximum in units of
-//     the temperature; correctness does not depend on them.
-//   * 16-bit logits have 16-bit keys: half the passes.
+//     the keys.  A pass sorts the logits between the bounds into 8 ways (it adds
+//     each weight to the sums of the thresholds below it, 21 instructions);
+//     register slots that hold none of these for a whole warp are skipped.  The
+//     first thresholds sit where a language model's boundary usually lies, 0.5
+//     to 16 below the maximum in units of the temperature.  Once at most 256
+//     logits are left between the bounds every CTA takes a copy of these and
+//     decides among them by itself.  Correctness depends on neither.
+//   * Exponentials are not kept: the first pass needs every logit's, what
+//     follows only those of the few between the bounds or kept.  That leaves 64
+//     registers a thread and two CTAs to an SM, one's barriers under the other's
+//     arithmetic.
 //   * Per pass one cluster barrier: warps reduce in two integer reductions of
 //     32 bits each, a CTA's sums go to every CTA of the cluster through
 //     distributed shared memory.
@@ -45,6 +49,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 16;            // 8 is the portable size; 16 only where a row needs it
 constexpr int kMaxPer = 32;                // logits a thread holds at most
+constexpr int kList = 256;                 // logits that a search finishes with directly
 constexpr int kMaxVocab = kMaxCluster * kThreads * kMaxPer;
 constexpr float kScale = 1099511627776.f;  // 2^40
 constexpr uint32_t kAll = 0xffffffffu;
@@ -148,39 +153,29 @@ struct Exchange {
     turn ^= 1;
     return s;
   }
-  __device__ __forceinline__ uint64_t max(uint64_t v) {  // of all threads, in every thread
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const uint64_t u = __shfl_xor_sync(kAll, v, o);
-      v = u > v ? u : v;
-    }
+  __device__ __forceinline__ uint32_t max(uint32_t v) {  // of all threads, in every thread
+    v = __reduce_max_sync(kAll, v);
     if (lane == 0) warp_sum[warp][0] = v;
     __syncthreads();
     if (warp == 0) {
-      v = warp_sum[lane & (kWarps - 1)][0];
-#pragma unroll
-      for (int o = kWarps / 2; o; o >>= 1) {
-        const uint64_t u = __shfl_xor_sync(kAll, v, o);
-        v = u > v ? u : v;
-      }
+      v = __reduce_max_sync(kAll, (uint32_t)warp_sum[lane & (kWarps - 1)][0]);
       if ((lane & 7) == 0) give(v);
     }
     cluster.sync();
-    v = slots[turn][0][0];
-    for (int r = 1; r < size; ++r) {
-      const uint64_t u = slots[turn][r][0];
-      v = u > v ? u : v;
-    }
+    v = __reduce_max_sync(kAll, lane < size ? (uint32_t)slots[turn][lane & (kMaxCluster - 1)][0] : 0u);
     turn ^= 1;
     return v;
   }
 };
 
 template <typename T, int PER>
-__global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const SampleArgs a) {
   using L = Logit<T>;
   constexpr int kVec = L::kVec, kIters = PER / kVec;
   __shared__ uint64_t s_warp[kWarps][8], s_slots[2][kMaxCluster][8];
+  __shared__ uint32_t s_list[kList], s_all[kList];
+  __shared__ uint64_t s_weight[kList], s_above;
+  __shared__ uint32_t s_count, s_key;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Exchange ex{cg::this_cluster(), 0, a.cluster, warp, lane, 0, s_warp, s_slots};
   ex.rank = blockIdx.x % a.cluster;
@@ -214,20 +209,20 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
   const float min_p = fminf(a.min_p[row], 1.f);  // above 1 the maxima stay
   const int k = a.top_k[row];
 
-  // ---- the maximum and its lowest index ----
-  uint64_t best = 0;
+  // ---- the maximum ----
+  uint32_t top = 0;
 #pragma unroll
-  for (int c = 0; c < PER; ++c) {
-    const uint32_t index = first + c / kVec * 32 * kVec + c % kVec;
-    const uint64_t v = (uint64_t)key[c] << 32 | (0xFFFFFFFFu - index);
-    best = v > best ? v : best;
-  }
+  for (int c = 0; c < PER; ++c) top = max(top, key[c]);
   ex.cluster.barrier_wait();
-  best = ex.max(best);
-  const uint32_t top = (uint32_t)(best >> 32);
-  if (!(temperature > 0.f) || k == 1) {
+  top = ex.max(top);
+  if (!(temperature > 0.f) || k == 1) {  // its lowest index
+    uint32_t index = 0xFFFFFFFFu;
+#pragma unroll
+    for (int c = PER - 1; c >= 0; --c)
+      if (key[c] == top) index = first + c / kVec * 32 * kVec + c % kVec;
+    index = ~ex.max(~index);
     if (ex.rank == 0 && threadIdx.x == 0) {
-      a.tokens[row] = 0xFFFFFFFFu - (uint32_t)best;
+      a.tokens[row] = index;
       a.probs[row] = 1.f;
     }
     return;
@@ -236,9 +231,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
   auto exp_of = [&](uint32_t key) {
     return key == top ? 1.f : key == 0 ? 0.f : expf(__fdiv_rn(L::value(key) - m, temperature));
   };
-  float e[PER];
-#pragma unroll
-  for (int c = 0; c < PER; ++c) e[c] = exp_of(key[c]);
+  if (threadIdx.x == 0) s_count = 0;
 
   // Sums of the weights (or counts) of the keys in [lo, hi) that are >= the
   // threshold t of lane 1 .. 7 (lane 0: >= t too), as lane j's result.
@@ -253,7 +246,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
 #pragma unroll
     for (int c = 0; c < PER; ++c) {
       if (!(used >> c & 1)) continue;
-      const uint64_t w = !(slots >> c & 1) ? 0ull : count ? 1ull : weight(e[c]);
+      const uint64_t w = !(slots >> c & 1) ? 0ull : count ? 1ull : weight(exp_of(key[c]));
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum[j] += key[c] >= th[j] ? w : 0ull;
     }
@@ -279,6 +272,61 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
         above = s_hi;
       }
       if (hi - lo <= 1) return Bound{lo, above};
+      // The logits between the bounds, if they are few, to every CTA.
+      uint32_t slots = 0;
+#pragma unroll
+      for (int c = 0; c < PER; ++c) slots |= (key[c] - lo < hi - lo ? 1u : 0u) << c;
+      const uint32_t used = __reduce_or_sync(kAll, slots);
+      uint64_t found[1] = {(uint64_t)__popc(slots)};
+      if (used) {
+        uint32_t at = 0;
+        if (slots) at = atomicAdd(&s_count, __popc(slots));
+#pragma unroll
+        for (int c = 0; c < PER; ++c)
+          if (slots >> c & 1) {
+            if (at < kList) s_list[at] = key[c];
+            ++at;
+          }
+      }
+      const uint64_t n = shfl64(ex.sum(found), 0);
+      if (n <= kList) {
+        int from = 0;
+        for (int r = 0; r < ex.size; ++r) {
+          const int held = (int)ex.slot(r, 0);
+          const uint32_t* list = ex.cluster.map_shared_rank(s_list, r);
+          for (int i = threadIdx.x; i < held; i += kThreads) {
+            const uint32_t kk = list[i];
+            s_all[from + i] = kk;
+            s_weight[from + i] = count ? 1ull : weight(exp_of(kk));
+          }
+          from += held;
+        }
+        if (threadIdx.x == 0) {
+          s_count = 0;
+          s_key = 0;
+        }
+        __syncthreads();
+        uint64_t over = 0, equal = 0;  // weights above and at the thread's key
+        uint32_t own = 0;
+        bool ok = false;
+        if (threadIdx.x < n) {
+          own = s_all[threadIdx.x];
+          for (int i = 0; i < (int)n; ++i) {
+            const uint32_t kk = s_all[i];
+            const uint64_t w = s_weight[i];
+            over += kk > own ? w : 0ull;
+            equal += kk == own ? w : 0ull;
+          }
+          ok = above + over + equal >= need;
+        }
+        const uint32_t found_key = __reduce_max_sync(kAll, ok ? own : 0u);
+        if (lane == 0 && found_key) atomicMax(&s_key, found_key);
+        __syncthreads();
+        if (threadIdx.x < n && own == s_key) s_above = above + over;  // the same value from each
+        __syncthreads();
+        return Bound{s_key, s_above};
+      }
+      if (threadIdx.x == 0) s_count = 0;  // read again after the next pass's barrier
       const uint32_t step = (hi - lo + 7) / 8;
       const uint64_t next = (uint64_t)lo + (uint64_t)step * (lane & 7);
       t = next < hi ? (uint32_t)next : hi;
@@ -319,15 +367,18 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
     cut = b.key;
   }
   // ---- what is kept, per warp and CTA ----
+  auto keeps = [&](uint32_t kk) {  // the weight of a key above the cut, if it is kept
+    const float e = exp_of(kk);
+    return e >= min_p ? weight(e) : 0ull;
+  };
   uint64_t sums[2] = {0, 0};
 #pragma unroll
   for (int c = 0; c < PER; ++c) {
-    if (key[c] > cut && e[c] >= min_p) sums[0] += weight(e[c]);
+    if (key[c] > cut) sums[0] += keeps(key[c]);
     if (key[c] == cut) ++sums[1];
   }
   ex.sum(sums);
-  const float e_cut = cut ? exp_of(cut) : 0.f;
-  const uint64_t w_cut = cut && e_cut >= min_p ? weight(e_cut) : 0ull;
+  const uint64_t w_cut = cut ? keeps(cut) : 0ull;
   auto kept = [&](uint64_t equal, uint64_t before) {  // of `equal` ties after `before` others
     return before >= ties ? 0ull : (ties - before < equal ? ties - before : equal);
   };
@@ -363,7 +414,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       const int c = i * kVec + j;
-      if (key[c] > cut && e[c] >= min_p) own += weight(e[c]);
+      if (key[c] > cut) own += keeps(key[c]);
       equal += key[c] == cut;
     }
     uint32_t equal_in = equal;
@@ -386,7 +437,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
         const int c = i * kVec + j;
-        uint64_t w = key[c] > cut && e[c] >= min_p ? weight(e[c]) : 0ull;
+        uint64_t w = key[c] > cut ? keeps(key[c]) : 0ull;
         if (key[c] == cut) {
           w = before < ties ? w_cut : 0ull;
           ++before;
@@ -432,9 +483,9 @@ int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t s) {
   return MOE_OK;
 }
 
-// CTAs of a row and logits of a thread: as many CTAs as give a thread 8 logits
-// while all rows' CTAs fit the GPU at once (two to an SM), else fewer and fuller
-// ones, whose passes have fewer barriers per logit.
+// CTAs of a row and logits of a thread: 8 logits, and so more CTAs, while all
+// rows' CTAs fit the GPU at once (two to an SM); else 16 (a cluster of up to 16
+// CTAs where a row needs it); 32 and one CTA to an SM for the longest rows.
 template <typename T>
 int launch_rows(SampleArgs& a, int64_t rows, cudaStream_t s) {
   int per = 8;
@@ -443,7 +494,8 @@ int launch_rows(SampleArgs& a, int64_t rows, cudaStream_t s) {
     while ((int64_t)c * kThreads * n < a.vocab) c *= 2;
     return c;
   };
-  while (per < kMaxPer && (ctas(per) > 8 || rows * ctas(per) > 2 * sm_count())) per *= 2;
+  if (ctas(8) > 8 || rows * ctas(8) > 2 * sm_count()) per = 16;
+  if (ctas(16) > kMaxCluster) per = 32;
   a.cluster = ctas(per);
   if (rows * a.cluster > INT32_MAX) return MOE_ERR_UNSUPPORTED;
   if (per == 8) return launch_sample<T, 8>(a, rows, s);
