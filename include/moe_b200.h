@@ -437,6 +437,8 @@ int moe_ep_return_partials_p2p(const float* y_part, int S, const int32_t* recv_c
  * p % page_size of page table[b][p / page_size].  Entries past a sequence's
  * last page are never read.  Two sequences may list the same page.
  *
+ * The entry points take their arguments as a structure of 8-byte fields, read
+ * before they return.
  * dtype: MOE_DTYPE_F16 or MOE_DTYPE_BF16; head_dim: 64 or 128; heads a
  * multiple of kv_heads (query head h reads KV head h / (heads / kv_heads)).
  * What is read from device memory (positions, sequence ids, pages, lengths,
@@ -444,7 +446,18 @@ int moe_ep_return_partials_p2p(const float* y_part, int S, const int32_t* recv_c
  * buffers and sets the device error word (MOE_ERR_PAGE from
  * moe_stream_check).
  *
- * moe_rope_append: rows of a fused q/k/v projection, [tokens, (heads + 2
+ */
+typedef struct moe_kv_pages {
+  uint16_t* k_pages;
+  uint16_t* v_pages;
+  int64_t k_page_stride, v_page_stride;
+  int64_t num_pages, kv_heads, page_size, head_dim;
+  int64_t dtype;
+  const int32_t* block_table;
+  int64_t table_stride, seqs, max_pages;
+} moe_kv_pages_t;
+
+/* moe_rope_append: rows of a fused q/k/v projection, [tokens, (heads + 2
  *   kv_heads) * head_dim], qkv_stride elements apart (a multiple of 8).
  *   Rotates q and k by the token's position p in fp32 (the two halves of a
  *   head are a pair: y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin; cos / sin
@@ -453,13 +466,21 @@ int moe_ep_return_partials_p2p(const float* y_part, int S, const int32_t* recv_c
  *   NULL: token t belongs to sequence t.  A token with a negative position is
  *   padding: a zero q row, nothing appended.
  */
-int moe_rope_append(const uint16_t* qkv, int64_t qkv_stride, const float* cos, const float* sin,
-                    int64_t max_pos, const int32_t* positions, const int32_t* seq_ids,
-                    int64_t tokens, uint16_t* k_pages, uint16_t* v_pages, int64_t k_page_stride,
-                    int64_t v_page_stride, int64_t num_pages, int page_size,
-                    const int32_t* block_table, int64_t table_stride, int seqs, int max_pages,
-                    int heads, int kv_heads, int head_dim, int dtype, uint16_t* q_out,
-                    void* stream);
+typedef struct moe_rope_append_args {
+  moe_kv_pages_t kv;
+  const uint16_t* qkv;
+  int64_t qkv_stride;
+  const float* cos;
+  const float* sin;
+  int64_t max_pos;
+  const int32_t* positions;
+  const int32_t* seq_ids; /* may be NULL */
+  int64_t tokens;
+  int64_t heads;
+  uint16_t* q_out;
+  void* stream;
+} moe_rope_append_args_t;
+int moe_rope_append(const moe_rope_append_args_t* args);
 
 /* moe_paged_attention: o[b,h] = softmax(scale q[b,h] . K_b^T) V_b over the
  *   first lengths[b] positions of sequence b (0: a row of zeros; the token
@@ -471,14 +492,21 @@ int moe_rope_append(const uint16_t* qkv, int64_t qkv_stride, const float* cos, c
  *   bytes of the workspace (counters) must be zero before its first call; every
  *   call leaves them zero, so a workspace serves calls of any shape it is large
  *   enough for, one after another.  Results do not vary from call to call. */
-size_t moe_paged_attention_workspace_size(int seqs, int max_pages, int page_size, int heads,
-                                          int kv_heads, int head_dim);
-int moe_paged_attention(const uint16_t* q, int64_t q_stride, uint16_t* k_pages,
-                        uint16_t* v_pages, int64_t k_page_stride, int64_t v_page_stride,
-                        int64_t num_pages, int page_size, const int32_t* block_table,
-                        int64_t table_stride, int seqs, int max_pages, const int32_t* lengths,
-                        int heads, int kv_heads, int head_dim, int dtype, float scale,
-                        uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
+typedef struct moe_paged_attention_args {
+  moe_kv_pages_t kv;
+  const uint16_t* q;
+  int64_t q_stride;
+  int64_t heads;
+  const int32_t* lengths;
+  double scale;
+  uint16_t* out;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} moe_paged_attention_args_t;
+size_t moe_paged_attention_workspace_size(int64_t seqs, int64_t max_pages, int64_t page_size,
+                                          int64_t heads, int64_t kv_heads, int64_t head_dim);
+int moe_paged_attention(const moe_paged_attention_args_t* args);
 
 /* moe_prompt_attention: o[t,h] = softmax(scale q[t,h] . K^T) V over t's own
  *   sequence, for packed sequences: sequence b's queries are rows
@@ -495,13 +523,23 @@ int moe_paged_attention(const uint16_t* q, int64_t q_stride, uint16_t* k_pages,
  *   scale > 0.  The workspace (counters) must be zero before its first call and
  *   is left zero, as moe_paged_attention's, which may be the same. */
 size_t moe_prompt_attention_workspace_size(void);
-int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t q_head_stride,
-                         int64_t q_rows, const uint16_t* k, int64_t k_stride,
-                         int64_t k_head_stride, const uint16_t* v, int64_t v_stride,
-                         int64_t v_head_stride, int64_t k_rows, const int32_t* cu_q,
-                         const int32_t* cu_k, int seqs, int max_q, int max_k, int heads,
-                         int kv_heads, int head_dim, int causal, int dtype, float scale,
-                         uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
+typedef struct moe_prompt_attention_args {
+  const uint16_t* q;
+  int64_t q_stride, q_head_stride, q_rows;
+  const uint16_t* k;
+  int64_t k_stride, k_head_stride;
+  const uint16_t* v;
+  int64_t v_stride, v_head_stride, k_rows;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int64_t seqs, max_q, max_k, heads, kv_heads, head_dim, causal, dtype;
+  double scale;
+  uint16_t* out;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} moe_prompt_attention_args_t;
+int moe_prompt_attention(const moe_prompt_attention_args_t* args);
 
 /* moe_sample_tokens: one token per row of logits [rows, vocab] (fp16, bf16 or
  *   fp32, rows stride elements apart, vocab <= 262144).  With m a row's maximum,
@@ -515,10 +553,19 @@ int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t q_head_str
  *   sum); probs[row] its share of that sum.  temperature <= 0 or top_k == 1: the
  *   lowest index of the maximum, probability 1.  Integer sums: the token depends
  *   on its row and numbers alone, not on the launch. */
-int moe_sample_tokens(const void* logits, int64_t stride, int64_t rows, int vocab, int dtype,
-                      const float* uniforms, const float* temperature, const int32_t* top_k,
-                      const float* top_p, const float* min_p, int64_t* tokens, float* probs,
-                      void* stream);
+typedef struct moe_sample_tokens_args {
+  const void* logits;
+  int64_t stride, rows, vocab, dtype;
+  const float* uniforms;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t* tokens;
+  float* probs;
+  void* stream;
+} moe_sample_tokens_args_t;
+int moe_sample_tokens(const moe_sample_tokens_args_t* args);
 
 #ifdef __cplusplus
 }

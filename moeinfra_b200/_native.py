@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
@@ -27,6 +28,15 @@ class NF4Matrix(ctypes.Structure):
 class NF4Expert(ctypes.Structure):
     _fields_ = [("w1", NF4Matrix), ("w3", NF4Matrix), ("w2", NF4Matrix)]
 
+
+# Argument structures of the serving operators, packed in one go: an entry point with some
+# twenty arguments costs ctypes ten times as long.  P: pointer, q: int64, d: double, in the
+# header's order; every field has 8 bytes.
+_KV_PAGES = "PPqqqqqqqPqqq"
+ROPE_APPEND = struct.Struct("@" + _KV_PAGES + "PqPPqPPqqPP")
+PAGED_ATTENTION = struct.Struct("@" + _KV_PAGES + "PqqPdPPqP")
+PROMPT_ATTENTION = struct.Struct("@PqqqPqqPqqqPPqqqqqqqqdPPqP")
+SAMPLE_TOKENS = struct.Struct("@PqqqqPPPPPPPP")
 
 # name -> (restype, argtypes); mirrors include/moe_b200.h one to one.
 SIGNATURES: dict[str, tuple] = {
@@ -92,22 +102,12 @@ SIGNATURES: dict[str, tuple] = {
     "moe_experts_forward_partials": (c_int, [ctypes.POINTER(NF4Expert), c_int, c_void_p, c_void_p,
                                              c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                              c_size_t, c_void_p]),
-    "moe_rope_append": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
-                                c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int,
-                                c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,
-                                c_void_p, c_void_p]),
-    "moe_paged_attention_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
-    "moe_paged_attention": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
-                                    c_int64, c_int, c_void_p, c_int64, c_int, c_int, c_void_p,
-                                    c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p,
-                                    c_size_t, c_void_p]),
-    "moe_prompt_attention": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64,
-                                     c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
-                                     c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                     c_int, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "moe_rope_append": (c_int, [c_void_p]),
+    "moe_paged_attention_workspace_size": (c_size_t, [c_int64] * 6),
+    "moe_paged_attention": (c_int, [c_void_p]),
     "moe_prompt_attention_workspace_size": (c_size_t, []),
-    "moe_sample_tokens": (c_int, [c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p,
-                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "moe_prompt_attention": (c_int, [c_void_p]),
+    "moe_sample_tokens": (c_int, [c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

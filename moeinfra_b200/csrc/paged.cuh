@@ -52,6 +52,29 @@ struct KvPages {
   int seqs, max_pages, page_size, kv_heads;
 };
 
+// The cache as a call describes it; MOE_OK, or what is wrong with it.
+inline int check_pages(const moe_kv_pages_t& c) {
+  if (c.seqs < 0 || c.seqs > INT32_MAX || c.max_pages < 0 || c.max_pages > INT32_MAX ||
+      c.kv_heads < 1 || c.kv_heads > 4096 ||
+      c.num_pages < 0 || c.page_size < 1 || c.page_size > (1 << 20))
+    return MOE_ERR_INVALID_ARG;
+  if ((c.dtype != MOE_DTYPE_F16 && c.dtype != MOE_DTYPE_BF16) ||
+      (c.head_dim != 64 && c.head_dim != 128) || c.max_pages * c.page_size > INT32_MAX)
+    return MOE_ERR_UNSUPPORTED;
+  const int64_t page = c.kv_heads * c.page_size * c.head_dim;
+  if (c.table_stride < c.max_pages ||
+      (c.num_pages > 1 && (c.k_page_stride < page || c.v_page_stride < page)))
+    return MOE_ERR_INVALID_ARG;
+  if (!aligned16(c.k_pages) || !aligned16(c.v_pages) || ((c.k_page_stride | c.v_page_stride) & 7))
+    return MOE_ERR_ALIGNMENT;
+  return MOE_OK;
+}
+inline KvPages pages_of(const moe_kv_pages_t& c) {
+  return KvPages{c.k_pages, c.v_pages, c.k_page_stride, c.v_page_stride, c.num_pages,
+                 c.block_table, c.table_stride, (int)c.seqs, (int)c.max_pages, (int)c.page_size,
+                 (int)c.kv_heads};
+}
+
 // d += a . b for one 16 x 8 x 16 tile, fp32 accumulation.
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,

@@ -637,67 +637,59 @@ int launch_wide(PagedArgs& a, const Shape& sh, cudaStream_t s) {
 }  // namespace
 }  // namespace moe
 
-extern "C" size_t moe_paged_attention_workspace_size(int seqs, int max_pages, int page_size,
-                                                     int heads, int kv_heads, int head_dim) {
+extern "C" size_t moe_paged_attention_workspace_size(int64_t seqs, int64_t max_pages,
+                                                     int64_t page_size, int64_t heads,
+                                                     int64_t kv_heads, int64_t head_dim) {
   using namespace moe;
   if (seqs < 1 || kv_heads < 1 || heads < kv_heads || max_pages < 0 || page_size < 1 ||
-      (head_dim != 64 && head_dim != 128))
+      (head_dim != 64 && head_dim != 128) || seqs > kMaxSeqs || heads > 4096)
     return 0;
-  const Shape sh = shape_of(seqs, kv_heads, heads / kv_heads, (int64_t)max_pages * page_size);
-  return workspace_size(sh, head_dim);
+  const Shape sh = shape_of(seqs, kv_heads, heads / kv_heads, max_pages * page_size);
+  return workspace_size(sh, static_cast<int>(head_dim));
 }
 
-extern "C" int moe_paged_attention(const uint16_t* q, int64_t q_stride, uint16_t* k_pages,
-                                   uint16_t* v_pages, int64_t k_page_stride,
-                                   int64_t v_page_stride, int64_t num_pages, int page_size,
-                                   const int32_t* block_table, int64_t table_stride, int seqs,
-                                   int max_pages, const int32_t* lengths, int heads, int kv_heads,
-                                   int head_dim, int dtype, float scale, uint16_t* out,
-                                   void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int moe_paged_attention(const moe_paged_attention_args_t* args) {
   using namespace moe;
-  if (seqs < 0 || max_pages < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || num_pages < 0 ||
-      page_size < 1 || !(scale > 0.f) || heads > 4096)
+  if (!args) return MOE_ERR_INVALID_ARG;
+  const moe_paged_attention_args_t& c = *args;
+  if (const int st = check_pages(c.kv); st != MOE_OK) return st;
+  const int64_t hd = c.kv.head_dim;
+  const float scale = static_cast<float>(c.scale);
+  if (c.heads < 1 || c.heads > 4096 || c.heads % c.kv.kv_heads || !(scale > 0.f && scale < INFINITY) ||
+      c.q_stride < c.heads * hd)
     return MOE_ERR_INVALID_ARG;
-  if (dtype != MOE_DTYPE_F16 && dtype != MOE_DTYPE_BF16) return MOE_ERR_UNSUPPORTED;
-  if ((head_dim != 64 && head_dim != 128) || page_size % kChunk || seqs > kMaxSeqs)
-    return MOE_ERR_UNSUPPORTED;
-  const int64_t page_elems = (int64_t)kv_heads * page_size * head_dim;
-  if (q_stride < (int64_t)heads * head_dim || table_stride < max_pages ||
-      (num_pages > 1 && (k_page_stride < page_elems || v_page_stride < page_elems)))
+  if (c.kv.page_size % kChunk || c.kv.seqs > kMaxSeqs) return MOE_ERR_UNSUPPORTED;
+  if (c.kv.seqs == 0) return MOE_OK;
+  if (!c.q || !c.lengths || !c.out ||
+      (c.kv.max_pages > 0 &&
+       (!c.kv.k_pages || !c.kv.v_pages || !c.kv.block_table || c.kv.num_pages < 1)))
     return MOE_ERR_INVALID_ARG;
-  if (seqs == 0) return MOE_OK;
-  if (!q || !lengths || !out || (max_pages > 0 && (!k_pages || !v_pages || !block_table || num_pages < 1)))
-    return MOE_ERR_INVALID_ARG;
-  if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) ||
-      (q_stride & 7) || (k_page_stride & 7) || (v_page_stride & 7))
-    return MOE_ERR_ALIGNMENT;
-  const Shape sh = shape_of(seqs, kv_heads, heads / kv_heads, (int64_t)max_pages * page_size);
-  // Chunk numbers are 32-bit on the device.
-  if ((int64_t)max_pages * page_size > INT32_MAX || sh.units * sh.chunks > INT32_MAX)
-    return MOE_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < workspace_size(sh, head_dim))
+  if (!aligned16(c.q) || !aligned16(c.out) || (c.q_stride & 7)) return MOE_ERR_ALIGNMENT;
+  const Shape sh = shape_of(c.kv.seqs, static_cast<int>(c.kv.kv_heads),
+                            static_cast<int>(c.heads / c.kv.kv_heads), c.kv.max_pages * c.kv.page_size);
+  if (sh.units * sh.chunks > INT32_MAX) return MOE_ERR_UNSUPPORTED;  // 32-bit on the device
+  if (!c.workspace || c.workspace_bytes < (int64_t)workspace_size(sh, static_cast<int>(hd)))
     return MOE_ERR_WORKSPACE;
-  if (!aligned16(workspace)) return MOE_ERR_ALIGNMENT;
+  if (!aligned16(c.workspace)) return MOE_ERR_ALIGNMENT;
   PagedArgs a{};
-  a.q = q;
-  a.q_stride = q_stride;
-  a.out = out;
-  a.lengths = lengths;
-  a.kv = KvPages{k_pages, v_pages, k_page_stride, v_page_stride, num_pages, block_table,
-                 table_stride, seqs, max_pages, page_size, kv_heads};
+  a.q = c.q;
+  a.q_stride = c.q_stride;
+  a.out = c.out;
+  a.lengths = c.lengths;
+  a.kv = pages_of(c.kv);
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.heads = heads;
-  a.per_seq = kv_heads * sh.parts;
+  a.heads = static_cast<int>(c.heads);
+  a.per_seq = static_cast<int>(c.kv.kv_heads) * sh.parts;
   a.tile = sh.tile;
   a.parts = sh.parts;
-  a.page_chunks = page_size / kChunk;
+  a.page_chunks = a.kv.page_size / kChunk;
   a.page_shift = -1;
   for (int i = 0; i < 27; ++i)
     if (a.page_chunks == 1 << i) a.page_shift = i;
-  a.counts = static_cast<int*>(workspace);
-  a.warp_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCountBytes);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == MOE_DTYPE_F16)
-    return head_dim == 64 ? launch_wide<F16, 64>(a, sh, s) : launch_wide<F16, 128>(a, sh, s);
-  return head_dim == 64 ? launch_wide<BF16, 64>(a, sh, s) : launch_wide<BF16, 128>(a, sh, s);
+  a.counts = static_cast<int*>(c.workspace);
+  a.warp_part = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + kCountBytes);
+  cudaStream_t s = static_cast<cudaStream_t>(c.stream);
+  if (c.kv.dtype == MOE_DTYPE_F16)
+    return hd == 64 ? launch_wide<F16, 64>(a, sh, s) : launch_wide<F16, 128>(a, sh, s);
+  return hd == 64 ? launch_wide<BF16, 64>(a, sh, s) : launch_wide<BF16, 128>(a, sh, s);
 }

@@ -718,72 +718,77 @@ bool bad_strides(int64_t row, int64_t head, int64_t heads, int64_t hd) {
 
 extern "C" size_t moe_prompt_attention_workspace_size(void) { return 16; }
 
-extern "C" int moe_prompt_attention(const uint16_t* q, int64_t q_stride, int64_t q_head_stride,
-                                    int64_t q_rows, const uint16_t* k, int64_t k_stride,
-                                    int64_t k_head_stride, const uint16_t* v, int64_t v_stride,
-                                    int64_t v_head_stride, int64_t k_rows, const int32_t* cu_q,
-                                    const int32_t* cu_k, int seqs, int max_q, int max_k, int heads,
-                                    int kv_heads, int head_dim, int causal, int dtype, float scale,
-                                    uint16_t* out, void* workspace, size_t workspace_bytes,
-                                    void* stream) {
+extern "C" int moe_prompt_attention(const moe_prompt_attention_args_t* args) {
   using namespace moe;
-  if (q_rows < 0 || k_rows < 0 || q_rows > INT32_MAX - 256 || k_rows > INT32_MAX - 256 || seqs < 0 ||
-      max_q < 0 || max_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || !(scale > 0.f))
+  if (!args) return MOE_ERR_INVALID_ARG;
+  const moe_prompt_attention_args_t& c = *args;
+  const float scale = static_cast<float>(c.scale);
+  // Rows, and so offsets and coordinates of a tile past the end, are 32-bit.
+  constexpr int64_t kMostRows = INT32_MAX - 256;
+  if (c.q_rows < 0 || c.k_rows < 0 || c.q_rows > kMostRows || c.k_rows > kMostRows || c.seqs < 0 ||
+      c.max_q < 0 || c.max_k < 0 || c.max_q > INT32_MAX || c.max_k > INT32_MAX || c.heads < 1 ||
+      c.heads > 4096 || c.kv_heads < 1 || c.heads % c.kv_heads || !(scale > 0.f && scale < INFINITY))
     return MOE_ERR_INVALID_ARG;
-  if (dtype != MOE_DTYPE_F16 && dtype != MOE_DTYPE_BF16) return MOE_ERR_UNSUPPORTED;
-  if (head_dim != 64 && head_dim != 128) return MOE_ERR_UNSUPPORTED;
-  if (bad_strides(q_stride, q_head_stride, heads, head_dim) ||
-      bad_strides(k_stride, k_head_stride, kv_heads, head_dim) ||
-      bad_strides(v_stride, v_head_stride, kv_heads, head_dim))
+  if (c.dtype != MOE_DTYPE_F16 && c.dtype != MOE_DTYPE_BF16) return MOE_ERR_UNSUPPORTED;
+  if (c.head_dim != 64 && c.head_dim != 128) return MOE_ERR_UNSUPPORTED;
+  const int hd = static_cast<int>(c.head_dim), heads = static_cast<int>(c.heads);
+  const int kv_heads = static_cast<int>(c.kv_heads);
+  if (bad_strides(c.q_stride, c.q_head_stride, heads, hd) ||
+      bad_strides(c.k_stride, c.k_head_stride, kv_heads, hd) ||
+      bad_strides(c.v_stride, c.v_head_stride, kv_heads, hd))
     return MOE_ERR_INVALID_ARG;
-  if (q_rows == 0 || seqs == 0 || max_q == 0) return MOE_OK;
-  if (ceil_div(max_q, 16) * seqs * heads > INT32_MAX) return MOE_ERR_UNSUPPORTED;
-  if (!q || !cu_q || !cu_k || !out || (k_rows > 0 && (!k || !v))) return MOE_ERR_INVALID_ARG;
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) ||
-      ((q_stride | q_head_stride | k_stride | k_head_stride | v_stride | v_head_stride) & 7))
+  if (c.q_rows == 0 || c.seqs == 0 || c.max_q == 0) return MOE_OK;
+  if (c.seqs > INT32_MAX / heads || ceil_div(c.max_q, 16) > INT32_MAX / (c.seqs * heads))
+    return MOE_ERR_UNSUPPORTED;
+  if (!c.q || !c.cu_q || !c.cu_k || !c.out || (c.k_rows > 0 && (!c.k || !c.v)))
+    return MOE_ERR_INVALID_ARG;
+  if (!aligned16(c.q) || !aligned16(c.k) || !aligned16(c.v) || !aligned16(c.out) ||
+      ((c.q_stride | c.q_head_stride | c.k_stride | c.k_head_stride | c.v_stride | c.v_head_stride) & 7))
     return MOE_ERR_ALIGNMENT;
-  if (!workspace || workspace_bytes < moe_prompt_attention_workspace_size())
+  if (!c.workspace || c.workspace_bytes < (int64_t)moe_prompt_attention_workspace_size())
     return MOE_ERR_WORKSPACE;
-  if (!aligned16(workspace)) return MOE_ERR_ALIGNMENT;
-  const bool bf16 = dtype == MOE_DTYPE_BF16;
-  CUtensorMap mq, mk, mv;
-  // Without any key no K or V tile is loaded: the maps then describe q.
-  const bool none = k_rows == 0;
+  if (!aligned16(c.workspace)) return MOE_ERR_ALIGNMENT;
+  const bool bf16 = c.dtype == MOE_DTYPE_BF16;
+  // Heads that share a tile's rows: see the kernel.
   int pack = 0;
   while (pack < 4 && heads / kv_heads % (2 << pack) == 0) ++pack;
-  const int keys = head_dim == 64 ? Cfg<64>::kN : Cfg<128>::kN;
-  CUtensorMap mo;  // a warp's rows of the output: 32 / P tokens x P heads
-  if (!make_map(&mo, out, q_rows, heads, head_dim, (int64_t)heads * head_dim, head_dim, bf16,
-                32 >> pack, 1 << pack))
-    return MOE_ERR_CUDA;
-  if (!make_map(&mq, q, q_rows, heads, head_dim, q_stride, q_head_stride, bf16, kM >> pack,
+  const int keys = hd == 64 ? Cfg<64>::kN : Cfg<128>::kN;
+  // Without any key no K or V tile is loaded: the maps then describe q.
+  const bool none = c.k_rows == 0;
+  const uint16_t *k = none ? c.q : c.k, *v = none ? c.q : c.v;
+  const int64_t k_rows = none ? c.q_rows : c.k_rows;
+  const int map_heads = none ? heads : kv_heads;
+  CUtensorMap mq, mk, mv, mo;  // mo: a warp's rows of the output, 32 / P tokens x P heads
+  if (!make_map(&mq, c.q, c.q_rows, heads, hd, c.q_stride, c.q_head_stride, bf16, kM >> pack,
                 1 << pack) ||
-      !make_map(&mk, none ? q : k, none ? q_rows : k_rows, none ? heads : kv_heads, head_dim,
-                none ? q_stride : k_stride, none ? q_head_stride : k_head_stride, bf16, keys, 1) ||
-      !make_map(&mv, none ? q : v, none ? q_rows : k_rows, none ? heads : kv_heads, head_dim,
-                none ? q_stride : v_stride, none ? q_head_stride : v_head_stride, bf16, keys, 1))
+      !make_map(&mk, k, k_rows, map_heads, hd, none ? c.q_stride : c.k_stride,
+                none ? c.q_head_stride : c.k_head_stride, bf16, keys, 1) ||
+      !make_map(&mv, v, k_rows, map_heads, hd, none ? c.q_stride : c.v_stride,
+                none ? c.q_head_stride : c.v_head_stride, bf16, keys, 1) ||
+      !make_map(&mo, c.out, c.q_rows, heads, hd, (int64_t)heads * hd, hd, bf16, 32 >> pack,
+                1 << pack))
     return MOE_ERR_CUDA;
   PromptArgs a{};
-  a.cu_q = cu_q;
-  a.cu_k = cu_k;
-  a.rows_q = q_rows;
-  a.rows_k = k_rows;
-  a.seqs = seqs;
+  a.cu_q = c.cu_q;
+  a.cu_k = c.cu_k;
+  a.rows_q = c.q_rows;
+  a.rows_k = c.k_rows;
+  a.seqs = static_cast<int>(c.seqs);
   a.heads = heads;
   a.group = heads / kv_heads;
-  a.max_q = max_q;
-  a.max_k = max_k;
+  a.max_q = static_cast<int>(c.max_q);
+  a.max_k = static_cast<int>(c.max_k);
   a.pack = pack;
-  a.blocks = static_cast<int>(ceil_div(max_q, 2 * kM >> pack));
-  a.causal = causal != 0;
+  a.blocks = static_cast<int>(ceil_div(c.max_q, 2 * kM >> pack));
+  a.causal = c.causal != 0;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.out = out;
-  a.counts = static_cast<uint32_t*>(workspace);
+  a.out = c.out;
+  a.counts = static_cast<uint32_t*>(c.workspace);
   a.wait_ns = wait_limit_ns();
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaStream_t s = static_cast<cudaStream_t>(c.stream);
   if (bf16)
-    return head_dim == 64 ? launch_prompt<BF16, 64>(a, mq, mk, mv, mo, s)
-                          : launch_prompt<BF16, 128>(a, mq, mk, mv, mo, s);
-  return head_dim == 64 ? launch_prompt<F16, 64>(a, mq, mk, mv, mo, s)
-                        : launch_prompt<F16, 128>(a, mq, mk, mv, mo, s);
+    return hd == 64 ? launch_prompt<BF16, 64>(a, mq, mk, mv, mo, s)
+                    : launch_prompt<BF16, 128>(a, mq, mk, mv, mo, s);
+  return hd == 64 ? launch_prompt<F16, 64>(a, mq, mk, mv, mo, s)
+                  : launch_prompt<F16, 128>(a, mq, mk, mv, mo, s);
 }

@@ -106,37 +106,27 @@ int launch_rope(const RopeArgs& a, int64_t tokens, cudaStream_t s) {
 }  // namespace
 }  // namespace moe
 
-extern "C" int moe_rope_append(const uint16_t* qkv, int64_t qkv_stride, const float* cos,
-                               const float* sin, int64_t max_pos, const int32_t* positions,
-                               const int32_t* seq_ids, int64_t tokens, uint16_t* k_pages,
-                               uint16_t* v_pages, int64_t k_page_stride, int64_t v_page_stride,
-                               int64_t num_pages, int page_size, const int32_t* block_table,
-                               int64_t table_stride, int seqs, int max_pages, int heads,
-                               int kv_heads, int head_dim, int dtype, uint16_t* q_out,
-                               void* stream) {
+extern "C" int moe_rope_append(const moe_rope_append_args_t* args) {
   using namespace moe;
-  if (tokens < 0 || tokens > INT32_MAX || seqs < 0 || max_pages < 0 || heads < 1 || kv_heads < 1 ||
-      heads > 1024 || kv_heads > 1024 || num_pages < 0 || max_pos < 0 || max_pos > INT32_MAX || page_size < 1)
+  if (!args) return MOE_ERR_INVALID_ARG;
+  const moe_rope_append_args_t& c = *args;
+  if (const int st = check_pages(c.kv); st != MOE_OK) return st;
+  if (c.tokens < 0 || c.tokens > INT32_MAX || c.heads < 1 || c.heads > 4096 || c.max_pos < 0 ||
+      c.max_pos > INT32_MAX || c.qkv_stride < (c.heads + 2 * c.kv.kv_heads) * c.kv.head_dim)
     return MOE_ERR_INVALID_ARG;
-  if (dtype != MOE_DTYPE_F16 && dtype != MOE_DTYPE_BF16) return MOE_ERR_UNSUPPORTED;
-  if (head_dim != 64 && head_dim != 128) return MOE_ERR_UNSUPPORTED;
-  const int64_t page_elems = (int64_t)kv_heads * page_size * head_dim;
-  if (qkv_stride < (int64_t)(heads + 2 * kv_heads) * head_dim || table_stride < max_pages ||
-      (num_pages > 1 && (k_page_stride < page_elems || v_page_stride < page_elems)))
+  if (c.tokens == 0) return MOE_OK;
+  if (!c.qkv || !c.cos || !c.sin || !c.positions || !c.kv.k_pages || !c.kv.v_pages ||
+      !c.kv.block_table || !c.q_out)
     return MOE_ERR_INVALID_ARG;
-  if (tokens == 0) return MOE_OK;
-  if (!qkv || !cos || !sin || !positions || !k_pages || !v_pages || !block_table || !q_out)
-    return MOE_ERR_INVALID_ARG;
-  if (!aligned16(qkv) || !aligned16(cos) || !aligned16(sin) || !aligned16(k_pages) ||
-      !aligned16(v_pages) || !aligned16(q_out) || (qkv_stride & 7) || (k_page_stride & 7) ||
-      (v_page_stride & 7))
+  if (!aligned16(c.qkv) || !aligned16(c.cos) || !aligned16(c.sin) || !aligned16(c.q_out) ||
+      (c.qkv_stride & 7))
     return MOE_ERR_ALIGNMENT;
-  RopeArgs a{qkv, qkv_stride, cos, sin, max_pos, positions, seq_ids,
-             KvPages{k_pages, v_pages, k_page_stride, v_page_stride, num_pages, block_table,
-                     table_stride, seqs, max_pages, page_size, kv_heads},
-             q_out, heads};
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == MOE_DTYPE_F16)
-    return head_dim == 64 ? launch_rope<F16, 64>(a, tokens, s) : launch_rope<F16, 128>(a, tokens, s);
-  return head_dim == 64 ? launch_rope<BF16, 64>(a, tokens, s) : launch_rope<BF16, 128>(a, tokens, s);
+  const RopeArgs a{c.qkv, c.qkv_stride, c.cos, c.sin, c.max_pos, c.positions, c.seq_ids,
+                   pages_of(c.kv), c.q_out, (int)c.heads};
+  cudaStream_t s = static_cast<cudaStream_t>(c.stream);
+  if (c.kv.dtype == MOE_DTYPE_F16)
+    return c.kv.head_dim == 64 ? launch_rope<F16, 64>(a, c.tokens, s)
+                               : launch_rope<F16, 128>(a, c.tokens, s);
+  return c.kv.head_dim == 64 ? launch_rope<BF16, 64>(a, c.tokens, s)
+                             : launch_rope<BF16, 128>(a, c.tokens, s);
 }

@@ -506,21 +506,22 @@ int launch_rows(SampleArgs& a, int64_t rows, cudaStream_t s) {
 }  // namespace
 }  // namespace moe
 
-extern "C" int moe_sample_tokens(const void* logits, int64_t stride, int64_t rows, int vocab,
-                                 int dtype, const float* uniforms, const float* temperature,
-                                 const int32_t* top_k, const float* top_p, const float* min_p,
-                                 int64_t* tokens, float* probs, void* stream) {
+extern "C" int moe_sample_tokens(const moe_sample_tokens_args_t* args) {
   using namespace moe;
-  if (rows < 0 || vocab < 1 || (rows > 1 && stride < vocab)) return MOE_ERR_INVALID_ARG;
-  if (dtype != MOE_DTYPE_F16 && dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F32)
+  if (!args) return MOE_ERR_INVALID_ARG;
+  const moe_sample_tokens_args_t& c = *args;
+  if (c.rows < 0 || c.vocab < 1 || (c.rows > 1 && c.stride < c.vocab)) return MOE_ERR_INVALID_ARG;
+  if (c.dtype != MOE_DTYPE_F16 && c.dtype != MOE_DTYPE_BF16 && c.dtype != MOE_DTYPE_F32)
     return MOE_ERR_UNSUPPORTED;
-  if (vocab > kMaxVocab) return MOE_ERR_UNSUPPORTED;
-  if (rows == 0) return MOE_OK;
-  if (!logits || !uniforms || !temperature || !top_k || !top_p || !min_p || !tokens || !probs)
+  if (c.vocab > kMaxVocab) return MOE_ERR_UNSUPPORTED;
+  if (c.rows == 0) return MOE_OK;
+  if (!c.logits || !c.uniforms || !c.temperature || !c.top_k || !c.top_p || !c.min_p ||
+      !c.tokens || !c.probs)
     return MOE_ERR_INVALID_ARG;
-  SampleArgs a{logits, stride, vocab, 1, uniforms, temperature, top_p, min_p, top_k, tokens, probs};
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == MOE_DTYPE_F16) return launch_rows<F16>(a, rows, s);
-  if (dtype == MOE_DTYPE_BF16) return launch_rows<BF16>(a, rows, s);
-  return launch_rows<float>(a, rows, s);
+  SampleArgs a{c.logits,      c.stride, (int)c.vocab, 1,       c.uniforms, c.temperature,
+               c.top_p,       c.min_p,  c.top_k,      c.tokens, c.probs};
+  cudaStream_t s = static_cast<cudaStream_t>(c.stream);
+  if (c.dtype == MOE_DTYPE_F16) return launch_rows<F16>(a, c.rows, s);
+  if (c.dtype == MOE_DTYPE_BF16) return launch_rows<BF16>(a, c.rows, s);
+  return launch_rows<float>(a, c.rows, s);
 }

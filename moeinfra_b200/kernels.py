@@ -587,15 +587,41 @@ def ep_return_partials_p2p(y_part: torch.Tensor, recv_counts: torch.Tensor, num_
 
 # ---------------------------------------------------------------------------
 # Ragged, paged serving: rotation + cache append, attention, sampling
+#
+# A call on one new token is a few microseconds on the GPU, so the wrappers check the usual form
+# (packed tensors of one device) in one expression and go through the detailed checks, which
+# name what is wrong or accept strided rows, only where that fails.
 # ---------------------------------------------------------------------------
 
 _DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 PROMPT_WORKSPACE_BYTES = 16
 _COUNTER_BYTES = 4096  # the part of a workspace that has to be zero before its first call
 _serve_ws: dict = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_HALVES = (torch.float16, torch.bfloat16)
 
 
-def _serve_scratch(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+def _plain(dev: int, dtype: torch.dtype, *tensors) -> bool:
+    """Whether all are packed tensors of one type on GPU ``dev``."""
+    for t in tensors:
+        if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+            return False
+    return dev >= 0
+
+
+def _on_first_device(fn):
+    """As :func:`_on_device`, by the device of the first argument alone."""
+    @functools.wraps(fn)
+    def wrapper(first, *args, **kwargs):
+        dev = first.get_device() if isinstance(first, torch.Tensor) else -1
+        if dev < 0 or dev == torch.cuda.current_device():
+            return fn(first, *args, **kwargs)
+        with torch.cuda.device(dev):
+            return fn(first, *args, **kwargs)
+    return wrapper
+
+
+def _serve_scratch(dev: int, stream: int, nbytes: int) -> torch.Tensor:
     """Scratch of the serving operators, its leading counters zeroed (every call leaves them so).
 
     One buffer per (device, stream, power of two), kept: calls on one stream are ordered and
@@ -604,19 +630,20 @@ def _serve_scratch(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     replayed side by side.
     """
     if torch.cuda.is_current_stream_capturing():
-        ws = _workspace(nbytes, dev)
+        ws = _workspace(max(nbytes, _COUNTER_BYTES), torch.device("cuda", dev))
         ws[:_COUNTER_BYTES].zero_()
         return ws
-    key = (dev.index, stream, max(nbytes - 1, 0).bit_length())
+    key = (dev, stream, max(nbytes - 1, _COUNTER_BYTES - 1).bit_length())
     ws = _serve_ws.get(key)
     if ws is None:
-        ws = _serve_ws[key] = torch.zeros(1 << key[2], dtype=torch.uint8, device=dev)
+        ws = _serve_ws[key] = torch.zeros(1 << key[2], dtype=torch.uint8,
+                                          device=torch.device("cuda", dev))
     return ws
 
 
-def _serve_check(what: str, dev: torch.device, *named) -> None:
-    """Each of ``named`` = (name, tensor, dtype, shape, contiguous dims): the last so many
-    dimensions packed; None in a shape is any size."""
+def _serve_check(what: str, dev: int, *named) -> None:
+    """Each of ``named`` = (name, tensor, dtype, shape, packed): dtype and shape as given (None: any
+    size), the last ``packed`` dimensions contiguous, on GPU ``dev``."""
     for name, t, dtype, shape, packed in named:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: {name} must be a torch.Tensor")
@@ -624,18 +651,15 @@ def _serve_check(what: str, dev: torch.device, *named) -> None:
             raise RuntimeError(
                 f"{what}: {name} is on {t.device}; the B200 kernels run on CUDA tensors only "
                 "(there is no CPU path)")
-        if t.device != dev:
-            raise ValueError(f"{what}: {name} is on {t.device}, expected {dev}")
+        if t.get_device() != dev:
+            raise ValueError(f"{what}: {name} is on {t.device}, expected cuda:{dev}")
         if t.dtype is not dtype:
             raise ValueError(f"{what}: {name} must be {dtype}, got {t.dtype}")
         size = t.shape
         if len(size) != len(shape) or any(w is not None and w != n for w, n in zip(shape, size)):
             want = ", ".join("*" if w is None else str(w) for w in shape)
             raise ValueError(f"{what}: {name} must be [{want}], got {tuple(size)}")
-        if t.is_contiguous():
-            continue
-        run = 1
-        stride = t.stride()
+        run, stride = 1, t.stride()
         for i in range(len(size) - 1, len(size) - 1 - packed, -1):
             if size[i] != 1 and stride[i] != run:
                 raise ValueError(f"{what}: {name} must be contiguous in its last {packed} "
@@ -643,27 +667,34 @@ def _serve_check(what: str, dev: torch.device, *named) -> None:
             run *= size[i]
 
 
-def _page_geometry(what: str, k_pages, v_pages, block_table):
-    """(dtype, num_pages, kv_heads, page_size, head_dim) of a paged cache."""
-    if not isinstance(k_pages, torch.Tensor) or k_pages.ndim != 4:
-        raise ValueError(f"{what}: k_pages must be [pages, kv_heads, page_size, head_dim]")
-    if k_pages.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"{what}: k_pages must be float16 or bfloat16, got {k_pages.dtype}")
-    n, kv, page, hd = shape = k_pages.shape
-    dev, dt = k_pages.device, k_pages.dtype
-    _serve_check(what, dev, ("k_pages", k_pages, dt, shape, 3), ("v_pages", v_pages, dt, shape, 3),
-                 ("block_table", block_table, torch.int32, (None, None), 1))
-    if hd not in (64, 128):
-        raise ValueError(f"{what}: head_dim must be 64 or 128, got {hd}")
-    return dt, n, kv, page, hd
-
-
 def _outer_stride(t: torch.Tensor) -> int:
     """Elements from one index of the first dimension to the next (packed when there is one)."""
     return t.stride(0) if t.shape[0] > 1 else t.numel()
 
 
-@_on_device
+def _row_strides(t: torch.Tensor) -> tuple[int, int]:
+    """Strides of [rows, heads, hd] in elements (packed where a dimension has one entry)."""
+    row, head, _ = t.stride()
+    if t.shape[1] <= 1:
+        head = t.shape[2]
+    if t.shape[0] <= 1:
+        row = max(t.shape[1], 1) * head
+    return row, head
+
+
+def _check_cache(what: str, k_pages, v_pages, block_table) -> None:
+    if not isinstance(k_pages, torch.Tensor) or k_pages.ndim != 4:
+        raise ValueError(f"{what}: k_pages must be [pages, kv_heads, page_size, head_dim]")
+    if k_pages.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{what}: k_pages must be float16 or bfloat16, got {k_pages.dtype}")
+    dev, dt, shape = k_pages.get_device(), k_pages.dtype, k_pages.shape
+    _serve_check(what, dev, ("k_pages", k_pages, dt, shape, 3), ("v_pages", v_pages, dt, shape, 3),
+                 ("block_table", block_table, torch.int32, (None, None), 1))
+    if shape[3] not in (64, 128):
+        raise ValueError(f"{what}: head_dim must be 64 or 128, got {shape[3]}")
+
+
+@_on_first_device
 def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
                 block_table: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                 num_heads: int, seq_ids: torch.Tensor | None = None,
@@ -679,31 +710,52 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positio
     nothing and shows in :func:`check_device`.
     """
     what = "rope_append"
-    dt, n_pages, kv, page, hd = _page_geometry(what, k_pages, v_pages, block_table)
-    dev = k_pages.device
-    _serve_check(what, dev, ("qkv", qkv, dt, (None, (num_heads + 2 * kv) * hd), 1),
-                 ("positions", positions, torch.int32, (None,), 1),
-                 ("cos", cos, torch.float32, (None, hd // 2), 2),
-                 ("sin", sin, torch.float32, tuple(cos.shape), 2))
-    T = qkv.shape[0]
-    if positions.shape[0] != T:
-        raise ValueError(f"{what}: positions must be [{T}], got {tuple(positions.shape)}")
-    seqs, max_pages = block_table.shape
-    if seq_ids is not None:
-        _serve_check(what, dev, ("seq_ids", seq_ids, torch.int32, (T,), 1))
-    elif seqs < T:
+    try:
+        n_pages, kv, page, hd = k_pages.shape
+        T, width = qkv.shape
+        max_pos, half = cos.shape
+        seqs, max_pages = block_table.shape
+        dt, dev = k_pages.dtype, k_pages.get_device()
+        plain = (dt in _HALVES and (hd == 64 or hd == 128) and half * 2 == hd
+                 and width == (num_heads + 2 * kv) * hd and sin.shape == cos.shape
+                 and v_pages.shape == k_pages.shape and positions.shape == (T,)
+                 and _plain(dev, dt, qkv, k_pages, v_pages)
+                 and _plain(dev, torch.float32, cos, sin)
+                 and _plain(dev, torch.int32, positions, block_table)
+                 and (seq_ids is None or seq_ids.shape == (T,) and _plain(dev, torch.int32, seq_ids)))
+    except (AttributeError, ValueError):
+        plain = False
+    if not plain:
+        _check_cache(what, k_pages, v_pages, block_table)
+        n_pages, kv, page, hd = k_pages.shape
+        dt, dev = k_pages.dtype, k_pages.get_device()
+        _serve_check(what, dev, ("qkv", qkv, dt, (None, (num_heads + 2 * kv) * hd), 1),
+                     ("cos", cos, torch.float32, (None, hd // 2), 2))
+        T, max_pos = qkv.shape[0], cos.shape[0]
+        _serve_check(what, dev, ("positions", positions, torch.int32, (T,), 1),
+                     ("sin", sin, torch.float32, cos.shape, 2))
+        if seq_ids is not None:
+            _serve_check(what, dev, ("seq_ids", seq_ids, torch.int32, (T,), 1))
+        seqs, max_pages = block_table.shape
+    if seq_ids is None and seqs < T:
         raise ValueError(f"{what}: block_table has {seqs} sequences for {T} tokens")
     if out is None:
-        out = torch.empty((T, num_heads, hd), dtype=dt, device=dev)
+        out = qkv.new_empty((T, num_heads, hd))
     else:
         _serve_check(what, dev, ("out", out, dt, (T, num_heads, hd), 3))
-    check(_native.lib().moe_rope_append(
-        qkv.data_ptr(), _outer_stride(qkv) if T else qkv.shape[1], cos.data_ptr(), sin.data_ptr(),
-        cos.shape[0], positions.data_ptr(), None if seq_ids is None else seq_ids.data_ptr(), T,
-        k_pages.data_ptr(), v_pages.data_ptr(), _outer_stride(k_pages), _outer_stride(v_pages), n_pages,
-        page, block_table.data_ptr(), _outer_stride(block_table) if seqs else max_pages, seqs,
-        max_pages, num_heads, kv, hd, _DTYPE_CODES[dt], out.data_ptr(),
-        torch.cuda.current_stream(dev).cuda_stream), "moe_rope_append")
+    page_elems = kv * page * hd
+    strides = ((page_elems, page_elems, max_pages, (num_heads + 2 * kv) * hd) if plain else
+               (_outer_stride(k_pages), _outer_stride(v_pages),
+                _outer_stride(block_table) if seqs else max_pages,
+                _outer_stride(qkv) if T else qkv.shape[1]))
+    status = _native.lib().moe_rope_append(_native.ROPE_APPEND.pack(
+        k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], n_pages, kv, page, hd,
+        _DTYPE_CODES[dt], block_table.data_ptr(), strides[2], seqs, max_pages, qkv.data_ptr(),
+        strides[3], cos.data_ptr(), sin.data_ptr(), max_pos,
+        positions.data_ptr(), 0 if seq_ids is None else seq_ids.data_ptr(), T, num_heads,
+        out.data_ptr(), _raw_stream(dev)))
+    if status:
+        check(status, "moe_rope_append")
     return out
 
 
@@ -716,12 +768,12 @@ def _paged_ws_bytes(device: int, seqs: int, max_pages: int, page: int, heads: in
 def paged_attention_workspace(block_table: torch.Tensor, page_size: int, num_heads: int,
                               kv_heads: int, head_dim: int) -> torch.Tensor:
     """A workspace for :func:`paged_attention` calls with tables of this size."""
-    nbytes = _paged_ws_bytes(block_table.device.index, *block_table.shape, page_size, num_heads,
+    nbytes = _paged_ws_bytes(block_table.get_device(), *block_table.shape, page_size, num_heads,
                              kv_heads, head_dim)
     return torch.zeros(nbytes, dtype=torch.uint8, device=block_table.device)
 
 
-@_on_device
+@_on_first_device
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                     block_table: torch.Tensor, lengths: torch.Tensor,
                     scale: float | None = None, out: torch.Tensor | None = None,
@@ -738,39 +790,57 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     call zeroes one of its own at every replay, which a given workspace spares).
     """
     what = "paged_attention"
-    dt, n_pages, kv, page, hd = _page_geometry(what, k_pages, v_pages, block_table)
-    dev = k_pages.device
-    seqs, max_pages = block_table.shape
-    _serve_check(what, dev, ("q", q, dt, (seqs, None, hd), 2),
-                 ("lengths", lengths, torch.int32, (seqs,), 1))
-    heads = q.shape[1]
+    try:
+        n_pages, kv, page, hd = k_pages.shape
+        seqs, max_pages = block_table.shape
+        rows, heads, _ = q.shape
+        dt, dev = k_pages.dtype, k_pages.get_device()
+        plain = (dt in _HALVES and (hd == 64 or hd == 128) and q.shape == (seqs, heads, hd)
+                 and v_pages.shape == k_pages.shape and lengths.shape == (seqs,)
+                 and _plain(dev, dt, q, k_pages, v_pages)
+                 and _plain(dev, torch.int32, lengths, block_table))
+    except (AttributeError, ValueError):
+        plain = False
+    if not plain:
+        _check_cache(what, k_pages, v_pages, block_table)
+        n_pages, kv, page, hd = k_pages.shape
+        dt, dev = k_pages.dtype, k_pages.get_device()
+        seqs, max_pages = block_table.shape
+        _serve_check(what, dev, ("q", q, dt, (seqs, None, hd), 2),
+                     ("lengths", lengths, torch.int32, (seqs,), 1))
+        heads = q.shape[1]
     if page % 16:
         raise ValueError(f"{what}: page_size must be a multiple of 16, got {page}")
     if heads == 0 or heads % kv:
         raise ValueError(f"{what}: {heads} query heads do not divide over {kv} KV heads")
     if out is None:
-        out = torch.empty((seqs, heads, hd), dtype=dt, device=dev)
+        out = q.new_empty((seqs, heads, hd))
     else:
         _serve_check(what, dev, ("out", out, dt, (seqs, heads, hd), 3))
     if seqs == 0:
         return out
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    nbytes = _paged_ws_bytes(dev.index, seqs, max_pages, page, heads, kv, hd)
+    stream = _raw_stream(dev)
+    nbytes = _paged_ws_bytes(dev, seqs, max_pages, page, heads, kv, hd)
     if workspace is None:
         workspace = _serve_scratch(dev, stream, nbytes)
     elif workspace.numel() * workspace.element_size() < nbytes:
         raise ValueError(f"{what}: workspace needs {nbytes} bytes")
-    check(_native.lib().moe_paged_attention(
-        q.data_ptr(), _outer_stride(q), k_pages.data_ptr(),
-        v_pages.data_ptr(), _outer_stride(k_pages), _outer_stride(v_pages), n_pages, page,
-        block_table.data_ptr(), _outer_stride(block_table), seqs, max_pages,
-        lengths.data_ptr(), heads, kv, hd, _DTYPE_CODES[dt],
-        hd ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(), nbytes, stream),
-        "moe_paged_attention")
+    page_elems = kv * page * hd
+    strides = ((page_elems, page_elems, max_pages, heads * hd) if plain else
+               (_outer_stride(k_pages), _outer_stride(v_pages), _outer_stride(block_table),
+                _outer_stride(q)))
+    status = _native.lib().moe_paged_attention(_native.PAGED_ATTENTION.pack(
+        k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], n_pages, kv, page, hd,
+        _DTYPE_CODES[dt], block_table.data_ptr(), strides[2], seqs, max_pages, q.data_ptr(),
+        strides[3], heads,
+        lengths.data_ptr(), hd ** -0.5 if scale is None else scale, out.data_ptr(),
+        workspace.data_ptr(), nbytes, stream))
+    if status:
+        check(status, "moe_paged_attention")
     return out
 
 
-@_on_device
+@_on_first_device
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                      max_seqlen: int, cu_seqlens_k: torch.Tensor | None = None,
                      max_seqlen_k: int | None = None, causal: bool = True,
@@ -787,17 +857,28 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ``PROMPT_WORKSPACE_BYTES`` zeroed bytes (the same buffer may serve both).
     """
     what = "prompt_attention"
-    if not isinstance(q, torch.Tensor) or q.ndim != 3:
-        raise ValueError(f"{what}: q must be [rows, heads, head_dim]")
-    dt, dev = q.dtype, q.device
-    if dt not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"{what}: q must be float16 or bfloat16, got {dt}")
-    T, heads, hd = q.shape
-    if hd not in (64, 128):
-        raise ValueError(f"{what}: head_dim must be 64 or 128, got {hd}")
-    _serve_check(what, dev, ("q", q, dt, q.shape, 1), ("k", k, dt, (None, None, hd), 1))
-    _serve_check(what, dev, ("v", v, dt, k.shape, 1),
-                 ("cu_seqlens", cu_seqlens, torch.int32, (None,), 1))
+    try:
+        T, heads, hd = q.shape
+        dt, dev = q.dtype, q.get_device()
+        plain = (dt in _HALVES and (hd == 64 or hd == 128) and dev >= 0 and k.shape == v.shape
+                 and k.ndim == 3 and k.shape[2] == hd and k.dtype is dt and v.dtype is dt
+                 and k.get_device() == dev and v.get_device() == dev and cu_seqlens.ndim == 1
+                 and q.stride(2) == 1 and k.stride(2) == 1 and v.stride(2) == 1
+                 and _plain(dev, torch.int32, cu_seqlens))
+    except (AttributeError, ValueError):
+        plain = False
+    if not plain:
+        if not isinstance(q, torch.Tensor) or q.ndim != 3:
+            raise ValueError(f"{what}: q must be [rows, heads, head_dim]")
+        dt, dev = q.dtype, q.get_device()
+        if dt not in _HALVES:
+            raise ValueError(f"{what}: q must be float16 or bfloat16, got {dt}")
+        T, heads, hd = q.shape
+        if hd not in (64, 128):
+            raise ValueError(f"{what}: head_dim must be 64 or 128, got {hd}")
+        _serve_check(what, dev, ("q", q, dt, q.shape, 1), ("k", k, dt, (None, None, hd), 1))
+        _serve_check(what, dev, ("v", v, dt, k.shape, 1),
+                     ("cu_seqlens", cu_seqlens, torch.int32, (None,), 1))
     kv, seqs = k.shape[1], cu_seqlens.shape[0] - 1
     if seqs < 0 or kv == 0 or heads == 0 or heads % kv:
         raise ValueError(f"{what}: {heads} query heads do not divide over {kv} KV heads, or "
@@ -811,34 +892,26 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     else:
         _serve_check(what, dev, ("cu_seqlens_k", cu_seqlens_k, torch.int32, (seqs + 1,), 1))
     if out is None:
-        out = torch.empty((T, heads, hd), dtype=dt, device=dev)
+        out = q.new_empty((T, heads, hd))
     else:
         _serve_check(what, dev, ("out", out, dt, (T, heads, hd), 3))
-    stream = torch.cuda.current_stream(dev).cuda_stream
+    stream = _raw_stream(dev)
     if workspace is None:
         workspace = _serve_scratch(dev, stream, PROMPT_WORKSPACE_BYTES)
     elif workspace.numel() * workspace.element_size() < PROMPT_WORKSPACE_BYTES:
         raise ValueError(f"{what}: workspace needs {PROMPT_WORKSPACE_BYTES} bytes")
-    check(_native.lib().moe_prompt_attention(
+    status = _native.lib().moe_prompt_attention(_native.PROMPT_ATTENTION.pack(
         q.data_ptr(), *_row_strides(q), T, k.data_ptr(), *_row_strides(k), v.data_ptr(),
         *_row_strides(v), k.shape[0], cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), seqs,
-        max_seqlen, max_seqlen_k, heads, kv, hd, causal, _DTYPE_CODES[dt],
+        max_seqlen, max_seqlen_k, heads, kv, hd, bool(causal), _DTYPE_CODES[dt],
         hd ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(),
-        PROMPT_WORKSPACE_BYTES, stream), "moe_prompt_attention")
+        PROMPT_WORKSPACE_BYTES, stream))
+    if status:
+        check(status, "moe_prompt_attention")
     return out
 
 
-def _row_strides(t: torch.Tensor) -> tuple[int, int]:
-    """Strides of [rows, heads, hd] in elements (packed where a dimension has one entry)."""
-    row, head, _ = t.stride()
-    if t.shape[1] <= 1:
-        head = t.shape[2]
-    if t.shape[0] <= 1:
-        row = max(t.shape[1], 1) * head
-    return row, head
-
-
-@_on_device
+@_on_first_device
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: torch.Tensor,
                   top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor):
     """``(tokens int64 [rows], probs fp32 [rows])``: one token per row of ``logits`` [rows, vocab].
@@ -855,18 +928,29 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: tor
     code = _DTYPE_CODES.get(logits.dtype)
     if code is None:
         raise ValueError(f"{what}: logits must be float16, bfloat16 or float32, got {logits.dtype}")
-    dev = logits.device
+    dev = logits.get_device()
     rows, vocab = logits.shape
     f32 = torch.float32
-    _serve_check(what, dev, ("logits", logits, logits.dtype, logits.shape, 1),
-                 ("uniforms", uniforms, f32, (rows,), 1), ("temperature", temperature, f32, (rows,), 1),
-                 ("top_k", top_k, torch.int32, (rows,), 1), ("top_p", top_p, f32, (rows,), 1),
-                 ("min_p", min_p, f32, (rows,), 1))
-    tokens = torch.empty(rows, dtype=torch.int64, device=dev)
-    probs = torch.empty(rows, dtype=f32, device=dev)
-    check(_native.lib().moe_sample_tokens(
+    per_row = (rows,)
+    try:
+        plain = (uniforms.shape == per_row and temperature.shape == per_row
+                 and top_k.shape == per_row and top_p.shape == per_row and min_p.shape == per_row
+                 and _plain(dev, f32, uniforms, temperature, top_p, min_p)
+                 and _plain(dev, torch.int32, top_k) and (logits.stride(1) == 1 or vocab == 1))
+    except AttributeError:
+        plain = False
+    if not plain:
+        _serve_check(what, dev, ("logits", logits, logits.dtype, logits.shape, 1),
+                     ("uniforms", uniforms, f32, per_row, 1),
+                     ("temperature", temperature, f32, per_row, 1),
+                     ("top_k", top_k, torch.int32, per_row, 1),
+                     ("top_p", top_p, f32, per_row, 1), ("min_p", min_p, f32, per_row, 1))
+    tokens = logits.new_empty(rows, dtype=torch.int64)
+    probs = logits.new_empty(rows, dtype=f32)
+    status = _native.lib().moe_sample_tokens(_native.SAMPLE_TOKENS.pack(
         logits.data_ptr(), _outer_stride(logits), rows, vocab, code, uniforms.data_ptr(),
         temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), min_p.data_ptr(),
-        tokens.data_ptr(), probs.data_ptr(), torch.cuda.current_stream(dev).cuda_stream),
-        "moe_sample_tokens")
+        tokens.data_ptr(), probs.data_ptr(), _raw_stream(dev)))
+    if status:
+        check(status, "moe_sample_tokens")
     return tokens, probs

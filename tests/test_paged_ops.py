@@ -308,23 +308,20 @@ def test_paged_attention_past_two_to_the_31_elements():
 
 def test_host_checks_precede_every_launch():
     """No pointer below is dereferenced: every refusal comes before the launch."""
-    import ctypes
-
     from moeinfra_b200 import _native
 
-    lib, f = _native.lib(), ctypes.c_void_p(0x100000)
+    lib, f, odd = _native.lib(), 0x100000, 0x100008
 
     def append(T=4, hd=128, page=16, dtype=0, stride=None, H=4, KV=2, p=f, pages=f, kstride=None):
         elems = KV * page * hd
-        return lib.moe_rope_append(p, (H + 2 * KV) * hd if stride is None else stride, f, f, 8, f,
-                                   None, T, pages, f, elems if kstride is None else kstride, elems,
-                                   4, page, f, 4, 4, 4, H, KV, hd, dtype, f, None)
+        return lib.moe_rope_append(_native.ROPE_APPEND.pack(
+            pages, f, elems if kstride is None else kstride, elems, 4, KV, page, hd, dtype, f, 4, 4, 4,
+            p, (H + 2 * KV) * hd if stride is None else stride, f, f, 8, f, 0, T, H, f, 0))
 
-    assert append(T=0) == 0
-    assert append(T=-1) == 1 and append(p=None) == 1 and append(H=0) == 1
+    assert append(T=0) == 0 and lib.moe_rope_append(None) == 1
+    assert append(T=-1) == 1 and append(p=0) == 1 and append(H=0) == 1
     assert append(stride=100) == 1 and append(kstride=64) == 1
     assert append(hd=96) == 2 and append(dtype=2) == 2
-    odd = ctypes.c_void_p(0x100008)
     assert append(p=odd) == 5 and append(pages=odd) == 5 and append(stride=1028) == 5
 
     need = lib.moe_paged_attention_workspace_size(4, 8, 16, 8, 2, 128)
@@ -333,16 +330,16 @@ def test_host_checks_precede_every_launch():
     def attend(seqs=4, hd=128, page=16, H=8, KV=2, dtype=0, scale=1.0, q=f, ws=f, bytes_=need,
                qs=None):
         elems = KV * page * hd
-        return lib.moe_paged_attention(q, H * hd if qs is None else qs, f, f, elems, elems, 9, page,
-                                       f, 8, seqs, 8, f, H, KV, hd, dtype, scale, f, ws, bytes_,
-                                       None)
+        return lib.moe_paged_attention(_native.PAGED_ATTENTION.pack(
+            f, f, elems, elems, 9, KV, page, hd, dtype, f, 8, seqs, 8, q,
+            H * hd if qs is None else qs, H, f, scale, f, ws, bytes_, 0))
 
-    assert attend(seqs=0) == 0
+    assert attend(seqs=0) == 0 and lib.moe_paged_attention(None) == 1
     assert attend(H=7) == 1 and attend(scale=0.0) == 1 and attend(scale=float("nan")) == 1
-    assert attend(q=None) == 1 and attend(qs=64) == 1
+    assert attend(scale=float("inf")) == 1 and attend(q=0) == 1 and attend(qs=64) == 1
     assert attend(hd=256) == 2 and attend(page=24) == 2 and attend(dtype=2) == 2
     assert attend(seqs=4096) == 2
-    assert attend(bytes_=need - 1) == 4 and attend(ws=None) == 4
+    assert attend(bytes_=need - 1) == 4 and attend(ws=0) == 4
     assert attend(q=odd) == 5 and attend(ws=odd) == 5
     assert _native.status_string(8) != "unknown status"
 

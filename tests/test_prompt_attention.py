@@ -180,25 +180,24 @@ def test_bad_offsets_are_reported():
 
 
 def test_host_checks_precede_every_launch():
-    import ctypes
-
     from moeinfra_b200 import _native
 
-    lib, f, odd = _native.lib(), ctypes.c_void_p(0x100000), ctypes.c_void_p(0x100008)
+    lib, f, odd = _native.lib(), 0x100000, 0x100008
 
     def attend(q=f, rows=10, seqs=2, H=4, KV=2, hd=128, dtype=0, scale=1.0, stride=None, out=f,
                max_q=8, k=f, head=None, ws=f, bytes_=16):
-        return lib.moe_prompt_attention(q, H * hd if stride is None else stride,
-                                        hd if head is None else head, rows, k, KV * hd, hd, f,
-                                        KV * hd, hd, rows, f, f, seqs, max_q, 8, H, KV, hd, 1, dtype,
-                                        scale, out, ws, bytes_, None)
+        return lib.moe_prompt_attention(_native.PROMPT_ATTENTION.pack(
+            q, H * hd if stride is None else stride, hd if head is None else head, rows, k, KV * hd,
+            hd, f, KV * hd, hd, rows, f, f, seqs, max_q, 8, H, KV, hd, 1, dtype, scale, out, ws,
+            bytes_, 0))
 
+    assert lib.moe_prompt_attention(None) == 1
     assert attend(rows=0) == 0 and attend(seqs=0) == 0 and attend(max_q=0) == 0
-    assert attend(rows=-1) == 1 and attend(H=5) == 1 and attend(q=None) == 1 and attend(k=None) == 1
+    assert attend(rows=-1) == 1 and attend(H=5) == 1 and attend(q=0) == 1 and attend(k=0) == 1
     assert attend(scale=0.0) == 1 and attend(scale=float("nan")) == 1 and attend(stride=8) == 1
     assert attend(head=64) == 1 and attend(seqs=-1) == 1
     assert attend(hd=96) == 2 and attend(dtype=2) == 2
-    assert attend(ws=None) == 4 and attend(bytes_=15) == 4 and attend(ws=odd) == 5
+    assert attend(ws=0) == 4 and attend(bytes_=15) == 4 and attend(ws=odd) == 5
     assert attend(q=odd) == 5 and attend(out=odd) == 5 and attend(stride=516) == 5
 
 

@@ -207,18 +207,17 @@ def test_frequencies_follow_the_probabilities():
 
 
 def test_host_checks_precede_every_launch():
-    import ctypes
-
     from moeinfra_b200 import _native
 
-    lib, f = _native.lib(), ctypes.c_void_p(0x100000)
+    lib, f = _native.lib(), 0x100000
 
     def sample(logits=f, stride=100, rows=3, vocab=100, dtype=0, u=f, out=f):
-        return lib.moe_sample_tokens(logits, stride, rows, vocab, dtype, u, f, f, f, f, out, f, None)
+        return lib.moe_sample_tokens(_native.SAMPLE_TOKENS.pack(
+            logits, stride, rows, vocab, dtype, u, f, f, f, f, out, f, 0))
 
-    assert sample(rows=0) == 0
+    assert sample(rows=0) == 0 and lib.moe_sample_tokens(None) == 1
     assert sample(rows=-1) == 1 and sample(vocab=0) == 1 and sample(stride=99) == 1
-    assert sample(logits=None) == 1 and sample(u=None) == 1 and sample(out=None) == 1
+    assert sample(logits=0) == 1 and sample(u=0) == 1 and sample(out=0) == 1
     assert sample(dtype=3) == 2 and sample(vocab=262145, stride=262145) == 2
 
 
