@@ -464,7 +464,9 @@ typedef struct moe_kv_pages {
  *   fp32 [max_pos, head_dim / 2]), rounds once, writes k and v to the token's
  *   slot and q to q_out [tokens, heads, head_dim].  seq_ids int32 [tokens], or
  *   NULL: token t belongs to sequence t.  A token with a negative position is
- *   padding: a zero q row, nothing appended.
+ *   padding: a zero q row, nothing appended.  k_out [tokens, kv_heads, head_dim],
+ *   if given, receives the rotated keys as well (a prompt's attention reads them
+ *   packed).
  */
 typedef struct moe_rope_append_args {
   moe_kv_pages_t kv;
@@ -478,6 +480,7 @@ typedef struct moe_rope_append_args {
   int64_t tokens;
   int64_t heads;
   uint16_t* q_out;
+  uint16_t* k_out; /* may be NULL */
   void* stream;
 } moe_rope_append_args_t;
 int moe_rope_append(const moe_rope_append_args_t* args);

@@ -33,7 +33,7 @@ class NF4Expert(ctypes.Structure):
 # twenty arguments costs ctypes ten times as long.  P: pointer, q: int64, d: double, in the
 # header's order; every field has 8 bytes.
 _KV_PAGES = "PPqqqqqqqPqqq"
-ROPE_APPEND = struct.Struct("@" + _KV_PAGES + "PqPPqPPqqPP")
+ROPE_APPEND = struct.Struct("@" + _KV_PAGES + "PqPPqPPqqPPP")
 PAGED_ATTENTION = struct.Struct("@" + _KV_PAGES + "PqqPdPPqP")
 PROMPT_ATTENTION = struct.Struct("@PqqqPqqPqqqPPqqqqqqqqdPPqP")
 SAMPLE_TOKENS = struct.Struct("@PqqqqPPPPPPPP")

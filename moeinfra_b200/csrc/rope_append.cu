@@ -26,6 +26,7 @@ struct RopeArgs {
   const int32_t *positions, *seq_ids;
   KvPages kv;
   uint16_t* q_out;
+  uint16_t* k_out;  // the rotated keys packed too (prompts attend to them), or null
   int heads;
 };
 
@@ -55,12 +56,13 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const RopeArgs a) 
   for (int i = threadIdx.x; i < items; i += kRopeThreads) {
     const int head = i / kPer, c = (i % kPer) * 8;
     const int kv_head = head - a.heads;  // < 0: a query head; >= kv_heads: a value head
-    uint16_t* dst;
+    uint16_t *dst, *copy = nullptr;
     if (kv_head < 0) {
       dst = a.q_out + (t * a.heads + head) * HD;
     } else {
-      if (page < 0) continue;
       const bool val = kv_head >= a.kv.kv_heads;
+      if (a.k_out && !val) copy = a.k_out + (t * a.kv.kv_heads + kv_head) * HD;
+      if (page < 0 && !copy) continue;
       const int j = val ? kv_head - a.kv.kv_heads : kv_head;
       dst = (val ? a.kv.v + page * a.kv.v_stride : a.kv.k + page * a.kv.k_stride) +
             ((int64_t)j * a.kv.page_size + slot) * HD;
@@ -88,6 +90,11 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const RopeArgs a) 
           }
         }
       }
+    }
+    if (copy) {
+      *reinterpret_cast<uint4*>(copy + c) = lo;
+      *reinterpret_cast<uint4*>(copy + c + HD / 2) = hi;
+      if (page < 0) continue;  // padding: a zero row there, nothing appended
     }
     *reinterpret_cast<uint4*>(dst + c) = lo;
     *reinterpret_cast<uint4*>(dst + c + HD / 2) = hi;
@@ -119,10 +126,10 @@ extern "C" int moe_rope_append(const moe_rope_append_args_t* args) {
       !c.kv.block_table || !c.q_out)
     return MOE_ERR_INVALID_ARG;
   if (!aligned16(c.qkv) || !aligned16(c.cos) || !aligned16(c.sin) || !aligned16(c.q_out) ||
-      (c.qkv_stride & 7))
+      !aligned16(c.k_out) || (c.qkv_stride & 7))
     return MOE_ERR_ALIGNMENT;
   const RopeArgs a{c.qkv, c.qkv_stride, c.cos, c.sin, c.max_pos, c.positions, c.seq_ids,
-                   pages_of(c.kv), c.q_out, (int)c.heads};
+                   pages_of(c.kv), c.q_out, c.k_out, (int)c.heads};
   cudaStream_t s = static_cast<cudaStream_t>(c.stream);
   if (c.kv.dtype == MOE_DTYPE_F16)
     return c.kv.head_dim == 64 ? launch_rope<F16, 64>(a, c.tokens, s)

@@ -99,18 +99,24 @@ class DenseStack:
         self.final_norm = final_norm.to(device=self.device, dtype=dtype).contiguous()
         self.lm_head = lm_head.to(device=self.device, dtype=dtype).contiguous()
         self.max_batch, self.max_len = max_batch, max_len
-        L, B, kv, hd = len(layers), max_batch, cfg.num_kv_heads, cfg.head_dim
-        self.k_cache = torch.zeros(L, B, kv, max_len, hd, device=self.device, dtype=dtype)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        hd = cfg.head_dim
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, hd, 2, dtype=torch.int64,
                                                       device=self.device).float() / hd))
         pos = torch.arange(max_len, device=self.device, dtype=torch.float32)
         freqs = torch.outer(pos, inv)
         emb = torch.cat((freqs, freqs), dim=-1)
-        self.cos = emb.cos().to(dtype)
-        self.sin = emb.sin().to(dtype)
+        self._make_cache(emb)
         self.scale = 1.0 / math.sqrt(hd)
         self.layer_hook = None  # called as hook(layer_id, moe_layer) after each MoE layer
+
+    def _make_cache(self, angles: torch.Tensor) -> None:
+        """The keys' and values' memory and the rotation table, from angles [max_len, head_dim]."""
+        cfg = self.cfg
+        self.k_cache = torch.zeros(len(self.layers), self.max_batch, cfg.num_kv_heads, self.max_len,
+                                   cfg.head_dim, device=self.device, dtype=self.dtype)
+        self.v_cache = torch.zeros_like(self.k_cache)
+        self.cos = angles.cos().to(self.dtype)
+        self.sin = angles.sin().to(self.dtype)
 
     # -- attention --------------------------------------------------------------------
     def _attention(self, li: int, x: torch.Tensor, pos0, T: int, decode_pos: Optional[torch.Tensor]):

@@ -24,12 +24,19 @@ Extra config keys (all optional): ``model.{num_attention_heads,
 num_key_value_heads, vocab_size, rope_theta, rms_norm_eps}`` when the
 checkpoint has no ``config.json``; ``cache.gpu_budget_bytes``;
 ``transfer.{prefetch_policy, staging_slots}``; ``engine.{max_batch,
-max_seq_len, cuda_graphs, preload_experts}``; ``parallel.expert_parallel``:
+max_seq_len, cuda_graphs, preload_experts, paged_kv, page_size, kv_pages}``; ``parallel.expert_parallel``:
 one process per GPU (``torch.distributed`` initialised), rank r keeps experts
 ``[r*E/G, (r+1)*E/G)`` of every layer resident and runs its own sequences;
 each MoE layer is an ``ExpertParallelMoE`` (peer-memory exchange for decode
 steps, NCCL all-to-all for prefill); every rank must call ``generate`` with
 the same batch shape.
+
+``engine.paged_kv`` serves prompts of different lengths (``attention_mask``
+marks the padding, on either side) over a paged cache of ``kv_pages`` pages
+(default: enough for ``max_batch`` sequences of ``max_seq_len``) of
+``page_size`` positions: :class:`~moeinfra_b200.engine.paged.PagedDenseStack`.
+``ForwardRequest.sampling`` draws tokens instead of taking the largest logit,
+with either cache.
 """
 from __future__ import annotations
 
@@ -45,9 +52,11 @@ from moeinfra_b200 import kernels
 from moeinfra_b200.cache.manager import CacheManager
 from moeinfra_b200.cache.types import EvictionPolicy
 from moeinfra_b200.engine.dense import DenseConfig, DenseStack
+from moeinfra_b200.engine.paged import PagedDenseStack
 from moeinfra_b200.engine.prefetch import PrefetchEngine
 from moeinfra_b200.engine.router import ExpertRouter
-from moeinfra_b200.engine.types import ForwardRequest, ForwardResult, PrefetchPolicy
+from moeinfra_b200.engine.types import (ForwardRequest, ForwardResult, PrefetchPolicy,
+                                        SamplingParams)
 from moeinfra_b200.model.loader import ModelLoader
 from moeinfra_b200.model.moe_layer import MoELayer
 from moeinfra_b200.transfer.pinned_memory import PinnedMemoryBudget
@@ -85,6 +94,45 @@ def expert_bytes(hidden: int, inter: int) -> int:
     return 3 * per
 
 
+class _Sampler:
+    """One generation's sampling parameters and random numbers on the device.
+
+    ``turn(i)`` puts step i's numbers in the buffer that ``draw`` reads, so a captured step draws
+    with the parameters and numbers ``lend`` copied into its own sampler.
+    """
+
+    def __init__(self, params: SamplingParams, batch: int, steps: int, device) -> None:
+        def row(name, value, dtype, least):
+            values = list(value) if isinstance(value, (list, tuple)) else [value] * batch
+            if len(values) != batch:
+                raise ValueError(f"sampling.{name} has {len(values)} values for {batch} sequences")
+            if not all(v >= least for v in values):
+                raise ValueError(f"sampling.{name} must be at least {least}, got {values}")
+            return torch.tensor(values, dtype=dtype, device=device)
+
+        f32 = torch.float32
+        self.params = [row("temperature", params.temperature, f32, 0.0),
+                       row("top_k", params.top_k, torch.int32, 0),
+                       row("top_p", params.top_p, f32, 0.0), row("min_p", params.min_p, f32, 0.0)]
+        gen = None
+        if params.seed is not None:
+            gen = torch.Generator(device=device).manual_seed(params.seed)
+        self._all = torch.rand(steps, batch, device=device, generator=gen)
+        self.uniforms = torch.zeros(batch, device=device)
+
+    def turn(self, step: int) -> None:
+        self.uniforms.copy_(self._all[step])
+
+    def lend(self, captured: "_Sampler") -> None:
+        """From now on drive ``captured``'s buffers, which a graph reads."""
+        for mine, its in zip(self.params, captured.params):
+            its.copy_(mine)
+        self.uniforms = captured.uniforms
+
+    def draw(self, logits: torch.Tensor) -> torch.Tensor:
+        return kernels.sample_tokens(logits, self.uniforms, *self.params)[0]
+
+
 class InferenceEngine:
     """Mixtral NF4 MoE inference with GPU-resident or CPU-offloaded experts."""
 
@@ -118,6 +166,12 @@ class InferenceEngine:
         self._preload = bool(engine_cfg.get("preload_experts", False))
         self._ep = bool(config.get("parallel", {}).get("expert_parallel", False))
         self._peer = None
+        self._paged = bool(engine_cfg.get("paged_kv", False))
+        self._page_size = int(engine_cfg.get("page_size", 64))
+        self._kv_pages = engine_cfg.get("kv_pages")
+        if self._paged and self._ep:
+            raise ValueError("engine.paged_kv does not combine with parallel.expert_parallel: its "
+                             "ranks' prompts must have one shape")
         if self._ep and not (torch.distributed.is_available() and torch.distributed.is_initialized()):
             raise RuntimeError("parallel.expert_parallel needs an initialised process group")
 
@@ -192,11 +246,16 @@ class InferenceEngine:
             moe.check_each_call = False  # generate() checks the device once per generation
             self._moe_layers.append(moe)
             layers.append(w)
-        self._stack = DenseStack(
-            DenseConfig.from_mixtral(self._mixtral_config), layers,
-            self._model.load_embeddings(), self._model.load_final_norm(),
-            self._model.load_lm_head(), self._moe_layers, dev, self._max_batch, self._max_len,
-            self._dtype)
+        stack_args = (DenseConfig.from_mixtral(self._mixtral_config), layers,
+                      self._model.load_embeddings(), self._model.load_final_norm(),
+                      self._model.load_lm_head(), self._moe_layers, dev, self._max_batch,
+                      self._max_len, self._dtype)
+        if self._paged:
+            with torch.cuda.device(dev):
+                self._stack = PagedDenseStack(*stack_args, page_size=self._page_size,
+                                              num_pages=self._kv_pages)
+        else:
+            self._stack = DenseStack(*stack_args)
         if self._prefetch_engine.policy != PrefetchPolicy.NONE:
             self._stack.layer_hook = self._after_layer
         if self._preload:
@@ -227,14 +286,20 @@ class InferenceEngine:
 
     # -- generation -----------------------------------------------------------------------
     def generate(self, request: ForwardRequest) -> ForwardResult:
-        """Prefill the prompt, then greedy-decode ``max_new_tokens`` tokens."""
+        """Prefill the prompts, then decode ``max_new_tokens`` tokens (greedy unless ``sampling``)."""
         self._initialize_runtime()
         timings: dict = {}
         B = request.input_ids.shape[0] if request.input_ids.ndim == 2 else 0
+        sampler = None
+        if request.sampling is not None and 0 < B <= self._max_batch:
+            sampler = _Sampler(request.sampling, B, max(request.max_new_tokens, 1), self._device)
+        if self._paged:
+            self._reserve(request)
         if (self._use_graphs and request.max_new_tokens > 1 and 0 < B <= self._max_batch
                 and self.all_experts_resident()):
             with torch.cuda.device(self._device):
-                self._graph_for(B)  # built once per batch size, outside the timed stages
+                # built once per batch size and kind, outside the timed stages
+                self._graph_for(B, sampler is not None)
         torch.cuda.synchronize(self._device)
         t0 = time.perf_counter()
         logits = self._prefill(request.input_ids, request.attention_mask)
@@ -242,7 +307,7 @@ class InferenceEngine:
         ttft_ms = (time.perf_counter() - t0) * 1e3
         timings["prefill"] = ttft_ms
         t1 = time.perf_counter()
-        tokens = self._decode(logits, request.max_new_tokens)
+        tokens = self._decode(logits, request.max_new_tokens, sampler)
         torch.cuda.synchronize(self._device)
         decode_ms = (time.perf_counter() - t1) * 1e3
         timings["decode"] = decode_ms
@@ -268,6 +333,13 @@ class InferenceEngine:
         if input_ids.ndim != 2:
             raise ValueError(f"input_ids must have shape (batch, seq_len), got {tuple(input_ids.shape)}")
         B, S = input_ids.shape
+        if self._paged:
+            prompts = self._prompts(input_ids, attention_mask)
+            with torch.cuda.device(self._device):
+                logits = self._stack.prefill(prompts)
+            self._prompt_lens = [int(p.numel()) for p in prompts]
+            self._last_logits = logits[:, None, :]
+            return self._last_logits
         if S <= 0:
             raise ValueError("input_ids must contain at least one token")
         if B > self._max_batch:
@@ -281,20 +353,59 @@ class InferenceEngine:
         ids = input_ids.to(device=self._device, dtype=torch.long, non_blocking=True)
         with torch.cuda.device(self._device):
             logits = self._stack.forward(ids, pos0=0)
-        self._prompt_len = S
+        self._prompt_lens = [S] * B
         self._last_logits = logits[:, None, :]
         return self._last_logits
 
-    def _decode_step_fn(self, ids_buf, pos_buf):
+    def _prompts(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor]) -> list:
+        """The rows of ``input_ids`` without their padding (paged mode)."""
+        if input_ids.ndim != 2:
+            raise ValueError(f"input_ids must have shape (batch, seq_len), got {tuple(input_ids.shape)}")
+        B, S = input_ids.shape
+        if not 0 < B <= self._max_batch:
+            raise ValueError(f"batch {B}: 1 to engine.max_batch={self._max_batch} are served")
+        if attention_mask is None:
+            rows = list(input_ids)
+        else:
+            if attention_mask.shape != input_ids.shape:
+                raise ValueError("attention_mask must have the same shape as input_ids")
+            rows = [ids[m != 0] for ids, m in zip(input_ids, attention_mask)]
+        if any(r.numel() == 0 for r in rows):
+            raise ValueError("every prompt must contain at least one token")
+        return rows
+
+    def _reserve(self, request: ForwardRequest) -> None:
+        """Pages for the whole generation, so that a captured step never needs the host."""
+        if request.max_new_tokens < 0:
+            raise ValueError("max_new_tokens must be non-negative")
+        # The last token drawn is never appended.
+        lens = [int(p.numel()) + max(request.max_new_tokens - 1, 0)
+                for p in self._prompts(request.input_ids, request.attention_mask)]
+        if max(lens) > self._max_len:
+            raise ValueError(f"{max(lens)} positions exceed engine.max_seq_len={self._max_len}")
+        self._stack.cache.reserve(lens)
+
+    def _decode_step_fn(self, ids_buf, pos_buf, sampler=None):
         def step():
-            logits = self._stack.forward(ids_buf, decode_pos=pos_buf)
-            ids_buf.copy_(logits.argmax(dim=-1, keepdim=True))
+            if self._paged:
+                logits = self._stack.decode(ids_buf, pos_buf)
+            else:
+                logits = self._stack.forward(ids_buf, decode_pos=pos_buf)
+            ids_buf.copy_(logits.argmax(dim=-1, keepdim=True) if sampler is None
+                          else sampler.draw(logits)[:, None])
             pos_buf.add_(1)
             return logits
         return step
 
+    def _positions(self, B: int) -> torch.Tensor:
+        """The device buffer of the next token's position: one for all, or one per sequence."""
+        if self._paged:
+            return torch.zeros(B, dtype=torch.int32, device=self._device)
+        return torch.zeros(1, dtype=torch.long, device=self._device)
+
     @torch.no_grad()
-    def _decode(self, next_token_logits: torch.Tensor, max_new_tokens: int) -> list:
+    def _decode(self, next_token_logits: torch.Tensor, max_new_tokens: int,
+                sampler: Optional["_Sampler"] = None) -> list:
         if self._stack is None:
             raise RuntimeError("Inference runtime has not been initialized")
         if max_new_tokens < 0:
@@ -302,47 +413,63 @@ class InferenceEngine:
         if max_new_tokens == 0:
             return [[] for _ in range(next_token_logits.shape[0])]
         B = next_token_logits.shape[0]
-        S = self._prompt_len
-        if S + max_new_tokens > self._max_len:
-            raise ValueError(f"{S + max_new_tokens} positions exceed engine.max_seq_len={self._max_len}")
+        lens = self._prompt_lens
+        if not self._paged and lens[0] + max_new_tokens > self._max_len:
+            raise ValueError(f"{lens[0] + max_new_tokens} positions exceed "
+                             f"engine.max_seq_len={self._max_len}")
         dev = self._device
+        start = torch.tensor(lens if self._paged else lens[:1])
         with torch.cuda.device(dev):
             hist = torch.empty(B, max_new_tokens, dtype=torch.long, device=dev)
-            first = next_token_logits[:, -1, :].argmax(dim=-1)
+            if sampler is None:
+                first = next_token_logits[:, -1, :].argmax(dim=-1)
+            else:
+                sampler.turn(0)
+                first = sampler.draw(next_token_logits[:, -1, :])
             hist[:, 0] = first
             if max_new_tokens > 1:
                 use_graph = self._use_graphs and self.all_experts_resident()
                 if use_graph:
-                    g, ids_buf, pos_buf, out = self._graph_for(B)
+                    g, ids_buf, pos_buf, out, captured = self._graph_for(B, sampler is not None)
                     ids_buf.copy_(first[:, None])
-                    pos_buf.fill_(S)
+                    pos_buf.copy_(start)
+                    if sampler is not None:
+                        sampler.lend(captured)
                     for i in range(1, max_new_tokens):
+                        if sampler is not None:
+                            sampler.turn(i)
                         g.replay()
                         hist[:, i] = ids_buf[:, 0]
                     self._last_logits = out[:, None, :]
                 else:
                     ids_buf = first[:, None].clone()
-                    pos_buf = torch.full((1,), S, dtype=torch.long, device=dev)
-                    step = self._decode_step_fn(ids_buf, pos_buf)
+                    pos_buf = self._positions(B)
+                    pos_buf.copy_(start)
+                    step = self._decode_step_fn(ids_buf, pos_buf, sampler)
                     for i in range(1, max_new_tokens):
+                        if sampler is not None:
+                            sampler.turn(i)
                         logits = step()
                         hist[:, i] = ids_buf[:, 0]
                     self._last_logits = logits[:, None, :]
         return hist.cpu().tolist()
 
-    def _graph_for(self, B: int):
+    @torch.no_grad()
+    def _graph_for(self, B: int, sampled: bool = False):
         """The captured decode step for batch B (built once; replays advance it on the device)."""
-        ent = self._graphs.get(B)
+        ent = self._graphs.get((B, sampled))
         if ent is not None:
             return ent
         dev = self._device
         ids_buf = torch.zeros(B, 1, dtype=torch.long, device=dev)
-        pos_buf = torch.zeros(1, dtype=torch.long, device=dev)
-        step = self._decode_step_fn(ids_buf, pos_buf)
+        pos_buf = self._positions(B)
+        sampler = _Sampler(SamplingParams(), B, 1, dev) if sampled else None
+        step = self._decode_step_fn(ids_buf, pos_buf, sampler)
         # Warm up on a side stream (allocations, one-time kernel setup), then
         # capture.  The warm-up runs at the last cache position, which a
-        # generation writes before it ever reads it.
-        pos_buf.fill_(self._max_len - 1)
+        # generation writes before it ever reads it; with pages at position -1,
+        # which appends nothing and sees nothing.
+        pos_buf.fill_(-1 if self._paged else self._max_len - 1)
         s = torch.cuda.Stream(dev)
         s.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(s):
@@ -352,8 +479,8 @@ class InferenceEngine:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             out = step()
-        ent = (g, ids_buf, pos_buf, out)
-        self._graphs[B] = ent
+        ent = (g, ids_buf, pos_buf, out, sampler)
+        self._graphs[B, sampled] = ent
         return ent
 
     def close(self) -> None:

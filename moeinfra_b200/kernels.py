@@ -698,7 +698,7 @@ def _check_cache(what: str, k_pages, v_pages, block_table) -> None:
 def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
                 block_table: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                 num_heads: int, seq_ids: torch.Tensor | None = None,
-                out: torch.Tensor | None = None) -> torch.Tensor:
+                out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotate q and k of fused projection rows and append k and v to the paged cache.
 
     ``qkv`` [tokens, (num_heads + 2 * kv_heads) * head_dim] (rows may be strided), fp16 or bf16;
@@ -706,8 +706,9 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positio
     token's own sequence (negative: padding, a zero q row and nothing appended); ``block_table``
     int32 [sequences, max_pages]; ``k_pages`` / ``v_pages`` [pages, kv_heads, page_size, head_dim],
     written in place; ``seq_ids`` int32 [tokens] (None: token t is sequence t, the decode step).
-    Returns q [tokens, num_heads, head_dim].  A position, sequence or page out of range appends
-    nothing and shows in :func:`check_device`.
+    Returns q [tokens, num_heads, head_dim]; ``k_out`` [tokens, kv_heads, head_dim], if given,
+    receives the rotated keys packed, as :func:`prompt_attention` reads them.  A position, sequence
+    or page out of range appends nothing and shows in :func:`check_device`.
     """
     what = "rope_append"
     try:
@@ -743,6 +744,8 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positio
         out = qkv.new_empty((T, num_heads, hd))
     else:
         _serve_check(what, dev, ("out", out, dt, (T, num_heads, hd), 3))
+    if k_out is not None:
+        _serve_check(what, dev, ("k_out", k_out, dt, (T, kv, hd), 3))
     page_elems = kv * page * hd
     strides = ((page_elems, page_elems, max_pages, (num_heads + 2 * kv) * hd) if plain else
                (_outer_stride(k_pages), _outer_stride(v_pages),
@@ -753,7 +756,7 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positio
         _DTYPE_CODES[dt], block_table.data_ptr(), strides[2], seqs, max_pages, qkv.data_ptr(),
         strides[3], cos.data_ptr(), sin.data_ptr(), max_pos,
         positions.data_ptr(), 0 if seq_ids is None else seq_ids.data_ptr(), T, num_heads,
-        out.data_ptr(), _raw_stream(dev)))
+        out.data_ptr(), 0 if k_out is None else k_out.data_ptr(), _raw_stream(dev)))
     if status:
         check(status, "moe_rope_append")
     return out

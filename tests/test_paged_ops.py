@@ -62,9 +62,14 @@ def test_rope_append(dtype, H, KV, hd, page, prompt):
     # Rows of a wider buffer: the projection's rows may be strided.
     wide = torch.randn(T, (H + 2 * KV) * hd + 64, generator=g).to(dtype)
     qkv = wide.cuda()[:, :(H + 2 * KV) * hd]
+    packed = torch.empty(T, KV, hd, dtype=dtype, device="cuda")
     q = kernels.rope_append(qkv, cos.cuda(), sin.cuda(), pos.int().cuda(), table.cuda(), kp, vp, H,
-                            seq_ids=seq.int().cuda() if prompt else None)
+                            seq_ids=seq.int().cuda() if prompt else None,
+                            k_out=packed if prompt else None)
     kernels.check_device()
+    if prompt:
+        at = table[seq, pos // page].long().cuda()
+        assert torch.equal(packed, kp[at, :, (pos % page).cuda()])
     x = wide[:, :(H + 2 * KV) * hd].view(T, H + 2 * KV, hd)
     rot = ref.rotate(x[:, :H + KV], cos[pos], sin[pos])
     size = x[:, :H + KV].double().abs()
@@ -96,7 +101,10 @@ def test_rope_append_leaves_padding_and_refuses_bad_places():
         one = [torch.tensor([v], dtype=torch.int32, device="cuda") for v in (pos, seq)]
         return kernels.rope_append(qkv, cos, sin, one[0], table, kp, vp, H, seq_ids=one[1])
 
-    assert not run(-1, 0).any()
+    packed = torch.full((1, KV, hd), 7.0, dtype=torch.float16, device="cuda")
+    none = torch.tensor([-1], dtype=torch.int32, device="cuda")
+    kernels.rope_append(qkv, cos, sin, none, table, kp, vp, H, k_out=packed)
+    assert not run(-1, 0).any() and not packed.any()
     kernels.check_device()
     for pos, seq in [(40, 0), (33, 0), (0, 3), (0, -1), (20, 1), (0, 2)]:
         assert not run(pos, seq).any()
@@ -312,17 +320,18 @@ def test_host_checks_precede_every_launch():
 
     lib, f, odd = _native.lib(), 0x100000, 0x100008
 
-    def append(T=4, hd=128, page=16, dtype=0, stride=None, H=4, KV=2, p=f, pages=f, kstride=None):
+    def append(T=4, hd=128, page=16, dtype=0, stride=None, H=4, KV=2, p=f, pages=f, kstride=None,
+               k_out=0):
         elems = KV * page * hd
         return lib.moe_rope_append(_native.ROPE_APPEND.pack(
             pages, f, elems if kstride is None else kstride, elems, 4, KV, page, hd, dtype, f, 4, 4, 4,
-            p, (H + 2 * KV) * hd if stride is None else stride, f, f, 8, f, 0, T, H, f, 0))
+            p, (H + 2 * KV) * hd if stride is None else stride, f, f, 8, f, 0, T, H, f, k_out, 0))
 
     assert append(T=0) == 0 and lib.moe_rope_append(None) == 1
     assert append(T=-1) == 1 and append(p=0) == 1 and append(H=0) == 1
     assert append(stride=100) == 1 and append(kstride=64) == 1
     assert append(hd=96) == 2 and append(dtype=2) == 2
-    assert append(p=odd) == 5 and append(pages=odd) == 5 and append(stride=1028) == 5
+    assert append(k_out=odd) == 5 and append(p=odd) == 5 and append(pages=odd) == 5 and append(stride=1028) == 5
 
     need = lib.moe_paged_attention_workspace_size(4, 8, 16, 8, 2, 128)
     assert need > 0 and lib.moe_paged_attention_workspace_size(4, 8, 16, 8, 2, 96) == 0
