@@ -22,14 +22,17 @@
 // rest is a chain of reductions), by instruction issue where they are many.  A
 // row is spread over a cluster of CTAs whose threads hold it in registers, as
 // integers of the same order ("keys"):
-//   * no sort: the k-th token and the top-p boundary are found by search over
-//     the keys.  A pass sorts the logits between the bounds into 8 ways (it adds
-//     each weight to the sums of the thresholds below it, 21 instructions);
-//     register slots that hold none of these for a whole warp are skipped.  The
-//     first thresholds sit where a language model's boundary usually lies, 0.5
-//     to 16 below the maximum in units of the temperature.  Once at most 256
-//     logits are left between the bounds every CTA takes a copy of these and
-//     decides among them by itself.  Correctness depends on neither.
+//   * A first pass adds each weight to the sums of 7 thresholds (21
+//     instructions a logit), 0.5 to 16 below the maximum in units of the
+//     temperature, where a language model's boundaries usually lie.  If then at
+//     most 256 logits are above the threshold that already holds enough, they go
+//     to one CTA of the cluster, which orders them and applies every filter by
+//     comparing each with each; the others are done.
+//   * Else no sort either: the k-th token and the top-p boundary are found by
+//     search over the keys, 8 ways a pass, over the logits still between the
+//     bounds; register slots that hold none of these for a whole warp are
+//     skipped, and once at most 256 are left every CTA takes a copy and decides
+//     by itself.
 //   * Exponentials are not kept: the first pass needs every logit's, what
 //     follows only those of the few between the bounds or kept.  That leaves 64
 //     registers a thread and two CTAs to an SM, one's barriers under the other's
@@ -173,9 +176,9 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   using L = Logit<T>;
   constexpr int kVec = L::kVec, kIters = PER / kVec;
   __shared__ uint64_t s_warp[kWarps][8], s_slots[2][kMaxCluster][8];
-  __shared__ uint32_t s_list[kList], s_all[kList];
+  __shared__ uint32_t s_list[kList], s_all[kList], s_index[kList];
   __shared__ uint64_t s_weight[kList], s_above;
-  __shared__ uint32_t s_count, s_key;
+  __shared__ uint32_t s_count, s_few, s_key;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Exchange ex{cg::this_cluster(), 0, a.cluster, warp, lane, 0, s_warp, s_slots};
   ex.rank = blockIdx.x % a.cluster;
@@ -228,10 +231,21 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     return;
   }
   const float m = L::value(top);
+  // (x - m) / temperature by the reciprocal, corrected twice by the remainder
+  // (Markstein 1990: the result is the correctly rounded quotient); below -104
+  // the exponential is 0, and a reciprocal out of range ends there too.
+  const float inverse = __frcp_rn(temperature);
   auto exp_of = [&](uint32_t key) {
-    return key == top ? 1.f : key == 0 ? 0.f : expf(__fdiv_rn(L::value(key) - m, temperature));
+    const float d = L::value(key) - m;
+    float q = d * inverse;
+    if (key == 0 || !(q >= -104.f)) return key == top ? 1.f : 0.f;
+    if (inverse != 0.f) {  // 0: an infinite temperature, q is right
+      q = fmaf(fmaf(-q, temperature, d), inverse, q);
+      q = fmaf(fmaf(-q, temperature, d), inverse, q);
+    }
+    return key == top ? 1.f : expf(q);
   };
-  if (threadIdx.x == 0) s_count = 0;
+  if (threadIdx.x == 0) s_count = s_few = 0;
 
   // Sums of the weights (or counts) of the keys in [lo, hi) that are >= the
   // threshold t of lane 1 .. 7 (lane 0: >= t too), as lane j's result.
@@ -251,6 +265,27 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
       for (int j = 0; j < 8; ++j) sum[j] += key[c] >= th[j] ? w : 0ull;
     }
     return ex.sum(sum);
+  };
+  auto block_sum = [&](uint64_t v) {  // over the CTA, in every thread
+    const uint32_t lo = __reduce_add_sync(kAll, (uint32_t)v & 0x7FFFFFFu);
+    const uint32_t hi = __reduce_add_sync(kAll, (uint32_t)(v >> 27));
+    __syncthreads();
+    if (lane == 0) s_warp[warp][0] = lo + ((uint64_t)hi << 27);
+    __syncthreads();
+    uint64_t s = s_warp[lane & (kWarps - 1)][0];
+#pragma unroll
+    for (int o = kWarps / 2; o; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
+    return s;
+  };
+  auto need_of = [&](uint64_t total) {  // what top-p asks for
+    const double want = ceil(__dmul_rn((double)p, __ull2double_rn(total)));
+    const uint64_t n = want >= 1.0 ? __double2ull_rz(want) : 1ull;
+    return n < total ? n : total;
+  };
+  auto draw_of = [&](uint64_t total) {  // the point of the kept weights that u stands for
+    const double at = floor(__dmul_rn((double)u, __ull2double_rn(total)));
+    const uint64_t r = at >= 1.0 ? __double2ull_rz(at) : 0ull;
+    return r < total ? r : total - 1;
   };
   // The largest key whose sum over it and all above is >= need, and the sum
   // above it.  t, s: thresholds of a first pass (rising with the lane, lane 0
@@ -290,16 +325,18 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
       }
       const uint64_t n = shfl64(ex.sum(found), 0);
       if (n <= kList) {
-        int from = 0;
-        for (int r = 0; r < ex.size; ++r) {
-          const int held = (int)ex.slot(r, 0);
-          const uint32_t* list = ex.cluster.map_shared_rank(s_list, r);
-          for (int i = threadIdx.x; i < held; i += kThreads) {
+        if (warp < ex.size) {  // warp r copies CTA r's
+          int from = 0, held = 0;
+          for (int r = 0; r <= warp; ++r) {
+            from += held;
+            held = (int)ex.slot(r, 0);
+          }
+          const uint32_t* list = ex.cluster.map_shared_rank(s_list, warp);
+          for (int i = lane; i < held; i += 32) {
             const uint32_t kk = list[i];
             s_all[from + i] = kk;
             s_weight[from + i] = count ? 1ull : weight(exp_of(kk));
           }
-          from += held;
         }
         if (threadIdx.x == 0) {
           s_count = 0;
@@ -333,6 +370,48 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
       s = above + pass(count, lo, hi, t);
     }
   };
+  // The first n of s_all / s_index hold every logit the filters may keep: apply
+  // them and draw.  Two threads per logit compare it with half of the others
+  // each.  need: what top-p asks for where top-k does not come first.
+  auto finish = [&](int n, bool by_k, bool by_p, uint64_t need) {
+    const int i = threadIdx.x >> 1, half = threadIdx.x & 1;
+    const bool real = i < n;
+    const uint32_t own = real ? s_all[i] : 0u, index = real ? s_index[i] : 0u;
+    const float e = exp_of(own);
+    uint64_t w = real ? weight(e) : 0ull;
+    if (real && half == 0) s_weight[i] = w;
+    __syncthreads();
+    uint32_t place = 0;   // in the order by falling logit and rising index
+    uint64_t before = 0;  // weights ahead of it
+    if (real)
+      for (int j = half; j < n; j += 2) {
+        const uint32_t kk = s_all[j];
+        const bool ahead = kk > own || (kk == own && s_index[j] < index);
+        place += ahead;
+        before += ahead ? s_weight[j] : 0ull;
+      }
+    place += __shfl_xor_sync(kAll, place, 1);
+    before += __shfl_xor_sync(kAll, before, 1);
+    bool keep = real && (!by_k || place < (uint32_t)k);
+    if (by_k && by_p) {
+      const uint64_t v[1] = {keep && half == 0 ? w : 0ull};
+      need = need_of(block_sum(v[0]));
+    }
+    keep = keep && (!by_p || before < need) && e >= min_p;
+    if (!keep) w = 0;
+    const uint64_t total = block_sum(half == 0 ? w : 0ull);  // its barriers order s_weight too
+    if (real && half == 0) s_weight[i] = w;
+    __syncthreads();
+    uint64_t run = 0;  // kept weights of lower indices
+    if (keep)
+      for (int j = half; j < n; j += 2) run += s_index[j] < index ? s_weight[j] : 0ull;
+    run += __shfl_xor_sync(kAll, run, 1);
+    const uint64_t r = draw_of(total);
+    if (keep && half == 0 && r >= run && r < run + w) {
+      a.tokens[row] = index;
+      a.probs[row] = (float)(__ull2double_rn(w) / __ull2double_rn(total));
+    }
+  };
   // First thresholds: lane 7 the nearest to the maximum.
   const float reach[8] = {0.f, 16.f, 11.f, 8.f, 5.5f, 3.5f, 1.75f, 0.5f};
   float mine = 0.f;
@@ -342,29 +421,67 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   uint32_t guess = L::key_near(m - mine * temperature);
   if (guess > top) guess = top;
 
-  // ---- top-k: keys above k_key, and the first k_ties of those equal to it ----
   uint32_t cut = 0;    // keys above it are kept
   uint64_t ties = 0;   // and so many of those equal to it, by index
-  const bool by_k = k > 0 && k < a.vocab;
-  if (by_k) {
-    const uint64_t s = pass(true, 1, top + 1, guess);
-    const Bound b = search(true, k, 1, top + 1, guess, s);
-    cut = b.key;
-    ties = k - b.above;
-  }
-  // ---- top-p ----
-  if (p < 1.f) {
-    const uint64_t s = pass(false, 1, top + 1, (lane & 7) == 0 ? cut + 1 : guess);
-    const uint64_t total = shfl64(s, 0) + ties * (cut ? weight(exp_of(cut)) : 0ull);
-    const double want = ceil(__dmul_rn((double)p, __ull2double_rn(total)));
-    uint64_t need = want >= 1.0 ? __double2ull_rz(want) : 1ull;
-    if (need > total) need = total;
-    const uint32_t lo = cut ? cut : 1u;
-    const Bound b = search(false, need, lo, top + 1, guess, s);
-    const uint64_t w = weight(exp_of(b.key));
-    const uint64_t n = (need - b.above + w - 1) / w;
-    ties = b.key == cut && n > ties ? ties : n;
-    cut = b.key;
+  const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.f;
+  if (by_k || by_p) {
+    uint64_t s = pass(by_k, 1, top + 1, (lane & 7) == 0 ? 1u : guess);
+    const uint64_t need = by_k ? (uint64_t)k : need_of(shfl64(s, 0));
+    // ---- few enough at or above the threshold that holds enough: one CTA takes them ----
+    const uint32_t enough = __ballot_sync(kAll, lane >= 1 && lane < 8 && s >= need) | 1u;
+    const int j = 31 - __clz(enough);
+    const uint32_t floor_key = j == 0 ? 1u : __shfl_sync(kAll, guess, j);
+    const int owner = static_cast<int>(row % a.cluster);
+    uint32_t slots = 0;
+#pragma unroll
+    for (int c = 0; c < PER; ++c) slots |= (key[c] >= floor_key ? 1u : 0u) << c;
+    uint64_t found[1] = {(uint64_t)__popc(slots)};
+    const uint32_t mine_n = __popc(slots), warp_n = __reduce_add_sync(kAll, mine_n);
+    if (warp_n > 0 && warp_n <= kList) {
+      uint32_t at = mine_n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(kAll, at, o);
+        if (lane >= o) at += v;
+      }
+      uint32_t base = 0;
+      if (lane == 0) base = atomicAdd(ex.cluster.map_shared_rank(&s_few, owner), warp_n);
+      at += __shfl_sync(kAll, base, 0) - mine_n;
+      uint32_t* keys = ex.cluster.map_shared_rank(s_all, owner);
+      uint32_t* indices = ex.cluster.map_shared_rank(s_index, owner);
+#pragma unroll
+      for (int c = 0; c < PER; ++c)
+        if (slots >> c & 1) {
+          if (at < kList) {
+            keys[at] = key[c];
+            indices[at] = first + c / kVec * 32 * kVec + c % kVec;
+          }
+          ++at;
+        }
+    }
+    const uint64_t total_n = shfl64(ex.sum(found), 0);
+    if (total_n <= kList) {
+      if (ex.rank == owner)
+        finish(static_cast<int>(total_n), by_k, by_p, by_k ? 0ull : need);
+      return;
+    }
+    // ---- top-k: keys above the cut, and the first `ties` of those equal to it ----
+    if (by_k) {
+      const Bound b = search(true, k, 1, top + 1, guess, s);
+      cut = b.key;
+      ties = k - b.above;
+    }
+    // ---- top-p ----
+    if (by_p) {
+      if (by_k) s = pass(false, 1, top + 1, (lane & 7) == 0 ? cut + 1 : guess);
+      const uint64_t total = shfl64(s, 0) + ties * (cut ? weight(exp_of(cut)) : 0ull);
+      const uint64_t want = need_of(total);
+      const Bound b = search(false, want, cut ? cut : 1u, top + 1, guess, s);
+      const uint64_t w = weight(exp_of(b.key));
+      const uint64_t n = (want - b.above + w - 1) / w;
+      ties = b.key == cut && n > ties ? ties : n;
+      cut = b.key;
+    }
   }
   // ---- what is kept, per warp and CTA ----
   auto keeps = [&](uint32_t kk) {  // the weight of a key above the cut, if it is kept
@@ -382,77 +499,72 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   auto kept = [&](uint64_t equal, uint64_t before) {  // of `equal` ties after `before` others
     return before >= ties ? 0ull : (ties - before < equal ? ties - before : equal);
   };
-  uint64_t total = 0, mine_before = 0, ties_before = 0, seen = 0, mine_all = 0;
-  for (int r = 0; r < a.cluster; ++r) {
-    const uint64_t n = ex.slot(r, 1), w = ex.slot(r, 0) + kept(n, seen) * w_cut;
-    if (r == ex.rank) {
-      mine_before = total;
-      mine_all = w;
-      ties_before = seen;
+  // Sums of pieces in order (lane i: piece i's weight above the cut and its ties)
+  // -> kept weight and ties before the piece, its kept weight, all kept weight.
+  struct Piece {
+    uint64_t before, ties_before, own, all;
+  };
+  auto place = [&](uint64_t w, uint64_t equal, uint64_t ties_ahead) {
+    uint64_t seen = equal;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t v = __shfl_up_sync(kAll, seen, o);
+      if (lane >= o) seen += v;
     }
-    total += w;
-    seen += n;
-  }
-  const double at = floor(__dmul_rn((double)u, __ull2double_rn(total)));
-  uint64_t r = at >= 1.0 ? __double2ull_rz(at) : 0ull;
-  if (r > total - 1) r = total - 1;
-  if (r < mine_before || r >= mine_before + mine_all) return;
+    seen += ties_ahead - equal;
+    const uint64_t own = w + kept(equal, seen) * w_cut;
+    uint64_t run = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t v = __shfl_up_sync(kAll, run, o);
+      if (lane >= o) run += v;
+    }
+    return Piece{run - own, seen, own, shfl64(run, 31)};
+  };
+  const bool is_cta = lane < a.cluster;
+  const Piece ctas = place(is_cta ? ex.slot(lane, 0) : 0ull, is_cta ? ex.slot(lane, 1) : 0ull, 0);
+  const uint64_t total = ctas.all, r = draw_of(total);
+  const uint64_t cta_before = shfl64(ctas.before, ex.rank), cta_own = shfl64(ctas.own, ex.rank);
+  if (r < cta_before || r >= cta_before + cta_own) return;
   // ---- the CTA that holds the token: its warp, step, lane, element ----
-  uint64_t run = mine_before, warp_all = 0;
-  for (int w = 0; w <= warp; ++w) {
-    if (w > 0) {
-      run += warp_all;
-      ties_before += s_warp[w - 1][1];
-    }
-    warp_all = s_warp[w][0] + kept(s_warp[w][1], ties_before) * w_cut;
-  }
-  if (r < run || r >= run + warp_all) return;
+  const bool is_warp = lane < kWarps;
+  const Piece warps = place(is_warp ? s_warp[lane][0] : 0ull, is_warp ? s_warp[lane][1] : 0ull,
+                            shfl64(ctas.ties_before, ex.rank));
+  uint64_t run = cta_before + shfl64(warps.before, warp);
+  uint64_t ties_before = shfl64(warps.ties_before, warp);
+  const uint64_t warp_own = shfl64(warps.own, warp);
+  if (r < run || r >= run + warp_own) return;
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
-    uint64_t own = 0;
-    uint32_t equal = 0;
+    uint64_t w[kVec], own = 0, equal = 0;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
-      const int c = i * kVec + j;
-      if (key[c] > cut) own += keeps(key[c]);
-      equal += key[c] == cut;
+      const uint32_t kk = key[i * kVec + j];
+      w[j] = kk > cut ? keeps(kk) : 0ull;
+      own += w[j];
+      equal += kk == cut;
     }
-    uint32_t equal_in = equal;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(kAll, equal_in, o);
-      if (lane >= o) equal_in += v;
-    }
-    uint64_t before = ties_before + equal_in - equal;
-    uint64_t in = own + kept(equal, before) * w_cut;
-    const uint64_t lane_all = in;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t v = __shfl_up_sync(kAll, in, o);
-      if (lane >= o) in += v;
-    }
-    uint64_t at_lane = run + in - lane_all;
-    if (r >= at_lane && r < at_lane + lane_all) {
+    const Piece lanes = place(own, equal, ties_before);
+    uint64_t at = run + lanes.before, seen = lanes.ties_before;
+    if (r >= at && r < at + lanes.own) {
       bool found = false;
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
-        const int c = i * kVec + j;
-        uint64_t w = key[c] > cut ? keeps(key[c]) : 0ull;
-        if (key[c] == cut) {
-          w = before < ties ? w_cut : 0ull;
-          ++before;
+        if (key[i * kVec + j] == cut) {
+          w[j] = seen < ties ? w_cut : 0ull;
+          ++seen;
         }
-        if (!found && r < at_lane + w) {
+        if (!found && r < at + w[j]) {
           found = true;
           a.tokens[row] = first + i * 32 * kVec + j;
-          a.probs[row] = (float)(__ull2double_rn(w) / __ull2double_rn(total));
+          a.probs[row] = (float)(__ull2double_rn(w[j]) / __ull2double_rn(total));
         }
-        at_lane += w;
+        at += w[j];
       }
     }
-    run += shfl64(in, 31);
-    ties_before += __shfl_sync(kAll, equal_in, 31);
+    run += lanes.all;
     if (r < run) return;
+    ties_before = shfl64(lanes.ties_before + equal, 31);
   }
 }
 

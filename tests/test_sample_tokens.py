@@ -139,7 +139,8 @@ def test_infinities_nan_and_extremes(dtype):
     x = torch.tensor(rows, device="cuda").to(dtype).repeat(8, 1)
     u = (torch.arange(64, device="cuda") + 0.5) / 64
     for kw in (dict(), dict(top_k=2), dict(top_p=0.6), dict(min_p=0.3), dict(temperature=0.0),
-               dict(temperature=1e-6), dict(temperature=1e6, top_k=3, top_p=0.8)):
+               dict(temperature=1e-6), dict(temperature=1e6, top_k=3, top_p=0.8), dict(temperature=3e38),
+               dict(temperature=1e-38), dict(temperature=1e-45, top_p=0.9)):
         tokens, _ = _compare(x, u, _params(64, **kw))
         for i, t in enumerate(tokens.tolist()):  # a masked token is drawn only where all are
             row = rows[i % 8]
