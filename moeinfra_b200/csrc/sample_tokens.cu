@@ -54,7 +54,6 @@ constexpr int kMaxCluster = 16;            // 8 is the portable size; 16 only wh
 constexpr int kMaxPer = 32;                // logits a thread holds at most
 constexpr int kList = 256;                 // logits that a search finishes with directly
 constexpr int kMaxVocab = kMaxCluster * kThreads * kMaxPer;
-constexpr float kScale = 1099511627776.f;  // 2^40
 constexpr uint32_t kAll = 0xffffffffu;
 
 struct SampleArgs {
@@ -112,7 +111,20 @@ struct Logit<float> {
 };
 
 __device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) { return __shfl_sync(kAll, v, lane); }
-__device__ __forceinline__ uint64_t weight(float e) { return __float2ull_rz(e * kScale); }
+// trunc(2^40 e) for e in [0, 1] as two limbs of 20 bits (every step is exact): a
+// thread adds up to kMaxPer of each, a warp 32 times that, in 32 bits.
+struct Limbs {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ Limbs limbs(float e) {
+  const float x = e * 1048576.f;
+  const uint32_t hi = __float2uint_rz(x);
+  return Limbs{hi, __float2uint_rz((x - __uint2float_rz(hi)) * 1048576.f)};
+}
+__device__ __forceinline__ uint64_t weight(float e) {
+  const Limbs w = limbs(e);
+  return ((uint64_t)w.hi << 20) + w.lo;
+}
 
 // Sums over the cluster, 8 values at a time: lane j of every warp ends up with
 // the sum of value j % 8.  slot(r, j): what CTA r contributed to the last one;
@@ -129,6 +141,7 @@ struct Exchange {
     uint64_t* at = &slots[turn][rank][j];
     for (int r = to; r < size; r += 4) *cluster.map_shared_rank(at, r) = mine;
   }
+  // A warp's sum of value j in lane j; v: limbs of 27 bits and the rest.
   template <int N>
   __device__ __forceinline__ uint64_t sum(const uint64_t (&v)[N]) {
     uint64_t mine = 0;
@@ -139,6 +152,34 @@ struct Exchange {
       if ((lane & 7) == j) mine = lo + ((uint64_t)hi << 27);
     }
     if (lane < 8) warp_sum[warp][lane] = mine;
+    return sum_of();
+  }
+  // The same by halves: a lane hands the values that the other half of its group
+  // keeps over, 8 -> 4 -> 2 -> 1, so that lanes 4j .. 4j + 3 end up with value j
+  // (18 shuffles; 16 warp-wide reductions took twice as long).
+  __device__ __forceinline__ uint64_t sum(const Limbs (&v)[8]) {
+    Limbs a[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = v[j];
+#pragma unroll
+    for (int half = 4; half; half >>= 1) {
+      const bool up = lane & 4 * half;
+#pragma unroll
+      for (int j = 0; j < half; ++j) {
+        const Limbs keep = up ? a[j + half] : a[j], give = up ? a[j] : a[j + half];
+        a[j].hi = keep.hi + __shfl_xor_sync(kAll, give.hi, 4 * half);
+        a[j].lo = keep.lo + __shfl_xor_sync(kAll, give.lo, 4 * half);
+      }
+    }
+#pragma unroll
+    for (int o = 2; o; o >>= 1) {
+      a[0].hi += __shfl_xor_sync(kAll, a[0].hi, o);
+      a[0].lo += __shfl_xor_sync(kAll, a[0].lo, o);
+    }
+    if ((lane & 3) == 0) warp_sum[warp][lane >> 2] = a[0].lo + ((uint64_t)a[0].hi << 20);
+    return sum_of();
+  }
+  __device__ __forceinline__ uint64_t sum_of() {  // of the warps' sums in warp_sum
     __syncthreads();
     if (warp == 0) {
       uint64_t s = 0;
@@ -178,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   __shared__ uint64_t s_warp[kWarps][8], s_slots[2][kMaxCluster][8];
   __shared__ uint32_t s_list[kList], s_all[kList], s_index[kList];
   __shared__ uint64_t s_weight[kList], s_above;
-  __shared__ uint32_t s_count, s_few, s_key;
+  __shared__ uint32_t s_count[2], s_few, s_key;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Exchange ex{cg::this_cluster(), 0, a.cluster, warp, lane, 0, s_warp, s_slots};
   ex.rank = blockIdx.x % a.cluster;
@@ -235,35 +276,45 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   // (Markstein 1990: the result is the correctly rounded quotient); below -104
   // the exponential is 0, and a reciprocal out of range ends there too.
   const float inverse = __frcp_rn(temperature);
-  auto exp_of = [&](uint32_t key) {
-    const float d = L::value(key) - m;
-    float q = d * inverse;
-    if (key == 0 || !(q >= -104.f)) return key == top ? 1.f : 0.f;
-    if (inverse != 0.f) {  // 0: an infinite temperature, q is right
-      q = fmaf(fmaf(-q, temperature, d), inverse, q);
-      q = fmaf(fmaf(-q, temperature, d), inverse, q);
-    }
-    return key == top ? 1.f : expf(q);
+  const float divisor = inverse != 0.f ? temperature : 0.f;  // infinite: nothing to correct
+  auto exp_of = [&](uint32_t key) {  // key 0 is a NaN
+    const float d = L::value(key) - m, q0 = d * inverse;
+    float q = fmaf(fmaf(-q0, divisor, d), inverse, q0);
+    q = fmaf(fmaf(-q, divisor, d), inverse, q);
+    const float e = expf(q);
+    return key == top ? 1.f : (q0 >= -104.f ? e : 0.f);
   };
-  if (threadIdx.x == 0) s_count = s_few = 0;
+  if (threadIdx.x == 0) s_count[0] = s_few = 0;
 
   // Sums of the weights (or counts) of the keys in [lo, hi) that are >= the
-  // threshold t of lane 1 .. 7 (lane 0: >= t too), as lane j's result.
-  auto pass = [&](bool count, uint32_t lo, uint32_t hi, uint32_t t) {
-    uint32_t th[8], slots = 0;
-    uint64_t sum[8] = {};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) th[j] = __shfl_sync(kAll, t, j);
+  // threshold t of lane 1 .. 7, as lane j's result.  Lane 0's is what `zero`
+  // says: the sum of those >= its threshold, or how many are in [lo, hi).
+  auto in_range = [&](uint32_t lo, uint32_t hi) {  // slots that hold one
+    uint32_t slots = 0;
 #pragma unroll
     for (int c = 0; c < PER; ++c) slots |= (key[c] - lo < hi - lo ? 1u : 0u) << c;
+    return slots;
+  };
+  auto pass = [&](bool count, uint32_t slots, uint32_t t, bool zero_counts) {
+    uint32_t th[8];
+    Limbs sum[8] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) th[j] = __shfl_sync(kAll, t, j);
     const uint32_t used = __reduce_or_sync(kAll, slots);
 #pragma unroll
     for (int c = 0; c < PER; ++c) {
       if (!(used >> c & 1)) continue;
-      const uint64_t w = !(slots >> c & 1) ? 0ull : count ? 1ull : weight(exp_of(key[c]));
+      Limbs w{0, 1};
+      if (!count) w = limbs(exp_of(key[c]));
+      const uint32_t kk = slots >> c & 1 ? key[c] : 0u;  // below every threshold
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum[j] += key[c] >= th[j] ? w : 0ull;
+      for (int j = 0; j < 8; ++j)
+        if (kk >= th[j]) {
+          sum[j].hi += w.hi;
+          sum[j].lo += w.lo;
+        }
     }
+    if (zero_counts) sum[0] = Limbs{0, (uint32_t)__popc(slots)};
     return ex.sum(sum);
   };
   auto block_sum = [&](uint64_t v) {  // over the CTA, in every thread
@@ -296,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   };
   auto search = [&](bool count, uint64_t need, uint32_t lo, uint32_t hi, uint32_t t, uint64_t s) {
     uint64_t above = 0;
-    for (;;) {
+    for (int turn = 0;; turn ^= 1) {
       const uint32_t enough = __ballot_sync(kAll, lane >= 1 && lane < 8 && s >= need) | 1u;
       const int j = 31 - __clz(enough);  // sums fall as thresholds rise
       const uint32_t t_lo = __shfl_sync(kAll, t, j), t_hi = __shfl_sync(kAll, t, (j + 1) & 7);
@@ -307,67 +358,63 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
         above = s_hi;
       }
       if (hi - lo <= 1) return Bound{lo, above};
-      // The logits between the bounds, if they are few, to every CTA.
-      uint32_t slots = 0;
+      // The next pass; and the logits between the bounds into a list, which
+      // decides at once if they turn out to be few.
+      const uint32_t slots = in_range(lo, hi);
+      if (slots) {
+        uint32_t at = atomicAdd(&s_count[turn], __popc(slots));
+        if (at < kList) {
 #pragma unroll
-      for (int c = 0; c < PER; ++c) slots |= (key[c] - lo < hi - lo ? 1u : 0u) << c;
-      const uint32_t used = __reduce_or_sync(kAll, slots);
-      uint64_t found[1] = {(uint64_t)__popc(slots)};
-      if (used) {
-        uint32_t at = 0;
-        if (slots) at = atomicAdd(&s_count, __popc(slots));
-#pragma unroll
-        for (int c = 0; c < PER; ++c)
-          if (slots >> c & 1) {
-            if (at < kList) s_list[at] = key[c];
-            ++at;
-          }
+          for (int c = 0; c < PER; ++c)
+            if (slots >> c & 1) {
+              if (at < kList) s_list[at] = key[c];
+              ++at;
+            }
+        }
       }
-      const uint64_t n = shfl64(ex.sum(found), 0);
-      if (n <= kList) {
-        if (warp < ex.size) {  // warp r copies CTA r's
-          int from = 0, held = 0;
-          for (int r = 0; r <= warp; ++r) {
-            from += held;
-            held = (int)ex.slot(r, 0);
-          }
-          const uint32_t* list = ex.cluster.map_shared_rank(s_list, warp);
-          for (int i = lane; i < held; i += 32) {
-            const uint32_t kk = list[i];
-            s_all[from + i] = kk;
-            s_weight[from + i] = count ? 1ull : weight(exp_of(kk));
-          }
-        }
-        if (threadIdx.x == 0) {
-          s_count = 0;
-          s_key = 0;
-        }
-        __syncthreads();
-        uint64_t over = 0, equal = 0;  // weights above and at the thread's key
-        uint32_t own = 0;
-        bool ok = false;
-        if (threadIdx.x < n) {
-          own = s_all[threadIdx.x];
-          for (int i = 0; i < (int)n; ++i) {
-            const uint32_t kk = s_all[i];
-            const uint64_t w = s_weight[i];
-            over += kk > own ? w : 0ull;
-            equal += kk == own ? w : 0ull;
-          }
-          ok = above + over + equal >= need;
-        }
-        const uint32_t found_key = __reduce_max_sync(kAll, ok ? own : 0u);
-        if (lane == 0 && found_key) atomicMax(&s_key, found_key);
-        __syncthreads();
-        if (threadIdx.x < n && own == s_key) s_above = above + over;  // the same value from each
-        __syncthreads();
-        return Bound{s_key, s_above};
-      }
-      if (threadIdx.x == 0) s_count = 0;  // read again after the next pass's barrier
+      if (threadIdx.x == 0) s_count[turn ^ 1] = 0;
       const uint32_t step = (hi - lo + 7) / 8;
       const uint64_t next = (uint64_t)lo + (uint64_t)step * (lane & 7);
       t = next < hi ? (uint32_t)next : hi;
-      s = above + pass(count, lo, hi, t);
+      s = pass(count, slots, t, true);
+      const uint64_t n = shfl64(s, 0);
+      s += above;
+      if (n > kList) continue;
+      if (warp < ex.size) {  // warp r copies CTA r's
+        int from = 0, held = 0;
+        for (int r = 0; r <= warp; ++r) {
+          from += held;
+          held = (int)ex.slot(r, 0);
+        }
+        const uint32_t* list = ex.cluster.map_shared_rank(s_list, warp);
+        for (int i = lane; i < held; i += 32) {
+          const uint32_t kk = list[i];
+          s_all[from + i] = kk;
+          s_weight[from + i] = count ? 1ull : weight(exp_of(kk));
+        }
+      }
+      if (threadIdx.x == 0) s_key = 0;
+      __syncthreads();
+      uint64_t over = 0, equal = 0;  // weights above and at the thread's key
+      uint32_t own = 0;
+      bool ok = false;
+      if (threadIdx.x < n) {
+        own = s_all[threadIdx.x];
+        for (int i = 0; i < (int)n; ++i) {
+          const uint32_t kk = s_all[i];
+          const uint64_t w = s_weight[i];
+          over += kk > own ? w : 0ull;
+          equal += kk == own ? w : 0ull;
+        }
+        ok = above + over + equal >= need;
+      }
+      const uint32_t found_key = __reduce_max_sync(kAll, ok ? own : 0u);
+      if (lane == 0 && found_key) atomicMax(&s_key, found_key);
+      if (threadIdx.x == 0) s_count[0] = 0;  // a second search begins with it
+      __syncthreads();
+      if (threadIdx.x < n && own == s_key) s_above = above + over;  // the same value from each
+      __syncthreads();
+      return Bound{s_key, s_above};
     }
   };
   // The first n of s_all / s_index hold every logit the filters may keep: apply
@@ -425,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   uint64_t ties = 0;   // and so many of those equal to it, by index
   const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.f;
   if (by_k || by_p) {
-    uint64_t s = pass(by_k, 1, top + 1, (lane & 7) == 0 ? 1u : guess);
+    uint64_t s = pass(by_k, kAll, (lane & 7) == 0 ? 1u : guess, false);
     const uint64_t need = by_k ? (uint64_t)k : need_of(shfl64(s, 0));
     // ---- few enough at or above the threshold that holds enough: one CTA takes them ----
     const uint32_t enough = __ballot_sync(kAll, lane >= 1 && lane < 8 && s >= need) | 1u;
@@ -473,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     }
     // ---- top-p ----
     if (by_p) {
-      if (by_k) s = pass(false, 1, top + 1, (lane & 7) == 0 ? cut + 1 : guess);
+      if (by_k) s = pass(false, kAll, (lane & 7) == 0 ? cut + 1 : guess, false);
       const uint64_t total = shfl64(s, 0) + ties * (cut ? weight(exp_of(cut)) : 0ull);
       const uint64_t want = need_of(total);
       const Bound b = search(false, want, cut ? cut : 1u, top + 1, guess, s);
