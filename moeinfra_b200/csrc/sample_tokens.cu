@@ -37,17 +37,22 @@
 //     follows only those of the few between the bounds or kept.  That leaves 64
 //     registers a thread and two CTAs to an SM, one's barriers under the other's
 //     arithmetic.
-//   * Per pass one cluster barrier: warps reduce in two integer reductions of
-//     32 bits each, a CTA's sums go to every CTA of the cluster through
-//     distributed shared memory.
+//   * Between passes the CTAs exchange sums, which is most of a small call: each
+//     stores its 8 into every CTA's shared memory with st.async, whose bytes
+//     complete an mbarrier there (a cluster barrier behind plain stores took 2000
+//     cycles, this a third).  Waits are bounded: on a timeout the error word is
+//     set and the CTA returns, as then do the others.
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
+#include "sm100_ptx.cuh"
 
 namespace moe {
 namespace {
 
 namespace cg = cooperative_groups;
+
+MOE_DEFINE_ERROR_WORD()
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 16;            // 8 is the portable size; 16 only where a row needs it
@@ -64,6 +69,7 @@ struct SampleArgs {
   const int32_t* top_k;
   int64_t* tokens;
   float* probs;
+  uint64_t wait_ns;
 };
 
 // Logits as keys: unsigned integers of the same order, NaN as -inf, -0 as 0.
@@ -126,22 +132,52 @@ __device__ __forceinline__ uint64_t weight(float e) {
   return ((uint64_t)w.hi << 20) + w.lo;
 }
 
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+
 // Sums over the cluster, 8 values at a time: lane j of every warp ends up with
 // the sum of value j % 8.  slot(r, j): what CTA r contributed to the last one;
 // warp_sum[w][j]: what warp w of this CTA did.
+//
+// Two sets of slots and barriers are used in turn.  A CTA sends its sums of
+// exchange n + 2 (the set of n) after it has those of n + 1 from every CTA, and
+// each of them sent these after all its warps had read n.
 struct Exchange {
-  cg::cluster_group cluster;
-  int rank, size, warp, lane, turn = 0;
+  int rank, size, warp, lane;
+  uint64_t wait_ns;
   uint64_t (*warp_sum)[8];
-  uint64_t (*slots)[kMaxCluster][8];  // two of these, used in turn
+  uint64_t (*slots)[kMaxCluster][8];
+  uint32_t bar;       // two mbarriers of one arrival (this CTA's, with the bytes to come)
+  uint32_t count = 0;
+  bool dead = false;  // a wait ran out
 
-  __device__ __forceinline__ uint64_t slot(int r, int j) const { return slots[turn ^ 1][r][j]; }
-  __device__ __forceinline__ void give(uint64_t mine) {  // lane j < 8: the CTA's value j
-    const uint32_t to = lane >> 3, j = lane & 7;
-    uint64_t* at = &slots[turn][rank][j];
-    for (int r = to; r < size; r += 4) *cluster.map_shared_rank(at, r) = mine;
+  __device__ __forceinline__ int turn() const { return count & 1; }
+  __device__ __forceinline__ uint64_t slot(int r, int j) const { return slots[turn() ^ 1][r][j]; }
+  // Warp 0: value lane % 8 of this CTA to every CTA (just value 0 if `one`).
+  __device__ __forceinline__ void give(uint64_t mine, bool one) {
+    const uint32_t here = bar + 8 * turn(), at = saddr(&slots[turn()][rank][lane & 7]);
+    if (lane == 0) mbar_expect_tx(here, size * (one ? 8 : 64));
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kMaxCluster / 4; ++i) {
+      const int r = (lane >> 3) + 4 * i;
+      if (r < size && (!one || (lane & 7) == 0))
+        asm volatile(
+            "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(
+                map_rank(at, r)),
+            "l"(mine), "r"(map_rank(here, r))
+            : "memory");
+    }
   }
-  // A warp's sum of value j in lane j; v: limbs of 27 bits and the rest.
+  __device__ __forceinline__ void wait() {
+    if (!mbar_poll_or(bar + 8 * turn(), count >> 1 & 1, wait_ns,
+                      [] { set_device_error(kErrWaitTimeout); }))
+      dead = true;
+    ++count;
+  }
   template <int N>
   __device__ __forceinline__ uint64_t sum(const uint64_t (&v)[N]) {
     uint64_t mine = 0;
@@ -155,8 +191,7 @@ struct Exchange {
     return sum_of();
   }
   // The same by halves: a lane hands the values that the other half of its group
-  // keeps over, 8 -> 4 -> 2 -> 1, so that lanes 4j .. 4j + 3 end up with value j
-  // (18 shuffles; 16 warp-wide reductions took twice as long).
+  // keeps over, 8 -> 4 -> 2 -> 1, so that lanes 4j .. 4j + 3 end up with value j.
   __device__ __forceinline__ uint64_t sum(const Limbs (&v)[8]) {
     Limbs a[8];
 #pragma unroll
@@ -187,28 +222,27 @@ struct Exchange {
       for (int w = 0; w < kWarps; w += 4) s += warp_sum[w + (lane >> 3)][lane & 7];
       s += __shfl_xor_sync(kAll, s, 8);
       s += __shfl_xor_sync(kAll, s, 16);
-      give(s);
+      give(s, false);
     }
-    cluster.sync();
+    wait();
     uint64_t s = 0;
-    for (int r = lane >> 3; r < size; r += 4) s += slots[turn][r][lane & 7];
+#pragma unroll
+    for (int i = 0; i < kMaxCluster / 4; ++i) {
+      const int r = (lane >> 3) + 4 * i;
+      if (r < size) s += slot(r, lane & 7);
+    }
     s += __shfl_xor_sync(kAll, s, 8);
     s += __shfl_xor_sync(kAll, s, 16);
-    turn ^= 1;
     return s;
   }
   __device__ __forceinline__ uint32_t max(uint32_t v) {  // of all threads, in every thread
     v = __reduce_max_sync(kAll, v);
     if (lane == 0) warp_sum[warp][0] = v;
     __syncthreads();
-    if (warp == 0) {
-      v = __reduce_max_sync(kAll, (uint32_t)warp_sum[lane & (kWarps - 1)][0]);
-      if ((lane & 7) == 0) give(v);
-    }
-    cluster.sync();
-    v = __reduce_max_sync(kAll, lane < size ? (uint32_t)slots[turn][lane & (kMaxCluster - 1)][0] : 0u);
-    turn ^= 1;
-    return v;
+    if (warp == 0)
+      give(__reduce_max_sync(kAll, (uint32_t)warp_sum[lane & (kWarps - 1)][0]), true);
+    wait();
+    return __reduce_max_sync(kAll, lane < size ? (uint32_t)slot(lane & (kMaxCluster - 1), 0) : 0u);
   }
 };
 
@@ -221,10 +255,18 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   __shared__ uint64_t s_weight[kList], s_above;
   __shared__ uint32_t s_count[2], s_few, s_key;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Exchange ex{cg::this_cluster(), 0, a.cluster, warp, lane, 0, s_warp, s_slots};
-  ex.rank = blockIdx.x % a.cluster;
+  __shared__ __align__(8) uint64_t s_bar[2];
+  cg::cluster_group cluster = cg::this_cluster();
   const int64_t row = blockIdx.x / a.cluster;
-  ex.cluster.barrier_arrive();  // waited for before the first store to another CTA
+  Exchange ex{static_cast<int>(blockIdx.x % a.cluster), a.cluster, warp, lane, a.wait_ns, s_warp,
+              s_slots, saddr(s_bar)};
+  if (threadIdx.x == 0) {
+    mbar_init(ex.bar, 1);
+    mbar_init(ex.bar + 8, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  cluster.barrier_arrive();  // waited for before the first store to another CTA
   pdl_trigger();
   pdl_wait();
 
@@ -257,15 +299,16 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   uint32_t top = 0;
 #pragma unroll
   for (int c = 0; c < PER; ++c) top = max(top, key[c]);
-  ex.cluster.barrier_wait();
+  cluster.barrier_wait();
   top = ex.max(top);
+  if (ex.dead) return;
   if (!(temperature > 0.f) || k == 1) {  // its lowest index
     uint32_t index = 0xFFFFFFFFu;
 #pragma unroll
     for (int c = PER - 1; c >= 0; --c)
       if (key[c] == top) index = first + c / kVec * 32 * kVec + c % kVec;
     index = ~ex.max(~index);
-    if (ex.rank == 0 && threadIdx.x == 0) {
+    if (!ex.dead && ex.rank == 0 && threadIdx.x == 0) {
       a.tokens[row] = index;
       a.probs[row] = 1.f;
     }
@@ -379,14 +422,16 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
       s = pass(count, slots, t, true);
       const uint64_t n = shfl64(s, 0);
       s += above;
+      if (ex.dead) return Bound{lo, above};
       if (n > kList) continue;
+      cluster.sync();  // the lists of the other CTAs
       if (warp < ex.size) {  // warp r copies CTA r's
         int from = 0, held = 0;
         for (int r = 0; r <= warp; ++r) {
           from += held;
           held = (int)ex.slot(r, 0);
         }
-        const uint32_t* list = ex.cluster.map_shared_rank(s_list, warp);
+        const uint32_t* list = cluster.map_shared_rank(s_list, warp);
         for (int i = lane; i < held; i += 32) {
           const uint32_t kk = list[i];
           s_all[from + i] = kk;
@@ -482,32 +527,25 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     uint32_t slots = 0;
 #pragma unroll
     for (int c = 0; c < PER; ++c) slots |= (key[c] >= floor_key ? 1u : 0u) << c;
-    uint64_t found[1] = {(uint64_t)__popc(slots)};
-    const uint32_t mine_n = __popc(slots), warp_n = __reduce_add_sync(kAll, mine_n);
-    if (warp_n > 0 && warp_n <= kList) {
-      uint32_t at = mine_n;
+    const uint64_t found[1] = {(uint64_t)__popc(slots)};
+    const uint64_t total_n = shfl64(ex.sum(found), 0);
+    if (ex.dead) return;
+    if (total_n <= kList) {
+      uint32_t base = 0;  // of this CTA's places
+      for (int r = 0; r < ex.rank; ++r) base += (uint32_t)ex.slot(r, 0);
+      if (slots) {
+        uint32_t at = base + atomicAdd(&s_few, __popc(slots));
+        uint32_t* keys = cluster.map_shared_rank(s_all, owner);
+        uint32_t* indices = cluster.map_shared_rank(s_index, owner);
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(kAll, at, o);
-        if (lane >= o) at += v;
-      }
-      uint32_t base = 0;
-      if (lane == 0) base = atomicAdd(ex.cluster.map_shared_rank(&s_few, owner), warp_n);
-      at += __shfl_sync(kAll, base, 0) - mine_n;
-      uint32_t* keys = ex.cluster.map_shared_rank(s_all, owner);
-      uint32_t* indices = ex.cluster.map_shared_rank(s_index, owner);
-#pragma unroll
-      for (int c = 0; c < PER; ++c)
-        if (slots >> c & 1) {
-          if (at < kList) {
+        for (int c = 0; c < PER; ++c)
+          if (slots >> c & 1) {
             keys[at] = key[c];
             indices[at] = first + c / kVec * 32 * kVec + c % kVec;
+            ++at;
           }
-          ++at;
-        }
-    }
-    const uint64_t total_n = shfl64(ex.sum(found), 0);
-    if (total_n <= kList) {
+      }
+      cluster.sync();
       if (ex.rank == owner)
         finish(static_cast<int>(total_n), by_k, by_p, by_k ? 0ull : need);
       return;
@@ -515,6 +553,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     // ---- top-k: keys above the cut, and the first `ties` of those equal to it ----
     if (by_k) {
       const Bound b = search(true, k, 1, top + 1, guess, s);
+      if (ex.dead) return;
       cut = b.key;
       ties = k - b.above;
     }
@@ -524,6 +563,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
       const uint64_t total = shfl64(s, 0) + ties * (cut ? weight(exp_of(cut)) : 0ull);
       const uint64_t want = need_of(total);
       const Bound b = search(false, want, cut ? cut : 1u, top + 1, guess, s);
+      if (ex.dead) return;
       const uint64_t w = weight(exp_of(b.key));
       const uint64_t n = (want - b.above + w - 1) / w;
       ties = b.key == cut && n > ties ? ties : n;
@@ -542,6 +582,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     if (key[c] == cut) ++sums[1];
   }
   ex.sum(sums);
+  if (ex.dead) return;
   const uint64_t w_cut = cut ? keeps(cut) : 0ull;
   auto kept = [&](uint64_t equal, uint64_t before) {  // of `equal` ties after `before` others
     return before >= ties ? 0ull : (ties - before < equal ? ties - before : equal);
@@ -677,8 +718,8 @@ extern "C" int moe_sample_tokens(const moe_sample_tokens_args_t* args) {
   if (!c.logits || !c.uniforms || !c.temperature || !c.top_k || !c.top_p || !c.min_p ||
       !c.tokens || !c.probs)
     return MOE_ERR_INVALID_ARG;
-  SampleArgs a{c.logits,      c.stride, (int)c.vocab, 1,       c.uniforms, c.temperature,
-               c.top_p,       c.min_p,  c.top_k,      c.tokens, c.probs};
+  SampleArgs a{c.logits, c.stride, (int)c.vocab, 1,        c.uniforms, c.temperature,
+               c.top_p,  c.min_p,  c.top_k,      c.tokens, c.probs,    wait_limit_ns()};
   cudaStream_t s = static_cast<cudaStream_t>(c.stream);
   if (c.dtype == MOE_DTYPE_F16) return launch_rows<F16>(a, c.rows, s);
   if (c.dtype == MOE_DTYPE_BF16) return launch_rows<BF16>(a, c.rows, s);
