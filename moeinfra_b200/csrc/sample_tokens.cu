@@ -29,10 +29,10 @@
 //     to one CTA of the cluster, which orders them and applies every filter by
 //     comparing each with each; the others are done.
 //   * Else no sort either: the k-th token and the top-p boundary are found by
-//     search over the keys, 8 ways a pass, over the logits still between the
-//     bounds; register slots that hold none of these for a whole warp are
-//     skipped, and once at most 256 are left every CTA takes a copy and decides
-//     by itself.
+//     search over the keys, 8 ways a pass.  The logits still between the bounds
+//     are gathered in shared memory before each pass, so that it works on full
+//     warps of them, and once at most 256 are left every CTA takes a copy and
+//     decides by itself.
 //   * Exponentials are not kept: the first pass needs every logit's, what
 //     follows only those of the few between the bounds or kept.  That leaves 64
 //     registers a thread and two CTAs to an SM, one's barriers under the other's
@@ -251,7 +251,8 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   using L = Logit<T>;
   constexpr int kVec = L::kVec, kIters = PER / kVec;
   __shared__ uint64_t s_warp[kWarps][8], s_slots[2][kMaxCluster][8];
-  __shared__ uint32_t s_list[kList], s_all[kList], s_index[kList];
+  extern __shared__ uint32_t s_dyn[];  // two lists of kThreads * PER keys
+  __shared__ uint32_t s_all[kList], s_index[kList];
   __shared__ uint64_t s_weight[kList], s_above;
   __shared__ uint32_t s_count[2], s_few, s_key;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -329,35 +330,36 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   };
   if (threadIdx.x == 0) s_count[0] = s_few = 0;
 
-  // Sums of the weights (or counts) of the keys in [lo, hi) that are >= the
-  // threshold t of lane 1 .. 7, as lane j's result.  Lane 0's is what `zero`
-  // says: the sum of those >= its threshold, or how many are in [lo, hi).
-  auto in_range = [&](uint32_t lo, uint32_t hi) {  // slots that hold one
-    uint32_t slots = 0;
+  // Sums of the weights (or counts) of the keys that are >= the threshold t of
+  // lane 0 .. 7, as lane j's result: of all logits, and of a list's, where lane
+  // 0's is the length of all CTAs' lists.
+  auto add = [&](Limbs (&sum)[8], const uint32_t (&th)[8], bool count, uint32_t kk) {
+    Limbs w{0, 1};
+    if (!count) w = limbs(exp_of(kk));
 #pragma unroll
-    for (int c = 0; c < PER; ++c) slots |= (key[c] - lo < hi - lo ? 1u : 0u) << c;
-    return slots;
+    for (int j = 0; j < 8; ++j)
+      if (kk >= th[j]) {
+        sum[j].hi += w.hi;
+        sum[j].lo += w.lo;
+      }
   };
-  auto pass = [&](bool count, uint32_t slots, uint32_t t, bool zero_counts) {
+  auto pass = [&](bool count, uint32_t t) {
     uint32_t th[8];
     Limbs sum[8] = {};
 #pragma unroll
     for (int j = 0; j < 8; ++j) th[j] = __shfl_sync(kAll, t, j);
-    const uint32_t used = __reduce_or_sync(kAll, slots);
 #pragma unroll
-    for (int c = 0; c < PER; ++c) {
-      if (!(used >> c & 1)) continue;
-      Limbs w{0, 1};
-      if (!count) w = limbs(exp_of(key[c]));
-      const uint32_t kk = slots >> c & 1 ? key[c] : 0u;  // below every threshold
+    for (int c = 0; c < PER; ++c) add(sum, th, count, key[c]);
+    return ex.sum(sum);
+  };
+  auto pass_list = [&](bool count, const uint32_t* list, uint32_t n, uint32_t t) {
+    uint32_t th[8];
+    Limbs sum[8] = {};
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (kk >= th[j]) {
-          sum[j].hi += w.hi;
-          sum[j].lo += w.lo;
-        }
-    }
-    if (zero_counts) sum[0] = Limbs{0, (uint32_t)__popc(slots)};
+    for (int j = 0; j < 8; ++j) th[j] = __shfl_sync(kAll, t, j);
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) add(sum, th, count, list[i]);
+    sum[0] = Limbs{0, threadIdx.x == 0 ? n : 0u};
     return ex.sum(sum);
   };
   auto block_sum = [&](uint64_t v) {  // over the CTA, in every thread
@@ -390,6 +392,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   };
   auto search = [&](bool count, uint64_t need, uint32_t lo, uint32_t hi, uint32_t t, uint64_t s) {
     uint64_t above = 0;
+    uint32_t held_n = ~0u;  // keys in the last list
     for (int turn = 0;; turn ^= 1) {
       const uint32_t enough = __ballot_sync(kAll, lane >= 1 && lane < 8 && s >= need) | 1u;
       const int j = 31 - __clz(enough);  // sums fall as thresholds rise
@@ -401,25 +404,31 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
         above = s_hi;
       }
       if (hi - lo <= 1) return Bound{lo, above};
-      // The next pass; and the logits between the bounds into a list, which
-      // decides at once if they turn out to be few.
-      const uint32_t slots = in_range(lo, hi);
-      if (slots) {
-        uint32_t at = atomicAdd(&s_count[turn], __popc(slots));
-        if (at < kList) {
+      // The logits between the bounds, from the registers or the last list.
+      uint32_t *list = s_dyn + turn * kThreads * PER, *counter = &s_count[turn];
+      if (held_n == ~0u) {
+        uint32_t slots = 0;
 #pragma unroll
-          for (int c = 0; c < PER; ++c)
-            if (slots >> c & 1) {
-              if (at < kList) s_list[at] = key[c];
-              ++at;
-            }
+        for (int c = 0; c < PER; ++c) slots |= (key[c] - lo < hi - lo ? 1u : 0u) << c;
+        uint32_t at = slots ? atomicAdd(counter, __popc(slots)) : 0u;
+#pragma unroll
+        for (int c = 0; c < PER; ++c)
+          if (slots >> c & 1) list[at++] = key[c];
+      } else {
+        const uint32_t* from = s_dyn + (turn ^ 1) * kThreads * PER;
+#pragma unroll 1
+        for (uint32_t i = threadIdx.x; i < held_n; i += kThreads) {
+          const uint32_t kk = from[i];
+          if (kk - lo < hi - lo) list[atomicAdd(counter, 1)] = kk;
         }
       }
       if (threadIdx.x == 0) s_count[turn ^ 1] = 0;
+      __syncthreads();
+      held_n = *counter;
       const uint32_t step = (hi - lo + 7) / 8;
       const uint64_t next = (uint64_t)lo + (uint64_t)step * (lane & 7);
       t = next < hi ? (uint32_t)next : hi;
-      s = pass(count, slots, t, true);
+      s = pass_list(count, list, held_n, t);
       const uint64_t n = shfl64(s, 0);
       s += above;
       if (ex.dead) return Bound{lo, above};
@@ -431,9 +440,9 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
           from += held;
           held = (int)ex.slot(r, 0);
         }
-        const uint32_t* list = cluster.map_shared_rank(s_list, warp);
+        const uint32_t* its = cluster.map_shared_rank(list, warp);
         for (int i = lane; i < held; i += 32) {
-          const uint32_t kk = list[i];
+          const uint32_t kk = its[i];
           s_all[from + i] = kk;
           s_weight[from + i] = count ? 1ull : weight(exp_of(kk));
         }
@@ -517,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   uint64_t ties = 0;   // and so many of those equal to it, by index
   const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.f;
   if (by_k || by_p) {
-    uint64_t s = pass(by_k, kAll, (lane & 7) == 0 ? 1u : guess, false);
+    uint64_t s = pass(by_k, (lane & 7) == 0 ? 1u : guess);
     const uint64_t need = by_k ? (uint64_t)k : need_of(shfl64(s, 0));
     // ---- few enough at or above the threshold that holds enough: one CTA takes them ----
     const uint32_t enough = __ballot_sync(kAll, lane >= 1 && lane < 8 && s >= need) | 1u;
@@ -559,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     }
     // ---- top-p ----
     if (by_p) {
-      if (by_k) s = pass(false, kAll, (lane & 7) == 0 ? cut + 1 : guess, false);
+      if (by_k) s = pass(false, (lane & 7) == 0 ? cut + 1 : guess);
       const uint64_t total = shfl64(s, 0) + ties * (cut ? weight(exp_of(cut)) : 0ull);
       const uint64_t want = need_of(total);
       const Bound b = search(false, want, cut ? cut : 1u, top + 1, guess, s);
@@ -659,7 +668,9 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
 template <typename T, int PER>
 bool sample_attr() {
   return cudaFuncSetAttribute(k_sample<T, PER>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) ==
-         cudaSuccess;
+             cudaSuccess &&
+         cudaFuncSetAttribute(k_sample<T, PER>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              2 * kThreads * PER * 4) == cudaSuccess;
 }
 
 template <typename T, int PER>
@@ -669,6 +680,7 @@ int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * a.cluster));
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = 2 * kThreads * PER * 4;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
