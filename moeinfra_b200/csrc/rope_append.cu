@@ -30,14 +30,24 @@ struct RopeArgs {
   int heads;
 };
 
-constexpr int kRopeThreads = 256;
+constexpr int kMaxThreads = 512;
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kRopeThreads) k_rope_append(const RopeArgs a) {
+__global__ void __launch_bounds__(kMaxThreads) k_rope_append(const RopeArgs a) {
   pdl_trigger();
   pdl_wait();
   constexpr int kPer = HD / 16;  // threads a head takes
   const int64_t t = blockIdx.x;
+  const int items = (a.heads + 2 * a.kv.kv_heads) * kPer;
+  // The first row pieces are on their way while the position, then the page
+  // and the angles are looked up.
+  const uint16_t* row = a.qkv + t * a.qkv_stride;
+  auto source = [&](int i) { return row + (int64_t)(i / kPer) * HD + i % kPer * 8; };
+  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+  if (threadIdx.x < items) {
+    lo = *reinterpret_cast<const uint4*>(source(threadIdx.x));
+    hi = *reinterpret_cast<const uint4*>(source(threadIdx.x) + HD / 2);
+  }
   const int32_t pos = a.positions[t];
   const int32_t seq = a.seq_ids ? a.seq_ids[t] : static_cast<int32_t>(t);
   // The token's slot: page >= 0, or -1 for a padding token (position < 0) and
@@ -52,8 +62,11 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const RopeArgs a) 
     if (page < 0 && threadIdx.x == 0) set_device_error(kErrPage);
   }
   const int slot = page < 0 ? 0 : pos % a.kv.page_size;
-  const int items = (a.heads + 2 * a.kv.kv_heads) * kPer;
-  for (int i = threadIdx.x; i < items; i += kRopeThreads) {
+  for (int i = threadIdx.x; i < items; i += blockDim.x) {
+    if (i != threadIdx.x) {
+      lo = *reinterpret_cast<const uint4*>(source(i));
+      hi = *reinterpret_cast<const uint4*>(source(i) + HD / 2);
+    }
     const int head = i / kPer, c = (i % kPer) * 8;
     const int kv_head = head - a.heads;  // < 0: a query head; >= kv_heads: a value head
     uint16_t *dst, *copy = nullptr;
@@ -64,30 +77,27 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const RopeArgs a) 
       if (a.k_out && !val) copy = a.k_out + (t * a.kv.kv_heads + kv_head) * HD;
       if (page < 0 && !copy) continue;
       const int j = val ? kv_head - a.kv.kv_heads : kv_head;
-      dst = (val ? a.kv.v + page * a.kv.v_stride : a.kv.k + page * a.kv.k_stride) +
+      const int64_t at = page < 0 ? 0 : page;
+      dst = (val ? a.kv.v + at * a.kv.v_stride : a.kv.k + at * a.kv.k_stride) +
             ((int64_t)j * a.kv.page_size + slot) * HD;
     }
-    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-    if (page >= 0) {
-      const uint16_t* src = a.qkv + t * a.qkv_stride + (int64_t)head * HD + c;
-      lo = *reinterpret_cast<const uint4*>(src);
-      hi = *reinterpret_cast<const uint4*>(src + HD / 2);
-      if (kv_head < a.kv.kv_heads) {
-        const float4* cp = reinterpret_cast<const float4*>(a.cos + (int64_t)pos * (HD / 2) + c);
-        const float4* sp = reinterpret_cast<const float4*>(a.sin + (int64_t)pos * (HD / 2) + c);
-        uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
-        uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
+    if (page < 0) {
+      lo = hi = make_uint4(0, 0, 0, 0);
+    } else if (kv_head < a.kv.kv_heads) {
+      const float4* cp = reinterpret_cast<const float4*>(a.cos + (int64_t)pos * (HD / 2) + c);
+      const float4* sp = reinterpret_cast<const float4*>(a.sin + (int64_t)pos * (HD / 2) + c);
+      uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
+      uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const float4 cs = __ldg(cp + v), sn = __ldg(sp + v);
+      for (int v = 0; v < 2; ++v) {
+        const float4 cs = __ldg(cp + v), sn = __ldg(sp + v);
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const float c0 = w ? cs.z : cs.x, c1 = w ? cs.w : cs.y;
-            const float s0 = w ? sn.z : sn.x, s1 = w ? sn.w : sn.y;
-            const float2 x = T::unpack(l[2 * v + w]), y = T::unpack(h[2 * v + w]);
-            l[2 * v + w] = T::pack(x.x * c0 - y.x * s0, x.y * c1 - y.y * s1);
-            h[2 * v + w] = T::pack(y.x * c0 + x.x * s0, y.y * c1 + x.y * s1);
-          }
+        for (int w = 0; w < 2; ++w) {
+          const float c0 = w ? cs.z : cs.x, c1 = w ? cs.w : cs.y;
+          const float s0 = w ? sn.z : sn.x, s1 = w ? sn.w : sn.y;
+          const float2 x = T::unpack(l[2 * v + w]), y = T::unpack(h[2 * v + w]);
+          l[2 * v + w] = T::pack(x.x * c0 - y.x * s0, x.y * c1 - y.y * s1);
+          h[2 * v + w] = T::pack(y.x * c0 + x.x * s0, y.y * c1 + x.y * s1);
         }
       }
     }
@@ -103,8 +113,13 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const RopeArgs a) 
 
 template <typename T, int HD>
 int launch_rope(const RopeArgs& a, int64_t tokens, cudaStream_t s) {
-  if (launch_pdl(k_rope_append<T, HD>, dim3(static_cast<unsigned>(tokens)), dim3(kRopeThreads), 0,
-                 s, a) != cudaSuccess)
+  // A thread per piece of the row and equal rounds: 32 + 16 heads of 128 are one
+  // round of 384 threads.
+  const int items = (a.heads + 2 * a.kv.kv_heads) * (HD / 16);
+  const int rounds = (items + kMaxThreads - 1) / kMaxThreads;
+  const int threads = ((items + rounds - 1) / rounds + 31) / 32 * 32;
+  if (launch_pdl(k_rope_append<T, HD>, dim3(static_cast<unsigned>(tokens)), dim3(threads), 0, s, a) !=
+      cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
   return MOE_OK;
