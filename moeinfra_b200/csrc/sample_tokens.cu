@@ -18,16 +18,18 @@
 // bits below the maximum leave every weight that has a chance to be drawn
 // fp32's precision, and 2^18 of them fit 64 bits with room to spare.
 //
-// Bound by latency where rows are few (a row is 64 KB at 32000 fp16 logits; the
-// rest is a chain of reductions), by instruction issue where they are many.  A
-// row is spread over a cluster of CTAs whose threads hold it in registers, as
-// integers of the same order ("keys"):
+// Many rows, or short ones, take a CTA each (sample_rows.cuh).  Here a row is
+// spread over a cluster of CTAs whose threads hold it in registers, as integers of
+// the same order ("keys").  Such a call is a chain of reductions and bound by their
+// latency: 11.3 us for one row of 32000 fp16 logits (64 KB), of which a plain copy
+// would take 0.01; 26 for one of 131072 fp32.
 //   * A first pass adds each weight to the sums of 7 thresholds (21
 //     instructions a logit), 0.5 to 16 below the maximum in units of the
 //     temperature, where a language model's boundaries usually lie.  If then at
 //     most 256 logits are above the threshold that already holds enough, they go
 //     to one CTA of the cluster, which orders them and applies every filter by
-//     comparing each with each; the others are done.
+//     comparing each with each (more would cost it longer than another pass); the
+//     others are done.
 //   * Else no sort either: the k-th token and the top-p boundary are found by
 //     search over the keys, 8 ways a pass.  The logits still between the bounds
 //     are gathered in shared memory before each pass, so that it works on full
@@ -37,14 +39,15 @@
 //     follows only those of the few between the bounds or kept.  That leaves 64
 //     registers a thread and two CTAs to an SM, one's barriers under the other's
 //     arithmetic.
-//   * Between passes the CTAs exchange sums, which is most of a small call: each
+//   * Between passes the CTAs exchange sums, which is most of a call: each
 //     stores its 8 into every CTA's shared memory with st.async, whose bytes
 //     complete an mbarrier there (a cluster barrier behind plain stores took 2000
-//     cycles, this a third).  Waits are bounded: on a timeout the error word is
-//     set and the CTA returns, as then do the others.
+//     cycles, this a third: 13.3 -> 12.0 us for the one row).  Waits are bounded:
+//     on a timeout the error word is set and the CTA returns, as then do the others.
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
+#include "sample_rows.cuh"
 #include "sm100_ptx.cuh"
 
 namespace moe {
@@ -59,78 +62,6 @@ constexpr int kMaxCluster = 16;            // 8 is the portable size; 16 only wh
 constexpr int kMaxPer = 32;                // logits a thread holds at most
 constexpr int kList = 256;                 // logits that a search finishes with directly
 constexpr int kMaxVocab = kMaxCluster * kThreads * kMaxPer;
-constexpr uint32_t kAll = 0xffffffffu;
-
-struct SampleArgs {
-  const void* logits;
-  int64_t stride;
-  int vocab, cluster;
-  const float *uniforms, *temperature, *top_p, *min_p;
-  const int32_t* top_k;
-  int64_t* tokens;
-  float* probs;
-  uint64_t wait_ns;
-};
-
-// Logits as keys: unsigned integers of the same order, NaN as -inf, -0 as 0.
-// Every key is above 0, which stands for "no logit".
-template <typename T>
-struct Logit;
-struct Half16 {
-  using Raw = uint16_t;
-  static constexpr int kVec = 8;
-  // `inf`: the format's infinity, above which are NaNs.
-  static __device__ __forceinline__ uint32_t key(uint32_t b, uint32_t inf) {
-    if ((b & 0x7FFFu) > inf) b = 0x8000u | inf;
-    if (b == 0x8000u) b = 0;
-    return b & 0x8000u ? (~b & 0xFFFFu) : (b | 0x8000u);
-  }
-  static __device__ __forceinline__ uint32_t raw(uint32_t k) {
-    return k & 0x8000u ? (k & 0x7FFFu) : (~k & 0xFFFFu);
-  }
-};
-template <>
-struct Logit<F16> : Half16 {
-  static __device__ __forceinline__ uint32_t key(uint16_t b) { return Half16::key(b, 0x7C00u); }
-  static __device__ __forceinline__ float value(uint32_t k) { return h2f((uint16_t)raw(k)); }
-  static __device__ __forceinline__ uint32_t key_near(float x) { return key(f2h(x)); }
-};
-template <>
-struct Logit<BF16> : Half16 {
-  static __device__ __forceinline__ uint32_t key(uint16_t b) { return Half16::key(b, 0x7F80u); }
-  static __device__ __forceinline__ float value(uint32_t k) { return __uint_as_float(raw(k) << 16); }
-  static __device__ __forceinline__ uint32_t key_near(float x) { return key(BF16::one(x)); }
-};
-template <>
-struct Logit<float> {
-  using Raw = float;
-  static constexpr int kVec = 4;
-  static __device__ __forceinline__ uint32_t key(float x) {
-    if (x != x) x = -INFINITY;
-    const uint32_t b = __float_as_uint(x + 0.f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-  }
-  static __device__ __forceinline__ float value(uint32_t k) {
-    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
-  }
-  static __device__ __forceinline__ uint32_t key_near(float x) { return key(x); }
-};
-
-__device__ __forceinline__ uint64_t shfl64(uint64_t v, int lane) { return __shfl_sync(kAll, v, lane); }
-// trunc(2^40 e) for e in [0, 1] as two limbs of 20 bits (every step is exact): a
-// thread adds up to kMaxPer of each, a warp 32 times that, in 32 bits.
-struct Limbs {
-  uint32_t hi, lo;
-};
-__device__ __forceinline__ Limbs limbs(float e) {
-  const float x = e * 1048576.f;
-  const uint32_t hi = __float2uint_rz(x);
-  return Limbs{hi, __float2uint_rz((x - __uint2float_rz(hi)) * 1048576.f)};
-}
-__device__ __forceinline__ uint64_t weight(float e) {
-  const Limbs w = limbs(e);
-  return ((uint64_t)w.hi << 20) + w.lo;
-}
 
 __device__ __forceinline__ uint32_t map_rank(uint32_t addr, int rank) {
   uint32_t a;
@@ -316,17 +247,9 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     return;
   }
   const float m = L::value(top);
-  // (x - m) / temperature by the reciprocal, corrected twice by the remainder
-  // (Markstein 1990: the result is the correctly rounded quotient); below -104
-  // the exponential is 0, and a reciprocal out of range ends there too.
-  const float inverse = __frcp_rn(temperature);
-  const float divisor = inverse != 0.f ? temperature : 0.f;  // infinite: nothing to correct
-  auto exp_of = [&](uint32_t key) {  // key 0 is a NaN
-    const float d = L::value(key) - m, q0 = d * inverse;
-    float q = fmaf(fmaf(-q0, divisor, d), inverse, q0);
-    q = fmaf(fmaf(-q, divisor, d), inverse, q);
-    const float e = expf(q);
-    return key == top ? 1.f : (q0 >= -104.f ? e : 0.f);
+  const Softmax soft(m, temperature);
+  auto exp_of = [&](uint32_t key) {  // key 0 is a NaN; m may be infinite
+    return key == top ? 1.f : soft.exp(L::value(key));
   };
   if (threadIdx.x == 0) s_count[0] = s_few = 0;
 
@@ -361,27 +284,6 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) add(sum, th, count, list[i]);
     sum[0] = Limbs{0, threadIdx.x == 0 ? n : 0u};
     return ex.sum(sum);
-  };
-  auto block_sum = [&](uint64_t v) {  // over the CTA, in every thread
-    const uint32_t lo = __reduce_add_sync(kAll, (uint32_t)v & 0x7FFFFFFu);
-    const uint32_t hi = __reduce_add_sync(kAll, (uint32_t)(v >> 27));
-    __syncthreads();
-    if (lane == 0) s_warp[warp][0] = lo + ((uint64_t)hi << 27);
-    __syncthreads();
-    uint64_t s = s_warp[lane & (kWarps - 1)][0];
-#pragma unroll
-    for (int o = kWarps / 2; o; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
-    return s;
-  };
-  auto need_of = [&](uint64_t total) {  // what top-p asks for
-    const double want = ceil(__dmul_rn((double)p, __ull2double_rn(total)));
-    const uint64_t n = want >= 1.0 ? __double2ull_rz(want) : 1ull;
-    return n < total ? n : total;
-  };
-  auto draw_of = [&](uint64_t total) {  // the point of the kept weights that u stands for
-    const double at = floor(__dmul_rn((double)u, __ull2double_rn(total)));
-    const uint64_t r = at >= 1.0 ? __double2ull_rz(at) : 0ull;
-    return r < total ? r : total - 1;
   };
   // The largest key whose sum over it and all above is >= need, and the sum
   // above it.  t, s: thresholds of a first pass (rising with the lane, lane 0
@@ -471,48 +373,6 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
       return Bound{s_key, s_above};
     }
   };
-  // The first n of s_all / s_index hold every logit the filters may keep: apply
-  // them and draw.  Two threads per logit compare it with half of the others
-  // each.  need: what top-p asks for where top-k does not come first.
-  auto finish = [&](int n, bool by_k, bool by_p, uint64_t need) {
-    const int i = threadIdx.x >> 1, half = threadIdx.x & 1;
-    const bool real = i < n;
-    const uint32_t own = real ? s_all[i] : 0u, index = real ? s_index[i] : 0u;
-    const float e = exp_of(own);
-    uint64_t w = real ? weight(e) : 0ull;
-    if (real && half == 0) s_weight[i] = w;
-    __syncthreads();
-    uint32_t place = 0;   // in the order by falling logit and rising index
-    uint64_t before = 0;  // weights ahead of it
-    if (real)
-      for (int j = half; j < n; j += 2) {
-        const uint32_t kk = s_all[j];
-        const bool ahead = kk > own || (kk == own && s_index[j] < index);
-        place += ahead;
-        before += ahead ? s_weight[j] : 0ull;
-      }
-    place += __shfl_xor_sync(kAll, place, 1);
-    before += __shfl_xor_sync(kAll, before, 1);
-    bool keep = real && (!by_k || place < (uint32_t)k);
-    if (by_k && by_p) {
-      const uint64_t v[1] = {keep && half == 0 ? w : 0ull};
-      need = need_of(block_sum(v[0]));
-    }
-    keep = keep && (!by_p || before < need) && e >= min_p;
-    if (!keep) w = 0;
-    const uint64_t total = block_sum(half == 0 ? w : 0ull);  // its barriers order s_weight too
-    if (real && half == 0) s_weight[i] = w;
-    __syncthreads();
-    uint64_t run = 0;  // kept weights of lower indices
-    if (keep)
-      for (int j = half; j < n; j += 2) run += s_index[j] < index ? s_weight[j] : 0ull;
-    run += __shfl_xor_sync(kAll, run, 1);
-    const uint64_t r = draw_of(total);
-    if (keep && half == 0 && r >= run && r < run + w) {
-      a.tokens[row] = index;
-      a.probs[row] = (float)(__ull2double_rn(w) / __ull2double_rn(total));
-    }
-  };
   // First thresholds: lane 7 the nearest to the maximum.
   const float reach[8] = {0.f, 16.f, 11.f, 8.f, 5.5f, 3.5f, 1.75f, 0.5f};
   float mine = 0.f;
@@ -527,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.f;
   if (by_k || by_p) {
     uint64_t s = pass(by_k, (lane & 7) == 0 ? 1u : guess);
-    const uint64_t need = by_k ? (uint64_t)k : need_of(shfl64(s, 0));
+    const uint64_t need = by_k ? (uint64_t)k : need_of(p, shfl64(s, 0));
     // ---- few enough at or above the threshold that holds enough: one CTA takes them ----
     const uint32_t enough = __ballot_sync(kAll, lane >= 1 && lane < 8 && s >= need) | 1u;
     const int j = 31 - __clz(enough);
@@ -556,7 +416,8 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
       }
       cluster.sync();
       if (ex.rank == owner)
-        finish(static_cast<int>(total_n), by_k, by_p, by_k ? 0ull : need);
+        finish_few<kThreads, kList>(a, row, (int)total_n, s_all, s_index, s_weight, by_k ? k : 0, p,
+                                    min_p, by_k ? 0ull : need, u, exp_of, &s_warp[0][0]);
       return;
     }
     // ---- top-k: keys above the cut, and the first `ties` of those equal to it ----
@@ -570,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     if (by_p) {
       if (by_k) s = pass(false, (lane & 7) == 0 ? cut + 1 : guess);
       const uint64_t total = shfl64(s, 0) + ties * (cut ? weight(exp_of(cut)) : 0ull);
-      const uint64_t want = need_of(total);
+      const uint64_t want = need_of(p, total);
       const Bound b = search(false, want, cut ? cut : 1u, top + 1, guess, s);
       if (ex.dead) return;
       const uint64_t w = weight(exp_of(b.key));
@@ -593,34 +454,12 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   ex.sum(sums);
   if (ex.dead) return;
   const uint64_t w_cut = cut ? keeps(cut) : 0ull;
-  auto kept = [&](uint64_t equal, uint64_t before) {  // of `equal` ties after `before` others
-    return before >= ties ? 0ull : (ties - before < equal ? ties - before : equal);
-  };
-  // Sums of pieces in order (lane i: piece i's weight above the cut and its ties)
-  // -> kept weight and ties before the piece, its kept weight, all kept weight.
-  struct Piece {
-    uint64_t before, ties_before, own, all;
-  };
-  auto place = [&](uint64_t w, uint64_t equal, uint64_t ties_ahead) {
-    uint64_t seen = equal;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t v = __shfl_up_sync(kAll, seen, o);
-      if (lane >= o) seen += v;
-    }
-    seen += ties_ahead - equal;
-    const uint64_t own = w + kept(equal, seen) * w_cut;
-    uint64_t run = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t v = __shfl_up_sync(kAll, run, o);
-      if (lane >= o) run += v;
-    }
-    return Piece{run - own, seen, own, shfl64(run, 31)};
+  auto place = [&](uint64_t w, uint64_t equal, uint64_t ahead) {
+    return place_pieces(w, equal, ahead, ties, w_cut);
   };
   const bool is_cta = lane < a.cluster;
   const Piece ctas = place(is_cta ? ex.slot(lane, 0) : 0ull, is_cta ? ex.slot(lane, 1) : 0ull, 0);
-  const uint64_t total = ctas.all, r = draw_of(total);
+  const uint64_t total = ctas.all, r = draw_of(u, total);
   const uint64_t cta_before = shfl64(ctas.before, ex.rank), cta_own = shfl64(ctas.own, ex.rank);
   if (r < cta_before || r >= cta_before + cta_own) return;
   // ---- the CTA that holds the token: its warp, step, lane, element ----
@@ -695,21 +534,17 @@ int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t s) {
   return MOE_OK;
 }
 
-// CTAs of a row and logits of a thread: 8 logits, and so more CTAs, while all
-// rows' CTAs fit the GPU at once (two to an SM); else 16 (a cluster of up to 16
-// CTAs where a row needs it); 32 and one CTA to an SM for the longest rows.
+// One CTA a row where rows are many or short.  Measured with mixed parameters
+// (cluster / one CTA, us): 2 x 16000 12.3 / 10.9, 16 x 16000 25.9 / 19.6; 24 x
+// 32000 30.5 / 31.2, 48 x 32000 45.5 / 32.4; 32 x 131072 66.7 / 91.5, 64 x 131072
+// 107 / 100, 256 x 131072 406 / 161; 1 x 32000 11.4 / 18.4.
+// In a cluster 8 logits a thread, and so more CTAs, as far as 8 CTAs go; then 16
+// (a cluster of up to 16 CTAs); 32 and one CTA to an SM for the longest rows.
 template <typename T>
 int launch_rows(SampleArgs& a, int64_t rows, cudaStream_t s) {
-  int per = 8;
-  auto ctas = [&](int n) {
-    int c = 1;
-    while ((int64_t)c * kThreads * n < a.vocab) c *= 2;
-    return c;
-  };
-  if (ctas(8) > 8 || rows * ctas(8) > 2 * sm_count()) per = 16;
-  if (ctas(16) > kMaxCluster) per = 32;
-  a.cluster = ctas(per);
-  if (rows * a.cluster > INT32_MAX) return MOE_ERR_UNSUPPORTED;
+  if (a.vocab <= 16384 || rows >= 20 + a.vocab / 4096) return launch_sample_rows<T>(a, rows, s);
+  const int per = a.vocab <= 8 * kThreads * 8 ? 8 : a.vocab <= kMaxCluster * kThreads * 16 ? 16 : 32;
+  a.cluster = a.vocab <= 8 * kThreads * per ? 8 : kMaxCluster;
   if (per == 8) return launch_sample<T, 8>(a, rows, s);
   if (per == 16) return launch_sample<T, 16>(a, rows, s);
   return launch_sample<T, 32>(a, rows, s);

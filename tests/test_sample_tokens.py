@@ -244,3 +244,52 @@ def test_wrapper_refuses_wrong_shapes_and_types():
                 dict(p=one.double()), dict(m=one[:1]), dict(x=x.t()), dict(u=one[:, None])):
         with pytest.raises(ValueError):
             sample(**bad)
+
+
+# Long rows, few of them and many: a row over several CTAs, and in one.
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(6, 20001), (40, 20001), (3, 70000), (40, 70000)])
+def test_long_rows_of_few_values(dtype, rows, vocab):
+    """Boundaries among thousands of equal logits, and of nearly equal ones."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    steps = torch.randint(0, 5, (rows, vocab), device="cuda", generator=g).float()
+    near = 4.0 + 1e-3 * torch.rand(rows, vocab, device="cuda", generator=g)
+    u = torch.rand(rows, device="cuda", generator=g)
+    for x in (steps.to(dtype), near.to(dtype), torch.zeros_like(steps).to(dtype)):
+        for kw in (dict(), dict(top_k=37), dict(top_p=0.7), dict(top_k=5000, top_p=0.31),
+                   dict(top_k=vocab - 1, top_p=0.999, min_p=0.2), dict(temperature=0.0)):
+            _compare(x, u, _params(rows, **kw))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [6, 60])
+def test_long_rows_of_infinities_and_nan(dtype, rows):
+    inf, nan = float("inf"), float("nan")
+    big = torch.finfo(dtype).max
+    heads = [[-inf, 1.0, 2.0, -inf], [nan, 1.0, 0.0, nan], [-inf] * 4, [inf, 1.0, inf, -inf],
+             [-big, -big, big, 0.0], [-big] * 4]
+    x = torch.full((rows, 20000), -inf, device="cuda")
+    x[:, 1::3] = nan
+    x[:, 9998:10002] = torch.tensor(heads, device="cuda").repeat(rows // 6, 1)
+    x = x.to(dtype)
+    u = (torch.arange(rows, device="cuda") + 0.5) / rows
+    for kw in (dict(), dict(top_k=2), dict(top_p=0.6), dict(min_p=0.3), dict(temperature=0.0),
+               dict(temperature=1e6, top_k=3, top_p=0.8), dict(temperature=3e38),
+               dict(temperature=1e-38), dict(temperature=1e-45, top_p=0.9)):
+        tokens, _ = _compare(x, u, _params(rows, **kw))
+        assert tokens.min() >= 0 and tokens.max() < 20000
+
+
+@gpu
+@pytest.mark.parametrize("top_k,top_p,min_p", [(0, 0.999, 0.0), (3000, 1.0, 0.0), (20000, 0.98, 0.0),
+                                               (0, 0.99, 1e-3), (300, 0.5, 0.0), (0, 0.01, 0.0)])
+def test_many_kept(top_k, top_p, min_p):
+    """More candidates than the lists hold, just as many, and few, in one call."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    rows, vocab = 60, 50000
+    x = torch.randn(rows, vocab, device="cuda", generator=g)
+    x *= torch.linspace(0.05, 6.0, rows, device="cuda")[:, None]
+    u = torch.rand(rows, device="cuda", generator=g)
+    _compare(x, u, _params(rows, 1.0, top_k, top_p, min_p))
