@@ -77,11 +77,16 @@ struct Limbs {
   uint32_t hi, lo;
   __device__ __forceinline__ uint64_t value() const { return ((uint64_t)hi << 20) + lo; }
 };
-__device__ __forceinline__ Limbs limbs(float e) {
+constexpr uint32_t kLimbBias = 0x4B000000u;  // the bits of 2^23
+__device__ __forceinline__ Limbs limbs_biased(float e) {
   const float scale = 1048576.f, whole = 8388608.f;
   const float hi = __fmaf_rz(e, scale, whole);
   const float lo = __fmaf_rz(fmaf(e, scale, whole - hi), scale, whole);
-  return Limbs{__float_as_uint(hi) & 0x7FFFFFu, __float_as_uint(lo) & 0x7FFFFFu};
+  return Limbs{__float_as_uint(hi), __float_as_uint(lo)};
+}
+__device__ __forceinline__ Limbs limbs(float e) {
+  const Limbs w = limbs_biased(e);
+  return Limbs{w.hi - kLimbBias, w.lo - kLimbBias};
 }
 __device__ __forceinline__ uint64_t weight(float e) { return limbs(e).value(); }
 
@@ -95,17 +100,15 @@ struct Softmax {
     divisor = inverse != 0.f ? temperature : 0.f;  // infinite: nothing to correct
     rest = inverse * fmaf(-inverse, divisor, 1.f);
   }
-  // The quotient where it is `in` range; below -104 the exponential is 0, and a
-  // reciprocal out of range and NaNs end there too.
-  __device__ __forceinline__ float quotient(float x, bool& in) const {
+  // NaN where it, or a reciprocal, is out of range.
+  __device__ __forceinline__ float quotient(float x) const {
     const float d = x - m, q = fmaf(d, inverse, d * rest);
-    in = q >= -104.f;
     return fmaf(fmaf(-q, divisor, d), inverse, q);
   }
-  __device__ __forceinline__ float exp(float x) const {  // 0 for a NaN; m finite
-    bool in;
-    const float e = expf(quotient(x, in));
-    return in ? e : 0.f;
+  // m finite.  Below -104 it is 0, and what is NaN there is too.
+  __device__ __forceinline__ float exp(float x) const {
+    const float q = quotient(x), e = expf(q);
+    return q >= -104.f ? e : 0.f;
   }
 };
 

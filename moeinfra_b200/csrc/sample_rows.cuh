@@ -13,14 +13,14 @@
 //     they do not fit, sums of contiguous parts of the row, and of parts of the part.
 // Sums are exact integers: the order in which atomics add them does not matter.
 //
-// Bound by instruction issue.  256 x 131072 fp32 of mixed parameters: 161 us, 134
-// MB, which a plain copy's rate would read in 21 (greedy rows alone: 36 us; no
-// filter: 90; top-p 0.95: 185).  Counted over such a call of top-p 0.95, 120
-// instructions a logit at 67 % of the issue slots.  What costs: the exponential of
-// a correctly rounded quotient and its 40 bits, in each of two passes.  64 x 32000
-// fp16: 33 us, as long as the slowest row's CTA (the histogram of a row 7.5 us).
-// 1024 threads and one CTA to an SM; with 512 and two, 64 x 32000 took 36 us and
-// 256 x 131072 194.  Bins in two copies, for fewer conflicts: no faster.
+// Bound by instruction issue.  256 x 131072 fp32 of mixed parameters: 128 us, 134
+// MB, which a plain copy's rate would read in 21 (greedy rows alone: 35).  What
+// costs: the exponential of a correctly rounded quotient and its 40 bits, in each
+// of two passes (13 and 15 cycles an SM for 32 logits, at two thirds of the issue
+// slots).  64 x 32000 fp16: 32 us, as long as the slowest row's CTA, 7.5 of them
+// its histogram.  1024 threads and one CTA to an SM; with 512 and two, 64 x 32000
+// took 4 us longer and 256 x 131072 32.  Bins in two copies, for fewer conflicts:
+// no faster.  Four pieces on their way in the first pass, not one: 26 us less.
 #pragma once
 
 #include "sample.cuh"
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
   if (threadIdx.x < 2) s_n[threadIdx.x] = 0;
   float m = -INFINITY;
   int where = INT_MAX;
-  each(from, to, [&](const float (&v)[kVec], int at) {
+  auto see = [&](const float (&v)[kVec], int at) {
     float most = v[0];
 #pragma unroll
     for (int j = 1; j < kVec; ++j) most = fmaxf(most, v[j]);
@@ -124,7 +124,19 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
       m = fmaxf(most, -INFINITY);
       where = at;
     }
-  });
+  };
+#pragma unroll 1
+  for (int at = from + lane * kVec; at - lane * kVec < to; at += 4 * kStep) {
+    uint4 raw[4];  // four pieces on their way: memory's latency
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = load(at + i * kStep, to);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v[kVec];
+      unpack(raw[i], at + i * kStep, to, v);
+      see(v, at + i * kStep);
+    }
+  }
   {
     const uint32_t own = Logit<float>::key(m);
     const uint32_t top = __reduce_max_sync(kAll, own);
@@ -158,9 +170,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
   // overlap.  Added to 2^23, a number leaves its whole part in the sum's low bits.
   auto bin_at = [&](float q) { return __float_as_uint(fmaf(-q, kBinsPerUnit, 8388608.f)) - 0x4B000000u; };
   auto bin_of = [&](float v) {
-    bool in;
-    const float q = soft.quotient(v, in);
-    return in ? (int)min(bin_at(q), kBins - 1u) : kBins - 1;
+    const float q = soft.quotient(v);
+    return q >= -32.f ? (int)min(bin_at(q), kBins - 1u) : kBins - 1;
   };
   // The lowest key whose bin is at most `bin`, by one warp, 5 bits at a time from
   // what the division undone gives, a bin's width and two keys to either side.
@@ -189,6 +200,19 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
     const uint32_t low = (uint32_t)w, carry = atomicAdd(&s_lo[bin], low) + low < low;
     const uint32_t high = (uint32_t)(w >> 32) + carry;
     if (high) atomicAdd(&s_hi[bin], high);
+  };
+  // The weights of a piece's logits above `cut` (NaN: of all) that min-p keeps.  An
+  // overflowed quotient has the exponential NaN, which nothing keeps.
+  auto add_up = [&](Limbs& sum, const float (&v)[kVec], float cut) {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const float e = expf(soft.quotient(v[j]));
+      const Limbs w = limbs_biased(e >= min_p && !(v[j] <= cut) ? e : 0.f);
+      sum.hi += w.hi;
+      sum.lo += w.lo;
+    }
+    sum.hi -= kVec * kLimbBias;
+    sum.lo -= kVec * kLimbBias;
   };
   // The first bin with which the sum reaches `need` (0: what top-p asks of the
   // total), then known to every thread; leaves the bins empty.
@@ -251,27 +275,33 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
 #pragma unroll
           for (int j0 = 0; j0 < kVec; j0 += 4) {
             // Four at a time: an atomic's result (for the carry) takes a while.
-            uint32_t high[4] = {}, low[4], old[4] = {}, bin[4];
+            uint32_t low[4], old[4] = {}, bin[4];
+            float e[4], most = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float x = v[j0 + j];
-              bool in;
-              const float q = soft.quotient(x, in), e = expf(q);
-              const Limbs w = limbs(e);
+              const float x = v[j0 + j], q = soft.quotient(x);
+              e[j] = expf(q);  // NaN where the quotient overflowed
+              const Limbs w = limbs(e[j]);
               low[j] = (w.hi << 20) + w.lo;
               bin[j] = bin_at(q);
-              if (in && e >= kLeast && !(x <= cut.x)) {
+              if (e[j] >= kLeast && !(x <= cut.x)) {
                 old[j] = atomicAdd(&s_lo[bin[j]], low[j]);
-                high[j] = w.hi >> 12;
+                most = fmaxf(most, e[j]);
+              } else {
+                low[j] = 0;
+                e[j] = 0.f;
               }
             }
-            uint32_t any = 0;
+            bool carry = false;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) any |= high[j] += old[j] + low[j] < low[j];
-            if (any)
+            for (int j = 0; j < 4; ++j) carry |= old[j] + low[j] < low[j];
+            if (carry || most >= 1.f / 256) {  // else the weights are below 2^32
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (high[j]) atomicAdd(&s_hi[bin[j]], high[j]);
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t high = (limbs(e[j]).hi >> 12) + (old[j] + low[j] < low[j]);
+                if (high) atomicAdd(&s_hi[bin[j]], high);
+              }
+            }
           }
         });
         if (threadIdx.x == 0 && at_cut) add(bin_of(cut.x), at_cut);
@@ -288,7 +318,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
       // has no place ----
       const bool last = !count || !(p < 1.f);
       const float x_lo = fmaxf(L::value(lo), count ? -INFINITY : cut.x);
-      const float x_hi = found.bin ? L::value(hi) : INFINITY;  // nothing reaches it
+      const float x_hi = L::value(hi - 1);
       Limbs sum{0, 0};
       each(from, to, [&](const float (&v)[kVec], int at) {
         float most = v[0];
@@ -296,30 +326,32 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
         for (int j = 1; j < kVec; ++j) most = fmaxf(most, v[j]);
         if (!__any_sync(kAll, most >= x_lo)) return;
         uint32_t in[2] = {0, 0};
+        const bool full = *(volatile int*)&s_n[0] > kHeld;
+        if (full && last) {
+          add_up(sum, v, x_hi);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          in[0] |= (v[j] >= x_hi ? 1u : 0u) << j;
-          in[1] |= (v[j] >= x_lo && !(v[j] >= x_hi) ? 1u : 0u) << j;
+          for (int j = 0; j < kVec; ++j) in[0] |= (v[j] > x_hi ? 1u : 0u) << j;
         }
-        uint32_t out = 0;  // above the bin, but without a place
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) in[1] |= (v[j] >= x_lo && v[j] <= x_hi ? 1u : 0u) << j;
+        uint32_t out = in[0];  // above the bin, but without a place
 #pragma unroll
         for (int l = 0; l < 2; ++l) {
-          if (!in[l]) continue;
-          int slot = kHeld;
-          if (*(volatile int*)&s_n[l] <= kHeld) slot = atomicAdd(&s_n[l], __popc(in[l]));
+          if (!in[l] || *(volatile int*)&s_n[l] > kHeld) continue;
+          int slot = atomicAdd(&s_n[l], __popc(in[l]));
 #pragma unroll
           for (int j = 0; j < kVec; ++j)
             if (in[l] >> j & 1) {
               if (slot < kHeld) {
                 s_x[l][slot] = v[j];
                 s_at[l][slot] = at + j;
-              } else if (l == 0) {
-                out |= 1u << j;
+                if (l == 0) out &= ~(1u << j);
               }
               ++slot;
             }
         }
-        if (last && __any_sync(kAll, out)) {
+        if (last && __any_sync(kAll, out)) {  // the list has just become full
 #pragma unroll
           for (int j = 0; j < kVec; ++j) {
             const float e = soft.exp(v[j]);
@@ -497,13 +529,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
     } else {
       Limbs own{0, 0};  // of at most 2^9 logits
       each(lo, hi, [&](const float (&v)[kVec], int) {
+        add_up(own, v, cut.x);
+        if (cut.ties) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          const float e = soft.exp(v[j]);
-          const Limbs w = limbs(e >= min_p && !(v[j] <= cut.x) ? e : 0.f);
-          own.hi += w.hi;
-          own.lo += w.lo;
-          equal += v[j] == cut.x;
+          for (int j = 0; j < kVec; ++j) equal += v[j] == cut.x;
         }
       });
       sum = warp_sum64(own.value());
