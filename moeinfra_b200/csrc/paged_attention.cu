@@ -10,10 +10,13 @@
 // Bound by memory: every key and value is read once for all query heads of
 // its KV head (4 flops a byte per head, far below the tensor cores' rate), so
 // what counts is bytes in flight and an even split.
-//   * The caches' rows, as chunks of 16 keys, form one line: sequence by
-//     sequence, KV head by KV head.  The line is cut evenly over the CTAs and
-//     within a CTA over its 8 warps, whatever the lengths are; the cuts are
-//     found on the device from the lengths, so a captured graph follows them.
+//   * Rows come in chunks of 16 keys.  Where the lengths cannot differ much, each
+//     (sequence, KV head) is a CTA's, its chunks cut evenly over 8 warps, or over 4
+//     with two CTAs to an SM, one's start and end under the other's loads.
+//   * Else all chunks form one line: sequence by sequence, KV head by KV head.  The
+//     line is cut evenly over the CTAs and within a CTA over its 8 warps, whatever
+//     the lengths are; the cuts are found on the device from the lengths, so a
+//     captured graph follows them.
 //   * Each warp owns a ring of chunks in shared memory that it fills with
 //     cp.async (rows past a sequence's end as zeros: what lies there is never
 //     read) and never waits for another warp: 192 KB in flight per SM at most.
@@ -24,7 +27,10 @@
 //     empty, and the memory bound is already reached.)
 //   * Pieces of a (sequence, KV head) are joined in the order of their keys:
 //     within a CTA through shared memory, between CTAs by the last of them to
-//     finish.  The sums' order depends on the lengths and the GPU only.
+//     finish.  The sums' order depends on the shapes, the lengths and the GPU only.
+// Measured (32 / 8 heads of 128): 64 sequences of 576 fp16 28.4 us (151 MB, 5.3
+// TB/s), 64 of 2048 81 us (6.6 TB/s, what a plain copy reaches), four of about
+// 100000 bf16 268 us (6.5 TB/s); one of 72 3.8 us, a chain of latencies.
 #include "paged.cuh"
 
 namespace moe {
@@ -32,12 +38,12 @@ namespace {
 
 MOE_DEFINE_ERROR_WORD()
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
+constexpr int kMaxWarps = 8;        // of a CTA that is alone on its SM; with two to an SM it has half
 constexpr int kChunk = 16;          // keys per chunk (a page holds whole chunks)
 constexpr int kMaxSeqs = 4095;      // their lengths and chunk counts sit in shared memory
 // Smallest share of a CTA in chunks when the line is cut: below it a CTA's
-// pieces cost more to join than they save.
+// pieces cost more to join than they save (1 x 4096: 13.9 us with 8, 9.8 with 16,
+// 10.0 with 32; 32 x 100: 10.9, 11.2, 13.6).
 constexpr int kMinShare = 16;
 
 struct PagedArgs {
@@ -54,7 +60,7 @@ struct PagedArgs {
   int page_shift;         // log2 of that, or -1
   int* counts;            // [CTAs]: pieces written of the unit that starts in a CTA; zero between calls
   float* part;            // [CTAs][2] pieces
-  float* warp_part;       // [CTAs][kWarps] pieces
+  float* warp_part;       // [CTAs][kMaxWarps] pieces
 };
 
 // A piece in memory: O [heads of a tile][HD + 4] fp32 (the pad keeps the 4
@@ -66,10 +72,10 @@ template <int HD>
 constexpr int stages() { return HD == 128 ? 3 : 6; }  // 192 KB of ring either way
 template <int HD>
 constexpr int stage_bytes() { return 2 * kChunk * HD * 2; }
-template <int HD>
-constexpr int ring_bytes() { return kWarps * stages<HD>() * stage_bytes<HD>(); }
-template <int HD>
-int smem_bytes(int seqs) { return ring_bytes<HD>() + (2 * seqs + 1) * 4; }
+template <int HD, int WARPS>
+constexpr int ring_bytes() { return WARPS * stages<HD>() * stage_bytes<HD>(); }
+template <int HD, bool WHOLE, int WARPS>
+int smem_bytes(int seqs) { return ring_bytes<HD, WARPS>() + (WHOLE ? 0 : (2 * seqs + 1) * 4); }
 
 // Chunk x of the line: its sequence b, unit u (head tile) in it, the unit's
 // number of chunks n and the chunk's place kc in it.  prefix counts the chunks
@@ -108,13 +114,14 @@ __device__ __forceinline__ void write_row(const PagedArgs& a, int b, int h, int 
 // WHOLE: CTA x has unit x to itself (see whole_units).  Then nothing depends on
 // the other sequences' lengths, and the unit's pages, its queries and its
 // length are read at once instead of one after the other.
-template <typename T, int HD, int NT, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, 1) k_paged_attention(const PagedArgs a) {
+template <typename T, int HD, int NT, bool WHOLE, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, kMaxWarps / WARPS) k_paged_attention(const PagedArgs a) {
+  constexpr int kWarps = WARPS, kThreads = WARPS * 32;
   constexpr int S = stages<HD>(), kHeads = NT * 8, kPitch = HD + 4;
   constexpr int kRow = HD * 2;                  // bytes of a row
   constexpr int kTile = kChunk * kRow;          // bytes of a chunk's keys (or values)
   extern __shared__ __align__(128) unsigned char smem[];
-  int* prefix = reinterpret_cast<int*>(smem + ring_bytes<HD>());
+  int* prefix = reinterpret_cast<int*>(smem + ring_bytes<HD, WARPS>());
   int* s_len = prefix + a.kv.seqs + 1;
   __shared__ int s_scan[kWarps];
   __shared__ int4 s_info[kWarps][S];            // b, u, rows that count, bit 0 first / bit 1 last
@@ -231,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_attention(const PagedArgs
     if (x >= we) return;
     if constexpr (!WHOLE) w = where(x, prefix, kv.seqs, per_seq);
     entry = a.page_shift >= 0 ? w.kc >> a.page_shift : w.kc / a.page_chunks;
-    if constexpr (!WHOLE) page = kv.table[w.b * kv.table_stride + entry];
+    if (!WHOLE || x >= 64) page = kv.table[w.b * kv.table_stride + entry];
     if (page < 0 || page >= kv.num_pages) {
       set_device_error(kErrPage);
       page = 0;
@@ -575,16 +582,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_attention(const PagedArgs
   }
 }
 
-template <typename T, int HD, int NT, bool WHOLE>
+template <typename T, int HD, int NT, bool WHOLE, int WARPS>
 bool paged_attr() {
-  return cudaFuncSetAttribute(k_paged_attention<T, HD, NT, WHOLE>,
+  return cudaFuncSetAttribute(k_paged_attention<T, HD, NT, WHOLE, WARPS>,
                               cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              smem_bytes<HD>(kMaxSeqs)) == cudaSuccess;
+                              smem_bytes<HD, WHOLE, WARPS>(kMaxSeqs)) == cudaSuccess;
 }
 
 // Whether a call gives each unit (sequence, KV head, head tile) a CTA of its
-// own: few units and a table that holds at most 64 chunks (1024 tokens) each.
-bool whole_units(int64_t units, int64_t chunks) { return units <= sm_count() && chunks <= 64; }
+// own, which joins nothing with others and reads its page numbers, queries and
+// length at once; or cuts the line evenly.  The table's width is all that is known
+// of the lengths here, so a CTA's share must not become too long where few units
+// are long.  Measured (fp16, 32 / 8 heads of 128, own CTAs / even cut, us): 1 x 72
+// 3.8 / 9.2, 8 x 576 7.1 / 10.9, 64 x 576 28.4 / 35.2, 64 x 2048 81.4 / 92.3, 64
+// ragged up to 1972 46.9 / 54.7; but 1 x 1024 8.8 / 7.9, one of 2048 and 63 of 16
+// 19.5 / 9.4, one of 4096 and 63 of 16 35.7 / 14.3.
+bool whole_units(int64_t units, int64_t chunks) {
+  return chunks <= (units <= sm_count() ? 64 : 128);
+}
 
 struct Shape {
   int parts, tile, nt;
@@ -611,27 +626,32 @@ constexpr size_t kCountBytes = 4096;
 size_t workspace_size(const Shape& s, int hd) {
   if (s.whole) return kCountBytes;
   return kCountBytes +
-         sizeof(float) * s.ctas * (2 + kWarps) * (s.nt * 8 * (hd + 4) + 2 * s.nt * 8);
+         sizeof(float) * s.ctas * (2 + kMaxWarps) * (s.nt * 8 * (hd + 4) + 2 * s.nt * 8);
 }
 
-template <typename T, int HD, int NT, bool WHOLE>
+template <typename T, int HD, int NT, bool WHOLE, int WARPS>
 int launch_paged(PagedArgs& a, const Shape& sh, cudaStream_t s) {
-  if (!once_per_device(reinterpret_cast<const void*>(&paged_attr<T, HD, NT, WHOLE>),
-                       &paged_attr<T, HD, NT, WHOLE>))
+  if (!once_per_device(reinterpret_cast<const void*>(&paged_attr<T, HD, NT, WHOLE, WARPS>),
+                       &paged_attr<T, HD, NT, WHOLE, WARPS>))
     return MOE_ERR_CUDA;
-  a.part = a.warp_part + (size_t)sh.ctas * kWarps * piece_floats<HD, NT>();
-  if (launch_pdl(k_paged_attention<T, HD, NT, WHOLE>, dim3(sh.ctas), dim3(kThreads),
-                 WHOLE ? ring_bytes<HD>() : smem_bytes<HD>(a.kv.seqs), s, a) != cudaSuccess)
+  a.part = a.warp_part + (size_t)sh.ctas * kMaxWarps * piece_floats<HD, NT>();
+  if (launch_pdl(k_paged_attention<T, HD, NT, WHOLE, WARPS>, dim3(sh.ctas), dim3(WARPS * 32),
+                 smem_bytes<HD, WHOLE, WARPS>(a.kv.seqs), s, a) != cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
   return MOE_OK;
 }
 
+template <typename T, int HD, int NT>
+int launch_tile(PagedArgs& a, const Shape& sh, cudaStream_t s) {
+  if (!sh.whole) return launch_paged<T, HD, NT, false, kMaxWarps>(a, sh, s);
+  return sh.units <= sm_count() ? launch_paged<T, HD, NT, true, kMaxWarps>(a, sh, s)
+                                : launch_paged<T, HD, NT, true, kMaxWarps / 2>(a, sh, s);
+}
+
 template <typename T, int HD>
 int launch_wide(PagedArgs& a, const Shape& sh, cudaStream_t s) {
-  if (sh.whole)
-    return sh.nt == 1 ? launch_paged<T, HD, 1, true>(a, sh, s) : launch_paged<T, HD, 2, true>(a, sh, s);
-  return sh.nt == 1 ? launch_paged<T, HD, 1, false>(a, sh, s) : launch_paged<T, HD, 2, false>(a, sh, s);
+  return sh.nt == 1 ? launch_tile<T, HD, 1>(a, sh, s) : launch_tile<T, HD, 2>(a, sh, s);
 }
 
 }  // namespace

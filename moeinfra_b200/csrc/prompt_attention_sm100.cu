@@ -171,11 +171,12 @@ __device__ __forceinline__ uint64_t exp2_fma(uint64_t x) {
   const uint32_t hi = (uint32_t)(p >> 32) + ((uint32_t)(r >> 32) << 23);
   return pair(__uint_as_float(lo), __uint_as_float(hi));
 }
-// Of 8 pairs, those that go through exp2_fma: see the kernel's comment.
-#ifndef FMA_OF_8
-#define FMA_OF_8 2
-#endif
-constexpr int kFmaOf8 = FMA_OF_8;
+// Of 8 pairs, those that go through exp2_fma.  With heads of 128 the tensor cores
+// (and the power limit) bound a step and it only costs: 1 x 8192 causal fp16 450 us
+// with none, 454 with 1, 461 with 2, 495 with 4.  With heads of 64 a step has twice
+// the exponentials per product: 2 x 4096 fp16 215, 207, 210, 241 us.
+template <int HD>
+constexpr int kFmaOf8 = HD == 128 ? 0 : 1;
 
 // kN consecutive columns of the thread's own lane.
 template <int N>
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < kN; c += 2) {
           const uint64_t x = fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2, r2);
-          const uint64_t e = c / 2 % 8 < kFmaOf8 ? exp2_fma<T>(x) : exp2_mufu(x);
+          const uint64_t e = c / 2 % 8 < kFmaOf8<HD> ? exp2_fma<T>(x) : exp2_mufu(x);
           sum[c / 2 & 1] = add2(sum[c / 2 & 1], e);
           p[c / 2] = T::pack(lo_of(e), hi_of(e));
         }
