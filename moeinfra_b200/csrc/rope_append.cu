@@ -10,7 +10,10 @@
 //
 // Bound by memory: each element is read once and written once.  A thread
 // takes 8 elements of a head's first half and the 8 that rotate with them, so
-// every access is 16 bytes and a head of 128 is 8 neighbouring threads.
+// every access is 16 bytes and a head of 128 is 8 neighbouring threads; a block
+// is one token, whose row is requested before the token's slot is looked up.
+// Measured, 32 / 8 heads of 128 fp16: 64 prompts (21527 tokens, 530 MB) 95 us, 5.6
+// TB/s (with 2, 3, 4 tokens a block 110, 103, 100 us); one token 1.9 us.
 #include "paged.cuh"
 
 namespace moe {

@@ -188,6 +188,20 @@ def test_paged_attention_lengths(lens, page, width):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd", [(8, 4, 64), (24, 4, 128), (48, 4, 128)])
+@pytest.mark.parametrize("width", [80, 128, 140])
+def test_paged_attention_many_sequences(dtype, H, KV, hd, width):
+    """More sequences than processors, in tables of every split's width; the lengths decide
+    nothing about the split, so they range from none to all of a table."""
+    page, lens = 16, [0, 1, 15, 16, 17, 1025, 1280, 79, 0] + [3 + 7 * i for i in range(40)]
+    table, n = _table(lens, page, 12, width)
+    kp, vp = (_cache(n, KV, page, hd, dtype, s) for s in (13, 14))
+    q = torch.randn(len(lens), H, hd, generator=torch.Generator().manual_seed(15)).to(dtype)
+    _check_paged(q, kp, vp, table, lens)
+
+
+@gpu
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("lens", [[5, 20], [1500, 16]])
 def test_paged_attention_ignores_what_lies_past_the_end(bad, lens):
