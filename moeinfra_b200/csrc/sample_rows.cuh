@@ -6,19 +6,20 @@
 //     the temperature, which hold every weight above 0.  A scan of the bins finds
 //     the one with the boundary.
 //   * The logits above that bin and those in it are gathered, at most 2048 of
-//     each, and the weights of those above that found no place added up instead.
+//     each, and the weights of those above that found no place added up instead (of
+//     all of them at once where the bins' sums tell that there are too many).
 //     Up to 256 are compared with each other and drawn from at once.  Of more, the
 //     bin's are cut to one value by histograms over their bits, 10 bits a round.
 //   * The draw is one more histogram, over the indices of the logits kept; or, if
 //     they do not fit, sums of contiguous parts of the row, and of parts of the part.
 // Sums are exact integers: the order in which atomics add them does not matter.
 //
-// Bound by instruction issue.  256 x 131072 fp32 of mixed parameters: 128 us, 134
+// Bound by instruction issue.  256 x 131072 fp32 of mixed parameters: 127 us, 134
 // MB, which a plain copy's rate would read in 21 (greedy rows alone: 35).  What
 // costs: the exponential of a correctly rounded quotient and its 40 bits, in each
 // of two passes (13 and 15 cycles an SM for 32 logits, at two thirds of the issue
-// slots).  64 x 32000 fp16: 32 us, as long as the slowest row's CTA, 7.5 of them
-// its histogram.  1024 threads and one CTA to an SM; with 512 and two, 64 x 32000
+// slots).  64 x 32000 fp16: 30 us, as long as the slowest row's CTA, 8 of them its
+// histogram, 8 the second pass.  1024 threads and one CTA to an SM; with 512 and two, 64 x 32000
 // took 4 us longer and 256 x 131072 32.  Bins in two copies, for fewer conflicts:
 // no faster.  Four pieces on their way in the first pass, not one: 26 us less.
 #pragma once
@@ -52,7 +53,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
   __shared__ uint64_t s_part[2][kRowWarps];
   struct Pick {
     uint64_t before, own, total;
-    int bin;
+    int bin, about;
   };
   __shared__ Pick s_pick;
   __shared__ uint64_t s_sum[kRowWarps];  // what the warps' parts of the row keep for sure
@@ -216,11 +217,20 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
   };
   // The first bin with which the sum reaches `need` (0: what top-p asks of the
   // total), then known to every thread; leaves the bins empty.
-  auto pick = [&](uint64_t& need) {
+  // `weights`: the bins hold weights of the first kind, and about counts the logits
+  // before the bin, to a few percent: each weighs what its bin's middle does.
+  auto pick = [&](uint64_t& need, bool weights) {
     __syncthreads();
     const uint64_t own = (uint64_t)s_hi[threadIdx.x] << 32 | s_lo[threadIdx.x];
     s_lo[threadIdx.x] = s_hi[threadIdx.x] = 0;
     const uint64_t of_warp = warp_sum64(own);
+    uint32_t count = 0;
+    if (weights) {
+      count = __float2uint_rn(__ull2float_rn(own) * kLeast *
+                              __expf((int)threadIdx.x * (1.f / kBinsPerUnit)));
+      const uint32_t all = __reduce_add_sync(kAll, min(count, 1u << 20));
+      if (lane == 0) s_part[1][warp] = all;
+    }
     if (lane == 0) s_part[0][warp] = of_warp;
     __syncthreads();
     const uint64_t of_lane = s_part[0][lane];
@@ -234,7 +244,14 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
         if (lane >= o) run += v;
       }
       const uint64_t before = ahead + run - own;
-      if (before < need && need <= before + own) s_pick = Pick{before, own, total, (int)threadIdx.x};
+      const bool here = before < need && need <= before + own;
+      int about = 0;
+      if (weights) {
+        const int at = __ffs(__ballot_sync(kAll, here)) - 1;
+        about = (int)__reduce_add_sync(kAll, (lane < at ? min(count, 1u << 20) : 0u) +
+                                                 (lane < warp ? (uint32_t)s_part[1][lane] : 0u));
+      }
+      if (here) s_pick = Pick{before, own, total, (int)threadIdx.x, about};
     }
     __syncthreads();
     return s_pick;
@@ -242,9 +259,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
 
   Cut cut;
   bool summed = false;  // s_sum and the lists have what may be kept
+  bool skip = false;    // the first list is not used
   bool held = false;    // all that may be kept is in the two lists
   auto held_each = [&](int list, auto f) {
-    const int n = min(s_n[list], kHeld);
+    const int n = list == 0 && skip ? 0 : min(s_n[list], kHeld);
 #pragma unroll 1
     for (int i = threadIdx.x; i < n; i += kRowThreads) f(s_x[list][i], s_at[list][i]);
   };
@@ -307,9 +325,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
         if (threadIdx.x == 0 && at_cut) add(bin_of(cut.x), at_cut);
       }
       if (threadIdx.x == 0) s_n[0] = s_n[1] = 0;
-      const Pick found = pick(need);
+      const Pick found = pick(need, !count);
       above = found.before;
       own = found.own;
+      // Too many above the bin for the first list: it stays empty.
+      skip = (count ? (int)above : found.about) > kHeld + kHeld / 4;
+      if (skip && threadIdx.x == 0) s_n[0] = kHeld + 1;
       if (warp < 2) s_key[warp] = key_from(found.bin - warp);
       __syncthreads();
       lo = s_key[0];
@@ -351,7 +372,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
               ++slot;
             }
         }
-        if (last && __any_sync(kAll, out)) {  // the list has just become full
+        if (last && !full && __any_sync(kAll, out)) {  // the list has just become full
 #pragma unroll
           for (int j = 0; j < kVec; ++j) {
             const float e = soft.exp(v[j]);
@@ -409,7 +430,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
         if (key - lo <= hi - lo) add((int)((hi - key) >> shift), at_cut);
       }
       uint64_t rest = need ? need - above : 0ull;
-      const Pick found = pick(rest);
+      const Pick found = pick(rest, false);
       if (!need) need = rest;
       above += found.before;
       own = found.own;
@@ -445,7 +466,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
       };
       equal([&](int at) { atomicAdd(&s_lo[at >> shift], 1u); });
       uint64_t need = cut.ties;
-      const Pick found = pick(need);
+      const Pick found = pick(need, false);
       equal([&](int at) {
         if (at >> shift == found.bin) s_lo[at & mask] = 1;
       });
@@ -476,7 +497,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
     }
     const uint64_t r = draw_of(u, total);
     uint64_t need = r + 1;
-    const Pick found = pick(need);
+    const Pick found = pick(need, false);
     kept([&](uint64_t w, int at) {
       if (at >> shift == found.bin) {
         s_lo[at & mask] = (uint32_t)w;

@@ -537,7 +537,7 @@ int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t s) {
 // One CTA a row where rows are many or short.  Measured with mixed parameters
 // (cluster / one CTA, us): 2 x 16000 12.3 / 10.9, 16 x 16000 25.9 / 19.6; 24 x
 // 32000 30.5 / 31.2, 48 x 32000 45.5 / 32.4; 32 x 131072 66.7 / 91.5, 64 x 131072
-// 107 / 100, 256 x 131072 406 / 161 (128 since); 1 x 32000 11.4 / 18.4.
+// 107 / 100, 256 x 131072 406 / 161 (127 since); 1 x 32000 11.4 / 18.4.
 // In a cluster 8 logits a thread, and so more CTAs, as far as 8 CTAs go; then 16
 // (a cluster of up to 16 CTAs); 32 and one CTA to an SM for the longest rows.
 template <typename T>
