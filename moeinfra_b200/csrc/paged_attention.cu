@@ -10,7 +10,7 @@
 // Bound by memory: every key and value is read once for all query heads of
 // its KV head (4 flops a byte per head, far below the tensor cores' rate), so
 // what counts is bytes in flight and an even split.
-//   * Rows come in chunks of 16 keys.  Where the lengths cannot differ much, each
+//   * Rows come in chunks of 16 keys.  Where it pays (whole_units), each
 //     (sequence, KV head) is a CTA's, its chunks cut evenly over 8 warps, or over 4
 //     with two CTAs to an SM, one's start and end under the other's loads.
 //   * Else all chunks form one line: sequence by sequence, KV head by KV head.  The
@@ -593,12 +593,17 @@ bool paged_attr() {
 // own, which joins nothing with others and reads its page numbers, queries and
 // length at once; or cuts the line evenly.  The table's width is all that is known
 // of the lengths here, so a CTA's share must not become too long where few units
-// are long.  Measured (fp16, 32 / 8 heads of 128, own CTAs / even cut, us): 1 x 72
-// 3.8 / 9.2, 8 x 576 7.1 / 10.9, 64 x 576 28.4 / 35.2, 64 x 2048 81.4 / 92.3, 64
-// ragged up to 1972 46.9 / 54.7; but 1 x 1024 8.8 / 7.9, one of 2048 and 63 of 16
-// 19.5 / 9.4, one of 4096 and 63 of 16 35.7 / 14.3.
+// are long; and a CTA for a few chunks is a wave of latencies for each 2 to an SM.
+// Measured (fp16, 32 heads of 128, 8 KV heads, own CTAs / even cut, us):
+//   1 x 72 3.8 / 9.2, 8 x 576 7.1 / 10.9, 64 x 576 28.4 / 35.2, 64 x 2048 81 / 92,
+//   64 ragged up to 1972 46.9 / 54.7; but 1 x 1024 8.8 / 7.9, one of 2048 and 63 of
+//   16 19.5 / 9.4, one of 4096 and 63 of 16 35.7 / 14.3;
+//   512 units of 48 6.8 / 11.8, of 100 8.8 / 13.8; but 2048 units of 48 26 / 12.6, of
+//   100 32 / 31, of 160 38.7 / 41.6, of 256 51 / 58.
 bool whole_units(int64_t units, int64_t chunks) {
-  return chunks <= (units <= sm_count() ? 64 : 128);
+  const int64_t sms = sm_count();
+  if (units <= sms) return chunks <= 64;
+  return chunks <= 128 && (chunks >= 12 || units <= 4 * sms);
 }
 
 struct Shape {
