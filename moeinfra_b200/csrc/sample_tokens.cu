@@ -535,14 +535,16 @@ int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t s) {
 }
 
 // One CTA a row where rows are many or short.  Measured with mixed parameters
-// (cluster / one CTA, us): 2 x 16000 12.3 / 10.9, 16 x 16000 25.9 / 19.6; 24 x
-// 32000 30.5 / 31.2, 48 x 32000 45.5 / 32.4; 32 x 131072 66.7 / 91.5, 64 x 131072
-// 107 / 100, 256 x 131072 406 / 161 (127 since); 1 x 32000 11.4 / 18.4.
+// (cluster / one CTA, us): 1 x 16000 9.4 / 10.9, 2 x 16000 12.3 / 10.9, 16 x 16000
+// 25.9 / 19.6; 1 x 32000 11.4 / 18.4, 8 x 32000 23.7 / 27.3, 16 x 32000 28.0 / 28.1,
+// 40 x 32000 34.4 / 29.5; 16 x 65536 37.8 / 43.3, 24 x 65536 46.1 / 42.6; 32 x
+// 131072 66.7 / 78.0, 40 x 131072 80.5 / 77.6, 256 x 131072 406 / 127; 24 x 200000
+// 88.9 / 109, 40 x 200000 139 / 111.
 // In a cluster 8 logits a thread, and so more CTAs, as far as 8 CTAs go; then 16
 // (a cluster of up to 16 CTAs); 32 and one CTA to an SM for the longest rows.
 template <typename T>
 int launch_rows(SampleArgs& a, int64_t rows, cudaStream_t s) {
-  if (a.vocab <= 16384 || rows >= 20 + a.vocab / 4096) return launch_sample_rows<T>(a, rows, s);
+  if (a.vocab <= 16384 || rows >= 36 || rows * 3000 >= a.vocab) return launch_sample_rows<T>(a, rows, s);
   const int per = a.vocab <= 8 * kThreads * 8 ? 8 : a.vocab <= kMaxCluster * kThreads * 16 ? 16 : 32;
   a.cluster = a.vocab <= 8 * kThreads * per ? 8 : kMaxCluster;
   if (per == 8) return launch_sample<T, 8>(a, rows, s);
