@@ -305,7 +305,12 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
         hi = t_hi;
         above = s_hi;
       }
-      if (hi - lo <= 1) return Bound{lo, above};
+      if (hi - lo <= 1) {
+        // A second search begins with list 0, empty: between this and its first
+        // entry lies an exchange (the sums of its first thresholds).
+        if (threadIdx.x == 0) s_count[0] = 0;
+        return Bound{lo, above};
+      }
       // The logits between the bounds, from the registers or the last list.
       uint32_t *list = s_dyn + turn * kThreads * PER, *counter = &s_count[turn];
       if (held_n == ~0u) {
@@ -366,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
       }
       const uint32_t found_key = __reduce_max_sync(kAll, ok ? own : 0u);
       if (lane == 0 && found_key) atomicMax(&s_key, found_key);
-      if (threadIdx.x == 0) s_count[0] = 0;  // a second search begins with it
+      if (threadIdx.x == 0) s_count[0] = 0;  // as above
       __syncthreads();
       if (threadIdx.x < n && own == s_key) s_above = above + over;  // the same value from each
       __syncthreads();

@@ -293,3 +293,37 @@ def test_many_kept(top_k, top_p, min_p):
     x *= torch.linspace(0.05, 6.0, rows, device="cuda")[:, None]
     u = torch.rand(rows, device="cuda", generator=g)
     _compare(x, u, _params(rows, 1.0, top_k, top_p, min_p))
+
+
+# Rows over several CTAs with top-k and top-p together: the boundary of the second lies among the
+# logits that the first one's search gathered last.
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(1, 32000), (7, 32000), (2, 131072), (10, 131072)])
+def test_top_p_near_the_cut_of_top_k(dtype, rows, vocab):
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = 2 * torch.randn(rows, vocab, device="cuda", generator=g)
+    x += (torch.rand(rows, vocab, device="cuda", generator=g) < 200 / vocab) * (
+        3 + 2.5 * torch.randn(rows, vocab, device="cuda", generator=g).abs())
+    u = torch.rand(rows, device="cuda", generator=g)
+    for t in (0.7, 1.0, 2.0):
+        for k in (1000, 2000, 5000, 10000, 20000):
+            for p in (0.9, 0.99, 0.999):
+                _compare(x.to(dtype), u, _params(rows, t, k, p))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(1, 32000), (5, 32000), (3, 131072), (1, 200000)])
+def test_top_p_near_the_cut_of_top_k_among_ties(dtype, rows, vocab):
+    """Thousands of logits equal to the cut, so that every search's lists are full of them."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    flat = torch.zeros(rows, vocab, device="cuda")
+    flat[:, 100:105] = 3.0
+    few = torch.randint(0, 3, (rows, vocab), device="cuda", generator=g) * 1e-3
+    few[:, ::7] = few[:, ::7] + 2 ** -9
+    u = torch.rand(rows, device="cuda", generator=g)
+    for x in (flat, few):
+        for k in (1000, 10000, 20000, vocab - 1):
+            for p in (0.5, 0.99, 0.9999):
+                _compare(x.to(dtype), u, _params(rows, 1.0, k, p))
