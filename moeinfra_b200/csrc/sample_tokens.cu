@@ -43,7 +43,8 @@
 //     stores its 8 into every CTA's shared memory with st.async, whose bytes
 //     complete an mbarrier there (a cluster barrier behind plain stores took 2000
 //     cycles, this a third: 13.3 -> 12.0 us for the one row).  Waits are bounded:
-//     on a timeout the error word is set and the CTA returns, as then do the others.
+//     on a timeout the error word is set and the CTA leaves, as then do the others
+//     (Exchange::leave).
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
@@ -61,6 +62,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 16;            // 8 is the portable size; 16 only where a row needs it
 constexpr int kMaxPer = 32;                // logits a thread holds at most
 constexpr int kList = 256;                 // logits that a search finishes with directly
+constexpr int kMaxSyncs = 2;               // cluster barriers: one a search, or one for the few
 constexpr int kMaxVocab = kMaxCluster * kThreads * kMaxPer;
 
 __device__ __forceinline__ uint32_t map_rank(uint32_t addr, int rank) {
@@ -82,8 +84,9 @@ struct Exchange {
   uint64_t (*warp_sum)[8];
   uint64_t (*slots)[kMaxCluster][8];
   uint32_t bar;       // two mbarriers of one arrival (this CTA's, with the bytes to come)
+  volatile int* s_dead;
   uint32_t count = 0;
-  bool dead = false;  // a wait ran out
+  bool dead = false;  // a wait of this CTA ran out: it gives nothing any more
 
   __device__ __forceinline__ int turn() const { return count & 1; }
   __device__ __forceinline__ uint64_t slot(int r, int j) const { return slots[turn() ^ 1][r][j]; }
@@ -103,11 +106,25 @@ struct Exchange {
             : "memory");
     }
   }
+  // Warp 0 waits for the bytes and the others for warp 0, so that a timeout is one
+  // for the whole CTA.
   __device__ __forceinline__ void wait() {
-    if (!mbar_poll_or(bar + 8 * turn(), count >> 1 & 1, wait_ns,
-                      [] { set_device_error(kErrWaitTimeout); }))
-      dead = true;
+    if (warp == 0 && !mbar_poll_or(bar + 8 * turn(), count >> 1 & 1, wait_ns,
+                                   [] { set_device_error(kErrWaitTimeout); }))
+      *s_dead = 1;
+    __syncthreads();
+    dead = *s_dead;
     ++count;
+  }
+  // After a timeout.  The other CTAs may have sums for this one on their way, of
+  // the exchange that ran out or the next, so its shared memory has to last: it goes
+  // along with their cluster barriers, of which a launch has kMaxSyncs at most after
+  // the first exchange.  The one after those is passed when every other CTA has ended
+  // or is in here too; their last stores are then given ample time to land.
+  __device__ __forceinline__ void leave() const {
+    for (int i = 0; i <= kMaxSyncs; ++i) cg::this_cluster().sync();
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 20000) __nanosleep(1000);
   }
   template <int N>
   __device__ __forceinline__ uint64_t sum(const uint64_t (&v)[N]) {
@@ -188,11 +205,13 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   __shared__ uint32_t s_count[2], s_few, s_key;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ __align__(8) uint64_t s_bar[2];
+  __shared__ int s_dead;
   cg::cluster_group cluster = cg::this_cluster();
   const int64_t row = blockIdx.x / a.cluster;
   Exchange ex{static_cast<int>(blockIdx.x % a.cluster), a.cluster, warp, lane, a.wait_ns, s_warp,
-              s_slots, saddr(s_bar)};
+              s_slots, saddr(s_bar), &s_dead};
   if (threadIdx.x == 0) {
+    s_dead = 0;
     mbar_init(ex.bar, 1);
     mbar_init(ex.bar + 8, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -233,14 +252,15 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   for (int c = 0; c < PER; ++c) top = max(top, key[c]);
   cluster.barrier_wait();
   top = ex.max(top);
-  if (ex.dead) return;
+  if (ex.dead) return ex.leave();
   if (!(temperature > 0.f) || k == 1) {  // its lowest index
     uint32_t index = 0xFFFFFFFFu;
 #pragma unroll
     for (int c = PER - 1; c >= 0; --c)
       if (key[c] == top) index = first + c / kVec * 32 * kVec + c % kVec;
     index = ~ex.max(~index);
-    if (!ex.dead && ex.rank == 0 && threadIdx.x == 0) {
+    if (ex.dead) return ex.leave();
+    if (ex.rank == 0 && threadIdx.x == 0) {
       a.tokens[row] = index;
       a.probs[row] = 1.f;
     }
@@ -392,6 +412,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
   const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.f;
   if (by_k || by_p) {
     uint64_t s = pass(by_k, (lane & 7) == 0 ? 1u : guess);
+    if (ex.dead) return ex.leave();
     const uint64_t need = by_k ? (uint64_t)k : need_of(p, shfl64(s, 0));
     // ---- few enough at or above the threshold that holds enough: one CTA takes them ----
     const uint32_t enough = __ballot_sync(kAll, lane >= 1 && lane < 8 && s >= need) | 1u;
@@ -403,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     for (int c = 0; c < PER; ++c) slots |= (key[c] >= floor_key ? 1u : 0u) << c;
     const uint64_t found[1] = {(uint64_t)__popc(slots)};
     const uint64_t total_n = shfl64(ex.sum(found), 0);
-    if (ex.dead) return;
+    if (ex.dead) return ex.leave();
     if (total_n <= kList) {
       uint32_t base = 0;  // of this CTA's places
       for (int r = 0; r < ex.rank; ++r) base += (uint32_t)ex.slot(r, 0);
@@ -428,17 +449,18 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     // ---- top-k: keys above the cut, and the first `ties` of those equal to it ----
     if (by_k) {
       const Bound b = search(true, k, 1, top + 1, guess, s);
-      if (ex.dead) return;
+      if (ex.dead) return ex.leave();
       cut = b.key;
       ties = k - b.above;
     }
     // ---- top-p ----
     if (by_p) {
       if (by_k) s = pass(false, (lane & 7) == 0 ? cut + 1 : guess);
+      if (ex.dead) return ex.leave();
       const uint64_t total = shfl64(s, 0) + ties * (cut ? weight(exp_of(cut)) : 0ull);
       const uint64_t want = need_of(p, total);
       const Bound b = search(false, want, cut ? cut : 1u, top + 1, guess, s);
-      if (ex.dead) return;
+      if (ex.dead) return ex.leave();
       const uint64_t w = weight(exp_of(b.key));
       const uint64_t n = (want - b.above + w - 1) / w;
       ties = b.key == cut && n > ties ? ties : n;
@@ -457,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, PER <= 16 ? 2 : 1) k_sample(const Sa
     if (key[c] == cut) ++sums[1];
   }
   ex.sum(sums);
-  if (ex.dead) return;
+  if (ex.dead) return ex.leave();
   const uint64_t w_cut = cut ? keeps(cut) : 0ull;
   auto place = [&](uint64_t w, uint64_t equal, uint64_t ahead) {
     return place_pieces(w, equal, ahead, ties, w_cut);

@@ -327,3 +327,32 @@ def test_top_p_near_the_cut_of_top_k_among_ties(dtype, rows, vocab):
         for k in (1000, 10000, 20000, vocab - 1):
             for p in (0.5, 0.99, 0.9999):
                 _compare(x.to(dtype), u, _params(rows, 1.0, k, p))
+
+
+@gpu
+def test_a_wait_that_runs_out_ends_the_call():
+    """With no time to wait, a row's CTAs give up at different points: the call ends with a status at
+    most, and the next one is right."""
+    from moeinfra_b200 import _native, kernels
+
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rows, vocab = 30, 131072
+    x = torch.randn(rows, vocab, device="cuda", generator=g).half()
+    u = torch.rand(rows, device="cuda", generator=g)
+    kinds = [dict(temperature=0.0), dict(), dict(top_p=0.9), dict(top_k=5000, top_p=0.99),
+             dict(temperature=0.1, top_k=20)]
+    old = _native.wait_limit_ns()
+    for kw in kinds:
+        params = _params(rows, **kw)
+        _native.set_wait_limit_ns(1000)
+        try:
+            for _ in range(20):
+                kernels.sample_tokens(x, u, *params)
+            try:
+                kernels.check_device()
+            except RuntimeError as e:
+                assert "timed out" in str(e)
+        finally:
+            _native.set_wait_limit_ns(old)
+        _compare(x, u, params)
+        kernels.check_device()
