@@ -347,6 +347,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
         for (int j = 1; j < kVec; ++j) most = fmaxf(most, v[j]);
         if (!__any_sync(kAll, most >= x_lo)) return;
         uint32_t in[2] = {0, 0};
+        // The other warps add to the count, so lanes may read it differently: a lane
+        // goes by its own reading, and no vote depends on it.
         const bool full = *(volatile int*)&s_n[0] > kHeld;
         if (full && last) {
           add_up(sum, v, x_hi);
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) k_sample_rows(const SampleArgs
               ++slot;
             }
         }
-        if (last && !full && __any_sync(kAll, out)) {  // the list has just become full
+        if (last && __any_sync(kAll, out)) {  // the list has just become full
 #pragma unroll
           for (int j = 0; j < kVec; ++j) {
             const float e = soft.exp(v[j]);

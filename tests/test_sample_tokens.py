@@ -356,3 +356,18 @@ def test_a_wait_that_runs_out_ends_the_call():
             _native.set_wait_limit_ns(old)
         _compare(x, u, params)
         kernels.check_device()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_lists_that_fill_while_they_are_gathered(dtype):
+    """From just under to just over the 2048 logits a list holds, row by row: warps meet a list that
+    others have filled in between."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rows, vocab = 150, 40000
+    x = torch.randn(rows, vocab, device="cuda", generator=g).to(dtype)
+    u = torch.rand(rows, device="cuda", generator=g)
+    k = [1800 + 5 * i for i in range(rows)]
+    for kw in (dict(top_k=k), dict(top_k=k, min_p=0.05), dict(top_k=k, top_p=0.9),
+               dict(top_p=[0.05 + 0.003 * i for i in range(rows)])):
+        _compare(x, u, _params(rows, 0.7, **kw))
