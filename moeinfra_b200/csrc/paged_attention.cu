@@ -40,7 +40,7 @@ MOE_DEFINE_ERROR_WORD()
 
 constexpr int kMaxWarps = 8;        // of a CTA that is alone on its SM; with two to an SM it has half
 constexpr int kChunk = 16;          // keys per chunk (a page holds whole chunks)
-constexpr int kMaxSeqs = 4095;      // their lengths and chunk counts sit in shared memory
+constexpr int kMaxSeqs = 4095;      // what they need of shared memory: see line_bytes
 // Smallest share of a CTA in chunks when the line is cut: below it a CTA's
 // pieces cost more to join than they save (1 x 4096: 13.9 us with 8, 9.8 with 16,
 // 10.0 with 32; 32 x 100: 10.9, 11.2, 13.6).
@@ -74,8 +74,16 @@ template <int HD>
 constexpr int stage_bytes() { return 2 * kChunk * HD * 2; }
 template <int HD, int WARPS>
 constexpr int ring_bytes() { return WARPS * stages<HD>() * stage_bytes<HD>(); }
+// The line in shared memory: prefix sums of the chunk counts, and the rows of each
+// sequence's last chunk (1 to 16) in a byte.
+constexpr int line_bytes(int seqs) { return (seqs + 1) * 4 + seqs; }
 template <int HD, bool WHOLE, int WARPS>
-int smem_bytes(int seqs) { return ring_bytes<HD, WARPS>() + (WHOLE ? 0 : (2 * seqs + 1) * 4); }
+constexpr int smem_bytes(int seqs) { return ring_bytes<HD, WARPS>() + (WHOLE ? 0 : line_bytes(seqs)); }
+// At most what the kernel's __shared__ arrays take, paddings included.
+template <int HD, int NT, int WARPS>
+constexpr int static_bytes() {
+  return 16 * (WARPS * stages<HD>() + 2 * WARPS + 2) + 4 * (WARPS + 2 * WARPS * 2 * NT * 8) + 256;
+}
 
 // Chunk x of the line: its sequence b, unit u (head tile) in it, the unit's
 // number of chunks n and the chunk's place kc in it.  prefix counts the chunks
@@ -121,8 +129,12 @@ __global__ void __launch_bounds__(WARPS * 32, kMaxWarps / WARPS) k_paged_attenti
   constexpr int kRow = HD * 2;                  // bytes of a row
   constexpr int kTile = kChunk * kRow;          // bytes of a chunk's keys (or values)
   extern __shared__ __align__(128) unsigned char smem[];
+  // Of an SM's 228 KB each CTA loses one.
+  static_assert(smem_bytes<HD, WHOLE, WARPS>(kMaxSeqs) + static_bytes<HD, NT, WARPS>() <=
+                    228 * 1024 * WARPS / kMaxWarps - 1024,
+                "shared memory");
   int* prefix = reinterpret_cast<int*>(smem + ring_bytes<HD, WARPS>());
-  int* s_len = prefix + a.kv.seqs + 1;
+  unsigned char* s_rest = reinterpret_cast<unsigned char*>(prefix + a.kv.seqs + 1);
   __shared__ int s_scan[kWarps];
   __shared__ int4 s_info[kWarps][S];            // b, u, rows that count, bit 0 first / bit 1 last
   __shared__ int4 s_piece[2 * kWarps];           // b (or -1), u, bit 0 first / bit 1 last
@@ -188,8 +200,8 @@ __global__ void __launch_bounds__(WARPS * 32, kMaxWarps / WARPS) k_paged_attenti
     if (b < kv.seqs) {
       const int len = a.lengths[b], c = clamp_len(len, kv);
       if (c != len && blockIdx.x == 0) set_device_error(kErrPage);
-      s_len[b] = c;
       n = (c + kChunk - 1) / kChunk;
+      s_rest[b] = c - (n - 1) * kChunk;  // not used where n is 0
     }
     int inc = n;
 #pragma unroll
@@ -250,8 +262,8 @@ __global__ void __launch_bounds__(WARPS * 32, kMaxWarps / WARPS) k_paged_attenti
     d_v = page * kv.v_stride + in_page;
     d_u = w.u;
     d_b = w.b;
-    d_rows = min(kChunk, (WHOLE ? own_len : s_len[w.b]) - w.kc * kChunk);
     d_ends = (w.kc == 0 ? 1 : 0) | (w.kc == w.n - 1 ? 2 : 0);
+    d_rows = d_ends < 2 ? kChunk : WHOLE ? own_len - w.kc * kChunk : s_rest[w.b];
   };
 
   // A unit's queries are loaded when its first chunk is issued, ahead of their

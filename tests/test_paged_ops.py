@@ -202,6 +202,32 @@ def test_paged_attention_many_sequences(dtype, H, KV, hd, width):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H,KV", [(16, 1), (12, 1), (24, 1), (32, 2), (8, 1)])
+def test_paged_attention_wide_groups_over_a_cut_line(dtype, hd, H, KV):
+    """Groups of 8 to 24 heads over tables too long for a CTA per unit."""
+    page, lens = 16, [3000, 17, 0, 1025, 16]
+    table, n = _table(lens, page, 21)
+    g = torch.Generator().manual_seed(H + hd)
+    q = torch.randn(len(lens), H, hd, generator=g).to(dtype)
+    kp, vp = (_cache(n, KV, page, hd, dtype, s) for s in (22, 23))
+    _check_paged(q, kp, vp, table, lens)
+
+
+@gpu
+@pytest.mark.parametrize("hd,H", [(64, 16), (128, 16), (64, 4)])
+def test_paged_attention_of_as_many_sequences_as_fit(hd, H):
+    page, lens = 16, [(37 * i) % 49 for i in range(4095)]
+    table, n = _table(lens, page, 24)
+    g = torch.Generator().manual_seed(25)
+    q = torch.randn(len(lens), H, hd, generator=g).half()
+    kp, vp = (_cache(n, 1, page, hd, torch.float16, s) for s in (26, 27))
+    got = _check_paged(q, kp, vp, table, lens)
+    assert not got[::49].any()  # those of no length
+
+
+@gpu
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("lens", [[5, 20], [1500, 16]])
 def test_paged_attention_ignores_what_lies_past_the_end(bad, lens):
