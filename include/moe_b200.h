@@ -494,7 +494,9 @@ int moe_rope_append(const moe_rope_append_args_t* args);
  *   page_size % 16 == 0, seqs <= 4095, scale > 0.  The first 4096
  *   bytes of the workspace (counters) must be zero before its first call; every
  *   call leaves them zero, so a workspace serves calls of any shape it is large
- *   enough for, one after another.  Results do not vary from call to call. */
+ *   enough for, one after another: its size depends on the device, heads / kv_heads
+ *   and head_dim alone, not on the number of sequences or pages (0: not supported).
+ *   Results do not vary from call to call. */
 typedef struct moe_paged_attention_args {
   moe_kv_pages_t kv;
   const uint16_t* q;

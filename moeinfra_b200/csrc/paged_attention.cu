@@ -638,12 +638,14 @@ Shape shape_of(int64_t seqs, int kv_heads, int group, int64_t max_tokens) {
   return s;
 }
 
-// The counters lead, so that calls of any shape keep them at the same place.
+// The counters lead, so that calls of any shape keep them at the same place.  The
+// pieces follow, as many as a cut line has: whether a call cuts it changes back and
+// forth with the number of sequences and the table's width, and a workspace made
+// for the largest batch has to serve the smaller ones.
 constexpr size_t kCountBytes = 4096;
 size_t workspace_size(const Shape& s, int hd) {
-  if (s.whole) return kCountBytes;
   return kCountBytes +
-         sizeof(float) * s.ctas * (2 + kMaxWarps) * (s.nt * 8 * (hd + 4) + 2 * s.nt * 8);
+         sizeof(float) * sm_count() * (2 + kMaxWarps) * (s.nt * 8 * (hd + 4) + 2 * s.nt * 8);
 }
 
 template <typename T, int HD, int NT, bool WHOLE, int WARPS>

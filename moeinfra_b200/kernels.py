@@ -768,9 +768,10 @@ def _paged_ws_bytes(device: int, seqs: int, max_pages: int, page: int, heads: in
     return _native.lib().moe_paged_attention_workspace_size(seqs, max_pages, page, heads, kv, hd)
 
 
+@_on_first_device
 def paged_attention_workspace(block_table: torch.Tensor, page_size: int, num_heads: int,
                               kv_heads: int, head_dim: int) -> torch.Tensor:
-    """A workspace for :func:`paged_attention` calls with tables of this size."""
+    """A workspace for :func:`paged_attention` calls with these heads, over tables of any size."""
     nbytes = _paged_ws_bytes(block_table.get_device(), *block_table.shape, page_size, num_heads,
                              kv_heads, head_dim)
     return torch.zeros(nbytes, dtype=torch.uint8, device=block_table.device)

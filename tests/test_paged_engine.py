@@ -98,6 +98,39 @@ def test_paged_stack_matches_the_static_one(heads, kv, hd):
 
 
 @gpu
+def test_every_batch_of_a_wide_stack_decodes():
+    """Batches of 1 to max_batch over tables of 2048 positions, which attention splits otherwise from
+    one number of sequences to the next, all with the stack's one workspace."""
+    from moeinfra_b200.engine.dense import DenseConfig
+    from moeinfra_b200.engine.paged import PagedDenseStack
+    from moeinfra_b200.model.types import LayerWeights
+
+    hidden, heads, kv, hd, vocab, g = 256, 32, 8, 64, 512, torch.Generator().manual_seed(9)
+
+    def r(*shape):
+        return torch.randn(*shape, generator=g) * 0.05
+
+    weights = [LayerWeights(1 + r(hidden), r(heads * hd, hidden), r(kv * hd, hidden),
+                            r(kv * hd, hidden), r(hidden, heads * hd), 1 + r(hidden),
+                            torch.zeros(8, hidden))]
+    args = (DenseConfig(hidden, heads, kv, hd, vocab, 1e6, 1e-5), weights, r(vocab, hidden),
+            1 + r(hidden), r(vocab, hidden), [LinearMoE(r(hidden, hidden).half().cuda())], "cuda")
+    rows, _, _ = _ragged([5 + 3 * i for i in range(32)])
+    tail = torch.randint(0, vocab, (32, 1), generator=g).cuda()
+    with torch.no_grad():
+        stack = PagedDenseStack(*args, max_batch=32, max_len=2048, page_size=64)
+        want = None
+        for B in (32, 19, 18, 8, 1):
+            stack.cache.reserve([len(x) + 1 for x in rows[:B]])
+            stack.prefill(rows[:B])
+            pos = torch.tensor([len(x) for x in rows[:B]], dtype=torch.int32, device="cuda")
+            got = stack.decode(tail[:B], pos).float()
+            want = got if want is None else want
+            err = (got - want[:B]).norm(dim=-1) / want[:B].norm(dim=-1)
+            assert float(err.max()) < 5e-3, B
+
+
+@gpu
 def test_padding_side_batch_order_and_graphs_do_not_matter(ckpt):  # noqa: F811
     rows, ids, mask = _ragged([12, 1, 33])
     _, lids, lmask = _ragged([12, 1, 33], left=True)

@@ -393,6 +393,19 @@ def test_host_checks_precede_every_launch():
     assert _native.status_string(8) != "unknown status"
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(32, 8, 128), (16, 1, 64), (17, 1, 128), (4, 4, 64)])
+def test_a_workspace_serves_smaller_tables_too(heads, kv, hd):
+    """Around 64 and 128 chunks of 16 positions, and the number of processors, the split changes."""
+    from moeinfra_b200 import _native
+
+    size = _native.lib().moe_paged_attention_workspace_size
+    most = size(64, 400, 16, heads, kv, hd)
+    assert most > 4096
+    for seqs in [1, 2, 4, 9, 18, 19, 20, 37, 38, 63, 64]:
+        for pages in [0, 1, 11, 12, 63, 64, 65, 127, 128, 129, 400]:
+            assert 0 < size(seqs, pages, 16, heads, kv, hd) <= most
+
+
 def test_wrappers_refuse_cpu_tensors():
     from moeinfra_b200 import kernels
 
