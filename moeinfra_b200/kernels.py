@@ -667,6 +667,17 @@ def _serve_check(what: str, dev: int, *named) -> None:
             run *= size[i]
 
 
+def _check_workspace(what: str, ws: torch.Tensor, dev: int, nbytes: int) -> None:
+    """A caller's own workspace: packed, on GPU ``dev``, of ``nbytes`` at least."""
+    if not isinstance(ws, torch.Tensor):
+        raise TypeError(f"{what}: workspace must be a torch.Tensor")
+    if ws.get_device() != dev or not ws.is_contiguous():
+        raise ValueError(f"{what}: workspace must be packed and on cuda:{dev}, got {ws.device} "
+                         f"with strides {tuple(ws.stride())}")
+    if ws.numel() * ws.element_size() < nbytes:
+        raise ValueError(f"{what}: workspace needs {nbytes} bytes")
+
+
 def _outer_stride(t: torch.Tensor) -> int:
     """Elements from one index of the first dimension to the next (packed when there is one)."""
     return t.stride(0) if t.shape[0] > 1 else t.numel()
@@ -827,8 +838,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     nbytes = _paged_ws_bytes(dev, seqs, max_pages, page, heads, kv, hd)
     if workspace is None:
         workspace = _serve_scratch(dev, stream, nbytes)
-    elif workspace.numel() * workspace.element_size() < nbytes:
-        raise ValueError(f"{what}: workspace needs {nbytes} bytes")
+    else:
+        _check_workspace(what, workspace, dev, nbytes)
     page_elems = kv * page * hd
     strides = ((page_elems, page_elems, max_pages, heads * hd) if plain else
                (_outer_stride(k_pages), _outer_stride(v_pages), _outer_stride(block_table),
@@ -902,8 +913,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     stream = _raw_stream(dev)
     if workspace is None:
         workspace = _serve_scratch(dev, stream, PROMPT_WORKSPACE_BYTES)
-    elif workspace.numel() * workspace.element_size() < PROMPT_WORKSPACE_BYTES:
-        raise ValueError(f"{what}: workspace needs {PROMPT_WORKSPACE_BYTES} bytes")
+    else:
+        _check_workspace(what, workspace, dev, PROMPT_WORKSPACE_BYTES)
     status = _native.lib().moe_prompt_attention(_native.PROMPT_ATTENTION.pack(
         q.data_ptr(), *_row_strides(q), T, k.data_ptr(), *_row_strides(k), v.data_ptr(),
         *_row_strides(v), k.shape[0], cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), seqs,

@@ -457,3 +457,30 @@ def test_wrappers_refuse_wrong_shapes_and_types():
         with pytest.raises(ValueError):
             kernels.rope_append(args["qkv"], args["cos"], cos, args["pos"], table, kp, kp, 4,
                                 seq_ids=pos)
+
+
+@gpu
+def test_a_callers_workspace_is_checked():
+    """One in host memory, on another device, too small or with gaps is refused before the launch."""
+    from moeinfra_b200 import kernels
+
+    kp = torch.randn(2, 2, 16, 64, device="cuda").half()
+    table = torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    at = torch.full((1,), 9, dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 4, 64, device="cuda").half()
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+
+    def paged(ws):
+        return kernels.paged_attention(q, kp, kp, table, at, workspace=ws)
+
+    def prompt(ws):
+        return kernels.prompt_attention(q, q[:, :2], q[:, 2:], cu, 1, workspace=ws)
+
+    own = kernels.paged_attention_workspace(table, 16, 4, 2, 64)
+    for call in (paged, prompt):
+        assert torch.equal(call(own), call(None))
+        for bad in (own.cpu(), own[:8], torch.zeros(2, own.numel(), device="cuda").t()):
+            with pytest.raises(ValueError, match="workspace"):
+                call(bad)
+        with pytest.raises(TypeError, match="workspace"):
+            call(own.data_ptr())
