@@ -610,14 +610,17 @@ def _plain(dev: int, dtype: torch.dtype, *tensors) -> bool:
 
 
 def _on_first_device(fn):
-    """As :func:`_on_device`, by the device of the first argument alone."""
+    """As :func:`_on_device`, by the device of the first parameter alone."""
+    name = fn.__code__.co_varnames[0]
+
     @functools.wraps(fn)
-    def wrapper(first, *args, **kwargs):
+    def wrapper(*args, **kwargs):
+        first = args[0] if args else kwargs.get(name)
         dev = first.get_device() if isinstance(first, torch.Tensor) else -1
         if dev < 0 or dev == torch.cuda.current_device():
-            return fn(first, *args, **kwargs)
+            return fn(*args, **kwargs)
         with torch.cuda.device(dev):
-            return fn(first, *args, **kwargs)
+            return fn(*args, **kwargs)
     return wrapper
 
 

@@ -5,6 +5,7 @@ roundings of terms at most |x| + |y|); attention's bound is ``oracle.serving.att
 """
 from __future__ import annotations
 
+import inspect
 import random
 
 import pytest
@@ -484,3 +485,58 @@ def test_a_callers_workspace_is_checked():
                 call(bad)
         with pytest.raises(TypeError, match="workspace"):
             call(own.data_ptr())
+
+
+def _one_step(device):
+    """Arguments of each serving operator by name, for one sequence."""
+    def at(t, dtype=torch.float16):
+        return t.to(dtype).to(device)
+
+    g = torch.Generator().manual_seed(1)
+    one, i32, f32 = torch.ones(1), torch.int32, torch.float32
+    pages = at(torch.randn(2, 2, 16, 64, generator=g))
+    cache = dict(k_pages=pages, v_pages=pages.clone(), block_table=at(0 * one[None], i32))
+    q = torch.randn(1, 4, 64, generator=g)
+    return {
+        "rope_append": cache | dict(
+            qkv=at(torch.randn(1, 512, generator=g)), cos=at(torch.rand(4, 32), f32),
+            sin=at(torch.rand(4, 32), f32), positions=at(2 * one, i32), num_heads=4),
+        "paged_attention": cache | dict(q=at(q), lengths=at(9 * one, i32)),
+        "prompt_attention": dict(q=at(q), k=at(q[:, :2]), v=at(q[:, 2:]), max_seqlen=1,
+                                 cu_seqlens=at(torch.arange(2), i32)),
+        "sample_tokens": dict(logits=at(q[0]), uniforms=at(torch.rand(4), f32),
+                              temperature=at(torch.ones(4), f32), top_k=at(torch.zeros(4), i32),
+                              top_p=at(torch.ones(4), f32), min_p=at(torch.zeros(4), f32)),
+        "paged_attention_workspace": dict(block_table=cache["block_table"], page_size=16,
+                                          num_heads=4, kv_heads=2, head_dim=64),
+    }
+
+
+@pytest.mark.parametrize("name", ["rope_append", "paged_attention", "prompt_attention",
+                                  "sample_tokens"])
+def test_arguments_by_name_reach_the_checks(name):
+    from moeinfra_b200 import kernels
+
+    args = _one_step("cpu")[name]
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        getattr(kernels, name)(**args)
+    missing = next(iter(inspect.signature(getattr(kernels, name)).parameters))
+    del args[missing]
+    with pytest.raises(TypeError, match=missing):
+        getattr(kernels, name)(**args)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["rope_append", "paged_attention", "prompt_attention",
+                                  "sample_tokens", "paged_attention_workspace"])
+def test_arguments_by_name_and_by_place(name):
+    from moeinfra_b200 import kernels
+
+    fn, args = getattr(kernels, name), _one_step("cuda")[name]
+    names = [n for n in inspect.signature(fn).parameters if n in args]
+    by_place = [args[n] for n in names]
+    got, want = fn(**args), fn(*by_place)
+    half = fn(by_place[0], **{n: args[n] for n in names[1:]})
+    for out in (got, half):
+        pairs = zip(out, want) if isinstance(want, tuple) else [(out, want)]
+        assert all(torch.equal(a, b) for a, b in pairs)
