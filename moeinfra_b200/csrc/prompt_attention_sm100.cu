@@ -135,6 +135,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -153,12 +158,12 @@ __device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
 // minimax polynomial, n added to the exponent.  Coefficients: Remez exchange
 // on the relative error over [-1/2, 1/2]; degree 3 is off by at most 7.5e-5 (a
 // bf16 probability rounds by 2e-3), degree 4 by 2.6e-6 (fp16: 4.9e-4).
-// Arguments below -120 give 2^-120 (a masked score too: a row that sees nothing
-// is told by its maximum).  NaN gives an infinite or NaN product with V.
+// 2^n is a factor of its own, its exponent's bits from n + 127: arguments of -127
+// and below (a masked score, -inf) give 0, NaN and +inf give NaN.
 template <typename T>
 __device__ __forceinline__ uint64_t exp2_fma(uint64_t x) {
   constexpr float kBig = 12582912.f;
-  x = pair(max_nan(lo_of(x), -120.f), max_nan(hi_of(x), -120.f));
+  x = pair(max_nan(lo_of(x), -127.f), max_nan(hi_of(x), -127.f));
   const uint64_t r = add2(x, pair(kBig, kBig));
   const uint64_t n = add2(r, pair(-kBig, -kBig));
   const uint64_t f = fma2(n, pair(-1.f, -1.f), x);
@@ -173,9 +178,9 @@ __device__ __forceinline__ uint64_t exp2_fma(uint64_t x) {
     p = fma2(p, f, pair(0.693121815f, 0.693121815f));
     p = fma2(p, f, pair(0.999999261f, 0.999999261f));
   }
-  const uint32_t lo = (uint32_t)p + ((uint32_t)r << 23);
-  const uint32_t hi = (uint32_t)(p >> 32) + ((uint32_t)(r >> 32) << 23);
-  return pair(__uint_as_float(lo), __uint_as_float(hi));
+  const uint32_t lo = ((uint32_t)r << 23) + 0x3F800000u;
+  const uint32_t hi = ((uint32_t)(r >> 32) << 23) + 0x3F800000u;
+  return mul2(p, pair(__uint_as_float(lo), __uint_as_float(hi)));
 }
 // Of 8 pairs, those that go through exp2_fma.  With heads of 128 the tensor cores
 // (and the power limit) bound a step and it only costs: 1 x 8192 causal fp16 450 us
@@ -401,7 +406,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       tc_fence_after();
-      const float inv = m == -INFINITY ? 0.f : __fdividef(1.f, l);
+      // A row without keys is zeros.  With keys l is above 0, unless every score is
+      // -inf (0 / 0), and NaN where one is NaN or +inf: the row then is NaN.
+      const bool blind = steps == 0 || seen <= 0;
+      const float inv = 1.f / l;
       // A thread holds a row; written out that way every 16 bytes would touch a
       // line of its own.  64 dims at a time the warp's 32 rows cross shared
       // memory (in the swizzle that the TMA store undoes); where the sequence
@@ -421,9 +429,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            w[hf / 2 + i] = inv == 0.f ? 0u
-                                       : T::pack(__uint_as_float(o[2 * i]) * inv,
-                                                 __uint_as_float(o[2 * i + 1]) * inv);
+            w[hf / 2 + i] = blind ? 0u
+                                  : T::pack(__uint_as_float(o[2 * i]) * inv,
+                                            __uint_as_float(o[2 * i + 1]) * inv);
         }
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store read it
         __syncwarp();

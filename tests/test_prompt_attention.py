@@ -231,3 +231,85 @@ def test_wrapper_refuses_wrong_shapes_and_types():
         attend(scale=0.0)
     with pytest.raises(ValueError, match="workspace"):
         attend(workspace=torch.zeros(8, dtype=torch.uint8, device="cuda"))
+
+
+def _spoilt(q, k, v, lens, sure):
+    """Runs the call; rows that ``sure`` marks must be NaN, the others within the usual bound of
+    what the formula gives without the spoilt rows' keys having an effect."""
+    from moeinfra_b200 import kernels
+
+    got = _run(q, k, v, lens, lens).double().cpu()
+    kernels.check_device()
+    a = 0
+    for n in lens:
+        rows = slice(a, a + n)
+        clean = [torch.nan_to_num(t[rows].double(), 0.0, 0.0, 0.0).to(t.dtype) for t in (q, k, v)]
+        want, weight, off = ref.attention(*clean, q.shape[2] ** -0.5, True)
+        bad = sure[rows]
+        assert got[rows][bad].isnan().all()
+        bound = ref.attention_bound(q.dtype, want, weight, off)
+        assert ((got[rows] - want).abs() <= bound)[~bad].all()
+        a += n
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_nan_of_a_key_or_query_reaches_the_rows_that_see_it(dtype, hd, bad):
+    """At every place of a step's 80 or 96 keys; an infinite score has a NaN softmax too."""
+    lens = [250, 40]
+    for at in list(range(0, 100, 7)) + list(range(1, 97, 8)) + [95, 96, 97, 191, 249, 250, 289]:
+        q, k, v = _inputs(lens, lens, 4, 2, hd, dtype, seed=at)
+        q = q.abs() + 0.1  # inf: every score with the key is +inf
+        k[at, 1] = bad
+        n = torch.arange(290)
+        sees = (n >= at) & ((n < 250) == (at < 250))
+        sure = torch.zeros(290, 4, dtype=torch.bool)
+        sure[sees, 2:] = True
+        _spoilt(q, k, v, lens, sure)
+    q, k, v = _inputs(lens, lens, 4, 2, hd, dtype, seed=1)
+    sure = torch.zeros(290, 4, dtype=torch.bool)
+    for at, h in ((0, 0), (17, 1), (100, 3), (249, 2), (251, 0)):
+        q[at, h] = float("nan")
+        sure[at, h] = True
+    _spoilt(q, k, v, lens, sure)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scores_of_minus_infinity(dtype, hd):
+    """One key of probability 0 leaves a row as if it were not there; with no other key it is 0 / 0."""
+    inf, n = float("inf"), 200
+    q, k, v = _inputs([n], [n], 2, 1, hd, dtype, seed=2)
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    rest = torch.ones(n, dtype=torch.bool)
+    for at in (0, 5, 8, 63, 130):
+        kk = k.clone()
+        kk[at, 0, 0] = -inf
+        got = _run(q, kk, v, [n], [n]).double().cpu()
+        assert got[:1].isnan().all() == (at == 0) and not got[1:].isnan().any()
+        rest[:], rest[at] = True, False
+        want, weight, off = ref.attention(q[-1:], k[rest], v[rest], hd ** -0.5, True)
+        bound = ref.attention_bound(dtype, want, weight, off)
+        assert ((got[-1:] - want).abs() <= bound).all()
+    k[:, 0, 0] = -inf
+    assert _run(q, k, v, [n], [n]).isnan().all()
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_large_values_of_keys_not_seen_have_no_effect(hd):
+    """bf16 values near the largest: a probability that is merely tiny would let them through."""
+    n = 150
+    q, k, v = _inputs([n], [n], 2, 1, hd, torch.bfloat16, seed=3)
+    clean = _run(q, k, v, [n], [n])
+    for at in (1, 8, 16, 79, 100):
+        w = v.clone()
+        w[at:] = 3e38
+        got = _run(q, k, w, [n], [n])
+        want, weight, off = ref.attention(q[:at], k[:at], v[:at], hd ** -0.5, True)
+        bound = ref.attention_bound(torch.bfloat16, want, weight, off)
+        assert ((got[:at].double().cpu() - want).abs() <= bound).all()
+    assert torch.equal(clean, _run(q, k, v, [n], [n]))
