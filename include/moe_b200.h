@@ -524,7 +524,8 @@ int moe_paged_attention(const moe_paged_attention_args_t* args);
  *   is counts as out of range, and so do offsets outside the rows; rows of such
  *   a sequence are not written).  out [q_rows, heads, head_dim] packed.  fp32
  *   scores, softmax and sums; the probabilities are rounded to the element type
- *   for the product with V.  Values of other sequences have no effect.
+ *   for the product with V.  Values of other sequences, and of keys that a row
+ *   does not see, have no effect, infinities and NaN included.
  *   scale > 0.  The workspace (counters) must be zero before its first call and
  *   is left zero, as moe_paged_attention's, which may be the same. */
 size_t moe_prompt_attention_workspace_size(void);

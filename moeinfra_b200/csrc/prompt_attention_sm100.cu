@@ -95,6 +95,8 @@ struct PromptArgs {
   int blocks;                   // ceil(max_q / tokens of an item)
   bool causal;
   float scale_log2;
+  const uint16_t *q, *k, *v;    // for redo_row alone; strides in elements
+  int64_t q_stride, q_head, k_stride, k_head, v_stride, v_head;
   uint16_t* out;                // [rows_q, heads, HD]
   uint32_t* counts;             // items claimed, CTAs done: zero between calls
   uint64_t wait_ns;
@@ -204,6 +206,68 @@ __device__ __forceinline__ void store_cols(uint32_t at, const uint32_t* v) {
   if constexpr (N % 32 == 16) tmem_st16(at + N / 32 * 32, v + N / 32 * 32);
 }
 
+// acc + 0 * v for two 16-bit values: NaN once one was infinite or NaN, else +0.
+template <typename T>
+__device__ __forceinline__ uint32_t trace_odd(uint32_t v, uint32_t acc) {
+  if constexpr (T::kBf16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0));
+  return acc;
+}
+
+// One row by the formula, by one warp: 32 keys a step, one to a lane, then their
+// values, HD / 32 dims to a lane.  q, k, v: the row's query, the first key and value
+// that it sees.
+template <typename T, int HD>
+__device__ __forceinline__ void redo_row(const uint16_t* q, const uint16_t* k, int64_t k_stride,
+                                         const uint16_t* v, int64_t v_stride, int seen,
+                                         float scale_log2, uint16_t* out) {
+  constexpr int kWords = HD / 64;
+  const int lane = threadIdx.x & 31;
+  float m = -INFINITY, l = 0.f;
+  float2 acc[kWords] = {};
+#pragma unroll 1
+  for (int j0 = 0; j0 < seen; j0 += 32) {
+    float s = -INFINITY;
+    if (j0 + lane < seen) {
+      const uint16_t* row = k + (j0 + lane) * k_stride;
+      s = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < HD; d += 2) {
+        const float2 x = T::unpack(*reinterpret_cast<const uint32_t*>(q + d));
+        const float2 y = T::unpack(*reinterpret_cast<const uint32_t*>(row + d));
+        s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
+      }
+      s *= scale_log2;
+    }
+    float top = s;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float nm = fmaxf(m, top), f = m == nm ? 1.f : exp2_approx(m - nm);
+    m = nm;
+    const float p = j0 + lane < seen ? exp2_approx(s - (m == -INFINITY ? 0.f : m)) : 0.f;
+    l = l * f + warp_sum(p);
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) acc[w] = make_float2(acc[w].x * f, acc[w].y * f);
+#pragma unroll 1
+    for (int i = 0; i < min(32, seen - j0); ++i) {
+      const float pi = __shfl_sync(0xffffffffu, p, i);
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        const float2 x = T::unpack(
+            *reinterpret_cast<const uint32_t*>(v + (j0 + i) * v_stride + w * 64 + lane * 2));
+        acc[w] = make_float2(fmaf(pi, x.x, acc[w].x), fmaf(pi, x.y, acc[w].y));
+      }
+    }
+    if (l != l) break;  // and stays so
+  }
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int w = 0; w < kWords; ++w)
+    *reinterpret_cast<uint32_t*>(out + w * 64 + lane * 2) = T::pack(acc[w].x * inv, acc[w].y * inv);
+}
+
 struct __align__(16) Item {
   int h, q0;            // first head (-1: no more items), first token in the sequence
   int len_q, len_k;
@@ -258,6 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       s_itfull[kItems], s_itempty[kItems];
   __shared__ Item s_item[kItems];
   __shared__ uint32_t s_tmem;
+  __shared__ int2 s_keys[kSoftWarps];  // first row and number of the keys a softmax warp is at
   __shared__ volatile int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (saddr(smem_raw) + 1023u) & ~1023u;
@@ -329,6 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int first = it.q0 + t * (kM >> a.pack), q = first + (row >> a.pack);  // the row's token
       if (first >= it.len_q) continue;
       const int steps = t ? it.steps1 : it.steps0;
+      if (lane == 0) s_keys[warp] = make_int2(it.row_k, it.len_k);
       // Keys this row sees.
       const int seen = a.causal ? min(it.len_k, q + 1 + it.len_k - it.len_q) : it.len_k;
       float m = -INFINITY, l = 0.f;
@@ -409,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // A row without keys is zeros.  With keys l is above 0, unless every score is
       // -inf (0 / 0), and NaN where one is NaN or +inf: the row then is NaN.
       const bool blind = steps == 0 || seen <= 0;
-      const float inv = 1.f / l;
+      const float inv = __fdividef(1.f, l);
       // A thread holds a row; written out that way every 16 bytes would touch a
       // line of its own.  64 dims at a time the warp's 32 rows cross shared
       // memory (in the swizzle that the TMA store undoes); where the sequence
@@ -417,6 +483,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int lane_row = (warp & 3) * 32, heads_mask = (1 << a.pack) - 1;
       const int warp_token = first + (lane_row >> a.pack);
       const bool whole = warp_token + (32 >> a.pack) <= it.len_q;
+      const uint64_t inv2 = pair(inv, inv);
+      uint64_t odd[2] = {0, 0};  // sums of products of O: not finite once an element is not
 #pragma unroll 1
       for (int c = 0; c < HD; c += 64) {
         uint32_t w[32];
@@ -428,10 +496,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_wait_ld();
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            w[hf / 2 + i] = blind ? 0u
-                                  : T::pack(__uint_as_float(o[2 * i]) * inv,
-                                            __uint_as_float(o[2 * i + 1]) * inv);
+          for (int i = 0; i < 16; i += 2) {
+            const uint64_t x = pair(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+            const uint64_t y = pair(__uint_as_float(o[2 * i + 2]), __uint_as_float(o[2 * i + 3]));
+            odd[i / 2 & 1] = fma2(x, y, odd[i / 2 & 1]);
+            const uint64_t xs = mul2(x, inv2), ys = mul2(y, inv2);
+            w[hf / 2 + i] = blind ? 0u : T::pack(lo_of(xs), hi_of(xs));
+            w[hf / 2 + i + 1] = blind ? 0u : T::pack(lo_of(ys), hi_of(ys));
+          }
         }
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last store read it
         __syncwarp();
@@ -463,6 +535,37 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (token < it.len_q)
             *reinterpret_cast<uint4*>(a.out + ((int64_t)(it.row_q + token) * a.heads + head) * HD +
                                       c + col8 * 8) = w;
+        }
+      }
+      // A probability of 0 does not silence an infinity or NaN among the values of
+      // a key that this row does not see and others of the tile do.  Rows that may
+      // have met one are computed again without the tile.  Looking costs 1 % (64
+      // prompts of 129..512: 119.6 -> 120.7 us in a graph; heads of 64 99 -> 101).
+      const uint64_t both = add2(odd[0], odd[1]);
+      const bool finite = fabsf(lo_of(both)) + fabsf(hi_of(both)) < INFINITY;
+      uint32_t again = __ballot_sync(0xffffffffu, !finite && !blind && q < it.len_q);
+      if (again) {
+        __syncwarp();
+        const int2 keys = s_keys[warp];  // kept out of the registers until here
+        const int loaded = min(steps * kN, keys.y), kv_head = it.h / a.group;
+        const uint16_t* v = a.v + keys.x * a.v_stride + kv_head * a.v_head;
+        again &= __ballot_sync(0xffffffffu, seen < loaded);
+        const int from = __reduce_min_sync(0xffffffffu, again >> lane & 1 ? seen : loaded);
+        uint32_t met = 0;
+        for (int i = lane; i < (loaded - from) * (HD / 2); i += 32)  // at most a tile and a step
+          met = trace_odd<T>(*reinterpret_cast<const uint32_t*>(
+                                 v + (from + i / (HD / 2)) * a.v_stride + i % (HD / 2) * 2), met);
+        if (!__any_sync(0xffffffffu, met)) again = 0;
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the rows are written once more
+        __syncwarp();
+        for (; again; again &= again - 1) {
+          const int r = __ffs(again) - 1;
+          const int64_t at = it.row_q + first + ((lane_row + r) >> a.pack);
+          const int head = it.h + (r & heads_mask);
+          redo_row<T, HD>(a.q + at * a.q_stride + head * a.q_head,
+                          a.k + keys.x * a.k_stride + kv_head * a.k_head, a.k_stride, v, a.v_stride,
+                          __shfl_sync(0xffffffffu, seen, r), a.scale_log2,
+                          a.out + (at * a.heads + head) * HD);
         }
       }
       tc_fence_before();
@@ -797,6 +900,15 @@ extern "C" int moe_prompt_attention(const moe_prompt_attention_args_t* args) {
   a.blocks = static_cast<int>(ceil_div(c.max_q, 2 * kM >> pack));
   a.causal = c.causal != 0;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.q = c.q;
+  a.k = c.k;
+  a.v = c.v;
+  a.q_stride = c.q_stride;
+  a.q_head = c.q_head_stride;
+  a.k_stride = c.k_stride;
+  a.k_head = c.k_head_stride;
+  a.v_stride = c.v_stride;
+  a.v_head = c.v_head_stride;
   a.out = c.out;
   a.counts = static_cast<uint32_t*>(c.workspace);
   a.wait_ns = wait_limit_ns();

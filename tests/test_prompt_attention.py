@@ -313,3 +313,57 @@ def test_large_values_of_keys_not_seen_have_no_effect(hd):
         bound = ref.attention_bound(torch.bfloat16, want, weight, off)
         assert ((got[:at].double().cpu() - want).abs() <= bound).all()
     assert torch.equal(clean, _run(q, k, v, [n], [n]))
+
+
+def _value_spoilt(lens, lens_k, H, KV, hd, dtype, at, dims, bad):
+    """Value row ``at`` of every KV head is ``bad`` in ``dims``: rows that see it are not finite there,
+    all else is as the formula says."""
+    from moeinfra_b200 import kernels
+
+    q, k, v = _inputs(lens, lens_k, H, KV, hd, dtype, seed=at)
+    spoilt = v.clone()
+    spoilt[at, :, dims] = bad
+    got = _run(q, k, spoilt, lens, lens_k).double().cpu()
+    kernels.check_device()
+    a = c = 0
+    for n, m in zip(lens, lens_k):
+        want, weight, off = ref.attention(q[a:a + n], k[c:c + m], v[c:c + m], hd ** -0.5, True)
+        sees = (torch.arange(n) + m - n + c >= at) & (c <= at < c + m)
+        odd = torch.zeros(n, H, hd, dtype=torch.bool)
+        odd[sees, :, dims] = True
+        mine = got[a:a + n]
+        assert not mine[odd].isfinite().any()
+        # The spoilt row counts in no other row, and in no other dim of the rows that see it.
+        bound = ref.attention_bound(dtype, want, weight, off)
+        assert ((mine - want).abs() <= bound)[~odd].all(), (at, n, m)
+        a, c = a + n, c + m
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H,KV", [(8, 2), (1, 1), (16, 1), (3, 1)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_values_of_keys_not_seen_have_no_effect(dtype, hd, H, KV, bad):
+    """Infinities and NaN among the values of later keys, which share tiles with the rows before."""
+    for at in (0, 1, 40, 79, 80, 95, 96, 127, 128, 170, 255, 299, 300, 330):
+        for dims in (slice(None), slice(3, 4)):
+            _value_spoilt([300, 35], [300, 35], H, KV, hd, dtype, at, dims, bad)
+    for at in (10, 333, 399, 400, 419):  # prompts that continue earlier keys; fewer keys than queries
+        _value_spoilt([130, 40], [400, 20], H, KV, hd, dtype, at, slice(None), bad)
+
+
+@gpu
+def test_values_not_seen_in_strided_rows():
+    from moeinfra_b200 import kernels
+
+    lens, H, KV, hd = [150, 33], 4, 2, 64
+    g = torch.Generator().manual_seed(3)
+    qkv = torch.randn(sum(lens), H + 2 * KV, hd, generator=g).half().cuda()
+    qkv[100, H + KV:] = float("inf")
+    cu = _offsets(lens).cuda()
+    q, k, v = qkv[:, :H], qkv[:, H:H + KV], qkv[:, H + KV:]
+    got = kernels.prompt_attention(q, k, v, cu, max(lens))
+    packed = kernels.prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu, max(lens))
+    assert torch.equal(got[:100], packed[:100]) and got[:100].isfinite().all()
+    assert not got[100:150].isfinite().any() and torch.equal(got[150:], packed[150:])
