@@ -41,6 +41,9 @@ MOE_DEFINE_ERROR_WORD()
 constexpr int kMaxWarps = 8;        // of a CTA that is alone on its SM; with two to an SM it has half
 constexpr int kChunk = 16;          // keys per chunk (a page holds whole chunks)
 constexpr int kMaxSeqs = 4095;      // what they need of shared memory: see line_bytes
+// Places in the line are 32-bit, and a share's end or a look ahead may lie a little
+// past the last one.
+constexpr int64_t kMostChunks = INT32_MAX - 4096;
 // Smallest share of a CTA in chunks when the line is cut: below it a CTA's
 // pieces cost more to join than they save (1 x 4096: 13.9 us with 8, 9.8 with 16,
 // 10.0 with 32; 32 x 100: 10.9, 11.2, 13.6).
@@ -706,7 +709,7 @@ extern "C" int moe_paged_attention(const moe_paged_attention_args_t* args) {
   if (!aligned16(c.q) || !aligned16(c.out) || (c.q_stride & 7)) return MOE_ERR_ALIGNMENT;
   const Shape sh = shape_of(c.kv.seqs, static_cast<int>(c.kv.kv_heads),
                             static_cast<int>(c.heads / c.kv.kv_heads), c.kv.max_pages * c.kv.page_size);
-  if (sh.units * sh.chunks > INT32_MAX) return MOE_ERR_UNSUPPORTED;  // 32-bit on the device
+  if (sh.units * sh.chunks > kMostChunks) return MOE_ERR_UNSUPPORTED;
   if (!c.workspace || c.workspace_bytes < (int64_t)workspace_size(sh, static_cast<int>(hd)))
     return MOE_ERR_WORKSPACE;
   if (!aligned16(c.workspace)) return MOE_ERR_ALIGNMENT;

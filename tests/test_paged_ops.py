@@ -407,6 +407,22 @@ def test_a_workspace_serves_smaller_tables_too(heads, kv, hd):
             assert 0 < size(seqs, pages, 16, heads, kv, hd) <= most
 
 
+def test_lines_too_long_for_32_bits_are_refused():
+    """16 sequences in tables of 134217727 pages of 16: 2^31 - 16 chunks.  Fewer sequences get as
+    far as the check of the workspace."""
+    from moeinfra_b200 import _native
+
+    lib, f = _native.lib(), 0x100000
+
+    def attend(seqs, pages, hd=128):
+        return lib.moe_paged_attention(_native.PAGED_ATTENTION.pack(
+            f, f, 16 * hd, 16 * hd, 9, 1, 16, hd, 0, f, pages, seqs, pages, f, hd, 1, f, 1.0, f, f, 0,
+            0))
+
+    assert attend(16, 134217727) == 2
+    assert attend(8, 134217727) == 4 and attend(15, 134217727) == 4
+
+
 def test_wrappers_refuse_cpu_tensors():
     from moeinfra_b200 import kernels
 
