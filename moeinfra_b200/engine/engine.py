@@ -403,6 +403,13 @@ class InferenceEngine:
             return torch.zeros(B, dtype=torch.int32, device=self._device)
         return torch.zeros(1, dtype=torch.long, device=self._device)
 
+    def _set_positions(self, positions: torch.Tensor) -> None:
+        """The first decoded tokens' positions, after the prompts; the host waits for nothing."""
+        if self._paged:
+            positions.copy_(self._stack.prompt_lengths)
+        else:
+            positions.fill_(self._prompt_lens[0])
+
     @torch.no_grad()
     def _decode(self, next_token_logits: torch.Tensor, max_new_tokens: int,
                 sampler: Optional["_Sampler"] = None) -> list:
@@ -418,7 +425,6 @@ class InferenceEngine:
             raise ValueError(f"{lens[0] + max_new_tokens} positions exceed "
                              f"engine.max_seq_len={self._max_len}")
         dev = self._device
-        start = torch.tensor(lens if self._paged else lens[:1])
         with torch.cuda.device(dev):
             hist = torch.empty(B, max_new_tokens, dtype=torch.long, device=dev)
             if sampler is None:
@@ -432,7 +438,7 @@ class InferenceEngine:
                 if use_graph:
                     g, ids_buf, pos_buf, out, captured = self._graph_for(B, sampler is not None)
                     ids_buf.copy_(first[:, None])
-                    pos_buf.copy_(start)
+                    self._set_positions(pos_buf)
                     if sampler is not None:
                         sampler.lend(captured)
                     for i in range(1, max_new_tokens):
@@ -444,7 +450,7 @@ class InferenceEngine:
                 else:
                     ids_buf = first[:, None].clone()
                     pos_buf = self._positions(B)
-                    pos_buf.copy_(start)
+                    self._set_positions(pos_buf)
                     step = self._decode_step_fn(ids_buf, pos_buf, sampler)
                     for i in range(1, max_new_tokens):
                         if sampler is not None:

@@ -102,7 +102,8 @@ class PagedDenseStack(DenseStack):
     def prefill(self, prompts: list[torch.Tensor]) -> torch.Tensor:
         """Whole prompts, packed: each a 1-D tensor of ids; fp16 logits of their last positions.
 
-        The cache must hold pages for them (``cache.reserve``)."""
+        The cache must hold pages for them (``cache.reserve``).  ``prompt_lengths`` then is their
+        lengths on the device, int32: the positions of the tokens that follow."""
         cfg = self.cfg
         lens = [int(p.numel()) for p in prompts]
         if not lens or min(lens) < 1 or max(lens) > self.max_len or len(lens) > self.max_batch:
@@ -116,6 +117,7 @@ class PagedDenseStack(DenseStack):
         pos = torch.arange(len(seq), dtype=torch.int32) - cu[seq.long()]
         last = (cu[1:] - 1).long().to(self.device)
         cu, seq, pos = (t.to(self.device) for t in (cu, seq, pos))
+        self.prompt_lengths = cu.diff()
         H, KV, hd = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
         table = self.cache.block_table
 

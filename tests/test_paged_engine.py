@@ -219,6 +219,36 @@ def test_request_checks(ckpt):  # noqa: F811
         InferenceEngine(_config(ckpt, engine=PAGED) | {"parallel": {"expert_parallel": True}})
 
 
+@gpu
+@pytest.mark.parametrize("paged", [True, False])
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("sampled", [True, False])
+def test_decoding_waits_for_the_device_once(ckpt, paged, graphs, sampled):  # noqa: F811
+    """The tokens' way back is the only point where the host waits in the decode stage."""
+    import warnings
+
+    from moeinfra_b200.engine.engine import InferenceEngine, _Sampler
+    from moeinfra_b200.engine.types import ForwardRequest, SamplingParams
+
+    over = (PAGED if paged else {"max_batch": 3}) | {"cuda_graphs": graphs}
+    ids = torch.randint(0, V, (3, 10), generator=torch.Generator().manual_seed(7))
+    params = SamplingParams(seed=1) if sampled else None
+    with InferenceEngine(_config(ckpt, engine=over)) as eng:
+        want = eng.generate(ForwardRequest(ids, None, 6, params)).token_ids
+        logits = eng._prefill(ids)
+        sampler = _Sampler(params, 3, 6, eng._device) if sampled else None
+        torch.cuda.synchronize()
+        torch.cuda.set_sync_debug_mode("warn")
+        try:
+            with warnings.catch_warnings(record=True) as seen:
+                warnings.simplefilter("always")
+                got = eng._decode(logits, 6, sampler)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+        assert got == want
+        assert sum("synchronizing" in str(w.message) for w in seen) == 1, [str(w) for w in seen]
+
+
 def test_cache_hands_out_and_takes_back_pages():
     """Host logic of the page pool (CPU)."""
     from moeinfra_b200.engine.paged import PagedKVCache
