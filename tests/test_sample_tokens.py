@@ -371,3 +371,31 @@ def test_lists_that_fill_while_they_are_gathered(dtype):
     for kw in (dict(top_k=k), dict(top_k=k, min_p=0.05), dict(top_k=k, top_p=0.9),
                dict(top_p=[0.05 + 0.003 * i for i in range(rows)])):
         _compare(x, u, _params(rows, 0.7, **kw))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [20001, 70001, 140001])
+def test_a_row_alone_and_in_a_batch(dtype, vocab):
+    """40 rows take a CTA each, one row is spread over a cluster (8, 16 or 32 logits a thread): the
+    same token and the same bits of its probability."""
+    from moeinfra_b200 import kernels
+
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    rows = 40
+    x = 2.5 * torch.randn(rows, vocab, device="cuda", generator=g)
+    x[::5] = x[::5].round()  # thousands of ties
+    x[::7, ::3] = float("nan")
+    x = x.to(dtype)
+    u = torch.rand(rows, device="cuda", generator=g)
+
+    def cycle(values):
+        return [values[i % len(values)] for i in range(rows)]
+
+    for shift in range(2):
+        params = _params(rows, cycle([0.8, 1.0, 0.0, 1.7][shift:]), cycle([0, 50, 3000, 0, 1, 1000][shift:]),
+                         cycle([0.95, 1.0, 0.999, 0.5][shift:]), cycle([0.0, 0.0, 0.05][shift:]))
+        tokens, probs = _compare(x, u, params)
+        for i in range(rows):
+            token, prob = kernels.sample_tokens(x[i:i + 1], u[i:i + 1], *(p[i:i + 1] for p in params))
+            assert torch.equal(token[0], tokens[i]) and torch.equal(prob[0], probs[i]), i
