@@ -277,15 +277,9 @@ struct __align__(16) Item {
 constexpr int kItems = 1;                   // items looked up ahead
 constexpr int kReaders = kSoftWarps + 3;    // warps that read each of them
 
-// Block x of the launch (all heads of 256 >> pack tokens of a sequence, the last
-// tokens first); false where the sequence has no such block.  A sequence whose
-// offsets do not describe rows of q and k, or that is longer than the call
-// said, counts as empty (error bit set).
-template <int HD>
-__device__ __forceinline__ bool get_block(const PromptArgs& a, uint32_t x, Item& it) {
-  const uint32_t blk = x / a.seqs, b = x - blk * a.seqs;
-  const int tokens = kM >> a.pack;
-  it.q0 = (a.blocks - 1 - (int)blk) * 2 * tokens;
+// A sequence's first rows and lengths; false, with the error bit set, if its offsets
+// do not describe rows of q and k or it is longer than the call said.
+__device__ __forceinline__ bool get_sequence(const PromptArgs& a, uint32_t b, Item& it) {
   const int q_lo = a.cu_q[b], q_hi = a.cu_q[b + 1], k_lo = a.cu_k[b], k_hi = a.cu_k[b + 1];
   it.len_q = q_hi - q_lo;
   it.len_k = k_hi - k_lo;
@@ -296,7 +290,17 @@ __device__ __forceinline__ bool get_block(const PromptArgs& a, uint32_t x, Item&
     set_device_error(kErrPage);
     return false;
   }
-  if (it.q0 >= it.len_q) return false;
+  return true;
+}
+
+// Block x of the launch (all heads of 256 >> pack tokens of a sequence, the last
+// tokens first); false where the sequence has no such block, or counts as empty.
+template <int HD>
+__device__ __forceinline__ bool get_block(const PromptArgs& a, uint32_t x, Item& it) {
+  const uint32_t blk = x / a.seqs, b = x - blk * a.seqs;
+  const int tokens = kM >> a.pack;
+  it.q0 = (a.blocks - 1 - (int)blk) * 2 * tokens;
+  if (!get_sequence(a, b, it) || it.q0 >= it.len_q) return false;
   constexpr int kN = Cfg<HD>::kN;
   auto steps = [&](int first) {
     int keys = it.len_k;
@@ -725,14 +729,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     // counter as it goes: lengths and clocks differ too much for a fixed share
     // (64 prompts of 129 to 512 tokens: 138 us, 103 of them at the median CTA).
     // To find an item's block, every CTA walks the blocks, 32 at a time, and
-    // counts those with rows.
+    // counts those with rows.  After some without any it looks for the next that has
+    // (the stated maximum may be far above the lengths, or one sequence above the
+    // others: 1000 prompts of 1..64 stated as up to 131072 took 60 ms, 64 prompts of
+    // 129..512 1.1).
     const uint32_t groups = a.heads >> a.pack, blocks = (uint32_t)a.blocks * a.seqs;
+    constexpr int kEmpty = 4;  // looks without a block before the next is searched for
     uint32_t n = 0, n_q = 0, at = 0, before = 0, live = 0;
+    int empty = 0;
     bool ok = true, mine = false;
     auto look = [&]() {  // the next 32 blocks
       mine = at + lane < blocks && get_block<HD>(a, at + lane, it);
       live = __ballot_sync(0xffffffffu, mine);
       at += 32;
+    };
+    auto skip = [&]() {  // from block `at` to the next that has rows
+      const uint32_t tokens = 2 * kM >> a.pack;
+      uint32_t next = blocks;
+      for (uint32_t b = lane; b < (uint32_t)a.seqs; b += 32) {
+        Item one;
+        if (!get_sequence(a, b, one)) continue;
+        const uint32_t first = a.blocks - ((uint32_t)one.len_q + tokens - 1) / tokens;
+        const uint32_t blk = max(first, at > b ? (at - b + a.seqs - 1) / a.seqs : 0u);
+        if (blk < (uint32_t)a.blocks) next = min(next, blk * a.seqs + b);
+      }
+      at = __reduce_min_sync(0xffffffffu, next);
     };
     auto push = [&](uint32_t from) {  // lane `from` hands its item on
       ok = ok && warp_wait(saddr(&s_itempty[n % kItems]), (n / kItems & 1) ^ 1, a.wait_ns);
@@ -749,6 +770,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t block = y / groups;
       while (block >= before + __popc(live) && at < blocks) {
         before += __popc(live);
+        empty = live ? 0 : empty + 1;
+        if (empty == kEmpty) {
+          skip();
+          empty = 0;
+        }
         look();
       }
       if (block >= before + __popc(live)) break;

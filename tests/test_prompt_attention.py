@@ -367,3 +367,48 @@ def test_values_not_seen_in_strided_rows():
     packed = kernels.prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu, max(lens))
     assert torch.equal(got[:100], packed[:100]) and got[:100].isfinite().all()
     assert not got[100:150].isfinite().any() and torch.equal(got[150:], packed[150:])
+
+
+@gpu
+@pytest.mark.parametrize("H,KV", [(4, 1), (2, 2), (16, 1)])
+@pytest.mark.parametrize("lens", [[5], [300, 1, 0, 64], [1 + i % 64 for i in range(1000)],
+                                  [0] * 700 + [40] + [0] * 700, [9] * 500 + [3000] + [17] * 500,
+                                  [0, 0, 0]])
+def test_lengths_far_below_the_stated_maximum(H, KV, lens):
+    from moeinfra_b200 import kernels
+
+    q, k, v = (t.cuda() for t in _inputs(lens, lens, H, KV, 64, torch.float16, seed=len(lens)))
+    cu = _offsets(lens).cuda()
+    want = kernels.prompt_attention(q, k, v, cu, max(max(lens), 1))
+    most = 131072 if len(lens) * H < 4000 else 32768
+    for stated in (max(lens) + 1, 4096, most):
+        assert torch.equal(kernels.prompt_attention(q, k, v, cu, stated), want)
+    kernels.check_device()
+    # Offsets that are wrong anywhere are still reported, those of empty sequences too.
+    bad_k = cu.clone()
+    bad_k[-1] = q.shape[0] + 1
+    kernels.prompt_attention(q, k, v, cu, most, cu_seqlens_k=bad_k, max_seqlen_k=most)
+    if q.shape[0]:
+        with pytest.raises(RuntimeError, match="out of range"):
+            kernels.check_device()
+    kernels.check_device()
+
+
+@gpu
+def test_a_stated_maximum_that_takes_long_to_walk():
+    """2 million blocks of which the last 2000 or so have rows (walking them took 15 ms): no wait runs
+    out."""
+    from moeinfra_b200 import _native, kernels
+
+    lens, H = [1 + i % 30 for i in range(1000)], 16
+    q, k, v = (t.cuda() for t in _inputs(lens, lens, H, 1, 64, torch.float16))
+    cu = _offsets(lens).cuda()
+    want = kernels.prompt_attention(q, k, v, cu, 30)
+    old = _native.wait_limit_ns()
+    _native.set_wait_limit_ns(5_000_000)
+    try:
+        got = kernels.prompt_attention(q, k, v, cu, 32768)
+        kernels.check_device()
+    finally:
+        _native.set_wait_limit_ns(old)
+    assert torch.equal(got, want)
