@@ -548,7 +548,7 @@ typedef struct moe_prompt_attention_args {
 int moe_prompt_attention(const moe_prompt_attention_args_t* args);
 
 /* moe_sample_tokens: one token per row of logits [rows, vocab] (fp16, bf16 or
- *   fp32, rows stride elements apart, vocab <= 262144).  With m a row's maximum,
+ *   fp32, rows stride elements apart, 0: one row for all, vocab <= 262144).  With m a row's maximum,
  *   e_i = exp((x_i - m) / temperature) in fp32 (1 where x_i == m; NaN logits
  *   count as -inf) and the integer weights w_i = trunc(2^40 e_i), over the tokens
  *   by falling logit, equal ones by rising index: top_k > 0 keeps the first

@@ -586,7 +586,8 @@ extern "C" int moe_sample_tokens(const moe_sample_tokens_args_t* args) {
   using namespace moe;
   if (!args) return MOE_ERR_INVALID_ARG;
   const moe_sample_tokens_args_t& c = *args;
-  if (c.rows < 0 || c.vocab < 1 || (c.rows > 1 && c.stride < c.vocab)) return MOE_ERR_INVALID_ARG;
+  if (c.rows < 0 || c.vocab < 1 || (c.rows > 1 && c.stride != 0 && c.stride < c.vocab))
+    return MOE_ERR_INVALID_ARG;
   if (c.dtype != MOE_DTYPE_F16 && c.dtype != MOE_DTYPE_BF16 && c.dtype != MOE_DTYPE_F32)
     return MOE_ERR_UNSUPPORTED;
   if (c.vocab > kMaxVocab) return MOE_ERR_UNSUPPORTED;

@@ -934,7 +934,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: tor
                   top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor):
     """``(tokens int64 [rows], probs fp32 [rows])``: one token per row of ``logits`` [rows, vocab].
 
-    ``logits`` fp16, bf16 or fp32 (rows may be strided, vocab <= 262144); ``uniforms`` fp32 [rows]
+    ``logits`` fp16, bf16 or fp32 (rows may be strided, or one row expanded; vocab <= 262144); ``uniforms`` fp32 [rows]
     in [0, 1), the row's random number; ``temperature`` / ``top_p`` / ``min_p`` fp32 and ``top_k``
     int32 [rows].  Temperature 0 takes the maximum (lowest index); top_k 0, top_p 1 and min_p 0 are
     off; the filters apply in that order, top-p to what top-k leaves.  ``probs`` is the token's

@@ -399,3 +399,14 @@ def test_a_row_alone_and_in_a_batch(dtype, vocab):
         for i in range(rows):
             token, prob = kernels.sample_tokens(x[i:i + 1], u[i:i + 1], *(p[i:i + 1] for p in params))
             assert torch.equal(token[0], tokens[i]) and torch.equal(prob[0], probs[i]), i
+
+
+@gpu
+@pytest.mark.parametrize("rows,vocab", [(5, 20001), (200, 3000)])
+def test_several_tokens_of_one_row(rows, vocab):
+    """A row expanded, not copied: as many draws as random numbers."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = 3 * torch.randn(1, vocab, device="cuda", generator=g).half()
+    u = torch.rand(rows, device="cuda", generator=g)
+    tokens, _ = _compare(x.expand(rows, vocab), u, _params(rows, 1.0, 0, 0.95))
+    assert len(set(tokens.tolist())) > 1
