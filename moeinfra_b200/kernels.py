@@ -829,7 +829,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         heads = q.shape[1]
     if page % 16:
         raise ValueError(f"{what}: page_size must be a multiple of 16, got {page}")
-    if heads == 0 or heads % kv:
+    if heads == 0 or kv == 0 or heads % kv:
         raise ValueError(f"{what}: {heads} query heads do not divide over {kv} KV heads")
     if out is None:
         out = q.new_empty((seqs, heads, hd))

@@ -556,3 +556,16 @@ def test_arguments_by_name_and_by_place(name):
     for out in (got, half):
         pairs = zip(out, want) if isinstance(want, tuple) else [(out, want)]
         assert all(torch.equal(a, b) for a, b in pairs)
+
+
+@gpu
+def test_a_cache_without_heads_is_refused():
+    from moeinfra_b200 import kernels
+
+    none = torch.zeros(2, 0, 16, 64, dtype=torch.float16, device="cuda")
+    at = torch.ones(1, dtype=torch.int32, device="cuda")
+    q = torch.zeros(1, 4, 64, dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError, match="KV heads"):
+        kernels.paged_attention(q, none, none, at[None], at)
+    with pytest.raises(ValueError, match="KV heads"):
+        kernels.prompt_attention(q, q[:, :0], q[:, :0], torch.arange(2).int().cuda(), 1)
