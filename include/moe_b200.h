@@ -434,8 +434,8 @@ int moe_ep_return_partials_p2p(const float* y_part, int S, const int32_t* recv_c
  * from one page to the next (at least a page, a multiple of 8), a page itself
  * is contiguous.  block_table int32 [seqs, max_pages] (rows table_stride
  * elements apart) lists each sequence's pages: its position p is row
- * p % page_size of page table[b][p / page_size].  Entries past a sequence's
- * last page are never read.  Two sequences may list the same page.
+ * p % page_size of page table[b][p / page_size].  What the entries past a
+ * sequence's last page hold has no effect.  Two sequences may list the same page.
  *
  * The entry points take their arguments as a structure of 8-byte fields, read
  * before they return.
@@ -521,11 +521,11 @@ int moe_paged_attention(const moe_paged_attention_args_t* args);
  *   in elements, multiples of 8.  causal != 0: the queries are the last of the
  *   sequence's positions, query i sees keys j <= i + len_k - len_q; a query
  *   without keys gives zeros.  max_q / max_k: no sequence is longer (one that
- *   is counts as out of range, and so do offsets outside the rows; rows of such
- *   a sequence are not written).  out [q_rows, heads, head_dim] packed.  fp32
- *   scores, softmax and sums; the probabilities are rounded to the element type
- *   for the product with V.  Values of other sequences, and of keys that a row
- *   does not see, have no effect, infinities and NaN included.
+ *   is counts as out of range, and so do offsets outside the rows).  Rows of q of
+ *   such a sequence, or of none, are not written.  out [q_rows, heads, head_dim]
+ *   packed.  fp32 scores, softmax and sums; the probabilities are rounded to the
+ *   element type for the product with V.  Values of other sequences, and of keys
+ *   that a row does not see, have no effect, infinities and NaN included.
  *   scale > 0.  The workspace (counters) must be zero before its first call and
  *   is left zero, as moe_paged_attention's, which may be the same. */
 size_t moe_prompt_attention_workspace_size(void);

@@ -28,9 +28,10 @@
 //   * Pieces of a (sequence, KV head) are joined in the order of their keys:
 //     within a CTA through shared memory, between CTAs by the last of them to
 //     finish.  The sums' order depends on the shapes, the lengths and the GPU only.
-// Measured (32 / 8 heads of 128): 64 sequences of 576 fp16 28.4 us (151 MB, 5.3
-// TB/s), 64 of 2048 81 us (6.6 TB/s, what a plain copy reaches), four of about
-// 100000 bf16 268 us (6.5 TB/s); one of 72 3.8 us, a chain of latencies.
+// Measured in a graph (32 / 8 heads of 128): 64 sequences of about 576 fp16 29.3 us
+// (152 MB, 5.2 TB/s), 64 of 2048 82 us (6.5 TB/s, what a plain copy reaches), four of
+// about 100000 bf16 263 us (6.6 TB/s); one of 72 4.0 us, a chain of latencies.
+// Heads of 64: 64 of about 576 bf16 14.8 us (5.1 TB/s).
 #include "paged.cuh"
 
 namespace moe {
@@ -609,7 +610,7 @@ bool paged_attr() {
 // length at once; or cuts the line evenly.  The table's width is all that is known
 // of the lengths here, so a CTA's share must not become too long where few units
 // are long; and a CTA for a few chunks is a wave of latencies for each 2 to an SM.
-// Measured (fp16, 32 heads of 128, 8 KV heads, own CTAs / even cut, us):
+// Measured in a graph (fp16, 32 heads of 128, 8 KV heads, own CTAs / even cut, us):
 //   1 x 72 3.8 / 9.2, 8 x 576 7.1 / 10.9, 64 x 576 28.4 / 35.2, 64 x 2048 81 / 92,
 //   64 ragged up to 1972 46.9 / 54.7; but 1 x 1024 8.8 / 7.9, one of 2048 and 63 of
 //   16 19.5 / 9.4, one of 4096 and 63 of 16 35.7 / 14.3;
@@ -629,7 +630,10 @@ struct Shape {
 };
 Shape shape_of(int64_t seqs, int kv_heads, int group, int64_t max_tokens) {
   Shape s;
-  // Groups above 16 heads are read by several units, of equal numbers of heads.
+  // Groups above 16 heads are read by several units, of equal numbers of heads: 24 by
+  // two of 12, but a prime number by as many units of one head, each of which reads
+  // the keys (from L2 at best: 64 sequences of about 576, 1 KV head of 128, 17 heads
+  // 35.8 us, 16 heads 11.3).
   s.parts = static_cast<int>(ceil_div(group, 16));
   while (group % s.parts) ++s.parts;
   s.tile = group / s.parts;

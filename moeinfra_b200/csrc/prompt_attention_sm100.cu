@@ -32,11 +32,13 @@
 // S, P and O: with head_dim 128 a step takes 80 keys (2 x (80 + 40 + 128)),
 // with head_dim 64 96 keys (the softmax's registers hold no more).
 //
-// Measured, 32 / 8 heads of 128, causal: one prompt of 8192 fp16 450 us, bf16 434
-// (1.22 and 1.27 PFLOP/s, 75 and 77 % of the library's best product; the clock falls
-// to 1.5-1.75 GHz under the power limit), 64 prompts of 129..512 120 us (412 MB and 61
-// GFLOP: an item has 3 to 7 steps, and as much again to start and to drain), one of
-// 2048 38 us, one of 40 7 us.
+// Measured in a graph of ten calls, 32 / 8 heads of 128, causal: one prompt of 8192
+// bf16 499 us, fp16 513 (1.10 and 1.07 PFLOP/s, 79 and 77 % of what the library's best
+// product sustains: the clock falls to 1.5-1.75 GHz under the power limit), 64 prompts of
+// 129..512 120 us (412 MB and 61 GFLOP: an item has 3 to 7 steps, and as much again to
+// start and to drain; 142 us call after call, at the lower clock), one of 2048 36 us,
+// one of 40 7.4 us.  Heads of 64: 2 x 4096 bf16 203 us, fp16 231 (119 us of exponentials
+// alone), 64 prompts of 129..512 bf16 101.
 //
 // O is rescaled only when a row's maximum grew by more than 2^8 since the
 // reference in use (m is then that reference): probabilities stay below 2^8,
@@ -60,7 +62,7 @@ constexpr int kM = 128;         // rows of a tile
 constexpr int kSoftWarps = 8, kTmaWarp = 8, kMmaWarp = 9;
 constexpr int kThreads = 12 * 32;  // three warpgroups: registers are moved between them
 // Registers a thread: 12 warps x 168 at launch, of which the softmax warps
-// (a row of 128 scores each) take kSoftRegs and the others keep kOtherRegs.
+// (a row of 80 or 96 scores each) take kSoftRegs and the others keep kOtherRegs.
 constexpr int kSoftRegs = 200, kOtherRegs = 104;
 constexpr int kRegs = 2 * 128 * kSoftRegs + 128 * kOtherRegs;
 constexpr float kLazy = 8.f;    // log2 of what a row's maximum may grow before O is rescaled
@@ -185,9 +187,9 @@ __device__ __forceinline__ uint64_t exp2_fma(uint64_t x) {
   return mul2(p, pair(__uint_as_float(lo), __uint_as_float(hi)));
 }
 // Of 8 pairs, those that go through exp2_fma.  With heads of 128 the tensor cores
-// (and the power limit) bound a step and it only costs: 1 x 8192 causal fp16 450 us
-// with none, 454 with 1, 461 with 2, 495 with 4.  With heads of 64 a step has twice
-// the exponentials per product: 2 x 4096 fp16 215, 207, 210, 241 us.
+// (and the power limit) bound a step and it only costs: 1 x 8192 causal fp16, at the
+// full clock, 450 us with none, 454 with 1, 461 with 2, 495 with 4.  With heads of 64 a
+// step has twice the exponentials per product: 2 x 4096 fp16 215, 207, 210, 241 us.
 template <int HD>
 constexpr int kFmaOf8 = HD == 128 ? 0 : 1;
 
@@ -731,8 +733,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // To find an item's block, every CTA walks the blocks, 32 at a time, and
     // counts those with rows.  After some without any it looks for the next that has
     // (the stated maximum may be far above the lengths, or one sequence above the
-    // others: 1000 prompts of 1..64 stated as up to 131072 took 60 ms, 64 prompts of
-    // 129..512 1.1).
+    // others: 1000 prompts of 1..64, 16 heads of 64, stated as up to 131072, took 60 ms
+    // and take 0.09; 64 prompts of 129..512 1.08 and 0.12).
     const uint32_t groups = a.heads >> a.pack, blocks = (uint32_t)a.blocks * a.seqs;
     constexpr int kEmpty = 4;  // looks without a block before the next is searched for
     uint32_t n = 0, n_q = 0, at = 0, before = 0, live = 0;

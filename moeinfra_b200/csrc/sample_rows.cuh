@@ -15,7 +15,8 @@
 // Sums are exact integers: the order in which atomics add them does not matter.
 //
 // Bound by instruction issue.  256 x 131072 fp32 of mixed parameters: 127 us, 134
-// MB, which a plain copy's rate would read in 21 (greedy rows alone: 35).  What
+// MB, which a plain copy's rate would read in 21 (greedy rows alone: 35); 256 CTAs are
+// 1.73 waves, so 40 SMs have nothing to do in the second.  What
 // costs: the exponential of a correctly rounded quotient and its 40 bits, in each
 // of two passes (13 and 15 cycles an SM for 32 logits, at two thirds of the issue
 // slots).  64 x 32000 fp16: 30 us, as long as the slowest row's CTA, 8 of them its

@@ -21,8 +21,9 @@
 // Many rows, or short ones, take a CTA each (sample_rows.cuh).  Here a row is
 // spread over a cluster of CTAs whose threads hold it in registers, as integers of
 // the same order ("keys").  Such a call is a chain of reductions and bound by their
-// latency: 11.3 us for one row of 32000 fp16 logits (64 KB), of which a plain copy
-// would take 0.01; 26 for one of 131072 fp32.
+// latency: in a graph 8 to 18 us for one row of 32000 fp16 logits at top-p 0.95, by
+// whether few logits hold it (64 KB: a plain copy would take 0.01), 22 for one of
+// 131072 fp32.
 //   * A first pass adds each weight to the sums of 7 thresholds (21
 //     instructions a logit), 0.5 to 16 below the maximum in units of the
 //     temperature, where a language model's boundaries usually lie.  If then at
@@ -38,11 +39,12 @@
 //   * Exponentials are not kept: the first pass needs every logit's, what
 //     follows only those of the few between the bounds or kept.  That leaves 64
 //     registers a thread and two CTAs to an SM, one's barriers under the other's
-//     arithmetic.
+//     arithmetic (16 logits a thread do not quite fit them: some 250 bytes of a thread
+//     are spilled).
 //   * Between passes the CTAs exchange sums, which is most of a call: each
 //     stores its 8 into every CTA's shared memory with st.async, whose bytes
 //     complete an mbarrier there (a cluster barrier behind plain stores took 2000
-//     cycles, this a third: 13.3 -> 12.0 us for the one row).  Waits are bounded:
+//     cycles, this a third: the one row 13.3 -> 12.0 us).  Waits are bounded:
 //     on a timeout the error word is set and the CTA leaves, as then do the others
 //     (Exchange::leave).
 #include <cooperative_groups.h>
@@ -561,12 +563,15 @@ int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t s) {
   return MOE_OK;
 }
 
-// One CTA a row where rows are many or short.  Measured with mixed parameters
-// (cluster / one CTA, us): 1 x 16000 9.4 / 10.9, 2 x 16000 12.3 / 10.9, 16 x 16000
-// 25.9 / 19.6; 1 x 32000 11.4 / 18.4, 8 x 32000 23.7 / 27.3, 16 x 32000 28.0 / 28.1,
-// 40 x 32000 34.4 / 29.5; 16 x 65536 37.8 / 43.3, 24 x 65536 46.1 / 42.6; 32 x
-// 131072 66.7 / 78.0, 40 x 131072 80.5 / 77.6, 256 x 131072 406 / 127; 24 x 200000
-// 88.9 / 109, 40 x 200000 139 / 111.
+// One CTA a row where rows are many or short.  Measured with mixed parameters, fp16,
+// in a graph (cluster / one CTA, us): 1 x 16000 10.8 / 12.8, 2 x 16000 13.5 / 12.7,
+// 16 x 16000 25.9 / 19.4; 1 x 32000 12.4 / 20.4, 8 x 32000 22.1 / 27.2, 16 x 32000
+// 26.2 / 28.4, 24 x 32000 29.3 / 28.5, 40 x 32000 32.6 / 29.3; 16 x 65536 35.2 / 42.9,
+// 32 x 65536 44.3 / 42.8; 32 x 131072 58.9 / 74.4, 40 x 131072 68.6 / 74.4, 48 x 131072
+// 79.9 / 75.4; 24 x 200000 90.8 / 108, 40 x 200000 140 / 110.  Between 11 and 21 rows of
+// 32000, 22 and 30 of 65536 and 36 and 44 of 131072 the cluster is up to a fifth
+// faster than the one CTA chosen here: the rule is from before one warp waited for an
+// exchange.
 // In a cluster 8 logits a thread, and so more CTAs, as far as 8 CTAs go; then 16
 // (a cluster of up to 16 CTAs); 32 and one CTA to an SM for the longest rows.
 template <typename T>

@@ -871,7 +871,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ``cu_seqlens[b] .. cu_seqlens[b+1]`` (int32, on the device), none longer than ``max_seqlen``;
     its keys likewise by ``cu_seqlens_k`` / ``max_seqlen_k`` (default: the queries').  Causal: the
     queries are the last of their sequence's positions; one that sees no key gives zeros.  Returns
-    [rows, heads, head_dim].  ``workspace``: as for :func:`paged_attention`, of at least
+    [rows, heads, head_dim]; rows that belong to no sequence are not written.  ``workspace``: as for :func:`paged_attention`, of at least
     ``PROMPT_WORKSPACE_BYTES`` zeroed bytes (the same buffer may serve both).
     """
     what = "prompt_attention"
