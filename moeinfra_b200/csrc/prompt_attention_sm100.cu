@@ -97,7 +97,7 @@ struct PromptArgs {
   int blocks;                   // ceil(max_q / tokens of an item)
   bool causal;
   float scale_log2;
-  const uint16_t *q, *k, *v;    // for redo_row alone; strides in elements
+  const uint16_t *q, *k, *v;    // for redo_rows alone; strides in elements
   int64_t q_stride, q_head, k_stride, k_head, v_stride, v_head;
   uint16_t* out;                // [rows_q, heads, HD]
   uint32_t* counts;             // items claimed, CTAs done: zero between calls
@@ -218,56 +218,91 @@ __device__ __forceinline__ uint32_t trace_odd(uint32_t v, uint32_t acc) {
   return acc;
 }
 
-// One row by the formula, by one warp: 32 keys a step, one to a lane, then their
-// values, HD / 32 dims to a lane.  q, k, v: the row's query, the first key and value
-// that it sees.
+// kRedo rows of one KV head by the formula, by one warp: 32 keys a step, one to a
+// lane, then their values, HD / 32 dims to a lane.  q, out: the rows' queries and
+// places; k, v: the first key and value; seen: how many of them each row sees (0: no
+// row).  A warp's 32 rows over 8192 keys take 13 ms, over 131072 0.2 s, latency of
+// loads mostly: the other warps' waits end after 2 s.
+constexpr int kRedo = 4;
 template <typename T, int HD>
-__device__ __forceinline__ void redo_row(const uint16_t* q, const uint16_t* k, int64_t k_stride,
-                                         const uint16_t* v, int64_t v_stride, int seen,
-                                         float scale_log2, uint16_t* out) {
+__device__ __forceinline__ void redo_rows(const uint16_t* const (&q)[kRedo], const uint16_t* k,
+                                          int64_t k_stride, const uint16_t* v, int64_t v_stride,
+                                          const int (&seen)[kRedo], float scale_log2,
+                                          uint16_t* const (&out)[kRedo]) {
   constexpr int kWords = HD / 64;
   const int lane = threadIdx.x & 31;
-  float m = -INFINITY, l = 0.f;
-  float2 acc[kWords] = {};
-#pragma unroll 1
-  for (int j0 = 0; j0 < seen; j0 += 32) {
-    float s = -INFINITY;
-    if (j0 + lane < seen) {
-      const uint16_t* row = k + (j0 + lane) * k_stride;
-      s = 0.f;
-#pragma unroll 4
-      for (int d = 0; d < HD; d += 2) {
-        const float2 x = T::unpack(*reinterpret_cast<const uint32_t*>(q + d));
-        const float2 y = T::unpack(*reinterpret_cast<const uint32_t*>(row + d));
-        s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
-      }
-      s *= scale_log2;
-    }
-    float top = s;
+  float m[kRedo], l[kRedo];
+  float2 acc[kRedo][kWords] = {};
+  int most = 0;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float nm = fmaxf(m, top), f = m == nm ? 1.f : exp2_approx(m - nm);
-    m = nm;
-    const float p = j0 + lane < seen ? exp2_approx(s - (m == -INFINITY ? 0.f : m)) : 0.f;
-    l = l * f + warp_sum(p);
-#pragma unroll
-    for (int w = 0; w < kWords; ++w) acc[w] = make_float2(acc[w].x * f, acc[w].y * f);
-#pragma unroll 1
-    for (int i = 0; i < min(32, seen - j0); ++i) {
-      const float pi = __shfl_sync(0xffffffffu, p, i);
-#pragma unroll
-      for (int w = 0; w < kWords; ++w) {
-        const float2 x = T::unpack(
-            *reinterpret_cast<const uint32_t*>(v + (j0 + i) * v_stride + w * 64 + lane * 2));
-        acc[w] = make_float2(fmaf(pi, x.x, acc[w].x), fmaf(pi, x.y, acc[w].y));
-      }
-    }
-    if (l != l) break;  // and stays so
+  for (int r = 0; r < kRedo; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+    most = max(most, seen[r]);
   }
-  const float inv = 1.f / l;
+#pragma unroll 1
+  for (int j0 = 0; j0 < most; j0 += 32) {
+    const int j = j0 + lane;
+    float s[kRedo] = {};
+    const uint16_t* row = k + min(j, most - 1) * k_stride;
+#pragma unroll 4
+    for (int d = 0; d < HD; d += 8) {
+      const uint4 ks = *reinterpret_cast<const uint4*>(row + d);
+      const uint32_t kw[4] = {ks.x, ks.y, ks.z, ks.w};
 #pragma unroll
-  for (int w = 0; w < kWords; ++w)
-    *reinterpret_cast<uint32_t*>(out + w * 64 + lane * 2) = T::pack(acc[w].x * inv, acc[w].y * inv);
+      for (int r = 0; r < kRedo; ++r) {
+        const uint4 qs = *reinterpret_cast<const uint4*>(q[r] + d);
+        const uint32_t qw[4] = {qs.x, qs.y, qs.z, qs.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = T::unpack(qw[i]), y = T::unpack(kw[i]);
+          s[r] = fmaf(x.x, y.x, fmaf(x.y, y.y, s[r]));
+        }
+      }
+    }
+    bool nan = true;
+#pragma unroll
+    for (int r = 0; r < kRedo; ++r) {
+      s[r] = j < seen[r] ? s[r] * scale_log2 : -INFINITY;
+      float top = s[r];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float nm = fmaxf(m[r], top), f = m[r] == nm ? 1.f : exp2_approx(m[r] - nm);
+      m[r] = nm;
+      s[r] = exp2_approx(s[r] - (nm == -INFINITY ? 0.f : nm));
+      l[r] = l[r] * f + warp_sum(s[r]);
+      nan &= l[r] != l[r] || seen[r] == 0;
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) acc[r][w] = make_float2(acc[r][w].x * f, acc[r][w].y * f);
+    }
+    if (nan) break;  // and they stay so
+    const int n = min(32, most - j0);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      float2 x[kWords];
+#pragma unroll
+      for (int w = 0; w < kWords; ++w)
+        x[w] = T::unpack(
+            *reinterpret_cast<const uint32_t*>(v + (j0 + i) * v_stride + w * 64 + lane * 2));
+#pragma unroll
+      for (int r = 0; r < kRedo; ++r) {
+        const float p = __shfl_sync(0xffffffffu, s[r], i);
+        if (j0 + i >= seen[r]) continue;
+#pragma unroll
+        for (int w = 0; w < kWords; ++w)
+          acc[r][w] = make_float2(fmaf(p, x[w].x, acc[r][w].x), fmaf(p, x[w].y, acc[r][w].y));
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kRedo; ++r) {
+    if (seen[r] == 0) continue;
+    const float inv = 1.f / l[r];
+#pragma unroll
+    for (int w = 0; w < kWords; ++w)
+      *reinterpret_cast<uint32_t*>(out[r] + w * 64 + lane * 2) =
+          T::pack(acc[r][w].x * inv, acc[r][w].y * inv);
+  }
 }
 
 struct __align__(16) Item {
@@ -564,14 +599,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!__any_sync(0xffffffffu, met)) again = 0;
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the rows are written once more
         __syncwarp();
-        for (; again; again &= again - 1) {
-          const int r = __ffs(again) - 1;
-          const int64_t at = it.row_q + first + ((lane_row + r) >> a.pack);
-          const int head = it.h + (r & heads_mask);
-          redo_row<T, HD>(a.q + at * a.q_stride + head * a.q_head,
-                          a.k + keys.x * a.k_stride + kv_head * a.k_head, a.k_stride, v, a.v_stride,
-                          __shfl_sync(0xffffffffu, seen, r), a.scale_log2,
-                          a.out + (at * a.heads + head) * HD);
+        while (again) {
+          const uint16_t* qs[kRedo];
+          uint16_t* outs[kRedo];
+          int sees[kRedo];
+#pragma unroll
+          for (int i = 0; i < kRedo; ++i) {  // past the last: the first row, seeing nothing
+            const int r = again ? __ffs(again) - 1 : 0;
+            const int64_t at = it.row_q + first + ((lane_row + r) >> a.pack);
+            const int head = it.h + (r & heads_mask);
+            qs[i] = a.q + at * a.q_stride + head * a.q_head;
+            outs[i] = a.out + (at * a.heads + head) * HD;
+            sees[i] = __shfl_sync(0xffffffffu, again ? seen : 0, r);
+            again &= again - 1;
+          }
+          redo_rows<T, HD>(qs, a.k + keys.x * a.k_stride + kv_head * a.k_head, a.k_stride, v,
+                           a.v_stride, sees, a.scale_log2, outs);
         }
       }
       tc_fence_before();

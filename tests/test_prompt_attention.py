@@ -412,3 +412,25 @@ def test_a_stated_maximum_that_takes_long_to_walk():
     finally:
         _native.set_wait_limit_ns(old)
     assert torch.equal(got, want)
+
+
+@gpu
+def test_values_not_seen_of_a_long_prompt():
+    """Rows that are computed again over 20000 keys keep no wait of the other warps too long."""
+    from moeinfra_b200 import kernels
+
+    n, H, KV, hd = 20000, 16, 1, 128
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q = torch.randn(n, H, hd, device="cuda", generator=g).bfloat16()
+    kv = torch.randn(n, 2 * KV, hd, device="cuda", generator=g).bfloat16()
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    clean = kernels.prompt_attention(q, kv[:, :KV], kv[:, KV:], cu, n)
+    kv[n - 3, KV:, 7] = float("inf")
+    got = kernels.prompt_attention(q, kv[:, :KV], kv[:, KV:], cu, n)
+    kernels.check_device()
+    assert not got[n - 3:, :, 7].isfinite().any()
+    # The same row twice, its probabilities rounded to 16 bits or not: two roundings and theirs.
+    # sum_j p_j |v_j| <= max |v| < 6, a probability's rounding is 2^-8 of it at most.
+    got[n - 3:, :, 7] = clean[n - 3:, :, 7]
+    assert got.isfinite().all()
+    assert float((got.float() - clean.float()).abs().max()) <= 6 * 2 ** -8
