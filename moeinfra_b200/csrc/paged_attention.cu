@@ -28,10 +28,10 @@
 //   * Pieces of a (sequence, KV head) are joined in the order of their keys:
 //     within a CTA through shared memory, between CTAs by the last of them to
 //     finish.  The sums' order depends on the shapes, the lengths and the GPU only.
-// Measured in a graph (32 / 8 heads of 128): 64 sequences of about 576 fp16 29.3 us
-// (152 MB, 5.2 TB/s), 64 of 2048 82 us (6.5 TB/s, what a plain copy reaches), four of
-// about 100000 bf16 263 us (6.6 TB/s); one of 72 4.0 us, a chain of latencies.
-// Heads of 64: 64 of about 576 bf16 14.8 us (5.1 TB/s).
+// Measured in a graph with a workspace given (32 / 8 heads of 128): 64 sequences of
+// about 576 fp16 29.3 us (152 MB, 5.2 TB/s), 64 of 2048 82 us (6.5 TB/s, what a plain
+// copy reaches), four of about 100000 bf16 263 us (6.6 TB/s); one of 72 4.0 us, a chain
+// of latencies.  Heads of 64: 64 of about 576 bf16 14.8 us (5.1 TB/s).
 #include "paged.cuh"
 
 namespace moe {

@@ -32,8 +32,8 @@
 // S, P and O: with head_dim 128 a step takes 80 keys (2 x (80 + 40 + 128)),
 // with head_dim 64 96 keys (the softmax's registers hold no more).
 //
-// Measured in a graph of ten calls, 32 / 8 heads of 128, causal: one prompt of 8192
-// bf16 499 us, fp16 513 (1.10 and 1.07 PFLOP/s, 79 and 77 % of what the library's best
+// Measured in a graph of ten calls, 32 / 8 heads of 128, causal: one prompt of 8192,
+// either type, 500 to 515 us (1.07 to 1.10 PFLOP/s, 77 to 79 % of what the library's best
 // product sustains: the clock falls to 1.5-1.75 GHz under the power limit), 64 prompts of
 // 129..512 120 us (412 MB and 61 GFLOP: an item has 3 to 7 steps, and as much again to
 // start and to drain; 142 us call after call, at the lower clock), one of 2048 36 us,
