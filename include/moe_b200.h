@@ -573,6 +573,61 @@ typedef struct moe_sample_tokens_args {
 } moe_sample_tokens_args_t;
 int moe_sample_tokens(const moe_sample_tokens_args_t* args);
 
+/* ---------------------------------------------------------------------------
+ * Several continuations of a sequence over the paged cache: trees of drafted
+ * tokens (speculative decoding) and beams.  No counterpart in the reference.
+ *
+ * Where a call takes `layers`, kv describes layer 0 of [layers, num_pages, ...]
+ * arrays that are *_layer_stride elements apart (multiples of 8; any value with
+ * one layer), and the call applies to every layer.
+ */
+
+/* moe_fork_pages: row i of the block table becomes a copy of row parents[i]
+ *   (as it was before the call; -1: the row is emptied), lengths[i] that of the
+ *   parent (0), and the pages of its positions lengths[i] .. lengths[i] + room - 1
+ *   (as far as the table reaches) its own.  block_table int32 [seqs, max_pages]
+ *   (the call writes it; entries that name no page are negative), lengths and
+ *   parents int32 [seqs], refs int32 [num_pages]: how many entries name each page,
+ *   0: free, are updated in place; holders outside the table (a kept prefix) may be
+ *   counted in refs as well.  Page by page, row after row: a missing page is taken from
+ *   the free ones, the lowest number first (pages that the call itself frees among
+ *   them); one that others hold too is replaced by such a page, the filled
+ *   positions (those below lengths[i]) copied in every layer.  Without a free page the entry
+ *   is -1 and the device error word is set (MOE_ERR_PAGE), as for a parent, length or page
+ *   out of range.  seqs <= 8192.  The first 4096 bytes of the workspace must be
+ *   zero before its first call and are left zero. */
+typedef struct moe_fork_pages_args {
+  moe_kv_pages_t kv;
+  int64_t layers, k_layer_stride, v_layer_stride;
+  int32_t* lengths;
+  const int32_t* parents;
+  int32_t* refs;
+  int64_t room;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} moe_fork_pages_args_t;
+size_t moe_fork_pages_workspace_size(int64_t seqs);
+int moe_fork_pages(const moe_fork_pages_args_t* args);
+
+/* moe_keep_nodes: for every layer, the keys and values at position lengths[b] +
+ *   keep[b][j] of sequence b move to position lengths[b] + j, for the entries of
+ *   keep[b] (int32 [seqs, most], rows keep_stride apart) up to its first negative one;
+ *   new_lengths[b] = lengths[b] + their number.  The entries must rise; a list that
+ *   does not, or whose positions have no page, ends before that entry and sets the device
+ *   error word (MOE_ERR_PAGE).  lengths[b] < 0: not a sequence, returned as it is.
+ *   The pages written to must not be another sequence's too. */
+typedef struct moe_keep_nodes_args {
+  moe_kv_pages_t kv;
+  int64_t layers, k_layer_stride, v_layer_stride;
+  const int32_t* lengths;
+  const int32_t* keep;
+  int64_t keep_stride, most;
+  int32_t* new_lengths;
+  void* stream;
+} moe_keep_nodes_args_t;
+int moe_keep_nodes(const moe_keep_nodes_args_t* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -37,6 +37,8 @@ ROPE_APPEND = struct.Struct("@" + _KV_PAGES + "PqPPqPPqqPPP")
 PAGED_ATTENTION = struct.Struct("@" + _KV_PAGES + "PqqPdPPqP")
 PROMPT_ATTENTION = struct.Struct("@PqqqPqqPqqqPPqqqqqqqqdPPqP")
 SAMPLE_TOKENS = struct.Struct("@PqqqqPPPPPPPP")
+FORK_PAGES = struct.Struct("@" + _KV_PAGES + "qqqPPPqPqP")
+KEEP_NODES = struct.Struct("@" + _KV_PAGES + "qqqPPqqPP")
 
 # name -> (restype, argtypes); mirrors include/moe_b200.h one to one.
 SIGNATURES: dict[str, tuple] = {
@@ -108,6 +110,9 @@ SIGNATURES: dict[str, tuple] = {
     "moe_prompt_attention_workspace_size": (c_size_t, []),
     "moe_prompt_attention": (c_int, [c_void_p]),
     "moe_sample_tokens": (c_int, [c_void_p]),
+    "moe_fork_pages_workspace_size": (c_size_t, [c_int64]),
+    "moe_fork_pages": (c_int, [c_void_p]),
+    "moe_keep_nodes": (c_int, [c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

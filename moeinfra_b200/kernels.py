@@ -972,3 +972,109 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: tor
     if status:
         check(status, "moe_sample_tokens")
     return tokens, probs
+
+
+# ---------------------------------------------------------------------------
+# Several continuations of a sequence over the paged cache: trees of drafted tokens, beams
+# ---------------------------------------------------------------------------
+
+
+def _check_layers(what: str, k_pages, v_pages, block_table) -> tuple:
+    """``(layers, k layer stride, v layer stride, first layer of each)`` of caches of one layer
+    [pages, ...] or of all [layers, pages, ...], checked."""
+    if not isinstance(k_pages, torch.Tensor) or k_pages.ndim not in (4, 5):
+        raise ValueError(f"{what}: k_pages must be [pages, kv_heads, page_size, head_dim], or that "
+                         "per layer")
+    if k_pages.ndim == 4:
+        _check_cache(what, k_pages, v_pages, block_table)
+        return 1, 0, 0, k_pages, v_pages
+    if not isinstance(v_pages, torch.Tensor) or v_pages.shape != k_pages.shape or not len(k_pages):
+        raise ValueError(f"{what}: v_pages must have k_pages' shape, of one layer at least")
+    k, v = k_pages[0], v_pages[0]
+    _check_cache(what, k, v, block_table)
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if t.shape[0] > 1 and t.stride(0) < (t.shape[1] - 1) * t.stride(1) + k[0:1].numel():
+            raise ValueError(f"{what}: {name}'s layers overlap")
+    return k_pages.shape[0], k_pages.stride(0), v_pages.stride(0), k, v
+
+
+@_on_first_device
+def fork_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+               lengths: torch.Tensor, parents: torch.Tensor, refs: torch.Tensor, room: int = 1,
+               workspace: torch.Tensor | None = None) -> None:
+    """Fork, end and grow the sequences of a paged cache, in place.
+
+    Row i of ``block_table`` int32 [sequences, max_pages] becomes a copy of row ``parents[i]``
+    (int32; i itself: it stays, -1: it ends and its pages are freed), ``lengths[i]`` int32 its
+    parent's.  Then the pages of its next ``room`` positions become its own: a missing one is taken
+    from the free pages, the lowest number first, and one that others list too is replaced by such a
+    page with the filled positions copied, in every layer.  ``k_pages`` / ``v_pages``: as in
+    :func:`rope_append`, or of all layers, [layers, pages, ...].  ``refs`` int32 [pages]: how many
+    entries of the table name each page (0: free), kept up to date; a holder elsewhere (a prefix kept
+    for later) adds one to keep its page from being written or freed.  Entries without a page are
+    negative.  When no page is free the entry is -1, which shows in :func:`check_device`, as do
+    parents, lengths and pages out of range.
+
+    ``workspace``: :func:`fork_pages_workspace`, as for :func:`paged_attention`.
+    """
+    what = "fork_pages"
+    layers, k_layer, v_layer, k, v = _check_layers(what, k_pages, v_pages, block_table)
+    n_pages, kv, page, hd = k.shape
+    dev = k.get_device()
+    seqs, max_pages = block_table.shape
+    _serve_check(what, dev, ("lengths", lengths, torch.int32, (seqs,), 1),
+                 ("parents", parents, torch.int32, (seqs,), 1),
+                 ("refs", refs, torch.int32, (n_pages,), 1))
+    if seqs > 1 and block_table.stride(0) < max_pages:
+        raise ValueError(f"{what}: block_table's rows overlap")
+    stream = _raw_stream(dev)
+    nbytes = _native.lib().moe_fork_pages_workspace_size(seqs)
+    if workspace is None:
+        workspace = _serve_scratch(dev, stream, nbytes)
+    else:
+        _check_workspace(what, workspace, dev, nbytes)
+    status = _native.lib().moe_fork_pages(_native.FORK_PAGES.pack(
+        k.data_ptr(), v.data_ptr(), _outer_stride(k), _outer_stride(v), n_pages, kv, page, hd,
+        _DTYPE_CODES[k.dtype], block_table.data_ptr(), max(_outer_stride(block_table), max_pages),
+        seqs, max_pages, layers, k_layer, v_layer, lengths.data_ptr(), parents.data_ptr(),
+        refs.data_ptr(), room, workspace.data_ptr(), nbytes, stream))
+    if status:
+        check(status, "moe_fork_pages")
+
+
+@_on_first_device
+def fork_pages_workspace(block_table: torch.Tensor) -> torch.Tensor:
+    """A workspace for :func:`fork_pages` calls on tables of as many rows."""
+    nbytes = _native.lib().moe_fork_pages_workspace_size(block_table.shape[0])
+    return torch.zeros(nbytes, dtype=torch.uint8, device=block_table.device)
+
+
+@_on_first_device
+def keep_nodes(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+               lengths: torch.Tensor, keep: torch.Tensor) -> torch.Tensor:
+    """Move the accepted nodes of drafted trees to the end of their sequences; the new lengths.
+
+    ``keep`` int32 [sequences, any number]: the accepted nodes' indices, rising, up to the first
+    negative entry (rows may be strided).  In every layer the keys and values of position
+    ``lengths[b] + keep[b, j]`` move to ``lengths[b] + j``; the cache as in :func:`fork_pages`.
+    Returns ``lengths`` plus the kept nodes' number, int32 [sequences]; ``lengths[b] < 0`` is no
+    sequence and stays.  A list that falls or has no pages ends there and shows in
+    :func:`check_device`.  The pages moved in must be the sequence's own (:func:`fork_pages`).
+    """
+    what = "keep_nodes"
+    layers, k_layer, v_layer, k, v = _check_layers(what, k_pages, v_pages, block_table)
+    n_pages, kv, page, hd = k.shape
+    dev = k.get_device()
+    seqs, max_pages = block_table.shape
+    _serve_check(what, dev, ("lengths", lengths, torch.int32, (seqs,), 1),
+                 ("keep", keep, torch.int32, (seqs, None), 1))
+    out = lengths.new_empty(seqs)
+    status = _native.lib().moe_keep_nodes(_native.KEEP_NODES.pack(
+        k.data_ptr(), v.data_ptr(), _outer_stride(k), _outer_stride(v), n_pages, kv, page, hd,
+        _DTYPE_CODES[k.dtype], block_table.data_ptr(), _outer_stride(block_table) if seqs else max_pages,
+        seqs, max_pages, layers, k_layer, v_layer, lengths.data_ptr(), keep.data_ptr(),
+        _outer_stride(keep) if seqs else keep.shape[1], keep.shape[1], out.data_ptr(),
+        _raw_stream(dev)))
+    if status:
+        check(status, "moe_keep_nodes")
+    return out
