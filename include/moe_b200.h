@@ -628,6 +628,32 @@ typedef struct moe_keep_nodes_args {
 } moe_keep_nodes_args_t;
 int moe_keep_nodes(const moe_keep_nodes_args_t* args);
 
+/* moe_beam_select: the `count` best continuations of each group of beams.  logits
+ *   [groups * beams, vocab] (fp16, bf16 or fp32, rows stride elements apart, 0: one
+ *   row for all), scores fp32 [groups, beams].  With m a row's maximum, token t of beam k
+ *   scores scores[k] + ((x_t - m) - ln sum_u exp(x_u - m)), each step in fp32 (x_t - m is
+ *   0 where x_t == m; NaN logits count as -inf).  out_scores fp32, out_parents int32 (the beam
+ *   in its group) and out_tokens int64 [groups, count]: larger scores first, equal ones by
+ *   rising beam, in a beam by falling logit, then rising token.  What scores
+ *   -inf (or NaN) is no candidate; places without one are (-inf, 0, 0).  beams
+ *   and count <= 64, vocab <= 2^20.  The first 4096 bytes of the workspace must be
+ *   zero before its first call and are left zero. */
+typedef struct moe_beam_select_args {
+  const void* logits;
+  int64_t stride, groups, beams, vocab, dtype;
+  const float* scores;
+  int64_t count;
+  float* out_scores;
+  int32_t* out_parents;
+  int64_t* out_tokens;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} moe_beam_select_args_t;
+size_t moe_beam_select_workspace_size(int64_t groups, int64_t beams, int64_t vocab, int64_t count,
+                                      int64_t dtype);
+int moe_beam_select(const moe_beam_select_args_t* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -38,6 +38,7 @@ PAGED_ATTENTION = struct.Struct("@" + _KV_PAGES + "PqqPdPPqP")
 PROMPT_ATTENTION = struct.Struct("@PqqqPqqPqqqPPqqqqqqqqdPPqP")
 SAMPLE_TOKENS = struct.Struct("@PqqqqPPPPPPPP")
 FORK_PAGES = struct.Struct("@" + _KV_PAGES + "qqqPPPqPqP")
+BEAM_SELECT = struct.Struct("@PqqqqqPqPPPPqP")
 KEEP_NODES = struct.Struct("@" + _KV_PAGES + "qqqPPqqPP")
 
 # name -> (restype, argtypes); mirrors include/moe_b200.h one to one.
@@ -113,6 +114,8 @@ SIGNATURES: dict[str, tuple] = {
     "moe_fork_pages_workspace_size": (c_size_t, [c_int64]),
     "moe_fork_pages": (c_int, [c_void_p]),
     "moe_keep_nodes": (c_int, [c_void_p]),
+    "moe_beam_select_workspace_size": (c_size_t, [c_int64] * 5),
+    "moe_beam_select": (c_int, [c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

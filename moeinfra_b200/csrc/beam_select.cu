@@ -1,0 +1,492 @@
+// Beam search's choice: the best continuations over beams and vocabulary.
+//
+// For beam k of a group with logits x and running score s_k, token t scores
+//   v[k,t] = s_k + ((x_t - m) - ln sum_u exp(x_u - m)),   m = max_u x_u
+// and the `count` largest of the group's beams x vocabulary are returned, larger
+// scores first, then lower beams, in a beam larger logits, then lower tokens.  In a
+// beam v follows x, so the order in it needs no sum: one pass over the logits
+// finds each row's maximum, sum and `count` largest, and the group's are chosen
+// among those.
+//
+// Bound by memory: every logit is read once.  A row is cut into `splits` CTAs
+// where there are few rows.  A CTA goes through its part in chunks of 4 vectors of
+// 16 bytes a thread, the next chunk's loads in flight:
+//   * each thread keeps a running maximum and the sum of exponentials
+//     below it (8 terms in fp32, those sums in fp64: 2 % of the arithmetic, and
+//     beams' scores can be compared to the last bit of their rounding);
+//   * logits above a threshold go to a list in shared memory.  The threshold is
+//     such that `count` logits are known to reach it: in the first chunk it comes
+//     from the threads' own maxima, of which the warps' largest few are taken.
+//     Later chunks put in about `count` logits each, and one comparison per
+//     vector skips the others.  A chunk with more than the list takes (equal
+//     logits, mostly) is searched round by round instead.
+// The last CTA of a group joins the lists of its rows.
+#include "sample.cuh"
+
+namespace moe {
+namespace {
+
+MOE_DEFINE_ERROR_WORD()
+
+constexpr int kMostBeams = 64, kMostCount = 64;
+constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
+constexpr int kVecs = 4;            // 16-byte vectors of a thread in a chunk
+constexpr int kList = 2048;         // entries of the list
+constexpr int kRank = 384;          // entries that are put in order by counting
+constexpr int kGroups = 1000;       // counters of a launch (the workspace's first 4096 bytes)
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct BeamArgs {
+  const void* logits;
+  int64_t stride;
+  int vocab, beams, count, splits;
+  const float* scores;              // [groups, beams]
+  float* out_scores;                // [groups, count]
+  int32_t* out_parents;
+  int64_t* out_tokens;
+  uint32_t* done;                   // [groups]: CTAs done, zero between calls
+  double2* sums;                    // [rows, splits]: sum, maximum
+  uint64_t* keys;                   // [rows, splits, count]: falling, 0: none
+};
+
+template <typename T>
+struct Vec {
+  static constexpr int kN = 8;
+  static constexpr uint32_t kNone = T::kBf16 ? 0xFF80u : 0xFC00u;  // -inf
+  static __device__ __forceinline__ void unpack(const uint4& r, float (&f)[kN]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = T::unpack(w[i]);
+      f[2 * i] = x.x;
+      f[2 * i + 1] = x.y;
+    }
+  }
+  // Elements outside [lo, hi) become -inf.
+  static __device__ __forceinline__ void cut(uint4& r, int64_t lo, int64_t hi) {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < lo || i >= hi)
+        w[i / 2] = i & 1 ? (w[i / 2] & 0xFFFFu) | kNone << 16 : (w[i / 2] & 0xFFFF0000u) | kNone;
+    r = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <>
+struct Vec<float> {
+  static constexpr int kN = 4;
+  static __device__ __forceinline__ void unpack(const uint4& r, float (&f)[kN]) {
+    f[0] = __uint_as_float(r.x);
+    f[1] = __uint_as_float(r.y);
+    f[2] = __uint_as_float(r.z);
+    f[3] = __uint_as_float(r.w);
+  }
+  static __device__ __forceinline__ void cut(uint4& r, int64_t lo, int64_t hi) {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < lo || i >= hi) w[i] = 0xFF800000u;
+    r = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// A logit and its token as one key: larger logits are larger, of equal ones lower
+// tokens.  0 stands for none; -inf and NaN never become keys.
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t token) {
+  return (uint64_t)Logit<float>::key(x) << 32 | (0xFFFFFFFFu - token);
+}
+__device__ __forceinline__ float logit_of(uint64_t key) {
+  return Logit<float>::value((uint32_t)(key >> 32));
+}
+
+struct Pick {  // a continuation's place in the group's order
+  uint64_t hi, lo;  // score and beam; logit and token
+  __device__ __forceinline__ bool above(const Pick& o) const {
+    return hi != o.hi ? hi > o.hi : lo > o.lo;
+  }
+};
+__device__ __forceinline__ Pick warp_best(Pick p) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const Pick q{__shfl_xor_sync(kAll, p.hi, o), __shfl_xor_sync(kAll, p.lo, o)};
+    if (q.above(p)) p = q;
+  }
+  return p;
+}
+// The block's largest, in every thread.
+__device__ __forceinline__ Pick block_best(Pick p, Pick* s_warp) {
+  p = warp_best(p);
+  if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x / 32] = p;
+  __syncthreads();
+  p = warp_best(s_warp[threadIdx.x % kBeamWarps]);
+  __syncthreads();
+  return p;
+}
+// A key that at least `count` of the threads' keys reach, or 0 where no warp is full: the
+// smallest of the full warps' ceil(count / full warps)-th largest.  Keys 0 do not count.
+__device__ __forceinline__ uint32_t reached_by(uint32_t key, int count, uint32_t* s_warp) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  if (lane == 0) s_warp[warp] = 0;
+  const bool full = __all_sync(kAll, key != 0);
+  const int warps = __syncthreads_count(full) / 32;
+  if (warps == 0) return 0;
+  const int each = (count + warps - 1) / warps;
+  if (full) {
+    uint32_t top = 0;
+    for (int i = 0; i < each; ++i) {
+      top = __reduce_max_sync(kAll, key);
+      const uint32_t who = __ballot_sync(kAll, key == top);
+      if (lane == __ffs(who) - 1) key = 0;
+    }
+    if (lane == 0) s_warp[warp] = top;
+  }
+  __syncthreads();
+  uint32_t low = 0xFFFFFFFFu;  // warps that are not full have left 0
+  for (int w = 0; w < kBeamWarps; ++w) low = min(low, s_warp[w] - 1u);
+  __syncthreads();
+  return each > 32 ? 0 : low + 1;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kBeamThreads, 3) k_beam_select(const BeamArgs a) {
+  constexpr int kN = Vec<T>::kN;
+  constexpr int kChunk = kBeamThreads * kVecs;  // vectors
+  __shared__ __align__(16) uint64_t s_list[kList];
+  __shared__ Pick s_best[kBeamWarps];
+  __shared__ uint64_t s_top[kMostCount];
+  __shared__ uint32_t s_warp[kBeamWarps];
+  __shared__ double s_sum[kBeamWarps];
+  __shared__ float s_max[kBeamWarps], s_rowmax[kMostBeams], s_rowsum[kMostBeams];
+  __shared__ int s_count, s_last;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, M = a.count;
+  const int row = blockIdx.x / (uint32_t)a.splits, split = blockIdx.x - row * a.splits;
+  using Raw = typename Logit<T>::Raw;
+  const Raw* x0 = static_cast<const Raw*>(a.logits) + row * a.stride;
+  // Vectors start at 16-byte boundaries: `skew` elements of the first are not the row's.
+  const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(Raw));
+  const uint4* vecs = reinterpret_cast<const uint4*>(x0 - skew);
+  const int total = (skew + a.vocab + kN - 1) / kN, share = (total + a.splits - 1) / a.splits;
+  const int lo = split * share, hi = min(total, lo + share);
+  if (tid == 0) s_count = 0;
+  pdl_trigger();
+  pdl_wait();
+
+  auto fetch = [&](int first, uint4 (&r)[kVecs]) {
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int v = first + u * kBeamThreads + tid;
+      r[u] = make_uint4(0, 0, 0, 0);
+      if (v < hi) r[u] = __ldcs(vecs + v);
+    }
+  };
+  float m = -INFINITY, thr = -INFINITY;
+  double sum = 0;
+  uint4 next[kVecs];
+  fetch(lo, next);
+  int had = 0;  // entries of the list before the chunk
+  for (int c = lo; c < hi; c += kChunk) {
+    uint4 r[kVecs];
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) r[u] = next[u];
+    if (c + kChunk < hi) fetch(c + kChunk, next);
+    float top[kVecs], mine = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      const int v = c + u * kBeamThreads + tid;
+      top[u] = -INFINITY;
+      if (v >= hi) continue;
+      const int64_t at = (int64_t)v * kN - skew;  // the token of its first element
+      if (at < 0 || at + kN > a.vocab) Vec<T>::cut(r[u], -at, a.vocab - at);
+      float f[kN];
+      Vec<T>::unpack(r[u], f);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) top[u] = fmaxf(top[u], f[i]);  // NaN: the other
+      mine = fmaxf(mine, top[u]);
+      if (top[u] > m) {
+        sum = m == -INFINITY ? 0 : sum * exp2_approx((m - top[u]) * kLog2e);
+        m = top[u];
+      }
+      if (top[u] == -INFINITY) continue;
+      float e[kN];
+      if (m == INFINITY) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) e[i] = f[i] == INFINITY ? 1.f : 0.f;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kN; i += 2) {
+          const uint64_t d = mul2(add2(pair(f[i], f[i + 1]), pair(-m, -m)), pair(kLog2e, kLog2e));
+          e[i] = exp2_approx(fmaxf(lo_of(d), -200.f));  // 0 for -inf and NaN
+          e[i + 1] = exp2_approx(fmaxf(hi_of(d), -200.f));
+        }
+      }
+#pragma unroll
+      for (int w = kN / 2; w; w /= 2)
+#pragma unroll
+        for (int i = 0; i < w; ++i) e[i] += e[i + w];
+      sum += e[0];
+    }
+    // Which logits are put into the list: those above thr, of which `count` are known to
+    // reach it in earlier chunks, or (level) those that reach it.
+    const int busy = __syncthreads_count(mine > thr);
+    if (busy == 0) continue;
+    bool level = false;
+    if (thr == -INFINITY || busy > 2 * M + 32) {
+      const uint32_t k = reached_by(mine == -INFINITY ? 0 : Logit<float>::key(mine), M, s_warp);
+      const float t = k ? Logit<float>::value(k) : -INFINITY;
+      if (t > thr) {
+        thr = t;
+        level = true;
+      }
+    }
+    auto token_of = [&](int u, int i) {
+      return static_cast<uint32_t>((c + u * kBeamThreads + tid) * kN - skew + i);
+    };
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+      if (!(level ? top[u] >= thr : top[u] > thr)) continue;
+      float f[kN];
+      Vec<T>::unpack(r[u], f);
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+        if (level ? f[i] >= thr : f[i] > thr) {
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kList) s_list[at] = key_of(f[i], token_of(u, i));
+        }
+    }
+    __syncthreads();
+    int n = s_count;
+    if (n <= kRank) {
+      had = n;
+      continue;
+    }
+    // Too many: the `count` best so far, round by round, of the list or (where it
+    // overflowed) of the list before and this chunk.
+    const bool over = n > kList;
+    if (over) n = had;
+    uint64_t last = ~0ull;
+    int found = 0;
+    for (; found < M; ++found) {
+      uint64_t best = 0;
+      for (int i = tid; i < n; i += kBeamThreads)
+        if (s_list[i] < last && s_list[i] > best) best = s_list[i];
+      if (over) {
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+          if (!(top[u] >= thr)) continue;
+          float f[kN];
+          Vec<T>::unpack(r[u], f);
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            const uint64_t k = f[i] > -INFINITY ? key_of(f[i], token_of(u, i)) : 0;
+            if (k < last && k > best) best = k;
+          }
+        }
+      }
+      last = block_best(Pick{best, 0}, s_best).hi;
+      if (last == 0) break;
+      if (tid == 0) s_top[found] = last;
+    }
+    __syncthreads();
+    if (tid < found) s_list[tid] = s_top[tid];
+    if (tid == 0) s_count = found;
+    had = found;
+    if (found == M) thr = logit_of(s_top[M - 1]);
+    __syncthreads();
+  }
+
+  // This part's maximum and sum, and its list in order.
+  {
+    float top = m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+    if (lane == 0) s_max[warp] = top;
+    __syncthreads();
+    top = s_max[lane % kBeamWarps];
+#pragma unroll
+    for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+    sum = m == -INFINITY || (m != top && top == INFINITY) ? 0 : m == top ? sum : sum * expf(m - top);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+    if (lane == 0) s_sum[warp] = sum;
+    const int n = s_count, part = row * a.splits + split;
+    uint64_t* keys = a.keys + (int64_t)part * M;
+    for (int i = tid; i < n; i += kBeamThreads) {
+      const uint64_t k = s_list[i];
+      int above = 0;
+      for (int j = 0; j < n; ++j) above += s_list[j] > k;
+      if (above < M) keys[above] = k;
+    }
+    for (int i = n + tid; i < M; i += kBeamThreads) keys[i] = 0;
+    __syncthreads();
+    if (tid == 0) {
+      double all = 0;
+      for (int w = 0; w < kBeamWarps; ++w) all += s_sum[w];
+      a.sums[part] = make_double2(all, top);
+    }
+  }
+  // The last CTA of the group goes on.
+  const int group = row / a.beams, parts = a.beams * a.splits;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) s_last = atomicAdd(a.done + group, 1) == parts - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  if (tid == 0) a.done[group] = 0;
+  const double2* sums = a.sums + (int64_t)group * parts;
+  if (tid < a.beams) {
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, (float)__ldcg(&sums[tid * a.splits + s].y));
+    double all = 0;
+    for (int s = 0; s < a.splits; ++s) {
+      const float of = (float)__ldcg(&sums[tid * a.splits + s].y);
+      const double part = __ldcg(&sums[tid * a.splits + s].x);
+      all += of == top ? part : part == 0 ? 0 : part * expf(of - top);
+    }
+    s_rowmax[tid] = top;
+    s_rowsum[tid] = (float)log(all);
+  }
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  const uint64_t* keys = a.keys + (int64_t)group * parts * M;
+  const float* scores = a.scores + (int64_t)group * a.beams;
+  const int all = parts * M, per_beam = a.splits * M;
+  auto score_of = [&](float x, int beam) {
+    const float top = s_rowmax[beam], d = x == top ? 0.f : x - top;
+    return __fadd_rn(scores[beam], __fsub_rn(d, s_rowsum[beam]));
+  };
+  auto pick = [&](int i) {
+    const uint64_t k = __ldcg(keys + i);
+    if (k == 0) return Pick{0, 0};
+    const int beam = i / per_beam;
+    const float v = score_of(logit_of(k), beam);
+    if (!(v > -INFINITY)) return Pick{0, 0};
+    return Pick{(uint64_t)Logit<float>::key(v) << 32 | (0xFFFFFFFFu - beam), k};
+  };
+  uint32_t limit = 0;  // scores below it are not among the best
+  if (all > kRank) {
+    uint32_t mine = 0;
+    for (int i = tid; i < all; i += kBeamThreads) mine = max(mine, (uint32_t)(pick(i).hi >> 32));
+    limit = reached_by(mine, M, s_warp);
+  }
+  Pick* list = reinterpret_cast<Pick*>(s_list);
+  for (int i = tid; i < all; i += kBeamThreads) {
+    const Pick p = pick(i);
+    if (p.hi == 0 || (uint32_t)(p.hi >> 32) < limit) continue;
+    const int at = atomicAdd(&s_count, 1);
+    if (at < kRank) list[at] = p;
+  }
+  __syncthreads();
+  const int n = s_count;
+  auto put = [&](int at, const Pick& p) {
+    const int beam = static_cast<int>(0xFFFFFFFFu - (uint32_t)p.hi);
+    const int64_t o = (int64_t)group * M + at;
+    a.out_scores[o] = p.hi ? score_of(logit_of(p.lo), beam) : -INFINITY;
+    a.out_parents[o] = p.hi ? beam : 0;
+    a.out_tokens[o] = p.hi ? 0xFFFFFFFFu - (uint32_t)p.lo : 0;
+  };
+  if (n <= kRank) {
+    for (int i = tid; i < n; i += kBeamThreads) {
+      const Pick p = list[i];
+      int above = 0;
+      for (int j = 0; j < n; ++j) above += list[j].above(p);
+      if (above < M) put(above, p);
+    }
+    for (int i = n + tid; i < M; i += kBeamThreads) put(i, Pick{0, 0});
+    return;
+  }
+  Pick last{~0ull, ~0ull};
+  for (int at = 0; at < M; ++at) {
+    Pick best{0, 0};
+    for (int i = tid; i < all && last.hi; i += kBeamThreads) {
+      const Pick p = pick(i);
+      if (last.above(p) && p.above(best)) best = p;
+    }
+    last = block_best(best, s_best);
+    if (tid == 0) put(at, last);
+  }
+}
+
+int splits_of(int64_t rows, int64_t vocab, int64_t vec) {
+  // Three CTAs an SM, each with a vector a thread at least.
+  const int64_t want = 3 * sm_count() / (rows > 0 ? rows : 1), most = ceil_div(vocab, vec * kBeamThreads);
+  const int64_t s = want < most ? want : most;
+  return static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+template <typename T>
+int launch_beams(BeamArgs a, int64_t groups, cudaStream_t s) {
+  using Raw = typename Logit<T>::Raw;
+  for (int64_t g = 0; g < groups; g += kGroups) {
+    const int64_t n = groups - g < kGroups ? groups - g : kGroups, parts = (int64_t)a.beams * a.splits;
+    BeamArgs b = a;
+    b.logits = static_cast<const Raw*>(a.logits) + g * a.beams * a.stride;
+    b.scores += g * a.beams;
+    b.out_scores += g * a.count;
+    b.out_parents += g * a.count;
+    b.out_tokens += g * a.count;
+    b.sums += g * parts;
+    b.keys += g * parts * a.count;
+    if (launch_pdl(k_beam_select<T>, dim3(static_cast<unsigned>(n * parts)), dim3(kBeamThreads), 0, s,
+                   b) != cudaSuccess)
+      return MOE_ERR_CUDA;
+    MOE_CHECK_LAUNCH();
+  }
+  return MOE_OK;
+}
+
+constexpr int64_t kSumsAt = 4096;  // behind the counters that every call leaves zero
+
+}  // namespace
+}  // namespace moe
+
+extern "C" size_t moe_beam_select_workspace_size(int64_t groups, int64_t beams, int64_t vocab,
+                                                 int64_t count, int64_t dtype) {
+  using namespace moe;
+  if (groups < 0 || beams < 1 || beams > kMostBeams || count < 1 || count > kMostCount || vocab < 1 ||
+      groups > INT32_MAX / beams)
+    return 0;
+  const int64_t rows = groups * beams;
+  return kSumsAt + rows * splits_of(rows, vocab, dtype == MOE_DTYPE_F32 ? 4 : 8) * (16 + 8 * count);
+}
+
+extern "C" int moe_beam_select(const moe_beam_select_args_t* args) {
+  using namespace moe;
+  if (!args) return MOE_ERR_INVALID_ARG;
+  const moe_beam_select_args_t& c = *args;
+  if (c.groups < 0 || c.beams < 1 || c.vocab < 1 || c.count < 1 || c.stride < 0 ||
+      (c.stride > 0 && c.stride < c.vocab && c.groups * c.beams > 1))
+    return MOE_ERR_INVALID_ARG;
+  if (c.beams > kMostBeams || c.count > kMostCount || c.vocab > (1 << 20) ||
+      c.groups > INT32_MAX / (kMostBeams * 64) ||
+      (c.dtype != MOE_DTYPE_F16 && c.dtype != MOE_DTYPE_BF16 && c.dtype != MOE_DTYPE_F32))
+    return MOE_ERR_UNSUPPORTED;
+  if (c.groups == 0) return MOE_OK;
+  if (!c.logits || !c.scores || !c.out_scores || !c.out_parents || !c.out_tokens)
+    return MOE_ERR_INVALID_ARG;
+  const int64_t size = c.dtype == MOE_DTYPE_F32 ? 4 : 2, rows = c.groups * c.beams;
+  if (reinterpret_cast<uintptr_t>(c.logits) % size) return MOE_ERR_ALIGNMENT;
+  if (!c.workspace || c.workspace_bytes < (int64_t)moe_beam_select_workspace_size(
+                                              c.groups, c.beams, c.vocab, c.count, c.dtype))
+    return MOE_ERR_WORKSPACE;
+  if (!aligned16(c.workspace)) return MOE_ERR_ALIGNMENT;
+  BeamArgs a{};
+  a.logits = c.logits;
+  a.stride = c.stride;
+  a.vocab = static_cast<int>(c.vocab);
+  a.beams = static_cast<int>(c.beams);
+  a.count = static_cast<int>(c.count);
+  a.splits = splits_of(rows, c.vocab, 16 / size);
+  a.scores = c.scores;
+  a.out_scores = c.out_scores;
+  a.out_parents = c.out_parents;
+  a.out_tokens = c.out_tokens;
+  a.done = static_cast<uint32_t*>(c.workspace);
+  char* ws = static_cast<char*>(c.workspace) + kSumsAt;
+  a.sums = reinterpret_cast<double2*>(ws);
+  a.keys = reinterpret_cast<uint64_t*>(ws + rows * a.splits * 16);
+  cudaStream_t s = static_cast<cudaStream_t>(c.stream);
+  if (c.dtype == MOE_DTYPE_F32) return launch_beams<float>(a, c.groups, s);
+  return c.dtype == MOE_DTYPE_BF16 ? launch_beams<BF16>(a, c.groups, s)
+                                   : launch_beams<F16>(a, c.groups, s);
+}

@@ -1078,3 +1078,72 @@ def keep_nodes(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.
     if status:
         check(status, "moe_keep_nodes")
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _beam_ws_bytes(device: int, groups: int, beams: int, vocab: int, count: int, code: int) -> int:
+    return _native.lib().moe_beam_select_workspace_size(groups, beams, vocab, count, code)
+
+
+@_on_first_device
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int | None = None,
+                workspace: torch.Tensor | None = None):
+    """``(scores fp32, parents int32, tokens int64)``, each [groups, count]: every group's best
+    continuations over its beams and the vocabulary, the best first.
+
+    ``logits`` [groups * beams, vocab], fp16, bf16 or fp32 (rows may be strided, or one row expanded;
+    vocab <= 2^20); ``scores`` fp32 [groups, beams]: the beams' running sums of log-probabilities, -inf
+    for a beam that is not there (as all but one are at the first step); ``count`` (default: beams)
+    and beams at most 64.  A continuation scores its beam's score plus the token's log-probability;
+    ``parents`` is the beam's index in its group.  Equal scores go to the lower beam, in a beam to the
+    larger logit, then the lower token.  Tokens at -inf are no candidates, NaN logits count as
+    -inf; places without a candidate hold (-inf, 0, 0).  A beam that has ended is carried along by a
+    row that is -inf but for its end token.
+
+    ``workspace``: a zeroed buffer of :func:`beam_select_workspace` that no call on another stream
+    uses at the same time, as for :func:`paged_attention`.
+    """
+    what = "beam_select"
+    if not isinstance(logits, torch.Tensor) or logits.ndim != 2:
+        raise ValueError(f"{what}: logits must be [groups * beams, vocab]")
+    code = _DTYPE_CODES.get(logits.dtype)
+    if code is None:
+        raise ValueError(f"{what}: logits must be float16, bfloat16 or float32, got {logits.dtype}")
+    if not isinstance(scores, torch.Tensor) or scores.ndim != 2:
+        raise ValueError(f"{what}: scores must be [groups, beams]")
+    dev = logits.get_device()
+    rows, vocab = logits.shape
+    groups, beams = scores.shape
+    if not (_plain(dev, torch.float32, scores) and logits.stride(1) == 1):
+        _serve_check(what, dev, ("logits", logits, logits.dtype, logits.shape, 1),
+                     ("scores", scores, torch.float32, scores.shape, 2))
+    if rows != groups * beams:
+        raise ValueError(f"{what}: logits has {rows} rows for {groups} groups of {beams} beams")
+    if count is None:
+        count = beams
+    if not (1 <= beams <= 64 and 1 <= count <= 64):
+        raise ValueError(f"{what}: 1 to 64 beams and 1 to 64 continuations are served, got {beams} "
+                         f"and {count}")
+    out = (scores.new_empty((groups, count)), scores.new_empty((groups, count), dtype=torch.int32),
+           scores.new_empty((groups, count), dtype=torch.int64))
+    stream = _raw_stream(dev)
+    nbytes = _beam_ws_bytes(dev, groups, beams, vocab, count, code)
+    if workspace is None:
+        workspace = _serve_scratch(dev, stream, nbytes)
+    else:
+        _check_workspace(what, workspace, dev, nbytes)
+    status = _native.lib().moe_beam_select(_native.BEAM_SELECT.pack(
+        logits.data_ptr(), _outer_stride(logits), groups, beams, vocab, code, scores.data_ptr(), count,
+        out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), workspace.data_ptr(), nbytes, stream))
+    if status:
+        check(status, "moe_beam_select")
+    return out
+
+
+@_on_first_device
+def beam_select_workspace(logits: torch.Tensor, beams: int, count: int | None = None) -> torch.Tensor:
+    """A workspace for :func:`beam_select` calls on logits of this shape and type."""
+    rows, vocab = logits.shape
+    nbytes = _beam_ws_bytes(logits.get_device(), rows // beams, beams, vocab,
+                            beams if count is None else count, _DTYPE_CODES[logits.dtype])
+    return torch.zeros(nbytes, dtype=torch.uint8, device=logits.device)
