@@ -654,6 +654,45 @@ size_t moe_beam_select_workspace_size(int64_t groups, int64_t beams, int64_t voc
                                       int64_t dtype);
 int moe_beam_select(const moe_beam_select_args_t* args);
 
+/* moe_rope_append_slots: moe_rope_append whose keys and values go to position
+ *   slots[t] (int32 [tokens]) of the token's sequence; positions[t] gives the
+ *   rotation alone.  A drafted node's position is its depth in the tree beyond the
+ *   cached tokens, its slot its index beyond them.  A slot without a page appends nothing
+ *   and sets the device error word, as a position does. */
+int moe_rope_append_slots(const moe_rope_append_args_t* args, const int32_t* slots);
+
+/* moe_tree_attention: o[b,t,h] = softmax(scale q[b,t,h] . K^T) V over the keys
+ *   that node t of sequence b sees: the first lengths[b] positions, and position
+ *   lengths[b] + i where bit i % 64 of visible[b][t][i / 64] is set, for the nodes
+ *   i < counts[b] (counts NULL: `nodes` everywhere).  q [seqs, nodes, heads,
+ *   head_dim], sequences q_seq_stride and nodes q_node_stride elements apart
+ *   (multiples of 8); visible uint64 [seqs, nodes, ceil(nodes / 64)], strides in elements (0:
+ *   one mask for all); out [seqs, nodes, heads, head_dim] packed.  A row that sees
+ *   nothing is zeros, and so are the rows of nodes past counts[b] and of sequences with
+ *   lengths[b] < 0.  fp32 scores, softmax and sums; the probabilities are rounded to
+ *   the element type for the product with V.  What lies in a page past a
+ *   sequence's end, and the values of nodes that a row does not see, have no effect,
+ *   infinities and NaN included.  page_size % 16 == 0, seqs <= 2048, nodes <= 1024,
+ *   scale > 0.  The workspace's size depends on the device and head_dim alone; its first 4096
+ *   bytes must be zero before its first call and are left zero.  Results do not
+ *   vary from call to call. */
+typedef struct moe_tree_attention_args {
+  moe_kv_pages_t kv;
+  const uint16_t* q;
+  int64_t q_seq_stride, q_node_stride, nodes, heads;
+  const int32_t* lengths;
+  const int32_t* counts; /* may be NULL */
+  const uint64_t* visible;
+  int64_t visible_seq_stride, visible_node_stride;
+  double scale;
+  uint16_t* out;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+} moe_tree_attention_args_t;
+size_t moe_tree_attention_workspace_size(int64_t head_dim);
+int moe_tree_attention(const moe_tree_attention_args_t* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -38,6 +38,7 @@ PAGED_ATTENTION = struct.Struct("@" + _KV_PAGES + "PqqPdPPqP")
 PROMPT_ATTENTION = struct.Struct("@PqqqPqqPqqqPPqqqqqqqqdPPqP")
 SAMPLE_TOKENS = struct.Struct("@PqqqqPPPPPPPP")
 FORK_PAGES = struct.Struct("@" + _KV_PAGES + "qqqPPPqPqP")
+TREE_ATTENTION = struct.Struct("@" + _KV_PAGES + "PqqqqPPPqqdPPqP")
 BEAM_SELECT = struct.Struct("@PqqqqqPqPPPPqP")
 KEEP_NODES = struct.Struct("@" + _KV_PAGES + "qqqPPqqPP")
 
@@ -114,6 +115,9 @@ SIGNATURES: dict[str, tuple] = {
     "moe_fork_pages_workspace_size": (c_size_t, [c_int64]),
     "moe_fork_pages": (c_int, [c_void_p]),
     "moe_keep_nodes": (c_int, [c_void_p]),
+    "moe_rope_append_slots": (c_int, [c_void_p, c_void_p]),
+    "moe_tree_attention_workspace_size": (c_size_t, [c_int64]),
+    "moe_tree_attention": (c_int, [c_void_p]),
     "moe_beam_select_workspace_size": (c_size_t, [c_int64] * 5),
     "moe_beam_select": (c_int, [c_void_p]),
 }

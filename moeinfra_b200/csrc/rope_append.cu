@@ -31,6 +31,7 @@ struct RopeArgs {
   uint16_t* q_out;
   uint16_t* k_out;  // the rotated keys packed too (prompts attend to them), or null
   int heads;
+  const int32_t* slots;  // the positions' places in their sequence, or null: themselves
 };
 
 constexpr int kMaxThreads = 512;
@@ -54,17 +55,18 @@ __global__ void __launch_bounds__(kMaxThreads) k_rope_append(const RopeArgs a) {
   const int32_t pos = a.positions[t];
   const int32_t seq = a.seq_ids ? a.seq_ids[t] : static_cast<int32_t>(t);
   // The token's slot: page >= 0, or -1 for a padding token (position < 0) and
-  // for one whose position, sequence or page is out of range (error bit set).
+  // for one whose position, slot, sequence or page is out of range (error bit set).
   int64_t page = -1;
+  const int32_t place = a.slots ? a.slots[t] : pos;
   if (pos >= 0) {
-    const int entry = pos / a.kv.page_size;
-    if (pos < a.max_pos && seq >= 0 && seq < a.kv.seqs && entry < a.kv.max_pages) {
+    const int entry = place / a.kv.page_size;
+    if (pos < a.max_pos && place >= 0 && seq >= 0 && seq < a.kv.seqs && entry < a.kv.max_pages) {
       const int32_t p = a.kv.table[seq * a.kv.table_stride + entry];
       if (p >= 0 && p < a.kv.num_pages) page = p;
     }
     if (page < 0 && threadIdx.x == 0) set_device_error(kErrPage);
   }
-  const int slot = page < 0 ? 0 : pos % a.kv.page_size;
+  const int slot = page < 0 ? 0 : place % a.kv.page_size;
   for (int i = threadIdx.x; i < items; i += blockDim.x) {
     if (i != threadIdx.x) {
       lo = *reinterpret_cast<const uint4*>(source(i));
@@ -131,7 +133,7 @@ int launch_rope(const RopeArgs& a, int64_t tokens, cudaStream_t s) {
 }  // namespace
 }  // namespace moe
 
-extern "C" int moe_rope_append(const moe_rope_append_args_t* args) {
+extern "C" int moe_rope_append_slots(const moe_rope_append_args_t* args, const int32_t* slots) {
   using namespace moe;
   if (!args) return MOE_ERR_INVALID_ARG;
   const moe_rope_append_args_t& c = *args;
@@ -147,11 +149,15 @@ extern "C" int moe_rope_append(const moe_rope_append_args_t* args) {
       !aligned16(c.k_out) || (c.qkv_stride & 7))
     return MOE_ERR_ALIGNMENT;
   const RopeArgs a{c.qkv, c.qkv_stride, c.cos, c.sin, c.max_pos, c.positions, c.seq_ids,
-                   pages_of(c.kv), c.q_out, c.k_out, (int)c.heads};
+                   pages_of(c.kv), c.q_out, c.k_out, (int)c.heads, slots};
   cudaStream_t s = static_cast<cudaStream_t>(c.stream);
   if (c.kv.dtype == MOE_DTYPE_F16)
     return c.kv.head_dim == 64 ? launch_rope<F16, 64>(a, c.tokens, s)
                                : launch_rope<F16, 128>(a, c.tokens, s);
   return c.kv.head_dim == 64 ? launch_rope<BF16, 64>(a, c.tokens, s)
                              : launch_rope<BF16, 128>(a, c.tokens, s);
+}
+
+extern "C" int moe_rope_append(const moe_rope_append_args_t* args) {
+  return moe_rope_append_slots(args, nullptr);
 }

@@ -712,7 +712,8 @@ def _check_cache(what: str, k_pages, v_pages, block_table) -> None:
 def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
                 block_table: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                 num_heads: int, seq_ids: torch.Tensor | None = None,
-                out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> torch.Tensor:
+                out: torch.Tensor | None = None, k_out: torch.Tensor | None = None,
+                slots: torch.Tensor | None = None) -> torch.Tensor:
     """Rotate q and k of fused projection rows and append k and v to the paged cache.
 
     ``qkv`` [tokens, (num_heads + 2 * kv_heads) * head_dim] (rows may be strided), fp16 or bf16;
@@ -721,8 +722,10 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positio
     int32 [sequences, max_pages]; ``k_pages`` / ``v_pages`` [pages, kv_heads, page_size, head_dim],
     written in place; ``seq_ids`` int32 [tokens] (None: token t is sequence t, the decode step).
     Returns q [tokens, num_heads, head_dim]; ``k_out`` [tokens, kv_heads, head_dim], if given,
-    receives the rotated keys packed, as :func:`prompt_attention` reads them.  A position, sequence
-    or page out of range appends nothing and shows in :func:`check_device`.
+    receives the rotated keys packed, as :func:`prompt_attention` reads them.  ``slots`` int32
+    [tokens]: where in its sequence a token's keys and values go, if not to its position: drafted
+    nodes are rotated by their depth and stored by their index (:func:`tree_attention`).  A
+    position, slot, sequence or page out of range appends nothing and shows in :func:`check_device`.
     """
     what = "rope_append"
     try:
@@ -760,17 +763,21 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positio
         _serve_check(what, dev, ("out", out, dt, (T, num_heads, hd), 3))
     if k_out is not None:
         _serve_check(what, dev, ("k_out", k_out, dt, (T, kv, hd), 3))
+    if slots is not None:
+        _serve_check(what, dev, ("slots", slots, torch.int32, (T,), 1))
     page_elems = kv * page * hd
     strides = ((page_elems, page_elems, max_pages, (num_heads + 2 * kv) * hd) if plain else
                (_outer_stride(k_pages), _outer_stride(v_pages),
                 _outer_stride(block_table) if seqs else max_pages,
                 _outer_stride(qkv) if T else qkv.shape[1]))
-    status = _native.lib().moe_rope_append(_native.ROPE_APPEND.pack(
+    args = _native.ROPE_APPEND.pack(
         k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], n_pages, kv, page, hd,
         _DTYPE_CODES[dt], block_table.data_ptr(), strides[2], seqs, max_pages, qkv.data_ptr(),
         strides[3], cos.data_ptr(), sin.data_ptr(), max_pos,
         positions.data_ptr(), 0 if seq_ids is None else seq_ids.data_ptr(), T, num_heads,
-        out.data_ptr(), 0 if k_out is None else k_out.data_ptr(), _raw_stream(dev)))
+        out.data_ptr(), 0 if k_out is None else k_out.data_ptr(), _raw_stream(dev))
+    status = (_native.lib().moe_rope_append(args) if slots is None else
+              _native.lib().moe_rope_append_slots(args, slots.data_ptr()))
     if status:
         check(status, "moe_rope_append")
     return out
@@ -996,6 +1003,117 @@ def _check_layers(what: str, k_pages, v_pages, block_table) -> tuple:
         if t.shape[0] > 1 and t.stride(0) < (t.shape[1] - 1) * t.stride(1) + k[0:1].numel():
             raise ValueError(f"{what}: {name}'s layers overlap")
     return k_pages.shape[0], k_pages.stride(0), v_pages.stride(0), k, v
+
+
+@functools.lru_cache(maxsize=None)
+def _tree_ws_bytes(device: int, hd: int) -> int:
+    return _native.lib().moe_tree_attention_workspace_size(hd)
+
+
+@_on_first_device
+def tree_attention_workspace(k_pages: torch.Tensor) -> torch.Tensor:
+    """A workspace for :func:`tree_attention` calls on caches with this head_dim."""
+    nbytes = _tree_ws_bytes(k_pages.get_device(), k_pages.shape[-1])
+    return torch.zeros(nbytes, dtype=torch.uint8, device=k_pages.device)
+
+
+@_on_first_device
+def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                   block_table: torch.Tensor, lengths: torch.Tensor, visible: torch.Tensor,
+                   counts: torch.Tensor | None = None, scale: float | None = None,
+                   out: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a tree of drafted tokens per sequence over its cached keys and values.
+
+    ``q`` [sequences, nodes, heads, head_dim] (sequences and nodes may be strided); ``lengths`` int32
+    [sequences]: cached positions before the tree, which every node sees; node i's own keys and
+    values are at position ``lengths[b] + i`` (:func:`rope_append` with ``slots``).  ``visible`` int64
+    [sequences, nodes, ceil(nodes / 64)] (may be expanded): bit ``i % 64`` of word ``i // 64`` is
+    set where the node sees node i, itself included (:func:`tree_masks` makes it from parents).
+    ``counts`` int32 [sequences]: the nodes that are there (None: all).  A row that sees nothing
+    is zeros, and so are rows past ``counts`` and of sequences with a negative length.  The cache as in
+    :func:`paged_attention`; ``scale`` defaults to ``head_dim ** -0.5``.  Returns
+    [sequences, nodes, heads, head_dim].
+
+    ``workspace``: a buffer from :func:`tree_attention_workspace`, as for :func:`paged_attention`.
+    """
+    what = "tree_attention"
+    try:
+        n_pages, kv, page, hd = k_pages.shape
+        seqs, max_pages = block_table.shape
+        _, nodes, heads, _ = q.shape
+        words = (nodes + 63) // 64
+        dt, dev = k_pages.dtype, k_pages.get_device()
+        plain = (dt in _HALVES and (hd == 64 or hd == 128) and q.shape == (seqs, nodes, heads, hd)
+                 and v_pages.shape == k_pages.shape and lengths.shape == (seqs,)
+                 and visible.shape == (seqs, nodes, words)
+                 and _plain(dev, dt, q, k_pages, v_pages)
+                 and _plain(dev, torch.int32, lengths, block_table)
+                 and _plain(dev, torch.int64, visible))
+    except (AttributeError, ValueError):
+        plain = False
+    if not plain:
+        _check_cache(what, k_pages, v_pages, block_table)
+        n_pages, kv, page, hd = k_pages.shape
+        dt, dev = k_pages.dtype, k_pages.get_device()
+        seqs, max_pages = block_table.shape
+        _serve_check(what, dev, ("q", q, dt, (seqs, None, None, hd), 2),
+                     ("lengths", lengths, torch.int32, (seqs,), 1))
+        nodes, heads = q.shape[1:3]
+        words = (nodes + 63) // 64
+        _serve_check(what, dev, ("visible", visible, torch.int64, (seqs, nodes, words), 1))
+        if min(q.stride()) < 0 or min(visible.stride()) < 0:
+            raise ValueError(f"{what}: strides must not be negative")
+    if page % 16:
+        raise ValueError(f"{what}: page_size must be a multiple of 16, got {page}")
+    if heads == 0 or kv == 0 or heads % kv:
+        raise ValueError(f"{what}: {heads} query heads do not divide over {kv} KV heads")
+    if counts is not None:
+        _serve_check(what, dev, ("counts", counts, torch.int32, (seqs,), 1))
+    if out is None:
+        out = q.new_empty((seqs, nodes, heads, hd))
+    else:
+        _serve_check(what, dev, ("out", out, dt, (seqs, nodes, heads, hd), 4))
+    if seqs == 0 or nodes == 0:
+        return out
+    stream = _raw_stream(dev)
+    nbytes = _tree_ws_bytes(dev, hd)
+    if workspace is None:
+        workspace = _serve_scratch(dev, stream, nbytes)
+    else:
+        _check_workspace(what, workspace, dev, nbytes)
+    page_elems, row = kv * page * hd, heads * hd
+    if plain:
+        strides = (page_elems, page_elems, max_pages, nodes * row, row, nodes * words, words)
+    else:
+        node = q.stride(1) if nodes > 1 else row
+        strides = (_outer_stride(k_pages), _outer_stride(v_pages), _outer_stride(block_table),
+                   q.stride(0) if seqs > 1 else nodes * node, node, visible.stride(0),
+                   visible.stride(1))
+    status = _native.lib().moe_tree_attention(_native.TREE_ATTENTION.pack(
+        k_pages.data_ptr(), v_pages.data_ptr(), strides[0], strides[1], n_pages, kv, page, hd,
+        _DTYPE_CODES[dt], block_table.data_ptr(), strides[2], seqs, max_pages, q.data_ptr(),
+        strides[3], strides[4], nodes, heads, lengths.data_ptr(),
+        0 if counts is None else counts.data_ptr(), visible.data_ptr(), strides[5], strides[6],
+        hd ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(), nbytes, stream))
+    if status:
+        check(status, "moe_tree_attention")
+    return out
+
+
+def tree_masks(parents) -> torch.Tensor:
+    """``visible`` of :func:`tree_attention` from a tree's parents: int64 [nodes, ceil(nodes / 64)] on
+    the CPU.  ``parents[i] < i`` is node i's parent, -1 where it follows the cached tokens."""
+    seen: list[int] = []
+    for i, p in enumerate(parents):
+        p = int(p)
+        if not -1 <= p < i:
+            raise ValueError(f"tree_masks: node {i}'s parent must be -1 to {i - 1}, got {p}")
+        seen.append((seen[p] if p >= 0 else 0) | 1 << i)
+    words = (len(seen) + 63) // 64
+    rows = [[(m >> 64 * w & (1 << 64) - 1) - (m >> 64 * w + 63 & 1) * (1 << 64) for w in range(words)]
+            for m in seen]
+    return torch.tensor(rows, dtype=torch.int64).view(len(seen), words)
 
 
 @_on_first_device
