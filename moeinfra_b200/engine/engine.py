@@ -36,7 +36,10 @@ marks the padding, on either side) over a paged cache of ``kv_pages`` pages
 (default: enough for ``max_batch`` sequences of ``max_seq_len``) of
 ``page_size`` positions: :class:`~moeinfra_b200.engine.paged.PagedDenseStack`.
 ``ForwardRequest.sampling`` draws tokens instead of taking the largest logit,
-with either cache.
+with either cache.  ``ForwardRequest.num_beams`` searches with beams over the
+paged cache (``max_batch`` counts sequences times beams): the beams of a prompt
+share its pages, and choosing and reordering them is part of the captured step;
+``token_ids`` are each prompt's best beam's, ``scores`` their log-probabilities.
 """
 from __future__ import annotations
 
@@ -131,6 +134,65 @@ class _Sampler:
 
     def draw(self, logits: torch.Tensor) -> torch.Tensor:
         return kernels.sample_tokens(logits, self.uniforms, *self.params)[0]
+
+
+class _BeamStep:
+    """One step of beam search for B prompts of K beams, on the device: decode, choose, reorder.
+
+    ``ids``, ``lengths`` (positions cached, and so the next token's), ``scores`` and ``parents`` are
+    its buffers, which a captured step reads and writes.
+    """
+
+    def __init__(self, engine: "InferenceEngine", B: int, K: int) -> None:
+        dev, self.stack, self.K = engine._device, engine._stack, K
+        self.ids = torch.zeros(B * K, 1, dtype=torch.long, device=dev)
+        self.lengths = torch.full((B * K,), -1, dtype=torch.int32, device=dev)
+        self.scores = torch.zeros(B, K, device=dev)
+        self.parents = torch.zeros(B, K, dtype=torch.int32, device=dev)
+        self.first = torch.arange(0, B * K, K, dtype=torch.int32, device=dev)[:, None]
+        self.graph = self.logits = None
+
+    def begin(self, logits: torch.Tensor, prompt_lengths: torch.Tensor) -> torch.Tensor:
+        """The first tokens [B, K] from the prompts' logits; every beam starts as its prompt's copy."""
+        B, K = self.scores.shape
+        scores, _, tokens = kernels.beam_select(logits, self.scores.new_zeros(B, 1), K)
+        self.scores.copy_(scores)
+        self.ids.copy_(tokens.view(-1, 1))
+        self.lengths.zero_()
+        self.lengths[::K] = prompt_lengths
+        self.stack.cache.fork(self.lengths, self.first.repeat(1, K).view(-1))
+        return tokens
+
+    def _step(self) -> torch.Tensor:
+        logits = self.stack.decode(self.ids, self.lengths)
+        self.lengths.add_(1)
+        scores, parents, tokens = kernels.beam_select(logits, self.scores, self.K)
+        self.scores.copy_(scores)
+        self.parents.copy_(parents)
+        self.ids.copy_(tokens.view(-1, 1))
+        self.stack.cache.fork(self.lengths, (parents + self.first).view(-1))
+        return logits
+
+    def run(self) -> torch.Tensor:
+        """The next step; the logits of the beams it started from [B * K, vocab]."""
+        if self.graph is None:
+            return self._step()
+        self.graph.replay()
+        return self.logits
+
+    def capture(self) -> "torch.cuda.CUDAGraph":
+        """Warm up at position -1, which appends nothing and sees nothing, then capture."""
+        dev = self.scores.device
+        s = torch.cuda.Stream(dev)
+        s.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(s):
+            self._step()
+        torch.cuda.current_stream(dev).wait_stream(s)
+        torch.cuda.synchronize(dev)
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self.logits = self._step()
+        return self.graph
 
 
 class InferenceEngine:
@@ -288,6 +350,8 @@ class InferenceEngine:
     def generate(self, request: ForwardRequest) -> ForwardResult:
         """Prefill the prompts, then decode ``max_new_tokens`` tokens (greedy unless ``sampling``)."""
         self._initialize_runtime()
+        if request.num_beams != 1:
+            return self._generate_beams(request)
         timings: dict = {}
         B = request.input_ids.shape[0] if request.input_ids.ndim == 2 else 0
         sampler = None
@@ -384,6 +448,81 @@ class InferenceEngine:
         if max(lens) > self._max_len:
             raise ValueError(f"{max(lens)} positions exceed engine.max_seq_len={self._max_len}")
         self._stack.cache.reserve(lens)
+
+    # -- beam search ----------------------------------------------------------------------
+    @torch.no_grad()
+    def _generate_beams(self, request: ForwardRequest) -> ForwardResult:
+        """As ``generate``, the ``num_beams`` best continuations of each prompt kept at every step.
+
+        Prompt b's beams are sequences ``b * num_beams ..``; until the first step has chosen their
+        tokens only the first of them exists."""
+        K, n = request.num_beams, request.max_new_tokens
+        if not self._paged:
+            raise ValueError("num_beams needs engine.paged_kv")
+        if not 1 < K <= 64:
+            raise ValueError(f"num_beams must be 1 to 64, got {K}")
+        if request.sampling is not None:
+            raise ValueError("num_beams does not combine with sampling")
+        if n < 1:
+            raise ValueError("beam search needs max_new_tokens of at least 1")
+        prompts = self._prompts(request.input_ids, request.attention_mask)
+        B, lens = len(prompts), [int(p.numel()) for p in prompts]
+        if B * K > self._max_batch:
+            raise ValueError(f"{B} prompts of {K} beams exceed engine.max_batch={self._max_batch}")
+        if max(lens) + n - 1 > self._max_len:
+            raise ValueError(f"{max(lens) + n - 1} positions exceed engine.max_seq_len={self._max_len}")
+        cache, dev = self._stack.cache, self._device
+        # A prompt's full pages are shared; from its last, partly filled one on each beam may come to
+        # hold its own, up to the page of the position behind its last token.
+        page = cache.page_size
+        need = sum(m // page + K * ((m + n - 1) // page + 1 - m // page) for m in lens)
+        if need > cache.refs.numel():
+            raise RuntimeError(f"the paged cache has {cache.refs.numel()} pages, {need} may be needed "
+                               "(engine.kv_pages)")
+        use_graph = self._use_graphs and n > 1 and self.all_experts_resident()
+        with torch.cuda.device(dev):
+            cache.clear()  # a graph's warm-up forks sequences of its own
+            step = self._beam_graph_for(B, K) if use_graph else _BeamStep(self, B, K)
+            cache.reserve([m if k == 0 else 0 for m in lens for k in range(K)])
+            torch.cuda.synchronize(dev)
+            t0 = time.perf_counter()
+            logits = self._stack.prefill(prompts, stride=K)
+            torch.cuda.synchronize(dev)
+            t1 = time.perf_counter()
+            self._prompt_lens = lens
+            tokens = torch.empty(n, B, K, dtype=torch.long, device=dev)
+            parents = torch.zeros(n, B, K, dtype=torch.int32, device=dev)
+            tokens[0] = step.begin(logits, self._stack.prompt_lengths)
+            for i in range(1, n):
+                logits = step.run()
+                tokens[i], parents[i] = step.ids.view(B, K), step.parents.view(B, K)
+            # The beams are sorted: the best path ends in beam 0 and leads back over the parents.
+            at = torch.zeros(B, 1, dtype=torch.long, device=dev)
+            path = torch.empty(n, B, 1, dtype=torch.long, device=dev)
+            for i in range(n - 1, -1, -1):
+                path[i] = tokens[i].gather(1, at)
+                at = parents[i].long().gather(1, at)
+            token_ids = path[..., 0].t().cpu().tolist()
+            scores = step.scores[:, 0].cpu().tolist()
+            torch.cuda.synchronize(dev)
+        t2 = time.perf_counter()
+        kernels.check_device(dev)
+        self._last_logits = logits[:, None, :]
+        timings = {"prefill": (t1 - t0) * 1e3, "decode": (t2 - t1) * 1e3,
+                   "cuda_graph_decode": use_graph, "h2d_bytes": sum(
+                       p.get("bytes_transferred", 0) for p in self._transfer_scheduler_profile())}
+        return ForwardResult(logits=self._last_logits, token_ids=token_ids[0] if B == 1 else token_ids,
+                             ttft_ms=(t1 - t0) * 1e3, tps=B * (n - 1) / (t2 - t1) if n > 1 else 0.0,
+                             stage_timings=timings, scores=scores)
+
+    def _beam_graph_for(self, B: int, K: int) -> "_BeamStep":
+        """The captured beam step for B prompts of K beams (built once); the cache must be empty."""
+        ent = self._graphs.get((B, K, "beams"))
+        if ent is None:
+            step = _BeamStep(self, B, K)
+            ent = self._graphs[B, K, "beams"] = (step.capture(), step)
+            self._stack.cache.clear()
+        return ent[1]
 
     def _decode_step_fn(self, ids_buf, pos_buf, sampler=None):
         def step():

@@ -34,6 +34,7 @@ class ForwardRequest:
     attention_mask: Optional[torch.Tensor] = None
     max_new_tokens: int = 128
     sampling: Optional[SamplingParams] = None  # None: greedy
+    num_beams: int = 1  # above 1: beam search (engine.paged_kv)
 
 
 @dataclasses.dataclass
@@ -43,3 +44,4 @@ class ForwardResult:
     ttft_ms: float
     tps: float
     stage_timings: dict
+    scores: Optional[list] = None  # beam search: each sequence's sum of log-probabilities
