@@ -15,19 +15,18 @@
 //     Its keys come in steps of 64.  All units' steps form one line, which is cut
 //     evenly over persistent CTAs, one to an SM; the cuts are found on the device
 //     from the lengths, so a captured graph follows them.
-//   * A CTA's pieces run through two pipelines, each with its own rows Q, scores
-//     S, probabilities P and result O in tensor memory: both take the same keys
-//     where a unit has two tiles; else they take turns, so that one's start and end
-//     lie under the other's steps.
+//   * A CTA's pieces run through two pipelines, each with its own scores S,
+//     probabilities P (two buffers) and result O in tensor memory.  Where a unit has
+//     two tiles, each has one of them and both take the same keys; a single tile they
+//     share, one taking the even and one the odd steps, and join their results at the end.
 //     warps 0-3, 4-7  softmax of pipeline 0 and 1, one thread per row: S -> registers,
 //                     maximum, p = 2^(c s - c m), P (16 bits) -> tensor memory
-//     warp 8          loads Q, K and V with TMA (no multicast), pages by the table
+//     warps 8, 11     load Q and K, and V, with TMA (no multicast), pages by the table;
+//                     V past a sequence's end becomes zeros in shared memory: what lies
+//                     in a page there has no effect
 //     warps 9, 10     tcgen05.mma of pipeline 0 and 1: S = Q K^T, O += P V
-//     warp 11         zeros V past a sequence's end in shared memory: what lies in a
-//                     page there has no effect
-//   * A unit that several CTAs share is joined by the last of them to finish, in the
-//     order of its keys; the order of all sums depends on the shapes, the lengths and
-//     the GPU only.
+//   * What CTAs hold of a unit that is cut is joined by a second kernel, in the order of
+//     its keys; the order of all sums depends on the shapes, the lengths and the GPU only.
 //
 // O is rescaled only when a row's maximum grew by more than 2^8 since the reference
 // in use: probabilities stay below 2^8, O and l are sums of the same factor.
@@ -43,8 +42,12 @@ MOE_DEFINE_ERROR_WORD()
 
 constexpr int kM = 128;        // rows of a tile
 constexpr int kN = 64;         // keys of a step
-constexpr int kSoftWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kTailWarp = 11;
+constexpr int kSoftWarps = 8, kKeyWarp = 8, kMmaWarp = 9, kValueWarp = 11;
 constexpr int kThreads = 12 * 32;
+// Registers a thread: 12 warps x 168 at launch, of which the softmax warps take kSoftRegs and
+// the others keep kOtherRegs.
+constexpr int kSoftRegs = 200, kOtherRegs = 104;
+constexpr int kRegs = 2 * 128 * kSoftRegs + 128 * kOtherRegs;
 constexpr int kMaxSeqs = 2048, kMaxNodes = 1024;
 constexpr float kLazy = 8.f;   // log2 of what a row's maximum may grow before O is rescaled
 // fp16 probabilities, up to 2^kLazy, take 2^7 on top: 2^15 fits, normal down to 2^-21.
@@ -62,10 +65,10 @@ struct Cfg {
   static constexpr int kStages = 8 * 2 / kHalves;  // K and V tiles in flight: 128 KB
   static constexpr uint32_t kRing = kStages * kTileK;
   static constexpr uint32_t smem(int seqs) { return 2 * kTileQ + kRing + 1024 + (3 * seqs + 1) * 4; }
-  // TMEM columns of pipeline 0, and how much further pipeline 1's are.
-  static constexpr uint32_t kS = 0, kS1 = kN, kP = 2 * kN, kP1 = kN / 2, kO = 3 * kN, kO1 = HD;
+  // TMEM columns of pipeline 0, and how much further pipeline 1's are; P twice each.
+  static constexpr uint32_t kS = 0, kS1 = kN, kP = 2 * kN, kP1 = kN, kO = 4 * kN, kO1 = HD;
   static_assert(kO + 2 * HD <= 512, "TMEM columns");
-  // Floats of a piece: O [HD / 4][2 kM rows][4], then m and l per row.
+  // Floats of a piece: O [2 kM rows][HD], then m and l per row.
   static constexpr int kPiece = 2 * kM * (HD + 2);
 };
 
@@ -84,20 +87,31 @@ struct TreeArgs {
   int per_seq;                  // units of a sequence
   int box;                      // rows of a K or V box: they lie in one page
   float scale_log2;
-  uint32_t* counters;           // [CTAs]: pieces written of the unit that starts there; zero between calls
-  float* part;                  // [CTAs][2] pieces
+  int4* jobs;                   // [CTAs]: sequence, unit, CTAs and nodes of the cut unit that starts there
+  float* part;                  // [CTAs][2] pieces: 0 of a unit that starts before, 1 of one that goes on
   uint64_t wait_ns;
 };
 
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
   return mbar_poll_or(bar, parity, limit_ns, [] { set_device_error(kErrWaitTimeout); });
 }
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
-                                            int y, int z, int w) {
+// For a warp that runs it as a whole, with the same operands in every lane: issued by
+// the lane with leader != 0.  Operands that differ between lanes make each load some 150
+// cycles.
+__device__ __forceinline__ void tma_load_4d_if(uint32_t leader, uint32_t dst, const CUtensorMap* map,
+                                               uint32_t bar, int x, int y, int z, int w) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
-      "{%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      "{\n .reg .pred q;\n setp.ne.b32 q, %7, 0;\n"
+      " @q cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+      "{%3, %4, %5, %6}], [%2];\n}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx_if(uint32_t leader, uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+      " @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}\n" ::"r"(bar),
+      "r"(bytes), "r"(leader)
       : "memory");
 }
 // fp32 accumulate, M = 128; b_rows: B is stored along N (V) instead of K.
@@ -117,6 +131,19 @@ __device__ __forceinline__ uint32_t trace_odd(uint32_t v, uint32_t acc) {
   return acc;
 }
 
+// A sequence's cached positions, and those with its nodes; false if out of range.  No
+// sequence, or none of its nodes there: no keys, nothing to compute.
+__device__ __forceinline__ bool span(const TreeArgs& a, int b, int& len, int& keys) {
+  const int64_t most = (int64_t)a.kv.max_pages * a.kv.page_size;
+  const int n = a.lengths[b], have = a.counts ? a.counts[b] : a.nodes;
+  const int real = min(have, a.nodes);
+  len = keys = 0;
+  if (n < 0 || real <= 0) return have <= a.nodes;
+  keys = static_cast<int>(min((int64_t)n + real, most));
+  len = min(n, keys);
+  return have <= a.nodes && (int64_t)n + real <= most;
+}
+
 // What shared memory knows of the sequences: prefix sums of the steps of one
 // unit, cached positions, positions with the nodes.
 struct Line {
@@ -126,23 +153,16 @@ struct Line {
 // A CTA's pieces in order: steps [s0, s1) of unit u of sequence b, which has n.
 struct Piece {
   int b, u, s0, s1, n;
-  int tiles;   // bit t: pipeline t has a tile of it
-  int ones;    // pieces of one tile so far: they take the pipelines in turn
-  int at, end; // places in the line: this piece's end, the CTA's end
+  int at, end;  // places in the line: this piece's end, the CTA's end
 
-  __device__ __forceinline__ void shape(const TreeArgs& a) {
+  __device__ __forceinline__ void cut() {
     s1 = min(n, s0 + end - at);
     at += s1 - s0;
-    const int block = u % a.blocks;
-    const bool two = a.nodes - block * 2 * a.tokens > a.tokens;
-    tiles = two ? 3 : 1 << (ones & 1);
-    ones += !two;
   }
   __device__ __forceinline__ bool start(const TreeArgs& a, const Line& line, int lo, int hi) {
     at = lo;
     end = hi;
-    ones = 0;
-    if (lo >= hi) return false;
+    if (lo < 0 || lo >= hi) return false;
     int x = 0, y = a.kv.seqs;  // last b with prefix[b] * per_seq <= lo
     while (y - x > 1) {
       const int mid = (x + y) >> 1;
@@ -154,7 +174,7 @@ struct Piece {
     const int r = lo - line.prefix[b] * a.per_seq;
     u = r / n;
     s0 = r - u * n;
-    shape(a);
+    cut();
     return true;
   }
   __device__ __forceinline__ bool next(const TreeArgs& a, const Line& line) {
@@ -166,10 +186,25 @@ struct Piece {
       while (line.prefix[b + 1] == line.prefix[b]);
       n = line.prefix[b + 1] - line.prefix[b];
     }
-    shape(a);
+    cut();
     return true;
   }
 };
+
+// A piece as the first producer describes it to the other warps.
+struct __align__(16) Item {
+  int b, node0, head0, len;  // sequence, the unit's first node and head, cached positions
+  int keys, s0, steps;       // positions with the nodes; first step, number of steps (0: no more items)
+  int flags;                 // kTwo, kFirst, kLast, Q buffer << 3 (of a single tile), KV head << 8
+
+  // Of a shared tile, pipeline t takes every second step from its t-th on.
+  __device__ __forceinline__ int steps_of(int t) const { return flags & 1 ? steps : (steps + 1 - t) >> 1; }
+};
+constexpr int kTwo = 1;    // two tiles of rows, one to a pipeline; else the pipelines share one
+constexpr int kFirst = 2;  // the unit starts with this piece
+constexpr int kLast = 4;   // and ends with it
+constexpr int kItems = 4;  // described ahead
+constexpr int kReaders = 11;
 
 // A row of a unit: its node and head; node < 0: no row.
 struct Row {
@@ -200,6 +235,20 @@ __device__ __forceinline__ uint64_t seen_keys(const TreeArgs& a, int b, int node
   return real >= 64 ? mask : real <= 0 ? 0 : mask & ((1ull << real) - 1);
 }
 
+// The same for trees of up to 64 nodes, whose word w is at hand.
+__device__ __forceinline__ uint64_t seen_keys(uint64_t w, int len, int keys, int j0) {
+  const int off = len - j0, real = keys - j0;
+  const uint64_t mask = off >= 64 ? ~0ull : off > 0 ? w << off | ((1ull << off) - 1) : off > -64 ? w >> -off : 0;
+  return real >= 64 ? mask : real <= 0 ? 0 : mask & ((1ull << real) - 1);
+}
+
+// Whether a node sees no key at all.
+__device__ __forceinline__ bool blind(const TreeArgs& a, int b, int node, int len, int keys) {
+  bool none = len == 0;
+  for (int j = 0; j < keys && none; j += 64) none = seen_keys(a, b, node, len, keys, j) == 0;
+  return none;
+}
+
 __device__ __forceinline__ int64_t page_at(const TreeArgs& a, int b, int entry) {
   const int64_t page = entry < a.kv.max_pages ? a.kv.table[b * a.kv.table_stride + entry] : -1;
   if (page >= 0 && page < a.kv.num_pages) return page;
@@ -208,11 +257,12 @@ __device__ __forceinline__ int64_t page_at(const TreeArgs& a, int b, int entry) 
 }
 
 // One row by the formula, by one warp: 32 keys a step, one to a lane, then the
-// values of those that the node sees, HD / 32 dims to a lane.  For rows that met an
+// values of those that the node sees, HD / 32 dims to a lane; dims [from, to) are written.  For rows that met an
 // infinity or NaN among the values of a node they do not see (a probability of 0
 // does not silence it).  131072 keys take some 10 ms; the other warps' waits end after 2 s.
 template <typename T, int HD>
-__device__ __noinline__ void redo_row(const TreeArgs& a, int b, int node, int head, int len, int keys) {
+__device__ __noinline__ void redo_row(const TreeArgs& a, int b, int node, int head, int len, int keys,
+                                      int from, int to) {
   constexpr int kWords = HD / 64;
   const int lane = threadIdx.x & 31, kv_head = head / a.group, page = a.kv.page_size;
   const uint16_t* q = a.q + b * a.q_seq + node * a.q_node + head * HD;
@@ -267,14 +317,15 @@ __device__ __noinline__ void redo_row(const TreeArgs& a, int b, int node, int he
   uint16_t* out = a.out + (((int64_t)b * a.nodes + node) * a.heads + head) * HD;
 #pragma unroll
   for (int w = 0; w < kWords; ++w)
-    *reinterpret_cast<uint32_t*>(out + w * 64 + lane * 2) = T::pack(acc[w].x * inv, acc[w].y * inv);
+    if (w * 64 + lane * 2 >= from && w * 64 + lane * 2 < to)
+      *reinterpret_cast<uint32_t*>(out + w * 64 + lane * 2) = T::pack(acc[w].x * inv, acc[w].y * inv);
 }
 
 // A warp's rows whose result is not finite (odd): computed again where a value of a
 // node that the row does not see is not.
 template <typename T, int HD>
 __device__ __noinline__ void mend_rows(const TreeArgs& a, uint32_t odd, int b, Row mine, int len,
-                                       int keys) {
+                                       int keys, int from, int to) {
   const int lane = threadIdx.x & 31, page = a.kv.page_size;
   __syncwarp();
   while (odd) {
@@ -291,26 +342,7 @@ __device__ __noinline__ void mend_rows(const TreeArgs& a, uint32_t odd, int b, R
       for (int w = 0; w < HD / 64; ++w)
         met = trace_odd<T>(*reinterpret_cast<const uint32_t*>(v + w * 64 + lane * 2), met);
     }
-    if (__any_sync(0xffffffffu, met)) redo_row<T, HD>(a, b, node, head, len, keys);
-  }
-}
-
-// 32 columns of a finished row, divided by its sum.  `odd` gathers products: not
-// finite once an element is not.
-template <typename T>
-__device__ __forceinline__ void put_columns(uint16_t* dst, const uint32_t (&o)[32], float inv,
-                                            bool blind, float& odd) {
-#pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    float f[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      f[e] = __uint_as_float(o[i + e]);
-      odd = fmaf(f[e], 0.f, odd);
-      f[e] = blind ? 0.f : f[e] * inv;
-    }
-    *reinterpret_cast<uint4*>(dst + i) = make_uint4(T::pack(f[0], f[1]), T::pack(f[2], f[3]),
-                                                    T::pack(f[4], f[5]), T::pack(f[6], f[7]));
+    if (__any_sync(0xffffffffu, met)) redo_row<T, HD>(a, b, node, head, len, keys, from, to);
   }
 }
 
@@ -322,11 +354,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<HD>;
   constexpr int NS = C::kStages;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t s_qfull[2], s_qempty[2], s_full[NS], s_empty[NS], s_tail[NS],
-      s_sfull[2], s_sfree[2], s_pready[2], s_pvdone[2], s_drain[2];
+  __shared__ __align__(8) uint64_t s_qfull[2], s_qempty[2], s_full[NS], s_empty[NS], s_tail,
+      s_sfull[2], s_sfree[2], s_pready[2][2], s_pvdone[2][2], s_drain[2], s_done[kSoftWarps],
+      s_read[kSoftWarps], s_itfull[kItems], s_itempty[kItems];
+  __shared__ Item s_item[kItems];
+  __shared__ float2 s_ml[kSoftWarps][32];  // a shared tile's rows: maximum and sum of each pipeline
   __shared__ uint32_t s_tmem;
   __shared__ int s_scan[kThreads / 32];
-  __shared__ int4 s_join[2];
   __shared__ volatile int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (saddr(smem_raw) + 1023u) & ~1023u;
@@ -338,17 +372,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(saddr(&s_qfull[t]), 1);
-      mbar_init(saddr(&s_qempty[t]), 1);
+      mbar_init(saddr(&s_qempty[t]), 2);
       mbar_init(saddr(&s_sfull[t]), 1);
       mbar_init(saddr(&s_sfree[t]), 4);
-      mbar_init(saddr(&s_pready[t]), 4);
-      mbar_init(saddr(&s_pvdone[t]), 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(saddr(&s_pready[t][i]), 4);
+        mbar_init(saddr(&s_pvdone[t][i]), 1);
+      }
       mbar_init(saddr(&s_drain[t]), 1);
+    }
+    for (int w = 0; w < kSoftWarps; ++w) {
+      mbar_init(saddr(&s_done[w]), 1);
+      mbar_init(saddr(&s_read[w]), 1);
+    }
+    mbar_init(saddr(&s_tail), 1);
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(saddr(&s_itfull[i]), 1);
+      mbar_init(saddr(&s_itempty[i]), kReaders);
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(saddr(&s_full[i]), 1);
       mbar_init(saddr(&s_empty[i]), 2);
-      mbar_init(saddr(&s_tail[i]), 1);
     }
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -364,21 +408,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   // The line: steps of a unit of each sequence, and their running sum.
   int run = 0;
-  const int64_t most = (int64_t)a.kv.max_pages * a.kv.page_size;
   for (int b0 = 0; b0 < a.kv.seqs; b0 += kThreads) {
     const int b = b0 + tid;
     int steps = 0;
     if (b < a.kv.seqs) {
-      const int len = a.lengths[b];
-      int have = a.counts ? a.counts[b] : a.nodes;
-      if (have > a.nodes || (len >= 0 && (int64_t)len + max(have, 0) > most)) {
-        if (blockIdx.x == 0) set_device_error(kErrPage);
-        have = min(have, a.nodes);
-      }
-      // No sequence, or none of its nodes are there: nothing to compute.
-      const bool none = len < 0 || have <= 0;
-      const int keys = none ? 0 : static_cast<int>(min((int64_t)len + have, most));
-      s_len[b] = none ? 0 : min(len, keys);
+      int len, keys;
+      if (!span(a, b, len, keys) && blockIdx.x == 0) set_device_error(kErrPage);
+      s_len[b] = len;
       s_keys[b] = keys;
       steps = (keys + kN - 1) / kN;
     }
@@ -410,27 +446,50 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lo = (int)min((int64_t)blockIdx.x * share, (int64_t)total), hi = (int)min((int64_t)lo + share, (int64_t)total);
   // A sequence's nodes that are there: rows of the others are zeros.
   auto have_of = [&](int b) { return min(s_keys[b] - s_len[b], a.nodes); };
-  float* parts = a.part + (int64_t)blockIdx.x * 2 * C::kPiece;
 
-  Piece it;
-  bool more = it.start(a, line, lo, hi);
+  // The next item; false at the end or after a timeout (then ok is false).
+  Item it;
+  uint32_t n_it = 0;
+  bool ok = true;
+  auto next_item = [&]() {
+    const uint32_t i = n_it % kItems;
+    ok = warp_wait(saddr(&s_itfull[i]), n_it / kItems & 1, a.wait_ns);
+    if (!ok) return false;
+    it = s_item[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(saddr(&s_itempty[i]));
+    ++n_it;
+    return it.steps > 0;
+  };
   if (warp < kSoftWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     // ---------------- softmax: one thread per row of pipeline t ----------------
-    const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane, pal = warp ^ 4;  // pal: the same rows' other warp
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + C::kS + t * C::kS1 + lane_base;
     const uint32_t p_at = tmem + C::kP + t * C::kP1 + lane_base;
     const uint32_t o_at = tmem + C::kO + t * C::kO1 + lane_base;
-    uint32_t n_s = 0, n_pv = 0;  // phases of s_full and pv_done
-    bool ok = true;
-    for (; more && ok; more = it.next(a, line)) {
-      if (!(it.tiles >> t & 1)) continue;
-      const int second = it.tiles == 3 ? t : 0, len = s_len[it.b], keys = s_keys[it.b];
-      const Row me = row_of(a, it.u, second, row, have_of(it.b));
-      const bool idle = !__any_sync(0xffffffffu, me.node >= 0);  // no row of this warp is one
+    const uint32_t o_pal = tmem + C::kO + (1 - t) * C::kO1 + lane_base;
+    const int row_node = row / a.tile_heads, row_head = row - row_node * a.tile_heads;
+    uint32_t n_s = 0, n_pair = 0;  // steps and shared tiles so far
+    // P V of step n (counted as n_s is), whose P was in buffer n & 1.
+    auto product_done = [&](uint32_t n) {
+      return warp_wait(saddr(&s_pvdone[t][n & 1]), n >> 1 & 1, a.wait_ns);
+    };
+    while (next_item()) {
+      const bool two = it.flags & kTwo;
+      const int second = two ? t : 0;
+      Row me{it.node0 + second * a.tokens + row_node, it.head0 + row_head};
+      if (row_node >= a.tokens || me.node >= it.keys - it.len) me.node = -1;
+      const bool real = me.node >= 0;
+      const bool idle = !__any_sync(0xffffffffu, real);  // no row of this warp is one
+      const int mine = it.steps_of(t);
+      uint64_t sees = 0;  // trees of up to 64 nodes: the row's mask
+      if (real && a.words == 1) sees = a.visible[it.b * a.vis_seq + me.node * a.vis_node];
       float m = -INFINITY, l = 0.f;
-      for (int j = it.s0; j < it.s1; ++j) {
-        if (!(ok = warp_wait(saddr(&s_sfull[t]), n_s++ & 1, a.wait_ns))) break;
+      for (int i = 0; i < mine; ++i, ++n_s) {
+        const int j0 = (it.s0 + (two ? i : 2 * i + t)) * kN;
+        if (!(ok = warp_wait(saddr(&s_sfull[t]), n_s & 1, a.wait_ns))) break;
         tc_fence_after();
         uint32_t s[kN];
         if (!idle) {
@@ -443,8 +502,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(saddr(&s_sfree[t]));
         float top = -INFINITY;
         if (!idle) {
-          if (j * kN + kN > len) {
-            const uint64_t mask = me.node >= 0 ? seen_keys(a, it.b, me.node, len, keys, j * kN) : 0;
+          if (j0 + kN > it.len) {
+            const uint64_t mask = a.words == 1 ? seen_keys(sees, it.len, it.keys, j0)
+                                  : real ? seen_keys(a, it.b, me.node, it.len, it.keys, j0) : 0;
             const uint32_t mlo = (uint32_t)mask, mhi = (uint32_t)(mask >> 32);
 #pragma unroll
             for (int c = 0; c < 32; ++c) {
@@ -458,25 +518,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             mx[c / 2 & 3] = max3(mx[c / 2 & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
           top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
         }
-        // P's columns and O are free once the previous product is done.
-        if (j > it.s0) {
-          if (!(ok = warp_wait(saddr(&s_pvdone[t]), n_pv++ & 1, a.wait_ns))) break;
-          tc_fence_after();
-        }
+        // The P buffer is free once the last product but one is done.
+        if (i >= 2 && !(ok = product_done(n_s - 2))) break;
         if (!idle) {
           if (__any_sync(0xffffffffu, top > m + (m == -INFINITY ? 0.f : kLazy))) {
             const float nm = fmaxf(m, top);
             const float f = m == nm ? 1.f : exp2_approx(m - nm);
             m = nm;
             l *= f;
-            if (j > it.s0) {
+            if (i > 0) {
+              if (!(ok = product_done(n_s - 1))) break;
+              tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
                 tmem_ld32(o_at + c, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
                 tmem_st32(o_at + c, o);
               }
             }
@@ -492,168 +551,228 @@ __global__ void __launch_bounds__(kThreads, 1)
             sum[c / 2 & 1] = add2(sum[c / 2 & 1], e);
             p[c / 2] = T::pack(lo_of(e), hi_of(e));
           }
-          tmem_st32(p_at, p);
+          tmem_st32(p_at + (n_s & 1) * (kN / 2), p);
           tmem_wait_st();
           sum[0] = add2(sum[0], sum[1]);
           l += lo_of(sum[0]) + hi_of(sum[0]);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(saddr(&s_pready[t]));
+        if (lane == 0) mbar_arrive(saddr(&s_pready[t][n_s & 1]));
       }
-      if (ok) ok = warp_wait(saddr(&s_pvdone[t]), n_pv++ & 1, a.wait_ns);
+      // The last two products; a barrier's next phase needs a P of the next piece.
+      if (ok && mine > 1) ok = product_done(n_s - 2);
+      if (ok && mine > 0) ok = product_done(n_s - 1);
       if (!ok) break;
       tc_fence_after();
-      if (!idle) {
-        const bool real = me.node >= 0;
-        if (it.s0 == 0 && it.s1 == it.n) {
-          // The whole unit.  A row without keys is zeros; one with keys has l above 0, unless every
-          // score is -inf (0 / 0), and NaN where one is NaN or +inf: the row then is NaN.
-          bool blind = false;
-          if (real && l == 0.f) {
-            blind = len == 0;
-            for (int j = 0; j < keys && blind; j += 64)
-              blind = seen_keys(a, it.b, me.node, len, keys, j) == 0;
-          }
-          const float inv = __fdividef(1.f, l);
-          uint16_t* dst = a.out + (((int64_t)it.b * a.nodes + max(me.node, 0)) * a.heads + me.head) * HD;
-          float odd = 0.f;
+      if (idle) continue;
+      // A tile of one's own, or half the columns of a shared one: both results, joined by the
+      // maxima that the warps tell each other.
+      int from = 0, to = HD;
+      float f = 1.f, f_pal = 0.f;
+      const bool pal_has = !two && it.steps_of(1 - t) > 0;
+      if (!two) {
+        from = t * (HD / 2);
+        to = from + HD / 2;
+        s_ml[warp][lane] = make_float2(m, l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(saddr(&s_done[warp]));
+        if (!(ok = warp_wait(saddr(&s_done[pal]), n_pair & 1, a.wait_ns))) break;
+        tc_fence_after();
+        const float2 other = s_ml[pal][lane];
+        const float nm = fmaxf(m, other.x);
+        f = m == nm ? 1.f : exp2_approx(m - nm);
+        f_pal = other.x == nm ? 1.f : exp2_approx(other.x - nm);
+        // The same order of the sum in both warps.
+        l = t == 0 ? l * f + other.y * f_pal : other.y * f_pal + l * f;
+        m = nm;
+      }
+      // Result columns go out 32 at a time: to the output, if the unit is whole, or to a piece (0:
+      // of a unit that starts before, 1: of one that goes on).
+      const bool whole = (it.flags & (kFirst | kLast)) == (kFirst | kLast);
+      // A row without keys is zeros; one with keys has l above 0, unless every score is -inf
+      // (0 / 0), and NaN where one is NaN or +inf: the row then is NaN.
+      const bool none = whole && real && l == 0.f && blind(a, it.b, me.node, it.len, it.keys);
+      const float inv = whole ? __fdividef(1.f, l) : 1.f;
+      float* piece = a.part + ((int64_t)blockIdx.x * 2 + (it.flags & kFirst ? 1 : 0)) * C::kPiece;
+      uint16_t* dst = a.out + (((int64_t)it.b * a.nodes + max(me.node, 0)) * a.heads + me.head) * HD;
+      float* dst_piece = piece + (second * kM + row) * HD;
+      float odd = 0.f;  // NaN once an element is not finite
 #pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(o_at + c, o);
-            tmem_wait_ld();
-            if (real) put_columns<T>(dst + c, o, inv, blind, odd);
-          }
-          const uint32_t again = __ballot_sync(0xffffffffu, real && !blind && odd != 0.f);
-          if (again) mend_rows<T, HD>(a, again, it.b, me, len, keys);
-        } else {
-          // A piece: the unit's start (its end is another CTA's) or what follows it.
-          float* dst = parts + (it.s0 == 0 ? C::kPiece : 0);
-          const int r = second * kM + row;
-#pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(o_at + c, o);
-            tmem_wait_ld();
+      for (int c = from; c < to; c += 32) {
+        uint32_t o[32], x[32];
+        tmem_ld32(o_at + c, o);
+        if (pal_has) tmem_ld32(o_pal + c, x);
+        tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              reinterpret_cast<uint4*>(dst)[((c + i) / 4) * 2 * kM + r] =
-                  make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-          }
-          dst[2 * kM * HD + r] = m;
-          dst[2 * kM * (HD + 1) + r] = l;
+        for (int e = 0; e < 32; ++e) {
+          float v = mine > 0 ? __uint_as_float(o[e]) * f : 0.f;
+          if (pal_has) v = fmaf(__uint_as_float(x[e]), f_pal, v);
+          odd = fmaf(v, 0.f, odd);
+          o[e] = __float_as_uint(none ? 0.f : v * inv);
         }
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<uint4*>(dst_piece + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else if (real) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = T::pack(__uint_as_float(o[e + 2 * i]), __uint_as_float(o[e + 2 * i + 1]));
+            *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (!whole && from == 0) {
+        piece[2 * kM * HD + second * kM + row] = m;
+        piece[2 * kM * (HD + 1) + second * kM + row] = l;
       }
       tc_fence_before();
+      if (!two) {  // neither result is overwritten before both warps have read it
+        __syncwarp();
+        if (lane == 0) mbar_arrive(saddr(&s_read[warp]));
+        if (!(ok = warp_wait(saddr(&s_read[pal]), n_pair++ & 1, a.wait_ns))) break;
+        tc_fence_after();
+      }
+      const uint32_t again = __ballot_sync(0xffffffffu, whole && real && !none && odd != 0.f);
+      if (again) mend_rows<T, HD>(a, again, it.b, me, it.len, it.keys, from, to);
     }
     if (!ok) s_abort = 1;
-  } else if (warp == kTmaWarp) {
-    // ---------------- TMA producer ----------------
-    // Q, K(0), then K(j + 1), V(j): the order of use.
-    uint32_t g = 0, n_q[2] = {0, 0};
-    bool ok = true;
-    const int boxes = kN / a.box, my_box = lane / C::kHalves, half = lane % C::kHalves;
-    // Pages of 32 boxes of the sequence from w_base on, one per lane, and of the 32 after them.
-    int w_base = 0, w_page = 0, w_next = 0;
-    auto look = [&](int x) -> int {  // the page of box x
-      const int j = x * a.box;
-      return j < s_keys[it.b] ? (int)page_at(a, it.b, j / a.kv.page_size) : 0;
-    };
-    int cur_page = 0, cur_y = 0, nxt_page = 0, nxt_y = 0;
-    auto find = [&](int j) {  // this lane's box of step j
-      const int x = j * boxes + my_box;
-      if (j * boxes >= w_base + 32) {
-        w_base += 32;
-        w_page = w_next;
-        w_next = look(w_base + 32 + lane);
-      }
-      nxt_page = __shfl_sync(0xffffffffu, w_page, (x - w_base) & 31);
-      nxt_y = x * a.box % a.kv.page_size;
-    };
-    auto load = [&](bool is_v, int j, int page, int y, int kv_head) {
-      const int s = g % NS;
-      ok = ok && warp_wait(saddr(&s_empty[s]), ((g / NS) & 1) ^ 1, a.wait_ns);
-      if (__any_sync(0xffffffffu, s_abort)) ok = false;
+  } else {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  if (warp == kKeyWarp || warp == kValueWarp) {
+    // ---------------- TMA producers: Q and K, or V ----------------
+    // Tiles of a piece stand in the ring in the order of their use: K(0), then K(j + 1), V(j).
+    const bool is_v = warp == kValueWarp;
+    const CUtensorMap* map = is_v ? &map_v : &map_k;
+    const uint32_t leader = elect_one();
+    const int boxes = kN / a.box, page_boxes = a.kv.page_size / a.box;
+    uint32_t g = 0, n_q0 = 0, n_q1 = 0, n_tail = 0, ones = 0;
+    Piece pc;
+    bool more = !is_v && pc.start(a, line, lo, hi);
+    // Describes the next piece, or the end.
+    auto publish = [&]() {
+      const uint32_t i = n_it % kItems;
+      ok = warp_wait(saddr(&s_itempty[i]), (n_it / kItems & 1) ^ 1, a.wait_ns);
       if (!ok) return;
-      ++g;
-      const int rows = s_keys[it.b] - j * kN;
-      const int count = min(boxes, (rows + a.box - 1) / a.box);
-      const uint32_t bar = saddr(is_v && rows < kN ? &s_tail[s] : &s_full[s]);
-      if (lane == 0) mbar_expect_tx(bar, count * a.box * 128 * C::kHalves);
+      ++n_it;
+      if (lane == 0) {
+        Item x{};
+        if (more) {
+          const int kp = pc.u / a.blocks, block = pc.u - kp * a.blocks;
+          const bool two = a.nodes - block * 2 * a.tokens > a.tokens;
+          x = Item{pc.b, block * 2 * a.tokens, kp * a.tile_heads, s_len[pc.b], s_keys[pc.b], pc.s0,
+                   pc.s1 - pc.s0,
+                   (two ? kTwo : 0) | (pc.s0 == 0 ? kFirst : 0) | (pc.s1 == pc.n ? kLast : 0) |
+                       (int)(ones & 1) << 3 | kp / a.parts << 8};
+          ones += !two;
+        }
+        s_item[i] = x;
+        mbar_arrive(saddr(&s_itfull[i]));
+      }
       __syncwarp();
-      if (my_box < count)
-        tma_load_4d(ring + s * C::kTileK + half * C::kHalfK + my_box * a.box * 128,
-                    is_v ? &map_v : &map_k, bar, half * 64, y, kv_head, page);
+      if (more) more = pc.next(a, line);
     };
-    for (; more && ok; more = it.next(a, line)) {
-      const int kp = it.u / a.blocks, block = it.u - kp * a.blocks, kv_head = kp / a.parts;
-      w_base = it.s0 * boxes / 32 * 32;
-      w_page = look(w_base + lane);
-      w_next = look(w_base + 32 + lane);
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (!(it.tiles >> t & 1)) continue;
-        ok = warp_wait(saddr(&s_qempty[t]), (n_q[t]++ & 1) ^ 1, a.wait_ns);
+    uint32_t n_mine = 0;
+    auto take = [&]() {  // the first producer's own items, one described ahead
+      if (is_v) return next_item();
+      if (n_mine == 0) publish();
+      if (!ok) return false;
+      it = s_item[n_mine % kItems];
+      ++n_mine;
+      if (__shfl_sync(0xffffffffu, it.steps, 0) == 0) return false;
+      publish();
+      return ok;
+    };
+    while (take()) {
+      const int flags = __shfl_sync(0xffffffffu, it.flags, 0), seq = __shfl_sync(0xffffffffu, it.b, 0);
+      const int s0 = __shfl_sync(0xffffffffu, it.s0, 0), all = __shfl_sync(0xffffffffu, it.steps, 0);
+      const int keys = __shfl_sync(0xffffffffu, it.keys, 0), kv_head = flags >> 8;
+      // Places of 32 boxes of the sequence from w_base on, one per lane, and pages of the 32
+      // after them.
+      auto look = [&](int x) -> int {  // the page of box x
+        return x * a.box < keys ? (int)page_at(a, seq, x / page_boxes) : 0;
+      };
+      int w_base = s0 * boxes / 32 * 32;
+      int w_page = look(w_base + lane), w_next = look(w_base + 32 + lane);
+      int w_y = (w_base + lane) % page_boxes * a.box;
+      for (int t = 0; !is_v && t < (flags & kTwo ? 2 : 1) && ok; ++t) {
+        const int slot = flags & kTwo ? t : flags >> 3 & 1;
+        const uint32_t turn = slot ? n_q1++ : n_q0++;
+        ok = warp_wait(saddr(&s_qempty[slot]), (turn & 1) ^ 1, a.wait_ns);
         if (!ok) break;
-        if (lane == 0) {
-          const uint32_t bar = saddr(&s_qfull[t]);
-          mbar_expect_tx(bar, a.tokens * a.tile_heads * 128 * C::kHalves);
+        const uint32_t bar = saddr(&s_qfull[slot]);
+        mbar_expect_tx_if(leader, bar, a.tokens * a.tile_heads * 128 * C::kHalves);
+        for (int hf = 0; hf < C::kHalves; ++hf)
+          tma_load_4d_if(leader, q_at + slot * C::kTileQ + hf * C::kHalfQ, &map_q, bar, hf * 64,
+                         __shfl_sync(0xffffffffu, it.head0, 0),
+                         __shfl_sync(0xffffffffu, it.node0, 0) + t * a.tokens, seq);
+      }
+      if (!ok || __any_sync(0xffffffffu, s_abort)) break;
+      for (int i = 0; i < all; ++i) {
+        const uint32_t x = g + (is_v ? (i + 1 == all ? 2 * all - 1 : 2 * i + 2) : i == 0 ? 0 : 2 * i - 1);
+        const uint32_t s = x % NS, dst = ring + s * C::kTileK;
+        const int from = (s0 + i) * boxes - w_base;
+        if (from >= 32) {
+          w_base += 32;
+          w_page = w_next;
+          w_y = (w_base + lane) % page_boxes * a.box;
+          w_next = look(w_base + 32 + lane);
+        }
+        const int rows = keys - (s0 + i) * kN, count = min(boxes, (rows + a.box - 1) / a.box);
+        const bool tail = is_v && rows < kN;
+        const uint32_t bar = tail ? saddr(&s_tail) : saddr(&s_full[s]);
+        ok = warp_wait(saddr(&s_empty[s]), (x / NS & 1) ^ 1, a.wait_ns);
+        if (!ok) break;
+        mbar_expect_tx_if(leader, bar, count * a.box * 128 * C::kHalves);
+        for (int n = 0; n < count; ++n) {
+          const int page = __shfl_sync(0xffffffffu, w_page, from + n);
+          const int y = __shfl_sync(0xffffffffu, w_y, from + n);
+#pragma unroll
           for (int hf = 0; hf < C::kHalves; ++hf)
-            tma_load_4d(q_at + t * C::kTileQ + hf * C::kHalfQ, &map_q, bar, hf * 64, kp * a.tile_heads,
-                        (block * 2 + (it.tiles == 3 ? t : 0)) * a.tokens, it.b);
+            tma_load_4d_if(leader, dst + hf * C::kHalfK + n * a.box * 128, map, bar, hf * 64, y, kv_head,
+                           page);
         }
+        if (!tail) continue;
+        ok = warp_wait(saddr(&s_tail), n_tail++ & 1, a.wait_ns);
+        if (!ok) break;
+        for (int hf = 0; hf < C::kHalves; ++hf)
+          for (uint32_t z = rows * 128 + lane * 16; z < C::kHalfK; z += 512)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + hf * C::kHalfK + z),
+                         "r"(0)
+                         : "memory");
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(saddr(&s_full[s]));
       }
-      if (!ok) break;
-      find(it.s0);
-      cur_page = nxt_page;
-      cur_y = nxt_y;
-      load(false, it.s0, cur_page, cur_y, kv_head);
-      for (int j = it.s0; j < it.s1 && ok; ++j) {
-        if (j + 1 < it.s1) {
-          find(j + 1);
-          load(false, j + 1, nxt_page, nxt_y, kv_head);
-        }
-        load(true, j, cur_page, cur_y, kv_head);
-        cur_page = nxt_page;
-        cur_y = nxt_y;
-      }
+      g += 2 * all;
     }
     if (!ok) s_abort = 1;
-    // After a timeout copies may be in flight: let them land (a tail's on its own barrier).
-    if (!ok && lane == 0) {
-      for (uint32_t j = g > (uint32_t)NS ? g - NS : 0; j < g; ++j) {
-        const uint32_t bar = saddr(&s_full[j % NS]);
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_poll(bar, (j / NS) & 1) && globaltimer_ns() - t0 < 1000000) {}
-      }
-      for (int t = 0; t < 2; ++t) {
-        const uint64_t t0 = globaltimer_ns();
-        while (n_q[t] && !mbar_poll(saddr(&s_qfull[t]), (n_q[t] - 1) & 1) &&
-               globaltimer_ns() - t0 < 1000000) {}
-      }
+    // After a timeout copies may be in flight: the CTA stays until they have landed.
+    if (s_abort) {
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
     }
-  } else if (warp == kTailWarp) {
-    // ---------------- V past a sequence's end becomes zeros ----------------
-    uint32_t g = 0, phases = 0;  // tiles so far; a bit per stage: parity of its next tail
-    for (; more; more = it.next(a, line)) {
-      g += 2 * (it.s1 - it.s0);
-      const int rows = s_keys[it.b] - (it.s1 - 1) * kN;
-      if (rows >= kN) continue;
-      const uint32_t s = (g - 1) % NS;
-      if (!warp_wait(saddr(&s_tail[s]), phases >> s & 1, a.wait_ns)) {
-        s_abort = 1;
-        break;
+    if (is_v) {
+      Piece last;
+      if (lane == 0) {  // what is to be joined
+        int4 job = make_int4(0, 0, 0, 0);
+        if (last.start(a, line, hi - 1, hi)) {
+          const int at = prefix[last.b] * a.per_seq + last.u * last.n, to = at + last.n;
+          if (at >= lo && to > hi) job = make_int4(last.b, last.u, (to - 1) / share - blockIdx.x + 1, have_of(last.b));
+        }
+        a.jobs[blockIdx.x] = job;
       }
-      phases ^= 1u << s;
-      const uint32_t dst = ring + s * C::kTileK;
-      for (int hf = 0; hf < C::kHalves; ++hf)
-        for (uint32_t z = rows * 128 + lane * 16; z < C::kHalfK; z += 512)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + hf * C::kHalfK + z),
-                       "r"(0)
-                       : "memory");
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(saddr(&s_full[s]));
+      // Rows of nodes that are not there: zeros.
+      for (int b = blockIdx.x; b < a.kv.seqs; b += gridDim.x) {
+        const int row = a.heads * HD / 8;
+        uint4* o = reinterpret_cast<uint4*>(a.out) + (int64_t)b * a.nodes * row;
+        for (int i = have_of(b) * row + lane; i < a.nodes * row; i += 32) o[i] = make_uint4(0, 0, 0, 0);
+      }
     }
   } else {
     // ---------------- MMA issuers: one warp per pipeline ----------------
@@ -662,36 +781,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = warp - kMmaWarp;
     const uint32_t d_qk = instr_desc<T>(kN, false), d_pv = instr_desc<T>(HD, true);
     const uint32_t leader = elect_one();
-    const uint64_t desc_q = smem_desc(q_at + t * C::kTileQ), desc_k = smem_desc(ring);
+    const uint64_t desc_q = smem_desc(q_at), desc_k = smem_desc(ring);
     const uint64_t desc_v = smem_desc_mn(ring, C::kHalfK);
     const uint32_t s_col = tmem + C::kS + t * C::kS1, p_col = tmem + C::kP + t * C::kP1;
     const uint32_t o_col = tmem + C::kO + t * C::kO1;
-    uint32_t slot = 0, turn = 0;  // of the ring: the next tile, and the parity of its barrier
-    uint32_t n_q = 0, n_qk = 0, n_pv = 0;
-    bool ok = true;
-    auto next = [&]() {  // waits for the ring's next tile and takes its slot
-      const uint32_t at = slot;
-      ok = ok && warp_wait(saddr(&s_full[slot]), turn, a.wait_ns);
-      if (++slot == NS) {
-        slot = 0;
-        turn ^= 1;
-      }
-      return at;
+    uint32_t g = 0;               // tiles of the ring before this piece
+    uint32_t n_q0 = 0, n_q1 = 0;  // uses of the Q buffers
+    uint32_t n_qk = 0, n_pv = 0;
+    auto tile = [&](uint32_t x) {  // waits for tile x of the ring; its slot
+      ok = ok && warp_wait(saddr(&s_full[x % NS]), x / NS & 1, a.wait_ns);
+      return x % NS;
     };
-    // A slot is released by both warps, by one that uses it after its product.
-    for (; more && ok; more = it.next(a, line)) {
-      const int steps = __shfl_sync(0xffffffffu, it.s1 - it.s0, 0);
-      if (!(__shfl_sync(0xffffffffu, it.tiles, 0) >> t & 1)) {
-        for (int i = 0; i < 2 * steps && ok; ++i) {
-          const uint32_t at = next();
-          if (ok && lane == 0) mbar_arrive(saddr(&s_empty[at]));
-        }
-        continue;
-      }
-      ok = warp_wait(saddr(&s_qfull[t]), n_q++ & 1, a.wait_ns);
-      for (int j = -1; j < steps && ok; ++j) {  // Q K^T of step j + 1, P V of step j
-        if (j + 1 < steps) {
-          const uint32_t k = next();
+    // A slot, like a Q buffer, counts two releases: of each pipeline, or of the only one twice.
+    while (ok && next_item()) {
+      const int flags = __shfl_sync(0xffffffffu, it.flags, 0);
+      const int all = __shfl_sync(0xffffffffu, it.steps, 0);
+      const bool two = flags & kTwo;
+      const int mine = two ? all : (all + 1 - t) >> 1, slot = two ? t : flags >> 3 & 1;
+      const uint32_t q_turn = slot ? n_q1 : n_q0;
+      n_q0 += two || slot == 0;
+      n_q1 += two || slot == 1;
+      ok = warp_wait(saddr(&s_qfull[slot]), q_turn & 1, a.wait_ns);
+      if (ok && mine == 0 && lane == 0) mbar_arrive(saddr(&s_qempty[slot]));
+      const uint64_t qd = desc_q + slot * (C::kTileQ >> 4);
+      for (int i = -1; i < mine && ok; ++i) {  // Q K^T of step i + 1, P V of step i
+        if (i + 1 < mine) {
+          const uint32_t j = two ? i + 1 : 2 * (i + 1) + t;
+          const uint32_t k = tile(g + (j == 0 ? 0 : 2 * j - 1));
           // S, once the last one is read.
           if (n_qk > 0) ok = ok && warp_wait(saddr(&s_sfree[t]), (n_qk - 1) & 1, a.wait_ns);
           if (!ok) break;
@@ -700,26 +816,34 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint64_t kd = desc_k + k * (C::kTileK >> 4);
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
-            tc_mma_if(leader, s_col, desc_q + ((kk / 4 * C::kHalfQ + kk % 4 * 32) >> 4),
+            tc_mma_if(leader, s_col, qd + ((kk / 4 * C::kHalfQ + kk % 4 * 32) >> 4),
                       kd + ((kk / 4 * C::kHalfK + kk % 4 * 32) >> 4), d_qk, kk != 0);
           tc_commit_if(leader, saddr(&s_sfull[t]));
           tc_commit_if(leader, saddr(&s_empty[k]));
-          if (j + 2 == steps) tc_commit_if(leader, saddr(&s_qempty[t]));
+          if (!two) tc_commit_if(leader, saddr(&s_empty[k]));
+          if (i + 2 == mine) {
+            tc_commit_if(leader, saddr(&s_qempty[slot]));
+            if (two) tc_commit_if(leader, saddr(&s_qempty[slot]));
+          }
         }
-        if (j < 0) continue;
-        const uint32_t v = next();
-        ok = ok && warp_wait(saddr(&s_pready[t]), n_pv & 1, a.wait_ns);
+        if (i < 0) continue;
+        const uint32_t j = two ? i : 2 * i + t;
+        const uint32_t v = tile(g + (j + 1 == (uint32_t)all ? 2 * all - 1 : 2 * j + 2));
+        ok = ok && warp_wait(saddr(&s_pready[t][n_pv & 1]), n_pv >> 1 & 1, a.wait_ns);
         if (!ok) break;
-        ++n_pv;
         tc_fence_after();
         const uint64_t vd = desc_v + v * (C::kTileK >> 4);
-        tc_mma_ta_if(leader, o_col, p_col, vd, d_pv, j == 0 ? 0 : 1);
+        const uint32_t pc = p_col + (n_pv & 1) * (kN / 2);
+        tc_mma_ta_if(leader, o_col, pc, vd, d_pv, i == 0 ? 0 : 1);
 #pragma unroll
         for (int kk = 1; kk < kN / 16; ++kk)
-          tc_mma_ta_if(leader, o_col, p_col + kk * 8, vd + (kk * 2048 >> 4), d_pv, 1);
-        tc_commit_if(leader, saddr(&s_pvdone[t]));
+          tc_mma_ta_if(leader, o_col, pc + kk * 8, vd + (kk * 2048 >> 4), d_pv, 1);
+        tc_commit_if(leader, saddr(&s_pvdone[t][n_pv & 1]));
         tc_commit_if(leader, saddr(&s_empty[v]));
+        if (!two) tc_commit_if(leader, saddr(&s_empty[v]));
+        ++n_pv;
       }
+      g += 2 * all;
     }
     if (!ok) s_abort = 1;
     // After a timeout, wait (bounded) for the MMAs already issued.
@@ -728,96 +852,120 @@ __global__ void __launch_bounds__(kThreads, 1)
       warp_wait(saddr(&s_drain[t]), 0, a.wait_ns);
     }
   }
-
-  // Rows of nodes that are not there: zeros.
-  for (int b = blockIdx.x; b < a.kv.seqs; b += gridDim.x) {
-    const int row = a.heads * HD / 8;
-    uint4* o = reinterpret_cast<uint4*>(a.out) + (int64_t)b * a.nodes * row;
-    for (int i = have_of(b) * row + tid; i < a.nodes * row; i += kThreads) o[i] = make_uint4(0, 0, 0, 0);
   }
-
   tc_fence_before();
-  __threadfence();
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u)
                  : "memory");
   }
-  // ---- join the CTAs' pieces: the last CTA of a unit to get here does it ----
-  // A unit is counted at the CTA that holds its start.  Whoever finds the count
-  // full sees every piece (each CTA's are fenced before its count) and sets the
-  // counter back to zero for the next launch.
-  if (tid < 2) {
-    int4 job = make_int4(0, 0, 0, 0);  // b, u, first CTA, pieces (0: not the last)
-    Piece p;
-    if (lo < hi) {
-      // 0: the unit that the CTA's first step belongs to; 1: that of its last.
-      p.start(a, line, tid ? hi - 1 : lo, hi);
-      const int from = prefix[p.b] * a.per_seq + p.u * p.n, to = from + p.n;
-      const int c0 = from / share, pieces = (to - 1) / share - c0 + 1;
-      // One unit over the whole CTA is counted once.
-      const bool mine = pieces > 1 && (tid == 0 ? from < lo || to > hi : from > lo);
-      if (mine && atomicAdd(a.counters + c0, 1) == (uint32_t)pieces - 1) {
-        a.counters[c0] = 0;
-        job = make_int4(p.b, p.u, c0, pieces);
-      }
-    }
-    s_join[tid] = job;
-  }
-  __syncthreads();
-  if (warp >= kSoftWarps) return;
-  for (int w = 0; w < 2; ++w) {
-    const int4 job = s_join[w];
-    if (job.w == 0 || s_abort) continue;
-    __threadfence();
-    const int second = warp >> 2, row = (warp & 3) * 32 + lane, r = second * kM + row;
-    const int len = s_len[job.x], keys = s_keys[job.x];
-    const Row me = row_of(a, job.y, second, row, have_of(job.x));
-    const bool real = me.node >= 0;
-    if (!__any_sync(0xffffffffu, real)) continue;
-    // Piece 0 is CTA c0's second, the others the first of the CTAs after it.
-    const float* first = a.part + (int64_t)job.z * 2 * C::kPiece;
-    auto piece = [&](int k) { return first + (int64_t)(k == 0 ? 1 : 2 * k) * C::kPiece; };
-    float m = -INFINITY, l = 0.f;
-    for (int k = 0; k < job.w; ++k) m = fmaxf(m, __ldcg(piece(k) + 2 * kM * HD + r));
-    auto factor = [&](int k) {
-      const float mk = __ldcg(piece(k) + 2 * kM * HD + r);
-      return mk == m ? 1.f : exp2_approx(mk - m);
-    };
-    for (int k = 0; k < job.w; ++k) l += factor(k) * __ldcg(piece(k) + 2 * kM * (HD + 1) + r);
-    bool blind = false;
-    if (real && l == 0.f) {
-      blind = len == 0;
-      for (int j = 0; j < keys && blind; j += 64) blind = seen_keys(a, job.x, me.node, len, keys, j) == 0;
-    }
-    const float inv = __fdividef(1.f, l);
-    uint16_t* dst = a.out + (((int64_t)job.x * a.nodes + max(me.node, 0)) * a.heads + me.head) * HD;
-    float odd = 0.f;
-#pragma unroll 1
-    for (int c = 0; c < HD; c += 32) {
-      float acc[32] = {};
-#pragma unroll 1
-      for (int k = 0; k < job.w; ++k) {
-        const float f = factor(k);
-        const float4* src = reinterpret_cast<const float4*>(piece(k)) + (c / 4) * 2 * kM + r;
+}
+
+// The cut units' results, in the order of the keys: CTA (c, y) takes part y of the rows of
+// the unit that is cut at the end of the main kernel's CTA c.  A warp has ROWS x AHEAD
+// (row, piece) pairs on its way at once.
+constexpr int kJoinThreads = 256, kJoinParts = 8, kPairs = 8;
+template <typename T, int HD, int AHEAD>
+__device__ __forceinline__ void join_rows(const TreeArgs& a, int4 job) {
+  constexpr int kPiece = Cfg<HD>::kPiece, kVec = HD / 32, ROWS = kPairs / AHEAD;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = job.x, n = job.z, have = job.w;
+  // Piece 0 is CTA c's second, the others the first of the CTAs after it.
+  const float* first = a.part + (int64_t)blockIdx.x * 2 * kPiece;
+  for (int r0 = (blockIdx.y * (kJoinThreads / 32) + warp) * ROWS; r0 < 2 * kM;
+       r0 += kJoinParts * (kJoinThreads / 32) * ROWS) {
+    Row me[ROWS];
+    bool some = false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 x = __ldcg(src + i * 2 * kM);
-          acc[4 * i] += f * x.x;
-          acc[4 * i + 1] += f * x.y;
-          acc[4 * i + 2] += f * x.z;
-          acc[4 * i + 3] += f * x.w;
+    for (int i = 0; i < ROWS; ++i) {
+      me[i] = row_of(a, job.y, (r0 + i) / kM, (r0 + i) % kM, have);
+      some |= me[i].node >= 0;
+    }
+    if (!some) continue;
+    float m[ROWS], l[ROWS] = {}, acc[ROWS][kVec] = {};
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) m[i] = -INFINITY;
+    for (int k0 = 0; k0 < n; k0 += AHEAD) {
+      float mk[AHEAD][ROWS], lk[AHEAD][ROWS], ok[AHEAD][ROWS][kVec] = {};
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const float* src = first + (int64_t)(k0 + k == 0 ? 1 : 2 * (k0 + k)) * kPiece;
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+          mk[k][i] = -INFINITY;
+          lk[k][i] = 0.f;
+          if (k0 + k >= n) continue;
+          mk[k][i] = src[2 * kM * HD + r0 + i];
+          lk[k][i] = src[2 * kM * (HD + 1) + r0 + i];
+          const float* x = src + (r0 + i) * HD + lane * kVec;
+          if constexpr (kVec == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(x);
+            ok[k][i][0] = v.x, ok[k][i][1] = v.y, ok[k][i][2] = v.z, ok[k][i][3] = v.w;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(x);
+            ok[k][i][0] = v.x, ok[k][i][1] = v.y;
+          }
         }
       }
-      uint32_t o[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(acc[i]);
-      if (real) put_columns<T>(dst + c, o, inv, blind, odd);
+      for (int i = 0; i < ROWS; ++i) {
+        float nm = m[i];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) nm = fmaxf(nm, mk[k][i]);
+        const float f = m[i] == nm ? 1.f : exp2_approx(m[i] - nm);
+        m[i] = nm;
+        l[i] *= f;
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) acc[i][c] *= f;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const float fk = mk[k][i] == nm ? 1.f : exp2_approx(mk[k][i] - nm);
+          l[i] = fmaf(fk, lk[k][i], l[i]);
+#pragma unroll
+          for (int c = 0; c < kVec; ++c) acc[i][c] = fmaf(fk, ok[k][i][c], acc[i][c]);
+        }
+      }
     }
-    const uint32_t again = __ballot_sync(0xffffffffu, real && !blind && odd != 0.f);
-    if (again) mend_rows<T, HD>(a, again, job.x, me, len, keys);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      if (me[i].node < 0) continue;
+      int len = 0, keys = 0;
+      bool none = false;
+      if (l[i] == 0.f) {
+        span(a, b, len, keys);
+        none = blind(a, b, me[i].node, len, keys);
+      }
+      const float inv = __fdividef(1.f, l[i]);
+      float odd = 0.f;
+      uint32_t o[kVec / 2];
+#pragma unroll
+      for (int c = 0; c < kVec; c += 2) {
+        odd = fmaf(acc[i][c], 0.f, fmaf(acc[i][c + 1], 0.f, odd));
+        o[c / 2] = none ? 0u : T::pack(acc[i][c] * inv, acc[i][c + 1] * inv);
+      }
+      uint32_t* dst = reinterpret_cast<uint32_t*>(
+          a.out + (((int64_t)b * a.nodes + me[i].node) * a.heads + me[i].head) * HD + lane * kVec);
+      if constexpr (kVec == 4)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
+      else
+        *dst = o[0];
+      if (__any_sync(0xffffffffu, odd != 0.f) && !none) {
+        span(a, b, len, keys);
+        mend_rows<T, HD>(a, 1, b, me[i], len, keys, 0, HD);
+      }
+    }
   }
+}
+template <typename T, int HD>
+__global__ void __launch_bounds__(kJoinThreads, 3) k_tree_join(const __grid_constant__ TreeArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const int4 job = a.jobs[blockIdx.x];
+  if (job.z == 0) return;
+  if (job.z == 2) join_rows<T, HD, 2>(a, job);
+  else if (job.z <= 4) join_rows<T, HD, 4>(a, job);
+  else join_rows<T, HD, 8>(a, job);
 }
 
 // Four dimensions, boxes of box[1] x box[2] rows of 64 elements, 128-byte swizzle.
@@ -836,7 +984,12 @@ bool make_map(CUtensorMap* map, const uint16_t* x, bool bf16, const cuuint64_t (
 
 template <typename T, int HD>
 bool tree_attr() {
-  return cudaFuncSetAttribute(k_tree_attention<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  // The warps' register shares must not exceed what the block is launched with: the last to
+  // ask would wait for good.
+  cudaFuncAttributes at;
+  return cudaFuncGetAttributes(&at, k_tree_attention<T, HD>) == cudaSuccess &&
+         at.numRegs * kThreads >= kRegs &&
+         cudaFuncSetAttribute(k_tree_attention<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               Cfg<HD>::smem(kMaxSeqs)) == cudaSuccess;
 }
 
@@ -849,10 +1002,13 @@ int launch_tree(const TreeArgs& a, const CUtensorMap& q, const CUtensorMap& k, c
                  k, v) != cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
+  if (launch_pdl(k_tree_join<T, HD>, dim3(grid, kJoinParts), dim3(kJoinThreads), 0, s, a) != cudaSuccess)
+    return MOE_ERR_CUDA;
+  MOE_CHECK_LAUNCH();
   return MOE_OK;
 }
 
-constexpr int64_t kPartAt = 4096;  // behind the counters that every call leaves zero
+constexpr int64_t kJobsAt = 4096;  // behind the counters of the calls that share a workspace
 
 }  // namespace
 }  // namespace moe
@@ -860,7 +1016,7 @@ constexpr int64_t kPartAt = 4096;  // behind the counters that every call leaves
 extern "C" size_t moe_tree_attention_workspace_size(int64_t head_dim) {
   using namespace moe;
   if (head_dim != 64 && head_dim != 128) return 0;
-  return kPartAt + (size_t)sm_count() * 2 * 4 * (head_dim == 64 ? Cfg<64>::kPiece : Cfg<128>::kPiece);
+  return kJobsAt + (size_t)sm_count() * 16 + (size_t)sm_count() * 2 * 4 * (head_dim == 64 ? Cfg<64>::kPiece : Cfg<128>::kPiece);
 }
 
 extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
@@ -918,8 +1074,8 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
   const size_t need = moe_tree_attention_workspace_size(hd);
   if (!c.workspace || c.workspace_bytes < (int64_t)need) return MOE_ERR_WORKSPACE;
   if (!aligned16(c.workspace)) return MOE_ERR_ALIGNMENT;
-  a.counters = static_cast<uint32_t*>(c.workspace);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + kPartAt);
+  a.jobs = reinterpret_cast<int4*>(static_cast<char*>(c.workspace) + kJobsAt);
+  a.part = reinterpret_cast<float*>(a.jobs + sm_count());
   a.wait_ns = wait_limit_ns();
   const bool bf16 = c.kv.dtype == MOE_DTYPE_BF16;
   const bool none = c.kv.max_pages == 0;  // no keys at all: the maps describe q
