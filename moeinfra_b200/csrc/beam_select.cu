@@ -9,28 +9,28 @@
 // among those.
 //
 // Bound by memory: every logit is read once.  A row is cut into `splits` CTAs
-// where there are few rows.  A CTA goes through its part in chunks of 4 vectors of
-// 16 bytes a thread, the next chunk's loads in flight:
-//   * each thread keeps a running maximum and the sum of exponentials
-//     below it (8 terms in fp32, those sums in fp64: 2 % of the arithmetic, and
-//     beams' scores can be compared to the last bit of their rounding);
-//   * logits above a threshold go to a list in shared memory.  The threshold is
-//     such that `count` logits are known to reach it: in the first chunk it comes
-//     from the threads' own maxima, of which the warps' largest few are taken.
-//     Later chunks put in about `count` logits each, and one comparison per
-//     vector skips the others.  A chunk with more than the list takes (equal
-//     logits, mostly) is searched round by round instead.
+// where there are few rows.  A thread takes groups of 4 vectors of 16 bytes, the next
+// group's loads in flight:
+//   * it keeps a running maximum and the sum of exponentials below it (a group's
+//     terms in fp32, their sums in fp64, so that beams' scores can be compared nearly to
+//     the last bit of their rounding);
+//   * logits above a threshold go to a list in shared memory, and `count` logits
+//     are known to reach the threshold.  A CTA's first chunk (a group a thread) sets it from
+//     the threads' own maxima, of which the warps' largest few are taken.  Then come stretches
+//     without a barrier, each as long as all before it: each puts in some `count` logits,
+//     and one comparison a group skips the others.
+//   * A stretch that puts in more than the list holds (rising logits) is looked at
+//     again chunk by chunk, each with a threshold of its own, and a chunk that still has too
+//     many (equal logits) is searched round by round.
 // The last CTA of a group joins the lists of its rows.
 #include "sample.cuh"
 
 namespace moe {
 namespace {
 
-MOE_DEFINE_ERROR_WORD()
-
 constexpr int kMostBeams = 64, kMostCount = 64;
 constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
-constexpr int kVecs = 4;            // 16-byte vectors of a thread in a chunk
+constexpr int kVecs = 4;            // 16-byte vectors of a thread in a group
 constexpr int kList = 2048;         // entries of the list
 constexpr int kRank = 384;          // entries that are put in order by counting
 constexpr int kGroups = 1000;       // counters of a launch (the workspace's first 4096 bytes)
@@ -46,7 +46,7 @@ struct BeamArgs {
   int64_t* out_tokens;
   uint32_t* done;                   // [groups]: CTAs done, zero between calls
   double2* sums;                    // [rows, splits]: sum, maximum
-  uint64_t* keys;                   // [rows, splits, count]: falling, 0: none
+  uint64_t* keys;                   // [rows, splits, count]: 0: none
 };
 
 template <typename T>
@@ -61,6 +61,16 @@ struct Vec {
       f[2 * i] = x.x;
       f[2 * i + 1] = x.y;
     }
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {  // NaN: the other
+    uint32_t d;
+    if constexpr (T::kBf16) asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  static __device__ __forceinline__ float top(const uint4& r) {  // NaN where all are
+    const float2 x = T::unpack(max2(max2(r.x, r.y), max2(r.z, r.w)));
+    return fmaxf(x.x, x.y);
   }
   // Elements outside [lo, hi) become -inf.
   static __device__ __forceinline__ void cut(uint4& r, int64_t lo, int64_t hi) {
@@ -80,6 +90,10 @@ struct Vec<float> {
     f[1] = __uint_as_float(r.y);
     f[2] = __uint_as_float(r.z);
     f[3] = __uint_as_float(r.w);
+  }
+  static __device__ __forceinline__ float top(const uint4& r) {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)),
+                 fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
   }
   static __device__ __forceinline__ void cut(uint4& r, int64_t lo, int64_t hi) {
     uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -122,6 +136,21 @@ __device__ __forceinline__ Pick block_best(Pick p, Pick* s_warp) {
   __syncthreads();
   return p;
 }
+// out(i, number of j < n with above(j, i)) for each i < n, as many threads to an i as there are.
+template <typename A, typename O>
+__device__ __forceinline__ void rank_all(int n, A above, O out) {
+  int per = 32;
+  while (per > 1 && per * n > kBeamThreads) per >>= 1;
+  const int tid = threadIdx.x, part = tid & (per - 1);
+  for (int i0 = 0; i0 < n; i0 += kBeamThreads / per) {
+    const int i = i0 + tid / per;
+    int count = 0;
+    if (i < n)
+      for (int j = part; j < n; j += per) count += above(j, i);
+    for (int o = per >> 1; o; o >>= 1) count += __shfl_xor_sync(kAll, count, o);
+    if (i < n && part == 0) out(i, count);
+  }
+}
 // A key that at least `count` of the threads' keys reach, or 0 where no warp is full: the
 // smallest of the full warps' ceil(count / full warps)-th largest.  Keys 0 do not count.
 __device__ __forceinline__ uint32_t reached_by(uint32_t key, int count, uint32_t* s_warp) {
@@ -147,8 +176,51 @@ __device__ __forceinline__ uint32_t reached_by(uint32_t key, int count, uint32_t
   return each > 32 ? 0 : low + 1;
 }
 
+// The sum of exponentials of a vector below m: ordinary arithmetic where all goes well.
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads, 3) k_beam_select(const BeamArgs a) {
+__device__ __forceinline__ float exp_sum(const uint4& r, float m) {
+  constexpr int kN = Vec<T>::kN;
+  float f[kN];
+  Vec<T>::unpack(r, f);
+  uint64_t e[kN / 2];
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) {
+    const uint64_t d = mul2(add2(pair(f[2 * i], f[2 * i + 1]), pair(-m, -m)), pair(kLog2e, kLog2e));
+    e[i] = pair(exp2_approx(lo_of(d)), exp2_approx(hi_of(d)));
+  }
+#pragma unroll
+  for (int w = kN / 4; w; w /= 2)
+#pragma unroll
+    for (int i = 0; i < w; ++i) e[i] = add2(e[i], e[i + w]);
+  return lo_of(e[0]) + hi_of(e[0]);
+}
+// The same where a logit is NaN (counts as -inf) or m is +inf (its equals count 1).
+template <typename T>
+__device__ __noinline__ float exp_sum_odd(uint4 r, float m) {
+  float f[Vec<T>::kN], sum = 0.f;
+  Vec<T>::unpack(r, f);
+  for (int i = 0; i < Vec<T>::kN; ++i)
+    sum += f[i] == m ? 1.f : f[i] < m && m < INFINITY ? exp2_approx((f[i] - m) * kLog2e) : 0.f;
+  return sum;
+}
+
+// A vector's logits above thr (level: those that reach it) go to the list.  A function of its
+// own: few vectors have one, and the loop around stays short.
+template <typename T>
+__device__ __noinline__ void put_vector(uint4 r, float thr, bool level, uint32_t token, uint64_t* list,
+                                        int* count) {
+  float f[Vec<T>::kN];
+  Vec<T>::unpack(r, f);
+#pragma unroll
+  for (int i = 0; i < Vec<T>::kN; ++i)
+    if (level ? f[i] >= thr : f[i] > thr) {
+      const int at = atomicAdd(count, 1);
+      if (at < kList) list[at] = key_of(f[i], token + i);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kBeamThreads, 4) k_beam_select(const BeamArgs a) {
   constexpr int kN = Vec<T>::kN;
   constexpr int kChunk = kBeamThreads * kVecs;  // vectors
   __shared__ __align__(16) uint64_t s_list[kList];
@@ -156,7 +228,7 @@ __global__ void __launch_bounds__(kBeamThreads, 3) k_beam_select(const BeamArgs 
   __shared__ uint64_t s_top[kMostCount];
   __shared__ uint32_t s_warp[kBeamWarps];
   __shared__ double s_sum[kBeamWarps];
-  __shared__ float s_max[kBeamWarps], s_rowmax[kMostBeams], s_rowsum[kMostBeams];
+  __shared__ float s_max[kBeamWarps], s_rowmax[kMostBeams], s_rowsum[kMostBeams], s_score[kMostBeams];
   __shared__ int s_count, s_last;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, M = a.count;
   const int row = blockIdx.x / (uint32_t)a.splits, split = blockIdx.x - row * a.splits;
@@ -171,130 +243,135 @@ __global__ void __launch_bounds__(kBeamThreads, 3) k_beam_select(const BeamArgs 
   pdl_trigger();
   pdl_wait();
 
-  auto fetch = [&](int first, uint4 (&r)[kVecs]) {
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      const int v = first + u * kBeamThreads + tid;
-      r[u] = make_uint4(0, 0, 0, 0);
-      if (v < hi) r[u] = __ldcs(vecs + v);
-    }
-  };
-  float m = -INFINITY, thr = -INFINITY;
-  double sum = 0;
-  uint4 next[kVecs];
-  fetch(lo, next);
-  int had = 0;  // entries of the list before the chunk
-  for (int c = lo; c < hi; c += kChunk) {
-    uint4 r[kVecs];
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) r[u] = next[u];
-    if (c + kChunk < hi) fetch(c + kChunk, next);
-    float top[kVecs], mine = -INFINITY;
+  uint4 r[kVecs], next[kVecs];
+  int next_at = -1;  // the group that `next` holds
+  auto fetch = [&](int c) {
+    next_at = c;
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
       const int v = c + u * kBeamThreads + tid;
-      top[u] = -INFINITY;
-      if (v >= hi) continue;
-      const int64_t at = (int64_t)v * kN - skew;  // the token of its first element
-      if (at < 0 || at + kN > a.vocab) Vec<T>::cut(r[u], -at, a.vocab - at);
-      float f[kN];
-      Vec<T>::unpack(r[u], f);
-#pragma unroll
-      for (int i = 0; i < kN; ++i) top[u] = fmaxf(top[u], f[i]);  // NaN: the other
-      mine = fmaxf(mine, top[u]);
-      if (top[u] > m) {
-        sum = m == -INFINITY ? 0 : sum * exp2_approx((m - top[u]) * kLog2e);
-        m = top[u];
-      }
-      if (top[u] == -INFINITY) continue;
-      float e[kN];
-      if (m == INFINITY) {
-#pragma unroll
-        for (int i = 0; i < kN; ++i) e[i] = f[i] == INFINITY ? 1.f : 0.f;
-      } else {
-#pragma unroll
-        for (int i = 0; i < kN; i += 2) {
-          const uint64_t d = mul2(add2(pair(f[i], f[i + 1]), pair(-m, -m)), pair(kLog2e, kLog2e));
-          e[i] = exp2_approx(fmaxf(lo_of(d), -200.f));  // 0 for -inf and NaN
-          e[i + 1] = exp2_approx(fmaxf(hi_of(d), -200.f));
-        }
-      }
-#pragma unroll
-      for (int w = kN / 2; w; w /= 2)
-#pragma unroll
-        for (int i = 0; i < w; ++i) e[i] += e[i + w];
-      sum += e[0];
+      next[u] = make_uint4(0, 0, 0, 0);
+      if (v < hi) next[u] = __ldcs(vecs + v);
     }
-    // Which logits are put into the list: those above thr, of which `count` are known to
-    // reach it in earlier chunks, or (level) those that reach it.
-    const int busy = __syncthreads_count(mine > thr);
-    if (busy == 0) continue;
-    bool level = false;
-    if (thr == -INFINITY || busy > 2 * M + 32) {
-      const uint32_t k = reached_by(mine == -INFINITY ? 0 : Logit<float>::key(mine), M, s_warp);
-      const float t = k ? Logit<float>::value(k) : -INFINITY;
-      if (t > thr) {
-        thr = t;
-        level = true;
+  };
+  float top[kVecs], gtop;
+  // The group at c to r, the next one's loads on their way; its maxima.
+  auto take = [&](int c) {
+    if (next_at != c) fetch(c);
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) r[u] = next[u];
+    if (c + kChunk < hi) fetch(c + kChunk);
+    if (c + kChunk > hi || (c == 0 && skew) || c + kChunk >= total) {  // not all are the row's
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u) {
+        const int64_t v = c + u * kBeamThreads + tid, at = v * kN - skew;
+        Vec<T>::cut(r[u], v < hi ? -at : kN, a.vocab - at);
       }
     }
-    auto token_of = [&](int u, int i) {
-      return static_cast<uint32_t>((c + u * kBeamThreads + tid) * kN - skew + i);
-    };
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      if (!(level ? top[u] >= thr : top[u] > thr)) continue;
-      float f[kN];
-      Vec<T>::unpack(r[u], f);
+    for (int u = 0; u < kVecs; ++u) top[u] = Vec<T>::top(r[u]);
+    gtop = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), -INFINITY);
+  };
+  float m = -INFINITY, thr = -INFINITY;
+  double sum = 0;
+  auto absorb = [&]() {
+    if (gtop > m) {
+      sum = m == -INFINITY ? 0 : sum * exp2_approx((m - gtop) * kLog2e);
+      m = gtop;
+    }
+    if (gtop == -INFINITY) return;
+    float e = 0.f;
 #pragma unroll
-      for (int i = 0; i < kN; ++i)
-        if (level ? f[i] >= thr : f[i] > thr) {
-          const int at = atomicAdd(&s_count, 1);
-          if (at < kList) s_list[at] = key_of(f[i], token_of(u, i));
+    for (int u = 0; u < kVecs; ++u) e += exp_sum<T>(r[u], m);
+    if (!(e < INFINITY)) {  // a NaN among them
+      e = 0.f;
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u) e += exp_sum_odd<T>(r[u], m);
+    }
+    sum += e;
+  };
+  auto put_above = [&](int c, bool level) {
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+      if (level ? top[u] >= thr : top[u] > thr)
+        put_vector<T>(r[u], thr, level, (uint32_t)((c + u * kBeamThreads + tid) * kN - skew), s_list,
+                      &s_count);
+  };
+  // The list holds every logit so far that is above thr, and of those that reach it as
+  // many as `count` needs.
+  int had = 0, summed = lo, one_by_one = lo + kChunk;
+  for (int pos = lo; pos < hi;) {
+    const bool chunk = pos < one_by_one;
+    const int end = min(pos + (chunk ? kChunk : max(kChunk, (pos - lo) / kChunk * kChunk)), hi);
+    for (int c = pos; c < end; c += kChunk) {
+      take(c);
+      if (c >= summed) absorb();
+      if (!chunk && gtop > thr) put_above(c, false);
+    }
+    summed = max(summed, end);
+    if (chunk) {
+      const int busy = __syncthreads_count(gtop > thr);
+      bool level = false;
+      if (busy > 0 && (thr == -INFINITY || busy > 2 * M + 32)) {
+        const uint32_t k = reached_by(gtop == -INFINITY ? 0 : Logit<float>::key(gtop), M, s_warp);
+        const float t = k ? Logit<float>::value(k) : -INFINITY;
+        if (t > thr) {
+          thr = t;
+          level = true;
         }
+      }
+      if (level ? gtop >= thr : gtop > thr) put_above(pos, level);
     }
     __syncthreads();
-    int n = s_count;
-    if (n <= kRank) {
-      had = n;
+    const int n = s_count;
+    __syncthreads();
+    if (n > kList && !chunk) {  // once more, chunk by chunk
+      if (tid == 0) s_count = had;
+      one_by_one = end;
       continue;
     }
-    // Too many: the `count` best so far, round by round, of the list or (where it
-    // overflowed) of the list before and this chunk.
-    const bool over = n > kList;
-    if (over) n = had;
-    uint64_t last = ~0ull;
-    int found = 0;
-    for (; found < M; ++found) {
-      uint64_t best = 0;
-      for (int i = tid; i < n; i += kBeamThreads)
-        if (s_list[i] < last && s_list[i] > best) best = s_list[i];
-      if (over) {
-#pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-          if (!(top[u] >= thr)) continue;
-          float f[kN];
-          Vec<T>::unpack(r[u], f);
-#pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            const uint64_t k = f[i] > -INFINITY ? key_of(f[i], token_of(u, i)) : 0;
-            if (k < last && k > best) best = k;
-          }
+    pos = end;
+    had = n;
+    if (n <= M) continue;
+    // The `count` best so far become the list, the last of them the threshold: by counting
+    // what is above each, or round by round of a long list, and of the chunk where it overflowed.
+    if (n <= kRank) {
+      rank_all(n, [&](int j, int i) { return s_list[j] > s_list[i]; },
+               [&](int i, int above) {
+                 if (above < M) s_top[above] = s_list[i];
+               });
+    } else {
+      uint64_t last = ~0ull;
+      for (int found = 0; found < M; ++found) {
+        uint64_t best = 0;
+        for (int i = tid; i < min(n, kList); i += kBeamThreads)
+          if (s_list[i] < last && s_list[i] > best) best = s_list[i];
+        if (n > kList && gtop >= thr) {  // the chunk's logits are read again
+          const int c = end - 1 - (end - 1 - lo) % kChunk;
+#pragma unroll 1
+          for (int v = c + tid; v < end; v += kBeamThreads)
+#pragma unroll 1
+            for (int i = 0; i < kN; ++i) {
+              const int token = v * kN - skew + i;
+              if ((uint32_t)token >= (uint32_t)a.vocab) continue;
+              const float f = Logit<T>::of(x0[token]);
+              const uint64_t k = f >= thr && f > -INFINITY ? key_of(f, token) : 0;
+              if (k < last && k > best) best = k;
+            }
         }
+        last = block_best(Pick{best, 0}, s_best).hi;
+        if (tid == 0) s_top[found] = last;
       }
-      last = block_best(Pick{best, 0}, s_best).hi;
-      if (last == 0) break;
-      if (tid == 0) s_top[found] = last;
     }
     __syncthreads();
-    if (tid < found) s_list[tid] = s_top[tid];
-    if (tid == 0) s_count = found;
-    had = found;
-    if (found == M) thr = logit_of(s_top[M - 1]);
+    if (tid < M) s_list[tid] = s_top[tid];
+    if (tid == 0) s_count = M;
+    had = M;
+    thr = logit_of(s_top[M - 1]);
     __syncthreads();
   }
 
-  // This part's maximum and sum, and its list in order.
+  // This part's maximum and sum, and its list.
   {
     float top = m;
 #pragma unroll
@@ -310,12 +387,7 @@ __global__ void __launch_bounds__(kBeamThreads, 3) k_beam_select(const BeamArgs 
     if (lane == 0) s_sum[warp] = sum;
     const int n = s_count, part = row * a.splits + split;
     uint64_t* keys = a.keys + (int64_t)part * M;
-    for (int i = tid; i < n; i += kBeamThreads) {
-      const uint64_t k = s_list[i];
-      int above = 0;
-      for (int j = 0; j < n; ++j) above += s_list[j] > k;
-      if (above < M) keys[above] = k;
-    }
+    for (int i = tid; i < n; i += kBeamThreads) keys[i] = s_list[i];  // at most M, in any order
     for (int i = n + tid; i < M; i += kBeamThreads) keys[i] = 0;
     __syncthreads();
     if (tid == 0) {
@@ -334,51 +406,60 @@ __global__ void __launch_bounds__(kBeamThreads, 3) k_beam_select(const BeamArgs 
   __threadfence();
   if (tid == 0) a.done[group] = 0;
   const double2* sums = a.sums + (int64_t)group * parts;
-  if (tid < a.beams) {
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, (float)__ldcg(&sums[tid * a.splits + s].y));
-    double all = 0;
-    for (int s = 0; s < a.splits; ++s) {
-      const float of = (float)__ldcg(&sums[tid * a.splits + s].y);
-      const double part = __ldcg(&sums[tid * a.splits + s].x);
-      all += of == top ? part : part == 0 ? 0 : part * expf(of - top);
+  // A thread's first key is on its way while the sums are joined.  Each warp looks at every
+  // 8th, so that none has a poor row's alone.
+  const uint64_t* keys = a.keys + (int64_t)group * parts * M;
+  const int all = parts * M, per_beam = a.splits * M, at0 = lane * kBeamWarps + warp;
+  const uint64_t key0 = at0 < all ? __ldcg(keys + at0) : 0;
+  const float* scores = a.scores + (int64_t)group * a.beams;
+  for (int k = warp; k < a.beams; k += kBeamWarps) {  // a row's parts: at most 64
+    const double2 none = make_double2(0, -INFINITY);
+    const double2 p = lane < a.splits ? __ldcg(sums + k * a.splits + lane) : none;
+    const double2 q = lane + 32 < a.splits ? __ldcg(sums + k * a.splits + lane + 32) : none;
+    float top = fmaxf((float)p.y, (float)q.y);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+    auto part = [&](const double2& x) {
+      return (float)x.y == top ? x.x : x.x == 0 ? 0 : x.x * expf((float)x.y - top);
+    };
+    double all = part(p) + part(q);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(kAll, all, o);
+    if (lane == 0) {
+      s_rowmax[k] = top;
+      s_rowsum[k] = (float)log(all);
+      s_score[k] = scores[k];
     }
-    s_rowmax[tid] = top;
-    s_rowsum[tid] = (float)log(all);
   }
   if (tid == 0) s_count = 0;
   __syncthreads();
-  const uint64_t* keys = a.keys + (int64_t)group * parts * M;
-  const float* scores = a.scores + (int64_t)group * a.beams;
-  const int all = parts * M, per_beam = a.splits * M;
   auto score_of = [&](float x, int beam) {
     const float top = s_rowmax[beam], d = x == top ? 0.f : x - top;
-    return __fadd_rn(scores[beam], __fsub_rn(d, s_rowsum[beam]));
+    return __fadd_rn(s_score[beam], __fsub_rn(d, s_rowsum[beam]));
   };
   auto pick = [&](int i) {
-    const uint64_t k = __ldcg(keys + i);
+    const uint64_t k = i == at0 ? key0 : __ldcg(keys + i);
     if (k == 0) return Pick{0, 0};
     const int beam = i / per_beam;
     const float v = score_of(logit_of(k), beam);
     if (!(v > -INFINITY)) return Pick{0, 0};
     return Pick{(uint64_t)Logit<float>::key(v) << 32 | (0xFFFFFFFFu - beam), k};
   };
-  uint32_t limit = 0;  // scores below it are not among the best
-  if (all > kRank) {
-    uint32_t mine = 0;
-    for (int i = tid; i < all; i += kBeamThreads) mine = max(mine, (uint32_t)(pick(i).hi >> 32));
-    limit = reached_by(mine, M, s_warp);
-  }
+  // Scores below `limit` are not among the best.
+  const Pick mine = at0 < all ? pick(at0) : Pick{0, 0};
+  uint32_t best = static_cast<uint32_t>(mine.hi >> 32);
+  for (int i = at0 + kBeamThreads; i < all; i += kBeamThreads) best = max(best, (uint32_t)(pick(i).hi >> 32));
+  const uint32_t limit = reached_by(best, M, s_warp);
   Pick* list = reinterpret_cast<Pick*>(s_list);
-  for (int i = tid; i < all; i += kBeamThreads) {
-    const Pick p = pick(i);
+  for (int i = at0; i < all; i += kBeamThreads) {
+    const Pick p = i == at0 ? mine : pick(i);
     if (p.hi == 0 || (uint32_t)(p.hi >> 32) < limit) continue;
     const int at = atomicAdd(&s_count, 1);
     if (at < kRank) list[at] = p;
   }
   __syncthreads();
   const int n = s_count;
-  auto put = [&](int at, const Pick& p) {
+  auto put_out = [&](int at, const Pick& p) {
     const int beam = static_cast<int>(0xFFFFFFFFu - (uint32_t)p.hi);
     const int64_t o = (int64_t)group * M + at;
     a.out_scores[o] = p.hi ? score_of(logit_of(p.lo), beam) : -INFINITY;
@@ -386,13 +467,11 @@ __global__ void __launch_bounds__(kBeamThreads, 3) k_beam_select(const BeamArgs 
     a.out_tokens[o] = p.hi ? 0xFFFFFFFFu - (uint32_t)p.lo : 0;
   };
   if (n <= kRank) {
-    for (int i = tid; i < n; i += kBeamThreads) {
-      const Pick p = list[i];
-      int above = 0;
-      for (int j = 0; j < n; ++j) above += list[j].above(p);
-      if (above < M) put(above, p);
-    }
-    for (int i = n + tid; i < M; i += kBeamThreads) put(i, Pick{0, 0});
+    rank_all(n, [&](int j, int i) { return list[j].above(list[i]); },
+             [&](int i, int above) {
+               if (above < M) put_out(above, list[i]);
+             });
+    for (int i = n + tid; i < M; i += kBeamThreads) put_out(i, Pick{0, 0});
     return;
   }
   Pick last{~0ull, ~0ull};
@@ -403,14 +482,16 @@ __global__ void __launch_bounds__(kBeamThreads, 3) k_beam_select(const BeamArgs 
       if (last.above(p) && p.above(best)) best = p;
     }
     last = block_best(best, s_best);
-    if (tid == 0) put(at, last);
+    if (tid == 0) put_out(at, last);
   }
 }
 
+// CTAs of a row: as many as the GPU takes at once, four to an SM, but one to an SM where the rows
+// are fewer than that, each with a vector a thread at least.
 int splits_of(int64_t rows, int64_t vocab, int64_t vec) {
-  // Three CTAs an SM, each with a vector a thread at least.
-  const int64_t want = 3 * sm_count() / (rows > 0 ? rows : 1), most = ceil_div(vocab, vec * kBeamThreads);
-  const int64_t s = want < most ? want : most;
+  if (rows < 1) rows = 1;
+  const int64_t sms = sm_count(), most = ceil_div(vocab, vec * kBeamThreads);
+  const int64_t want = rows <= sms ? sms / rows : 4 * sms / rows, s = want < most ? want : most;
   return static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 

@@ -75,27 +75,30 @@ __device__ __forceinline__ int block_scan(int v, int* s_warp, int& total) {
 __global__ void __launch_bounds__(kForkThreads) k_fork_tables(const ForkArgs a) {
   extern __shared__ int s_mem[];
   __shared__ int s_warp[32], s_free[kForkThreads], s_copies, s_last;
+  __shared__ __align__(16) int s_held[kForkThreads];
   __shared__ int64_t s_cursor;
-  const int S = a.rows, tid = threadIdx.x, cols = 1 << a.col_shift;
-  int *s_par = s_mem, *s_tile = s_mem + S;
+  const int S = a.rows, tid = threadIdx.x, threads = blockDim.x, cols = 1 << a.col_shift;
+  int *s_par = s_mem, *s_old = s_mem + S, *s_tile = s_mem + 2 * S;
   pdl_trigger();
   pdl_wait();
   auto listed = [&](int g) { return g >= 0 && g < a.num_pages; };
-  for (int i = tid; i < S; i += kForkThreads) {
+  const int c0 = blockIdx.x << a.col_shift;
+  for (int i = tid; i < S; i += threads) {
     int p = a.parents[i];
+    s_old[i] = a.lengths[i];  // written by the last CTA alone, after all have read
     if (p >= S) {
       set_device_error(kErrPage);
       p = -1;
     }
     s_par[i] = max(p, -1);
   }
-  const int c0 = blockIdx.x << a.col_shift;
-  for (int e = tid; e < S << a.col_shift; e += kForkThreads) {
+#pragma unroll 4
+  for (int e = tid; e < S << a.col_shift; e += threads) {
     const int i = e >> a.col_shift, col = c0 + (e & (cols - 1));
     s_tile[e] = col < a.max_pages ? a.table[i * a.table_stride + col] : -1;
   }
   __syncthreads();
-  for (int e = tid; e < S << a.col_shift; e += kForkThreads) {
+  for (int e = tid; e < S << a.col_shift; e += threads) {
     const int i = e >> a.col_shift, c = e & (cols - 1), p = s_par[i];
     const int was = s_tile[e], is = p >= 0 ? s_tile[(p << a.col_shift) + c] : -1;
     if (is == was || c0 + c >= a.max_pages) continue;
@@ -103,23 +106,24 @@ __global__ void __launch_bounds__(kForkThreads) k_fork_tables(const ForkArgs a) 
     if (listed(was)) atomicSub(a.refs + was, 1);
     if (listed(is)) atomicAdd(a.refs + is, 1);
   }
-  __threadfence();
+  const bool alone = gridDim.x == 1;  // the whole table passes through this CTA's shared memory
+  if (!alone) __threadfence();
   __syncthreads();
   if (tid == 0) {
-    s_last = atomicAdd(a.done, 1) == gridDim.x - 1;
+    s_last = alone || atomicAdd(a.done, 1) == gridDim.x - 1;
     s_copies = 0;
     s_cursor = 0;
   }
   __syncthreads();
   if (!s_last) return;
-  __threadfence();
-  if (tid == 0) *a.done = 0;
+  if (!alone) {
+    __threadfence();
+    if (tid == 0) *a.done = 0;
+  }
 
-  int *s_old = s_tile, *s_len = s_tile + S;
   const int page = a.kv.page_size;
-  for (int i = tid; i < S; i += kForkThreads) s_old[i] = a.lengths[i];
-  __syncthreads();
-  for (int i = tid; i < S; i += kForkThreads) {
+  int* s_len = s_tile + (alone ? S << a.col_shift : 0);
+  for (int i = tid; i < S; i += threads) {
     int n = s_par[i] >= 0 ? max(s_old[s_par[i]], 0) : 0;
     if (n > a.max_pages * page) {  // no table's row holds so many
       set_device_error(kErrPage);
@@ -135,34 +139,38 @@ __global__ void __launch_bounds__(kForkThreads) k_fork_tables(const ForkArgs a) 
     return static_cast<int>(c < a.max_pages ? c : a.max_pages - 1);
   };
   const int64_t asked = (int64_t)S * a.entries;
-  for (int64_t base = 0; base < asked; base += kForkThreads) {
+  for (int64_t base = 0; base < asked; base += threads) {
     const int64_t at = base + tid;
     const int i = static_cast<int>(min(at / a.entries, (int64_t)S - 1));
     const int64_t col = first_of(i) + (at - (int64_t)i * a.entries);
     const bool use = at < asked && s_par[i] >= 0 && col <= last_of(i);
     int32_t* entry = a.table + i * a.table_stride + (use ? col : 0);
-    int g = use ? __ldcg(entry) : -1;
+    int g = -1;
+    if (use) g = alone && base == 0 ? s_tile[(s_par[i] << a.col_shift) + (int)col] : __ldcg(entry);
     if (g >= a.num_pages) {
       set_device_error(kErrPage);
       g = -1;
     }
     const int holders = use && g >= 0 ? __ldcg(a.refs + g) : 0;
-    bool copy = false;
+    // Of the rows that ask in this round and list a page, those before one leave it to
+    // it (those of earlier rounds have): the last keeps it.
+    const int held = holders > 1 ? g : -1 - tid;
+    s_held[tid] = held;
+    __syncthreads();
+    int before = __popc(__match_any_sync(0xffffffffu, held) & ((1u << (tid & 31)) - 1));
     if (holders > 1) {
-      // Of the rows that ask in this round and list g, those before this one
-      // leave it (those of earlier rounds have): the last keeps it.
-      int before = 0;
-      for (int j = static_cast<int>(base / a.entries); j < i; ++j) {
-        const int64_t e = col - first_of(j);
-        if (s_par[j] < 0 || e < 0 || col > last_of(j) || (int64_t)j * a.entries + e < base) continue;
-        before += __ldcg(a.table + j * a.table_stride + col) == g;
+      const int4* s4 = reinterpret_cast<const int4*>(s_held);
+#pragma unroll 4
+      for (int j = 0; j < (tid & ~31) / 4; ++j) {
+        const int4 v = s4[j];
+        before += (v.x == g) + (v.y == g) + (v.z == g) + (v.w == g);
       }
-      copy = holders - before > 1;
     }
+    const bool copy = holders > 1 && holders - before > 1;
     const bool need = use && (copy || g < 0);
     int wanted, found = 0;
     const int turn = block_scan(need, s_warp, wanted);
-    constexpr int kLook = 4;  // counts a thread looks at in a go
+    constexpr int kLook = 8;  // counts a thread looks at in a go
     while (found < wanted && s_cursor < a.num_pages) {
       const int64_t from = s_cursor + tid * kLook;
       int32_t r[kLook];
@@ -172,7 +180,7 @@ __global__ void __launch_bounds__(kForkThreads) k_fork_tables(const ForkArgs a) 
 #pragma unroll
       for (int u = 0; u < kLook; ++u) mine += r[u] == 0;
       int place = found + block_scan(mine, s_warp, more);
-      if (tid == 0) s_cursor += kForkThreads * kLook;
+      if (tid == 0) s_cursor += threads * kLook;
       __syncthreads();
 #pragma unroll
       for (int u = 0; u < kLook; ++u) {
@@ -208,7 +216,7 @@ __global__ void __launch_bounds__(kForkThreads) k_fork_tables(const ForkArgs a) 
 // a warp: eight 16-byte loads of a lane are in flight before the first store.
 template <int HD>
 __global__ void __launch_bounds__(kCopyThreads) k_fork_copy(const ForkArgs a) {
-  constexpr int kPieces = 8, kRows = kPieces * 32 / (HD / 8);  // positions of a warp's turn
+  constexpr int kLoads = 8, kRows = kLoads * 32 / (HD / 8);  // positions of a warp's turn
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -227,12 +235,12 @@ __global__ void __launch_bounds__(kCopyThreads) k_fork_copy(const ForkArgs a) {
     const int64_t in = ((int64_t)head * a.kv.page_size + from) * HD;
     const uint4* src = reinterpret_cast<const uint4*>(pages + job.x * stride + in);
     uint4* dst = reinterpret_cast<uint4*>(pages + job.y * stride + in);
-    uint4 r[kPieces];
+    uint4 r[kLoads];
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
+    for (int u = 0; u < kLoads; ++u)
       if (u * 32 + lane < n) r[u] = src[u * 32 + lane];
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
+    for (int u = 0; u < kLoads; ++u)
       if (u * 32 + lane < n) dst[u * 32 + lane] = r[u];
   }
 }
@@ -250,11 +258,13 @@ struct KeepArgs {
   int32_t* new_lengths;
 };
 
-constexpr int kKeepThreads = 256;
+constexpr int kKeepThreads = 256, kPieces = 2;
 
-// A thread has one 16-byte piece of a (layer, keys or values, head) row and
-// moves it for every kept node of its sequence: lists rise, so a node's place is
+// A thread has kPieces 16-byte pieces of (layer, keys or values, head) rows and
+// moves them for every kept node of its sequence: lists rise, so a node's place is
 // never read after it was written, and pieces have nothing to do with each other.
+// Bound by latency (length, list, pages, rows), so all sequences' CTAs are resident at
+// once where that is possible: 64 x 32 layers x 8 heads of 128 take 1024 CTAs.
 template <int HD>
 __global__ void __launch_bounds__(kKeepThreads) k_keep_nodes(const KeepArgs a) {
   __shared__ int4 s_move[kKeepThreads];  // source page and slot, destination page and slot
@@ -265,15 +275,21 @@ __global__ void __launch_bounds__(kKeepThreads) k_keep_nodes(const KeepArgs a) {
   const int part = blockIdx.x - b * a.parts, page = a.kv.page_size;
   const int len = a.lengths[b];
   const int32_t *list = a.keep + b * a.keep_stride, *table = a.table + b * a.table_stride;
-  // This thread's piece.
+  // This thread's pieces.
   constexpr int kPer = HD / 8;
-  const int64_t x = (int64_t)part * kKeepThreads + tid, row = x / kPer;
-  const int64_t lk = row / a.kv.kv_heads;
-  const int head = static_cast<int>(row - lk * a.kv.kv_heads), layer = static_cast<int>(lk >> 1);
-  const bool is_v = lk & 1, mine = layer < a.kv.layers;
-  uint16_t* base = (is_v ? a.kv.v + layer * a.kv.v_layer : a.kv.k + layer * a.kv.k_layer) +
-                   (int64_t)head * page * HD + x % kPer * 8;
-  const int64_t stride = is_v ? a.kv.v_page : a.kv.k_page;
+  const uint16_t* from[kPieces];
+  int64_t stride[kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int64_t x = ((int64_t)part * kPieces + i) * kKeepThreads + tid, row = x / kPer;
+    const int64_t lk = row / a.kv.kv_heads;
+    const int head = static_cast<int>(row - lk * a.kv.kv_heads), layer = static_cast<int>(lk >> 1);
+    const bool is_v = lk & 1;
+    stride[i] = is_v ? a.kv.v_page : a.kv.k_page;
+    from[i] = layer >= a.kv.layers ? nullptr
+                                   : (is_v ? a.kv.v + layer * a.kv.v_layer : a.kv.k + layer * a.kv.k_layer) +
+                                         (int64_t)head * page * HD + x % kPer * 8;
+  }
   int kept = 0;
   for (int base_j = 0; len >= 0 && base_j < a.most; base_j += kKeepThreads) {
     if (tid == 0) s_end = s_bad = kKeepThreads;
@@ -300,18 +316,25 @@ __global__ void __launch_bounds__(kKeepThreads) k_keep_nodes(const KeepArgs a) {
     if (moves) s_move[at] = move;
     __syncthreads();
     kept += end;
-    if (mine) {
-      constexpr int kAhead = 4;
-      for (int m = 0; m < n; m += kAhead) {
-        uint4 r[kAhead];
+    constexpr int kAhead = 4;
+    for (int m = 0; m < n; m += kAhead) {
+      uint4 r[kPieces][kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-          if (m + u < n)
-            r[u] = *reinterpret_cast<const uint4*>(base + s_move[m + u].x * stride + s_move[m + u].y * HD);
+      for (int u = 0; u < kAhead; ++u) {
+        if (m + u >= n) continue;
+        const int4 mv = s_move[m + u];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-          if (m + u < n)
-            *reinterpret_cast<uint4*>(base + s_move[m + u].z * stride + s_move[m + u].w * HD) = r[u];
+        for (int i = 0; i < kPieces; ++i)
+          if (from[i]) r[i][u] = *reinterpret_cast<const uint4*>(from[i] + mv.x * stride[i] + mv.y * HD);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (m + u >= n) continue;
+        const int4 mv = s_move[m + u];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+          if (from[i])
+            *reinterpret_cast<uint4*>(const_cast<uint16_t*>(from[i]) + mv.z * stride[i] + mv.w * HD) = r[i][u];
       }
     }
     __syncthreads();
@@ -344,8 +367,11 @@ template <int HD>
 int launch_fork(const ForkArgs& a, cudaStream_t s) {
   if (!once_per_device(reinterpret_cast<const void*>(&fork_attr), &fork_attr)) return MOE_ERR_CUDA;
   const int cols = 1 << a.col_shift;
-  const size_t smem = (size_t)a.rows * 4 * (1 + (cols > 2 ? cols : 2));
-  if (launch_pdl(k_fork_tables, dim3((unsigned)ceil_div(a.max_pages, cols)), dim3(kForkThreads), smem, s,
+  // A barrier of 1024 threads costs twice that of 256, and there are a dozen; a large tile
+  // wants them all the same (64 rows x 16 columns: 7.0 us with 256, 8.1 with 1024; 256 x 16: 13.6, 10.0).
+  const int threads = a.rows * cols <= 2048 && a.entries <= 2 ? 256 : kForkThreads;
+  const size_t smem = (size_t)a.rows * 4 * (3 + cols);
+  if (launch_pdl(k_fork_tables, dim3((unsigned)ceil_div(a.max_pages, cols)), dim3(threads), smem, s,
                  a) != cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
@@ -434,7 +460,8 @@ extern "C" int moe_keep_nodes(const moe_keep_nodes_args_t* args) {
   a.keep = c.keep;
   a.keep_stride = c.keep_stride;
   a.most = static_cast<int>(c.most);
-  const int64_t parts = ceil_div(2 * c.layers * c.kv.kv_heads * (c.kv.head_dim / 8), kKeepThreads);
+  const int64_t parts = ceil_div(2 * c.layers * c.kv.kv_heads * (c.kv.head_dim / 8),
+                                kPieces * kKeepThreads);
   if (parts > INT32_MAX / c.kv.seqs) return MOE_ERR_UNSUPPORTED;
   a.parts = static_cast<int>(c.most > 0 ? parts : 1);
   a.new_lengths = c.new_lengths;

@@ -120,43 +120,6 @@ __device__ __forceinline__ uint32_t instr_desc(int n, bool b_rows) {
          ((uint32_t)(kM >> 4) << 24);
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one is
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
-  return pair(exp2_approx(lo_of(x)), exp2_approx(hi_of(x)));
-}
-// 2^x of a pair in ordinary arithmetic: x = n + f with n = round(x) (adding
-// 1.5 * 2^23 leaves n in the low bits of the sum) and |f| <= 1/2, 2^f by its
-// minimax polynomial, n added to the exponent.  Coefficients: Remez exchange
-// on the relative error over [-1/2, 1/2]; degree 3 is off by at most 7.5e-5 (a
-// bf16 probability rounds by 2e-3), degree 4 by 2.6e-6 (fp16: 4.9e-4).
-// 2^n is a factor of its own, its exponent's bits from n + 127: arguments of -127
-// and below (a masked score, -inf) give 0, NaN and +inf give NaN.
-template <typename T>
-__device__ __forceinline__ uint64_t exp2_fma(uint64_t x) {
-  constexpr float kBig = 12582912.f;
-  x = pair(max_nan(lo_of(x), -127.f), max_nan(hi_of(x), -127.f));
-  const uint64_t r = add2(x, pair(kBig, kBig));
-  const uint64_t n = add2(r, pair(-kBig, -kBig));
-  const uint64_t f = fma2(n, pair(-1.f, -1.f), x);
-  uint64_t p;
-  if constexpr (T::kBf16) {
-    p = fma2(pair(0.0551716691f, 0.0551716691f), f, pair(0.242611122f, 0.242611122f));
-    p = fma2(p, f, pair(0.693260985f, 0.693260985f));
-    p = fma2(p, f, pair(0.999928074f, 0.999928074f));
-  } else {
-    p = fma2(pair(0.00957010201f, 0.00957010201f), f, pair(0.0559178603f, 0.0559178603f));
-    p = fma2(p, f, pair(0.240247448f, 0.240247448f));
-    p = fma2(p, f, pair(0.693121815f, 0.693121815f));
-    p = fma2(p, f, pair(0.999999261f, 0.999999261f));
-  }
-  const uint32_t lo = ((uint32_t)r << 23) + 0x3F800000u;
-  const uint32_t hi = ((uint32_t)(r >> 32) << 23) + 0x3F800000u;
-  return mul2(p, pair(__uint_as_float(lo), __uint_as_float(hi)));
-}
 // Of 8 pairs, those that go through exp2_fma.  With heads of 128 the tensor cores
 // (and the power limit) bound a step and it only costs: 1 x 8192 causal fp16, at the
 // full clock, 450 us with none, 454 with 1, 461 with 2, 495 with 4.  With heads of 64 a

@@ -15,8 +15,8 @@
 //     Its keys come in steps of 64.  All units' steps form one line, which is cut
 //     evenly over persistent CTAs, one to an SM; the cuts are found on the device
 //     from the lengths, so a captured graph follows them.
-//   * A CTA's pieces run through two pipelines, each with its own scores S,
-//     probabilities P (two buffers) and result O in tensor memory.  Where a unit has
+//   * A CTA's pieces run through two pipelines, each with its own scores S (two buffers, in
+//     which the probabilities P take their place) and result O in tensor memory.  Where a unit has
 //     two tiles, each has one of them and both take the same keys; a single tile they
 //     share, one taking the even and one the odd steps, and join their results at the end.
 //     warps 0-3, 4-7  softmax of pipeline 0 and 1, one thread per row: S -> registers,
@@ -53,6 +53,11 @@ constexpr float kLazy = 8.f;   // log2 of what a row's maximum may grow before O
 // fp16 probabilities, up to 2^kLazy, take 2^7 on top: 2^15 fits, normal down to 2^-21.
 template <typename T>
 constexpr float prob_shift() { return T::kBf16 ? 0.f : 7.f; }
+// Of 8 pairs of exponentials, those that go through ordinary arithmetic.
+constexpr int kFmaOf8 = 0;
+// Places of a unit's start, in steps (64 x 576, 8 nodes: a start and an end take some 5000 cycles,
+// a step 1300).
+constexpr int kStart = 5;
 // Smallest share of a CTA in steps.
 constexpr int kMinShare = 2;
 
@@ -64,9 +69,14 @@ struct Cfg {
   static constexpr uint32_t kTileQ = kHalfQ * kHalves, kTileK = kHalfK * kHalves;
   static constexpr int kStages = 8 * 2 / kHalves;  // K and V tiles in flight: 128 KB
   static constexpr uint32_t kRing = kStages * kTileK;
-  static constexpr uint32_t smem(int seqs) { return 2 * kTileQ + kRing + 1024 + (3 * seqs + 1) * 4; }
-  // TMEM columns of pipeline 0, and how much further pipeline 1's are; P twice each.
-  static constexpr uint32_t kS = 0, kS1 = kN, kP = 2 * kN, kP1 = kN, kO = 4 * kN, kO1 = HD;
+  // On its way out a softmax warp's result passes 32 rows x 64 bytes of shared memory.
+  static constexpr uint32_t kOut = 32 * 64;
+  static constexpr uint32_t smem(int seqs) {
+    return 2 * kTileQ + kRing + kSoftWarps * kOut + 1024 + (seqs + 1) * 4;
+  }
+  // TMEM columns of pipeline 0, and how much further pipeline 1's are.  S has two buffers, and
+  // P takes its step's S's place: the next step's S is computed while this one's softmax runs.
+  static constexpr uint32_t kS = 0, kS1 = 2 * kN, kO = 4 * kN, kO1 = HD;
   static_assert(kO + 2 * HD <= 512, "TMEM columns");
   // Floats of a piece: O [2 kM rows][HD], then m and l per row.
   static constexpr int kPiece = 2 * kM * (HD + 2);
@@ -92,8 +102,11 @@ struct TreeArgs {
   uint64_t wait_ns;
 };
 
+// A whole warp's wait, with one result for all lanes.  After a first look the warp sleeps in
+// hardware: with twelve warps to four schedulers those that poll slow down those that work.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
-  return mbar_poll_or(bar, parity, limit_ns, [] { set_device_error(kErrWaitTimeout); });
+  if (__all_sync(0xffffffffu, mbar_poll(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait_or(bar, parity, limit_ns, [] { set_device_error(kErrWaitTimeout); }));
 }
 // For a warp that runs it as a whole, with the same operands in every lane: issued by
 // the lane with leader != 0.  Operands that differ between lanes make each load some 150
@@ -144,50 +157,49 @@ __device__ __forceinline__ bool span(const TreeArgs& a, int b, int& len, int& ke
   return have <= a.nodes && (int64_t)n + real <= most;
 }
 
-// What shared memory knows of the sequences: prefix sums of the steps of one
-// unit, cached positions, positions with the nodes.
-struct Line {
-  const int *prefix, *len, *keys;
-};
-
-// A CTA's pieces in order: steps [s0, s1) of unit u of sequence b, which has n.
+// A CTA's pieces in order: steps [s0, s1) of unit u of sequence b, which has n.  In the
+// line a unit has kStart places before its steps: what it costs to begin and end one.
 struct Piece {
   int b, u, s0, s1, n;
-  int at, end;  // places in the line: this piece's end, the CTA's end
+  int left, end;  // places from the unit's first step to the CTA's first and last (excluded)
 
-  __device__ __forceinline__ void cut() {
-    s1 = min(n, s0 + end - at);
-    at += s1 - s0;
-  }
-  __device__ __forceinline__ bool start(const TreeArgs& a, const Line& line, int lo, int hi) {
-    at = lo;
-    end = hi;
-    if (lo < 0 || lo >= hi) return false;
-    int x = 0, y = a.kv.seqs;  // last b with prefix[b] * per_seq <= lo
-    while (y - x > 1) {
-      const int mid = (x + y) >> 1;
-      if (line.prefix[mid] * a.per_seq <= lo) x = mid;
+  // The unit that place x lies in; left, end: the CTA's places.
+  __device__ __forceinline__ void find(const TreeArgs& a, const int* prefix, int x, int lo, int hi) {
+    int low = 0, y = a.kv.seqs;  // last b with prefix[b] * per_seq <= x
+    while (y - low > 1) {
+      const int mid = (low + y) >> 1;
+      if (prefix[mid] * a.per_seq <= x) low = mid;
       else y = mid;
     }
-    b = x;
-    n = line.prefix[b + 1] - line.prefix[b];
-    const int r = lo - line.prefix[b] * a.per_seq;
-    u = r / n;
-    s0 = r - u * n;
-    cut();
-    return true;
+    b = low;
+    n = prefix[b + 1] - prefix[b] - kStart;
+    const int r = x - prefix[b] * a.per_seq;
+    u = r / (n + kStart);
+    const int first = x - r + u * (n + kStart) + kStart;
+    left = lo - first;
+    end = hi - first;
   }
-  __device__ __forceinline__ bool next(const TreeArgs& a, const Line& line) {
-    if (at >= end) return false;
-    s0 = 0;
+  __device__ __forceinline__ bool cut() {  // false: the CTA has no step of the unit
+    s0 = max(left, 0);
+    s1 = min(n, end);
+    return s0 < s1;
+  }
+  __device__ __forceinline__ bool start(const TreeArgs& a, const int* prefix, int lo, int hi) {
+    if (lo >= hi) return false;
+    find(a, prefix, lo, lo, hi);
+    return cut() || next(a, prefix);
+  }
+  __device__ __forceinline__ bool next(const TreeArgs& a, const int* prefix) {
+    left -= n + kStart;
+    end -= n + kStart;
+    if (end <= 0) return false;
     if (++u == a.per_seq) {
       u = 0;
       do ++b;
-      while (line.prefix[b + 1] == line.prefix[b]);
-      n = line.prefix[b + 1] - line.prefix[b];
+      while (prefix[b + 1] == prefix[b]);
+      n = prefix[b + 1] - prefix[b] - kStart;
     }
-    cut();
-    return true;
+    return cut();
   }
 };
 
@@ -355,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int NS = C::kStages;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t s_qfull[2], s_qempty[2], s_full[NS], s_empty[NS], s_tail,
-      s_sfull[2], s_sfree[2], s_pready[2][2], s_pvdone[2][2], s_drain[2], s_done[kSoftWarps],
+      s_sfull[2][2], s_pready[2][2], s_pvdone[2][2], s_drain[2], s_done[kSoftWarps],
       s_read[kSoftWarps], s_itfull[kItems], s_itempty[kItems];
   __shared__ Item s_item[kItems];
   __shared__ float2 s_ml[kSoftWarps][32];  // a shared tile's rows: maximum and sum of each pipeline
@@ -365,17 +377,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (saddr(smem_raw) + 1023u) & ~1023u;
   const uint32_t q_at = base, ring = base + 2 * C::kTileQ;
-  int* prefix = reinterpret_cast<int*>(smem_raw + (base - saddr(smem_raw)) + 2 * C::kTileQ + C::kRing);
-  int *s_len = prefix + a.kv.seqs + 1, *s_keys = s_len + a.kv.seqs;
-  const Line line{prefix, s_len, s_keys};
+  // Prefix sums of the steps of a unit of each sequence.
+  int* prefix = reinterpret_cast<int*>(smem_raw + (base - saddr(smem_raw)) + 2 * C::kTileQ + C::kRing +
+                                       kSoftWarps * C::kOut);
 
   if (tid == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(saddr(&s_qfull[t]), 1);
       mbar_init(saddr(&s_qempty[t]), 2);
-      mbar_init(saddr(&s_sfull[t]), 1);
-      mbar_init(saddr(&s_sfree[t]), 4);
       for (int i = 0; i < 2; ++i) {
+        mbar_init(saddr(&s_sfull[t][i]), 1);
         mbar_init(saddr(&s_pready[t][i]), 4);
         mbar_init(saddr(&s_pvdone[t][i]), 1);
       }
@@ -414,11 +425,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (b < a.kv.seqs) {
       int len, keys;
       if (!span(a, b, len, keys) && blockIdx.x == 0) set_device_error(kErrPage);
-      s_len[b] = len;
-      s_keys[b] = keys;
       steps = (keys + kN - 1) / kN;
     }
-    int inc = steps;
+    const int places = steps > 0 ? steps + kStart : 0;
+    int inc = places;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -432,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (w < warp) before += s_scan[w];
       all += s_scan[w];
     }
-    if (b < a.kv.seqs) prefix[b] = before + inc - steps;
+    if (b < a.kv.seqs) prefix[b] = before + inc - places;
     run += all;
     __syncthreads();
   }
@@ -442,10 +452,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   const int total = run * a.per_seq;
-  const int share = max((int)(((uint32_t)total + gridDim.x - 1) / gridDim.x), kMinShare);
+  const int share = max((int)(((uint32_t)total + gridDim.x - 1) / gridDim.x), kMinShare + kStart);
   const int lo = (int)min((int64_t)blockIdx.x * share, (int64_t)total), hi = (int)min((int64_t)lo + share, (int64_t)total);
-  // A sequence's nodes that are there: rows of the others are zeros.
-  auto have_of = [&](int b) { return min(s_keys[b] - s_len[b], a.nodes); };
 
   // The next item; false at the end or after a timeout (then ok is false).
   Item it;
@@ -461,21 +469,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     ++n_it;
     return it.steps > 0;
   };
+  // P V of a pipeline's step n, counted from the first.
+  const int t = warp < kSoftWarps ? warp >> 2 : warp - kMmaWarp;  // the pipeline, of softmax and MMA warps
+  auto product_done = [&](uint32_t n) {
+    return warp_wait(saddr(&s_pvdone[t][n & 1]), n >> 1 & 1, a.wait_ns);
+  };
   if (warp < kSoftWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     // ---------------- softmax: one thread per row of pipeline t ----------------
-    const int t = warp >> 2, row = (warp & 3) * 32 + lane, pal = warp ^ 4;  // pal: the same rows' other warp
+    const int row = (warp & 3) * 32 + lane, pal = warp ^ 4;  // pal: the same rows' other warp
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + C::kS + t * C::kS1 + lane_base;
-    const uint32_t p_at = tmem + C::kP + t * C::kP1 + lane_base;
     const uint32_t o_at = tmem + C::kO + t * C::kO1 + lane_base;
     const uint32_t o_pal = tmem + C::kO + (1 - t) * C::kO1 + lane_base;
     const int row_node = row / a.tile_heads, row_head = row - row_node * a.tile_heads;
     uint32_t n_s = 0, n_pair = 0;  // steps and shared tiles so far
-    // P V of step n (counted as n_s is), whose P was in buffer n & 1.
-    auto product_done = [&](uint32_t n) {
-      return warp_wait(saddr(&s_pvdone[t][n & 1]), n >> 1 & 1, a.wait_ns);
-    };
     while (next_item()) {
       const bool two = it.flags & kTwo;
       const int second = two ? t : 0;
@@ -489,19 +497,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (int i = 0; i < mine; ++i, ++n_s) {
         const int j0 = (it.s0 + (two ? i : 2 * i + t)) * kN;
-        if (!(ok = warp_wait(saddr(&s_sfull[t]), n_s & 1, a.wait_ns))) break;
+        if (!(ok = warp_wait(saddr(&s_sfull[t][n_s & 1]), n_s >> 1 & 1, a.wait_ns))) break;
         tc_fence_after();
-        uint32_t s[kN];
         if (!idle) {
-          tmem_ld32(s_at, s);
-          tmem_ld32(s_at + 32, s + 32);
+          const uint32_t sp = s_at + (n_s & 1) * kN;
+          uint32_t s[kN];
+          tmem_ld32(sp, s);
+          tmem_ld32(sp + 32, s + 32);
           tmem_wait_ld();
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(saddr(&s_sfree[t]));
-        float top = -INFINITY;
-        if (!idle) {
           if (j0 + kN > it.len) {
             const uint64_t mask = a.words == 1 ? seen_keys(sees, it.len, it.keys, j0)
                                   : real ? seen_keys(a, it.b, me.node, it.len, it.keys, j0) : 0;
@@ -516,11 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < kN; c += 2)
             mx[c / 2 & 3] = max3(mx[c / 2 & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-          top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
-        }
-        // The P buffer is free once the last product but one is done.
-        if (i >= 2 && !(ok = product_done(n_s - 2))) break;
-        if (!idle) {
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
           if (__any_sync(0xffffffffu, top > m + (m == -INFINITY ? 0.f : kLazy))) {
             const float nm = fmaxf(m, top);
             const float f = m == nm ? 1.f : exp2_approx(m - nm);
@@ -547,11 +546,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < kN; c += 2) {
             const uint64_t x = fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2, r2);
-            const uint64_t e = pair(exp2_approx(lo_of(x)), exp2_approx(hi_of(x)));
+            const uint64_t e = c / 2 % 8 < kFmaOf8 ? exp2_fma<T>(x) : exp2_mufu(x);
             sum[c / 2 & 1] = add2(sum[c / 2 & 1], e);
             p[c / 2] = T::pack(lo_of(e), hi_of(e));
           }
-          tmem_st32(p_at + (n_s & 1) * (kN / 2), p);
+          tmem_st32(sp, p);
           tmem_wait_st();
           sum[0] = add2(sum[0], sum[1]);
           l += lo_of(sum[0]) + hi_of(sum[0]);
@@ -596,8 +595,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool none = whole && real && l == 0.f && blind(a, it.b, me.node, it.len, it.keys);
       const float inv = whole ? __fdividef(1.f, l) : 1.f;
       float* piece = a.part + ((int64_t)blockIdx.x * 2 + (it.flags & kFirst ? 1 : 0)) * C::kPiece;
-      uint16_t* dst = a.out + (((int64_t)it.b * a.nodes + max(me.node, 0)) * a.heads + me.head) * HD;
-      float* dst_piece = piece + (second * kM + row) * HD;
+      // A thread has a row; stored that way every 16 bytes touch a line of their own (8 warps' rows of
+      // 128 fp32: 6 us), which is still faster for the few rows of a shared tile.  Else 64 bytes of a row at a time cross shared memory, the 16-byte pieces
+      // exchanged by the row's bits against bank conflicts, and leave as 8 rows a store.
+      const uint32_t stage = ring + C::kRing + warp * C::kOut;
+      const int place = real ? me.node * a.heads * HD + me.head * HD : -1;  // in the sequence's output
+      uint16_t* out = a.out + (int64_t)it.b * a.nodes * a.heads * HD;
+      auto leave = [&](const uint32_t* w, auto where) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 +
+                                                                        ((i ^ (lane >> 1 & 3)) << 4)),
+                       "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3])
+                       : "memory");
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + (lane >> 2);
+          uint4 x;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                       : "r"(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4))
+                       : "memory");
+          uint4* dst = where(r);
+          if (dst) *dst = x;
+        }
+      };
       float odd = 0.f;  // NaN once an element is not finite
 #pragma unroll 1
       for (int c = from; c < to; c += 32) {
@@ -612,18 +636,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           odd = fmaf(v, 0.f, odd);
           o[e] = __float_as_uint(none ? 0.f : v * inv);
         }
-        if (!whole) {
+        if (whole) {
+          uint32_t w[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4*>(dst_piece + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        } else if (real) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint32_t w[4];
+          for (int e = 0; e < 16; ++e) w[e] = T::pack(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+          if (two) {
+            leave(w, [&](int r) {
+              const int at = __shfl_sync(0xffffffffu, place, r);
+              return at < 0 ? nullptr : reinterpret_cast<uint4*>(out + at + c) + (lane & 3);
+            });
+          } else if (real) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              w[i] = T::pack(__uint_as_float(o[e + 2 * i]), __uint_as_float(o[e + 2 * i + 1]));
-            *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+              reinterpret_cast<uint4*>(out + place + c)[i] =
+                  make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          }
+        } else {
+          float* rows = piece + (second * kM + (warp & 3) * 32) * HD + c;
+          if (two) {
+            leave(o, [&](int r) { return reinterpret_cast<uint4*>(rows + r * HD) + (lane & 3); });
+            leave(o + 16, [&](int r) { return reinterpret_cast<uint4*>(rows + r * HD + 16) + (lane & 3); });
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              reinterpret_cast<uint4*>(rows + lane * HD)[i] =
+                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
         }
       }
@@ -653,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int boxes = kN / a.box, page_boxes = a.kv.page_size / a.box;
     uint32_t g = 0, n_q0 = 0, n_q1 = 0, n_tail = 0, ones = 0;
     Piece pc;
-    bool more = !is_v && pc.start(a, line, lo, hi);
+    bool more = !is_v && pc.start(a, prefix, lo, hi);
     // Describes the next piece, or the end.
     auto publish = [&]() {
       const uint32_t i = n_it % kItems;
@@ -664,8 +701,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         Item x{};
         if (more) {
           const int kp = pc.u / a.blocks, block = pc.u - kp * a.blocks;
+          int len, keys;
+          span(a, pc.b, len, keys);
           const bool two = a.nodes - block * 2 * a.tokens > a.tokens;
-          x = Item{pc.b, block * 2 * a.tokens, kp * a.tile_heads, s_len[pc.b], s_keys[pc.b], pc.s0,
+          x = Item{pc.b, block * 2 * a.tokens, kp * a.tile_heads, len, keys, pc.s0,
                    pc.s1 - pc.s0,
                    (two ? kTwo : 0) | (pc.s0 == 0 ? kFirst : 0) | (pc.s1 == pc.n ? kLast : 0) |
                        (int)(ones & 1) << 3 | kp / a.parts << 8};
@@ -675,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(saddr(&s_itfull[i]));
       }
       __syncwarp();
-      if (more) more = pc.next(a, line);
+      if (more) more = pc.next(a, prefix);
     };
     uint32_t n_mine = 0;
     auto take = [&]() {  // the first producer's own items, one described ahead
@@ -758,12 +797,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
     }
     if (is_v) {
+      auto have_of = [&](int b) {
+        int len, keys;
+        span(a, b, len, keys);
+        return keys - len;
+      };
       Piece last;
       if (lane == 0) {  // what is to be joined
         int4 job = make_int4(0, 0, 0, 0);
-        if (last.start(a, line, hi - 1, hi)) {
-          const int at = prefix[last.b] * a.per_seq + last.u * last.n, to = at + last.n;
-          if (at >= lo && to > hi) job = make_int4(last.b, last.u, (to - 1) / share - blockIdx.x + 1, have_of(last.b));
+        if (lo < hi) {
+          last.find(a, prefix, hi - 1, lo, hi);
+          // Its first step is this CTA's, its last another's.
+          if (last.left <= 0 && last.end > 0 && last.end < last.n)
+            job = make_int4(last.b, last.u, (hi - last.end + last.n - 1) / share - blockIdx.x + 1, have_of(last.b));
         }
         a.jobs[blockIdx.x] = job;
       }
@@ -778,12 +824,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- MMA issuers: one warp per pipeline ----------------
     // The whole warp walks the loop and one elected lane issues: addresses and
     // descriptors are then uniform over the warp and stay in uniform registers.
-    const int t = warp - kMmaWarp;
     const uint32_t d_qk = instr_desc<T>(kN, false), d_pv = instr_desc<T>(HD, true);
     const uint32_t leader = elect_one();
     const uint64_t desc_q = smem_desc(q_at), desc_k = smem_desc(ring);
     const uint64_t desc_v = smem_desc_mn(ring, C::kHalfK);
-    const uint32_t s_col = tmem + C::kS + t * C::kS1, p_col = tmem + C::kP + t * C::kP1;
+    const uint32_t s_col = tmem + C::kS + t * C::kS1;
     const uint32_t o_col = tmem + C::kO + t * C::kO1;
     uint32_t g = 0;               // tiles of the ring before this piece
     uint32_t n_q0 = 0, n_q1 = 0;  // uses of the Q buffers
@@ -804,44 +849,46 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = warp_wait(saddr(&s_qfull[slot]), q_turn & 1, a.wait_ns);
       if (ok && mine == 0 && lane == 0) mbar_arrive(saddr(&s_qempty[slot]));
       const uint64_t qd = desc_q + slot * (C::kTileQ >> 4);
-      for (int i = -1; i < mine && ok; ++i) {  // Q K^T of step i + 1, P V of step i
-        if (i + 1 < mine) {
-          const uint32_t j = two ? i + 1 : 2 * (i + 1) + t;
-          const uint32_t k = tile(g + (j == 0 ? 0 : 2 * j - 1));
-          // S, once the last one is read.
-          if (n_qk > 0) ok = ok && warp_wait(saddr(&s_sfree[t]), (n_qk - 1) & 1, a.wait_ns);
+      // P V of step i, then, once it has read P, Q K^T of step i + 2 into the same buffer.
+      for (int i = -2; i < mine && ok; ++i) {
+        if (i >= 0) {
+          const uint32_t j = two ? i : 2 * i + t;
+          const uint32_t v = tile(g + (j + 1 == (uint32_t)all ? 2 * all - 1 : 2 * j + 2));
+          ok = ok && warp_wait(saddr(&s_pready[t][n_pv & 1]), n_pv >> 1 & 1, a.wait_ns);
           if (!ok) break;
-          ++n_qk;
+          tc_fence_after();
+          const uint64_t vd = desc_v + v * (C::kTileK >> 4);
+          const uint32_t pc = s_col + (n_pv & 1) * kN;
+          tc_mma_ta_if(leader, o_col, pc, vd, d_pv, i == 0 ? 0 : 1);
+#pragma unroll
+          for (int kk = 1; kk < kN / 16; ++kk)
+            tc_mma_ta_if(leader, o_col, pc + kk * 8, vd + (kk * 2048 >> 4), d_pv, 1);
+          tc_commit_if(leader, saddr(&s_pvdone[t][n_pv & 1]));
+          tc_commit_if(leader, saddr(&s_empty[v]));
+          if (!two) tc_commit_if(leader, saddr(&s_empty[v]));
+          ++n_pv;
+        }
+        if (i + 2 < mine) {
+          const uint32_t j = two ? i + 2 : 2 * (i + 2) + t;
+          const uint32_t k = tile(g + (j == 0 ? 0 : 2 * j - 1));
+          if (n_qk >= 2) ok = ok && product_done(n_qk - 2);
+          if (!ok) break;
           tc_fence_after();
           const uint64_t kd = desc_k + k * (C::kTileK >> 4);
+          const uint32_t sc = s_col + (n_qk & 1) * kN;
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
-            tc_mma_if(leader, s_col, qd + ((kk / 4 * C::kHalfQ + kk % 4 * 32) >> 4),
+            tc_mma_if(leader, sc, qd + ((kk / 4 * C::kHalfQ + kk % 4 * 32) >> 4),
                       kd + ((kk / 4 * C::kHalfK + kk % 4 * 32) >> 4), d_qk, kk != 0);
-          tc_commit_if(leader, saddr(&s_sfull[t]));
+          tc_commit_if(leader, saddr(&s_sfull[t][n_qk & 1]));
           tc_commit_if(leader, saddr(&s_empty[k]));
           if (!two) tc_commit_if(leader, saddr(&s_empty[k]));
-          if (i + 2 == mine) {
+          if (i + 3 == mine) {
             tc_commit_if(leader, saddr(&s_qempty[slot]));
             if (two) tc_commit_if(leader, saddr(&s_qempty[slot]));
           }
+          ++n_qk;
         }
-        if (i < 0) continue;
-        const uint32_t j = two ? i : 2 * i + t;
-        const uint32_t v = tile(g + (j + 1 == (uint32_t)all ? 2 * all - 1 : 2 * j + 2));
-        ok = ok && warp_wait(saddr(&s_pready[t][n_pv & 1]), n_pv >> 1 & 1, a.wait_ns);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t vd = desc_v + v * (C::kTileK >> 4);
-        const uint32_t pc = p_col + (n_pv & 1) * (kN / 2);
-        tc_mma_ta_if(leader, o_col, pc, vd, d_pv, i == 0 ? 0 : 1);
-#pragma unroll
-        for (int kk = 1; kk < kN / 16; ++kk)
-          tc_mma_ta_if(leader, o_col, pc + kk * 8, vd + (kk * 2048 >> 4), d_pv, 1);
-        tc_commit_if(leader, saddr(&s_pvdone[t][n_pv & 1]));
-        tc_commit_if(leader, saddr(&s_empty[v]));
-        if (!two) tc_commit_if(leader, saddr(&s_empty[v]));
-        ++n_pv;
       }
       g += 2 * all;
     }
@@ -1064,7 +1111,7 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
   a.tokens = kM / a.tile_heads;
   a.blocks = (a.nodes + 2 * a.tokens - 1) / (2 * a.tokens);
   const int64_t per_seq = (int64_t)a.kv.kv_heads * a.parts * a.blocks;
-  const int64_t steps = ceil_div(c.kv.max_pages * c.kv.page_size, kN);
+  const int64_t steps = ceil_div(c.kv.max_pages * c.kv.page_size, kN) + kStart;
   if (per_seq > INT32_MAX || c.kv.seqs * per_seq > INT32_MAX / (steps > 0 ? steps : 1) - 4096)
     return MOE_ERR_UNSUPPORTED;
   a.per_seq = static_cast<int>(per_seq);
@@ -1095,7 +1142,7 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
   if (!make_map(&mq, c.q, bf16, q_dims, q_strides, q_box) ||
       !kv_map(&mk, c.kv.k_pages, c.kv.k_page_stride) || !kv_map(&mv, c.kv.v_pages, c.kv.v_page_stride))
     return MOE_ERR_CUDA;
-  const int64_t line = c.kv.seqs * per_seq * steps, most = ceil_div(line, kMinShare);
+  const int64_t line = c.kv.seqs * per_seq * steps, most = ceil_div(line, kMinShare + kStart);
   const int sms = sm_count(), grid = static_cast<int>(most < 1 ? 1 : most < sms ? most : sms);
   cudaStream_t s = static_cast<cudaStream_t>(c.stream);
   if (bf16)

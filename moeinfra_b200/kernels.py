@@ -987,22 +987,43 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: tor
 
 
 def _check_layers(what: str, k_pages, v_pages, block_table) -> tuple:
-    """``(layers, k layer stride, v layer stride, first layer of each)`` of caches of one layer
-    [pages, ...] or of all [layers, pages, ...], checked."""
+    """The cache's shape and strides as ``FORK_PAGES`` and ``KEEP_NODES`` take them, checked: caches of
+    one layer [pages, ...] or of all [layers, pages, ...]."""
     if not isinstance(k_pages, torch.Tensor) or k_pages.ndim not in (4, 5):
         raise ValueError(f"{what}: k_pages must be [pages, kv_heads, page_size, head_dim], or that "
                          "per layer")
     if k_pages.ndim == 4:
         _check_cache(what, k_pages, v_pages, block_table)
-        return 1, 0, 0, k_pages, v_pages
-    if not isinstance(v_pages, torch.Tensor) or v_pages.shape != k_pages.shape or not len(k_pages):
-        raise ValueError(f"{what}: v_pages must have k_pages' shape, of one layer at least")
-    k, v = k_pages[0], v_pages[0]
-    _check_cache(what, k, v, block_table)
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.shape[0] > 1 and t.stride(0) < (t.shape[1] - 1) * t.stride(1) + k[0:1].numel():
-            raise ValueError(f"{what}: {name}'s layers overlap")
-    return k_pages.shape[0], k_pages.stride(0), v_pages.stride(0), k, v
+        layers, k_layer, v_layer, k, v = 1, 0, 0, k_pages, v_pages
+    else:
+        if not isinstance(v_pages, torch.Tensor) or v_pages.shape != k_pages.shape or not len(k_pages):
+            raise ValueError(f"{what}: v_pages must have k_pages' shape, of one layer at least")
+        layers, k_layer, v_layer = k_pages.shape[0], k_pages.stride(0), v_pages.stride(0)
+        k, v = k_pages[0], v_pages[0]
+        _check_cache(what, k, v, block_table)
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            if layers > 1 and t.stride(0) < (t.shape[1] - 1) * t.stride(1) + k[0:1].numel():
+                raise ValueError(f"{what}: {name}'s layers overlap")
+    return (*k.shape, _outer_stride(k), _outer_stride(v), layers, k_layer, v_layer)
+
+
+def _layers_of(what: str, k_pages, v_pages, block_table, *int32) -> tuple:
+    """``(n_pages, kv, page, hd, k page stride, v page stride, layers, k and v layer stride)``, GPU,
+    type code, and whether the tensors ``int32`` of the call were found packed and on that GPU."""
+    try:
+        dt, dev, ndim = k_pages.dtype, k_pages.get_device(), k_pages.ndim
+        if (ndim in (4, 5) and dt in _HALVES and v_pages.shape == k_pages.shape
+                and _plain(dev, dt, k_pages, v_pages) and block_table.ndim == 2
+                and _plain(dev, torch.int32, block_table, *int32)):
+            layers = k_pages.shape[0] if ndim == 5 else 1
+            n_pages, kv, page, hd = k_pages.shape[-4:]
+            one = kv * page * hd
+            if layers and (hd == 64 or hd == 128):
+                return (n_pages, kv, page, hd, one, one, layers, n_pages * one, n_pages * one), dev, dt, True
+    except AttributeError:
+        pass
+    return (_check_layers(what, k_pages, v_pages, block_table), k_pages.get_device(), k_pages.dtype,
+            False)
 
 
 @functools.lru_cache(maxsize=None)
@@ -1136,34 +1157,39 @@ def fork_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.
     ``workspace``: :func:`fork_pages_workspace`, as for :func:`paged_attention`.
     """
     what = "fork_pages"
-    layers, k_layer, v_layer, k, v = _check_layers(what, k_pages, v_pages, block_table)
-    n_pages, kv, page, hd = k.shape
-    dev = k.get_device()
+    cache, dev, dt, plain = _layers_of(what, k_pages, v_pages, block_table, lengths, parents, refs)
     seqs, max_pages = block_table.shape
-    _serve_check(what, dev, ("lengths", lengths, torch.int32, (seqs,), 1),
-                 ("parents", parents, torch.int32, (seqs,), 1),
-                 ("refs", refs, torch.int32, (n_pages,), 1))
-    if seqs > 1 and block_table.stride(0) < max_pages:
-        raise ValueError(f"{what}: block_table's rows overlap")
+    if not (plain and lengths.shape == parents.shape == (seqs,) and refs.shape == cache[:1]):
+        _serve_check(what, dev, ("lengths", lengths, torch.int32, (seqs,), 1),
+                     ("parents", parents, torch.int32, (seqs,), 1),
+                     ("refs", refs, torch.int32, cache[:1], 1))
+        if seqs > 1 and block_table.stride(0) < max_pages:
+            raise ValueError(f"{what}: block_table's rows overlap")
     stream = _raw_stream(dev)
-    nbytes = _native.lib().moe_fork_pages_workspace_size(seqs)
+    nbytes = _fork_ws_bytes(seqs)
     if workspace is None:
         workspace = _serve_scratch(dev, stream, nbytes)
     else:
         _check_workspace(what, workspace, dev, nbytes)
+    n_pages, kv, page, hd, k_page, v_page, layers, k_layer, v_layer = cache
     status = _native.lib().moe_fork_pages(_native.FORK_PAGES.pack(
-        k.data_ptr(), v.data_ptr(), _outer_stride(k), _outer_stride(v), n_pages, kv, page, hd,
-        _DTYPE_CODES[k.dtype], block_table.data_ptr(), max(_outer_stride(block_table), max_pages),
+        k_pages.data_ptr(), v_pages.data_ptr(), k_page, v_page, n_pages, kv, page, hd, _DTYPE_CODES[dt],
+        block_table.data_ptr(), max_pages if plain else max(_outer_stride(block_table), max_pages),
         seqs, max_pages, layers, k_layer, v_layer, lengths.data_ptr(), parents.data_ptr(),
         refs.data_ptr(), room, workspace.data_ptr(), nbytes, stream))
     if status:
         check(status, "moe_fork_pages")
 
 
+@functools.lru_cache(maxsize=1024)
+def _fork_ws_bytes(seqs: int) -> int:
+    return _native.lib().moe_fork_pages_workspace_size(seqs)
+
+
 @_on_first_device
 def fork_pages_workspace(block_table: torch.Tensor) -> torch.Tensor:
     """A workspace for :func:`fork_pages` calls on tables of as many rows."""
-    nbytes = _native.lib().moe_fork_pages_workspace_size(block_table.shape[0])
+    nbytes = _fork_ws_bytes(block_table.shape[0])
     return torch.zeros(nbytes, dtype=torch.uint8, device=block_table.device)
 
 
@@ -1180,19 +1206,20 @@ def keep_nodes(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.
     :func:`check_device`.  The pages moved in must be the sequence's own (:func:`fork_pages`).
     """
     what = "keep_nodes"
-    layers, k_layer, v_layer, k, v = _check_layers(what, k_pages, v_pages, block_table)
-    n_pages, kv, page, hd = k.shape
-    dev = k.get_device()
+    cache, dev, dt, plain = _layers_of(what, k_pages, v_pages, block_table, lengths, keep)
     seqs, max_pages = block_table.shape
-    _serve_check(what, dev, ("lengths", lengths, torch.int32, (seqs,), 1),
-                 ("keep", keep, torch.int32, (seqs, None), 1))
+    if not (plain and lengths.shape == (seqs,) and keep.ndim == 2 and keep.shape[0] == seqs):
+        _serve_check(what, dev, ("lengths", lengths, torch.int32, (seqs,), 1),
+                     ("keep", keep, torch.int32, (seqs, None), 1))
+    most = keep.shape[1]
     out = lengths.new_empty(seqs)
+    n_pages, kv, page, hd, k_page, v_page, layers, k_layer, v_layer = cache
+    strides = ((max_pages, most) if plain or not seqs else (_outer_stride(block_table),
+                                                            _outer_stride(keep)))
     status = _native.lib().moe_keep_nodes(_native.KEEP_NODES.pack(
-        k.data_ptr(), v.data_ptr(), _outer_stride(k), _outer_stride(v), n_pages, kv, page, hd,
-        _DTYPE_CODES[k.dtype], block_table.data_ptr(), _outer_stride(block_table) if seqs else max_pages,
-        seqs, max_pages, layers, k_layer, v_layer, lengths.data_ptr(), keep.data_ptr(),
-        _outer_stride(keep) if seqs else keep.shape[1], keep.shape[1], out.data_ptr(),
-        _raw_stream(dev)))
+        k_pages.data_ptr(), v_pages.data_ptr(), k_page, v_page, n_pages, kv, page, hd, _DTYPE_CODES[dt],
+        block_table.data_ptr(), strides[0], seqs, max_pages, layers, k_layer, v_layer,
+        lengths.data_ptr(), keep.data_ptr(), strides[1], most, out.data_ptr(), _raw_stream(dev)))
     if status:
         check(status, "moe_keep_nodes")
     return out
