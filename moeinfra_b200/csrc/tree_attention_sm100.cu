@@ -833,11 +833,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t g = 0;               // tiles of the ring before this piece
     uint32_t n_q0 = 0, n_q1 = 0;  // uses of the Q buffers
     uint32_t n_qk = 0, n_pv = 0;
-    auto tile = [&](uint32_t x) {  // waits for tile x of the ring; its slot
-      ok = ok && warp_wait(saddr(&s_full[x % NS]), x / NS & 1, a.wait_ns);
+    uint32_t seen = 0;            // tiles of the ring that this warp has waited for
+    // Tile x of the ring, of a piece of `all` steps: its slot, once it is there.  A warp waits for
+    // every tile before it too, in order, and releases those that the other pipeline alone
+    // uses: a barrier's parity says no more than whether one phase is over, so a warp that
+    // skipped tiles could take an older phase of a slot for the one it wants.
+    auto tile = [&](uint32_t x, uint32_t all, bool two) {
+      while (ok && seen <= x) {
+        const uint32_t s = seen % NS, r = seen - g;
+        ok = warp_wait(saddr(&s_full[s]), seen / NS & 1, a.wait_ns);
+        const uint32_t j = r == 0 ? 0 : r == 2 * all - 1 ? all - 1 : r & 1 ? (r + 1) / 2 : r / 2 - 1;
+        if (!two && (int)(j & 1) != t && ok && lane == 0) mbar_arrive(saddr(&s_empty[s]));
+        ++seen;
+      }
       return x % NS;
     };
-    // A slot, like a Q buffer, counts two releases: of each pipeline, or of the only one twice.
+    // A slot, like a Q buffer, counts two releases: one of each pipeline.
     while (ok && next_item()) {
       const int flags = __shfl_sync(0xffffffffu, it.flags, 0);
       const int all = __shfl_sync(0xffffffffu, it.steps, 0);
@@ -853,7 +864,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = -2; i < mine && ok; ++i) {
         if (i >= 0) {
           const uint32_t j = two ? i : 2 * i + t;
-          const uint32_t v = tile(g + (j + 1 == (uint32_t)all ? 2 * all - 1 : 2 * j + 2));
+          const uint32_t v = tile(g + (j + 1 == (uint32_t)all ? 2 * all - 1 : 2 * j + 2), all, two);
           ok = ok && warp_wait(saddr(&s_pready[t][n_pv & 1]), n_pv >> 1 & 1, a.wait_ns);
           if (!ok) break;
           tc_fence_after();
@@ -865,12 +876,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_mma_ta_if(leader, o_col, pc + kk * 8, vd + (kk * 2048 >> 4), d_pv, 1);
           tc_commit_if(leader, saddr(&s_pvdone[t][n_pv & 1]));
           tc_commit_if(leader, saddr(&s_empty[v]));
-          if (!two) tc_commit_if(leader, saddr(&s_empty[v]));
           ++n_pv;
         }
         if (i + 2 < mine) {
           const uint32_t j = two ? i + 2 : 2 * (i + 2) + t;
-          const uint32_t k = tile(g + (j == 0 ? 0 : 2 * j - 1));
+          const uint32_t k = tile(g + (j == 0 ? 0 : 2 * j - 1), all, two);
           if (n_qk >= 2) ok = ok && product_done(n_qk - 2);
           if (!ok) break;
           tc_fence_after();
@@ -882,7 +892,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                       kd + ((kk / 4 * C::kHalfK + kk % 4 * 32) >> 4), d_qk, kk != 0);
           tc_commit_if(leader, saddr(&s_sfull[t][n_qk & 1]));
           tc_commit_if(leader, saddr(&s_empty[k]));
-          if (!two) tc_commit_if(leader, saddr(&s_empty[k]));
           if (i + 3 == mine) {
             tc_commit_if(leader, saddr(&s_qempty[slot]));
             if (two) tc_commit_if(leader, saddr(&s_qempty[slot]));
@@ -890,14 +899,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++n_qk;
         }
       }
+      tile(g + 2 * all - 1, all, two);
       g += 2 * all;
     }
     if (!ok) s_abort = 1;
-    // After a timeout, wait (bounded) for the MMAs already issued.
-    if (__any_sync(0xffffffffu, s_abort)) {
-      tc_commit_if(leader, saddr(&s_drain[t]));
-      warp_wait(saddr(&s_drain[t]), 0, a.wait_ns);
-    }
+    // What was issued is over before the CTA ends, after a timeout too.
+    tc_commit_if(leader, saddr(&s_drain[t]));
+    warp_wait(saddr(&s_drain[t]), 0, a.wait_ns);
   }
   }
   tc_fence_before();
