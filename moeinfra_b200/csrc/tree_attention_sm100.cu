@@ -830,24 +830,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t desc_v = smem_desc_mn(ring, C::kHalfK);
     const uint32_t s_col = tmem + C::kS + t * C::kS1;
     const uint32_t o_col = tmem + C::kO + t * C::kO1;
-    uint32_t g = 0;               // tiles of the ring before this piece
-    uint32_t n_q0 = 0, n_q1 = 0;  // uses of the Q buffers
+    uint32_t ring_slot = 0, ring_turn = 0;  // of the ring's next tile, and the parity of its barrier
+    uint32_t n_q0 = 0, n_q1 = 0;            // uses of the Q buffers
     uint32_t n_qk = 0, n_pv = 0;
-    uint32_t seen = 0;            // tiles of the ring that this warp has waited for
-    // Tile x of the ring, of a piece of `all` steps: its slot, once it is there.  A warp waits for
-    // every tile before it too, in order, and releases those that the other pipeline alone
-    // uses: a barrier's parity says no more than whether one phase is over, so a warp that
-    // skipped tiles could take an older phase of a slot for the one it wants.
-    auto tile = [&](uint32_t x, uint32_t all, bool two) {
-      while (ok && seen <= x) {
-        const uint32_t s = seen % NS, r = seen - g;
-        ok = warp_wait(saddr(&s_full[s]), seen / NS & 1, a.wait_ns);
-        const uint32_t j = r == 0 ? 0 : r == 2 * all - 1 ? all - 1 : r & 1 ? (r + 1) / 2 : r / 2 - 1;
-        if (!two && (int)(j & 1) != t && ok && lane == 0) mbar_arrive(saddr(&s_empty[s]));
-        ++seen;
-      }
-      return x % NS;
-    };
     // A slot, like a Q buffer, counts two releases: one of each pipeline.
     while (ok && next_item()) {
       const int flags = __shfl_sync(0xffffffffu, it.flags, 0);
@@ -860,47 +845,58 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = warp_wait(saddr(&s_qfull[slot]), q_turn & 1, a.wait_ns);
       if (ok && mine == 0 && lane == 0) mbar_arrive(saddr(&s_qempty[slot]));
       const uint64_t qd = desc_q + slot * (C::kTileQ >> 4);
-      // P V of step i, then, once it has read P, Q K^T of step i + 2 into the same buffer.
-      for (int i = -2; i < mine && ok; ++i) {
-        if (i >= 0) {
-          const uint32_t j = two ? i : 2 * i + t;
-          const uint32_t v = tile(g + (j + 1 == (uint32_t)all ? 2 * all - 1 : 2 * j + 2), all, two);
-          ok = ok && warp_wait(saddr(&s_pready[t][n_pv & 1]), n_pv >> 1 & 1, a.wait_ns);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t vd = desc_v + v * (C::kTileK >> 4);
-          const uint32_t pc = s_col + (n_pv & 1) * kN;
-          tc_mma_ta_if(leader, o_col, pc, vd, d_pv, i == 0 ? 0 : 1);
-#pragma unroll
-          for (int kk = 1; kk < kN / 16; ++kk)
-            tc_mma_ta_if(leader, o_col, pc + kk * 8, vd + (kk * 2048 >> 4), d_pv, 1);
-          tc_commit_if(leader, saddr(&s_pvdone[t][n_pv & 1]));
-          tc_commit_if(leader, saddr(&s_empty[v]));
-          ++n_pv;
+      // The piece's tiles in the ring's order: K(0), then K(j + 1), V(j).  A warp waits for all of
+      // them and releases those that the other pipeline alone uses: a barrier's parity tells one
+      // phase from the next only, so a warp that skipped tiles could take an older phase of a
+      // slot for the one it wants.
+      int j_k = 0, j_v = 0, qk_left = mine;
+      bool first = true;
+      for (int r = 0; r < 2 * all && ok; ++r) {
+        const bool is_k = j_k < all && (r == 0 || (r & 1));
+        const int j = is_k ? j_k++ : j_v++;
+        const uint32_t at = ring_slot;
+        ok = warp_wait(saddr(&s_full[at]), ring_turn, a.wait_ns);
+        if (++ring_slot == NS) {
+          ring_slot = 0;
+          ring_turn ^= 1;
         }
-        if (i + 2 < mine) {
-          const uint32_t j = two ? i + 2 : 2 * (i + 2) + t;
-          const uint32_t k = tile(g + (j == 0 ? 0 : 2 * j - 1), all, two);
-          if (n_qk >= 2) ok = ok && product_done(n_qk - 2);
+        if (!ok) break;
+        if (!two && (j & 1) != t) {
+          if (lane == 0) mbar_arrive(saddr(&s_empty[at]));
+          continue;
+        }
+        if (is_k) {  // Q K^T, into the buffer whose P the last product but one has read
+          if (n_qk >= 2) ok = product_done(n_qk - 2);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t kd = desc_k + k * (C::kTileK >> 4);
+          const uint64_t kd = desc_k + at * (C::kTileK >> 4);
           const uint32_t sc = s_col + (n_qk & 1) * kN;
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
             tc_mma_if(leader, sc, qd + ((kk / 4 * C::kHalfQ + kk % 4 * 32) >> 4),
                       kd + ((kk / 4 * C::kHalfK + kk % 4 * 32) >> 4), d_qk, kk != 0);
           tc_commit_if(leader, saddr(&s_sfull[t][n_qk & 1]));
-          tc_commit_if(leader, saddr(&s_empty[k]));
-          if (i + 3 == mine) {
+          if (--qk_left == 0) {
             tc_commit_if(leader, saddr(&s_qempty[slot]));
             if (two) tc_commit_if(leader, saddr(&s_qempty[slot]));
           }
           ++n_qk;
+        } else {
+          ok = warp_wait(saddr(&s_pready[t][n_pv & 1]), n_pv >> 1 & 1, a.wait_ns);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t vd = desc_v + at * (C::kTileK >> 4);
+          const uint32_t pc = s_col + (n_pv & 1) * kN;
+          tc_mma_ta_if(leader, o_col, pc, vd, d_pv, first ? 0 : 1);
+#pragma unroll
+          for (int kk = 1; kk < kN / 16; ++kk)
+            tc_mma_ta_if(leader, o_col, pc + kk * 8, vd + (kk * 2048 >> 4), d_pv, 1);
+          tc_commit_if(leader, saddr(&s_pvdone[t][n_pv & 1]));
+          first = false;
+          ++n_pv;
         }
+        tc_commit_if(leader, saddr(&s_empty[at]));
       }
-      tile(g + 2 * all - 1, all, two);
-      g += 2 * all;
     }
     if (!ok) s_abort = 1;
     // What was issued is over before the CTA ends, after a timeout too.
