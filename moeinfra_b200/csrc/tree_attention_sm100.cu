@@ -32,8 +32,8 @@
 // in use: probabilities stay below 2^8, O and l are sums of the same factor.
 // Every wait is bounded: on a timeout the error word is set, the roles stop, and
 // the CTA waits (bounded) for what it issued before it frees its tensor memory.
-#include "paged.cuh"
 #include "sm100_ptx.cuh"
+#include "tree.cuh"
 
 namespace moe {
 namespace {
@@ -53,8 +53,6 @@ constexpr float kLazy = 8.f;   // log2 of what a row's maximum may grow before O
 // fp16 probabilities, up to 2^kLazy, take 2^7 on top: 2^15 fits, normal down to 2^-21.
 template <typename T>
 constexpr float prob_shift() { return T::kBf16 ? 0.f : 7.f; }
-// Of 8 pairs of exponentials, those that go through ordinary arithmetic.
-constexpr int kFmaOf8 = 0;
 // Places of a unit's start, in steps (64 x 576, 8 nodes: a start and an end take some 5000 cycles,
 // a step 1300).
 constexpr int kStart = 5;
@@ -82,21 +80,12 @@ struct Cfg {
   static constexpr int kPiece = 2 * kM * (HD + 2);
 };
 
-struct TreeArgs {
-  KvPages kv;
-  const uint16_t* q;
-  int64_t q_seq, q_node;        // elements from one sequence's (node's) queries to the next
-  uint16_t* out;                // [seqs, nodes, heads, HD]
-  const int32_t *lengths, *counts;
-  const uint64_t* visible;      // [seqs, nodes, words]
-  int64_t vis_seq, vis_node;
-  int nodes, words, heads, group;
+struct TreeArgs : TreeRows {
   int parts, tile_heads;        // a group's heads in tiles: parts x tile_heads
   int tokens;                   // nodes of a tile
   int blocks;                   // blocks of rows (two tiles) of a KV head's part
   int per_seq;                  // units of a sequence
   int box;                      // rows of a K or V box: they lie in one page
-  float scale_log2;
   int4* jobs;                   // [CTAs]: sequence, unit, CTAs and nodes of the cut unit that starts there
   float* part;                  // [CTAs][2] pieces: 0 of a unit that starts before, 1 of one that goes on
   uint64_t wait_ns;
@@ -134,29 +123,6 @@ __device__ __forceinline__ uint32_t instr_desc(int n, bool b_rows) {
   return (1u << 4) | ab | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(kM >> 4) << 24);
 }
-// acc + 0 * v for two 16-bit values: NaN once one was infinite or NaN, else +0.
-template <typename T>
-__device__ __forceinline__ uint32_t trace_odd(uint32_t v, uint32_t acc) {
-  if constexpr (T::kBf16)
-    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0));
-  else
-    asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0));
-  return acc;
-}
-
-// A sequence's cached positions, and those with its nodes; false if out of range.  No
-// sequence, or none of its nodes there: no keys, nothing to compute.
-__device__ __forceinline__ bool span(const TreeArgs& a, int b, int& len, int& keys) {
-  const int64_t most = (int64_t)a.kv.max_pages * a.kv.page_size;
-  const int n = a.lengths[b], have = a.counts ? a.counts[b] : a.nodes;
-  const int real = min(have, a.nodes);
-  len = keys = 0;
-  if (n < 0 || real <= 0) return have <= a.nodes;
-  keys = static_cast<int>(min((int64_t)n + real, most));
-  len = min(n, keys);
-  return have <= a.nodes && (int64_t)n + real <= most;
-}
-
 // A CTA's pieces in order: steps [s0, s1) of unit u of sequence b, which has n.  In the
 // line a unit has kStart places before its steps: what it costs to begin and end one.
 struct Piece {
@@ -217,6 +183,9 @@ constexpr int kFirst = 2;  // the unit starts with this piece
 constexpr int kLast = 4;   // and ends with it
 constexpr int kItems = 4;  // described ahead
 constexpr int kReaders = 11;
+// How many steps a piece's keys are ahead of its values: one of a pipeline's own, so that its next
+// scores are on their way during a softmax.
+__device__ __forceinline__ int lead_of(bool two) { return two ? 1 : 2; }
 
 // A row of a unit: its node and head; node < 0: no row.
 struct Row {
@@ -231,133 +200,6 @@ __device__ __forceinline__ Row row_of(const TreeArgs& a, int u, int second, int 
   if (in >= a.tokens || w.node >= have) w.node = -1;
   return w;
 }
-// Which of the 64 keys from j0 on a node sees.
-__device__ __forceinline__ uint64_t seen_keys(const TreeArgs& a, int b, int node, int len, int keys,
-                                              int j0) {
-  uint64_t mask = ~0ull;
-  const int off = len - j0;  // keys of the cache among them
-  if (off < 64) {
-    const uint64_t* w = a.visible + b * a.vis_seq + node * a.vis_node;
-    const int i0 = off > 0 ? 0 : -off, word = i0 >> 6, sh = i0 & 63;
-    mask = word < a.words ? w[word] >> sh : 0;
-    if (sh && word + 1 < a.words) mask |= w[word + 1] << (64 - sh);
-    if (off > 0) mask = mask << off | ((1ull << off) - 1);
-  }
-  const int real = keys - j0;
-  return real >= 64 ? mask : real <= 0 ? 0 : mask & ((1ull << real) - 1);
-}
-
-// The same for trees of up to 64 nodes, whose word w is at hand.
-__device__ __forceinline__ uint64_t seen_keys(uint64_t w, int len, int keys, int j0) {
-  const int off = len - j0, real = keys - j0;
-  const uint64_t mask = off >= 64 ? ~0ull : off > 0 ? w << off | ((1ull << off) - 1) : off > -64 ? w >> -off : 0;
-  return real >= 64 ? mask : real <= 0 ? 0 : mask & ((1ull << real) - 1);
-}
-
-// Whether a node sees no key at all.
-__device__ __forceinline__ bool blind(const TreeArgs& a, int b, int node, int len, int keys) {
-  bool none = len == 0;
-  for (int j = 0; j < keys && none; j += 64) none = seen_keys(a, b, node, len, keys, j) == 0;
-  return none;
-}
-
-__device__ __forceinline__ int64_t page_at(const TreeArgs& a, int b, int entry) {
-  const int64_t page = entry < a.kv.max_pages ? a.kv.table[b * a.kv.table_stride + entry] : -1;
-  if (page >= 0 && page < a.kv.num_pages) return page;
-  set_device_error(kErrPage);
-  return 0;
-}
-
-// One row by the formula, by one warp: 32 keys a step, one to a lane, then the
-// values of those that the node sees, HD / 32 dims to a lane; dims [from, to) are written.  For rows that met an
-// infinity or NaN among the values of a node they do not see (a probability of 0
-// does not silence it).  131072 keys take some 10 ms; the other warps' waits end after 2 s.
-template <typename T, int HD>
-__device__ __noinline__ void redo_row(const TreeArgs& a, int b, int node, int head, int len, int keys,
-                                      int from, int to) {
-  constexpr int kWords = HD / 64;
-  const int lane = threadIdx.x & 31, kv_head = head / a.group, page = a.kv.page_size;
-  const uint16_t* q = a.q + b * a.q_seq + node * a.q_node + head * HD;
-  float m = -INFINITY, l = 0.f;
-  float2 acc[kWords] = {};
-  for (int j0 = 0; j0 < keys; j0 += 32) {
-    const int j = j0 + lane;
-    const bool sees = seen_keys(a, b, node, len, keys, j0) >> lane & 1;
-    int64_t row_v = 0;
-    float s = -INFINITY;
-    if (sees) {
-      const int64_t p = page_at(a, b, j / page), in = ((int64_t)kv_head * page + j % page) * HD;
-      const uint16_t* k = a.kv.k + p * a.kv.k_stride + in;
-      row_v = p * a.kv.v_stride + in;
-      s = 0.f;
-#pragma unroll 4
-      for (int d = 0; d < HD; d += 8) {
-        const uint4 ks = *reinterpret_cast<const uint4*>(k + d);
-        const uint4 qs = *reinterpret_cast<const uint4*>(q + d);
-        const uint32_t kw[4] = {ks.x, ks.y, ks.z, ks.w}, qw[4] = {qs.x, qs.y, qs.z, qs.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 x = T::unpack(qw[i]), y = T::unpack(kw[i]);
-          s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
-        }
-      }
-      s *= a.scale_log2;
-    }
-    float top = s;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float nm = fmaxf(m, top), f = m == nm ? 1.f : exp2_approx(m - nm);
-    m = nm;
-    const float p = exp2_approx(s - (nm == -INFINITY ? 0.f : nm));
-    l = l * f + warp_sum(p);
-#pragma unroll
-    for (int w = 0; w < kWords; ++w) acc[w] = make_float2(acc[w].x * f, acc[w].y * f);
-    uint32_t todo = __ballot_sync(0xffffffffu, sees);
-    while (todo) {
-      const int i = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const float pi = __shfl_sync(0xffffffffu, p, i);
-      const uint16_t* v = a.kv.v + __shfl_sync(0xffffffffu, row_v, i);
-#pragma unroll
-      for (int w = 0; w < kWords; ++w) {
-        const float2 x = T::unpack(*reinterpret_cast<const uint32_t*>(v + w * 64 + lane * 2));
-        acc[w] = make_float2(fmaf(pi, x.x, acc[w].x), fmaf(pi, x.y, acc[w].y));
-      }
-    }
-  }
-  const float inv = 1.f / l;
-  uint16_t* out = a.out + (((int64_t)b * a.nodes + node) * a.heads + head) * HD;
-#pragma unroll
-  for (int w = 0; w < kWords; ++w)
-    if (w * 64 + lane * 2 >= from && w * 64 + lane * 2 < to)
-      *reinterpret_cast<uint32_t*>(out + w * 64 + lane * 2) = T::pack(acc[w].x * inv, acc[w].y * inv);
-}
-
-// A warp's rows whose result is not finite (odd): computed again where a value of a
-// node that the row does not see is not.
-template <typename T, int HD>
-__device__ __noinline__ void mend_rows(const TreeArgs& a, uint32_t odd, int b, Row mine, int len,
-                                       int keys, int from, int to) {
-  const int lane = threadIdx.x & 31, page = a.kv.page_size;
-  __syncwarp();
-  while (odd) {
-    const int r = __ffs(odd) - 1;
-    odd &= odd - 1;
-    const int node = __shfl_sync(0xffffffffu, mine.node, r);
-    const int head = __shfl_sync(0xffffffffu, mine.head, r);
-    uint32_t met = 0;
-    for (int j = len; j < keys; ++j) {
-      if (seen_keys(a, b, node, len, keys, j) & 1) continue;
-      const uint16_t* v = a.kv.v + page_at(a, b, j / page) * a.kv.v_stride +
-                          ((int64_t)(head / a.group) * page + j % page) * HD;
-#pragma unroll
-      for (int w = 0; w < HD / 64; ++w)
-        met = trace_odd<T>(*reinterpret_cast<const uint32_t*>(v + w * 64 + lane * 2), met);
-    }
-    if (__any_sync(0xffffffffu, met)) redo_row<T, HD>(a, b, node, head, len, keys, from, to);
-  }
-}
-
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     k_tree_attention(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap map_q,
@@ -546,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int c = 0; c < kN; c += 2) {
             const uint64_t x = fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2, r2);
-            const uint64_t e = c / 2 % 8 < kFmaOf8 ? exp2_fma<T>(x) : exp2_mufu(x);
+            const uint64_t e = exp2_mufu(x);
             sum[c / 2 & 1] = add2(sum[c / 2 & 1], e);
             p[c / 2] = T::pack(lo_of(e), hi_of(e));
           }
@@ -596,8 +438,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = whole ? __fdividef(1.f, l) : 1.f;
       float* piece = a.part + ((int64_t)blockIdx.x * 2 + (it.flags & kFirst ? 1 : 0)) * C::kPiece;
       // A thread has a row; stored that way every 16 bytes touch a line of their own (8 warps' rows of
-      // 128 fp32: 6 us), which is still faster for the few rows of a shared tile.  Else 64 bytes of a row at a time cross shared memory, the 16-byte pieces
-      // exchanged by the row's bits against bank conflicts, and leave as 8 rows a store.
+      // 128 fp32: 6 us), which is still faster for the few rows of a shared tile.  Else 64 bytes of
+      // a row at a time cross shared memory, the 16-byte pieces exchanged by the row's bits against
+      // bank conflicts, and leave as 8 rows a store.
       const uint32_t stage = ring + C::kRing + warp * C::kOut;
       const int place = real ? me.node * a.heads * HD + me.head * HD : -1;  // in the sequence's output
       uint16_t* out = a.out + (int64_t)it.b * a.nodes * a.heads * HD;
@@ -675,15 +518,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = warp_wait(saddr(&s_read[pal]), n_pair++ & 1, a.wait_ns))) break;
         tc_fence_after();
       }
-      const uint32_t again = __ballot_sync(0xffffffffu, whole && real && !none && odd != 0.f);
-      if (again) mend_rows<T, HD>(a, again, it.b, me, it.len, it.keys, from, to);
+      uint32_t again = __ballot_sync(0xffffffffu, whole && real && !none && odd != 0.f);
+      for (; again; again &= again - 1) {
+        const int r = __ffs(again) - 1;
+        mend_row<T, HD>(a, it.b, __shfl_sync(0xffffffffu, me.node, r),
+                        __shfl_sync(0xffffffffu, me.head, r), it.len, it.keys, from, to);
+      }
     }
     if (!ok) s_abort = 1;
   } else {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == kKeyWarp || warp == kValueWarp) {
     // ---------------- TMA producers: Q and K, or V ----------------
-    // Tiles of a piece stand in the ring in the order of their use: K(0), then K(j + 1), V(j).
+    // Tiles of a piece stand in the ring in the order of their use: K(0) .. K(lead - 1), then
+    // K(j + lead), V(j).
     const bool is_v = warp == kValueWarp;
     const CUtensorMap* map = is_v ? &map_v : &map_k;
     const uint32_t leader = elect_one();
@@ -731,10 +579,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int flags = __shfl_sync(0xffffffffu, it.flags, 0), seq = __shfl_sync(0xffffffffu, it.b, 0);
       const int s0 = __shfl_sync(0xffffffffu, it.s0, 0), all = __shfl_sync(0xffffffffu, it.steps, 0);
       const int keys = __shfl_sync(0xffffffffu, it.keys, 0), kv_head = flags >> 8;
+      const int lead = lead_of(flags & kTwo);
       // Places of 32 boxes of the sequence from w_base on, one per lane, and pages of the 32
       // after them.
       auto look = [&](int x) -> int {  // the page of box x
-        return x * a.box < keys ? (int)page_at(a, seq, x / page_boxes) : 0;
+        if (x * a.box >= keys) return 0;
+        const int entry = x / page_boxes;
+        const int64_t page = entry < a.kv.max_pages ? a.kv.table[seq * a.kv.table_stride + entry] : -1;
+        if (page >= 0 && page < a.kv.num_pages) return (int)page;
+        set_device_error(kErrPage);
+        return 0;
       };
       int w_base = s0 * boxes / 32 * 32;
       int w_page = look(w_base + lane), w_next = look(w_base + 32 + lane);
@@ -753,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok || __any_sync(0xffffffffu, s_abort)) break;
       for (int i = 0; i < all; ++i) {
-        const uint32_t x = g + (is_v ? (i + 1 == all ? 2 * all - 1 : 2 * i + 2) : i == 0 ? 0 : 2 * i - 1);
+        const uint32_t x = g + (is_v ? (i + lead < all ? 2 * i + lead + 1 : all + i) : i < lead ? i : 2 * i - lead);
         const uint32_t s = x % NS, dst = ring + s * C::kTileK;
         const int from = (s0 + i) * boxes - w_base;
         if (from >= 32) {
@@ -838,21 +692,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int flags = __shfl_sync(0xffffffffu, it.flags, 0);
       const int all = __shfl_sync(0xffffffffu, it.steps, 0);
       const bool two = flags & kTwo;
-      const int mine = two ? all : (all + 1 - t) >> 1, slot = two ? t : flags >> 3 & 1;
+      const int lead = lead_of(two), mine = two ? all : (all + 1 - t) >> 1, slot = two ? t : flags >> 3 & 1;
       const uint32_t q_turn = slot ? n_q1 : n_q0;
       n_q0 += two || slot == 0;
       n_q1 += two || slot == 1;
       ok = warp_wait(saddr(&s_qfull[slot]), q_turn & 1, a.wait_ns);
       if (ok && mine == 0 && lane == 0) mbar_arrive(saddr(&s_qempty[slot]));
       const uint64_t qd = desc_q + slot * (C::kTileQ >> 4);
-      // The piece's tiles in the ring's order: K(0), then K(j + 1), V(j).  A warp waits for all of
+      // The piece's tiles in the ring's order (see the producers).  A warp waits for all of
       // them and releases those that the other pipeline alone uses: a barrier's parity tells one
       // phase from the next only, so a warp that skipped tiles could take an older phase of a
       // slot for the one it wants.
       int j_k = 0, j_v = 0, qk_left = mine;
       bool first = true;
       for (int r = 0; r < 2 * all && ok; ++r) {
-        const bool is_k = j_k < all && (r == 0 || (r & 1));
+        const bool is_k = j_k < all && (r <= lead || !(r - lead & 1));
         const int j = is_k ? j_k++ : j_v++;
         const uint32_t at = ring_slot;
         ok = warp_wait(saddr(&s_full[at]), ring_turn, a.wait_ns);
@@ -1003,7 +857,7 @@ __device__ __forceinline__ void join_rows(const TreeArgs& a, int4 job) {
         *dst = o[0];
       if (__any_sync(0xffffffffu, odd != 0.f) && !none) {
         span(a, b, len, keys);
-        mend_rows<T, HD>(a, 1, b, me[i], len, keys, 0, HD);
+        mend_row<T, HD>(a, b, me[i].node, me[i].head, len, keys, 0, HD);
       }
     }
   }
@@ -1067,7 +921,8 @@ constexpr int64_t kJobsAt = 4096;  // behind the counters of the calls that shar
 extern "C" size_t moe_tree_attention_workspace_size(int64_t head_dim) {
   using namespace moe;
   if (head_dim != 64 && head_dim != 128) return 0;
-  return kJobsAt + (size_t)sm_count() * 16 + (size_t)sm_count() * 2 * 4 * (head_dim == 64 ? Cfg<64>::kPiece : Cfg<128>::kPiece);
+  return kJobsAt + (size_t)sm_count() * 16 +
+         (size_t)sm_count() * 2 * 4 * (head_dim == 64 ? Cfg<64>::kPiece : Cfg<128>::kPiece);
 }
 
 extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
@@ -1107,6 +962,13 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
   a.words = (a.nodes + 63) / 64;
   a.heads = static_cast<int>(c.heads);
   a.group = a.heads / a.kv.kv_heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  const size_t need = moe_tree_attention_workspace_size(hd);
+  if (!c.workspace || c.workspace_bytes < (int64_t)need) return MOE_ERR_WORKSPACE;
+  if (!aligned16(c.workspace)) return MOE_ERR_ALIGNMENT;
+  cudaStream_t s = static_cast<cudaStream_t>(c.stream);
+  const bool bf16 = c.kv.dtype == MOE_DTYPE_BF16;
+  if (tree_is_few(a)) return tree_attention_few(a, static_cast<int>(hd), bf16, s);
   // A tile's rows are the heads of a group for neighbouring nodes; a group above 128
   // heads is cut.
   a.parts = (a.group + kM - 1) / kM;
@@ -1121,14 +983,9 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
   a.per_seq = static_cast<int>(per_seq);
   a.box = 16;
   while (a.box < kN && a.kv.page_size % (2 * a.box) == 0) a.box *= 2;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  const size_t need = moe_tree_attention_workspace_size(hd);
-  if (!c.workspace || c.workspace_bytes < (int64_t)need) return MOE_ERR_WORKSPACE;
-  if (!aligned16(c.workspace)) return MOE_ERR_ALIGNMENT;
   a.jobs = reinterpret_cast<int4*>(static_cast<char*>(c.workspace) + kJobsAt);
   a.part = reinterpret_cast<float*>(a.jobs + sm_count());
   a.wait_ns = wait_limit_ns();
-  const bool bf16 = c.kv.dtype == MOE_DTYPE_BF16;
   const bool none = c.kv.max_pages == 0;  // no keys at all: the maps describe q
   CUtensorMap mq, mk, mv;
   const cuuint64_t q_dims[4] = {(cuuint64_t)hd, (cuuint64_t)c.heads, (cuuint64_t)c.nodes,
@@ -1148,7 +1005,6 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
     return MOE_ERR_CUDA;
   const int64_t line = c.kv.seqs * per_seq * steps, most = ceil_div(line, kMinShare + kStart);
   const int sms = sm_count(), grid = static_cast<int>(most < 1 ? 1 : most < sms ? most : sms);
-  cudaStream_t s = static_cast<cudaStream_t>(c.stream);
   if (bf16)
     return hd == 64 ? launch_tree<BF16, 64>(a, mq, mk, mv, grid, s)
                     : launch_tree<BF16, 128>(a, mq, mk, mv, grid, s);

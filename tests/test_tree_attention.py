@@ -1,5 +1,8 @@
 """tree_attention against the formula in 64 bits, at every edge of nodes, keys, pages and splits.
 
+Up to 16 rows (nodes x heads of a group) to a KV head take one kernel, more another: where that is
+not plain from the sizes, tests run with a number of nodes for each.
+
 The bound is :func:`oracle.serving.attention_bound`'s: what rounding scores, probabilities and outputs
 to their types allows, for the row's own numbers.
 """
@@ -123,14 +126,15 @@ def test_wide_trees_over_cut_units(dtype, H, KV):
 
 
 @gpu
-def test_counts_and_rows_without_keys():
+@pytest.mark.parametrize("KV", [2, 8])
+def test_counts_and_rows_without_keys(KV):
     """Trees of different sizes in one call; nodes that see nothing, or only others; no pages needed
     past a tree's own nodes."""
     from moeinfra_b200 import kernels
 
     lens, counts, nodes = [0, 30, 64, 5, -1, 100], [3, 10, 0, -2, 7, 1], 10
     table, n = _table([max(m, 0) + max(c, 0) for m, c in zip(lens, counts)], 16, 4)
-    kp, vp = (_cache(n, 2, 16, 64, torch.float16, s) for s in (7, 8))
+    kp, vp = (_cache(n, KV, 16, 64, torch.float16, s) for s in (7, 8))
     visible = _trees(6, nodes, 3)
     visible[0, 1] = 0                  # sees nothing: no cached positions
     visible[0, 2] = 1 << 9             # sees only a node that is not there
@@ -150,9 +154,10 @@ def test_counts_and_rows_without_keys():
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("lens", [[5, 20], [1500, 64]])
-def test_what_a_row_does_not_see_has_no_effect(dtype, bad, lens):
+@pytest.mark.parametrize("nodes,KV", [(9, 2), (5, 4)])
+def test_what_a_row_does_not_see_has_no_effect(dtype, bad, lens, nodes, KV):
     """Pages past the end, pages of nobody, and nodes outside a row's branch hold NaN or infinities."""
-    H, KV, hd, page, nodes = 8, 2, 128, 32, 9
+    H, hd, page = 8, 128, 32
     table, n = _table([m + nodes for m in lens], page, 8)
     kp, vp = (_cache(n, KV, page, hd, dtype, s) for s in (5, 6))
     used = {int(p) for row in table for p in row if p >= 0}
@@ -186,8 +191,9 @@ def test_what_a_row_does_not_see_has_no_effect(dtype, bad, lens):
 
 
 @gpu
-def test_scores_of_infinity_and_nan_make_a_row_nan():
-    H, KV, hd, page, nodes = 4, 1, 64, 16, 3
+@pytest.mark.parametrize("nodes", [3, 10])
+def test_scores_of_infinity_and_nan_make_a_row_nan(nodes):
+    H, KV, hd, page = 4, 1, 64, 16
     table, n = _table([40 + nodes] * 2, page, 8)
     kp, vp = (_cache(n, KV, page, hd, torch.float16, s) for s in (5, 6))
     q = _q(2, nodes, H, hd, torch.float16).cuda()
@@ -204,9 +210,10 @@ def test_scores_of_infinity_and_nan_make_a_row_nan():
 
 
 @gpu
-def test_peaked_and_faint_softmax():
+@pytest.mark.parametrize("nodes", [2, 12])
+def test_peaked_and_faint_softmax(nodes):
     """One key far above the others, scores far below zero, and a maximum that keeps growing."""
-    H, KV, hd, page, nodes, m = 4, 1, 64, 16, 2, 700
+    H, KV, hd, page, m = 4, 1, 64, 16, 700
     table, n = _table([m + nodes] * 3, page, 2)
     kp = torch.zeros(n, KV, page, hd)
     vp = torch.randn(n, KV, page, hd, generator=torch.Generator().manual_seed(0))
@@ -221,12 +228,13 @@ def test_peaked_and_faint_softmax():
 
 
 @gpu
-def test_strided_inputs_shared_pages_and_repeats():
+@pytest.mark.parametrize("nodes", [4, 12])
+def test_strided_inputs_shared_pages_and_repeats(nodes):
     """Keys and values side by side, queries from a wider buffer, one mask for all sequences, one page
     in two sequences; the same call twice gives the same bits."""
     from moeinfra_b200 import kernels
 
-    H, KV, hd, page, lens, nodes = 8, 2, 128, 16, [40, 2000, 33], 6
+    H, KV, hd, page, lens = 8, 2, 128, 16, [40, 2000, 33]
     table, n = _table([m + nodes for m in lens], page, 9)
     table[2, 0] = table[0, 0]
     both = _cache(2 * n, KV, page, hd, torch.bfloat16, 7).view(n, 2, KV, page, hd)
@@ -260,11 +268,12 @@ def test_one_node_is_paged_attention():
 
 
 @gpu
-def test_graphs_follow_their_inputs_side_by_side():
+@pytest.mark.parametrize("nodes", [20, 4])
+def test_graphs_follow_their_inputs_side_by_side(nodes):
     """Captured calls read lengths, masks and pages at replay; two on one stream, replayed on two."""
     from moeinfra_b200 import kernels
 
-    H, KV, hd, page, nodes = 8, 2, 64, 16, 20
+    H, KV, hd, page = 8, 2, 64, 16
     table, n = _table([2500, 2500], page, 3)
     kp, vp = (_cache(n, KV, page, hd, torch.float16, s) for s in (8, 9))
     tab = table.cuda()
@@ -312,9 +321,10 @@ def test_bad_lengths_and_pages_are_reported():
 
 
 @gpu
-def test_past_two_to_the_31_elements():
+@pytest.mark.parametrize("nodes", [3, 20])
+def test_past_two_to_the_31_elements(nodes):
     """Pages whose elements lie past 2^31 (and bytes past 2^32) of the cache."""
-    KV, page, hd, nodes = 8, 64, 128, 3
+    KV, page, hd = 8, 64, 128
     n = 2 ** 31 // (KV * page * hd) + 40
     kp = torch.zeros(n, KV, page, hd, dtype=torch.float16, device="cuda")
     vp = torch.zeros_like(kp)
@@ -330,6 +340,25 @@ def test_past_two_to_the_31_elements():
     at = table[0].long()
     small = torch.arange(3, dtype=torch.int32)[None]
     _check(q, kp[at], vp[at], small, [150], _trees(1, nodes, 1), got=got)
+
+
+@gpu
+@pytest.mark.parametrize("H,KV,nodes", [(32, 8, 16), (32, 8, 64), (16, 8, 7)])
+def test_a_long_batch_many_times(H, KV, nodes):
+    """Sequences of some 30 steps each, whose two pipelines drift apart; the same bits every time."""
+    from moeinfra_b200 import kernels
+
+    lens, page, hd = [1800 + 7 * i for i in range(48)], 64, 128
+    table, n = _table([m + nodes for m in lens], page, 3)
+    kp, vp = (_cache(n, KV, page, hd, torch.bfloat16, s) for s in (1, 2))
+    q, vis = _q(48, nodes, H, hd, torch.bfloat16), _trees(48, nodes, 3)
+    at = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    args = (q.cuda(), kp, vp, table.cuda(), at, vis.cuda())
+    first = kernels.tree_attention(*args)
+    for _ in range(20):
+        assert torch.equal(kernels.tree_attention(*args), first)
+    kernels.check_device()
+    _check(q[45:], kp, vp, table[45:], lens[45:], vis[45:], got=first[45:])
 
 
 @gpu
