@@ -298,10 +298,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lo = (int)min((int64_t)blockIdx.x * share, (int64_t)total), hi = (int)min((int64_t)lo + share, (int64_t)total);
 
   // The next item; false at the end or after a timeout (then ok is false).
-  Item it;
   uint32_t n_it = 0;
   bool ok = true;
-  auto next_item = [&]() {
+  auto next_item = [&](Item& it) {
     const uint32_t i = n_it % kItems;
     ok = warp_wait(saddr(&s_itfull[i]), n_it / kItems & 1, a.wait_ns);
     if (!ok) return false;
@@ -326,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t o_pal = tmem + C::kO + (1 - t) * C::kO1 + lane_base;
     const int row_node = row / a.tile_heads, row_head = row - row_node * a.tile_heads;
     uint32_t n_s = 0, n_pair = 0;  // steps and shared tiles so far
-    while (next_item()) {
+    for (Item it; next_item(it);) {
       const bool two = it.flags & kTwo;
       const int second = two ? t : 0;
       Row me{it.node0 + second * a.tokens + row_node, it.head0 + row_head};
@@ -466,44 +465,57 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       float odd = 0.f;  // NaN once an element is not finite
+      if (!two) {
 #pragma unroll 1
-      for (int c = from; c < to; c += 32) {
-        uint32_t o[32], x[32];
-        tmem_ld32(o_at + c, o);
-        if (pal_has) tmem_ld32(o_pal + c, x);
-        tmem_wait_ld();
+        for (int c = from; c < to; c += 16) {
+          uint32_t o[16], x[16];
+          tmem_ld16(o_at + c, o);
+          tmem_ld16(o_pal + c, x);
+          tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float v = mine > 0 ? __uint_as_float(o[e]) * f : 0.f;
-          if (pal_has) v = fmaf(__uint_as_float(x[e]), f_pal, v);
-          odd = fmaf(v, 0.f, odd);
-          o[e] = __float_as_uint(none ? 0.f : v * inv);
+          for (int e = 0; e < 16; ++e) {
+            float v = mine > 0 ? __uint_as_float(o[e]) * f : 0.f;
+            if (pal_has) v = fmaf(__uint_as_float(x[e]), f_pal, v);
+            odd = fmaf(v, 0.f, odd);
+            o[e] = __float_as_uint(none ? 0.f : v * inv);
+          }
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              reinterpret_cast<uint4*>(piece + row * HD + c)[i] =
+                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          } else if (real) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = T::pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              reinterpret_cast<uint4*>(out + place + c)[i] =
+                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
         }
-        if (whole) {
-          uint32_t w[16];
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_at + c, o);
+          tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = T::pack(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
-          if (two) {
-            leave(w, [&](int r) {
+          for (int e = 0; e < 32; ++e) {
+            const float v = __uint_as_float(o[e]);
+            odd = fmaf(v, 0.f, odd);
+            o[e] = __float_as_uint(none ? 0.f : v * inv);
+          }
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = T::pack(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+            leave(o, [&](int r) {
               const int at = __shfl_sync(0xffffffffu, place, r);
               return at < 0 ? nullptr : reinterpret_cast<uint4*>(out + at + c) + (lane & 3);
             });
-          } else if (real) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              reinterpret_cast<uint4*>(out + place + c)[i] =
-                  make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-          }
-        } else {
-          float* rows = piece + (second * kM + (warp & 3) * 32) * HD + c;
-          if (two) {
+          } else {
+            float* rows = piece + (second * kM + (warp & 3) * 32) * HD + c;
             leave(o, [&](int r) { return reinterpret_cast<uint4*>(rows + r * HD) + (lane & 3); });
             leave(o + 16, [&](int r) { return reinterpret_cast<uint4*>(rows + r * HD + 16) + (lane & 3); });
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              reinterpret_cast<uint4*>(rows + lane * HD)[i] =
-                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
         }
       }
@@ -564,34 +576,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (more) more = pc.next(a, prefix);
     };
-    uint32_t n_mine = 0;
-    auto take = [&]() {  // the first producer's own items, one described ahead
-      if (is_v) return next_item();
-      if (n_mine == 0) publish();
-      if (!ok) return false;
-      it = s_item[n_mine % kItems];
-      ++n_mine;
-      if (__shfl_sync(0xffffffffu, it.steps, 0) == 0) return false;
-      publish();
-      return ok;
+    auto look = [&](const Item& x, int box) {  // the table's entry for a box
+      if (box * a.box >= x.keys) return 0;
+      const int entry = box / page_boxes;
+      return entry < a.kv.max_pages ? a.kv.table[x.b * a.kv.table_stride + entry] : -1;
     };
-    while (take()) {
+    auto checked = [&](int page) {
+      if (page >= 0 && page < a.kv.num_pages) return page;
+      set_device_error(kErrPage);
+      return 0;
+    };
+    // The item after the one at hand, and its first 64 boxes' pages, on their way while this one's
+    // loads are issued.
+    Item nx;
+    int nx_page = 0, nx_next = 0;
+    uint32_t n_mine = 0;
+    auto prepare = [&]() {
+      if (is_v) {
+        next_item(nx);
+      } else {
+        publish();
+        nx = s_item[n_mine++ % kItems];
+      }
+      if (!ok || __shfl_sync(0xffffffffu, nx.steps, 0) == 0) return;
+      const int first = nx.s0 * boxes / 32 * 32 + lane;
+      nx_page = look(nx, first);
+      nx_next = look(nx, first + 32);
+    };
+    prepare();
+    while (ok && __shfl_sync(0xffffffffu, nx.steps, 0) > 0) {
+      const Item it = nx;
       const int flags = __shfl_sync(0xffffffffu, it.flags, 0), seq = __shfl_sync(0xffffffffu, it.b, 0);
       const int s0 = __shfl_sync(0xffffffffu, it.s0, 0), all = __shfl_sync(0xffffffffu, it.steps, 0);
       const int keys = __shfl_sync(0xffffffffu, it.keys, 0), kv_head = flags >> 8;
       const int lead = lead_of(flags & kTwo);
-      // Places of 32 boxes of the sequence from w_base on, one per lane, and pages of the 32
-      // after them.
-      auto look = [&](int x) -> int {  // the page of box x
-        if (x * a.box >= keys) return 0;
-        const int entry = x / page_boxes;
-        const int64_t page = entry < a.kv.max_pages ? a.kv.table[seq * a.kv.table_stride + entry] : -1;
-        if (page >= 0 && page < a.kv.num_pages) return (int)page;
-        set_device_error(kErrPage);
-        return 0;
-      };
+      // Pages and places in them of 32 boxes of the sequence from w_base on, one per lane, and the
+      // table's entries of the 32 after them.
       int w_base = s0 * boxes / 32 * 32;
-      int w_page = look(w_base + lane), w_next = look(w_base + 32 + lane);
+      int w_page = checked(nx_page), w_next = nx_next;
       int w_y = (w_base + lane) % page_boxes * a.box;
       for (int t = 0; !is_v && t < (flags & kTwo ? 2 : 1) && ok; ++t) {
         const int slot = flags & kTwo ? t : flags >> 3 & 1;
@@ -612,9 +634,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int from = (s0 + i) * boxes - w_base;
         if (from >= 32) {
           w_base += 32;
-          w_page = w_next;
+          w_page = checked(w_next);
           w_y = (w_base + lane) % page_boxes * a.box;
-          w_next = look(w_base + 32 + lane);
+          w_next = look(it, w_base + 32 + lane);
         }
         const int rows = keys - (s0 + i) * kN, count = min(boxes, (rows + a.box - 1) / a.box);
         const bool tail = is_v && rows < kN;
@@ -630,6 +652,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_4d_if(leader, dst + hf * C::kHalfK + n * a.box * 128, map, bar, hf * 64, y, kv_head,
                            page);
         }
+        if (i == 0) prepare();
+        if (!ok) break;
         if (!tail) continue;
         ok = warp_wait(saddr(&s_tail), n_tail++ & 1, a.wait_ns);
         if (!ok) break;
@@ -688,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t n_q0 = 0, n_q1 = 0;            // uses of the Q buffers
     uint32_t n_qk = 0, n_pv = 0;
     // A slot, like a Q buffer, counts two releases: one of each pipeline.
-    while (ok && next_item()) {
+    for (Item it; ok && next_item(it);) {
       const int flags = __shfl_sync(0xffffffffu, it.flags, 0);
       const int all = __shfl_sync(0xffffffffu, it.steps, 0);
       const bool two = flags & kTwo;
