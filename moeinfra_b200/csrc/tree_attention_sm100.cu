@@ -466,18 +466,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       float odd = 0.f;  // NaN once an element is not finite
       if (!two) {
+        const uint64_t f2 = pair(f * inv, f * inv), f_pal2 = pair(f_pal * inv, f_pal * inv);
+        uint64_t odd2 = 0;
 #pragma unroll 1
         for (int c = from; c < to; c += 16) {
-          uint32_t o[16], x[16];
-          tmem_ld16(o_at + c, o);
-          tmem_ld16(o_pal + c, x);
+          uint32_t o[16] = {}, x[16] = {};
+          if (mine > 0) tmem_ld16(o_at + c, o);
+          if (pal_has) tmem_ld16(o_pal + c, x);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float v = mine > 0 ? __uint_as_float(o[e]) * f : 0.f;
-            if (pal_has) v = fmaf(__uint_as_float(x[e]), f_pal, v);
-            odd = fmaf(v, 0.f, odd);
-            o[e] = __float_as_uint(none ? 0.f : v * inv);
+          for (int e = 0; e < 16; e += 2) {
+            const uint64_t v = fma2(pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f_pal2,
+                                    mul2(pair(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), f2));
+            odd2 = fma2(v, 0, odd2);
+            o[e] = __float_as_uint(lo_of(v));
+            o[e + 1] = __float_as_uint(hi_of(v));
+          }
+          if (none) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = 0;
           }
           if (!whole) {
 #pragma unroll
@@ -493,6 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
         }
+        odd = lo_of(odd2) + hi_of(odd2);
       } else {
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
