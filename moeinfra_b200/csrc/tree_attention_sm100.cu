@@ -85,7 +85,7 @@ struct TreeArgs : TreeRows {
   int tokens;                   // nodes of a tile
   int blocks;                   // blocks of rows (two tiles) of a KV head's part
   int per_seq;                  // units of a sequence
-  int box;                      // rows of a K or V box: they lie in one page
+  int box, box_shift;           // rows of a K or V box, which lie in one page, and their log2
   int4* jobs;                   // [CTAs]: sequence, unit, CTAs and nodes of the cut unit that starts there
   float* part;                  // [CTAs][2] pieces: 0 of a unit that starts before, 1 of one that goes on
   uint64_t wait_ns;
@@ -559,25 +559,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t g = 0, n_q0 = 0, n_q1 = 0, n_tail = 0, ones = 0;
     Piece pc;
     bool more = !is_v && pc.start(a, prefix, lo, hi);
+    int len = 0, keys = 0, of = -1;  // of sequence `of`
+    // The item after the one at hand, and its first 64 boxes' pages, on their way while this one's
+    // loads are issued.
+    Item nx;
     // Describes the next piece, or the end.
     auto publish = [&]() {
       const uint32_t i = n_it % kItems;
       ok = warp_wait(saddr(&s_itempty[i]), (n_it / kItems & 1) ^ 1, a.wait_ns);
       if (!ok) return;
       ++n_it;
+      Item x{};
+      if (more) {
+        if (pc.b != of) span(a, of = pc.b, len, keys);
+        const int kp = pc.u / a.blocks, block = pc.u - kp * a.blocks;
+        const bool two = a.nodes - block * 2 * a.tokens > a.tokens;
+        x = Item{pc.b, block * 2 * a.tokens, kp * a.tile_heads, len, keys, pc.s0,
+                 pc.s1 - pc.s0,
+                 (two ? kTwo : 0) | (pc.s0 == 0 ? kFirst : 0) | (pc.s1 == pc.n ? kLast : 0) |
+                     (int)(ones & 1) << 3 | kp / a.parts << 8};
+        ones += !two;
+      }
+      nx = x;
       if (lane == 0) {
-        Item x{};
-        if (more) {
-          const int kp = pc.u / a.blocks, block = pc.u - kp * a.blocks;
-          int len, keys;
-          span(a, pc.b, len, keys);
-          const bool two = a.nodes - block * 2 * a.tokens > a.tokens;
-          x = Item{pc.b, block * 2 * a.tokens, kp * a.tile_heads, len, keys, pc.s0,
-                   pc.s1 - pc.s0,
-                   (two ? kTwo : 0) | (pc.s0 == 0 ? kFirst : 0) | (pc.s1 == pc.n ? kLast : 0) |
-                       (int)(ones & 1) << 3 | kp / a.parts << 8};
-          ones += !two;
-        }
         s_item[i] = x;
         mbar_arrive(saddr(&s_itfull[i]));
       }
@@ -594,18 +598,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       set_device_error(kErrPage);
       return 0;
     };
-    // The item after the one at hand, and its first 64 boxes' pages, on their way while this one's
-    // loads are issued.
-    Item nx;
     int nx_page = 0, nx_next = 0;
-    uint32_t n_mine = 0;
     auto prepare = [&]() {
-      if (is_v) {
-        next_item(nx);
-      } else {
-        publish();
-        nx = s_item[n_mine++ % kItems];
-      }
+      if (is_v) next_item(nx);
+      else publish();
       if (!ok || __shfl_sync(0xffffffffu, nx.steps, 0) == 0) return;
       const int first = nx.s0 * boxes / 32 * 32 + lane;
       nx_page = look(nx, first);
@@ -616,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item it = nx;
       const int flags = __shfl_sync(0xffffffffu, it.flags, 0), seq = __shfl_sync(0xffffffffu, it.b, 0);
       const int s0 = __shfl_sync(0xffffffffu, it.s0, 0), all = __shfl_sync(0xffffffffu, it.steps, 0);
-      const int keys = __shfl_sync(0xffffffffu, it.keys, 0), kv_head = flags >> 8;
+      const int end = __shfl_sync(0xffffffffu, it.keys, 0), kv_head = flags >> 8;
       const int lead = lead_of(flags & kTwo);
       // Pages and places in them of 32 boxes of the sequence from w_base on, one per lane, and the
       // table's entries of the 32 after them.
@@ -646,21 +642,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           w_y = (w_base + lane) % page_boxes * a.box;
           w_next = look(it, w_base + 32 + lane);
         }
-        const int rows = keys - (s0 + i) * kN, count = min(boxes, (rows + a.box - 1) / a.box);
+        const int rows = end - (s0 + i) * kN, count = min(boxes, (rows + a.box - 1) >> a.box_shift);
         const bool tail = is_v && rows < kN;
         const uint32_t bar = tail ? saddr(&s_tail) : saddr(&s_full[s]);
         ok = warp_wait(saddr(&s_empty[s]), (x / NS & 1) ^ 1, a.wait_ns);
         if (!ok) break;
         mbar_expect_tx_if(leader, bar, count * a.box * 128 * C::kHalves);
-        for (int n = 0; n < count; ++n) {
-          const int page = __shfl_sync(0xffffffffu, w_page, from + n);
-          const int y = __shfl_sync(0xffffffffu, w_y, from + n);
+        int page[kN / 16], y[kN / 16];
 #pragma unroll
-          for (int hf = 0; hf < C::kHalves; ++hf)
-            tma_load_4d_if(leader, dst + hf * C::kHalfK + n * a.box * 128, map, bar, hf * 64, y, kv_head,
-                           page);
+        for (int n = 0; n < kN / 16; ++n) {
+          page[n] = __shfl_sync(0xffffffffu, w_page, from + n);
+          y[n] = __shfl_sync(0xffffffffu, w_y, from + n);
         }
-        if (i == 0) prepare();
+#pragma unroll
+        for (int n = 0; n < kN / 16; ++n)
+          if (n < count)
+#pragma unroll
+            for (int hf = 0; hf < C::kHalves; ++hf)
+              tma_load_4d_if(leader, dst + hf * C::kHalfK + n * a.box * 128, map, bar, hf * 64, y[n],
+                             kv_head, page[n]);
+        if (i == (is_v ? min(2, all - 1) : 0)) prepare();  // the item that V waits for is K's
         if (!ok) break;
         if (!tail) continue;
         ok = warp_wait(saddr(&s_tail), n_tail++ & 1, a.wait_ns);
@@ -1013,8 +1014,9 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
   if (per_seq > INT32_MAX || c.kv.seqs * per_seq > INT32_MAX / (steps > 0 ? steps : 1) - 4096)
     return MOE_ERR_UNSUPPORTED;
   a.per_seq = static_cast<int>(per_seq);
-  a.box = 16;
-  while (a.box < kN && a.kv.page_size % (2 * a.box) == 0) a.box *= 2;
+  a.box_shift = 4;
+  while ((1 << a.box_shift) < kN && a.kv.page_size % (2 << a.box_shift) == 0) ++a.box_shift;
+  a.box = 1 << a.box_shift;
   a.jobs = reinterpret_cast<int4*>(static_cast<char*>(c.workspace) + kJobsAt);
   a.part = reinterpret_cast<float*>(a.jobs + sm_count());
   a.wait_ns = wait_limit_ns();
