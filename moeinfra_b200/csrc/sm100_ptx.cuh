@@ -229,17 +229,17 @@ __device__ __forceinline__ void tc_commit_if(uint32_t leader, uint32_t bar) {
 }
 
 // Shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row groups
-// 1024 bytes apart (rows are 128 bytes = 64 fp16 of K).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+// `group` bytes apart (rows are 128 bytes = 64 fp16 of K).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t group = 1024) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(group >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 // The same for an operand stored along its M or N: rows of 64 elements of M or
-// N (128 bytes, swizzled), one row per K; 8 rows are 1024 bytes, the next 64
-// elements of M or N lie `block` bytes on.
-__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t block) {
+// N (128 bytes, swizzled), one row per K; the next 8 rows lie `group` bytes on, the next 64
+// elements of M or N `block` bytes.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t block, uint32_t group = 1024) {
   return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(block >> 4) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+         ((uint64_t)(group >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
 // The driver's tensor-map encoder, or null.

@@ -61,10 +61,12 @@ constexpr int kMinShare = 2;
 
 template <int HD>
 struct Cfg {
-  // A tile's 64 dims: rows of 128 bytes, in swizzled groups of 8 (1024 bytes).
+  // 64 dims of a row are 128 bytes, 8 rows of them a swizzled atom of 1024 bytes.  A tile of Q has its
+  // first 64 dims' atoms first, a tile of keys or values those of 8 keys together (kGroup bytes): a
+  // box of any number of keys lies in one piece, one load.
   static constexpr int kHalves = HD / 64;
-  static constexpr uint32_t kHalfQ = kM * 128, kHalfK = kN * 128;
-  static constexpr uint32_t kTileQ = kHalfQ * kHalves, kTileK = kHalfK * kHalves;
+  static constexpr uint32_t kHalfQ = kM * 128, kGroup = 1024 * kHalves;
+  static constexpr uint32_t kTileQ = kHalfQ * kHalves, kTileK = kN / 8 * kGroup;
   static constexpr int kStages = 8 * 2 / kHalves;  // K and V tiles in flight: 128 KB
   static constexpr uint32_t kRing = kStages * kTileK;
   // On its way out a softmax warp's result passes 32 rows x 64 bytes of shared memory.
@@ -86,6 +88,7 @@ struct TreeArgs : TreeRows {
   int blocks;                   // blocks of rows (two tiles) of a KV head's part
   int per_seq;                  // units of a sequence
   int box, box_shift;           // rows of a K or V box, which lie in one page, and their log2
+  int page_shift;               // log2 of a page's boxes, or -1
   int4* jobs;                   // [CTAs]: sequence, unit, CTAs and nodes of the cut unit that starts there
   float* part;                  // [CTAs][2] pieces: 0 of a unit that starts before, 1 of one that goes on
   uint64_t wait_ns;
@@ -107,6 +110,15 @@ __device__ __forceinline__ void tma_load_4d_if(uint32_t leader, uint32_t dst, co
       " @q cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
       "{%3, %4, %5, %6}], [%2];\n}\n" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d_if(uint32_t leader, uint32_t dst, const CUtensorMap* map,
+                                               uint32_t bar, int w, int v) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %5, 0;\n"
+      " @q cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+      "{%6, %6, %6, %3, %4}], [%2];\n}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(w), "r"(v), "r"(leader), "r"(0)
       : "memory");
 }
 __device__ __forceinline__ void mbar_expect_tx_if(uint32_t leader, uint32_t bar, uint32_t bytes) {
@@ -572,12 +584,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item x{};
       if (more) {
         if (pc.b != of) span(a, of = pc.b, len, keys);
-        const int kp = pc.u / a.blocks, block = pc.u - kp * a.blocks;
+        const int kp = a.blocks == 1 ? pc.u : pc.u / a.blocks, block = pc.u - kp * a.blocks;
         const bool two = a.nodes - block * 2 * a.tokens > a.tokens;
         x = Item{pc.b, block * 2 * a.tokens, kp * a.tile_heads, len, keys, pc.s0,
                  pc.s1 - pc.s0,
                  (two ? kTwo : 0) | (pc.s0 == 0 ? kFirst : 0) | (pc.s1 == pc.n ? kLast : 0) |
-                     (int)(ones & 1) << 3 | kp / a.parts << 8};
+                     (int)(ones & 1) << 3 | (a.parts == 1 ? kp : kp / a.parts) << 8};
         ones += !two;
       }
       nx = x;
@@ -588,9 +600,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (more) more = pc.next(a, prefix);
     };
+    auto entry_of = [&](int box) { return a.page_shift >= 0 ? box >> a.page_shift : box / page_boxes; };
     auto look = [&](const Item& x, int box) {  // the table's entry for a box
       if (box * a.box >= x.keys) return 0;
-      const int entry = box / page_boxes;
+      const int entry = entry_of(box);
       return entry < a.kv.max_pages ? a.kv.table[x.b * a.kv.table_stride + entry] : -1;
     };
     auto checked = [&](int page) {
@@ -614,11 +627,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int s0 = __shfl_sync(0xffffffffu, it.s0, 0), all = __shfl_sync(0xffffffffu, it.steps, 0);
       const int end = __shfl_sync(0xffffffffu, it.keys, 0), kv_head = flags >> 8;
       const int lead = lead_of(flags & kTwo);
-      // Pages and places in them of 32 boxes of the sequence from w_base on, one per lane, and the
-      // table's entries of the 32 after them.
+      // Pages and places in them (in groups of 8 rows) of 32 boxes of the sequence from w_base on,
+      // one per lane, and the table's entries of the 32 after them.
       int w_base = s0 * boxes / 32 * 32;
       int w_page = checked(nx_page), w_next = nx_next;
-      int w_y = (w_base + lane) % page_boxes * a.box;
+      auto place_of = [&](int box) {
+        return (kv_head * page_boxes + box - entry_of(box) * page_boxes) * (a.box / 8);
+      };
+      int w_at = place_of(w_base + lane);
       for (int t = 0; !is_v && t < (flags & kTwo ? 2 : 1) && ok; ++t) {
         const int slot = flags & kTwo ? t : flags >> 3 & 1;
         const uint32_t turn = slot ? n_q1++ : n_q0++;
@@ -639,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (from >= 32) {
           w_base += 32;
           w_page = checked(w_next);
-          w_y = (w_base + lane) % page_boxes * a.box;
+          w_at = place_of(w_base + lane);
           w_next = look(it, w_base + 32 + lane);
         }
         const int rows = end - (s0 + i) * kN, count = min(boxes, (rows + a.box - 1) >> a.box_shift);
@@ -648,27 +664,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = warp_wait(saddr(&s_empty[s]), (x / NS & 1) ^ 1, a.wait_ns);
         if (!ok) break;
         mbar_expect_tx_if(leader, bar, count * a.box * 128 * C::kHalves);
-        int page[kN / 16], y[kN / 16];
+        int page[kN / 16], at[kN / 16];
 #pragma unroll
         for (int n = 0; n < kN / 16; ++n) {
           page[n] = __shfl_sync(0xffffffffu, w_page, from + n);
-          y[n] = __shfl_sync(0xffffffffu, w_y, from + n);
+          at[n] = __shfl_sync(0xffffffffu, w_at, from + n);
         }
 #pragma unroll
         for (int n = 0; n < kN / 16; ++n)
           if (n < count)
-#pragma unroll
-            for (int hf = 0; hf < C::kHalves; ++hf)
-              tma_load_4d_if(leader, dst + hf * C::kHalfK + n * a.box * 128, map, bar, hf * 64, y[n],
-                             kv_head, page[n]);
+            tma_load_5d_if(leader, dst + n * a.box * 128 * C::kHalves, map, bar, at[n], page[n]);
         if (i == (is_v ? min(2, all - 1) : 0)) prepare();  // the item that V waits for is K's
         if (!ok) break;
         if (!tail) continue;
         ok = warp_wait(saddr(&s_tail), n_tail++ & 1, a.wait_ns);
         if (!ok) break;
-        for (int hf = 0; hf < C::kHalves; ++hf)
-          for (uint32_t z = rows * 128 + lane * 16; z < C::kHalfK; z += 512)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + hf * C::kHalfK + z),
+        for (uint32_t z = rows * 128 + lane * 16; z < kN * 128; z += 512)
+          for (int hf = 0; hf < C::kHalves; ++hf)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                             dst + (z >> 10) * C::kGroup + hf * 1024 + (z & 1023)),
                          "r"(0)
                          : "memory");
         fence_proxy_async();
@@ -713,8 +727,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // descriptors are then uniform over the warp and stay in uniform registers.
     const uint32_t d_qk = instr_desc<T>(kN, false), d_pv = instr_desc<T>(HD, true);
     const uint32_t leader = elect_one();
-    const uint64_t desc_q = smem_desc(q_at), desc_k = smem_desc(ring);
-    const uint64_t desc_v = smem_desc_mn(ring, C::kHalfK);
+    const uint64_t desc_q = smem_desc(q_at), desc_k = smem_desc(ring, C::kGroup);
+    const uint64_t desc_v = smem_desc_mn(ring, 1024, C::kGroup);
     const uint32_t s_col = tmem + C::kS + t * C::kS1;
     const uint32_t o_col = tmem + C::kO + t * C::kO1;
     uint32_t ring_slot = 0, ring_turn = 0;  // of the ring's next tile, and the parity of its barrier
@@ -761,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
             tc_mma_if(leader, sc, qd + ((kk / 4 * C::kHalfQ + kk % 4 * 32) >> 4),
-                      kd + ((kk / 4 * C::kHalfK + kk % 4 * 32) >> 4), d_qk, kk != 0);
+                      kd + ((kk / 4 * 1024 + kk % 4 * 32) >> 4), d_qk, kk != 0);
           tc_commit_if(leader, saddr(&s_sfull[t][n_qk & 1]));
           if (--qk_left == 0) {
             tc_commit_if(leader, saddr(&s_qempty[slot]));
@@ -777,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_mma_ta_if(leader, o_col, pc, vd, d_pv, first ? 0 : 1);
 #pragma unroll
           for (int kk = 1; kk < kN / 16; ++kk)
-            tc_mma_ta_if(leader, o_col, pc + kk * 8, vd + (kk * 2048 >> 4), d_pv, 1);
+            tc_mma_ta_if(leader, o_col, pc + kk * 8, vd + (kk * 2 * C::kGroup >> 4), d_pv, 1);
           tc_commit_if(leader, saddr(&s_pvdone[t][n_pv & 1]));
           first = false;
           ++n_pv;
@@ -906,16 +920,18 @@ __global__ void __launch_bounds__(kJoinThreads, 3) k_tree_join(const __grid_cons
   else join_rows<T, HD, 8>(a, job);
 }
 
-// Four dimensions, boxes of box[1] x box[2] rows of 64 elements, 128-byte swizzle.
-bool make_map(CUtensorMap* map, const uint16_t* x, bool bf16, const cuuint64_t (&dims)[4],
-              const int64_t (&stride)[3], const cuuint32_t (&box)[4]) {
+// N dimensions of which the innermost box is 64 elements, 128-byte swizzle.
+template <int N>
+bool make_map(CUtensorMap* map, const uint16_t* x, bool bf16, const cuuint64_t (&dims)[N],
+              const int64_t (&stride)[N - 1], const cuuint32_t (&box)[N]) {
   auto fn = encode_fn();
   if (!fn) return false;
-  const cuuint64_t strides[3] = {(cuuint64_t)stride[0] * 2, (cuuint64_t)stride[1] * 2,
-                                 (cuuint64_t)stride[2] * 2};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-            const_cast<uint16_t*>(x), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  cuuint64_t strides[N - 1];
+  cuuint32_t ones[N];
+  for (int i = 0; i < N; ++i) ones[i] = 1;
+  for (int i = 0; i < N - 1; ++i) strides[i] = (cuuint64_t)stride[i] * 2;
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, N,
+            const_cast<uint16_t*>(x), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1017,22 +1033,27 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
   a.box_shift = 4;
   while ((1 << a.box_shift) < kN && a.kv.page_size % (2 << a.box_shift) == 0) ++a.box_shift;
   a.box = 1 << a.box_shift;
+  a.page_shift = -1;
+  for (int i = 0; i < 17; ++i)  // pages have 2^20 rows at most
+    if (a.kv.page_size == a.box << i) a.page_shift = i;
   a.jobs = reinterpret_cast<int4*>(static_cast<char*>(c.workspace) + kJobsAt);
   a.part = reinterpret_cast<float*>(a.jobs + sm_count());
   a.wait_ns = wait_limit_ns();
-  const bool none = c.kv.max_pages == 0;  // no keys at all: the maps describe q
   CUtensorMap mq, mk, mv;
   const cuuint64_t q_dims[4] = {(cuuint64_t)hd, (cuuint64_t)c.heads, (cuuint64_t)c.nodes,
                                 (cuuint64_t)c.kv.seqs};
   const int64_t q_strides[3] = {hd, c.q_node_stride, c.kv.seqs > 1 ? c.q_seq_stride : c.q_node_stride * c.nodes};
   const cuuint32_t q_box[4] = {64, (cuuint32_t)a.tile_heads, (cuuint32_t)a.tokens, 1};
-  const cuuint64_t kv_dims[4] = {(cuuint64_t)hd, (cuuint64_t)c.kv.page_size, (cuuint64_t)c.kv.kv_heads,
-                                 (cuuint64_t)c.kv.num_pages};
-  const int64_t in_page = c.kv.page_size * hd, whole = in_page * c.kv.kv_heads;
-  const cuuint32_t kv_box[4] = {64, (cuuint32_t)a.box, 1, 1};
+  // Keys and values as (64 dims, 8 rows, the dims' halves, 8 rows each of all KV heads, pages).
+  const bool none = c.kv.max_pages == 0;  // no keys at all: the maps describe q, unread
+  const cuuint64_t kv_dims[5] = {64, 8, (cuuint64_t)hd / 64,
+                                 none ? 1 : (cuuint64_t)(c.kv.kv_heads * c.kv.page_size / 8),
+                                 none ? 1 : (cuuint64_t)c.kv.num_pages};
+  const cuuint32_t kv_box[5] = {64, 8, (cuuint32_t)hd / 64, none ? 1 : (cuuint32_t)a.box / 8, 1};
   auto kv_map = [&](CUtensorMap* m, const uint16_t* x, int64_t page_stride) {
-    if (none) return make_map(m, c.q, bf16, q_dims, q_strides, q_box);
-    return make_map(m, x, bf16, kv_dims, {hd, in_page, c.kv.num_pages > 1 ? page_stride : whole}, kv_box);
+    const int64_t whole = c.kv.kv_heads * c.kv.page_size * hd;
+    return make_map(m, none ? c.q : x, bf16, kv_dims,
+                    {hd, 64, 8 * hd, c.kv.num_pages > 1 && !none ? page_stride : whole}, kv_box);
   };
   if (!make_map(&mq, c.q, bf16, q_dims, q_strides, q_box) ||
       !kv_map(&mk, c.kv.k_pages, c.kv.k_page_stride) || !kv_map(&mv, c.kv.v_pages, c.kv.v_page_stride))
