@@ -78,7 +78,7 @@ struct Cfg {
   // P takes its step's S's place: the next step's S is computed while this one's softmax runs.
   static constexpr uint32_t kS = 0, kS1 = 2 * kN, kO = 4 * kN, kO1 = HD;
   static_assert(kO + 2 * HD <= 512, "TMEM columns");
-  // Floats of a piece: O [2 kM rows][HD], then m and l per row.
+  // Floats of a piece: O [kM / 16 warps of 32 rows][HD / 4][32 rows][4], then m and l per row.
   static constexpr int kPiece = 2 * kM * (HD + 2);
 };
 
@@ -448,10 +448,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool none = whole && real && l == 0.f && blind(a, it.b, me.node, it.len, it.keys);
       const float inv = whole ? __fdividef(1.f, l) : 1.f;
       float* piece = a.part + ((int64_t)blockIdx.x * 2 + (it.flags & kFirst ? 1 : 0)) * C::kPiece;
-      // A thread has a row; stored that way every 16 bytes touch a line of their own (8 warps' rows of
-      // 128 fp32: 6 us), which is still faster for the few rows of a shared tile.  Else 64 bytes of
-      // a row at a time cross shared memory, the 16-byte pieces exchanged by the row's bits against
-      // bank conflicts, and leave as 8 rows a store.
+      // A thread has a row; the 32 of a warp lie side by side in a piece, 4 columns after 4.  Stored
+      // to the output that way every 16 bytes touch a line of their own, which is still faster for
+      // the few rows of a shared tile.  Else 64 bytes of a row at a time cross shared memory, the
+      // 16-byte pieces exchanged by the row's bits against bank conflicts, and leave as 8 rows a store.
+      uint4* piece_o = reinterpret_cast<uint4*>(piece) + (second * 4 + (warp & 3)) * (HD / 4) * 32 + lane;
       const uint32_t stage = ring + C::kRing + warp * C::kOut;
       const int place = real ? me.node * a.heads * HD + me.head * HD : -1;  // in the sequence's output
       uint16_t* out = a.out + (int64_t)it.b * a.nodes * a.heads * HD;
@@ -501,8 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!whole) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              reinterpret_cast<uint4*>(piece + row * HD + c)[i] =
-                  make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+              piece_o[(c / 4 + i) * 32] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           } else if (real) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = T::pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
@@ -533,9 +533,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               return at < 0 ? nullptr : reinterpret_cast<uint4*>(out + at + c) + (lane & 3);
             });
           } else {
-            float* rows = piece + (second * kM + (warp & 3) * 32) * HD + c;
-            leave(o, [&](int r) { return reinterpret_cast<uint4*>(rows + r * HD) + (lane & 3); });
-            leave(o + 16, [&](int r) { return reinterpret_cast<uint4*>(rows + r * HD + 16) + (lane & 3); });
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              piece_o[(c / 4 + i) * 32] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
         }
       }
@@ -814,99 +814,86 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// The cut units' results, in the order of the keys: CTA (c, y) takes part y of the rows of
-// the unit that is cut at the end of the main kernel's CTA c.  A warp has ROWS x AHEAD
-// (row, piece) pairs on its way at once.
-constexpr int kJoinThreads = 256, kJoinParts = 8, kPairs = 8;
+// The cut units' results, in the order of the keys: a warp takes 16 columns of 32 rows, a row to a
+// lane, of the unit that is cut at the end of the main kernel's CTA blockIdx.x.  AHEAD pieces are on
+// their way at once.
+constexpr int kJoinThreads = 256, kJoinCols = 16;
 template <typename T, int HD, int AHEAD>
 __device__ __forceinline__ void join_rows(const TreeArgs& a, int4 job) {
-  constexpr int kPiece = Cfg<HD>::kPiece, kVec = HD / 32, ROWS = kPairs / AHEAD;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = job.x, n = job.z, have = job.w;
+  constexpr int kPiece = Cfg<HD>::kPiece, kSets = HD / kJoinCols, kVec = kJoinCols / 4;
+  const int item = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int quad = item / kSets, c0 = item % kSets * kJoinCols;  // rows 32 quad ..
+  const int b = job.x, n = job.z, r = quad * 32 + lane;
+  const Row me = row_of(a, job.y, r / kM, r % kM, job.w);
+  const bool real = me.node >= 0;
+  if (!__any_sync(0xffffffffu, real)) return;
   // Piece 0 is CTA c's second, the others the first of the CTAs after it.
   const float* first = a.part + (int64_t)blockIdx.x * 2 * kPiece;
-  for (int r0 = (blockIdx.y * (kJoinThreads / 32) + warp) * ROWS; r0 < 2 * kM;
-       r0 += kJoinParts * (kJoinThreads / 32) * ROWS) {
-    Row me[ROWS];
-    bool some = false;
+  float m = -INFINITY, l = 0.f, acc[kJoinCols] = {};
+  for (int k0 = 0; k0 < n && real; k0 += AHEAD) {
+    float mk[AHEAD], lk[AHEAD];
+    float4 ok[AHEAD][kVec];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      me[i] = row_of(a, job.y, (r0 + i) / kM, (r0 + i) % kM, have);
-      some |= me[i].node >= 0;
+    for (int k = 0; k < AHEAD; ++k) {
+      mk[k] = -INFINITY;
+      lk[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) ok[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k0 + k >= n) continue;
+      const float* src = first + (int64_t)(k0 + k == 0 ? 1 : 2 * (k0 + k)) * kPiece;
+      mk[k] = src[2 * kM * HD + r];
+      lk[k] = src[2 * kM * (HD + 1) + r];
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        ok[k][i] = reinterpret_cast<const float4*>(src)[(quad * (HD / 4) + c0 / 4 + i) * 32 + lane];
     }
-    if (!some) continue;
-    float m[ROWS], l[ROWS] = {}, acc[ROWS][kVec] = {};
+    float nm = m;
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) m[i] = -INFINITY;
-    for (int k0 = 0; k0 < n; k0 += AHEAD) {
-      float mk[AHEAD][ROWS], lk[AHEAD][ROWS], ok[AHEAD][ROWS][kVec] = {};
+    for (int k = 0; k < AHEAD; ++k) nm = fmaxf(nm, mk[k]);
+    const float f = m == nm ? 1.f : exp2_approx(m - nm);
+    m = nm;
+    l *= f;
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const float* src = first + (int64_t)(k0 + k == 0 ? 1 : 2 * (k0 + k)) * kPiece;
+    for (int c = 0; c < kJoinCols; ++c) acc[c] *= f;
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-          mk[k][i] = -INFINITY;
-          lk[k][i] = 0.f;
-          if (k0 + k >= n) continue;
-          mk[k][i] = src[2 * kM * HD + r0 + i];
-          lk[k][i] = src[2 * kM * (HD + 1) + r0 + i];
-          const float* x = src + (r0 + i) * HD + lane * kVec;
-          if constexpr (kVec == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(x);
-            ok[k][i][0] = v.x, ok[k][i][1] = v.y, ok[k][i][2] = v.z, ok[k][i][3] = v.w;
-          } else {
-            const float2 v = *reinterpret_cast<const float2*>(x);
-            ok[k][i][0] = v.x, ok[k][i][1] = v.y;
-          }
-        }
-      }
+    for (int k = 0; k < AHEAD; ++k) {
+      const float fk = mk[k] == nm ? 1.f : exp2_approx(mk[k] - nm);
+      l = fmaf(fk, lk[k], l);
 #pragma unroll
-      for (int i = 0; i < ROWS; ++i) {
-        float nm = m[i];
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) nm = fmaxf(nm, mk[k][i]);
-        const float f = m[i] == nm ? 1.f : exp2_approx(m[i] - nm);
-        m[i] = nm;
-        l[i] *= f;
-#pragma unroll
-        for (int c = 0; c < kVec; ++c) acc[i][c] *= f;
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-          const float fk = mk[k][i] == nm ? 1.f : exp2_approx(mk[k][i] - nm);
-          l[i] = fmaf(fk, lk[k][i], l[i]);
-#pragma unroll
-          for (int c = 0; c < kVec; ++c) acc[i][c] = fmaf(fk, ok[k][i][c], acc[i][c]);
-        }
+      for (int i = 0; i < kVec; ++i) {
+        acc[4 * i] = fmaf(fk, ok[k][i].x, acc[4 * i]);
+        acc[4 * i + 1] = fmaf(fk, ok[k][i].y, acc[4 * i + 1]);
+        acc[4 * i + 2] = fmaf(fk, ok[k][i].z, acc[4 * i + 2]);
+        acc[4 * i + 3] = fmaf(fk, ok[k][i].w, acc[4 * i + 3]);
       }
     }
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      if (me[i].node < 0) continue;
-      int len = 0, keys = 0;
-      bool none = false;
-      if (l[i] == 0.f) {
-        span(a, b, len, keys);
-        none = blind(a, b, me[i].node, len, keys);
-      }
-      const float inv = __fdividef(1.f, l[i]);
-      float odd = 0.f;
-      uint32_t o[kVec / 2];
-#pragma unroll
-      for (int c = 0; c < kVec; c += 2) {
-        odd = fmaf(acc[i][c], 0.f, fmaf(acc[i][c + 1], 0.f, odd));
-        o[c / 2] = none ? 0u : T::pack(acc[i][c] * inv, acc[i][c + 1] * inv);
-      }
-      uint32_t* dst = reinterpret_cast<uint32_t*>(
-          a.out + (((int64_t)b * a.nodes + me[i].node) * a.heads + me[i].head) * HD + lane * kVec);
-      if constexpr (kVec == 4)
-        *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
-      else
-        *dst = o[0];
-      if (__any_sync(0xffffffffu, odd != 0.f) && !none) {
-        span(a, b, len, keys);
-        mend_row<T, HD>(a, b, me[i].node, me[i].head, len, keys, 0, HD);
-      }
+  }
+  bool none = false;
+  float odd = 0.f;
+  if (real) {
+    int len = 0, keys = 0;
+    if (l == 0.f) {
+      span(a, b, len, keys);
+      none = blind(a, b, me.node, len, keys);
     }
+    const float inv = __fdividef(1.f, l);
+    uint32_t o[kJoinCols / 2];
+#pragma unroll
+    for (int c = 0; c < kJoinCols; c += 2) {
+      odd = fmaf(acc[c], 0.f, fmaf(acc[c + 1], 0.f, odd));
+      o[c / 2] = none ? 0u : T::pack(acc[c] * inv, acc[c + 1] * inv);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(a.out +
+                                          (((int64_t)b * a.nodes + me.node) * a.heads + me.head) * HD + c0);
+    dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+  for (uint32_t again = __ballot_sync(0xffffffffu, odd != 0.f && !none); again; again &= again - 1) {
+    const int at = __ffs(again) - 1;
+    int len, keys;
+    span(a, b, len, keys);
+    mend_row<T, HD>(a, b, __shfl_sync(0xffffffffu, me.node, at), __shfl_sync(0xffffffffu, me.head, at),
+                    len, keys, c0, c0 + kJoinCols);
   }
 }
 template <typename T, int HD>
@@ -916,8 +903,7 @@ __global__ void __launch_bounds__(kJoinThreads, 3) k_tree_join(const __grid_cons
   const int4 job = a.jobs[blockIdx.x];
   if (job.z == 0) return;
   if (job.z == 2) join_rows<T, HD, 2>(a, job);
-  else if (job.z <= 4) join_rows<T, HD, 4>(a, job);
-  else join_rows<T, HD, 8>(a, job);
+  else join_rows<T, HD, 3>(a, job);
 }
 
 // N dimensions of which the innermost box is 64 elements, 128-byte swizzle.
@@ -956,7 +942,7 @@ int launch_tree(const TreeArgs& a, const CUtensorMap& q, const CUtensorMap& k, c
                  k, v) != cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
-  if (launch_pdl(k_tree_join<T, HD>, dim3(grid, kJoinParts), dim3(kJoinThreads), 0, s, a) != cudaSuccess)
+  if (launch_pdl(k_tree_join<T, HD>, dim3(grid, 2 * kM / 32 * (HD / kJoinCols) / (kJoinThreads / 32)), dim3(kJoinThreads), 0, s, a) != cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
   return MOE_OK;
