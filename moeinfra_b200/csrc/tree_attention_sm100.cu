@@ -817,7 +817,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // The cut units' results, in the order of the keys: a warp takes 16 columns of 32 rows, a row to a
 // lane, of the unit that is cut at the end of the main kernel's CTA blockIdx.x.  AHEAD pieces are on
 // their way at once.
-constexpr int kJoinThreads = 256, kJoinCols = 16;
+constexpr int kJoinThreads = 128, kJoinCols = 16;
 template <typename T, int HD, int AHEAD>
 __device__ __forceinline__ void join_rows(const TreeArgs& a, int4 job) {
   constexpr int kPiece = Cfg<HD>::kPiece, kSets = HD / kJoinCols, kVec = kJoinCols / 4;
@@ -897,13 +897,13 @@ __device__ __forceinline__ void join_rows(const TreeArgs& a, int4 job) {
   }
 }
 template <typename T, int HD>
-__global__ void __launch_bounds__(kJoinThreads, 3) k_tree_join(const __grid_constant__ TreeArgs a) {
+__global__ void __launch_bounds__(kJoinThreads, 4) k_tree_join(const __grid_constant__ TreeArgs a) {
   pdl_trigger();
   pdl_wait();
   const int4 job = a.jobs[blockIdx.x];
   if (job.z == 0) return;
   if (job.z == 2) join_rows<T, HD, 2>(a, job);
-  else join_rows<T, HD, 3>(a, job);
+  else join_rows<T, HD, 4>(a, job);
 }
 
 // N dimensions of which the innermost box is 64 elements, 128-byte swizzle.
