@@ -31,7 +31,8 @@ namespace {
 constexpr int kMostBeams = 64, kMostCount = 64;
 constexpr int kBeamThreads = 256, kBeamWarps = kBeamThreads / 32;
 constexpr int kVecs = 4;            // 16-byte vectors of a thread in a group
-constexpr int kList = 2048;         // entries of the list
+constexpr int kList = 1024;         // entries of the list
+constexpr int kFound = 512;         // vectors that may have some for it
 constexpr int kRank = 384;          // entries that are put in order by counting
 constexpr int kGroups = 1000;       // counters of a launch (the workspace's first 4096 bytes)
 constexpr float kLog2e = 1.4426950408889634f;
@@ -204,32 +205,19 @@ __device__ __noinline__ float exp_sum_odd(uint4 r, float m) {
   return sum;
 }
 
-// A vector's logits above thr (level: those that reach it) go to the list.  A function of its
-// own: few vectors have one, and the loop around stays short.
-template <typename T>
-__device__ __noinline__ void put_vector(uint4 r, float thr, bool level, uint32_t token, uint64_t* list,
-                                        int* count) {
-  float f[Vec<T>::kN];
-  Vec<T>::unpack(r, f);
-#pragma unroll
-  for (int i = 0; i < Vec<T>::kN; ++i)
-    if (level ? f[i] >= thr : f[i] > thr) {
-      const int at = atomicAdd(count, 1);
-      if (at < kList) list[at] = key_of(f[i], token + i);
-    }
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_select(const BeamArgs a) {
   constexpr int kN = Vec<T>::kN;
   constexpr int kChunk = kBeamThreads * kVecs;  // vectors
   __shared__ __align__(16) uint64_t s_list[kList];
+  __shared__ uint4 s_found[kFound];
+  __shared__ int s_found_at[kFound];
   __shared__ Pick s_best[kBeamWarps];
   __shared__ uint64_t s_top[kMostCount];
   __shared__ uint32_t s_warp[kBeamWarps];
   __shared__ double s_sum[kBeamWarps];
   __shared__ float s_max[kBeamWarps], s_rowmax[kMostBeams], s_rowsum[kMostBeams], s_score[kMostBeams];
-  __shared__ int s_count, s_last;
+  __shared__ int s_count, s_founds, s_last;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, M = a.count;
   const int row = blockIdx.x / (uint32_t)a.splits, split = blockIdx.x - row * a.splits;
   using Raw = typename Logit<T>::Raw;
@@ -239,7 +227,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_select(const BeamArgs 
   const uint4* vecs = reinterpret_cast<const uint4*>(x0 - skew);
   const int total = (skew + a.vocab + kN - 1) / kN, share = (total + a.splits - 1) / a.splits;
   const int lo = split * share, hi = min(total, lo + share);
-  if (tid == 0) s_count = 0;
+  if (tid == 0) s_count = s_founds = 0;
   pdl_trigger();
   pdl_wait();
 
@@ -290,28 +278,37 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_select(const BeamArgs 
     }
     sum += e;
   };
-  auto put_above = [&](int c, bool level) {
+  // Vectors with a logit above thr (level: that reaches it) are set aside as they are: the loop
+  // stays short, and the threads share their elements out at the stretch's end.
+  bool some = false;  // this thread has, in this stretch
+  auto find = [&](int c, bool level) {
+    some = true;
 #pragma unroll
     for (int u = 0; u < kVecs; ++u)
-      if (level ? top[u] >= thr : top[u] > thr)
-        put_vector<T>(r[u], thr, level, (uint32_t)((c + u * kBeamThreads + tid) * kN - skew), s_list,
-                      &s_count);
+      if (level ? top[u] >= thr : top[u] > thr) {
+        const int at = atomicAdd(&s_founds, 1);
+        if (at < kFound) {
+          s_found[at] = r[u];
+          s_found_at[at] = c + u * kBeamThreads + tid;
+        }
+      }
   };
   // The list holds every logit so far that is above thr, and of those that reach it as
   // many as `count` needs.
   int had = 0, summed = lo, one_by_one = lo + kChunk;
   for (int pos = lo; pos < hi;) {
     const bool chunk = pos < one_by_one;
+    some = false;
     const int end = min(pos + (chunk ? kChunk : max(kChunk, (pos - lo) / kChunk * kChunk)), hi);
     for (int c = pos; c < end; c += kChunk) {
       take(c);
       if (c >= summed) absorb();
-      if (!chunk && gtop > thr) put_above(c, false);
+      if (!chunk && gtop > thr) find(c, false);
     }
     summed = max(summed, end);
+    bool level = false;
     if (chunk) {
       const int busy = __syncthreads_count(gtop > thr);
-      bool level = false;
       if (busy > 0 && (thr == -INFINITY || busy > 2 * M + 32)) {
         const uint32_t k = reached_by(gtop == -INFINITY ? 0 : Logit<float>::key(gtop), M, s_warp);
         const float t = k ? Logit<float>::value(k) : -INFINITY;
@@ -320,10 +317,25 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_select(const BeamArgs 
           level = true;
         }
       }
-      if (level ? gtop >= thr : gtop > thr) put_above(pos, level);
+      if (level ? gtop >= thr : gtop > thr) find(pos, level);
     }
+    if (!__syncthreads_or(some)) {
+      pos = end;
+      continue;
+    }
+    const int found = s_founds;
+    if (found <= kFound)
+      for (int i = tid; i < found * kN; i += kBeamThreads) {
+        const int e = i % kN;
+        const float f = Logit<T>::of(reinterpret_cast<const Raw*>(s_found + i / kN)[e]);
+        if (level ? f >= thr : f > thr) {
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kList) s_list[at] = key_of(f, (uint32_t)(s_found_at[i / kN] * kN - skew + e));
+        }
+      }
     __syncthreads();
-    const int n = s_count;
+    const int n = found <= kFound ? s_count : kList + 1, kept = found <= kFound ? min(n, kList) : had;
+    if (tid == 0) s_founds = 0;
     __syncthreads();
     if (n > kList && !chunk) {  // once more, chunk by chunk
       if (tid == 0) s_count = had;
@@ -344,7 +356,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_select(const BeamArgs 
       uint64_t last = ~0ull;
       for (int found = 0; found < M; ++found) {
         uint64_t best = 0;
-        for (int i = tid; i < min(n, kList); i += kBeamThreads)
+        for (int i = tid; i < kept; i += kBeamThreads)
           if (s_list[i] < last && s_list[i] > best) best = s_list[i];
         if (n > kList && gtop >= thr) {  // the chunk's logits are read again
           const int c = end - 1 - (end - 1 - lo) % kChunk;

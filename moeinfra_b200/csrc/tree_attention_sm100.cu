@@ -53,10 +53,11 @@ constexpr float kLazy = 8.f;   // log2 of what a row's maximum may grow before O
 // fp16 probabilities, up to 2^kLazy, take 2^7 on top: 2^15 fits, normal down to 2^-21.
 template <typename T>
 constexpr float prob_shift() { return T::kBf16 ? 0.f : 7.f; }
-// Places of a unit's start, in steps (64 x 576, 8 nodes: a start and an end take some 5000 cycles,
-// a step 1300).
-constexpr int kStart = 5;
-// Smallest share of a CTA in steps.
+// Places of a unit's start, in steps: what it takes to begin and end one.  8 nodes over 1 x 600 keys
+// 12.4 us with 2, 13.1 with 3, 14.4 with 5, 15.1 with 7; over 1 x 4000 16.6, 15.4, 16.0, 16.5; 64
+// nodes over 16 x 2049..4095 72.2, 71.6, 72.0, 73.1.
+constexpr int kStart = 3;
+// Smallest share of a CTA in steps: 16 nodes over 1 x 72 11.1 us with 1, 10.3 with 2, 13.5 with 3.
 constexpr int kMinShare = 2;
 
 template <int HD>
