@@ -17,8 +17,9 @@
 //   * logits above a threshold go to a list in shared memory, and `count` logits
 //     are known to reach the threshold.  A CTA's first chunk (a group a thread) sets it from
 //     the threads' own maxima, of which the warps' largest few are taken.  Then come stretches
-//     without a barrier, each as long as all before it: each puts in some `count` logits,
-//     and one comparison a group skips the others.
+//     without a barrier, each kGrow times as long as all before it: each puts in some kGrow x
+//     `count` logits, and one comparison a group skips the others.  Vectors that have one are set
+//     aside whole and looked at by all threads at the stretch's end, where the threshold rises.
 //   * A stretch that puts in more than the list holds (rising logits) is looked at
 //     again chunk by chunk, each with a threshold of its own, and a chunk that still has too
 //     many (equal logits) is searched round by round.
@@ -34,6 +35,12 @@ constexpr int kVecs = 4;            // 16-byte vectors of a thread in a group
 constexpr int kList = 1024;         // entries of the list
 constexpr int kFound = 512;         // vectors that may have some for it
 constexpr int kRank = 384;          // entries that are put in order by counting
+constexpr int kCounted = 64;        // and those of which that is the quicker way to the largest
+                                    // (16 x 4 rows of 32000, 8 of them 13.6 us, 15.7 with 32; 64 of
+                                    // 32 x 8 rows of 131072 56.5, 62.8 with 128, 75.3 with 384)
+// A stretch is so many times as long as all before it: it puts in kGrow x `count` logits.  32 x 8 rows
+// of 131072 fp32, 16 and 64 of them: 40.6 and 56.5 us with 1, 38.3 and 52.0 with 3, 38.6 and 52.2 with 5.
+constexpr int kGrow = 3;
 constexpr int kGroups = 1000;       // counters of a launch (the workspace's first 4096 bytes)
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -293,13 +300,55 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_select(const BeamArgs 
         }
       }
   };
+  int had = 0;  // entries of the list
+  // A logit that exactly M of the list's n reach, by bisection, becomes the threshold and they the
+  // list; false where equal logits leave none.
+  auto narrow = [&](int n) {
+    constexpr int kEach = kList / kBeamThreads;
+    uint64_t k[kEach];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = tid + i * kBeamThreads;
+      k[i] = at < n ? s_list[at] : 0;
+      top = max(top, (uint32_t)(k[i] >> 32));
+    }
+    top = __reduce_max_sync(kAll, top);
+    if (lane == 0) s_warp[warp] = top;
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    for (int w = 0; w < kBeamWarps; ++w) top = max(top, s_warp[w]);
+    uint32_t low = Logit<float>::key(thr), high = top;  // more than M reach low; fewer, high + 1
+    bool exact = false;
+    while (low < high && !exact) {
+      const uint32_t mid = high - (high - low) / 2;  // above low
+      int reach = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (i * kBeamThreads < n) reach += __syncthreads_count((uint32_t)(k[i] >> 32) >= mid);
+      exact = reach == M;
+      if (reach >= M) low = mid;
+      else high = mid - 1;
+    }
+    if (exact) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if ((uint32_t)(k[i] >> 32) >= low) s_list[atomicAdd(&s_count, 1)] = k[i];
+      thr = Logit<float>::value(low);
+      had = M;
+    } else if (tid == 0) {
+      s_count = n;
+    }
+    __syncthreads();
+    return exact;
+  };
   // The list holds every logit so far that is above thr, and of those that reach it as
   // many as `count` needs.
-  int had = 0, summed = lo, one_by_one = lo + kChunk;
+  int summed = lo, one_by_one = lo + kChunk;
   for (int pos = lo; pos < hi;) {
     const bool chunk = pos < one_by_one;
     some = false;
-    const int end = min(pos + (chunk ? kChunk : max(kChunk, (pos - lo) / kChunk * kChunk)), hi);
+    const int end = min(pos + (chunk ? kChunk : max(kChunk, kGrow * ((pos - lo) / kChunk * kChunk))), hi);
     for (int c = pos; c < end; c += kChunk) {
       take(c);
       if (c >= summed) absorb();
@@ -347,6 +396,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_select(const BeamArgs 
     if (n <= M) continue;
     // The `count` best so far become the list, the last of them the threshold: by counting
     // what is above each, or round by round of a long list, and of the chunk where it overflowed.
+    if (n > kCounted && n <= kList && narrow(n)) continue;
     if (n <= kRank) {
       rank_all(n, [&](int j, int i) { return s_list[j] > s_list[i]; },
                [&](int i, int above) {

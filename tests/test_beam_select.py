@@ -124,6 +124,29 @@ def test_equal_and_sorted_logits(dtype, count):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("count", [1, 16, 64])
+def test_long_stretches_of_sorted_and_tied_logits(dtype, count):
+    """As many rows as leave each to one CTA, so that its stretches grow: rising (every stretch
+    overflows), falling, noise of few values (ties at the threshold) and of many, a late plateau."""
+    from moeinfra_b200 import kernels
+
+    vocab, rows = 70001, 600
+    ramp = torch.arange(vocab, dtype=torch.float32)
+    noise = torch.randn(vocab, generator=torch.Generator().manual_seed(5))
+    x = torch.stack([ramp / 8192, -ramp / 8192, noise.mul(2).round(), noise, noise + ramp / 65536,
+                     torch.where(ramp < 30000, noise, 5.0),
+                     torch.where((ramp > 9000) & (ramp < 9000 + count), 7.0, noise.clamp(max=3))])
+    x = x.to(dtype).cuda()
+    for k in range(len(x)):
+        got = kernels.beam_select(x[k:k + 1].expand(rows, vocab), torch.zeros(rows, 1, device="cuda"), count)
+        want = torch.sort(x[k].cpu(), descending=True, stable=True).indices[:count]
+        assert torch.equal(got[2].cpu(), want.expand(rows, count)), k
+        assert not bool(got[1].any()) and bool((got[0] == got[0][:1]).all())
+    kernels.check_device()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_infinities_and_nan(dtype):
     from moeinfra_b200 import kernels
 
