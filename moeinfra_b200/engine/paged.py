@@ -180,13 +180,14 @@ class PagedDenseStack(DenseStack):
         [nodes] or [B, nodes], a node's steps from its root (0 for one that follows the cached
         tokens); ``visible`` as :func:`~moeinfra_b200.kernels.tree_attention` takes it, of one tree
         or of each.  Node i's keys and values go to position ``lengths[b] + i`` (the cache must hold
-        pages for them); ``accept`` then keeps a path."""
+        pages for them); ``accept`` then keeps a path.  ``lengths[b] < 0`` is no sequence: nothing is
+        appended, its nodes see nothing."""
         cfg, (B, T) = self.cfg, ids.shape
         table = self.cache.block_table[:B]
         if visible.ndim == 2:
             visible = visible.expand(B, *visible.shape)
         start = lengths[:, None]
-        pos = (start + depths).to(torch.int32).reshape(-1)
+        pos = (start + depths).masked_fill(start < 0, -1).to(torch.int32).reshape(-1)
         nodes = torch.arange(T, dtype=torch.int32, device=self.device)
         slots = (start + nodes).reshape(-1)
         seq = torch.arange(B, dtype=torch.int32, device=self.device).repeat_interleave(T)

@@ -164,6 +164,34 @@ def test_verified_trees_continue_as_decoding_does(heads, kv, hd, page):
         assert float((got[b] - y).norm() / y.norm()) < CLOSE
 
 
+@gpu
+@torch.no_grad()
+def test_verify_passes_over_rows_without_a_sequence():
+    from moeinfra_b200 import kernels
+
+    stack = _stack()
+    rows = _ragged([12, 20])[0]
+    stack.cache.reserve([40, 40])
+    stack.prefill([r.clone() for r in rows])
+    lengths = torch.tensor([12, -1], dtype=torch.int32, device="cuda")
+    ids = torch.tensor([[5, 6, 7, 8]] * 2, device="cuda")
+    depths = torch.tensor([0, 1, 1, 2], dtype=torch.int32, device="cuda")
+    visible = kernels.tree_masks([-1, 0, 0, 2]).cuda()
+    own = stack.cache.block_table[1][stack.cache.block_table[1] >= 0].long()
+    before = [p[:, own].clone() for p in (stack.cache.k_pages, stack.cache.v_pages)]
+    logits = stack.verify(ids, lengths, depths, visible)
+    kernels.check_device()
+    for pages, was in zip((stack.cache.k_pages, stack.cache.v_pages), before):
+        assert torch.equal(pages[:, own], was)
+    alone = stack.verify(ids[:1], lengths[:1], depths, visible)
+    assert float((logits[0] - alone[0]).float().norm() / alone.float().norm()) < CLOSE
+    keep = torch.tensor([[0, 2], [0, 2]], dtype=torch.int32, device="cuda")
+    assert stack.accept(lengths, keep).tolist() == [14, -1]
+    for pages, was in zip((stack.cache.k_pages, stack.cache.v_pages), before):
+        assert torch.equal(pages[:, own], was)
+    kernels.check_device()
+
+
 def _beams(cfg, ids, mask, n, beams):
     from moeinfra_b200.engine.engine import InferenceEngine
     from moeinfra_b200.engine.types import ForwardRequest
