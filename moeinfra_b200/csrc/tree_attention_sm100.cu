@@ -25,6 +25,7 @@
 //                     V past a sequence's end becomes zeros in shared memory: what lies
 //                     in a page there has no effect
 //     warps 9, 10     tcgen05.mma of pipeline 0 and 1: S = Q K^T, O += P V
+//   * Few short units have a CTA each (kWholeSteps).
 //   * What CTAs hold of a unit that is cut is joined by a second kernel, in the order of
 //     its keys; the order of all sums depends on the shapes, the lengths and the GPU only.
 //
@@ -37,12 +38,14 @@
 // (165 MB, 3.7 TB/s: a unit's 9 steps stream at a copy's rate, its end and the next one's start do
 // not; the join 4 us); 64 nodes over 16 x 2049..4095 bf16 70 us (shared memory: Q K^T reads 6 KB
 // for 32 cycles of products, 1280 of a step's 1640 cycles; 38 MB of pieces of cut units); 27 nodes
-// over 65537 + 131071 bf16 154 us (888 MB, 5.8 TB/s); 16 nodes over 72 10.3 us, a chain of latencies.
+// over 65537 + 131071 bf16 154 us (888 MB, 5.8 TB/s); 16 nodes over 72 9.3 us, a chain of latencies.
 //
 // O is rescaled only when a row's maximum grew by more than 2^8 since the reference
 // in use: probabilities stay below 2^8, O and l are sums of the same factor.
 // Every wait is bounded: on a timeout the error word is set, the roles stop, and
 // the CTA waits (bounded) for what it issued before it frees its tensor memory.
+#include <algorithm>
+
 #include "sm100_ptx.cuh"
 #include "tree.cuh"
 
@@ -70,6 +73,12 @@ constexpr float prob_shift() { return T::kBf16 ? 0.f : 7.f; }
 constexpr int kStart = 3;
 // Smallest share of a CTA in steps: 16 nodes over 1 x 72 11.1 us with 1, 10.3 with 2, 13.5 with 3.
 constexpr int kMinShare = 2;
+// Steps of a table up to which units have CTAs of their own, where the GPU has as many: nothing is
+// joined then.  More where there are many units (own CTAs / even cut, us): 8 units, 16 nodes over 72
+// 9.5 / 10.4, over 300 11.4 / 13.1, over 400 12.7 / 13.2, over 600 14.5 / 13.4, over 1000 18.8 / 13.4;
+// 64 units, 8 nodes over 600 14.6 / 17.2, over 1000 18.6 / 18.9; 128 units, 64 nodes over 250..1000
+// 29.6 / 34.8.
+constexpr int64_t kWholeSteps = 6;
 
 template <int HD>
 struct Cfg {
@@ -99,6 +108,7 @@ struct TreeArgs : TreeRows {
   int tokens;                   // nodes of a tile
   int blocks;                   // blocks of rows (two tiles) of a KV head's part
   int per_seq;                  // units of a sequence
+  bool whole;                   // a CTA has one unit, and none is cut
   int box, box_shift;           // rows of a K or V box, which lie in one page, and their log2
   int page_shift;               // log2 of a page's boxes, or -1
   int4* jobs;                   // [CTAs]: sequence, unit, CTAs and nodes of the cut unit that starts there
@@ -319,7 +329,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = s_tmem;
   const int total = run * a.per_seq;
   const int share = max((int)(((uint32_t)total + gridDim.x - 1) / gridDim.x), kMinShare + kStart);
-  const int lo = (int)min((int64_t)blockIdx.x * share, (int64_t)total), hi = (int)min((int64_t)lo + share, (int64_t)total);
+  int lo = (int)min((int64_t)blockIdx.x * share, (int64_t)total), hi = (int)min((int64_t)lo + share, (int64_t)total);
+  if (a.whole) {  // the unit that the CTA has to itself
+    const int b = blockIdx.x / (uint32_t)a.per_seq, u = blockIdx.x - b * a.per_seq;
+    const int places = prefix[b + 1] - prefix[b];
+    lo = prefix[b] * a.per_seq + u * places;
+    hi = lo + places;
+  }
 
   // The next item; false at the end or after a timeout (then ok is false).
   uint32_t n_it = 0;
@@ -954,6 +970,7 @@ int launch_tree(const TreeArgs& a, const CUtensorMap& q, const CUtensorMap& k, c
                  k, v) != cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
+  if (a.whole) return MOE_OK;
   if (launch_pdl(k_tree_join<T, HD>, dim3(grid, 2 * kM / 32 * (HD / kJoinCols) / (kJoinThreads / 32)), dim3(kJoinThreads), 0, s, a) != cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
@@ -984,7 +1001,9 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
       (c.kv.seqs > 1 && c.q_seq_stride < c.heads * hd) || c.visible_seq_stride < 0 ||
       c.visible_node_stride < 0)
     return MOE_ERR_INVALID_ARG;
-  if (c.kv.page_size % 16 || c.kv.seqs > kMaxSeqs || c.nodes > kMaxNodes || c.kv.num_pages > INT32_MAX)
+  // Places of boxes are looked up some thousand positions past a table's end, in 32 bits.
+  if (c.kv.page_size % 16 || c.kv.seqs > kMaxSeqs || c.nodes > kMaxNodes || c.kv.num_pages > INT32_MAX ||
+      c.kv.max_pages * c.kv.page_size > 1 << 30)
     return MOE_ERR_UNSUPPORTED;
   if (c.kv.seqs == 0 || c.nodes == 0) return MOE_OK;
   if (!c.q || !c.lengths || !c.visible || !c.out ||
@@ -1057,7 +1076,9 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
       !kv_map(&mk, c.kv.k_pages, c.kv.k_page_stride) || !kv_map(&mv, c.kv.v_pages, c.kv.v_page_stride))
     return MOE_ERR_CUDA;
   const int64_t line = c.kv.seqs * per_seq * steps, most = ceil_div(line, kMinShare + kStart);
-  const int sms = sm_count(), grid = static_cast<int>(most < 1 ? 1 : most < sms ? most : sms);
+  const int64_t units = c.kv.seqs * per_seq, sms = sm_count();
+  a.whole = units <= sms && steps - kStart <= std::max(kWholeSteps, units / 6);
+  const int grid = static_cast<int>(a.whole ? units : most < 1 ? 1 : most < sms ? most : sms);
   if (bf16)
     return hd == 64 ? launch_tree<BF16, 64>(a, mq, mk, mv, grid, s)
                     : launch_tree<BF16, 128>(a, mq, mk, mv, grid, s);

@@ -303,15 +303,16 @@ def test_graphs_follow_their_inputs_side_by_side(nodes):
 
 
 @gpu
-def test_bad_lengths_and_pages_are_reported():
+@pytest.mark.parametrize("nodes", [3, 20])
+def test_bad_lengths_and_pages_are_reported(nodes):
     from moeinfra_b200 import kernels
 
     H, KV, hd, page = 4, 2, 64, 16
     kp, vp = (_cache(2, KV, page, hd, torch.float16, s) for s in (8, 9))
-    q = torch.ones(1, 3, H, hd, dtype=torch.float16, device="cuda")
-    vis = _trees(1, 3, 0).cuda()
-    for table, n, count in (([0, 1], 30, 3), ([0, 7], 29, 3), ([-1, 0], 2, 3), ([0, 1], 4, 4),
-                            ([0, 1], 2 ** 31 - 1, 3)):
+    q = torch.ones(1, nodes, H, hd, dtype=torch.float16, device="cuda")
+    vis = _trees(1, nodes, 0).cuda()
+    for table, n, count in (([0, 1], 33 - nodes, nodes), ([0, 7], 32 - nodes, nodes), ([-1, 0], 2, nodes),
+                            ([0, 1], 4, nodes + 1), ([0, 1], 2 ** 31 - 1, nodes)):
         kernels.tree_attention(q, kp, vp, torch.tensor([table], dtype=torch.int32, device="cuda"),
                                torch.tensor([n], dtype=torch.int32, device="cuda"), vis,
                                counts=torch.tensor([count], dtype=torch.int32, device="cuda"))
@@ -449,7 +450,7 @@ def test_refusals_on_the_host():
     assert call(scale=math.inf) == 1 and call(qn=255) == 1 and call(qs=0) == 1 and call(vs=-1) == 1
     assert call(q=0) == 1 and call(lengths=0) == 1 and call(visible=0) == 1 and call(out=0) == 1
     assert call(page=24, ks=4096) == 2 and call(seqs=2049) == 2 and call(nodes=1025) == 2
-    assert call(hd=96, ks=4096) == 2
+    assert call(hd=96, ks=4096) == 2 and call(most=(1 << 26) + 1, ts=1 << 27) == 2
     assert call(dt=2) == 2 and call(seqs=0) == 0 and call(nodes=0) == 0
     assert call(q=fake + 8) == 5 and call(qn=260) == 5 and call(visible=fake + 4) == 5
     assert call(ws=0) == 4 and call(nbytes=4096) == 4 and call(ws=fake + 8) == 5
