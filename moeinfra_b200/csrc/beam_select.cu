@@ -162,18 +162,18 @@ __device__ __forceinline__ void rank_all(int n, A above, O out) {
     if (i < n && part == 0) out(i, count);
   }
 }
-// A key that at least `count` of the threads' keys reach, or 0 where no warp is full: the
-// smallest of the full warps' ceil(count / full warps)-th largest.  Keys 0 do not count.
+// A key that at least `count` of the threads' keys reach, or 0: the smallest of the warps'
+// ceil(count / warps)-th largest, of those warps that have 16 keys.  Keys 0 do not count.
 __device__ __forceinline__ uint32_t reached_by(uint32_t key, int count, uint32_t* s_warp) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   if (lane == 0) s_warp[warp] = 0;
-  const bool full = __all_sync(kAll, key != 0);
+  const bool full = __popc(__ballot_sync(kAll, key != 0)) >= 16;
   const int warps = __syncthreads_count(full) / 32;
   if (warps == 0) return 0;
   const int each = (count + warps - 1) / warps;
   if (full) {
     uint32_t top = 0;
-    for (int i = 0; i < each; ++i) {
+    for (int i = 0; i < min(each, 16); ++i) {
       top = __reduce_max_sync(kAll, key);
       const uint32_t who = __ballot_sync(kAll, key == top);
       if (lane == __ffs(who) - 1) key = 0;
@@ -184,7 +184,7 @@ __device__ __forceinline__ uint32_t reached_by(uint32_t key, int count, uint32_t
   uint32_t low = 0xFFFFFFFFu;  // warps that are not full have left 0
   for (int w = 0; w < kBeamWarps; ++w) low = min(low, s_warp[w] - 1u);
   __syncthreads();
-  return each > 32 ? 0 : low + 1;
+  return each > 16 ? 0 : low + 1;
 }
 
 // The sum of exponentials of a vector below m: ordinary arithmetic where all goes well.
@@ -471,10 +471,10 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_select(const BeamArgs 
   __threadfence();
   if (tid == 0) a.done[group] = 0;
   const double2* sums = a.sums + (int64_t)group * parts;
-  // A thread's first key is on its way while the sums are joined.  Each warp looks at every
-  // 8th, so that none has a poor row's alone.
+  // A thread's first key is on its way while the sums are joined.  Each warp looks at one of
+  // every 8, so that none has a poor row's alone, nor all parts' last (their keys may be in order).
   const uint64_t* keys = a.keys + (int64_t)group * parts * M;
-  const int all = parts * M, per_beam = a.splits * M, at0 = lane * kBeamWarps + warp;
+  const int all = parts * M, per_beam = a.splits * M, at0 = lane * kBeamWarps + (warp + lane) % kBeamWarps;
   const uint64_t key0 = at0 < all ? __ldcg(keys + at0) : 0;
   const float* scores = a.scores + (int64_t)group * a.beams;
   for (int k = warp; k < a.beams; k += kBeamWarps) {  // a row's parts: at most 64

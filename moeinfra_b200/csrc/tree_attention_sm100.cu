@@ -25,10 +25,9 @@
 //                     V past a sequence's end becomes zeros in shared memory: what lies
 //                     in a page there has no effect
 //     warps 9, 10     tcgen05.mma of pipeline 0 and 1: S = Q K^T, O += P V
-//   * Few short units have a CTA each (kWholeSteps).
 //   * What CTAs hold of a unit that is cut is joined by a second kernel, in the order of
 //     its keys; the order of all sums depends on the shapes, the lengths and the GPU only.
-//
+//     Short units are not cut: a few have a CTA each, of many the line is cut between them.
 //   * Keys and values stand in one ring in the order of their use, and both MMA warps walk it tile
 //     by tile: a barrier's parity tells one phase from the next only.  The keys are ahead of the
 //     values by a step of a pipeline's own, so that its next scores are on their way during a softmax.
@@ -79,6 +78,10 @@ constexpr int kMinShare = 2;
 // 64 units, 8 nodes over 600 14.6 / 17.2, over 1000 18.6 / 18.9; 128 units, 64 nodes over 250..1000
 // 29.6 / 34.8.
 constexpr int64_t kWholeSteps = 6;
+// And up to which the line is cut between units where there are more (8 nodes, between / anywhere):
+// 64 x 160..200 26.9 / 31.6, 64 x 320..400 36.0 / 37.5, 64 x 8..200 25.2 / 27.3; but 64 x 512..640
+// 44.4 / 44.4, 64 x 720..900 54.6 / 51.2, 20 x 512..640 25.0 / 23.2.
+constexpr int kBetweenSteps = 8;
 
 template <int HD>
 struct Cfg {
@@ -108,7 +111,7 @@ struct TreeArgs : TreeRows {
   int tokens;                   // nodes of a tile
   int blocks;                   // blocks of rows (two tiles) of a KV head's part
   int per_seq;                  // units of a sequence
-  bool whole;                   // a CTA has one unit, and none is cut
+  bool whole, between;          // a CTA has one unit; the line is cut between units: then none is cut
   int box, box_shift;           // rows of a K or V box, which lie in one page, and their log2
   int page_shift;               // log2 of a page's boxes, or -1
   int4* jobs;                   // [CTAs]: sequence, unit, CTAs and nodes of the cut unit that starts there
@@ -178,6 +181,14 @@ struct Piece {
     const int first = x - r + u * (n + kStart) + kStart;
     left = lo - first;
     end = hi - first;
+  }
+  // The place between units that is nearest to place x.
+  static __device__ __forceinline__ int between(const TreeArgs& a, const int* prefix, int x, int total) {
+    if (x >= total) return total;
+    Piece p;
+    p.find(a, prefix, x, x, x);
+    const int places = p.n + kStart, in = p.left + kStart;
+    return x - in + (2 * in >= places ? places : 0);
   }
   __device__ __forceinline__ bool cut() {  // false: the CTA has no step of the unit
     s0 = max(left, 0);
@@ -598,6 +609,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int boxes = kN / a.box, page_boxes = a.kv.page_size / a.box;
     uint32_t g = 0, n_q0 = 0, n_q1 = 0, n_tail = 0, ones = 0;
     Piece pc;
+    if (a.between) {
+      const int x = Piece::between(a, prefix, lane & 1 ? hi : lo, total);
+      lo = __shfl_sync(0xffffffffu, x, 0);
+      hi = __shfl_sync(0xffffffffu, x, 1);
+    }
     bool more = !is_v && pc.start(a, prefix, lo, hi);
     int len = 0, keys = 0, of = -1;  // of sequence `of`
     // The item after the one at hand, and its first 64 boxes' pages, on their way while this one's
@@ -970,7 +986,7 @@ int launch_tree(const TreeArgs& a, const CUtensorMap& q, const CUtensorMap& k, c
                  k, v) != cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
-  if (a.whole) return MOE_OK;
+  if (a.whole || a.between) return MOE_OK;
   if (launch_pdl(k_tree_join<T, HD>, dim3(grid, 2 * kM / 32 * (HD / kJoinCols) / (kJoinThreads / 32)), dim3(kJoinThreads), 0, s, a) != cudaSuccess)
     return MOE_ERR_CUDA;
   MOE_CHECK_LAUNCH();
@@ -1078,6 +1094,7 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
   const int64_t line = c.kv.seqs * per_seq * steps, most = ceil_div(line, kMinShare + kStart);
   const int64_t units = c.kv.seqs * per_seq, sms = sm_count();
   a.whole = units <= sms && steps - kStart <= std::max(kWholeSteps, units / 6);
+  a.between = !a.whole && steps - kStart <= kBetweenSteps;
   const int grid = static_cast<int>(a.whole ? units : most < 1 ? 1 : most < sms ? most : sms);
   if (bf16)
     return hd == 64 ? launch_tree<BF16, 64>(a, mq, mk, mv, grid, s)
