@@ -105,7 +105,8 @@ def test_heads(dtype, hd, H, KV, nodes):
     ([0], 16, 1), ([1024], 16, 8), ([3000], 64, 5), ([5000, 1, 0, 700], 64, 33),
     ([2047, 2048, 2049], 48, 12), ([257] * 40, 32, 9), ([31, 4000] * 20, 128, 4), ([1] * 300, 16, 2),
     ([-1] * 50 + [1500] + [-1] * 40, 16, 6), ([20000], 16, 70), ([300], 80, 200), ([0, 3], 16, 129),
-    ([40000, 7], 96, 3)])
+    ([40000, 7], 96, 3), ([0, 1, 400, 64, -1, 250] * 20, 16, 9), ([0, 1, 700, 64, -1, 250] * 20, 16, 9),
+    ([55] * 75, 64, 9), ([119, -1, -1, -1] * 38 + [0], 16, 9)])
 def test_lengths(lens, page, nodes):
     """Units in a CTA's share and over many CTAs, several blocks of rows, empty sequences between."""
     H, KV, hd = 8, 2, 64
