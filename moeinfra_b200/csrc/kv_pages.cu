@@ -7,9 +7,9 @@
 // a row is about to write into a page that others list too, and there only the
 // positions that are filled.  No counterpart in the reference (one sequence
 // over a growing DynamicCache, engine/engine.py:326-378).
-// Measured in a graph (8 KV heads of 128, fp16 but the last): fork of 1 x 4 rows, 32 layers 9.2 us, of
+// Measured in a graph (8 KV heads of 128, fp16 but the last): fork of 1 x 4 rows, 32 layers 8.7 us, of
 // 16 x 4, pages of 64 36.6 us (180 MB, 4.9 TB/s), of 32 x 8 rows, 8 layers bf16 44 us, 12 of them the
-// tables; nodes of 1 sequence, 32 layers 3.7 us, of 64 11.8 us (34 MB).
+// tables; nodes of 1 sequence, 32 layers 3.5 us, of 64 11.9 us (34 MB).
 #include "paged.cuh"
 
 namespace moe {
