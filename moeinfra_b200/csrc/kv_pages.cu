@@ -86,6 +86,15 @@ __global__ void __launch_bounds__(kForkThreads) k_fork_tables(const ForkArgs a) 
   pdl_wait();
   auto listed = [&](int g) { return g >= 0 && g < a.num_pages; };
   const int c0 = blockIdx.x << a.col_shift;
+  // The first entries are on their way while the parents are looked at.
+  constexpr int kFirst = 4;
+  auto entry_at = [&](int e) {
+    const int i = e >> a.col_shift, col = c0 + (e & (cols - 1));
+    return e < S << a.col_shift && col < a.max_pages ? a.table[i * a.table_stride + col] : -1;
+  };
+  int first[kFirst];
+#pragma unroll
+  for (int u = 0; u < kFirst; ++u) first[u] = entry_at(tid + u * threads);
   for (int i = tid; i < S; i += threads) {
     int p = a.parents[i];
     s_old[i] = a.lengths[i];  // written by the last CTA alone, after all have read
@@ -95,11 +104,11 @@ __global__ void __launch_bounds__(kForkThreads) k_fork_tables(const ForkArgs a) 
     }
     s_par[i] = max(p, -1);
   }
+#pragma unroll
+  for (int u = 0; u < kFirst; ++u)
+    if (tid + u * threads < S << a.col_shift) s_tile[tid + u * threads] = first[u];
 #pragma unroll 4
-  for (int e = tid; e < S << a.col_shift; e += threads) {
-    const int i = e >> a.col_shift, col = c0 + (e & (cols - 1));
-    s_tile[e] = col < a.max_pages ? a.table[i * a.table_stride + col] : -1;
-  }
+  for (int e = tid + kFirst * threads; e < S << a.col_shift; e += threads) s_tile[e] = entry_at(e);
   __syncthreads();
   for (int e = tid; e < S << a.col_shift; e += threads) {
     const int i = e >> a.col_shift, c = e & (cols - 1), p = s_par[i];
@@ -155,6 +164,15 @@ __global__ void __launch_bounds__(kForkThreads) k_fork_tables(const ForkArgs a) 
       g = -1;
     }
     const int holders = use && g >= 0 ? __ldcg(a.refs + g) : 0;
+    // The counts where the search for free pages goes on come with it.
+    constexpr int kLook = 8;  // that a thread looks at in a go
+    int32_t r[kLook];
+    auto look = [&](int64_t from) {
+#pragma unroll
+      for (int u = 0; u < kLook; ++u) r[u] = from + u < a.num_pages ? __ldcg(a.refs + from + u) : 1;
+    };
+    const int64_t ahead = s_cursor;
+    look(ahead + tid * kLook);
     // Of the rows that ask in this round and list a page, those before one leave it to
     // it (those of earlier rounds have): the last keeps it.
     const int held = holders > 1 ? g : -1 - tid;
@@ -173,12 +191,9 @@ __global__ void __launch_bounds__(kForkThreads) k_fork_tables(const ForkArgs a) 
     const bool need = use && (copy || g < 0);
     int wanted, found = 0;
     const int turn = block_scan(need, s_warp, wanted);
-    constexpr int kLook = 8;  // counts a thread looks at in a go
     while (found < wanted && s_cursor < a.num_pages) {
       const int64_t from = s_cursor + tid * kLook;
-      int32_t r[kLook];
-#pragma unroll
-      for (int u = 0; u < kLook; ++u) r[u] = from + u < a.num_pages ? __ldcg(a.refs + from + u) : 1;
+      if (s_cursor != ahead) look(from);
       int mine = 0, more;
 #pragma unroll
       for (int u = 0; u < kLook; ++u) mine += r[u] == 0;
@@ -276,8 +291,10 @@ __global__ void __launch_bounds__(kKeepThreads) k_keep_nodes(const KeepArgs a) {
   pdl_wait();
   const int tid = threadIdx.x, b = blockIdx.x / (uint32_t)a.parts;
   const int part = blockIdx.x - b * a.parts, page = a.kv.page_size;
-  const int len = a.lengths[b];
   const int32_t *list = a.keep + b * a.keep_stride, *table = a.table + b * a.table_stride;
+  // The list's start comes with the length, not after it.
+  int node = tid < a.most ? list[tid] : -1, node_before = tid > 0 && tid < a.most ? list[tid - 1] : -1;
+  const int len = a.lengths[b];
   // This thread's pieces.
   constexpr int kPer = HD / 8;
   const uint16_t* from[kPieces];
@@ -296,14 +313,18 @@ __global__ void __launch_bounds__(kKeepThreads) k_keep_nodes(const KeepArgs a) {
   int kept = 0;
   for (int base_j = 0; len >= 0 && base_j < a.most; base_j += kKeepThreads) {
     if (tid == 0) s_end = s_bad = kKeepThreads;
+    const int j = base_j + tid;
+    if (base_j > 0) {
+      node = j < a.most ? list[j] : -1;
+      node_before = j < a.most ? list[j - 1] : -1;
+    }
     __syncthreads();
-    const int j = base_j + tid, node = j < a.most ? list[j] : -1;
     if (node < 0) atomicMin(&s_end, tid);
     __syncthreads();
     int4 move = make_int4(-1, 0, 0, 0);
     if (tid < s_end) {  // a list that falls or leaves the table ends there
       const int64_t src = (int64_t)len + node, dst = (int64_t)len + j;
-      bool ok = node > (j > 0 ? list[j - 1] : -1) && src < (int64_t)a.max_pages * page;
+      bool ok = node > node_before && src < (int64_t)a.max_pages * page;
       if (ok) {
         move = make_int4(table[src / page], src % page, table[dst / page], dst % page);
         ok = move.x >= 0 && move.x < a.num_pages && move.z >= 0 && move.z < a.num_pages;
