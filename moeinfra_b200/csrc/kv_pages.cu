@@ -7,9 +7,9 @@
 // a row is about to write into a page that others list too, and there only the
 // positions that are filled.  No counterpart in the reference (one sequence
 // over a growing DynamicCache, engine/engine.py:326-378).
-// Measured in a graph (8 KV heads of 128, fp16 but the last): fork of 1 x 4 rows, 32 layers 8.7 us, of
-// 16 x 4, pages of 64 36.6 us (180 MB, 4.9 TB/s), of 32 x 8 rows, 8 layers bf16 44 us, 12 of them the
-// tables; nodes of 1 sequence, 32 layers 3.5 us, of 64 11.9 us (34 MB).
+// Measured in a graph (8 KV heads of 128, fp16 but the last): fork of 1 x 4 rows, 32 layers 8.5 us, of
+// 16 x 4, pages of 64 35.8 us (180 MB, 5.0 TB/s), of 32 x 8 rows, 8 layers bf16 43 us, 11 of them the
+// tables; nodes of 1 sequence, 32 layers 3.2 us, of 64 9.8 us (34 MB).
 #include "paged.cuh"
 
 namespace moe {
@@ -276,15 +276,16 @@ struct KeepArgs {
   int32_t* new_lengths;
 };
 
-constexpr int kKeepThreads = 256, kPieces = 2;
+constexpr int kKeepThreads = 128, kPieces = 2;
 
 // A thread has kPieces 16-byte pieces of (layer, keys or values, head) rows and
 // moves them for every kept node of its sequence: lists rise, so a node's place is
 // never read after it was written, and pieces have nothing to do with each other.
-// Bound by latency (length, list, pages, rows), so all sequences' CTAs are resident at
-// once where that is possible: 64 x 32 layers x 8 heads of 128 take 1024 CTAs.
+// Bound by latency (length and list, pages, rows) and by how many rows are on their way: 64
+// sequences x 32 layers x 8 heads of 128 take 2048 CTAs, 8 to an SM at once, 9.8 us; 10.1 without the
+// bound on registers, 11.4 with CTAs of 256, 11.4 with one piece a thread.
 template <int HD>
-__global__ void __launch_bounds__(kKeepThreads) k_keep_nodes(const KeepArgs a) {
+__global__ void __launch_bounds__(kKeepThreads, 8) k_keep_nodes(const KeepArgs a) {
   __shared__ int4 s_move[kKeepThreads];  // source page and slot, destination page and slot
   __shared__ int s_warp[32], s_end, s_bad;
   pdl_trigger();

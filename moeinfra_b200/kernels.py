@@ -1092,7 +1092,7 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     if counts is not None:
         _serve_check(what, dev, ("counts", counts, torch.int32, (seqs,), 1))
     if out is None:
-        out = q.new_empty((seqs, nodes, heads, hd))
+        out = torch.empty_like(q) if plain else q.new_empty((seqs, nodes, heads, hd))
     else:
         _serve_check(what, dev, ("out", out, dt, (seqs, nodes, heads, hd), 4))
     if seqs == 0 or nodes == 0:
@@ -1212,7 +1212,7 @@ def keep_nodes(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.
         _serve_check(what, dev, ("lengths", lengths, torch.int32, (seqs,), 1),
                      ("keep", keep, torch.int32, (seqs, None), 1))
     most = keep.shape[1]
-    out = lengths.new_empty(seqs)
+    out = torch.empty_like(lengths)
     n_pages, kv, page, hd, k_page, v_page, layers, k_layer, v_layer = cache
     strides = ((max_pages, most) if plain or not seqs else (_outer_stride(block_table),
                                                             _outer_stride(keep)))
@@ -1269,8 +1269,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int | None = 
     if not (1 <= beams <= 64 and 1 <= count <= 64):
         raise ValueError(f"{what}: 1 to 64 beams and 1 to 64 continuations are served, got {beams} "
                          f"and {count}")
-    out = (scores.new_empty((groups, count)), scores.new_empty((groups, count), dtype=torch.int32),
-           scores.new_empty((groups, count), dtype=torch.int64))
+    like = scores if count == beams else scores.new_empty((groups, count))
+    out = (torch.empty_like(like) if like is scores else like, torch.empty_like(like, dtype=torch.int32),
+           torch.empty_like(like, dtype=torch.int64))
     stream = _raw_stream(dev)
     nbytes = _beam_ws_bytes(dev, groups, beams, vocab, count, code)
     if workspace is None:
