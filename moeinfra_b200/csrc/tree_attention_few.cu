@@ -23,7 +23,7 @@ Shape few_shape(const TreeRows& r) {
   s.nt = s.tile <= 8 ? 1 : 2;
   s.units = (int64_t)r.kv.seqs * r.kv.kv_heads;
   s.chunks = ceil_div((int64_t)r.kv.max_pages * r.kv.page_size, kChunk);
-  s.whole = whole_units(s.units, s.chunks);
+  s.whole = true;
   s.ctas = static_cast<int>(s.units);
   return s;
 }
@@ -33,19 +33,23 @@ int launch_few(PagedArgs& a, const Shape& sh, cudaStream_t s) {
   return sh.nt == 1 ? launch_tile<T, HD, 1, true>(a, sh, s) : launch_tile<T, HD, 2, true>(a, sh, s);
 }
 
-// Measured in a graph (bf16, 32 heads of 128 unless said, us; this kernel / the tcgen05 one):
-//   64 x 576 cached keys, 1 node 32.2 / 55.8, 2 nodes 33.7 / 55.6, 4 nodes 39.1 / 56.9;
-//   1 x 72, 2 nodes 6.7 / 10.5, 4 nodes 8.9 / 10.5; 1 x 600 12.8 / 17.4; 8 x 600 12.9 / 19.5;
-//   heads of 64, 64 x 576, 4 nodes 28.8 / 47.5; 32 KV heads, 8 nodes 105 / 172, 16 nodes 130 / 166.
-// Not for 17 to 32 rows (64 x 576, 8 nodes: 77 / 57: four column tiles' sums leave the
-// registers), nor where the even cut of paged_line.cuh would have to share units out
-// (1 x 4000: 26.7 / 17.8, 64 x about 2050 114.6 / 108.8, 2 x about 100000 177 / 167).
-constexpr int kMostRows = 16;
+// Rows, and the table's width in chunks of 16 keys where each unit has a place of its own on the
+// GPU, and where there are more units: a unit is one CTA's here.  In a graph (32 / 8 heads of 128
+// unless said, us; this kernel / the tcgen05 one):
+//   64 x 512..640 cached keys, 1 node 32.0 / 43.7, 2 nodes 33.4 / 44.2, 4 nodes 38.8 / 44.2; heads of
+//   64, 4 nodes 28.7 / 38.9; 32 KV heads, 8 nodes 104 / 130, 16 nodes 128 / 131; of 64, 64 x 20..40,
+//   4 nodes 31.8 / 54.4, 16 nodes 52.9 / 54.7; 1 x 72, 2 nodes 6.2 / 9.4, 4 nodes 8.5 / 9.4;
+//   4 nodes over 1 x 600 12.4 / 12.9, over 8 x 600 12.7 / 14.8.
+// Not for 17 to 32 rows (64 x 512..640, 8 nodes: 77 / 44: four column tiles' sums leave the
+// registers), nor for longer tables (4 nodes over 1 x 800 14.7 / 13.2, over 20 x 500..2000 38.3 /
+// 31.6, over 64 x 500..2000 69.7 / 68.0; but 64 x 250..1000 42.7 / 44.8).
+constexpr int kMostRows = 16, kChunksAlone = 40, kMostChunksOfMany = 64;
 
 }  // namespace
 
 bool tree_is_few(const TreeRows& r) {
-  return (int64_t)r.nodes * r.group <= kMostRows && few_shape(r).whole;
+  const Shape sh = few_shape(r);
+  return sh.tile <= kMostRows && sh.chunks <= (sh.units <= sm_count() ? kChunksAlone : kMostChunksOfMany);
 }
 
 int tree_attention_few(const TreeRows& r, int hd, bool bf16, cudaStream_t s) {
