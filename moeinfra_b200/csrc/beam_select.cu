@@ -27,6 +27,8 @@
 // Measured in a graph: 32 groups of 8 rows of 131072 fp32, 16 of each 38.4 us (134 MB, 3.5 TB/s; 56 %
 // of the issue slots, and the barriers at a stretch's end), 64 of each 51; 16 x 4 rows of 32000 fp16
 // 13.7 us, 1 x 4 10.4, chains of latencies (first chunk, up to three stretches, the join's 4 us).
+#include <algorithm>
+
 #include "sample.cuh"
 
 namespace moe {
@@ -551,12 +553,15 @@ __global__ void __launch_bounds__(kBeamThreads, 4) k_beam_select(const BeamArgs 
   }
 }
 
-// CTAs of a row: as many as the GPU takes at once, four to an SM, but one to an SM where the rows
-// are fewer than that, each with a vector a thread at least.
+// CTAs of a row: as many as the GPU takes at once, four to an SM; where rows are fewer than the SMs
+// one to an SM, each with a vector a thread at least, and more only if each still has four chunks
+// (16 x 8 rows of 37025 fp32 19.9 us, 21.1 with one to an SM; 16 x 8 of 131072 fp16 23.2 / 26.7, 16 x 4
+// of them 17.4 / 20.3; with one chunk each 16 x 4 of 32000 16.0 / 13.7).
 int splits_of(int64_t rows, int64_t vocab, int64_t vec) {
   if (rows < 1) rows = 1;
-  const int64_t sms = sm_count(), most = ceil_div(vocab, vec * kBeamThreads);
-  const int64_t want = rows <= sms ? sms / rows : 4 * sms / rows, s = want < most ? want : most;
+  const int64_t sms = sm_count(), most = ceil_div(vocab, vec * kBeamThreads), full = 4 * sms / rows;
+  const int64_t long_ones = std::min(full, vocab / (vec * kBeamThreads * kVecs * 4));
+  const int64_t want = rows > sms ? full : std::max(sms / rows, long_ones), s = std::min(want, most);
   return static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
