@@ -592,9 +592,12 @@ int moe_sample_tokens(const moe_sample_tokens_args_t* args);
  *   counted in refs as well.  Page by page, row after row: a missing page is taken from
  *   the free ones, the lowest number first (pages that the call itself frees among
  *   them); one that others hold too is replaced by such a page, the filled
- *   positions (those below lengths[i]) copied in every layer.  Without a free page the entry
- *   is -1 and the device error word is set (MOE_ERR_PAGE), as for a parent, length or page
- *   out of range.  seqs <= 8192.  The first 4096 bytes of the workspace must be
+ *   positions (those below lengths[i]) copied in every layer.  A parent with a negative
+ *   length is no sequence: its copies, itself among them, keep that length and its entries
+ *   and are given no page.  An emptied row is a sequence of length 0, which is given its
+ *   first page once it is its own parent: set its length below 0 to have it passed over.
+ *   Without a free page the entry is -1 and the device error word is set (MOE_ERR_PAGE),
+ *   as for a parent or page out of range and a length past the table.  seqs <= 8192.  The first 4096 bytes of the workspace must be
  *   zero before its first call and are left zero. */
 typedef struct moe_fork_pages_args {
   moe_kv_pages_t kv;

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kForkThreads) k_fork_tables(const ForkArgs a) 
   const int page = a.kv.page_size;
   int* s_len = s_tile + (alone ? S << a.col_shift : 0);
   for (int i = tid; i < S; i += threads) {
-    int n = s_par[i] >= 0 ? max(s_old[s_par[i]], 0) : 0;
+    int n = s_par[i] >= 0 ? s_old[s_par[i]] : 0;  // negative: no sequence, which is given no page
     if (n > a.max_pages * page) {  // no table's row holds so many
       set_device_error(kErrPage);
       n = a.max_pages * page;
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kForkThreads) k_fork_tables(const ForkArgs a) 
     const int64_t at = base + tid;
     const int i = static_cast<int>(min(at / a.entries, (int64_t)S - 1));
     const int64_t col = first_of(i) + (at - (int64_t)i * a.entries);
-    const bool use = at < asked && s_par[i] >= 0 && col <= last_of(i);
+    const bool use = at < asked && s_par[i] >= 0 && s_len[i] >= 0 && col <= last_of(i);
     int32_t* entry = a.table + i * a.table_stride + (use ? col : 0);
     int g = -1;
     if (use) g = alone && base == 0 ? s_tile[(s_par[i] << a.col_shift) + (int)col] : __ldcg(entry);

@@ -83,7 +83,8 @@ class PagedKVCache:
         """Sequence i becomes a copy of sequence ``parents[i]`` (-1: it ends), on the device.
 
         ``lengths`` int32, one per sequence, is updated with it; the pages of the next ``room``
-        positions become the sequence's own (:func:`~moeinfra_b200.kernels.fork_pages`)."""
+        positions become the sequence's own (:func:`~moeinfra_b200.kernels.fork_pages`).  A negative
+        length is no sequence and stays; one that ended has length 0."""
         kernels.fork_pages(self.k_pages, self.v_pages, self.block_table[:parents.shape[0]], lengths,
                            parents, self.refs, room)
 

@@ -1151,8 +1151,10 @@ def fork_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.
     :func:`rope_append`, or of all layers, [layers, pages, ...].  ``refs`` int32 [pages]: how many
     entries of the table name each page (0: free), kept up to date; a holder elsewhere (a prefix kept
     for later) adds one to keep its page from being written or freed.  Entries without a page are
-    negative.  When no page is free the entry is -1, which shows in :func:`check_device`, as do
-    parents, lengths and pages out of range.
+    negative.  A row of a negative length is no sequence: it and its copies stay so and are given no
+    page.  A row that ended has length 0: if later calls are to pass it over (a decode step would
+    look for its first page) set its length below 0.  When no page is free the entry is -1, which
+    shows in :func:`check_device`, as do parents and pages out of range and lengths past the table.
 
     ``workspace``: :func:`fork_pages_workspace`, as for :func:`paged_attention`.
     """

@@ -27,9 +27,9 @@ def fork(k_pages, v_pages, table, lengths, parents, refs, room: int = 1) -> bool
         table[i] = torch.tensor(new, dtype=table.dtype)
         lengths[i] = n_old[p] if p >= 0 else 0
     for i, p in enumerate(parents.tolist()):
-        if p < 0 or room == 0:
-            continue
         n = int(lengths[i])
+        if p < 0 or n < 0 or room == 0:
+            continue
         for c in range(n // page, min((n + room - 1) // page + 1, P)):
             g = int(table[i, c])
             if g >= 0 and int(refs[g]) == 1:

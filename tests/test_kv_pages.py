@@ -356,3 +356,31 @@ def test_the_oracle_keeps_its_counts():
         for i, n in enumerate(lengths.tolist()):
             if parents[i] >= 0 and n // 4 < 6:
                 assert int(refs[table[i, n // 4]]) == 1
+
+
+@gpu
+@pytest.mark.parametrize("seqs,max_pages,page,room", [(6, 5, 16, 1), (5, 3, 7, 0), (40, 40, 16, 20),
+                                                       (300, 3, 4, 9), (1500, 2, 1, 1)])
+def test_fork_passes_over_rows_without_a_sequence(seqs, max_pages, page, room):
+    """Rows of a negative length stay so, as do their copies; neither is given a page."""
+    rng = random.Random(seqs)
+    state = _state(rng, seqs, max_pages, page, spare=seqs * (room // page + 2))
+    idle = torch.tensor([rng.random() < 0.4 for _ in range(seqs)])
+    idle[0], idle[1] = True, False
+    state[3][idle] = torch.tensor([rng.choice([-1, -1, -7, -2 ** 31]) for _ in range(seqs)],
+                                  dtype=torch.int32)[idle]
+    for b in range(0, seqs, 2):  # half of them hold no pages
+        if idle[b]:
+            for g in state[2][b].tolist():
+                if g >= 0:
+                    state[4][g] -= 1
+            state[2][b] = -1
+    for parents in (torch.arange(seqs, dtype=torch.int32), torch.zeros(seqs, dtype=torch.int32),
+                    _parents(rng, seqs)):
+        want = [t.clone() for t in state]
+        assert branches.fork(*want[:4], parents, want[4], room)
+        assert torch.equal(want[3], torch.where(parents >= 0, state[3][parents.clamp(min=0).long()], 0))
+        got = _fork(state, parents, room)
+        _equal(got, want)
+        none = want[3] < 0
+        assert torch.equal(want[2][none], state[2][parents[none].long()])
