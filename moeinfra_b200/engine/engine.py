@@ -473,9 +473,9 @@ class InferenceEngine:
             raise ValueError(f"{max(lens) + n - 1} positions exceed engine.max_seq_len={self._max_len}")
         cache, dev = self._stack.cache, self._device
         # A prompt's full pages are shared; from its last, partly filled one on each beam may come to
-        # hold its own, up to the page of the position behind its last token.
-        page = cache.page_size
-        need = sum(m // page + K * ((m + n - 1) // page + 1 - m // page) for m in lens)
+        # hold its own, up to the page of the position behind its last token if the table reaches it.
+        page, width = cache.page_size, cache.block_table.shape[1]
+        need = sum(m // page + K * (min((m + n - 1) // page + 1, width) - m // page) for m in lens)
         if need > cache.refs.numel():
             raise RuntimeError(f"the paged cache has {cache.refs.numel()} pages, {need} may be needed "
                                "(engine.kv_pages)")

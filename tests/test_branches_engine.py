@@ -267,3 +267,21 @@ def test_cache_counts_its_pages():
     assert sorted(c.refs.tolist()) == [0, 0, 0, 0, 1] and int(c.refs[c.block_table[0, 0]]) == 1
     c.clear()
     assert c.free_pages == 5 and not c.refs.any() and bool((c.block_table == -1).all())
+
+
+@gpu
+@pytest.mark.parametrize("K,max_batch", [(2, 2), (4, 4), (2, 4)])
+def test_beams_reach_the_cache_s_last_position(ckpt, K, max_batch):  # noqa: F811
+    """The default pool holds max_batch sequences of max_seq_len, so it does for their beams: the
+    position behind the last one has no page and needs none."""
+    prompts = max_batch // K
+    _, ids, mask = _ragged([5] * prompts)
+    over = PAGED | {"max_batch": max_batch}          # 64 positions in pages of 16
+    a = _beams(_config(ckpt, engine=over), ids, mask, 60, K)
+    b = _beams(_config(ckpt, engine=over | {"kv_pages": 40}), ids, mask, 60, K)
+    assert a.token_ids == b.token_ids and a.scores == b.scores
+    rows = a.token_ids if prompts > 1 else [a.token_ids]
+    assert [len(t) for t in rows] == [60] * prompts
+    _, ids, mask = _ragged([64] * prompts)           # a prompt that fills its table
+    one = _beams(_config(ckpt, engine=over), ids, mask, 1, K)
+    assert len(one.scores) == prompts
