@@ -507,7 +507,7 @@ class InferenceEngine:
             torch.cuda.synchronize(dev)
         t2 = time.perf_counter()
         kernels.check_device(dev)
-        self._last_logits = logits[:, None, :]
+        self._last_logits = logits[:, None, :].clone()  # the next replay writes them again
         timings = {"prefill": (t1 - t0) * 1e3, "decode": (t2 - t1) * 1e3,
                    "cuda_graph_decode": use_graph, "h2d_bytes": sum(
                        p.get("bytes_transferred", 0) for p in self._transfer_scheduler_profile())}
@@ -585,7 +585,7 @@ class InferenceEngine:
                             sampler.turn(i)
                         g.replay()
                         hist[:, i] = ids_buf[:, 0]
-                    self._last_logits = out[:, None, :]
+                    self._last_logits = out[:, None, :].clone()  # the next replay writes out again
                 else:
                     ids_buf = first[:, None].clone()
                     pos_buf = self._positions(B)

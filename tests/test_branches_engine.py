@@ -285,3 +285,23 @@ def test_beams_reach_the_cache_s_last_position(ckpt, K, max_batch):  # noqa: F81
     _, ids, mask = _ragged([64] * prompts)           # a prompt that fills its table
     one = _beams(_config(ckpt, engine=over), ids, mask, 1, K)
     assert len(one.scores) == prompts
+
+
+@gpu
+@pytest.mark.parametrize("over", [{}, {"num_beams": 2}, {"seed": 1}])
+@pytest.mark.parametrize("paged", [True, False])
+def test_a_result_s_logits_stay(ckpt, paged, over):  # noqa: F811
+    """The next request of the same kind does not write into a result that the caller still holds."""
+    from moeinfra_b200.engine.engine import InferenceEngine
+    from moeinfra_b200.engine.types import ForwardRequest, SamplingParams
+
+    if over.get("num_beams") and not paged:
+        pytest.skip("beams need pages")
+    kind = {"sampling": SamplingParams(**over)} if "seed" in over else over
+    first, second = (torch.randint(0, V, (2, 9), generator=torch.Generator().manual_seed(s)) for s in (1, 2))
+    with InferenceEngine(_config(ckpt, engine=(PAGED if paged else {}) | {"max_batch": 4})) as eng:
+        a = eng.generate(ForwardRequest(first, None, 5, **kind))
+        held = a.logits.clone()
+        b = eng.generate(ForwardRequest(second, None, 5, **kind))
+        assert a.stage_timings["cuda_graph_decode"]
+        assert torch.equal(a.logits, held) and not torch.equal(a.logits, b.logits)
