@@ -39,7 +39,8 @@ marks the padding, on either side) over a paged cache of ``kv_pages`` pages
 with either cache.  ``ForwardRequest.num_beams`` searches with beams over the
 paged cache (``max_batch`` counts sequences times beams): the beams of a prompt
 share its pages, and choosing and reordering them is part of the captured step;
-``token_ids`` are each prompt's best beam's, ``scores`` their log-probabilities.
+``token_ids`` are each prompt's best beam's, ``scores`` their log-probabilities, ``logits`` what their
+last tokens were chosen from.
 """
 from __future__ import annotations
 
@@ -502,12 +503,14 @@ class InferenceEngine:
             for i in range(n - 1, -1, -1):
                 path[i] = tokens[i].gather(1, at)
                 at = parents[i].long().gather(1, at)
+            if n > 1:  # of each best beam's parent; a copy: the next replay writes the step's again
+                logits = logits.view(B, K, -1)[torch.arange(B, device=dev), parents[n - 1, :, 0].long()]
             token_ids = path[..., 0].t().cpu().tolist()
             scores = step.scores[:, 0].cpu().tolist()
             torch.cuda.synchronize(dev)
         t2 = time.perf_counter()
         kernels.check_device(dev)
-        self._last_logits = logits[:, None, :].clone()  # the next replay writes them again
+        self._last_logits = logits[:, None, :]
         timings = {"prefill": (t1 - t0) * 1e3, "decode": (t2 - t1) * 1e3,
                    "cuda_graph_decode": use_graph, "h2d_bytes": sum(
                        p.get("bytes_transferred", 0) for p in self._transfer_scheduler_profile())}

@@ -39,7 +39,7 @@ class ForwardRequest:
 
 @dataclasses.dataclass
 class ForwardResult:
-    logits: torch.Tensor
+    logits: torch.Tensor  # [sequences, 1, vocab]: what each sequence's last token was chosen from
     token_ids: list
     ttft_ms: float
     tps: float

@@ -305,3 +305,23 @@ def test_a_result_s_logits_stay(ckpt, paged, over):  # noqa: F811
         b = eng.generate(ForwardRequest(second, None, 5, **kind))
         assert a.stage_timings["cuda_graph_decode"]
         assert torch.equal(a.logits, held) and not torch.equal(a.logits, b.logits)
+
+
+@gpu
+def test_beam_logits_are_the_returned_sequences_(ckpt):  # noqa: F811
+    """[prompts, 1, vocab] for any number of tokens: what each sequence's last token was chosen from."""
+    from moeinfra_b200.engine.engine import InferenceEngine
+    from moeinfra_b200.engine.types import ForwardRequest
+
+    _, ids, mask = _ragged([12, 33])
+    with InferenceEngine(_config(ckpt, engine=PAGED | {"max_batch": 8})) as eng:
+        one = eng.generate(ForwardRequest(ids, mask, 1, num_beams=4))
+        greedy = eng.generate(ForwardRequest(ids, mask, 1))
+        assert one.logits.shape == (2, 1, V) and torch.equal(one.logits, greedy.logits)
+        for n in (2, 9):
+            many = eng.generate(ForwardRequest(ids, mask, n, num_beams=4))
+            assert many.logits.shape == (2, 1, V)
+            step = eng._graphs[2, 4, "beams"][1]
+            rows = step.logits.view(2, 4, V)
+            for b in range(2):
+                assert torch.equal(many.logits[b, 0], rows[b, int(step.parents[b, 0])])
