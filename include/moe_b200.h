@@ -639,8 +639,10 @@ int moe_keep_nodes(const moe_keep_nodes_args_t* args);
  *   in its group) and out_tokens int64 [groups, count]: larger scores first, equal ones by
  *   rising beam, in a beam by falling logit, then rising token.  What scores
  *   -inf (or NaN) is no candidate; places without one are (-inf, 0, 0).  beams
- *   and count <= 64, vocab <= 2^20.  The first 4096 bytes of the workspace must be
- *   zero before its first call and are left zero. */
+ *   and count <= 64, vocab <= 2^20.  The workspace's size depends on the device, count and
+ *   the number of rows alone and rises with both: one made for the largest batch serves
+ *   the smaller ones.  Its first 4096 bytes must be zero before its first call and are
+ *   left zero. */
 typedef struct moe_beam_select_args {
   const void* logits;
   int64_t stride, groups, beams, vocab, dtype;

@@ -597,8 +597,11 @@ extern "C" size_t moe_beam_select_workspace_size(int64_t groups, int64_t beams, 
   if (groups < 0 || beams < 1 || beams > kMostBeams || count < 1 || count > kMostCount || vocab < 1 ||
       groups > INT32_MAX / beams)
     return 0;
-  const int64_t rows = groups * beams;
-  return kSumsAt + rows * splits_of(rows, vocab, dtype == MOE_DTYPE_F32 ? 4 : 8) * (16 + 8 * count);
+  // Rows times splits go up and down with the rows (148 rows of 131072 fp16 have 4 each, 149 have 3)
+  // and never above 4 CTAs to an SM unless each row has one: a workspace made for the largest batch
+  // has to serve the smaller ones.
+  const int64_t most = std::max(groups * beams, (int64_t)4 * sm_count());
+  return kSumsAt + most * (16 + 8 * count);
 }
 
 extern "C" int moe_beam_select(const moe_beam_select_args_t* args) {

@@ -1248,7 +1248,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int | None = 
     row that is -inf but for its end token.
 
     ``workspace``: a zeroed buffer of :func:`beam_select_workspace` that no call on another stream
-    uses at the same time, as for :func:`paged_attention`.
+    uses at the same time, as for :func:`paged_attention`; one made for the largest batch and count
+    serves the smaller ones.
     """
     what = "beam_select"
     if not isinstance(logits, torch.Tensor) or logits.ndim != 2:
@@ -1290,7 +1291,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int | None = 
 
 @_on_first_device
 def beam_select_workspace(logits: torch.Tensor, beams: int, count: int | None = None) -> torch.Tensor:
-    """A workspace for :func:`beam_select` calls on logits of this shape and type."""
+    """A workspace for :func:`beam_select` calls on up to as many rows of logits, and up to ``count``."""
     rows, vocab = logits.shape
     nbytes = _beam_ws_bytes(logits.get_device(), rows // beams, beams, vocab,
                             beams if count is None else count, _DTYPE_CODES[logits.dtype])

@@ -266,3 +266,32 @@ def test_refusals_by_name():
             kernels.beam_select(*args)
     with pytest.raises(ValueError, match="workspace"):
         kernels.beam_select(x, s, workspace=s)
+
+
+def test_workspace_sizes_rise_with_the_rows():
+    """A buffer made for the largest batch serves the smaller ones, of whatever vocabulary and type."""
+    from moeinfra_b200 import _native
+
+    size = _native.lib().moe_beam_select_workspace_size
+    for count in (1, 8, 64):
+        for beams in (1, 4, 64):
+            for vocab, dtype in ((1, 0), (32000, 0), (131072, 0), (131072, 2), (1 << 20, 1)):
+                sizes = [size(groups, beams, vocab, count, dtype) for groups in range(0, 1300, 1)]
+                assert all(a <= b for a, b in zip(sizes, sizes[1:])), (count, beams, vocab, dtype)
+                assert sizes[700] >= size(40, beams, 131072, count, 0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_a_workspace_for_the_largest_batch_serves_every_smaller_one(dtype):
+    from moeinfra_b200 import kernels
+
+    vocab, count = 65536, 8
+    x, s = _logits(149, vocab, dtype, 3), _scores(149, 1, 3)
+    ws = kernels.beam_select_workspace(x, 1, count)
+    for rows in (149, 148, 128, 75, 37, 4, 1):
+        got = kernels.beam_select(x[:rows], s[:rows], count, workspace=ws)
+        want = kernels.beam_select(x[:rows], s[:rows], count)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), rows
+    kernels.check_device()
+    _check(x[:4], s[:4], count, [t[:4] for t in kernels.beam_select(x, s, count, workspace=ws)])
