@@ -245,6 +245,57 @@ __device__ __forceinline__ Row row_of(const TreeArgs& a, int u, int second, int 
   if (in >= a.tokens || w.node >= have) w.node = -1;
   return w;
 }
+
+// By a softmax warp of pipeline t that has written a result which is not finite, once all of the
+// CTA's pieces are done: looks at its rows of the whole units again and mends them.  It may take longer
+// than a wait is allowed to, and nobody waits for the warp any more.
+template <typename T, int HD>
+__device__ __noinline__ void mend_units(const TreeArgs& a, const int* prefix, int t, int quad) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t inf = T::kBf16 ? 0x7F80u : 0x7C00u;
+  // The CTA's places, as the kernel finds them (one function for both costs it up to 1 %).
+  const int total = prefix[a.kv.seqs] * a.per_seq;
+  const int share = max((int)(((uint32_t)total + gridDim.x - 1) / gridDim.x), kMinShare + kStart);
+  int lo = (int)min((int64_t)blockIdx.x * share, (int64_t)total), hi = (int)min((int64_t)lo + share, (int64_t)total);
+  if (a.whole) {
+    const int b = blockIdx.x / (uint32_t)a.per_seq, u = blockIdx.x - b * a.per_seq;
+    lo = prefix[b] * a.per_seq + u * (prefix[b + 1] - prefix[b]);
+    hi = lo + prefix[b + 1] - prefix[b];
+  }
+  if (a.between) {
+    lo = Piece::between(a, prefix, lo, total);
+    hi = Piece::between(a, prefix, hi, total);
+  }
+  __syncwarp();  // the lanes have written one another's rows
+  Piece pc;
+  for (bool more = pc.start(a, prefix, lo, hi); more; more = pc.next(a, prefix)) {
+    if (pc.s0 > 0 || pc.s1 < pc.n) continue;  // joined, and mended there
+    int len, keys;
+    span(a, pc.b, len, keys);
+    const int block = a.blocks == 1 ? 0 : pc.u % a.blocks;
+    const bool two = a.nodes - block * 2 * a.tokens > a.tokens;
+    const int from = two ? 0 : t * (HD / 2), to = two ? HD : from + HD / 2;
+    const Row me = row_of(a, pc.u, two ? t : 0, quad * 32 + lane, keys - len);
+    bool odd = false;
+    if (me.node >= 0) {
+      const uint4* o = reinterpret_cast<const uint4*>(
+          a.out + (((int64_t)pc.b * a.nodes + me.node) * a.heads + me.head) * HD);
+#pragma unroll 1
+      for (int c = from / 8; c < to / 8; ++c) {
+        const uint4 x = o[c];
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd |= (w[i] & inf) == inf || (w[i] >> 16 & inf) == inf;
+      }
+    }
+    for (uint32_t again = __ballot_sync(0xffffffffu, odd); again; again &= again - 1) {
+      const int r = __ffs(again) - 1;
+      mend_row<T, HD>(a, pc.b, __shfl_sync(0xffffffffu, me.node, r), __shfl_sync(0xffffffffu, me.head, r),
+                      len, keys, from, to);
+    }
+  }
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     k_tree_attention(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap map_q,
@@ -376,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t o_pal = tmem + C::kO + (1 - t) * C::kO1 + lane_base;
     const int row_node = row / a.tile_heads, row_head = row - row_node * a.tile_heads;
     uint32_t n_s = 0, n_pair = 0;  // steps and shared tiles so far
+    bool mend = false;  // a row has met an infinity or NaN
     for (Item it; next_item(it);) {
       const bool two = it.flags & kTwo;
       const int second = two ? t : 0;
@@ -589,13 +641,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = warp_wait(saddr(&s_read[pal]), n_pair++ & 1, a.wait_ns))) break;
         tc_fence_after();
       }
-      uint32_t again = __ballot_sync(0xffffffffu, whole && real && !none && odd != 0.f);
-      for (; again; again &= again - 1) {
-        const int r = __ffs(again) - 1;
-        mend_row<T, HD>(a, it.b, __shfl_sync(0xffffffffu, me.node, r),
-                        __shfl_sync(0xffffffffu, me.head, r), it.len, it.keys, from, to);
-      }
+      mend |= whole && real && !none && odd != 0.f;
     }
+    if (ok && __any_sync(0xffffffffu, mend)) mend_units<T, HD>(a, prefix, t, warp & 3);
     if (!ok) s_abort = 1;
   } else {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));

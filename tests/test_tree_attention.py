@@ -484,3 +484,83 @@ def test_refusals_by_name():
         kernels.rope_append(torch.zeros(2, 8 * 64, device="cuda").half(), torch.zeros(8, 32, device="cuda"),
                             torch.zeros(8, 32, device="cuda"), lens, table, k, k.clone(), 4,
                             slots=lens.long())
+
+
+@gpu
+def test_rows_computed_again_outlast_no_wait():
+    """Rows are computed again when no other warp waits for the one that does it: 32 rows of 8192 keys
+    take longer than the 2 ms allowed here."""
+    from moeinfra_b200 import _native, kernels
+
+    # 300 units of 131 places over the SMs: every CTA has a whole one between two that are cut.
+    seqs, nodes, H, hd, page, n = 300, 4, 16, 64, 64, 8188
+    kp, vp = (_cache(128, 1, page, hd, torch.float16, s) for s in (1, 2))
+    table = torch.arange(128, dtype=torch.int32).repeat(seqs, 1)
+    q = _q(seqs, nodes, H, hd, torch.float16)
+    visible = kernels.tree_masks([-1] * nodes)[None].expand(seqs, nodes, 1)
+    at = torch.full((seqs,), n, dtype=torch.int32, device="cuda")
+    args = (q.cuda(), kp, vp, table.cuda(), at, visible.cuda())
+    clean = kernels.tree_attention(*args)
+    _check(q[:2], kp, vp, table[:2], [n, n], visible[:2], got=clean[:2])
+    vp[127, 0, page - 1, 7] = math.inf  # node 3's, which the other nodes do not see
+    old = _native.wait_limit_ns()
+    _native.set_wait_limit_ns(2_000_000)
+    try:
+        got = kernels.tree_attention(*args)
+        kernels.check_device()
+    finally:
+        _native.set_wait_limit_ns(old)
+    assert not got[:, 3, :, 7].isfinite().any()
+    got[:, 3, :, 7] = clean[:, 3, :, 7]
+    assert got.isfinite().all()
+    # The same rows with probabilities rounded to 16 bits or not, and two results rounded: each by
+    # 2^-11 of at most max |v| < 6.
+    assert float((got.float() - clean.float()).abs().max()) <= 3 * 6 * 2.0 ** -11
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("seqs,lo", [(4, 100), (90, 100), (90, 700), (3, 5000)])
+@pytest.mark.parametrize("nodes", [9, 40])
+def test_rows_are_computed_again_in_every_form(seqs, lo, nodes, hd):
+    """An infinity in a node that others do not see, in units of one tile and of two, that have a CTA each,
+    lie whole between cuts, or are cut: the rows that do not see it are as without it."""
+    from moeinfra_b200 import kernels
+
+    H, KV, page = 8, 2, 16
+    lens = [lo + 13 * i % 50 for i in range(seqs)]
+    table, n = _table([m + nodes for m in lens], page, 8)
+    kp, vp = (_cache(n, KV, page, hd, torch.float16, s) for s in (5, 6))
+    q, visible = _q(seqs, nodes, H, hd, torch.float16), _trees(seqs, nodes, 2)
+    at = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    args = (q.cuda(), kp, vp, table.cuda(), at, visible.cuda())
+    clean = kernels.tree_attention(*args)
+    _check(q[:2], kp, vp, table[:2], lens[:2], visible[:2], got=clean[:2])
+    for b, m in enumerate(lens):
+        vp[int(table[b, (m + 4) // page]), :, (m + 4) % page, hd - 1] = math.inf
+    got = kernels.tree_attention(*args)
+    kernels.check_device()
+    sees = _bits(visible, nodes)[:, :, 4].cuda()
+    assert not got[sees][..., hd - 1].isfinite().any()
+    got[..., hd - 1] = torch.where(sees[..., None], clean[..., hd - 1], got[..., hd - 1])
+    assert got.isfinite().all()
+    # Probabilities rounded to 16 bits or not, and two results rounded: each by 2^-11 of at most
+    # max |v| < 6.
+    assert float((got.float() - clean.float()).abs().max()) <= 3 * 6 * 2.0 ** -11
+
+
+@gpu
+@pytest.mark.parametrize("H,KV,nodes", [(32, 8, 4), (32, 8, 1), (8, 2, 16), (8, 8, 9), (32, 8, 64)])
+@pytest.mark.parametrize("seqs", [1, 5, 64])
+def test_tables_wider_than_the_sequences(H, KV, nodes, seqs):
+    """A table as wide as the longest sequence that may come, over short ones: the results are those of a
+    table that ends with them, whichever kernel and cut its width picks."""
+    from moeinfra_b200 import kernels
+
+    lens, page, hd = [(29 * i) % 97 for i in range(seqs)], 16, 64
+    narrow, n = _table([m + nodes for m in lens], page, 7)
+    wide, _ = _table([m + nodes for m in lens], page, 7, width=2048 // page)
+    kp, vp = (_cache(n, KV, page, hd, torch.bfloat16, s) for s in (1, 2))
+    q, visible = _q(seqs, nodes, H, hd, torch.bfloat16), _trees(seqs, nodes, 5)
+    for table in (narrow, wide):
+        _check(q, kp, vp, table, lens, visible)
