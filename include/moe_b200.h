@@ -619,7 +619,8 @@ int moe_fork_pages(const moe_fork_pages_args_t* args);
  *   new_lengths[b] = lengths[b] + their number.  The entries must rise; a list that
  *   does not, or whose positions have no page, ends before that entry and sets the device
  *   error word (MOE_ERR_PAGE).  lengths[b] < 0: not a sequence, returned as it is.
- *   The pages written to must not be another sequence's too. */
+ *   The pages written to must not be another sequence's too, and new_lengths must not
+ *   share memory with lengths. */
 typedef struct moe_keep_nodes_args {
   moe_kv_pages_t kv;
   int64_t layers, k_layer_stride, v_layer_stride;

@@ -475,6 +475,8 @@ extern "C" int moe_keep_nodes(const moe_keep_nodes_args_t* args) {
   if (!c.lengths || !c.new_lengths || (c.most > 0 && (!c.keep || !c.kv.block_table)) ||
       (c.most > 0 && (!c.kv.k_pages || !c.kv.v_pages)))
     return MOE_ERR_INVALID_ARG;
+  // A sequence's CTAs read its length while one of them writes the new one.
+  if (overlap(c.lengths, 4 * c.kv.seqs, c.new_lengths, 4 * c.kv.seqs)) return MOE_ERR_INVALID_ARG;
   KeepArgs a{};
   a.kv = layers_of(c.kv, c.layers, c.k_layer_stride, c.v_layer_stride);
   a.num_pages = c.kv.num_pages;

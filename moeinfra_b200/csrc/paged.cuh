@@ -42,6 +42,12 @@ struct BF16 {
   }
 };
 
+// Whether two ranges of memory share a byte.
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + b_bytes && y < x + a_bytes;
+}
+
 struct KvPages {
   uint16_t* k;
   uint16_t* v;

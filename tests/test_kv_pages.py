@@ -384,3 +384,18 @@ def test_fork_passes_over_rows_without_a_sequence(seqs, max_pages, page, room):
         _equal(got, want)
         none = want[3] < 0
         assert torch.equal(want[2][none], state[2][parents[none].long()])
+
+
+def test_new_lengths_over_the_old_ones_are_refused():
+    """The CTAs of a sequence read its length while one writes the new one.  On the host; the pointers are
+    never used."""
+    from moeinfra_b200 import _native
+
+    fake = 0x100000
+
+    def keep(lengths, new, seqs=3):
+        return _native.lib().moe_keep_nodes(_native.KEEP_NODES.pack(
+            fake, fake, 2048, 2048, 3, 2, 16, 64, 0, fake, 4, seqs, 4, 1, 0, 0, lengths, fake, 5, 5, new, 0))
+
+    for new in (fake, fake + 8, fake - 8):
+        assert keep(fake, new) == 1, new
