@@ -673,7 +673,8 @@ int moe_rope_append_slots(const moe_rope_append_args_t* args, const int32_t* slo
  *   i < counts[b] (counts NULL: `nodes` everywhere).  q [seqs, nodes, heads,
  *   head_dim], sequences q_seq_stride and nodes q_node_stride elements apart
  *   (multiples of 8); visible uint64 [seqs, nodes, ceil(nodes / 64)], strides in elements (0:
- *   one mask for all); out [seqs, nodes, heads, head_dim] packed.  A row that sees
+ *   one mask for all); out [seqs, nodes, heads, head_dim] packed, over none of the
+ *   sequences' stretches of q (first node's row to last node's).  A row that sees
  *   nothing is zeros, and so are the rows of nodes past counts[b] and of sequences with
  *   lengths[b] < 0.  fp32 scores, softmax and sums; the probabilities are rounded to
  *   the element type for the product with V.  What lies in a page past a

@@ -1096,6 +1096,12 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
   const size_t need = moe_tree_attention_workspace_size(hd);
   if (!c.workspace || c.workspace_bytes < (int64_t)need) return MOE_ERR_WORKSPACE;
   if (!aligned16(c.workspace)) return MOE_ERR_ALIGNMENT;
+  // Rows may be computed again from their queries after results have been written.
+  const int64_t row = 2 * c.heads * hd, rows = 2 * (c.nodes - 1) * c.q_node_stride + row;
+  if (overlap(c.out, c.kv.seqs * c.nodes * row, c.q, 2 * (c.kv.seqs - 1) * c.q_seq_stride + rows))
+    for (int64_t b = 0; b < c.kv.seqs; ++b)
+      if (overlap(c.out, c.kv.seqs * c.nodes * row, c.q + b * c.q_seq_stride, rows))
+        return MOE_ERR_INVALID_ARG;
   cudaStream_t s = static_cast<cudaStream_t>(c.stream);
   const bool bf16 = c.kv.dtype == MOE_DTYPE_BF16;
   if (tree_is_few(a)) return tree_attention_few(a, static_cast<int>(hd), bf16, s);

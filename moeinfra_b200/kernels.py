@@ -1054,7 +1054,7 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     ``counts`` int32 [sequences]: the nodes that are there (None: all).  A row that sees nothing
     is zeros, and so are rows past ``counts`` and of sequences with a negative length.  The cache as in
     :func:`paged_attention`; at most 2048 sequences and 1024 nodes.  ``scale`` defaults to ``head_dim ** -0.5``.  Returns
-    [sequences, nodes, heads, head_dim].
+    [sequences, nodes, heads, head_dim]; ``out``, if given, must not share memory with ``q``.
 
     ``workspace``: a buffer from :func:`tree_attention_workspace`, as for :func:`paged_attention`.
     """

@@ -564,3 +564,22 @@ def test_tables_wider_than_the_sequences(H, KV, nodes, seqs):
     q, visible = _q(seqs, nodes, H, hd, torch.bfloat16), _trees(seqs, nodes, 5)
     for table in (narrow, wide):
         _check(q, kp, vp, table, lens, visible)
+
+
+@gpu
+@pytest.mark.parametrize("nodes,heads", [(3, 4), (9, 8)])
+def test_a_result_over_the_queries_is_refused(nodes, heads):
+    """A row may be computed again from its query after results were written.  A result between two
+    sequences' queries is none over them."""
+    from moeinfra_b200 import kernels
+
+    k = _cache(4, 2, 16, 64, torch.float16, 1)
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2)
+    lens, vis = torch.full((2,), 5, dtype=torch.int32, device="cuda"), _trees(2, nodes, 1).cuda()
+    buf = _q(8, nodes, heads, 64, torch.float16).cuda()
+    want = kernels.tree_attention(buf[::7], k, k, table, lens, vis)
+    for q, out in ((buf[:2], buf[:2]), (buf[:2], buf[1:3]), (buf[1:3], buf[:2]), (buf[::7], buf[6:8])):
+        with pytest.raises(RuntimeError, match="status 1"):
+            kernels.tree_attention(q, k, k, table, lens, vis, out=out)
+    got = kernels.tree_attention(buf[::7], k, k, table, lens, vis, out=buf[3:5])
+    assert got.data_ptr() == buf[3].data_ptr() and torch.equal(got, want)
