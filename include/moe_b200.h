@@ -639,7 +639,8 @@ int moe_keep_nodes(const moe_keep_nodes_args_t* args);
  *   0 where x_t == m; NaN logits count as -inf).  out_scores fp32, out_parents int32 (the beam
  *   in its group) and out_tokens int64 [groups, count]: larger scores first, equal ones by
  *   rising beam, in a beam by falling logit, then rising token.  What scores
- *   -inf (or NaN) is no candidate; places without one are (-inf, 0, 0).  beams
+ *   -inf (or NaN) is no candidate; places without one are (-inf, 0, 0).  out_scores may
+ *   be scores itself where count is beams, and must not share memory with it otherwise.  beams
  *   and count <= 64, vocab <= 2^20.  The workspace's size depends on the device, count and
  *   the number of rows alone and rises with both: one made for the largest batch serves
  *   the smaller ones.  Its first 4096 bytes must be zero before its first call and are

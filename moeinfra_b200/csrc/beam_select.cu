@@ -619,6 +619,10 @@ extern "C" int moe_beam_select(const moe_beam_select_args_t* args) {
   if (!c.logits || !c.scores || !c.out_scores || !c.out_parents || !c.out_tokens)
     return MOE_ERR_INVALID_ARG;
   const int64_t size = c.dtype == MOE_DTYPE_F32 ? 4 : 2, rows = c.groups * c.beams;
+  // A group's scores are read by the CTA that writes its new ones, at the same place or none of theirs.
+  if (overlap(c.scores, 4 * rows, c.out_scores, 4 * c.groups * c.count) &&
+      (c.scores != c.out_scores || c.beams != c.count))
+    return MOE_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(c.logits) % size) return MOE_ERR_ALIGNMENT;
   if (!c.workspace || c.workspace_bytes < (int64_t)moe_beam_select_workspace_size(
                                               c.groups, c.beams, c.vocab, c.count, c.dtype))

@@ -295,3 +295,33 @@ def test_a_workspace_for_the_largest_batch_serves_every_smaller_one(dtype):
         assert all(torch.equal(a, b) for a, b in zip(got, want)), rows
     kernels.check_device()
     _check(x[:4], s[:4], count, [t[:4] for t in kernels.beam_select(x, s, count, workspace=ws)])
+
+
+def _in_place(x, scores, out, beams, count, groups):
+    """The library's call with its new scores at ``out``; status, parents, tokens."""
+    from moeinfra_b200 import _native, kernels
+
+    parents = torch.zeros(groups, count, dtype=torch.int32, device=x.device)
+    tokens = torch.zeros(groups, count, dtype=torch.int64, device=x.device)
+    ws = kernels.beam_select_workspace(x, beams, count)
+    status = _native.lib().moe_beam_select(_native.BEAM_SELECT.pack(
+        x.data_ptr(), x.shape[1], groups, beams, x.shape[1], 2, scores, count, out, parents.data_ptr(),
+        tokens.data_ptr(), ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+    return status, parents, tokens
+
+
+@gpu
+def test_new_scores_may_take_the_old_ones_place():
+    """Of the same shape; at another place over them they are refused."""
+    from moeinfra_b200 import kernels
+
+    x = _logits(40 * 4, 5000, torch.float32, 1)
+    s = _scores(40, 4, 1)
+    want = kernels.beam_select(x, s, 4)
+    at = s.data_ptr()
+    for out, count in ((at + 16, 4), (at - 16, 4), (at, 3), (at, 5)):
+        assert _in_place(x, at, out, 4, count, 40)[0] == 1
+    status, parents, tokens = _in_place(x, at, at, 4, 4, 40)
+    kernels.check_device()
+    assert status == 0
+    assert torch.equal(s, want[0]) and torch.equal(parents, want[1]) and torch.equal(tokens, want[2])
