@@ -325,3 +325,46 @@ def test_beam_logits_are_the_returned_sequences_(ckpt):  # noqa: F811
             rows = step.logits.view(2, 4, V)
             for b in range(2):
                 assert torch.equal(many.logits[b, 0], rows[b, int(step.parents[b, 0])])
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv,hd", [(4, 2, 64), (4, 1, 128)])
+@torch.no_grad()
+def test_forked_beams_are_what_recomputed_sequences_are(heads, kv, hd):
+    """At every step the logits over the forked cache are those of each beam's own sequence computed from
+    scratch, row by row and without what earlier steps were off, and the step's choice is the
+    definition's for its own logits and scores."""
+    from moeinfra_b200 import kernels
+    from moeinfra_b200.engine.engine import _BeamStep
+    from oracle import branches
+    from tests.test_beam_select import _off
+
+    B, K, steps = 2, 3, 36  # three page crossings of 16
+    stack, plain = _stack(heads, kv, hd), _stack(heads, kv, hd)
+    rows = [r.tolist() for r in _ragged([14, 33])[0]]
+    step = _BeamStep(SimpleNamespace(_device=stack.device, _stack=stack), B, K)
+    stack.cache.clear()
+    stack.cache.reserve([len(rows[0]), 0, 0, len(rows[1]), 0, 0])
+    first = step.begin(stack.prefill([torch.tensor(r) for r in rows], stride=K), stack.prompt_lengths)
+    paths = [[rows[b] + [t] for t in first[b].tolist()] for b in range(B)]
+    forks = 0
+    for i in range(1, steps):
+        before = step.scores.clone().cpu()
+        logits = step.run()
+        full = _logits_after(plain, [p for b in range(B) for p in paths[b]])
+        err = (logits.float() - full).norm(dim=-1) / full.norm(dim=-1)
+        assert float(err.max()) < CLOSE, (i, err.tolist())
+        tokens, parents = step.ids.view(B, K).tolist(), step.parents.tolist()
+        x = logits.double().cpu().view(B, K, -1)
+        for b in range(B):
+            want = branches.beam_select(logits.view(B, K, -1)[b].cpu(), before[b], K)[0]
+            every = before[b].double()[:, None] + torch.log_softmax(x[b], -1)
+            for j, (p, t) in enumerate(zip(parents[b], tokens[b])):
+                v = float(every[p, t])
+                off = _off(v, float(before[b, p]))
+                assert abs(v - float(want[j])) <= 2 * off and abs(v - float(step.scores[b, j])) <= off
+            forks += len(set(parents[b])) < K
+            paths[b] = [paths[b][p] + [t] for p, t in zip(parents[b], tokens[b])]
+            assert len({tuple(p) for p in paths[b]}) == K
+    assert forks > 0  # rows were shared and copied, not only carried on
+    kernels.check_device()
