@@ -681,8 +681,11 @@ int moe_rope_append_slots(const moe_rope_append_args_t* args, const int32_t* slo
  *   the element type for the product with V.  What lies in a page past a
  *   sequence's end, and the values of nodes that a row does not see, have no effect,
  *   infinities and NaN included.  page_size % 16 == 0, seqs <= 2048, nodes <= 1024,
- *   max_pages * page_size <= 2^30, scale > 0.  The workspace's size depends on the device and head_dim alone; its first 4096
- *   bytes must be zero before its first call and are left zero.  Results do not
+ *   max_pages * page_size <= 2^30, scale > 0; a unit is up to 256 rows (nodes times the
+ *   heads of a group) of a sequence's KV head, and the number of units times
+ *   (max_pages * page_size / 64 + 3) has to stay below 2^31 - 4096.  The workspace's size
+ *   depends on the device and head_dim alone; its first 4096 bytes must be zero before its
+ *   first call and are left zero.  Results do not
  *   vary from call to call. */
 typedef struct moe_tree_attention_args {
   moe_kv_pages_t kv;

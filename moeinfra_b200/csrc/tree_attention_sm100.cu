@@ -1114,7 +1114,7 @@ extern "C" int moe_tree_attention(const moe_tree_attention_args_t* args) {
   a.blocks = (a.nodes + 2 * a.tokens - 1) / (2 * a.tokens);
   const int64_t per_seq = (int64_t)a.kv.kv_heads * a.parts * a.blocks;
   const int64_t steps = ceil_div(c.kv.max_pages * c.kv.page_size, kN) + kStart;
-  if (per_seq > INT32_MAX || c.kv.seqs * per_seq > INT32_MAX / (steps > 0 ? steps : 1) - 4096)
+  if (per_seq > INT32_MAX || c.kv.seqs * per_seq > (INT32_MAX - 4096) / steps)  // the line's places: 32 bits
     return MOE_ERR_UNSUPPORTED;
   a.per_seq = static_cast<int>(per_seq);
   a.box_shift = 4;

@@ -1053,7 +1053,7 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     set where the node sees node i, itself included (:func:`tree_masks` makes it from parents).
     ``counts`` int32 [sequences]: the nodes that are there (None: all).  A row that sees nothing
     is zeros, and so are rows past ``counts`` and of sequences with a negative length.  The cache as in
-    :func:`paged_attention`; at most 2048 sequences and 1024 nodes.  ``scale`` defaults to ``head_dim ** -0.5``.  Returns
+    :func:`paged_attention`; at most 2048 sequences, 1024 nodes and a table of 2^30 positions.  ``scale`` defaults to ``head_dim ** -0.5``.  Returns
     [sequences, nodes, heads, head_dim]; ``out``, if given, must not share memory with ``q``.
 
     ``workspace``: a buffer from :func:`tree_attention_workspace`, as for :func:`paged_attention`.

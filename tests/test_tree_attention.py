@@ -583,3 +583,23 @@ def test_a_result_over_the_queries_is_refused(nodes, heads):
             kernels.tree_attention(q, k, k, table, lens, vis, out=out)
     got = kernels.tree_attention(buf[::7], k, k, table, lens, vis, out=buf[3:5])
     assert got.data_ptr() == buf[3].data_ptr() and torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("nodes", [2, 20])
+def test_a_table_of_two_to_the_30_positions(nodes):
+    lens, page = [70000], 65536
+    table, n = _table([lens[0] + nodes], page, 3, width=(1 << 30) // page)
+    kp, vp = (_cache(n, 1, page, 64, torch.float16, s) for s in (1, 2))
+    _check(_q(1, nodes, 4, 64, torch.float16), kp, vp, table, lens, _trees(1, nodes, 4))
+
+
+def test_a_line_past_32_bits_is_refused():
+    """Units times a table's steps; on the host, the pointers are never used."""
+    from moeinfra_b200 import _native
+
+    fake = 0x100000
+    for seqs, kv, pages in ((128, 1, 1 << 14), (16, 8, 1 << 14), (2048, 8, 1 << 11)):  # of 65536
+        assert _native.lib().moe_tree_attention(_native.TREE_ATTENTION.pack(
+            fake, fake, kv << 22, kv << 22, 3, kv, 1 << 16, 64, 0, fake, pages, seqs, pages, fake,
+            20 * 64 * 8, 64 * 8, 20, 8, fake, 0, fake, 20, 1, 0.125, 1 << 40, fake, 1 << 30, 0)) == 2
