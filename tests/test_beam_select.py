@@ -325,3 +325,15 @@ def test_new_scores_may_take_the_old_ones_place():
     kernels.check_device()
     assert status == 0
     assert torch.equal(s, want[0]) and torch.equal(parents, want[1]) and torch.equal(tokens, want[2])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_as_many_tokens_as_are_served(dtype):
+    from moeinfra_b200 import kernels
+
+    x, s = _logits(4, 1 << 20, dtype, 11), _scores(2, 2, 11)
+    x[1, -1] = x[3, 0] = 30.0
+    got = kernels.beam_select(x, s, 64)
+    kernels.check_device()
+    _check(x, s, 64, got)

@@ -399,3 +399,15 @@ def test_new_lengths_over_the_old_ones_are_refused():
 
     for new in (fake, fake + 8, fake - 8):
         assert keep(fake, new) == 1, new
+
+
+@gpu
+@pytest.mark.parametrize("max_pages", [2, 3])
+def test_as_many_rows_as_fork(max_pages):
+    """8192 rows, their table in one CTA's shared memory and in two CTAs'."""
+    rng = random.Random(max_pages)
+    state = _state(rng, 8192, max_pages, 2, kv=1, layers=1, spare=8192)
+    parents = _parents(rng, 8192)
+    want = [t.clone() for t in state]
+    assert branches.fork(*want[:4], parents, want[4])
+    _equal(_fork(state, parents, 1), want)
