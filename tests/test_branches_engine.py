@@ -368,3 +368,95 @@ def test_forked_beams_are_what_recomputed_sequences_are(heads, kv, hd):
             assert len({tuple(p) for p in paths[b]}) == K
     assert forks > 0  # rows were shared and copied, not only carried on
     kernels.check_device()
+
+
+@gpu
+@pytest.mark.parametrize("captured", [False, True])
+@torch.no_grad()
+def test_trees_grow_their_pages_beside_an_idle_row(captured):
+    """A step is fork (each row its own parent, room for a tree), verify, accept, captured or not: pages come
+    as they are needed, the row without a sequence gets none, and the logits are those of decoding."""
+    from moeinfra_b200 import kernels
+
+    rng = random.Random(17)
+    stack, plain = _stack(), _stack()
+    rows = [r.tolist() for r in _ragged([12, 1, 40])[0]]
+    lens, T, steps = [12, -1, 1, 40], 6, 9  # row 1 is idle
+    live = [b for b, n in enumerate(lens) if n >= 0]
+    tail = {b: [rng.randrange(512) for _ in range(steps * T + 1)] for b in live}
+    plain.cache.reserve([len(r) + steps * T + 1 for r in rows])
+    plain.prefill([torch.tensor(r) for r in rows])
+    pos = torch.tensor([len(r) for r in rows], dtype=torch.int32, device="cuda")
+    want = []
+    for i in range(steps * T):
+        ids = torch.tensor([tail[b][i] for b in live], device="cuda")[:, None]
+        want.append(dict(zip(live, plain.decode(ids, pos).float())))
+        pos += 1
+    cache = stack.cache
+    cache.clear()
+
+    def prompts():
+        cache.reserve([max(n, 0) for n in lens])
+        for b, r in zip(live, rows):  # one after the other, each in its own row of the table
+            alone = stack.cache.block_table
+            stack.cache.block_table = alone[b:b + 1]
+            stack.prefill([torch.tensor(r)])
+            stack.cache.block_table = alone
+
+    lengths = torch.full((4,), -1, dtype=torch.int32, device="cuda")
+    ids = torch.zeros(4, T, dtype=torch.long, device="cuda")
+    depths = torch.zeros(4, T, dtype=torch.int32, device="cuda")
+    visible = torch.zeros(4, T, 1, dtype=torch.int64, device="cuda")
+    keep = torch.full((4, T), -1, dtype=torch.int32, device="cuda")
+    parents = torch.arange(4, dtype=torch.int32, device="cuda")
+
+    def step():
+        cache.fork(lengths, parents, T)
+        out = stack.verify(ids, lengths, depths, visible)
+        lengths.copy_(stack.accept(lengths, keep))
+        return out
+
+    if captured:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step()  # all rows idle
+        torch.cuda.synchronize()
+        assert not bool(cache.refs.any()) and lengths.tolist() == [-1] * 4
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+    prompts()
+    lengths.copy_(torch.tensor(lens))
+    done = dict.fromkeys(live, 0)
+    for _ in range(steps):
+        drafts = {}
+        for b in live:
+            tree = [-1] + [rng.randint(max(0, j - 3), j - 1) for j in range(1, T)]
+            depth, on, token = [0], [0], [tail[b][done[b]]]
+            for j in range(1, T):
+                depth.append(depth[tree[j]] + 1)
+                real = tree[j] == on[-1] and rng.random() < 0.7
+                token.append(tail[b][done[b] + depth[j]] if real else rng.randrange(512))
+                on += [j] if real else []
+            drafts[b] = on
+            ids[b], depths[b] = torch.tensor(token), torch.tensor(depth)
+            visible[b] = kernels.tree_masks(tree)
+            keep[b] = torch.tensor(on + [-1] * (T - len(on)))
+        keep[1] = 0
+        if captured:
+            graph.replay()
+            logits = out.float()
+        else:
+            logits = step().float()
+        for b, on in drafts.items():
+            for d, node in enumerate(on):
+                y = want[done[b] + d][b]
+                assert float((logits[b, node] - y).norm() / y.norm()) < CLOSE, (b, d)
+            done[b] += len(on)
+        assert lengths.tolist() == [n + done[b] if n >= 0 else -1 for b, n in enumerate(lens)]
+        assert bool((cache.block_table[1] == -1).all())
+    kernels.check_device()
+    table, refs = cache.block_table, cache.refs
+    assert torch.equal(torch.bincount(table[table >= 0].long(), minlength=len(refs)).int(), refs)
+    assert max(done.values()) > 16
