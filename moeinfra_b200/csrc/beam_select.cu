@@ -24,9 +24,9 @@
 //     again chunk by chunk, each with a threshold of its own, and a chunk that still has too
 //     many (equal logits) is searched round by round.
 // The last CTA of a group joins the lists of its rows.
-// Measured in a graph: 32 groups of 8 rows of 131072 fp32, 16 of each 38.4 us (134 MB, 3.5 TB/s; 56 %
+// Measured in a graph: 32 groups of 8 rows of 131072 fp32, 16 of each 38.7 us (134 MB, 3.5 TB/s; 56 %
 // of the issue slots, and the barriers at a stretch's end), 64 of each 51; 16 x 4 rows of 32000 fp16
-// 13.7 us, 1 x 4 10.4, chains of latencies (first chunk, up to three stretches, the join's 4 us).
+// 13.8 us, 1 x 4 10.7, chains of latencies (first chunk, up to three stretches, the join's 4 us).
 #include <algorithm>
 
 #include "sample.cuh"

@@ -7,9 +7,9 @@
 // a row is about to write into a page that others list too, and there only the
 // positions that are filled.  No counterpart in the reference (one sequence
 // over a growing DynamicCache, engine/engine.py:326-378).
-// Measured in a graph (8 KV heads of 128, fp16 but the last): fork of 1 x 4 rows, 32 layers 8.5 us, of
-// 16 x 4, pages of 64 35.8 us (180 MB, 5.0 TB/s), of 32 x 8 rows, 8 layers bf16 43 us, 11 of them the
-// tables; nodes of 1 sequence, 32 layers 3.2 us, of 64 9.8 us (34 MB).
+// Measured in a graph (8 KV heads of 128, fp16 but for 8 layers): fork of 1 x 4 rows, 32 layers 8.6 us, of
+// 16 x 4, pages of 64 35.8 us (180 MB, 5.0 TB/s), of 32 x 8 rows, 8 layers bf16 44 us, 11 of them the
+// tables; nodes of 1 sequence, 32 layers 3.0 us, of 64 9.6 us (34 MB).
 #include "paged.cuh"
 
 namespace moe {
@@ -282,7 +282,7 @@ constexpr int kKeepThreads = 128, kPieces = 2;
 // moves them for every kept node of its sequence: lists rise, so a node's place is
 // never read after it was written, and pieces have nothing to do with each other.
 // Bound by latency (length and list, pages, rows) and by how many rows are on their way: 64
-// sequences x 32 layers x 8 heads of 128 take 2048 CTAs, 8 to an SM at once, 9.8 us; 10.1 without the
+// sequences x 32 layers x 8 heads of 128 take 2048 CTAs, 8 to an SM at once, 9.6 us; 10.1 without the
 // bound on registers, 11.4 with CTAs of 256, 11.4 with one piece a thread.
 template <int HD>
 __global__ void __launch_bounds__(kKeepThreads, 8) k_keep_nodes(const KeepArgs a) {
