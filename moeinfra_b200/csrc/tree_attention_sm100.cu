@@ -37,8 +37,8 @@
 // (165 MB, 3.7 TB/s: a unit's 9 steps stream at a copy's rate, its end and the next one's start do
 // not; the join 4 us); 64 nodes over 16 x 2049..4095 bf16 70 us (shared memory: Q K^T reads 6 KB
 // for 32 cycles of products, 1280 of a step's 1640 cycles; 38 MB of pieces of cut units); 27 nodes
-// over 131071 + 85413 bf16 148 to 156 us by the box (888 MB, 5.7 to 6.0 TB/s); 16 nodes over 72 9.8 us, a
-// chain of latencies.
+// over 131071 + 85413 bf16 148 to 156 us from one GPU to another (888 MB, 5.7 to 6.0 TB/s); 16 nodes
+// over 72 9.8 us, a chain of latencies.
 //
 // O is rescaled only when a row's maximum grew by more than 2^8 since the reference
 // in use: probabilities stay below 2^8, O and l are sums of the same factor.
